@@ -116,6 +116,18 @@ static inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// The driver entry needs a current context, which a thread has from its first call of the runtime on: a thread of autograd's may
+// come here before one.
+static inline CUresult encode_tiled(EncodeTiledFn fn, CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                                    const cuuint32_t* box, const cuuint32_t* estr, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo) {
+  for (int attempt = 0;; ++attempt) {
+    const CUresult r = fn(map, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    int dev = 0;
+    if (r != CUDA_ERROR_INVALID_CONTEXT || attempt > 0 || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return r;
+  }
+}
+
 // 2-D row-major tensor [rows, inner] with a row pitch in bytes; box = [box_rows, box_inner];
 // swizzle = 128 or 64 (bytes) or 0 for none; out-of-range elements read as zero and are not written.
 static inline int32_t make_map(CUtensorMap* map, CUtensorMapDataType dt, int64_t esz, const void* base, int64_t inner,
@@ -132,8 +144,8 @@ static inline int32_t make_map(CUtensorMap* map, CUtensorMapDataType dt, int64_t
 #ifdef METIS_TIMING_KNOBS
   if (const char* e = getenv("METIS_DEV_L2PROMO")) promo = (CUtensorMapL2promotion)atoi(e);
 #endif
-  const CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(fn, map, dt, 2, base, dims, strides, box, estr,
+                                  swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, promo);
   if (r != CUDA_SUCCESS) return fail(METIS_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with %d", what, (int)r);
   return METIS_OK;
 }
@@ -146,8 +158,8 @@ static inline int32_t make_row_map(CUtensorMap* map, const void* base, int64_t g
   const cuuint64_t strides[2] = {128, (cuuint64_t)pitch_bytes};
   const cuuint32_t box[3] = {64, (cuuint32_t)groups, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(fn, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (r != CUDA_SUCCESS) return fail(METIS_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with %d", what, (int)r);
   return METIS_OK;
 }
