@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmetis_nvfp4.so"
 
 DTYPE_BF16, DTYPE_F32 = 0, 1
 SF_ROWMAJOR, SF_MMA = 0, 1
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
 Q_TRANSPOSE, Q_STOCHASTIC, Q_OFFSET_ON_DEVICE, Q_HADAMARD = 1, 2, 4, 8
 Q_DEFER_ROWMAJOR, Q_DEFER_TRANSPOSED, Q_SR16 = 16, 32, 64
 QUANTIZE_EXTRA_WORKSPACE = 8192
@@ -42,6 +43,8 @@ EXPORTS = (
     "metis_bf16_panel_gemm_workspace_bytes", "metis_bf16_panel_gemm",
     "metis_lowrank_dts_workspace_bytes", "metis_lowrank_dts", "metis_lowrank_dts_mean", "metis_lowrank_du_workspace_bytes", "metis_lowrank_du",
     "metis_rope_pair", "metis_silu_mul",
+    "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product",
+    "metis_head_loss_workspace_bytes", "metis_head_loss", "metis_head_sum", "metis_head_backward_workspace_bytes", "metis_head_backward",
 )
 
 
@@ -62,6 +65,40 @@ class GemmArgs(C.Structure):
         ("status", C.c_void_p), ("stream", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
         ("sm_limit", C.c_int32), ("reserved2", C.c_int32),
+    ]
+
+
+class LinearArgs(C.Structure):
+    """struct metis_linear_args"""
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+        ("bias", C.c_void_p), ("bias_dtype", C.c_int32), ("activation", C.c_int32),
+        ("gate", C.c_void_p), ("ldgate", C.c_int64), ("residual", C.c_void_p), ("ldr", C.c_int64),
+        ("y", C.c_void_p), ("ldy", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64),
+        ("status", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class LinearPointwiseArgs(C.Structure):
+    """struct metis_linear_pointwise_args"""
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int64),
+        ("dy", C.c_void_p), ("lddy", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64),
+        ("dz", C.c_void_p), ("lddz", C.c_int64), ("dgate", C.c_void_p), ("lddg", C.c_int64),
+        ("dbias", C.c_void_p), ("dbias_dtype", C.c_int32), ("activation", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
+class HeadArgs(C.Structure):
+    """struct metis_head_args"""
+    _fields_ = [
+        ("M", C.c_int64), ("V", C.c_int64), ("K", C.c_int64),
+        ("h", C.c_void_p), ("ldh", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+        ("target", C.c_void_p), ("ignore_index", C.c_int64), ("scale", C.c_float), ("negate", C.c_int32),
+        ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("status", C.c_void_p), ("stream", C.c_void_p),
     ]
 
 
@@ -146,6 +183,24 @@ def lib() -> C.CDLL:
     L.metis_rope_pair.restype = i32
     L.metis_silu_mul.argtypes = [vp, vp, vp, i64, vp]
     L.metis_silu_mul.restype = i32
+    L.metis_linear.argtypes = [C.POINTER(LinearArgs)]
+    L.metis_linear.restype = i32
+    L.metis_linear_pointwise_workspace_bytes.argtypes = [i64, i64]
+    L.metis_linear_pointwise_workspace_bytes.restype = i64
+    L.metis_linear_pointwise.argtypes = [C.POINTER(LinearPointwiseArgs)]
+    L.metis_linear_pointwise.restype = i32
+    L.metis_bf16_product.argtypes = [vp, i32, i64, vp, i64, i64, i64, i64, vp, i64, vp, vp]
+    L.metis_bf16_product.restype = i32
+    L.metis_head_loss_workspace_bytes.argtypes = [i64, i64, i64, i32]
+    L.metis_head_loss_workspace_bytes.restype = i64
+    L.metis_head_loss.argtypes = [C.POINTER(HeadArgs), vp, vp]
+    L.metis_head_loss.restype = i32
+    L.metis_head_sum.argtypes = [vp, vp, i64, i64, i32, vp, vp, vp]
+    L.metis_head_sum.restype = i32
+    L.metis_head_backward_workspace_bytes.argtypes = [i64, i64, i64]
+    L.metis_head_backward_workspace_bytes.restype = i64
+    L.metis_head_backward.argtypes = [C.POINTER(HeadArgs), vp, i32, vp, vp, i64, vp, i64]
+    L.metis_head_backward.restype = i32
     _lib = L
     return L
 

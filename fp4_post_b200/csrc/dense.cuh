@@ -1,0 +1,117 @@
+// The bf16 products outside the NVFP4 layers (a linear layer with its epilogue, the head with its loss): parameters and epilogue
+// arithmetic that the kernels of dense_gemm.cu and dense_small.cu share.
+#pragma once
+
+#include "gemm_common.cuh"
+
+namespace metis {
+
+struct DenseParams {
+  int64_t M, N, K;
+  int32_t* status;
+  int32_t band;                                            // row tiles per band of the tile order
+  // linear layer: d = act(A B^T + bias) * gate + residual, and z, what act was applied to
+  const void* bias;  int32_t bias_f32;
+  int32_t act;
+  const __nv_bfloat16* gate;      int64_t ldgate;  int32_t gate_vec;       // *_vec: rows of 16-byte pieces
+  const __nv_bfloat16* residual;  int64_t ldr;     int32_t residual_vec;
+  __nv_bfloat16* d;               int64_t ldd;     int32_t d_tma;          // *_tma: stored by the TMA unit
+  __nv_bfloat16* z;               int64_t ldz;     int32_t z_tma;
+  // head: logits l = scale * (A B^T); columns of the vocabulary [0, N) of this launch are [col0, col0 + N) of all
+  const int64_t* target;  int64_t ignore;
+  int64_t vocab;  int64_t col0;
+  float scale, scale_log2e;                                // 1 / temperature, and that times log2(e)
+  float weight_scale;                                      // scale, with the sign of the loss
+  float2* stats;                                           // [slots, M]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum)
+  float* stats_e;                                          // [slots, M]: sum of 2^(..) (l log2(e) - maximum), or null
+  float* picked;                                           // [M]: logit of the target
+  const float* lse;                                        // [M]
+  const float* gout;  int32_t gout_stride;                 // gradient of each row's loss: gout[row * stride] times *inv_count (null: 1)
+  const float* inv_count;
+  // sum of pieces: fp32 addend
+  const float* c;  int64_t ldc;
+};
+
+#ifdef __CUDACC__
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// act(z).  The forms keep their relative accuracy for large negative z (no difference of nearly equal numbers): silu and the tanh
+// form of gelu are z times a logistic function, since (1 + tanh u) / 2 = 1 / (1 + exp(-2u)); the erf form is z times the
+// normal distribution's function.
+template <int kAct> __device__ __forceinline__ float activate(float z) {
+  if constexpr (kAct == METIS_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
+  if constexpr (kAct == METIS_ACT_GELU) return z * normcdff(z);
+  if constexpr (kAct == METIS_ACT_GELU_TANH) {
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);      // 2 sqrt(2 / pi) (z + 0.044715 z^3)
+    return __fdividef(z, 1.0f + __expf(-u2));
+  }
+  return z;
+}
+// act(z) and act'(z)
+template <int kAct> __device__ __forceinline__ void activate_both(float z, float& a, float& slope) {
+  a = z;
+  slope = 1.0f;
+  if constexpr (kAct == METIS_ACT_SILU) {
+    const float p = __fdividef(1.0f, 1.0f + __expf(-z));
+    a = z * p;
+    slope = fmaf(a, 1.0f - p, p);
+  }
+  if constexpr (kAct == METIS_ACT_GELU) {
+    const float p = normcdff(z);
+    a = z * p;
+    slope = fmaf(0.3989422804014327f * z, __expf(-0.5f * z * z), p);
+  }
+  if constexpr (kAct == METIS_ACT_GELU_TANH) {
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+    const float p = __fdividef(1.0f, 1.0f + __expf(-u2));
+    a = z * p;
+    slope = fmaf(a * (1.0f - p), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), p);
+  }
+}
+template <int kN> __device__ __forceinline__ void activate_all(int act, float (&v)[kN]) {
+  if (act == METIS_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = activate<METIS_ACT_SILU>(v[i]);
+  } else if (act == METIS_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = activate<METIS_ACT_GELU>(v[i]);
+  } else if (act == METIS_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = activate<METIS_ACT_GELU_TANH>(v[i]);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 w = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&w);
+}
+
+// Running softmax statistics of one row: m, the maximum of the logits seen (times log2 e), s, the sum of 2^(l - m), and e, the
+// sum of 2^(l - m) (l - m).  m starts at -infinity; base() replaces it there, so that no difference of two infinities is formed.
+struct RowStats {
+  float m, s, e;
+};
+__device__ __forceinline__ float stats_base(float m) { return m == -INFINITY ? 0.0f : m; }
+// b into a
+template <bool kEntropy> __device__ __forceinline__ void stats_merge(RowStats& a, const RowStats& b) {
+  const float m = fmaxf(a.m, b.m), base = stats_base(m);
+  const float fa = exp2_fast(a.m - base), fb = exp2_fast(b.m - base);
+  if constexpr (kEntropy) {
+    // (an empty side has e = 0; its distance is -infinity)
+    const float da = a.m == -INFINITY ? 0.0f : a.m - base, db = b.m == -INFINITY ? 0.0f : b.m - base;
+    a.e = fmaf(fa, fmaf(da, a.s, a.e), fb * fmaf(db, b.s, b.e));
+  }
+  a.s = fmaf(a.s, fa, b.s * fb);
+  a.m = m;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace metis

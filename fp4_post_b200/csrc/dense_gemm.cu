@@ -1,0 +1,898 @@
+// bf16 products on CTA pairs (tcgen05 kind::f16, cta_group::2) with the epilogues of the layers that stay in bf16, for sm_100a:
+//
+//   D [M, N] = A B^T, A [M, K] and B [N, K], either operand stored with the contraction in its rows instead (MN-major: the
+//   gradients read their operands as they lie, nothing is transposed in memory), and behind it
+//     linear   act(D + bias) * gate + residual in bf16, and the value in front of act where a backward pass will want it
+//     stats    for each row the maximum of the logits and the sum of their exponentials over this tile's columns, the entropy's
+//              sum, and the target's logit: the logits themselves are never stored
+//     grad     the logits' gradient (softmax - one-hot) times the row's weight, in bf16: the operand of the two products behind it
+//     sum      D, or D plus an fp32 addend, in bf16 or fp32: gradients, summed over pieces of the vocabulary
+//
+// A pair computes 256 x 256 tiles: CTA r has rows [128 r, +128) of A and of B and rows [128 r, +128) of the accumulator.  Two whole
+// accumulators fit tensor memory (2 x 256 columns), so the epilogue of a tile runs beside all of the next tile's MMAs.  A stage is 64
+// elements of the contraction (32 KiB per CTA), six of them are in flight.  Roles as in the NVFP4 product: warp 0 loads, warp 1 of
+// the leader issues, warps 2 to 9 are the epilogue (two for each 32-lane quarter of tensor memory, 128 columns each).
+// No copy is multicast.  Every wait is bounded; both CTAs meet at a cluster barrier before they free tensor memory.
+#include "dense.cuh"
+#include "pair.cuh"
+
+namespace metis {
+
+enum DenseEpilogue { kEpiLinear, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
+
+struct DenseCfg {
+  static constexpr int kStages = 6;
+  static constexpr int kHalfBytes = 128 * 128;             // 128 rows x 64 elements of A or of B
+  static constexpr int kBoxBytes = 64 * 128;               // one MN-major box: 64 contraction rows x 64 elements
+  static constexpr int kStageBytes = 2 * kHalfBytes;
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+  static constexpr int kStagingBytes = kEpilogueWarps * 2 * 2048;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
+};
+
+// ---- epilogue pieces ----------------------------------------------------------------------------------------
+
+// A warp's buffers of 32 rows x 64 bytes, used in turn by the stores that leave through the TMA unit.
+struct Staging {
+  uint8_t* base;
+  uint32_t flip = 0;
+  __device__ __forceinline__ uint8_t* next() {
+    uint8_t* buf = base + flip * 2048;
+    flip ^= 1u;
+    if ((threadIdx.x & 31) == 0) bulk_store_wait_read<1>();
+    __syncwarp();
+    return buf;
+  }
+};
+
+// 32 rows x 64 bytes, one row per lane (four 16-byte pieces), through shared memory to the tensor at (row0, x): 64-byte swizzle.
+__device__ __forceinline__ void store_piece_tma(Staging& st, const CUtensorMap* map, const uint32_t (&w)[16], int32_t x, int32_t row0) {
+  const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  uint8_t* buf = st.next();
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  fence_async_shared();
+  __syncwarp();
+  if (lane == 0) tma_store_2d(map, smem_u32(buf), x, row0);
+}
+
+// The same 32 x 32 bf16 for rows that no TMA store reaches (a pitch or an address that 16 bytes do not divide): a row at a time,
+// 64 contiguous bytes of it by the 32 lanes.
+__device__ __forceinline__ void store_piece_rows(Staging& st, __nv_bfloat16* out, int64_t ld, const uint32_t (&w)[16], int64_t col0, int64_t row0,
+                                                 int64_t M, int64_t N) {
+  const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  uint8_t* buf = st.next();
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  __syncwarp();
+  const bool live = col0 + lane < N;
+  const int rows = M - row0 < 32 ? (int)(M - row0) : 32;
+  for (int r = 0; r < rows; ++r) {
+    const uint8_t* at = buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2;
+    if (live) out[(row0 + r) * ld + col0 + lane] = *reinterpret_cast<const __nv_bfloat16*>(at);
+  }
+  __syncwarp();
+}
+
+// This lane's 32 elements of a row of a bf16 operand of the epilogue, as words; those past N are zero.
+__device__ __forceinline__ void load_row32(const __nv_bfloat16* src, bool vec, int64_t left, uint32_t (&w)[16]) {
+  if (vec && left >= 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+    }
+  } else {
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t lo = 2 * i < left ? __ldg(s + 2 * i) : 0, hi = 2 * i + 1 < left ? __ldg(s + 2 * i + 1) : 0;
+      w[i] = lo | (hi << 16);
+    }
+  }
+}
+
+__device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p, int64_t col0, bool full) {
+  if (p.bias_f32) {
+    const float* b = static_cast<const float*>(p.bias) + col0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += __ldg(b + i);
+  } else {
+    const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.bias) + col0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += __bfloat162float(__ldg(b + i));
+  }
+}
+
+__device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z,
+                                             const uint32_t (&r)[32], int64_t row0, int64_t col0) {
+  const int64_t row = row0 + (threadIdx.x & 31);
+  const bool live = row < p.M, full = col0 + 32 <= p.N;
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  uint32_t w[16];
+  if (p.bias) add_bias32(v, p, col0, full);
+  if (p.z) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    if (p.z_tma) store_piece_tma(st, map_z, w, (int32_t)col0, (int32_t)row0);
+    else store_piece_rows(st, p.z, p.ldz, w, col0, row0, p.M, p.N);
+  }
+  activate_all(p.act, v);
+  if (p.gate) {
+    if (live) {
+      load_row32(p.gate + row * p.ldgate + col0, p.gate_vec, p.N - col0, w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
+    }
+  }
+  if (p.residual) {
+    if (live) {
+      load_row32(p.residual + row * p.ldr + col0, p.residual_vec, p.N - col0, w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+  if (p.d_tma) store_piece_tma(st, map_d, w, (int32_t)col0, (int32_t)row0);
+  else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
+}
+
+// The statistics of this lane's row take 32 more logits: maximum of the chunk, then one exponential per element.
+template <bool kEntropy>
+__device__ __forceinline__ void stats_chunk(const DenseParams& p, RowStats& a, const uint32_t (&r)[32], int64_t col0) {
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * p.scale_log2e;
+  const bool full = col0 + 32 <= p.N;
+  float m = a.m;
+  if (full) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) m = max3(m, v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) if (col0 + i < p.N) m = fmaxf(m, v[i]);
+  }
+  const float base = stats_base(m);
+  const float f = exp2_fast(a.m - base);
+  float s[2] = {0.0f, 0.0f}, e[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (full || col0 + i < p.N) {
+      const float d = v[i] - base;
+      const float x = exp2_fast(d);
+      s[i & 1] += x;
+      if constexpr (kEntropy) e[i & 1] = fmaf(x, fmaxf(d, -1e30f), e[i & 1]);     // (a logit of -infinity adds 0)
+    }
+  }
+  if constexpr (kEntropy) {
+    const float d = a.m == -INFINITY ? 0.0f : a.m - base;
+    a.e = fmaf(f, fmaf(d, a.s, a.e), e[0] + e[1]);
+  }
+  a.s = fmaf(a.s, f, s[0] + s[1]);
+  a.m = m;
+}
+
+// ---- the kernel ---------------------------------------------------------------------------------------------
+
+template <bool kAMn, bool kBMn, int kEpi>
+__global__ void __launch_bounds__(DenseCfg::kThreads, 1)
+dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_z, const DenseParams p) {
+  using Cfg = DenseCfg;
+  constexpr int kStages = Cfg::kStages;
+  constexpr int BN = 256;
+
+  extern __shared__ uint8_t smem_raw[];
+  // the dynamic window starts at the same offset in both CTAs: descriptors and barrier offsets are valid across the pair
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* staging = smem + kStages * Cfg::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + Cfg::kStagingBytes);
+  uint64_t* full = bars;                                   // [kStages]  leader's: all bytes of the stage of both CTAs
+  uint64_t* empty = bars + kStages;                        // [kStages]  local: consumed (commit to both CTAs)
+  uint64_t* acc_full = bars + 2 * kStages;                 // [2]        local: accumulator complete (commit to both CTAs)
+  uint64_t* acc_empty = bars + 2 * kStages + 2;            // [2]        leader's: drained by every epilogue warp of both CTAs
+  uint64_t* drain = bars + 2 * kStages + 4;                // error path only
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();                  // 0 = leader
+  const int64_t pair = blockIdx.x >> 1;
+  const int64_t num_pairs = gridDim.x >> 1;
+  const int64_t tiles_m = (p.M + 255) / 256;
+  const int64_t tiles_n = (p.N + BN - 1) / BN;
+  const int64_t num_tiles = tiles_m * tiles_n;
+  const int iters = (int)((p.K + 63) / 64);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * Cfg::kEpilogueWarps); }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                      // the peer's barriers exist before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();                                  // everything above touches shared and tensor memory only
+
+  if (warp == 0) {
+    // ===== TMA producer (both CTAs): every copy reports to the leader's barrier =====
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t smem_base = smem_u32(smem);
+    const uint32_t full_local = smem_u32(full);
+    const uint32_t full_leader = map_to_cta(full_local, 0);
+    for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      int64_t tm, tn;
+      tile_coords(tile, tiles_m, tiles_n, p.band, tm, tn);
+      const int32_t m0 = (int32_t)(tm * 256 + cta * 128);             // this CTA's rows of A
+      const int32_t n0 = (int32_t)(tn * BN + cta * 128);              // this CTA's rows of B
+      for (int it = 0; it < iters; ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag));
+        if (!ok) {
+          if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_MMA);
+          break;
+        }
+        const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
+        const uint32_t sb = sa + Cfg::kHalfBytes;
+        const uint32_t bar = full_leader + stage * 8;
+        const int32_t k0 = it * 64;
+        if (elect_one()) {
+          if (cta == 0) mbar_expect_tx_addr(full_local + stage * 8, 2 * Cfg::kStageBytes);
+          if (kAMn) {
+            tma_load_2d_pair(sa, &map_a, m0, k0, bar);
+            tma_load_2d_pair(sa + Cfg::kBoxBytes, &map_a, m0 + 64, k0, bar);
+          } else {
+            tma_load_2d_pair(sa, &map_a, k0, m0, bar);
+          }
+          if (kBMn) {
+            tma_load_2d_pair(sb, &map_b, n0, k0, bar);
+            tma_load_2d_pair(sb + Cfg::kBoxBytes, &map_b, n0 + 64, k0, bar);
+          } else {
+            tma_load_2d_pair(sb, &map_b, k0, n0, bar);
+          }
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    grid_launch_dependents();                                // the last loads of this CTA are on their way: let the next kernel's CTAs in
+  } else if (warp == 1) {
+    // ===== tensor-core issuer (leader only) =====
+    if (cta == 0) {
+      int stage = 0;
+      uint32_t phase = 0, local_tile = 0;
+      bool ok = true, issued = false;
+      // descriptor low words: address, and for an MN-major tile the distance between its 64-element boxes as the leading byte offset;
+      // one MMA takes 16 elements of the contraction: 32 bytes along a K-major row, 16 rows of an MN-major tile
+      constexpr uint32_t a_lead = kAMn ? (uint32_t)(Cfg::kBoxBytes >> 4) : 1u, b_lead = kBMn ? (uint32_t)(Cfg::kBoxBytes >> 4) : 1u;
+      constexpr uint32_t a_step = kAMn ? (16u * 128u) >> 4 : 2u, b_step = kBMn ? (16u * 128u) >> 4 : 2u;
+      constexpr uint32_t idesc = idesc_bf16(BN, 256) | (kAMn ? (1u << 15) : 0u) | (kBMn ? (1u << 16) : 0u);
+      const uint32_t smem_base = smem_u32(smem);
+      const uint32_t empty_base = smem_u32(empty);
+      for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local_tile) {
+        const uint32_t buf = local_tile & 1u;
+        if (local_tile > 1) {
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[buf], ((local_tile >> 1) - 1u) & 1u, abort_flag));
+          if (!ok) {
+            if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_EPI);
+            break;
+          }
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * BN;
+        for (int it = 0; it < iters; ++it) {
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[stage], phase, abort_flag));
+          if (!ok) {
+            if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_TMA);
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
+          const uint32_t a_lo = ((sa & 0x3FFFFu) >> 4) | (a_lead << 16);
+          const uint32_t b_lo = (((sa + Cfg::kHalfBytes) & 0x3FFFFu) >> 4) | (b_lead << 16);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tc_mma_bf16_pair(d_tmem, a_lo + a_step * j, b_lo + b_step * j, kOperandDescHi, idesc, (it > 0 || j > 0) ? 1u : 0u);
+            tc_commit_pair(empty_base + stage * 8);
+            if (it == iters - 1) tc_commit_pair(smem_u32(&acc_full[buf]));
+          }
+          issued = true;
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok && issued && elect_one()) {
+        // error path: let the tensor core finish what was issued before tensor memory is freed
+        tc_commit_pair(smem_u32(drain));
+        const uint64_t t0 = global_ns();
+        while (!mbar_try(drain, 0) && global_ns() - t0 < kWaitLimitNs) {}
+      }
+      __syncwarp();
+    }
+  } else {
+    // ===== epilogue (both CTAs): warps 2 to 9; warp w owns tensor-memory lanes 32*(w%4) .. +31 and 128 columns =====
+    const int q = warp & 3;
+    const int part = (warp - 2) >> 2;
+    const uint32_t empty_leader = map_to_cta(smem_u32(acc_empty), 0);
+    Staging st{staging + (warp - 2) * 4096};
+    uint32_t local_tile = 0;
+    for (int64_t tile = pair; tile < num_tiles; tile += num_pairs, ++local_tile) {
+      int64_t tm, tn;
+      tile_coords(tile, tiles_m, tiles_n, p.band, tm, tn);
+      const uint32_t buf = local_tile & 1u;
+      const int64_t row0 = tm * 256 + cta * 128 + q * 32;
+      const int64_t row = row0 + lane;
+      const int64_t n0 = tn * BN + part * 128;
+      const bool rows = row0 < p.M;                        // warp-uniform: the tile's rows of this warp are not all past the end
+      int64_t hit = -1;                                    // the target's column in this launch
+      float lse2 = 0.0f, weight = 0.0f;
+      bool dead = true;
+      if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy || kEpi == kEpiGrad) {
+        if (row < p.M) {
+          const int64_t t = __ldg(p.target + row);
+          if (t != p.ignore && t >= 0 && t < p.vocab) hit = t - p.col0;
+          if constexpr (kEpi == kEpiGrad) {
+            dead = t == p.ignore;
+            lse2 = __ldg(p.lse + row) * kLog2e;
+            weight = __ldg(p.gout + row * p.gout_stride) * p.weight_scale;
+            if (p.inv_count) weight *= __ldg(p.inv_count);
+            if (t < 0 || t >= p.vocab) weight = NAN;       // (a target outside the vocabulary; ignored rows are dead)
+          }
+        }
+      }
+      if (!mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
+        if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_MMA);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * 128;
+      RowStats stats = {-INFINITY, 0.0f, 0.0f};
+      float picked = 0.0f;
+      bool found = false;
+      uint32_t r[2][32];
+      tc_load32(t_row, r[0]);
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {
+        uint32_t(&v)[32] = r[ch & 1];
+        tc_wait_ld(v);
+        if (ch < 3) {
+          tc_load32(t_row + (ch + 1) * 32, r[(ch + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(empty_leader + buf * 8);
+        }
+        const int64_t col0 = n0 + ch * 32;
+        if (rows && col0 < p.N) {
+          const int64_t at = hit - col0;                   // the target's place in this chunk
+          const bool here = at >= 0 && at < 32;
+          if constexpr (kEpi == kEpiLinear) linear_chunk(p, st, &map_d, &map_z, v, row0, col0);
+          if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
+            stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
+            if (here) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) if (at == i) picked = __uint_as_float(v[i]) * p.scale;
+              found = true;
+            }
+          }
+          if constexpr (kEpi == kEpiGrad) {
+            float g[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = exp2_fast(fmaf(__uint_as_float(v[i]), p.scale_log2e, -lse2)) * weight;
+            if (here) {
+              // the one-hot's place: (p - 1) weight
+#pragma unroll
+              for (int i = 0; i < 32; ++i) if (at == i) g[i] -= weight;
+            }
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : pack_bf16(g[2 * i], g[2 * i + 1]);
+            store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+          }
+          if constexpr (kEpi == kEpiSum || kEpi == kEpiSumF32) {
+            float g[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(v[i]);
+            if (p.c && row < p.M) {
+              const float* c = p.c + row * p.ldc + col0;
+              if (col0 + 32 <= p.N) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 f = *reinterpret_cast<const float4*>(c + 4 * i);
+                  g[4 * i] += f.x; g[4 * i + 1] += f.y; g[4 * i + 2] += f.z; g[4 * i + 3] += f.w;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) if (col0 + i < p.N) g[i] += c[i];
+              }
+            }
+            uint32_t w[16];
+            if constexpr (kEpi == kEpiSum) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = pack_bf16(g[2 * i], g[2 * i + 1]);
+              store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(g[16 * h + i]);
+                store_piece_tma(st, &map_d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
+              }
+            }
+          }
+        }
+      }
+      if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
+        if (row < p.M) {
+          const int64_t slot = (tn * 2 + part) * p.M + row;
+          p.stats[slot] = make_float2(stats.m, stats.s);
+          if constexpr (kEpi == kEpiStatsEntropy) p.stats_e[slot] = stats.e;
+          if (found) p.picked[row] = picked;
+        }
+      }
+    }
+    if (lane == 0) bulk_store_wait_all();                    // shared memory stays until the TMA unit has read it
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                      // nobody signals or reads the peer after this
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---- statistics of the pieces into losses ---------------------------------------------------------------------
+
+// nll, lse and entropy of each row from the statistics of its `slots` pieces (slots of a row lie M apart: neighbouring threads read
+// neighbouring rows).  A block takes 32 rows; its eight warps take the slots in turn and are merged in a fixed order.
+template <bool kEntropy>
+__global__ void __launch_bounds__(256)
+head_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ stats_e, const float* __restrict__ picked,
+                 const int64_t* __restrict__ target, int64_t ignore, int64_t vocab, int64_t M, int slots,
+                 float sign, float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ entropy) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  __shared__ RowStats s_part[8][32];
+  RowStats a = {-INFINITY, 0.0f, 0.0f};
+  if (row < M) {
+    constexpr int kFly = 8;                                // loads in flight
+    for (int s0 = warp; s0 < slots; s0 += 8 * kFly) {
+      float2 v[kFly];
+      float e[kFly];
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int s = s0 + 8 * i;
+        v[i] = make_float2(-INFINITY, 0.0f);
+        e[i] = 0.0f;
+        if (s < slots) {
+          v[i] = stats[(int64_t)s * M + row];
+          if constexpr (kEntropy) e[i] = stats_e[(int64_t)s * M + row];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) stats_merge<kEntropy>(a, RowStats{v[i].x, v[i].y, e[i]});
+    }
+  }
+  s_part[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && row < M) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
+    const float all = fmaf(a.m, kLn2, logf(a.s));
+    const int64_t t = target[row];
+    lse[row] = all;
+    nll[row] = t == ignore ? 0.0f : (t < 0 || t >= vocab) ? NAN : sign * (all - picked[row]);
+    // H = log s - sum p (l - m): p = 2^(l - m) / s, l - m in units of log2
+    if constexpr (kEntropy) entropy[row] = logf(a.s) - kLn2 * (a.e / a.s);
+  }
+}
+
+// loss = sum of nll, or that over the number of rows that are not ignored; inv_count = 1 / that number (1 for the sum).  One block,
+// fixed order.
+__global__ void __launch_bounds__(1024)
+head_sum_kernel(const float* __restrict__ nll, const int64_t* __restrict__ target, int64_t ignore, int64_t M, int mean,
+                float* __restrict__ loss, float* __restrict__ inv_count) {
+  grid_dependency_wait();
+  __shared__ double s_sum[32];
+  __shared__ unsigned long long s_count[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sum = 0.0;
+  unsigned long long count = 0;
+  for (int64_t i = threadIdx.x; i < M; i += 1024) {
+    sum += (double)nll[i];
+    count += target[i] != ignore;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if (lane == 0) { s_sum[warp] = sum; s_count[warp] = count; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) { sum += s_sum[w]; count += s_count[w]; }
+    *loss = (float)(mean ? sum / (double)count : sum);     // (no row at all: 0 / 0, as torch has it)
+    *inv_count = mean ? (float)(1.0 / (double)count) : 1.0f;
+  }
+}
+
+// ---- backward of the epilogue -----------------------------------------------------------------------------------
+
+// dz = dy * gate * act'(z), dgate = dy * act(z), and column sums of dz before its rounding.  A warp's lane has kVec columns of a row,
+// the block's eight warps take eight rows at a time; a block owns 32 * kVec columns and every gridDim.y-th group of rows.
+template <int kAct, int kVec>
+__global__ void __launch_bounds__(256)
+linear_pointwise_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, const __nv_bfloat16* __restrict__ z, int64_t ldz,
+                        const __nv_bfloat16* __restrict__ gate, int64_t ldgate, int64_t M, int64_t N,
+                        __nv_bfloat16* __restrict__ dz, int64_t lddz, __nv_bfloat16* __restrict__ dgate, int64_t lddg,
+                        float* __restrict__ sums) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * kVec;
+  float acc[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
+  auto load = [](const __nv_bfloat16* at, float (&v)[kVec]) {
+    if constexpr (kVec == 8) Load8<__nv_bfloat16>::load(at, v);
+    else v[0] = __bfloat162float(__ldg(at));
+  };
+  auto store = [](__nv_bfloat16* at, const float (&v)[kVec]) {
+    if constexpr (kVec == 8) *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    else *at = __float2bfloat16_rn(v[0]);
+  };
+  if (col < N) {
+    for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < M; row += (int64_t)gridDim.y * 8) {
+      float d[kVec], a[kVec], out[kVec];
+      load(dy + row * lddy + col, d);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) { a[i] = 1.0f; out[i] = d[i]; }
+      if (kAct != METIS_ACT_NONE || dgate) {
+        float zv[kVec];
+        load(z + row * ldz + col, zv);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          float slope;
+          activate_both<kAct>(zv[i], a[i], slope);
+          out[i] = d[i] * slope;
+        }
+      }
+      if (gate) {
+        float g[kVec];
+        load(gate + row * ldgate + col, g);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) out[i] *= g[i];
+      }
+      if (dgate) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) a[i] *= d[i];
+        store(dgate + row * lddg + col, a);
+      }
+      if (dz) store(dz + row * lddz + col, out);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) acc[i] += out[i];
+    }
+  }
+  if (sums) {
+    __shared__ float s_sum[8][32 * kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) s_sum[warp][lane * kVec + i] = acc[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * kVec; c += 256) {
+      float t = s_sum[0][c];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) t += s_sum[w][c];
+      const int64_t at = (int64_t)blockIdx.x * 32 * kVec + c;
+      if (at < N) sums[(int64_t)blockIdx.y * N + at] = t;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_bias_kernel(const float* __restrict__ sums, int groups, int64_t N, T* __restrict__ out) {
+  grid_dependency_wait();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  float t = 0.0f;
+#pragma unroll 8
+  for (int g = 0; g < groups; ++g) t += sums[(int64_t)g * N + c];
+  if constexpr (sizeof(T) == 2) out[c] = __float2bfloat16_rn(t);
+  else out[c] = t;
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------
+
+static int32_t check_rows(const void* p, int64_t ld, int64_t cols, const char* what) {
+  if (!p) return fail(METIS_ERR_BAD_ARGUMENT, "%s is null", what);
+  if (!aligned16(p) || ld < cols || ld % 8 != 0) return fail(METIS_ERR_BAD_ALIGNMENT, "%s must be 16-byte aligned with a leading dimension that is a multiple of 8", what);
+  return METIS_OK;
+}
+// coordinates of a copy are 32 bits
+static int32_t check_extent(int64_t n, const char* what) {
+  if (n <= 0) return fail(METIS_ERR_BAD_SHAPE, "%s = %lld must be positive", what, (long long)n);
+  if (n >= ((int64_t)1 << 31) - 512) return fail(METIS_ERR_TOO_LARGE, "%s = %lld does not fit 32 bits", what, (long long)n);
+  return METIS_OK;
+}
+
+struct DenseOperand {
+  const void* p;
+  int64_t ld;
+  bool mn;                                                 // the contraction lies in the rows
+};
+
+template <bool kAMn, bool kBMn, int kEpi>
+static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const CUtensorMap& map_d, const CUtensorMap& map_z, DenseParams p, cudaStream_t st) {
+  const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap ma, mb;
+  if (kAMn) { if (int32_t rc = make_map(&ma, dt, 2, a.p, p.M, p.K, a.ld * 2, 64, 64, "A (MN-major)")) return rc; }
+  else      { if (int32_t rc = make_map(&ma, dt, 2, a.p, p.K, p.M, a.ld * 2, 64, 128, "A (K-major)")) return rc; }
+  if (kBMn) { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.N, p.K, b.ld * 2, 64, 64, "B (MN-major)")) return rc; }
+  else      { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.K, p.N, b.ld * 2, 64, 128, "B (K-major)")) return rc; }
+  p.band = 8;
+  const int64_t tiles = ceil_div(p.M, 256) * ceil_div(p.N, 256);
+  int64_t pairs = device_sm_count() / 2;
+  if (pairs > tiles) pairs = tiles;
+  pairs = ceil_div(tiles, ceil_div(tiles, pairs));         // the fewest that finish in the same number of rounds
+  auto kern = dense_gemm_pair_kernel<kAMn, kBMn, kEpi>;
+  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DenseCfg::kSmemBytes));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(DenseCfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = DenseCfg::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = launch_overlap_enabled(kLaunchGemm) ? 2 : 1;
+  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_z, p));
+  return METIS_OK;
+}
+
+static int32_t map_bf16_out(CUtensorMap* map, void* d, int64_t ld, int64_t M, int64_t N, const char* what) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, d, N, M, ld * 2, 32, 32, what, 64);
+}
+
+// D (bf16 or fp32) = A B^T + C, gradients: (A K-major, B MN-major) or (both MN-major)
+static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M, int64_t N, int64_t K, const float* c, int64_t ldc,
+                         void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st) {
+  DenseParams p = {};
+  p.M = M; p.N = N; p.K = K; p.status = status; p.c = c; p.ldc = ldc;
+  CUtensorMap md = {}, mz = {};
+  if (d_f32) {
+    if (int32_t rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
+    return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, md, mz, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, md, mz, p, st);
+  }
+  if (int32_t rc = map_bf16_out(&md, d, ldd, M, N, "D")) return rc;
+  return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, mz, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, mz, p, st);
+}
+
+// Columns of the vocabulary that the backward pass takes at a time: their gradients G [M, columns] in bf16 go through memory.
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+static int64_t piece_columns(int64_t M, int64_t V) {
+  int64_t columns = kPieceBytes / (2 * M) / 256 * 256;
+  if (columns < 256) columns = 256;
+  if (columns >= V) return ceil_div(V, 8) * 8;
+  return ceil_div(ceil_div(V, ceil_div(V, columns)), 256) * 256;       // pieces of one size
+}
+
+}  // namespace metis
+
+using namespace metis;
+
+extern "C" int32_t metis_linear(const metis_linear_args* a) {
+  if (!a) return fail(METIS_ERR_BAD_ARGUMENT, "args is null");
+  if (int32_t rc = check_extent(a->M, "M")) return rc;
+  if (int32_t rc = check_extent(a->N, "N")) return rc;
+  if (int32_t rc = check_extent(a->K, "K")) return rc;
+  if (a->K % 8 != 0) return fail(METIS_ERR_BAD_SHAPE, "K = %lld must be a multiple of 8", (long long)a->K);
+  if (a->activation < METIS_ACT_NONE || a->activation > METIS_ACT_GELU_TANH) return fail(METIS_ERR_BAD_ARGUMENT, "unknown activation %d", a->activation);
+  if (a->bias && a->bias_dtype != METIS_DTYPE_BF16 && a->bias_dtype != METIS_DTYPE_F32) return fail(METIS_ERR_BAD_ARGUMENT, "unknown bias_dtype %d", a->bias_dtype);
+  if (int32_t rc = check_rows(a->x, a->ldx, a->K, "x")) return rc;
+  if (int32_t rc = check_rows(a->w, a->ldw, a->K, "w")) return rc;
+  if (!a->y) return fail(METIS_ERR_BAD_ARGUMENT, "y is null");
+  if (a->ldy < a->N || (a->z && a->ldz < a->N) || (a->gate && a->ldgate < a->N) || (a->residual && a->ldr < a->N))
+    return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
+  DenseParams p = {};
+  p.M = a->M; p.N = a->N; p.K = a->K; p.status = a->status;
+  p.bias = a->bias; p.bias_f32 = a->bias_dtype == METIS_DTYPE_F32; p.act = a->activation;
+  auto wide = [](const void* t, int64_t ld) { return aligned16(t) && ld % 8 == 0; };
+  p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_vec = wide(a->gate, a->ldgate);
+  p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_vec = wide(a->residual, a->ldr);
+  p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_tma = wide(a->y, a->ldy);
+  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_tma = a->z && wide(a->z, a->ldz);
+  CUtensorMap md = {}, mz = {};
+  if (p.d_tma) if (int32_t rc = map_bf16_out(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
+  if (p.z_tma) if (int32_t rc = map_bf16_out(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
+  return launch_dense<false, false, kEpiLinear>({a->x, a->ldx, false}, {a->w, a->ldw, false}, md, mz, p, reinterpret_cast<cudaStream_t>(a->stream));
+}
+
+constexpr int kPointwiseGroups = 64;
+extern "C" int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N) {
+  if (M <= 0 || N <= 0) return 0;
+  return kPointwiseGroups * N * (int64_t)sizeof(float);
+}
+
+template <int kAct>
+static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool vec, dim3 grid, float* sums) {
+  auto launch = [&](auto kern) {
+    return launch_overlapped(kLaunchStream, kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(a->stream),
+                             static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __nv_bfloat16*>(a->z), a->ldz,
+                             static_cast<const __nv_bfloat16*>(a->gate), a->ldgate, a->M, a->N, static_cast<__nv_bfloat16*>(a->dz), a->lddz,
+                             static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
+  };
+  METIS_CUDA_OK(vec ? launch(linear_pointwise_kernel<kAct, 8>) : launch(linear_pointwise_kernel<kAct, 1>));
+  return METIS_OK;
+}
+
+extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) {
+  if (!a) return fail(METIS_ERR_BAD_ARGUMENT, "args is null");
+  if (int32_t rc = check_extent(a->M, "M")) return rc;
+  if (int32_t rc = check_extent(a->N, "N")) return rc;
+  if (!a->dy || (!a->dz && !a->dgate && !a->dbias)) return fail(METIS_ERR_BAD_ARGUMENT, "dy is null, or nothing is asked for");
+  if (a->activation < METIS_ACT_NONE || a->activation > METIS_ACT_GELU_TANH) return fail(METIS_ERR_BAD_ARGUMENT, "unknown activation %d", a->activation);
+  if ((a->activation != METIS_ACT_NONE || a->dgate) && !a->z) return fail(METIS_ERR_BAD_ARGUMENT, "z is null");
+  if (a->dbias && a->dbias_dtype != METIS_DTYPE_BF16 && a->dbias_dtype != METIS_DTYPE_F32) return fail(METIS_ERR_BAD_ARGUMENT, "unknown dbias_dtype %d", a->dbias_dtype);
+  if (a->lddy < a->N || (a->z && a->ldz < a->N) || (a->gate && a->ldgate < a->N) || (a->dz && a->lddz < a->N) || (a->dgate && a->lddg < a->N))
+    return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
+  if (a->dbias && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_linear_pointwise_workspace_bytes(a->M, a->N)))
+    return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
+  auto wide = [](const void* t, int64_t ld) { return !t || (aligned16(t) && ld % 8 == 0); };
+  const bool vec = a->N % 8 == 0 && wide(a->dy, a->lddy) && wide(a->z, a->ldz) && wide(a->gate, a->ldgate) && wide(a->dz, a->lddz) && wide(a->dgate, a->lddg);
+  const int64_t columns = ceil_div(a->N, vec ? 256 : 32);
+  // with sums no more groups of rows than the workspace has; else about 16 blocks for each SM
+  int64_t groups = ceil_div(a->M, 8), most = ceil_div((int64_t)device_sm_count() * 16, columns);
+  if (a->dbias && most > kPointwiseGroups) most = kPointwiseGroups;
+  if (groups > most) groups = most;
+  if (groups > 65535) groups = 65535;
+  float* sums = a->dbias ? static_cast<float*>(a->workspace) : nullptr;
+  const dim3 grid((unsigned)columns, (unsigned)groups);
+  int32_t rc = METIS_OK;
+  switch (a->activation) {
+    case METIS_ACT_SILU: rc = launch_pointwise<METIS_ACT_SILU>(a, vec, grid, sums); break;
+    case METIS_ACT_GELU: rc = launch_pointwise<METIS_ACT_GELU>(a, vec, grid, sums); break;
+    case METIS_ACT_GELU_TANH: rc = launch_pointwise<METIS_ACT_GELU_TANH>(a, vec, grid, sums); break;
+    default: rc = launch_pointwise<METIS_ACT_NONE>(a, vec, grid, sums);
+  }
+  if (rc || !a->dbias) return rc;
+  const dim3 blocks((unsigned)ceil_div(a->N, 256));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  if (a->dbias_dtype == METIS_DTYPE_BF16)
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, linear_bias_kernel<__nv_bfloat16>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<__nv_bfloat16*>(a->dbias)));
+  else
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, linear_bias_kernel<float>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<float*>(a->dbias)));
+  return METIS_OK;
+}
+
+extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
+                                      void* d, int64_t ldd, int32_t* status, void* stream) {
+  if (int32_t rc = check_extent(M, "M")) return rc;
+  if (int32_t rc = check_extent(N, "N")) return rc;
+  if (int32_t rc = check_extent(K, "K")) return rc;
+  if (int32_t rc = check_rows(a, lda, a_mn_major ? M : K, "a")) return rc;
+  if (int32_t rc = check_rows(b, ldb, N, "b")) return rc;
+  if (int32_t rc = check_rows(d, ldd, N, "d")) return rc;
+  return dense_sum({a, lda, a_mn_major != 0}, {b, ldb, true}, M, N, K, nullptr, 0, d, false, ldd, status, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ---- head ---------------------------------------------------------------------------------------------------------
+
+static int32_t check_head(const metis_head_args* a) {
+  if (!a) return fail(METIS_ERR_BAD_ARGUMENT, "args is null");
+  if (int32_t rc = check_extent(a->M, "M")) return rc;
+  if (int32_t rc = check_extent(a->V, "V")) return rc;
+  if (int32_t rc = check_extent(a->K, "K")) return rc;
+  if (a->K % 8 != 0) return fail(METIS_ERR_BAD_SHAPE, "K = %lld must be a multiple of 8", (long long)a->K);
+  if (int32_t rc = check_rows(a->h, a->ldh, a->K, "h")) return rc;
+  if (int32_t rc = check_rows(a->w, a->ldw, a->K, "w")) return rc;
+  if (a->negate != 0 && a->negate != 1) return fail(METIS_ERR_BAD_ARGUMENT, "negate must be 0 or 1");
+  if (!a->target || !a->lse) return fail(METIS_ERR_BAD_ARGUMENT, "target or lse is null");
+  return METIS_OK;
+}
+static DenseParams head_params(const metis_head_args* a) {
+  DenseParams p = {};
+  p.M = a->M; p.N = a->V; p.K = a->K; p.status = a->status;
+  p.target = a->target; p.ignore = a->ignore_index; p.vocab = a->V;
+  p.weight_scale = a->negate ? -a->scale : a->scale;
+  p.scale = a->scale; p.scale_log2e = a->scale * 1.4426950408889634f;
+  return p;
+}
+static int64_t head_slots(int64_t V) { return 2 * ceil_div(V, 256); }
+
+extern "C" int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy) {
+  if (M <= 0 || V <= 0 || K <= 0) return 0;
+  return ceil_div(M * 4, 16) * 16 + head_slots(V) * M * (entropy ? 12 : 8);
+}
+
+extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) {
+  if (int32_t rc = check_head(a)) return rc;
+  if (!nll) return fail(METIS_ERR_BAD_ARGUMENT, "nll is null");
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_loss_workspace_bytes(a->M, a->V, a->K, entropy != nullptr))
+    return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  DenseParams p = head_params(a);
+  const int64_t slots = head_slots(a->V);
+  p.picked = static_cast<float*>(a->workspace);
+  p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + ceil_div(a->M * 4, 16) * 16);
+  p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
+  const DenseOperand h = {a->h, a->ldh, false}, w = {a->w, a->ldw, false};
+  const CUtensorMap none = {};
+  if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, none, p, st)) return rc;
+  const dim3 blocks((unsigned)ceil_div(a->M, 32));
+  auto rows = entropy ? head_rows_kernel<true> : head_rows_kernel<false>;
+  METIS_CUDA_OK(launch_overlapped(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
+                                  a->target, a->ignore_index, a->V, a->M, (int)slots, a->negate ? -1.0f : 1.0f, nll, a->lse, entropy));
+  return METIS_OK;
+}
+
+extern "C" int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_index, int64_t M, int32_t mean, float* loss, float* inv_count, void* stream) {
+  if (int32_t rc = check_extent(M, "M")) return rc;
+  if (!nll || !target || !loss || !inv_count) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
+  METIS_CUDA_OK(launch_overlapped(kLaunchShort, head_sum_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), nll, target, ignore_index, M, (int)(mean != 0), loss, inv_count));
+  return METIS_OK;
+}
+
+extern "C" int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K) {
+  if (M <= 0 || V <= 0 || K <= 0) return 0;
+  const int64_t columns = piece_columns(M, V);
+  return ceil_div(2 * M * columns, 256) * 256 + (columns < V ? 4 * M * K : 0);
+}
+
+extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* gout, int32_t gout_stride, const float* inv_count,
+                                       void* dh, int64_t lddh, void* dw, int64_t lddw) {
+  if (int32_t rc = check_head(a)) return rc;
+  if (!gout || (!dh && !dw)) return fail(METIS_ERR_BAD_ARGUMENT, "gout is null, or nothing is asked for");
+  if (gout_stride != 0 && gout_stride != 1) return fail(METIS_ERR_BAD_ARGUMENT, "gout_stride must be 0 or 1");
+  if (dh) if (int32_t rc = check_rows(dh, lddh, a->K, "dh")) return rc;
+  if (dw) if (int32_t rc = check_rows(dw, lddw, a->K, "dw")) return rc;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_backward_workspace_bytes(a->M, a->V, a->K))
+    return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  const int64_t columns = piece_columns(a->M, a->V);
+  __nv_bfloat16* g = static_cast<__nv_bfloat16*>(a->workspace);
+  float* acc = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + ceil_div(2 * a->M * columns, 256) * 256);
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a->w);
+  DenseParams p = head_params(a);
+  p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride; p.inv_count = inv_count;
+  for (int64_t v0 = 0; v0 < a->V; v0 += columns) {
+    const int64_t n = a->V - v0 < columns ? a->V - v0 : columns;
+    const bool last = v0 + n == a->V;
+    CUtensorMap mg, none = {};
+    p.N = n;
+    p.col0 = v0;
+    if (int32_t rc = map_bf16_out(&mg, g, columns, a->M, n, "G")) return rc;
+    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, mg, none, p, st)) return rc;
+    if (dh) {
+      if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
+                                 last ? dh : acc, !last, last ? lddh : a->K, a->status, st)) return rc;
+    }
+    if (dw) {
+      if (int32_t rc = dense_sum({g, columns, true}, {a->h, a->ldh, true}, n, a->K, a->M, nullptr, 0,
+                                 static_cast<__nv_bfloat16*>(dw) + v0 * lddw, false, lddw, a->status, st)) return rc;
+    }
+  }
+  return METIS_OK;
+}

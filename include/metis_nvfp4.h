@@ -53,6 +53,12 @@ extern "C" {
 #define METIS_DTYPE_BF16 0
 #define METIS_DTYPE_F32  1
 
+/* activations of metis_linear */
+#define METIS_ACT_NONE      0
+#define METIS_ACT_SILU      1
+#define METIS_ACT_GELU      2  /* z Phi(z), the erf form */
+#define METIS_ACT_GELU_TANH 3
+
 /* scale-factor layouts */
 #define METIS_SF_ROWMAJOR 0
 #define METIS_SF_MMA      1
@@ -441,6 +447,91 @@ int32_t metis_rope_pair(const void* q, const void* k, const void* cos, const voi
                         void* stream);
 /* out = bf16(bf16(silu(gate)) * up) for n bf16 elements (a multiple of 8). */
 int32_t metis_silu_mul(const void* gate, const void* up, void* out, int64_t n, void* stream);
+
+/* ---- products that stay in bf16: linear layer with its epilogue -------------------------------------------- */
+
+/*
+ * y = act(x W^T + bias) * gate + residual, x [M, K], W [N, K], y [M, N], all bf16, sums in fp32, one rounding at the end.
+ * bias (bf16 or fp32 [N]), gate and residual ([M, N]) may be null; z, where given, receives bf16(x W^T + bias), from which
+ * metis_linear_pointwise forms the gradients.  x and w: 16-byte aligned rows (leading dimensions multiples of 8), K a
+ * multiple of 8; the others any, 16-byte aligned rows being the fast ones.  What nn.Linear and the elementwise kernels behind
+ * it do for a projection that replace_linear_with_metis leaves as it is (src/grpo/grpo.py:119-196, target_modules).
+ */
+typedef struct metis_linear_args {
+  int64_t M, N, K;
+  const void* x;  int64_t ldx;
+  const void* w;  int64_t ldw;
+  const void* bias;  int32_t bias_dtype;
+  int32_t activation;       /* METIS_ACT_* */
+  const void* gate;      int64_t ldgate;
+  const void* residual;  int64_t ldr;
+  void* y;  int64_t ldy;
+  void* z;  int64_t ldz;
+  int32_t* status;          /* optional device int32: 0, or a METIS_DEV_* code */
+  void* stream;
+} metis_linear_args;
+int32_t metis_linear(const metis_linear_args* args);
+
+/*
+ * Gradients through that epilogue: dz = bf16(dy * gate * act'(z)), dgate = bf16(dy * act(z)), dbias = sum over rows of
+ * dy * gate * act'(z) in fp32, rounded once.  Each output may be null; gate null: 1.  z is not read where neither the
+ * activation nor dgate needs it.  The workspace is for dbias alone.
+ */
+typedef struct metis_linear_pointwise_args {
+  int64_t M, N;
+  const void* dy;    int64_t lddy;
+  const void* z;     int64_t ldz;
+  const void* gate;  int64_t ldgate;
+  void* dz;     int64_t lddz;
+  void* dgate;  int64_t lddg;
+  void* dbias;  int32_t dbias_dtype;
+  int32_t activation;
+  void* workspace;  int64_t workspace_bytes;
+  void* stream;
+} metis_linear_pointwise_args;
+int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N);
+int32_t metis_linear_pointwise(const metis_linear_pointwise_args* args);
+
+/*
+ * D [M, N] = A B^T in bf16, sums in fp32: b is [K, N], a is [M, K] (a_mn_major = 0: an input's gradient, dz W) or [K, M]
+ * (1: a weight's, dz^T x).  All three have 16-byte aligned rows.
+ */
+int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
+                           int64_t K, void* d, int64_t ldd, int32_t* status, void* stream);
+
+/* ---- head: losses over the vocabulary without the logits ----------------------------------------------------- */
+
+/*
+ * l = scale * h W^T [M, V] with h [M, K] and W [V, K] in bf16; l is formed tile by tile in fp32 and not stored.
+ * metis_head_loss: lse[m] = log sum_j exp l[m][j]; nll[m] = lse[m] - l[m][target[m]], 0 where target[m] = ignore_index, NaN
+ * where it is no other index of the vocabulary; entropy (optional) = lse - sum_j p l.  h and w as x and w of metis_linear.
+ */
+typedef struct metis_head_args {
+  int64_t M, V, K;
+  const void* h;  int64_t ldh;
+  const void* w;  int64_t ldw;
+  const int64_t* target;
+  int64_t ignore_index;
+  float scale;
+  int32_t negate;           /* 1: nll holds -nll, the target's log-probability, and gout is the gradient of that */
+  float* lse;               /* [M]: written by metis_head_loss, read by metis_head_backward */
+  void* workspace;  int64_t workspace_bytes;     /* 16-byte aligned */
+  int32_t* status;
+  void* stream;
+} metis_head_args;
+int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy);
+int32_t metis_head_loss(const metis_head_args* args, float* nll, float* entropy);
+/* loss = sum of nll, over the number of rows that are not ignored where mean is set; *inv_count = 1 over that number, or 1. */
+int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_index, int64_t M, int32_t mean, float* loss,
+                       float* inv_count, void* stream);
+/*
+ * dh [M, K] = G W and dw [V, K] = G^T h (bf16, either may be null) with G[m][j] = scale * g_m (softmax(l)[m][j] - [j = target[m]]),
+ * g_m = gout[m * gout_stride] * (inv_count ? *inv_count : 1), 0 where target[m] = ignore_index.  The logits are formed
+ * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, dh's sum over the pieces in fp32.
+ */
+int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K);
+int32_t metis_head_backward(const metis_head_args* args, const float* gout, int32_t gout_stride, const float* inv_count,
+                            void* dh, int64_t lddh, void* dw, int64_t lddw);
 
 #ifdef __cplusplus
 }

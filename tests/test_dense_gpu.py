@@ -1,0 +1,333 @@
+"""The bf16 products with their epilogues and the head's losses (fp4_post_b200/dense.py) against plain torch in 64 bits.
+
+Tolerances count roundings: a bf16 output is off by at most half a step, 2^-8 of its value; sums of K products in fp32 by at most
+K 2^-23 of the sum of their magnitudes (each addition rounds or cuts at 2^-23 of what it adds up to); gradients that pass through a bf16
+intermediate (dz, the logits' gradient, the z that act' is taken at) by 2^-8 for each, independent from element to element, so that the
+2-norm of a product's error is that part of its norm."""
+import math
+
+import pytest
+import torch
+
+from fp4_post_b200 import dense, ops
+
+pytestmark = pytest.mark.gpu
+STEP = 2.0 ** -8
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib(built_library):
+    return built_library
+
+
+def normal(*shape, scale=1.0, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def act64(name, z):
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "gelu":
+        return z * 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+    if name == "gelu_tanh":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z
+
+
+def rel(a, b):
+    return float((a.double() - b).norm() / b.norm().clamp(min=1e-300))
+
+
+def linear64(x, w, b, act, gate, residual):
+    z = x @ w.t()
+    if b is not None:
+        z = z + b
+    y = act64(act, z)
+    if gate is not None:
+        y = y * gate
+    if residual is not None:
+        y = y + residual
+    return y
+
+
+def check_linear(M, N, K, act=None, bias=None, gate=False, residual=False, grad=True, seed=0, prefix=()):
+    prefix = prefix or (M,)
+    x, w, dy = normal(*prefix, K, seed=seed), normal(N, K, scale=K ** -0.5, seed=seed + 1), normal(*prefix, N, seed=seed + 2)
+    b = None if bias is None else normal(N, seed=seed + 3, dtype=bias)
+    g = normal(*prefix, N, seed=seed + 4) if gate else None
+    r = normal(*prefix, N, seed=seed + 5) if residual else None
+    leaves = [t for t in (x, w, b, g, r) if t is not None]
+    copies = [None if t is None else t.detach().double().requires_grad_(grad) for t in (x, w, b, g, r)]
+    want = linear64(copies[0].reshape(-1, K), copies[1], copies[2], act, *(None if t is None else t.reshape(-1, N) for t in copies[3:]))
+    if grad:
+        for t in leaves:
+            t.requires_grad_(True)
+        y = dense.linear(x, w, b, activation=act, gate=g, residual=r)
+        grads = torch.autograd.grad(y, leaves, dy)
+    else:
+        y = dense.linear(x, w, b, activation=act, gate=g, residual=r)
+    assert y.shape == (*prefix, N) and y.dtype == torch.bfloat16
+    with torch.no_grad():
+        # the value's own rounding and the sum's error, through an activation of slope at most 1.13 and the gate
+        slack = (K * 2.0 ** -23 * (copies[0].reshape(-1, K).abs() @ copies[1].abs().t()) + 2.0 ** -22 * (0 if b is None else copies[2].abs())) * 1.13
+        # ... whose own functions are good to 2^-20 of their value
+        slack = slack + 2.0 ** -20 * act64(act, (copies[0].reshape(-1, K) @ copies[1].t()) + (0 if b is None else copies[2])).abs()
+        if gate:
+            slack = slack * copies[3].reshape(-1, N).abs()
+        tol = STEP * want.abs() + slack * (1 + STEP) + 1e-30
+        assert ((y.double().reshape(-1, N) - want).abs() <= tol).all()
+    if grad:
+        exact = torch.autograd.grad(want, [t for t in copies if t is not None], dy.double().reshape(-1, N))
+        for t, got, ref in zip(leaves, grads, exact):
+            assert got.shape == t.shape and got.dtype == t.dtype
+            # its own rounding, that of dz and that of z
+            assert rel(got.reshape(ref.shape), ref) <= 3 * STEP, (tuple(t.shape), rel(got.reshape(ref.shape), ref))
+        if residual:
+            assert torch.equal(grads[-1], dy)
+
+
+@pytest.mark.parametrize("act", [None, "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("gate,residual,bias", [(False, False, None), (True, True, torch.bfloat16), (False, True, torch.float32), (True, False, None)])
+def test_linear_and_its_gradients(act, gate, residual, bias):
+    check_linear(300, 520, 264, act, bias, gate, residual)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 8), (1, 33, 64), (2, 7, 16), (3, 8, 8), (17, 1003, 520), (64, 256, 64), (128, 130, 1000), (129, 129, 136), (255, 257, 72),
+                                   (256, 256, 256), (257, 511, 24), (1021, 769, 40), (33, 2049, 3592), (700, 64, 2048)])
+def test_linear_of_every_size(M, N, K):
+    check_linear(M, N, K, "silu", torch.bfloat16, True, True, seed=M)
+    check_linear(M, N, K, seed=N)
+
+
+def test_linear_of_more_tiles_than_pairs():
+    check_linear(2500, 2600, 192, "gelu", torch.float32, False, True)
+
+
+def test_linear_keeps_leading_dimensions():
+    check_linear(0, 136, 64, "silu", None, True, True, prefix=(2, 3, 5))
+    x, w = normal(64), normal(24, 64, seed=1)
+    assert torch.equal(dense.linear(x, w), dense.linear(x[None], w)[0])
+
+
+def test_linear_reads_pitched_and_misaligned_rows():
+    M, N, K = 150, 200, 128
+    base, w, g = normal(M, 3 * K + 8), normal(N, 2 * K, seed=1), normal(M, 2 * N + 3, seed=2)
+    for x in (base[:, K:2 * K], base[:, 3:3 + K], base[::2, :K].repeat(2, 1)[:M], base.t()[:K].t(), base[:1, :K].expand(M, K)):
+        for weight in (w[:, :K], w[:, 5:5 + K], w.t()[:K].t()):
+            for gate in (g[:, :N], g[:, 1:1 + N], g[:, ::2][:, :N]):
+                got = dense.linear(x, weight, activation="silu", gate=gate, residual=gate)
+                assert torch.equal(got, dense.linear(x.clone().contiguous(), weight.clone().contiguous(), activation="silu",
+                                                     gate=gate.clone().contiguous(), residual=gate.clone().contiguous()))
+
+
+def test_linear_of_no_rows():
+    x, w, b, r = normal(0, 64), normal(24, 64, seed=1), normal(24, seed=2), normal(0, 24, seed=3)
+    for t in (x, w, b, r):
+        t.requires_grad_(True)
+    y = dense.linear(x, w, b, activation="silu", residual=r)
+    assert y.shape == (0, 24)
+    gx, gw, gb, gr = torch.autograd.grad(y, (x, w, b, r), torch.empty_like(y))
+    assert gx.shape == x.shape and gr.shape == r.shape and not gw.any() and not gb.any()
+
+
+def test_linear_gradients_of_some_inputs_only():
+    M, N, K = 70, 72, 64
+    x, w, b, g = normal(M, K), normal(N, K, seed=1), normal(N, seed=2), normal(M, N, seed=3)
+    dy = normal(M, N, seed=4)
+    every = [t.clone().requires_grad_(True) for t in (x, w, b, g)]
+    want = torch.autograd.grad(dense.linear(*every[:3], activation="gelu", gate=every[3]), every, dy)
+    for i in range(4):
+        some = [t.clone().requires_grad_(i == j) for j, t in enumerate((x, w, b, g))]
+        got, = torch.autograd.grad(dense.linear(*some[:3], activation="gelu", gate=some[3]), some[i], dy)
+        assert torch.equal(got, want[i])
+    # a gradient that is one value for all, as that of a sum
+    y = dense.linear(*every[:3], activation="gelu", gate=every[3])
+    got = torch.autograd.grad(y.sum(), every)
+    want = torch.autograd.grad(dense.linear(*every[:3], activation="gelu", gate=every[3]), every, torch.ones_like(y))
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_linear_with_infinities_and_nan():
+    x, w = normal(40, 64), normal(48, 64, seed=1).abs()
+    x[3, 5] = float("inf")
+    x[4, 5] = float("nan")
+    for act in (None, "silu", "gelu", "gelu_tanh"):
+        y = dense.linear(x, w, activation=act)
+        assert torch.isinf(y[3]).all() and torch.isnan(y[4]).all() and torch.isfinite(y[5:]).all() and torch.isfinite(y[:3]).all()
+    # far tails: nothing overflows into NaN
+    far = torch.tensor([[-60000.0], [-300.0], [-90.0], [-20.0], [0.0], [20.0], [90.0], [60000.0]], device="cuda").bfloat16().expand(8, 8).contiguous()
+    eye = torch.eye(8, device="cuda").bfloat16()
+    for act in ("silu", "gelu", "gelu_tanh"):
+        want = act64(act, far.double())
+        got = dense.linear(far, eye, activation=act).double()
+        assert torch.isfinite(got).all() and ((got - want).abs() <= STEP * want.abs() * 1.01 + 1e-30).all()
+
+
+# ---- head -------------------------------------------------------------------------------------------------------
+
+def head64(h, w, t, temperature, ignore_index=-100):
+    logits = (h @ w.t()) / temperature
+    logp = torch.log_softmax(logits, dim=1)
+    live = t != ignore_index
+    picked = logp.gather(1, torch.where(live, t, 0)[:, None])[:, 0]
+    return torch.where(live, picked, 0.0), -(logp.exp() * logp).sum(dim=1), logits
+
+
+def head_inputs(M, V, K, ignored=0.2, seed=0, size=2.0):
+    h, w = normal(M, K, seed=seed), normal(V, K, scale=size * K ** -0.5, seed=seed + 1)
+    g = torch.Generator(device="cuda").manual_seed(seed + 2)
+    t = torch.randint(0, V, (M,), device="cuda", generator=g)
+    t[torch.rand(M, device="cuda", generator=g) < ignored] = -100
+    t[0] = V - 1
+    return h, w, t
+
+
+def check_head_gradients(got, exact, h64, w64, logits, g, t, temperature, tol):
+    """Two roundings: the gradient's own and that of the logits' gradient G = g / T (p - [j = t]).  And p = exp(l - lse) is off by the
+    error of its argument, at most 2 tol (1 + tol) p, before the one-hot is taken from it: where p is near 1 (a vocabulary of one token) G itself
+    is nearly nothing and that error is what there is.  It reaches dh as (2 tol p |g| / T) |W| at most, dw as its transpose by |h|."""
+    with torch.no_grad():
+        p = torch.softmax(logits, dim=1) * (torch.where(t != -100, g.double(), 0.0).abs() / temperature).expand(logits.shape[0])[:, None]
+        reach = ((p @ w64.abs()).norm(), (p.t() @ h64.abs()).norm())
+        for a, e, r in zip(got, exact, reach):
+            assert a.dtype == torch.bfloat16 and a.shape == e.shape
+            assert float((a.double() - e).norm()) <= 2 * STEP * float(e.norm()) + 4 * tol * float(r)
+
+
+def check_head(M, V, K, temperature=1.0, seed=0, ignored=0.2):
+    h, w, t = head_inputs(M, V, K, ignored, seed)
+    h64, w64 = h.double().requires_grad_(True), w.double().requires_grad_(True)
+    logp, entropy, logits = head64(h64, w64, t, temperature)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    # the error of a logit, and what the sum over the vocabulary and its logarithm add
+    with torch.no_grad():
+        tol = (K * 2.0 ** -23 * (h64.abs() @ w64.abs().t()).max() / temperature + 2.0 ** -20 * (1 + logits.abs().max())).item()
+    g = normal(M, seed=seed + 5, dtype=torch.float32)
+
+    got, ent = dense.token_logprobs(h, w, t, temperature=temperature, entropy=True)
+    assert got.dtype == torch.float32 and got.shape == t.shape and not ent.requires_grad
+    assert (got.double() - logp).abs().max() <= 2 * tol
+    assert (ent.double() - entropy).abs().max() <= (2 + 2 * math.log(V)) * tol
+    assert not got[t == -100].any()
+    for upstream, forms in ((g, "none"), (torch.tensor(0.7, device="cuda"), "sum"), (torch.tensor(0.7, device="cuda"), "mean")):
+        loss = dense.linear_cross_entropy(h, w, t, reduction=forms, temperature=temperature)
+        want = -logp if forms == "none" else -logp.sum() if forms == "sum" else -logp.sum() / (t != -100).sum()
+        assert loss.shape == want.shape and loss.dtype == torch.float32
+        assert (loss.double() - want).abs().max() <= 2 * tol * (M if forms == "sum" else 1) + 2.0 ** -23 * float(want.detach().abs().max())
+        grads = torch.autograd.grad(loss, (h, w), upstream)
+        exact = torch.autograd.grad(want, (h64, w64), upstream.double(), retain_graph=True)
+        rows = upstream / (t != -100).sum() if forms == "mean" else upstream
+        check_head_gradients(grads, exact, h64, w64, logits, rows, t, temperature, tol)
+    back = torch.autograd.grad(got, (h, w), g)
+    exact = torch.autograd.grad(logp, (h64, w64), g.double())
+    check_head_gradients(back, exact, h64, w64, logits.detach(), g, t, temperature, tol)
+
+
+@pytest.mark.parametrize("M,V,K", [(1, 2, 8), (1, 97, 64), (3, 1, 8), (24, 97, 64), (16, 4099, 256), (33, 256, 72), (128, 257, 64), (129, 1000, 128), (257, 513, 1000),
+                                   (300, 5003, 96), (1021, 777, 40), (2, 30001, 64), (64, 6000, 3584)])
+def test_losses_and_their_gradients(M, V, K):
+    check_head(M, V, K, seed=M + V)
+    check_head(M, V, K, temperature=0.6, ignored=0.0, seed=M)
+
+
+def test_losses_over_many_tiles():
+    check_head(700, 40003, 128)
+
+
+def test_gradients_over_several_pieces_of_the_vocabulary(monkeypatch):
+    # 65536 rows take the vocabulary in pieces of 4096 columns: 9001 of them are three
+    M, V, K = 65536, 9001, 16
+    h, w, t = head_inputs(M, V, K)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = dense.linear_cross_entropy(h, w, t, reduction="sum")
+    got = torch.autograd.grad(loss, (h, w))
+    h64, w64 = h.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    logp, _, _ = head64(h64, w64, t, 1.0)
+    exact = torch.autograd.grad(-logp.sum(), (h64, w64))
+    for a, e in zip(got, exact):
+        assert rel(a, e) <= 2 * STEP
+
+
+def test_rows_that_are_ignored():
+    h, w, t = head_inputs(50, 300, 64)
+    t[:] = -100
+    h[7] = float("nan")                                   # a padded row may hold anything
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    assert not dense.linear_cross_entropy(h, w, t, reduction="none").any()
+    loss = dense.linear_cross_entropy(h, w, t, reduction="sum")
+    assert loss == 0
+    dh, = torch.autograd.grad(loss, h)
+    assert not dh.any()
+    assert torch.isnan(dense.linear_cross_entropy(h, w, t))
+    t[3] = 5
+    a = dense.linear_cross_entropy(h, w, t)
+    b = dense.linear_cross_entropy(h, w, torch.where(t == -100, 299, t), ignore_index=299)
+    assert torch.isfinite(a) and torch.equal(a, b)
+    # int32 targets, leading dimensions
+    c = dense.linear_cross_entropy(h.view(2, 25, 64), w, t.view(2, 25).int())
+    assert torch.equal(a, c)
+
+
+def test_targets_outside_the_vocabulary_give_nan_and_nothing_else():
+    h, w, t = head_inputs(40, 300, 64, ignored=0.0)
+    good = dense.linear_cross_entropy(h, w, t, reduction="none")
+    for bad in (300, -1, 1 << 40, -(1 << 62)):
+        u = t.clone()
+        u[5] = bad
+        hh = h.clone().requires_grad_(True)
+        loss = dense.linear_cross_entropy(hh, w, u, reduction="none")
+        assert torch.isnan(loss[5]) and torch.equal(loss[:5], good[:5]) and torch.equal(loss[6:], good[6:])
+        dh, = torch.autograd.grad(loss, hh, torch.ones_like(loss))
+        assert torch.isnan(dh[5]).all() and torch.isfinite(dh[:5]).all() and torch.isfinite(dh[6:]).all()
+
+
+def test_extreme_logits():
+    h, w, t = head_inputs(64, 1000, 64, ignored=0.0)
+    big = (h.float() * 3000).bfloat16()                    # logits of thousands: one token takes it all
+    logp, entropy, logits = head64(big.double(), w.double(), t, 1.0)
+    got, ent = dense.token_logprobs(big, w, t, entropy=True)
+    tol = 64 * 2.0 ** -23 * float((big.double().abs() @ w.double().abs().t()).max()) + 2.0 ** -20 * float(logits.abs().max())
+    assert (got.double() - logp).abs().max() <= 2 * tol and torch.isfinite(ent).all() and (ent >= -1e-3).all()
+    same = dense.token_logprobs(torch.zeros_like(h), w, t, entropy=True)       # all logits equal
+    assert (same[0] + math.log(1000)).abs().max() <= 1e-5 and (same[1] - math.log(1000)).abs().max() <= 1e-5
+    h[9, 3] = float("inf")
+    got = dense.linear_cross_entropy(h, w, t, reduction="none")
+    assert torch.isnan(got[9]) and torch.isfinite(got[:9]).all() and torch.isfinite(got[10:]).all()
+
+
+def test_losses_of_no_rows():
+    h, w, t = normal(0, 64), normal(100, 64, seed=1), torch.empty(0, dtype=torch.int64, device="cuda")
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    assert dense.linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+    loss = dense.linear_cross_entropy(h, w, t, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    assert loss == 0 and dh.shape == h.shape and not dw.any()
+    assert torch.isnan(dense.linear_cross_entropy(h, w, t))
+    logp, ent = dense.token_logprobs(h, w, t, entropy=True)
+    assert logp.shape == ent.shape == (0,)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------
+
+def test_what_the_calls_refuse():
+    x, w, t = normal(4, 64), normal(24, 64, seed=1), torch.zeros(4, dtype=torch.int64, device="cuda")
+    y = normal(4, 24)
+    cases = [(ValueError, lambda: dense.linear(x, w[:, :56])), (ValueError, lambda: dense.linear(x[:, :60].contiguous(), w[:, :60].contiguous())),
+             (ValueError, lambda: dense.linear(x, w, y[0, :23])), (ValueError, lambda: dense.linear(x, w, gate=y[:1])), (ValueError, lambda: dense.linear(x, w, residual=y[0])),
+             (TypeError, lambda: dense.linear(x.float(), w)), (TypeError, lambda: dense.linear(x, w.half())), (TypeError, lambda: dense.linear(x, w, y[0].half())),
+             (TypeError, lambda: dense.linear(x, w, gate=y.float())), (ValueError, lambda: dense.linear(x, w, activation="tanh")),
+             (ValueError, lambda: dense.linear(x, w, gate=y.cpu())), (ValueError, lambda: dense.linear(x, w[:0])),
+             (ValueError, lambda: dense.linear_cross_entropy(x, w, t[:3])), (TypeError, lambda: dense.linear_cross_entropy(x, w, t.float())),
+             (TypeError, lambda: dense.linear_cross_entropy(x.float(), w, t)), (TypeError, lambda: dense.linear_cross_entropy(x, w.float(), t)),
+             (ValueError, lambda: dense.linear_cross_entropy(x, w, t, temperature=0.0)), (ValueError, lambda: dense.linear_cross_entropy(x, w, t, temperature=float("nan"))),
+             (ValueError, lambda: dense.linear_cross_entropy(x, w.cpu(), t)), (ValueError, lambda: dense.token_logprobs(x, w, t.cpu())),
+             (ValueError, lambda: dense.token_logprobs(x, w[:0], t)), (ValueError, lambda: ops.bf16_product(x, w))]
+    for i, (error, call) in enumerate(cases):
+        with pytest.raises(error):
+            call()
+            raise AssertionError(f"case {i} was not refused")
