@@ -15,7 +15,7 @@ struct DenseParams {
   int32_t act;
   const __nv_bfloat16* gate;      int64_t ldgate;  int32_t gate_vec;       // *_vec: rows of 16-byte pieces
   const __nv_bfloat16* residual;  int64_t ldr;     int32_t residual_vec;
-  __nv_bfloat16* d;               int64_t ldd;     int32_t d_tma;          // *_tma: stored by the TMA unit
+  __nv_bfloat16* d;               int64_t ldd;     int32_t d_tma;          // *_tma: rows that the TMA unit can store
   __nv_bfloat16* z;               int64_t ldz;     int32_t z_tma;
   // head: logits l = scale * (A B^T); columns of the vocabulary [0, N) of this launch are [col0, col0 + N) of all
   const int64_t* target;  int64_t ignore;

@@ -621,6 +621,11 @@ linear_bias_kernel(const float* __restrict__ sums, int groups, int64_t N, T* __r
 
 // ---- host side ------------------------------------------------------------------------------------------------
 
+// dense_small.cu
+int32_t launch_dense_small(const void* t, int64_t ldt, const void* w, bool w_mn, int64_t ldw, const DenseParams& p, cudaStream_t st);
+int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int64_t ldw, const DenseParams& p, cudaStream_t st);
+int64_t small_stats_slots(int64_t V);
+
 static int32_t check_rows(const void* p, int64_t ld, int64_t cols, const char* what) {
   if (!p) return fail(METIS_ERR_BAD_ARGUMENT, "%s is null", what);
   if (!aligned16(p) || ld < cols || ld % 8 != 0) return fail(METIS_ERR_BAD_ALIGNMENT, "%s must be 16-byte aligned with a leading dimension that is a multiple of 8", what);
@@ -690,6 +695,14 @@ static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M
   return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, mz, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, mz, p, st);
 }
 
+// Whether a product of M tokens goes to the kernels for few of them (dense_small.cu).
+static bool few_tokens(int64_t M, int64_t N, int64_t K) {
+#ifdef METIS_TIMING_KNOBS
+  if (const char* e = getenv("METIS_DEV_DENSE_SMALL")) return atoi(e) != 0;
+#endif
+  return M <= 128;
+}
+
 // Columns of the vocabulary that the backward pass takes at a time: their gradients G [M, columns] in bf16 go through memory.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 static int64_t piece_columns(int64_t M, int64_t V) {
@@ -724,6 +737,7 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_vec = wide(a->residual, a->ldr);
   p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_tma = wide(a->y, a->ldy);
   p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_tma = a->z && wide(a->z, a->ldz);
+  if (few_tokens(a->M, a->N, a->K)) return launch_dense_small(a->x, a->ldx, a->w, false, a->ldw, p, reinterpret_cast<cudaStream_t>(a->stream));
   CUtensorMap md = {}, mz = {};
   if (p.d_tma) if (int32_t rc = map_bf16_out(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
   if (p.z_tma) if (int32_t rc = map_bf16_out(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
@@ -795,6 +809,12 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (int32_t rc = check_rows(a, lda, a_mn_major ? M : K, "a")) return rc;
   if (int32_t rc = check_rows(b, ldb, N, "b")) return rc;
   if (int32_t rc = check_rows(d, ldd, N, "d")) return rc;
+  if (!a_mn_major && few_tokens(M, N, K)) {
+    DenseParams p = {};
+    p.M = M; p.N = N; p.K = K; p.status = status;
+    p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_tma = 1;
+    return launch_dense_small(a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
+  }
   return dense_sum({a, lda, a_mn_major != 0}, {b, ldb, true}, M, N, K, nullptr, 0, d, false, ldd, status, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -820,11 +840,12 @@ static DenseParams head_params(const metis_head_args* a) {
   p.scale = a->scale; p.scale_log2e = a->scale * 1.4426950408889634f;
   return p;
 }
-static int64_t head_slots(int64_t V) { return 2 * ceil_div(V, 256); }
+constexpr int64_t kFewRows = 64;                           // rows of a head that the weight's read bounds
+static int64_t head_slots(int64_t M, int64_t V) { return M <= kFewRows ? small_stats_slots(V) : 2 * ceil_div(V, 256); }
 
 extern "C" int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
-  return ceil_div(M * 4, 16) * 16 + head_slots(V) * M * (entropy ? 12 : 8);
+  return ceil_div(M * 4, 16) * 16 + head_slots(M, V) * M * (entropy ? 12 : 8);
 }
 
 extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) {
@@ -834,13 +855,15 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
   DenseParams p = head_params(a);
-  const int64_t slots = head_slots(a->V);
+  const int64_t slots = head_slots(a->M, a->V);
   p.picked = static_cast<float*>(a->workspace);
   p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + ceil_div(a->M * 4, 16) * 16);
   p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
   const DenseOperand h = {a->h, a->ldh, false}, w = {a->w, a->ldw, false};
   const CUtensorMap none = {};
-  if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, none, p, st)) return rc;
+  if (a->M <= kFewRows) {
+    if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
+  } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, none, p, st)) return rc;
   const dim3 blocks((unsigned)ceil_div(a->M, 32));
   auto rows = entropy ? head_rows_kernel<true> : head_rows_kernel<false>;
   METIS_CUDA_OK(launch_overlapped(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
