@@ -2,8 +2,8 @@
 
     python -m fp4_post_b200.build        # or: from fp4_post_b200.build import build; build()
 
-Output: fp4_post_b200/_lib/libmetis_nvfp4.so, and cabi.HOST_PATH, the native part of the tensor-level wrappers (g++ against the
-installed torch and Python, whose versions are in its name).  nvcc cross-compiles without a GPU.
+Output: fp4_post_b200/_lib/libmetis_nvfp4.so, and cabi.HOST_PATH and cabi.DENSE_PATH, the native parts of the tensor-level wrappers
+and of dense.py (g++ against the installed torch and Python, whose versions are in their names).  nvcc cross-compiles without a GPU.
 
     python -m fp4_post_b200.build --timing-knobs
 
@@ -22,7 +22,7 @@ import sys
 import sysconfig
 from pathlib import Path
 
-from .cabi import HOST_PATH
+from .cabi import DENSE_PATH, HOST_PATH
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -30,6 +30,7 @@ OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libmetis_nvfp4.so"
 KNOBS_LIB = OUT_DIR / "libmetis_nvfp4_knobs.so"
 HOST_SOURCE = CSRC / "host_ops.cpp"
+DENSE_SOURCE = CSRC / "dense_host.cpp"
 SOURCES = ["api.cu", "quantize.cu", "rmsnorm_quant.cu", "dequantize.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "lowrank_bwd.cu", "decoder_ops.cu", "dense_gemm.cu", "dense_small.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,12 +54,12 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def _host_command() -> list[str]:
+def _host_command(source: Path = HOST_SOURCE, target: Path = HOST_PATH, libraries: tuple = ()) -> list[str]:
     import torch
     root = Path(torch.__file__).resolve().parent
-    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"]]
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], Path(_nvcc()).resolve().parent.parent / "include"]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *(f"-I{p}" for p in include), str(HOST_SOURCE), "-o", str(HOST_PATH), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            *(f"-I{p}" for p in include), str(source), "-o", str(target), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", *libraries]
 
 
 def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False) -> Path:
@@ -81,9 +82,10 @@ def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False
                 cmd.insert(1, "-Xptxas=-v")
                 print(" ".join(cmd), file=sys.stderr)
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-    host = None
-    if not timing_knobs and (force or _stale(HOST_PATH, [HOST_SOURCE, PKG.parent / "include" / "metis_nvfp4.h"])):
-        host = subprocess.Popen(_host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    hosts = []
+    for source, target, libraries in ((HOST_SOURCE, HOST_PATH, ()), (DENSE_SOURCE, DENSE_PATH, ("-lc10_cuda",))):
+        if not timing_knobs and (force or _stale(target, [source, PKG.parent / "include" / "metis_nvfp4.h"])):
+            hosts.append((source, subprocess.Popen(_host_command(source, target, libraries), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -91,10 +93,10 @@ def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False
             print(out, file=sys.stderr)
         if p.returncode != 0:
             failed.append((src, out))
-    if host is not None:
+    for source, host in hosts:
         out, _ = host.communicate()
         if host.returncode != 0:
-            raise RuntimeError(f"g++ failed:\n--- {HOST_SOURCE.name} ---\n{out}")
+            raise RuntimeError(f"g++ failed:\n--- {source.name} ---\n{out}")
     if failed:
         raise RuntimeError("nvcc failed:\n" + "\n".join(f"--- {s} ---\n{o}" for s, o in failed))
     if force or procs or _stale(lib, objs):

@@ -15,11 +15,12 @@ import torch                # the native wrappers below link against it: it has 
 # The native part of the wrappers is compiled against one torch and one Python: their versions are in its name, so that no other
 # loads it and build.py makes one for each.
 HOST_PATH = Path(__file__).resolve().parent / "_lib" / f"metis_host-{sysconfig.get_config_var('SOABI')}-torch-{torch.__version__}.so"
+DENSE_PATH = HOST_PATH.with_name(HOST_PATH.name.replace("metis_host", "metis_dense", 1))
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmetis_nvfp4.so"
 
 DTYPE_BF16, DTYPE_F32 = 0, 1
 SF_ROWMAJOR, SF_MMA = 0, 1
-ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
 Q_TRANSPOSE, Q_STOCHASTIC, Q_OFFSET_ON_DEVICE, Q_HADAMARD = 1, 2, 4, 8
 Q_DEFER_ROWMAJOR, Q_DEFER_TRANSPOSED, Q_SR16 = 16, 32, 64
 QUANTIZE_EXTRA_WORKSPACE = 8192
@@ -105,6 +106,8 @@ class HeadArgs(C.Structure):
 _lib = None
 _host = None
 _host_lib = None            # the library whose entry points _host has
+_dense = None
+_dense_lib = None
 
 
 class MetisLibraryError(RuntimeError):
@@ -205,19 +208,36 @@ def lib() -> C.CDLL:
     return L
 
 
+def _native(name: str, path: Path):
+    if not path.exists():
+        raise MetisLibraryError(f"{path} is missing: build it with `python -m fp4_post_b200.build` under this Python and torch")
+    spec = importlib.util.spec_from_file_location(name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def _bind(module, L: C.CDLL) -> None:
+    for name in EXPORTS:
+        module.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
+
+
 def _bind_host() -> None:
     global _host, _host_lib
     L = lib()
     if _host is None:
-        if not HOST_PATH.exists():
-            raise MetisLibraryError(f"{HOST_PATH} is missing: build it with `python -m fp4_post_b200.build` under this Python and torch")
-        spec = importlib.util.spec_from_file_location("metis_host", HOST_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _host = module
-    for name in EXPORTS:
-        _host.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
+        _host = _native("metis_host", HOST_PATH)
+    _bind(_host, L)
     _host_lib = L
+
+
+def _bind_dense() -> None:
+    global _dense, _dense_lib
+    L = lib()
+    if _dense is None:
+        _dense = _native("metis_dense", DENSE_PATH)
+    _bind(_dense, L)
+    _dense_lib = L
 
 
 def host():
@@ -226,6 +246,18 @@ def host():
     if _host_lib is None or _host_lib is not _lib:
         _bind_host()
     return _host
+
+
+def dense_host():
+    """The native part of dense.py (csrc/dense_host.cpp), with the entry points of lib()."""
+    if _dense_lib is None or _dense_lib is not _lib:
+        _bind_dense()
+    return _dense
+
+
+def dense_launches() -> int:
+    """Kernels that dense.py's calls have launched since import."""
+    return 0 if _dense is None else _dense.launches()
 
 
 def check(rc: int, what: str) -> None:

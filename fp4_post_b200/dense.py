@@ -5,9 +5,11 @@
     token_logprobs         log-probabilities of given tokens under that head (and its entropy): what a policy-gradient step
                            takes of the policy and of its reference model
 
-All three run on tcgen05 kernels of this library (csrc/dense_gemm.cu) and need CUDA tensors; nothing here computes on the CPU.
-Operands are bfloat16, sums and softmax statistics fp32.  The inner size is a multiple of 8; rows may have any pitch that 16 bytes
-divide (others are copied first).  A call runs on the current stream of its tensors' device and can be captured in a CUDA graph.
+All three run on tcgen05 kernels of this library (csrc/dense_gemm.cu, csrc/dense_small.cu for few tokens) and need CUDA tensors;
+nothing here computes on the CPU.  Operands are bfloat16, sums and softmax statistics fp32.  The inner size is a multiple of 8; rows may
+have any pitch that 16 bytes divide (others are copied first).  A call runs on the current stream of its tensors' device and can be
+captured in a CUDA graph.  The calls and their gradients are native (csrc/dense_host.cpp); what is here is what they refuse, and the
+copies of tensors that the kernels cannot read as they lie.
 The reference leaves all of this to torch (nn.Linear, F.cross_entropy and TRL's selective log-softmax around src/grpo/grpo.py:199-215).
 """
 from __future__ import annotations
@@ -15,52 +17,40 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import cabi
+
+_ACTIVATIONS = {None: cabi.ACT_NONE, "silu": cabi.ACT_SILU, "gelu": cabi.ACT_GELU, "gelu_tanh": cabi.ACT_GELU_TANH}
+_FORMS = {"none": 0, "sum": 1, "mean": 2}
+_LOGPROBS = 3
 
 
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, gate, residual, activation):
-        needs_x, needs_w, needs_b, needs_gate, _, _ = ctx.needs_input_grad
-        keep_z = needs_gate or (activation is not None and (needs_x or needs_w or needs_b))
-        out = ops.linear(x, weight, bias, activation=activation, gate=gate, residual=residual, return_preactivation=keep_z)
-        y, z = out if keep_z else (out, None)
-        ctx.activation = activation
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.save_for_backward(x if needs_w else None, weight if needs_x else None, gate if needs_x or needs_w or needs_b else None, z)
-        ctx.x_shape, ctx.n = x.shape, weight.shape[0]
-        return y
+def _check(t, what: str, device: Optional[torch.device] = None, dtypes=(torch.bfloat16,)) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor, not {type(t).__name__}")
+    if device is None and not t.is_cuda:
+        raise RuntimeError(f"{what} must be a CUDA tensor: the bf16 products have no CPU fallback")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)}, got {t.dtype}")
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, gate, z = ctx.saved_tensors
-        needs_x, needs_w, needs_b, needs_gate, needs_residual, _ = ctx.needs_input_grad
-        n, k = ctx.n, ctx.x_shape[-1]
-        dy2 = dy.reshape(-1, n)
-        rows = dy2.shape[0]
-        dx = dw = db = dgate = None
-        if rows == 0:
-            dx = dy.new_zeros(ctx.x_shape) if needs_x else None
-            dw = dy.new_zeros((n, k)) if needs_w else None
-            db = dy.new_zeros(n, dtype=ctx.bias_dtype) if needs_b else None
-            return dx, dw, db, dy if needs_gate else None, dy if needs_residual else None, None
-        product = needs_x or needs_w
-        gate2 = None if gate is None else gate.reshape(-1, n)
-        # the gradient itself where nothing changes it and its rows can be read as they lie
-        dz = dy2
-        changed = product and (ctx.activation is not None or gate is not None or n % 8 != 0)
-        if changed or needs_b or needs_gate:
-            dz_new, dgate, db = ops.linear_pointwise(dy2, z, gate2, ctx.activation, want_dz=changed, want_dgate=needs_gate,
-                                                     bias_dtype=ctx.bias_dtype if needs_b else None)
-            dz = dz_new if changed else dz
-        if needs_x:
-            dx = ops.bf16_product(dz, weight).view(ctx.x_shape)
-        if needs_w:
-            dw = ops.bf16_product(dz, x.reshape(-1, k), a_mn_major=True)
-        return dx, dw, db, None if dgate is None else dgate.view(dy.shape), dy if needs_residual else None, None
+
+def _check_product(x, weight, what: str) -> None:
+    _check(x, what)
+    _check(weight, "weight", x.device)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"shapes do not fit: {what} {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8 != 0:
+        raise ValueError(f"weight {tuple(weight.shape)}: the inner size must be a positive multiple of 8")
+
+
+def _readable(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t with contiguous elements on an address that 16 bytes divide."""
+    if t is None:
+        return None
+    t = t.resolve_neg().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
@@ -71,74 +61,52 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     [..., N] (no broadcasting).  activation: None, "silu", "gelu" (erf form) or "gelu_tanh".  A SwiGLU block is
     linear(linear(h, w_gate, activation="silu", gate=linear(h, w_up)), w_down, residual=x).
     Differentiable once in all tensors; the backward pass keeps bf16(x @ weight.T + bias)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, gate, residual)):
-        return _Linear.apply(x, weight, bias, gate, residual, activation)
-    return ops.linear(x, weight, bias, activation=activation, gate=gate, residual=residual)
-
-
-class _HeadLoss(torch.autograd.Function):
-    """form: "none" (a loss for each row), "sum", "mean", or "logprobs" (a log-probability for each row, and perhaps entropies)."""
-
-    @staticmethod
-    def forward(ctx, h, w, target, ignore_index, scale, form, entropy):
-        ctx.set_materialize_grads(False)
-        negate = form == "logprobs"
-        nll, lse, ent = ops.head_loss(h, w, target, ignore_index=ignore_index, scale=scale, negate=negate, entropy=entropy)
-        inv_count = None
-        if form in ("sum", "mean"):
-            nll, inv_count = ops.head_sum(nll, target, ignore_index=ignore_index, mean=form == "mean")
-        ctx.save_for_backward(h, w, target, lse, inv_count)
-        ctx.options = dict(ignore_index=ignore_index, scale=scale, negate=negate)
-        if ent is not None:
-            ctx.mark_non_differentiable(ent)
-        return nll, ent
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _gent):
-        if g is None:
-            return None, None, None, None, None, None, None
-        h, w, target, lse, inv_count = ctx.saved_tensors
-        dh, dw = ops.head_backward(h, w, target, lse, g, inv_count=inv_count, want_dh=ctx.needs_input_grad[0],
-                                   want_dw=ctx.needs_input_grad[1], **ctx.options)
-        return dh, dw, None, None, None, None, None
+    try:
+        code = _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', not {activation!r}") from None
+    host = cabi.dense_host()
+    out = host.linear(x, weight, bias, gate, residual, code)
+    if out is not None:
+        return out
+    _check_product(x, weight, "x")
+    if bias is not None:
+        _check(bias, "bias", x.device, (torch.bfloat16, torch.float32))
+        if bias.shape != weight.shape[:1]:
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, not ({weight.shape[0]},)")
+    shape = (*x.shape[:-1], weight.shape[0])
+    for name, t in (("gate", gate), ("residual", residual)):
+        if t is not None:
+            _check(t, name, x.device)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, not that of the output, {shape}")
+    out = host.linear(*(_readable(t) for t in (x, weight, bias, gate, residual)), code)
+    if out is None:
+        raise RuntimeError("linear cannot read these tensors")
+    return out
 
 
 def _head(hidden, weight, target, ignore_index, temperature, form, entropy):
-    ops._need_cuda(hidden, "hidden")
-    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
-        raise ValueError(f"shapes do not fit: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}")
-    if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8 != 0:
-        raise ValueError(f"weight {tuple(weight.shape)}: the inner size must be a positive multiple of 8")
-    if target.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"targets must be int64 or int32, got {target.dtype}")
+    scale = 1.0 / temperature if temperature else 0.0
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, not {temperature}")
+    host = cabi.dense_host()
+    out = host.head(hidden, weight, target, ignore_index, scale, form, entropy)
+    if out is not None:
+        return out
+    _check_product(hidden, weight, "hidden")
+    _check(target, "target", hidden.device, (torch.int64, torch.int32))
     if target.shape != hidden.shape[:-1]:
         raise ValueError(f"targets have shape {tuple(target.shape)}, hidden states {tuple(hidden.shape)}")
-    temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, not {temperature}")
-    ops._same_device(hidden, weight=weight, target=target)
-    for name, t in (("hidden", hidden), ("weight", weight)):
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-    with ops._on_device(hidden.device):
-        h, w = ops._operand_rows(hidden, "hidden"), ops._operand_rows(weight, "weight")
-        t = target.reshape(-1).to(torch.int64).contiguous()
-        if t.numel() == 0:
-            # nothing to do, but the graph stays connected: the gradients are zeros
-            rows = h.sum(dim=-1).float() * 0.0 + w.sum() * 0.0
-            out = rows.sum() / (0.0 if form == "mean" else 1.0) if form in ("sum", "mean") else rows.view(target.shape)
-            return out, rows.detach().view(target.shape)
-        if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
-            out, ent = _HeadLoss.apply(h, w, t, int(ignore_index), 1.0 / temperature, form, entropy)
-        else:
-            negate = form == "logprobs"
-            out, _, ent = ops.head_loss(h, w, t, ignore_index=int(ignore_index), scale=1.0 / temperature, negate=negate, entropy=entropy)
-            if form in ("sum", "mean"):
-                out = ops.head_sum(out, t, ignore_index=int(ignore_index), mean=form == "mean")[0]
-    if out.dim() == 1:
-        out = out.view(target.shape)
-    return out, None if ent is None else ent.view(target.shape)
+    if target.numel() == 0:
+        # nothing to do, but the graph stays connected: the gradients are zeros
+        rows = hidden.sum(dim=-1, dtype=torch.float32) + (weight[:1].float() * 0.0).sum()
+        out = rows if form in (_FORMS["none"], _LOGPROBS) else rows.sum() / (0.0 if form == _FORMS["mean"] else 1.0)
+        return out, rows.detach()
+    out = host.head(_readable(hidden), _readable(weight), target.to(torch.int64).contiguous(), ignore_index, scale, form, entropy)
+    if out is None:
+        raise RuntimeError("the head's losses cannot read these tensors")
+    return out
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
@@ -149,9 +117,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     into each row's maximum and sum; the backward pass forms them again, piece by piece of the vocabulary, and differentiates
     hidden and weight (once).  A target that is neither ignore_index nor in the vocabulary makes its loss NaN.  The mean over no
     row at all is NaN, as torch has it."""
-    if reduction not in ("mean", "sum", "none"):
-        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
-    return _head(hidden, weight, target, ignore_index, temperature, reduction, False)[0]
+    try:
+        form = _FORMS[reduction]
+    except (KeyError, TypeError):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}") from None
+    return _head(hidden, weight, target, ignore_index, temperature, form, False)[0]
 
 
 def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor, *, temperature: float = 1.0, entropy: bool = False,
@@ -159,5 +129,5 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor
     """log softmax(hidden @ weight.T / temperature) at the given token ids, fp32, shaped like ids; 0 where ids is ignore_index.
 
     With entropy=True also the entropy of each row's distribution (ignored rows included), which carries no gradient."""
-    out, ent = _head(hidden, weight, ids, ignore_index, temperature, "logprobs", entropy)
-    return (out, ent) if entropy else out
+    out = _head(hidden, weight, ids, ignore_index, temperature, _LOGPROBS, entropy)
+    return out if entropy else out[0]

@@ -19,11 +19,11 @@ _DTYPES = {torch.bfloat16: cabi.DTYPE_BF16, torch.float32: cabi.DTYPE_F32}
 # Kernels of this library launched since import, by entry point (two per quantizer call: the
 # streaming pass and the scale pass; a memset in front of them is not a kernel).  The quantizers and the column
 # mean have one-launch forms for small inputs; those calls are counted as two all the same.
-LAUNCHES = {"quantize": 0, "rmsnorm_quantize": 0, "dequantize": 0, "col_mean": 0, "gemv": 0, "gemm": 0, "lowrank_bwd": 0, "decoder": 0, "dense": 0}
+LAUNCHES = {"quantize": 0, "rmsnorm_quantize": 0, "dequantize": 0, "col_mean": 0, "gemv": 0, "gemm": 0, "lowrank_bwd": 0, "decoder": 0}
 
 
 def launch_count() -> int:
-    return sum(LAUNCHES.values())
+    return sum(LAUNCHES.values()) + cabi.dense_launches()          # (dense.py's calls are counted where they are made)
 
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:
@@ -637,198 +637,3 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     cabi.check(rc, "metis_silu_mul")
     LAUNCHES["decoder"] += 1
     return out
-
-
-# ---- products that stay in bf16 (the differentiable calls are in dense.py) ----------------------------------------
-
-def _operand_rows(t: torch.Tensor, what: str) -> torch.Tensor:
-    """t viewed as a bf16 matrix of 16-byte aligned rows, copied only if it has to be."""
-    _need_cuda(t, what)
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{what} must be bfloat16, got {t.dtype}")
-    t = _rows2d(t)
-    if t.data_ptr() % 16 != 0 or (t.shape[0] > 1 and t.stride(0) % 8 != 0):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Leading dimension of a matrix with contiguous rows (a single row may have any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _epilogue_rows(t: Optional[torch.Tensor], what: str, like: torch.Tensor, shape) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{what} must be bfloat16, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, not that of the output, {tuple(shape)}")
-    _same_device(like, **{what: t})
-    return _rows2d(t)
-
-
-def _linear_shapes(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]):
-    _need_cuda(x, "x")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    N, K = weight.shape
-    if N == 0 or K == 0 or K % 8 != 0:
-        raise ValueError(f"weight {tuple(weight.shape)}: the inner size must be a positive multiple of 8")
-    _same_device(x, weight=weight)
-    if bias is not None:
-        if bias.shape != (N,):
-            raise ValueError(f"bias has shape {tuple(bias.shape)}, not ({N},)")
-        _dtype_code(bias, "bias")
-        _same_device(x, bias=bias)
-    return N, K
-
-
-def _activation_code(activation: Optional[str]) -> int:
-    try:
-        return cabi.ACTIVATIONS[activation]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', not {activation!r}") from None
-
-
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
-           gate: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, return_preactivation: bool = False,
-           status: Optional[torch.Tensor] = None):
-    """act(x @ weight.T + bias) * gate + residual for bf16 x [..., K] and weight [N, K] in one launch, rounded once.  bias: bf16 or
-    fp32 [N]; gate, residual: bf16, shaped like the output.  With return_preactivation also bf16(x @ weight.T + bias).  No autograd."""
-    code = _activation_code(activation)
-    N, K = _linear_shapes(x, weight, bias)
-    shape = (*x.shape[:-1], N)
-    gate, residual = _epilogue_rows(gate, "gate", x, shape), _epilogue_rows(residual, "residual", x, shape)
-    x2, w = _operand_rows(x, "x"), _operand_rows(weight, "weight")
-    M = x2.shape[0]
-    with _on_device(x.device):
-        y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
-        z = torch.empty_like(y) if return_preactivation else None
-        if M > 0:
-            a = cabi.LinearArgs(M=M, N=N, K=K, x=x2.data_ptr(), ldx=_pitch(x2), w=w.data_ptr(), ldw=_pitch(w), activation=code,
-                                y=y.data_ptr(), ldy=N, status=_ptr(status), stream=_stream())
-            if bias is not None:
-                bias = bias.contiguous()
-                a.bias, a.bias_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
-            if gate is not None:
-                a.gate, a.ldgate = gate.data_ptr(), _pitch(gate)
-            if residual is not None:
-                a.residual, a.ldr = residual.data_ptr(), _pitch(residual)
-            if z is not None:
-                a.z, a.ldz = z.data_ptr(), N
-            cabi.check(cabi.lib().metis_linear(a), "metis_linear")
-            LAUNCHES["dense"] += 1
-    y = y.view(shape)
-    return (y, z) if return_preactivation else y
-
-
-def linear_pointwise(dy: torch.Tensor, z: Optional[torch.Tensor], gate: Optional[torch.Tensor], activation: Optional[str], *, want_dz: bool,
-                     want_dgate: bool, bias_dtype: Optional[torch.dtype]):
-    """Gradients through the epilogue of `linear` for dy, z and gate [M, N] (bf16): (dz, dgate, dbias), None where not wanted.  dz
-    = dy * gate * act'(z) has rows of whole 16-byte pieces: [M, N] of [M, N rounded up to 8]; dbias is its sum over the rows."""
-    M, N = dy.shape
-    L = cabi.lib()
-    dev = dy.device
-    dy, z, gate = (None if t is None else _rows2d(t) for t in (dy, z, gate))
-    with _on_device(dev):
-        dz = torch.empty((M, (N + 7) // 8 * 8), dtype=torch.bfloat16, device=dev)[:, :N] if want_dz else None
-        dgate = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if want_dgate else None
-        dbias = ws = None
-        a = cabi.LinearPointwiseArgs(M=M, N=N, dy=dy.data_ptr(), lddy=_pitch(dy), activation=_activation_code(activation), stream=_stream())
-        if z is not None:
-            a.z, a.ldz = z.data_ptr(), _pitch(z)
-        if gate is not None:
-            a.gate, a.ldgate = gate.data_ptr(), _pitch(gate)
-        if dz is not None:
-            a.dz, a.lddz = dz.data_ptr(), dz.stride(0)
-        if dgate is not None:
-            a.dgate, a.lddg = dgate.data_ptr(), N
-        if bias_dtype is not None:
-            dbias = torch.empty(N, dtype=bias_dtype, device=dev)
-            ws = torch.empty(L.metis_linear_pointwise_workspace_bytes(M, N), dtype=torch.uint8, device=dev)
-            a.dbias, a.dbias_dtype, a.workspace, a.workspace_bytes = dbias.data_ptr(), _DTYPES[bias_dtype], ws.data_ptr(), ws.numel()
-        cabi.check(L.metis_linear_pointwise(a), "metis_linear_pointwise")
-    LAUNCHES["dense"] += 1 if dbias is None else 2
-    return dz, dgate, dbias
-
-
-def bf16_product(a: torch.Tensor, b: torch.Tensor, *, a_mn_major: bool = False, status: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """a @ b (a [M, K], b [K, N]), or a.T @ b with a_mn_major (a [K, M]), in bf16 with sums in fp32; N a multiple of 8."""
-    a, b = _operand_rows(a, "a"), _operand_rows(b, "b")
-    (K, M) = a.shape if a_mn_major else (a.shape[1], a.shape[0])
-    N = b.shape[1]
-    if b.shape[0] != K:
-        raise ValueError(f"inner dimensions differ: {K} vs {b.shape[0]}")
-    _same_device(a, b=b)
-
-    def pitch(t):                                        # (a single row of any size: its pitch is not read)
-        return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
-    with _on_device(a.device):
-        d = torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
-        rc = cabi.lib().metis_bf16_product(a.data_ptr(), int(a_mn_major), pitch(a), b.data_ptr(), pitch(b), M, N, K, d.data_ptr(), N, _ptr(status), _stream())
-    cabi.check(rc, "metis_bf16_product")
-    LAUNCHES["dense"] += 1
-    return d
-
-
-def _head_args(h, w, target, lse, ignore_index, scale, negate, status):
-    return cabi.HeadArgs(M=h.shape[0], V=w.shape[0], K=h.shape[1], h=h.data_ptr(), ldh=_pitch(h), w=w.data_ptr(), ldw=_pitch(w),
-                         target=target.data_ptr(), ignore_index=ignore_index, scale=scale, negate=int(negate), lse=lse.data_ptr(),
-                         status=_ptr(status), stream=_stream())
-
-
-def head_loss(h: torch.Tensor, w: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, scale: float = 1.0, negate: bool = False,
-              entropy: bool = False, status: Optional[torch.Tensor] = None):
-    """(nll, lse, entropy or None), fp32 [M], of the logits scale * h @ w.T for rows h [M, K] and w [V, K] from _operand_rows and
-    int64 targets [M]; with negate the targets' log-probabilities in place of nll.  The logits are not stored.  No autograd."""
-    L = cabi.lib()
-    M, K = h.shape
-    V = w.shape[0]
-    dev = h.device
-    with _on_device(dev):
-        nll, lse = torch.empty(M, dtype=torch.float32, device=dev), torch.empty(M, dtype=torch.float32, device=dev)
-        ent = torch.empty(M, dtype=torch.float32, device=dev) if entropy else None
-        ws = torch.empty(L.metis_head_loss_workspace_bytes(M, V, K, int(entropy)), dtype=torch.uint8, device=dev)
-        a = _head_args(h, w, target, lse, ignore_index, scale, negate, status)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        rc = L.metis_head_loss(a, nll.data_ptr(), _ptr(ent))
-    cabi.check(rc, "metis_head_loss")
-    LAUNCHES["dense"] += 2
-    return nll, lse, ent
-
-
-def head_sum(nll: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, mean: bool = False):
-    """(loss, inv_count), fp32: the sum of nll [M] and 1, or, with mean, that over the number of rows that are not ignored and 1 over it."""
-    with _on_device(nll.device):
-        loss, inv_count = torch.empty((), dtype=torch.float32, device=nll.device), torch.empty(1, dtype=torch.float32, device=nll.device)
-        rc = cabi.lib().metis_head_sum(nll.data_ptr(), target.data_ptr(), ignore_index, nll.numel(), int(mean), loss.data_ptr(), inv_count.data_ptr(), _stream())
-    cabi.check(rc, "metis_head_sum")
-    LAUNCHES["dense"] += 1
-    return loss, inv_count
-
-
-def head_backward(h: torch.Tensor, w: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, gout: torch.Tensor, *, ignore_index: int = -100,
-                  scale: float = 1.0, negate: bool = False, inv_count: Optional[torch.Tensor] = None, want_dh: bool = True, want_dw: bool = True,
-                  status: Optional[torch.Tensor] = None):
-    """(dh, dw) of the losses of `head_loss` (None where not wanted).  gout: fp32, one gradient for all rows or one for each; inv_count
-    (fp32 [1]) multiplies them."""
-    L = cabi.lib()
-    M, K = h.shape
-    V = w.shape[0]
-    dev = h.device
-    if gout.dtype != torch.float32 or gout.device != dev or gout.numel() not in (1, M):
-        raise ValueError(f"gout must be 1 or {M} fp32 values on {dev}")
-    each = gout.numel() == M and M > 1 and gout.stride(-1) != 0
-    if each:
-        gout = gout.contiguous()
-    with _on_device(dev):
-        dh = torch.empty((M, K), dtype=torch.bfloat16, device=dev) if want_dh else None
-        dw = torch.empty((V, K), dtype=torch.bfloat16, device=dev) if want_dw else None
-        ws = torch.empty(L.metis_head_backward_workspace_bytes(M, V, K), dtype=torch.uint8, device=dev)
-        a = _head_args(h, w, target, lse, ignore_index, scale, negate, status)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        rc = L.metis_head_backward(a, gout.data_ptr(), int(each), _ptr(inv_count), _ptr(dh), K, _ptr(dw), K)
-    cabi.check(rc, "metis_head_backward")
-    LAUNCHES["dense"] += 1 + int(want_dh) + int(want_dw)
-    return dh, dw

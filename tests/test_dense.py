@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from fp4_post_b200 import cabi, dense, ops
+from fp4_post_b200 import cabi, dense
 
 
 @pytest.fixture(scope="module")
@@ -96,8 +96,6 @@ def test_cpu_tensors_are_refused(built_library):
         dense.linear_cross_entropy(x, w, t)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         dense.token_logprobs(x, w, t)
-    with pytest.raises(RuntimeError, match="no CPU fallback"):
-        ops.bf16_product(x, w.t())
     with pytest.raises(ValueError, match="reduction"):
         dense.linear_cross_entropy(x, w, t, reduction="average")
     with pytest.raises(ValueError, match="activation"):

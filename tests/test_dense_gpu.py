@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from fp4_post_b200 import dense, ops
+from fp4_post_b200 import dense
 
 pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -8
@@ -326,7 +326,7 @@ def test_what_the_calls_refuse():
              (TypeError, lambda: dense.linear_cross_entropy(x.float(), w, t)), (TypeError, lambda: dense.linear_cross_entropy(x, w.float(), t)),
              (ValueError, lambda: dense.linear_cross_entropy(x, w, t, temperature=0.0)), (ValueError, lambda: dense.linear_cross_entropy(x, w, t, temperature=float("nan"))),
              (ValueError, lambda: dense.linear_cross_entropy(x, w.cpu(), t)), (ValueError, lambda: dense.token_logprobs(x, w, t.cpu())),
-             (ValueError, lambda: dense.token_logprobs(x, w[:0], t)), (ValueError, lambda: ops.bf16_product(x, w))]
+             (ValueError, lambda: dense.token_logprobs(x, w[:0], t)), (TypeError, lambda: dense.linear(x, None)), (TypeError, lambda: dense.linear(x, w, 3.0))]
     for i, (error, call) in enumerate(cases):
         with pytest.raises(error):
             call()
