@@ -18,18 +18,20 @@
 
 namespace metis {
 
-enum DenseEpilogue { kEpiLinear, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
+enum DenseEpilogue { kEpiLinear, kEpiLinearOperands, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
 
-struct DenseCfg {
-  static constexpr int kStages = 6;
+template <bool kOperands> struct DenseCfg {                // kOperands: the epilogue reads a gate or a residual
+  static constexpr int kStages = kOperands ? 5 : 6;
   static constexpr int kHalfBytes = 128 * 128;             // 128 rows x 64 elements of A or of B
   static constexpr int kBoxBytes = 64 * 128;               // one MN-major box: 64 contraction rows x 64 elements
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kEpilogueWarps = 8;
   static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
   static constexpr int kStagingBytes = kEpilogueWarps * 2 * 2048;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
+  static constexpr int kOperandBytes = kOperands ? kEpilogueWarps * 2 * 2048 : 0;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kOperandBytes + 1024 + 512;
 };
+static_assert(DenseCfg<true>::kSmemBytes <= 227 * 1024 && DenseCfg<false>::kSmemBytes <= 227 * 1024);
 
 // ---- epilogue pieces ----------------------------------------------------------------------------------------
 
@@ -77,22 +79,32 @@ __device__ __forceinline__ void store_piece_rows(Staging& st, __nv_bfloat16* out
   __syncwarp();
 }
 
-// This lane's 32 elements of a row of a bf16 operand of the epilogue, as words; those past N are zero.
-__device__ __forceinline__ void load_row32(const __nv_bfloat16* src, bool vec, int64_t left, uint32_t (&w)[16]) {
-  if (vec && left >= 32) {
+// This lane's 32 elements of a row of a bf16 operand of the epilogue, as words, where no TMA load reads it (a pitch or an address that 16
+// bytes do not divide): the warp reads row after row, a lane an element, eight rows in flight, and turns them through shared memory.
+// What lies outside the tensor is zero.
+__device__ __forceinline__ void load_piece_rows(Staging& st, const __nv_bfloat16* src, int64_t ld, int64_t col0, int64_t row0, int64_t M, int64_t N,
+                                                uint32_t (&w)[16]) {
+  const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  uint8_t* buf = st.next();
+  const unsigned short* s = reinterpret_cast<const unsigned short*>(src) + row0 * ld + col0 + lane;
+  const bool live = col0 + lane < N;
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    unsigned short v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-    }
-  } else {
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
+    for (int i = 0; i < 8; ++i) v[i] = live && row0 + r0 + i < M ? __ldg(s + (r0 + i) * ld) : (unsigned short)0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t lo = 2 * i < left ? __ldg(s + 2 * i) : 0, hi = 2 * i + 1 < left ? __ldg(s + 2 * i + 1) : 0;
-      w[i] = lo | (hi << 16);
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + i;
+      *reinterpret_cast<unsigned short*>(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) = v[i];
     }
   }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint4 q = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((k ^ swz) << 4));
+    w[4 * k] = q.x; w[4 * k + 1] = q.y; w[4 * k + 2] = q.z; w[4 * k + 3] = q.w;
+  }
+  __syncwarp();
 }
 
 __device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p, int64_t col0, bool full) {
@@ -107,10 +119,47 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p,
   }
 }
 
-__device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z,
-                                             const uint32_t (&r)[32], int64_t row0, int64_t col0) {
-  const int64_t row = row0 + (threadIdx.x & 31);
-  const bool live = row < p.M, full = col0 + 32 <= p.N;
+// An operand of the epilogue, [M, N] bf16: its pieces of 32 rows x 64 bytes come into a buffer of the warp's by the TMA unit, the next
+// one while the last one is worked on.  (Loads into registers, a lane a row, take a sector for every 16 bytes once the lines of eight
+// warps outgrow what shared memory leaves of the L1 cache: 8192 x 8960 x 1536 with silu, gate and z 209 us, fetched a chunk ahead 226.)
+struct EpilogueOperand {
+  const CUtensorMap* map;
+  const __nv_bfloat16* src;  int64_t ld;                   // null: there is none
+  bool tma;
+  uint32_t buf, bar;                                       // shared memory
+  uint32_t uses = 0;
+  bool pending = false;
+  __device__ __forceinline__ void fetch(int64_t col0, int64_t row0) {
+    if (!src || !tma) return;
+    __syncwarp();                                          // every lane has read what the buffer held
+    if ((threadIdx.x & 31) == 0) {
+      mbar_expect_tx_addr(bar, 2048);
+      tma_load_2d_addr(buf, map, (int32_t)col0, (int32_t)row0, bar);
+    }
+    pending = true;
+  }
+  __device__ __forceinline__ void wait(const DenseParams& p, uint64_t* bar_ptr, volatile int* abort_flag) {
+    if (!mbar_wait(bar_ptr, uses & 1u, abort_flag) && (threadIdx.x & 31) == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_TMA);
+    __syncwarp();
+    ++uses;
+    pending = false;
+  }
+  __device__ __forceinline__ void drain(uint64_t* bar_ptr) {
+    const uint64_t t0 = global_ns();
+    while (!mbar_try(bar_ptr, uses & 1u) && global_ns() - t0 < kWaitLimitNs) {}
+  }
+};
+
+// Where the warp's operand buffers and their barriers lie.
+struct OperandSmem {
+  uint8_t* buf;                                            // two of 2 KiB
+  uint64_t* bar;                                           // two
+};
+
+template <bool kOperands>
+__device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, const uint32_t (&r)[32],
+                                             EpilogueOperand (&ops)[2], const OperandSmem& os, volatile int* abort_flag, int64_t row0, int64_t col0, bool more) {
+  const bool full = col0 + 32 <= p.N;
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -123,18 +172,28 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
     else store_piece_rows(st, p.z, p.ldz, w, col0, row0, p.M, p.N);
   }
   activate_all(p.act, v);
-  if (p.gate) {
-    if (live) {
-      load_row32(p.gate + row * p.ldgate + col0, p.gate_vec, p.N - col0, w);
+  if constexpr (kOperands) {
+    const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
-    }
-  }
-  if (p.residual) {
-    if (live) {
-      load_row32(p.residual + row * p.ldr + col0, p.residual_vec, p.N - col0, w);
+    for (int k = 0; k < 2; ++k) {                          // gate, residual
+      EpilogueOperand& o = ops[k];
+      if (!o.src) continue;
+      if (o.tma) {
+        o.wait(p, os.bar + k, abort_flag);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+        for (int i = 0; i < 4; ++i) {
+          const uint4 q = *reinterpret_cast<const uint4*>(os.buf + k * 2048 + lane * 64 + ((i ^ swz) << 4));
+          w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+        }
+        if (more) o.fetch(col0 + 32, row0);
+      } else {
+        load_piece_rows(st, o.src, o.ld, col0, row0, p.M, p.N, w);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (k == 0) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
+        else        { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+      }
     }
   }
 #pragma unroll
@@ -180,11 +239,14 @@ __device__ __forceinline__ void stats_chunk(const DenseParams& p, RowStats& a, c
 
 // ---- the kernel ---------------------------------------------------------------------------------------------
 
+struct DenseMaps { CUtensorMap d, z, gate, residual; };
+
 template <bool kAMn, bool kBMn, int kEpi>
-__global__ void __launch_bounds__(DenseCfg::kThreads, 1)
-dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_z, const DenseParams p) {
-  using Cfg = DenseCfg;
+__global__ void __launch_bounds__(DenseCfg<false>::kThreads, 1)
+dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ DenseMaps maps,
+                       const DenseParams p) {
+  using Cfg = DenseCfg<kEpi == kEpiLinearOperands>;
+  constexpr bool kLinear = kEpi == kEpiLinear || kEpi == kEpiLinearOperands;
   constexpr int kStages = Cfg::kStages;
   constexpr int BN = 256;
 
@@ -192,13 +254,15 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   // the dynamic window starts at the same offset in both CTAs: descriptors and barrier offsets are valid across the pair
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staging = smem + kStages * Cfg::kStageBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + Cfg::kStagingBytes);
+  uint8_t* operand_bufs = staging + Cfg::kStagingBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(operand_bufs + Cfg::kOperandBytes);
   uint64_t* full = bars;                                   // [kStages]  leader's: all bytes of the stage of both CTAs
   uint64_t* empty = bars + kStages;                        // [kStages]  local: consumed (commit to both CTAs)
   uint64_t* acc_full = bars + 2 * kStages;                 // [2]        local: accumulator complete (commit to both CTAs)
   uint64_t* acc_empty = bars + 2 * kStages + 2;            // [2]        leader's: drained by every epilogue warp of both CTAs
   uint64_t* drain = bars + 2 * kStages + 4;                // error path only
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
+  uint64_t* operand_bars = bars + 2 * kStages + 5;         // [epilogue warps][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(operand_bars + 2 * Cfg::kEpilogueWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -215,6 +279,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * Cfg::kEpilogueWarps); }
     mbar_init(drain, 1);
+    for (int i = 0; i < 2 * Cfg::kEpilogueWarps; ++i) mbar_init(&operand_bars[i], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -331,6 +396,9 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const int part = (warp - 2) >> 2;
     const uint32_t empty_leader = map_to_cta(smem_u32(acc_empty), 0);
     Staging st{staging + (warp - 2) * 4096};
+    const OperandSmem os = {operand_bufs + (warp - 2) * 4096, operand_bars + (warp - 2) * 2};
+    EpilogueOperand ops[2] = {{&maps.gate, p.gate, p.ldgate, p.gate_tma != 0, smem_u32(os.buf), smem_u32(os.bar)},
+                              {&maps.residual, p.residual, p.ldr, p.residual_tma != 0, smem_u32(os.buf) + 2048, smem_u32(os.bar + 1)}};
     uint32_t local_tile = 0;
     for (int64_t tile = pair; tile < num_tiles; tile += num_pairs, ++local_tile) {
       int64_t tm, tn;
@@ -354,6 +422,12 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             if (p.inv_count) weight *= __ldg(p.inv_count);
             if (t < 0 || t >= p.vocab) weight = NAN;       // (a target outside the vocabulary; ignored rows are dead)
           }
+        }
+      }
+      if constexpr (kEpi == kEpiLinearOperands) {
+        if (rows && n0 < p.N) {
+          ops[0].fetch(n0, row0);
+          ops[1].fetch(n0, row0);
         }
       }
       if (!mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
@@ -382,7 +456,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         if (rows && col0 < p.N) {
           const int64_t at = hit - col0;                   // the target's place in this chunk
           const bool here = at >= 0 && at < 32;
-          if constexpr (kEpi == kEpiLinear) linear_chunk(p, st, &map_d, &map_z, v, row0, col0);
+          if constexpr (kLinear) linear_chunk<kEpi == kEpiLinearOperands>(p, st, &maps.d, &maps.z, v, ops, os, abort_flag, row0, col0, ch < 3 && col0 + 32 < p.N);
           if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
             stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
             if (here) {
@@ -403,7 +477,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : pack_bf16(g[2 * i], g[2 * i + 1]);
-            store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+            store_piece_tma(st, &maps.d, w, (int32_t)col0, (int32_t)row0);
           }
           if constexpr (kEpi == kEpiSum || kEpi == kEpiSumF32) {
             float g[32];
@@ -426,13 +500,13 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             if constexpr (kEpi == kEpiSum) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) w[i] = pack_bf16(g[2 * i], g[2 * i + 1]);
-              store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+              store_piece_tma(st, &maps.d, w, (int32_t)col0, (int32_t)row0);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(g[16 * h + i]);
-                store_piece_tma(st, &map_d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
+                store_piece_tma(st, &maps.d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
               }
             }
           }
@@ -446,6 +520,10 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           if (found) p.picked[row] = picked;
         }
       }
+    }
+    if constexpr (kEpi == kEpiLinearOperands) {              // error path: copies that nothing has waited for
+#pragma unroll
+      for (int k = 0; k < 2; ++k) if (ops[k].pending) ops[k].drain(os.bar + k);
     }
     if (lane == 0) bulk_store_wait_all();                    // shared memory stays until the TMA unit has read it
   }
@@ -645,7 +723,8 @@ struct DenseOperand {
 };
 
 template <bool kAMn, bool kBMn, int kEpi>
-static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const CUtensorMap& map_d, const CUtensorMap& map_z, DenseParams p, cudaStream_t st) {
+static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const DenseMaps& maps, DenseParams p, cudaStream_t st) {
+  using Cfg = DenseCfg<kEpi == kEpiLinearOperands>;
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ma, mb;
   if (kAMn) { if (int32_t rc = make_map(&ma, dt, 2, a.p, p.M, p.K, a.ld * 2, 64, 64, "A (MN-major)")) return rc; }
@@ -658,11 +737,11 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   if (pairs > tiles) pairs = tiles;
   pairs = ceil_div(tiles, ceil_div(tiles, pairs));         // the fewest that finish in the same number of rounds
   auto kern = dense_gemm_pair_kernel<kAMn, kBMn, kEpi>;
-  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DenseCfg::kSmemBytes));
+  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(DenseCfg::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = DenseCfg::kSmemBytes;
+  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -673,11 +752,12 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap_enabled(kLaunchGemm) ? 2 : 1;
-  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_z, p));
+  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, maps, p));
   return METIS_OK;
 }
 
-static int32_t map_bf16_out(CUtensorMap* map, void* d, int64_t ld, int64_t M, int64_t N, const char* what) {
+// pieces of 32 rows x 64 bytes that the epilogue stores or loads
+static int32_t map_bf16(CUtensorMap* map, const void* d, int64_t ld, int64_t M, int64_t N, const char* what) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, d, N, M, ld * 2, 32, 32, what, 64);
 }
 
@@ -686,13 +766,13 @@ static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M
                          void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st) {
   DenseParams p = {};
   p.M = M; p.N = N; p.K = K; p.status = status; p.c = c; p.ldc = ldc;
-  CUtensorMap md = {}, mz = {};
+  DenseMaps maps = {};
   if (d_f32) {
-    if (int32_t rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
-    return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, md, mz, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, md, mz, p, st);
+    if (int32_t rc = make_map(&maps.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
+    return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, maps, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, maps, p, st);
   }
-  if (int32_t rc = map_bf16_out(&md, d, ldd, M, N, "D")) return rc;
-  return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, mz, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, mz, p, st);
+  if (int32_t rc = map_bf16(&maps.d, d, ldd, M, N, "D")) return rc;
+  return a.mn ? launch_dense<true, true, kEpiSum>(a, b, maps, p, st) : launch_dense<false, true, kEpiSum>(a, b, maps, p, st);
 }
 
 // Whether a product of M tokens goes to the kernels for few of them (dense_small.cu).
@@ -732,16 +812,20 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   DenseParams p = {};
   p.M = a->M; p.N = a->N; p.K = a->K; p.status = a->status;
   p.bias = a->bias; p.bias_f32 = a->bias_dtype == METIS_DTYPE_F32; p.act = a->activation;
-  auto wide = [](const void* t, int64_t ld) { return aligned16(t) && ld % 8 == 0; };
-  p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_vec = wide(a->gate, a->ldgate);
-  p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_vec = wide(a->residual, a->ldr);
+  auto wide = [](const void* t, int64_t ld) { return t && aligned16(t) && ld % 8 == 0; };
+  p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_tma = wide(a->gate, a->ldgate);
+  p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_tma = wide(a->residual, a->ldr);
   p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_tma = wide(a->y, a->ldy);
-  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_tma = a->z && wide(a->z, a->ldz);
-  if (few_tokens(a->M, a->N, a->K)) return launch_dense_small(a->x, a->ldx, a->w, false, a->ldw, p, reinterpret_cast<cudaStream_t>(a->stream));
-  CUtensorMap md = {}, mz = {};
-  if (p.d_tma) if (int32_t rc = map_bf16_out(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
-  if (p.z_tma) if (int32_t rc = map_bf16_out(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
-  return launch_dense<false, false, kEpiLinear>({a->x, a->ldx, false}, {a->w, a->ldw, false}, md, mz, p, reinterpret_cast<cudaStream_t>(a->stream));
+  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_tma = wide(a->z, a->ldz);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  if (few_tokens(a->M, a->N, a->K)) return launch_dense_small(a->x, a->ldx, a->w, false, a->ldw, p, st);
+  DenseMaps maps = {};
+  if (p.d_tma) if (int32_t rc = map_bf16(&maps.d, a->y, a->ldy, a->M, a->N, "y")) return rc;
+  if (p.z_tma) if (int32_t rc = map_bf16(&maps.z, a->z, a->ldz, a->M, a->N, "z")) return rc;
+  if (p.gate_tma) if (int32_t rc = map_bf16(&maps.gate, a->gate, a->ldgate, a->M, a->N, "gate")) return rc;
+  if (p.residual_tma) if (int32_t rc = map_bf16(&maps.residual, a->residual, a->ldr, a->M, a->N, "residual")) return rc;
+  const DenseOperand x = {a->x, a->ldx, false}, w = {a->w, a->ldw, false};
+  return a->gate || a->residual ? launch_dense<false, false, kEpiLinearOperands>(x, w, maps, p, st) : launch_dense<false, false, kEpiLinear>(x, w, maps, p, st);
 }
 
 constexpr int kPointwiseGroups = 64;
@@ -860,10 +944,10 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + ceil_div(a->M * 4, 16) * 16);
   p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
   const DenseOperand h = {a->h, a->ldh, false}, w = {a->w, a->ldw, false};
-  const CUtensorMap none = {};
+  const DenseMaps none = {};
   if (a->M <= kFewRows) {
     if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
-  } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, none, p, st)) return rc;
+  } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, p, st)) return rc;
   const dim3 blocks((unsigned)ceil_div(a->M, 32));
   auto rows = entropy ? head_rows_kernel<true> : head_rows_kernel<false>;
   METIS_CUDA_OK(launch_overlapped(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
@@ -903,11 +987,11 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   for (int64_t v0 = 0; v0 < a->V; v0 += columns) {
     const int64_t n = a->V - v0 < columns ? a->V - v0 : columns;
     const bool last = v0 + n == a->V;
-    CUtensorMap mg, none = {};
+    DenseMaps maps = {};
     p.N = n;
     p.col0 = v0;
-    if (int32_t rc = map_bf16_out(&mg, g, columns, a->M, n, "G")) return rc;
-    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, mg, none, p, st)) return rc;
+    if (int32_t rc = map_bf16(&maps.d, g, columns, a->M, n, "G")) return rc;
+    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, maps, p, st)) return rc;
     if (dh) {
       if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
                                  last ? dh : acc, !last, last ? lddh : a->K, a->status, st)) return rc;

@@ -217,8 +217,8 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       const int e = e0 + k * step;
       const int64_t n = n0 + 8 * (e & ((1 << shift) - 1)), m = m0 + (e >> shift);
       if (e < tokens << shift && n < p.N) {
-        if (p.gate) load_row8(p.gate + m * p.ldgate + n, p.gate_vec, p.N - n, gate[k]);
-        if (p.residual) load_row8(p.residual + m * p.ldr + n, p.residual_vec, p.N - n, residual[k]);
+        if (p.gate) load_row8(p.gate + m * p.ldgate + n, p.gate_tma, p.N - n, gate[k]);
+        if (p.residual) load_row8(p.residual + m * p.ldr + n, p.residual_tma, p.N - n, residual[k]);
       }
     }
 #pragma unroll
