@@ -13,10 +13,10 @@ struct DenseParams {
   // linear layer: d = act(A B^T + bias) * gate + residual, and z, what act was applied to
   const void* bias;  int32_t bias_f32;
   int32_t act;
-  const __nv_bfloat16* gate;      int64_t ldgate;  int32_t gate_tma;       // *_tma: rows of 16-byte pieces, which the TMA unit moves
-  const __nv_bfloat16* residual;  int64_t ldr;     int32_t residual_tma;
-  __nv_bfloat16* d;               int64_t ldd;     int32_t d_tma;
-  __nv_bfloat16* z;               int64_t ldz;     int32_t z_tma;
+  const __nv_bfloat16* gate;      int64_t ldgate;  int32_t gate_wide;       // *_wide: rows of 16-byte pieces
+  const __nv_bfloat16* residual;  int64_t ldr;     int32_t residual_wide;
+  __nv_bfloat16* d;               int64_t ldd;     int32_t d_wide;
+  __nv_bfloat16* z;               int64_t ldz;     int32_t z_wide;
   // head: logits l = scale * (A B^T); columns of the vocabulary [0, N) of this launch are [col0, col0 + N) of all
   const int64_t* target;  int64_t ignore;
   int64_t vocab;  int64_t col0;

@@ -18,20 +18,23 @@
 
 namespace metis {
 
-enum DenseEpilogue { kEpiLinear, kEpiLinearOperands, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
+enum DenseEpilogue { kEpiLinear, kEpiLinearWide, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
 
-template <bool kOperands> struct DenseCfg {                // kOperands: the epilogue reads a gate or a residual
-  static constexpr int kStages = kOperands ? 5 : 6;
+template <int kEpi> struct DenseCfg {
+  static constexpr bool kWide = kEpi == kEpiLinearWide;
+  static constexpr int kParts = 2;                         // epilogue warps for each 32-lane quarter of tensor memory
+  static constexpr int kStages = kWide ? 5 : 6;
   static constexpr int kHalfBytes = 128 * 128;             // 128 rows x 64 elements of A or of B
   static constexpr int kBoxBytes = 64 * 128;               // one MN-major box: 64 contraction rows x 64 elements
   static constexpr int kStageBytes = 2 * kHalfBytes;
-  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kEpilogueWarps = 4 * kParts;
+  static constexpr int kChunks = 8 / kParts;               // of 32 columns, that a warp takes of a tile
   static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-  static constexpr int kStagingBytes = kEpilogueWarps * 2 * 2048;
-  static constexpr int kOperandBytes = kOperands ? kEpilogueWarps * 2 * 2048 : 0;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kOperandBytes + 1024 + 512;
+  static constexpr int kBuffers = kWide ? 4 : 2;           // of 32 rows x 64 bytes, for each epilogue warp
+  static constexpr int kStagingBytes = kEpilogueWarps * kBuffers * 2048;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 };
-static_assert(DenseCfg<true>::kSmemBytes <= 227 * 1024 && DenseCfg<false>::kSmemBytes <= 227 * 1024);
+static_assert(DenseCfg<kEpiLinear>::kSmemBytes <= 227 * 1024 && DenseCfg<kEpiLinearWide>::kSmemBytes <= 227 * 1024);
 
 // ---- epilogue pieces ----------------------------------------------------------------------------------------
 
@@ -39,12 +42,18 @@ static_assert(DenseCfg<true>::kSmemBytes <= 227 * 1024 && DenseCfg<false>::kSmem
 struct Staging {
   uint8_t* base;
   uint32_t flip = 0;
-  __device__ __forceinline__ uint8_t* next() {
+  __device__ __forceinline__ uint8_t* next() {             // (the stores of one buffer are read while the other is filled)
     uint8_t* buf = base + flip * 2048;
     flip ^= 1u;
     if ((threadIdx.x & 31) == 0) bulk_store_wait_read<1>();
     __syncwarp();
     return buf;
+  }
+  // one for other uses: no store reads it any more, and no lane
+  __device__ __forceinline__ uint8_t* idle() {
+    if ((threadIdx.x & 31) == 0) bulk_store_wait_read<0>();
+    __syncwarp();
+    return base;
   }
 };
 
@@ -65,7 +74,7 @@ __device__ __forceinline__ void store_piece_tma(Staging& st, const CUtensorMap* 
 __device__ __forceinline__ void store_piece_rows(Staging& st, __nv_bfloat16* out, int64_t ld, const uint32_t (&w)[16], int64_t col0, int64_t row0,
                                                  int64_t M, int64_t N) {
   const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
-  uint8_t* buf = st.next();
+  uint8_t* buf = st.idle();
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
@@ -85,7 +94,7 @@ __device__ __forceinline__ void store_piece_rows(Staging& st, __nv_bfloat16* out
 __device__ __forceinline__ void load_piece_rows(Staging& st, const __nv_bfloat16* src, int64_t ld, int64_t col0, int64_t row0, int64_t M, int64_t N,
                                                 uint32_t (&w)[16]) {
   const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
-  uint8_t* buf = st.next();
+  uint8_t* buf = st.idle();
   const unsigned short* s = reinterpret_cast<const unsigned short*>(src) + row0 * ld + col0 + lane;
   const bool live = col0 + lane < N;
   for (int r0 = 0; r0 < 32; r0 += 8) {
@@ -119,46 +128,66 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p,
   }
 }
 
-// An operand of the epilogue, [M, N] bf16: its pieces of 32 rows x 64 bytes come into a buffer of the warp's by the TMA unit, the next
-// one while the last one is worked on.  (Loads into registers, a lane a row, take a sector for every 16 bytes once the lines of eight
-// warps outgrow what shared memory leaves of the L1 cache: 8192 x 8960 x 1536 with silu, gate and z 209 us, fetched a chunk ahead 226.)
+// An operand of the epilogue, [M, N] bf16.  Its pieces of 32 rows x 64 bytes come into a buffer of the warp's by asynchronous copies (four
+// lanes a row: whole sectors), the next one on its way while the last one is worked on; each fetch is a group of copies, empty or not.
 struct EpilogueOperand {
-  const CUtensorMap* map;
-  const __nv_bfloat16* src;  int64_t ld;                   // null: there is none
-  bool tma;
-  uint32_t buf, bar;                                       // shared memory
-  uint32_t uses = 0;
-  bool pending = false;
-  __device__ __forceinline__ void fetch(int64_t col0, int64_t row0) {
-    if (!src || !tma) return;
+  const __nv_bfloat16* src;                                // null: there is none
+  int64_t ld;
+  bool wide;                                               // 16-byte aligned rows
+  uint8_t* buf;
+  __device__ __forceinline__ void fetch(bool valid, int64_t col0, int64_t row0, int64_t M, int64_t N) {
     __syncwarp();                                          // every lane has read what the buffer held
-    if ((threadIdx.x & 31) == 0) {
-      mbar_expect_tx_addr(bar, 2048);
-      tma_load_2d_addr(buf, map, (int32_t)col0, (int32_t)row0, bar);
+    if (src && wide && valid && col0 + 32 <= N) {
+      const int lane = threadIdx.x & 31;
+      const __nv_bfloat16* at = src + (row0 + (lane >> 2)) * ld + col0 + (lane & 3) * 8;
+      const uint32_t to = smem_u32(buf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        if (row0 + r < M)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)), "l"(at + 8 * i * ld) : "memory");
+      }
     }
-    pending = true;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ void wait(const DenseParams& p, uint64_t* bar_ptr, volatile int* abort_flag) {
-    if (!mbar_wait(bar_ptr, uses & 1u, abort_flag) && (threadIdx.x & 31) == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_TMA);
+  // this lane's 32 elements of its row, of the piece that was fetched two groups ago
+  __device__ __forceinline__ void take(uint32_t (&w)[16]) {
+    const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
-    ++uses;
-    pending = false;
-  }
-  __device__ __forceinline__ void drain(uint64_t* bar_ptr) {
-    const uint64_t t0 = global_ns();
-    while (!mbar_try(bar_ptr, uses & 1u) && global_ns() - t0 < kWaitLimitNs) {}
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 t = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((k ^ swz) << 4));
+      w[4 * k] = t.x; w[4 * k + 1] = t.y; w[4 * k + 2] = t.z; w[4 * k + 3] = t.w;
+    }
   }
 };
+// The output alone: bias and activation, a store through the TMA unit.
+__device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const uint32_t (&r)[32], int64_t row0, int64_t col0) {
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  if (p.bias) add_bias32(v, p, col0, col0 + 32 <= p.N);
+  activate_all(p.act, v);
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+  if (p.d_wide) store_piece_tma(st, map_d, w, (int32_t)col0, (int32_t)row0);
+  else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
+}
 
-// Where the warp's operand buffers and their barriers lie.
-struct OperandSmem {
-  uint8_t* buf;                                            // two of 2 KiB
-  uint64_t* bar;                                           // two
+// With z, gate or residual: several tensors of the output's size pass by.  What is read comes by asynchronous copies of the load/store unit
+// a piece ahead; what is written leaves by the TMA unit.  Tried, 8192 x 8960 x 1536, us, plain 150 to 158: silu, gate and z / gate and residual by
+// this form 211 / 188 (five stages in place of six pay for the buffers); loads into registers where they are used 238 / 220; loads by the
+// TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores by the load/store
+// unit 235 / 188.  `next`: the piece that this warp takes after this one.
+struct PieceAt {
+  bool valid;
+  int64_t row0, col0;
 };
-
-template <bool kOperands>
-__device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, const uint32_t (&r)[32],
-                                             EpilogueOperand (&ops)[2], const OperandSmem& os, volatile int* abort_flag, int64_t row0, int64_t col0, bool more) {
+__device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, EpilogueOperand& gate,
+                                                  EpilogueOperand& residual, const uint32_t (&r)[32],
+                                                  int64_t row0, int64_t col0, const PieceAt& next) {
   const bool full = col0 + 32 <= p.N;
   float v[32];
 #pragma unroll
@@ -168,37 +197,27 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
   if (p.z) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (p.z_tma) store_piece_tma(st, map_z, w, (int32_t)col0, (int32_t)row0);
+    if (p.z_wide) store_piece_tma(st, map_z, w, (int32_t)col0, (int32_t)row0);
     else store_piece_rows(st, p.z, p.ldz, w, col0, row0, p.M, p.N);
   }
   activate_all(p.act, v);
-  if constexpr (kOperands) {
-    const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  if (gate.src) {
+    if (gate.wide && full) gate.take(w);
+    else load_piece_rows(st, gate.src, gate.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {                          // gate, residual
-      EpilogueOperand& o = ops[k];
-      if (!o.src) continue;
-      if (o.tma) {
-        o.wait(p, os.bar + k, abort_flag);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 q = *reinterpret_cast<const uint4*>(os.buf + k * 2048 + lane * 64 + ((i ^ swz) << 4));
-          w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-        }
-        if (more) o.fetch(col0 + 32, row0);
-      } else {
-        load_piece_rows(st, o.src, o.ld, col0, row0, p.M, p.N, w);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (k == 0) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
-        else        { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
-      }
-    }
+    for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
   }
+  gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
+  if (residual.src) {
+    if (residual.wide && full) residual.take(w);
+    else load_piece_rows(st, residual.src, residual.ld, col0, row0, p.M, p.N, w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
+  }
+  residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-  if (p.d_tma) store_piece_tma(st, map_d, w, (int32_t)col0, (int32_t)row0);
+  if (p.d_wide) store_piece_tma(st, map_d, w, (int32_t)col0, (int32_t)row0);
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
 
@@ -239,14 +258,11 @@ __device__ __forceinline__ void stats_chunk(const DenseParams& p, RowStats& a, c
 
 // ---- the kernel ---------------------------------------------------------------------------------------------
 
-struct DenseMaps { CUtensorMap d, z, gate, residual; };
-
 template <bool kAMn, bool kBMn, int kEpi>
-__global__ void __launch_bounds__(DenseCfg<false>::kThreads, 1)
-dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ DenseMaps maps,
-                       const DenseParams p) {
-  using Cfg = DenseCfg<kEpi == kEpiLinearOperands>;
-  constexpr bool kLinear = kEpi == kEpiLinear || kEpi == kEpiLinearOperands;
+__global__ void __launch_bounds__(DenseCfg<kEpi>::kThreads, 1)
+dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
+                       const __grid_constant__ CUtensorMap map_z, const DenseParams p) {
+  using Cfg = DenseCfg<kEpi>;
   constexpr int kStages = Cfg::kStages;
   constexpr int BN = 256;
 
@@ -254,15 +270,13 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   // the dynamic window starts at the same offset in both CTAs: descriptors and barrier offsets are valid across the pair
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staging = smem + kStages * Cfg::kStageBytes;
-  uint8_t* operand_bufs = staging + Cfg::kStagingBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(operand_bufs + Cfg::kOperandBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + Cfg::kStagingBytes);
   uint64_t* full = bars;                                   // [kStages]  leader's: all bytes of the stage of both CTAs
   uint64_t* empty = bars + kStages;                        // [kStages]  local: consumed (commit to both CTAs)
   uint64_t* acc_full = bars + 2 * kStages;                 // [2]        local: accumulator complete (commit to both CTAs)
   uint64_t* acc_empty = bars + 2 * kStages + 2;            // [2]        leader's: drained by every epilogue warp of both CTAs
   uint64_t* drain = bars + 2 * kStages + 4;                // error path only
-  uint64_t* operand_bars = bars + 2 * kStages + 5;         // [epilogue warps][2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(operand_bars + 2 * Cfg::kEpilogueWarps);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -279,7 +293,6 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * Cfg::kEpilogueWarps); }
     mbar_init(drain, 1);
-    for (int i = 0; i < 2 * Cfg::kEpilogueWarps; ++i) mbar_init(&operand_bars[i], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -395,10 +408,17 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const int q = warp & 3;
     const int part = (warp - 2) >> 2;
     const uint32_t empty_leader = map_to_cta(smem_u32(acc_empty), 0);
-    Staging st{staging + (warp - 2) * 4096};
-    const OperandSmem os = {operand_bufs + (warp - 2) * 4096, operand_bars + (warp - 2) * 2};
-    EpilogueOperand ops[2] = {{&maps.gate, p.gate, p.ldgate, p.gate_tma != 0, smem_u32(os.buf), smem_u32(os.bar)},
-                              {&maps.residual, p.residual, p.ldr, p.residual_tma != 0, smem_u32(os.buf) + 2048, smem_u32(os.bar + 1)}};
+    Staging st{staging + (warp - 2) * (Cfg::kStagingBytes / Cfg::kEpilogueWarps)};
+    // operands of the epilogue; `ahead` is the piece whose copies are on their way
+    EpilogueOperand gate = {p.gate, p.ldgate, p.gate_wide != 0, st.base + 4096}, residual = {p.residual, p.ldr, p.residual_wide != 0, st.base + 6144};
+    PieceAt ahead = {false, 0, 0};
+    auto first_piece = [&](int64_t t) {                      // this warp's first piece of tile t
+      int64_t tm = 0, tn = 0;
+      if (t < num_tiles) tile_coords(t, tiles_m, tiles_n, p.band, tm, tn);
+      PieceAt at = {t < num_tiles, tm * 256 + cta * 128 + q * 32, tn * BN + part * (32 * Cfg::kChunks)};
+      at.valid = at.valid && at.row0 < p.M && at.col0 < p.N;
+      return at;
+    };
     uint32_t local_tile = 0;
     for (int64_t tile = pair; tile < num_tiles; tile += num_pairs, ++local_tile) {
       int64_t tm, tn;
@@ -406,7 +426,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const uint32_t buf = local_tile & 1u;
       const int64_t row0 = tm * 256 + cta * 128 + q * 32;
       const int64_t row = row0 + lane;
-      const int64_t n0 = tn * BN + part * 128;
+      const int64_t n0 = tn * BN + part * (32 * Cfg::kChunks);
       const bool rows = row0 < p.M;                        // warp-uniform: the tile's rows of this warp are not all past the end
       int64_t hit = -1;                                    // the target's column in this launch
       float lse2 = 0.0f, weight = 0.0f;
@@ -424,29 +444,33 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           }
         }
       }
-      if constexpr (kEpi == kEpiLinearOperands) {
-        if (rows && n0 < p.N) {
-          ops[0].fetch(n0, row0);
-          ops[1].fetch(n0, row0);
+      if constexpr (kEpi == kEpiLinearWide) {
+        if (rows && n0 < p.N && !ahead.valid) {
+          gate.fetch(true, n0, row0, p.M, p.N);
+          residual.fetch(true, n0, row0, p.M, p.N);
         }
+        ahead.valid = false;
       }
       if (!mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
         if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_MMA);
         break;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * 128;
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * (32 * Cfg::kChunks);
       RowStats stats = {-INFINITY, 0.0f, 0.0f};
       float picked = 0.0f;
       bool found = false;
-      uint32_t r[2][32];
-      tc_load32(t_row, r[0]);
+      // the next chunk of the accumulator is read while this one is worked on, where the registers allow it
+      constexpr bool kAhead = kEpi != kEpiLinearWide;
+      uint32_t r[kAhead ? 2 : 1][32];
+      if (kAhead) tc_load32(t_row, r[0]);
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        uint32_t(&v)[32] = r[ch & 1];
+      for (int ch = 0; ch < Cfg::kChunks; ++ch) {
+        uint32_t(&v)[32] = r[kAhead ? ch & 1 : 0];
+        if (!kAhead) tc_load32(t_row + ch * 32, v);
         tc_wait_ld(v);
-        if (ch < 3) {
-          tc_load32(t_row + (ch + 1) * 32, r[(ch + 1) & 1]);
+        if (ch < Cfg::kChunks - 1) {
+          if (kAhead) tc_load32(t_row + (ch + 1) * 32, r[kAhead ? (ch + 1) & 1 : 0]);
         } else {
           tc_fence_before();
           __syncwarp();
@@ -456,7 +480,12 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         if (rows && col0 < p.N) {
           const int64_t at = hit - col0;                   // the target's place in this chunk
           const bool here = at >= 0 && at < 32;
-          if constexpr (kLinear) linear_chunk<kEpi == kEpiLinearOperands>(p, st, &maps.d, &maps.z, v, ops, os, abort_flag, row0, col0, ch < 3 && col0 + 32 < p.N);
+          if constexpr (kEpi == kEpiLinear) linear_chunk(p, st, &map_d, v, row0, col0);
+          if constexpr (kEpi == kEpiLinearWide) {
+            PieceAt next = {ch + 1 < Cfg::kChunks && col0 + 32 < p.N, row0, col0 + 32};
+            if (!next.valid) next = ahead = first_piece(tile + num_pairs);
+            linear_wide_chunk(p, st, &map_d, &map_z, gate, residual, v, row0, col0, next);
+          }
           if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
             stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
             if (here) {
@@ -477,7 +506,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : pack_bf16(g[2 * i], g[2 * i + 1]);
-            store_piece_tma(st, &maps.d, w, (int32_t)col0, (int32_t)row0);
+            store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
           }
           if constexpr (kEpi == kEpiSum || kEpi == kEpiSumF32) {
             float g[32];
@@ -500,13 +529,13 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             if constexpr (kEpi == kEpiSum) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) w[i] = pack_bf16(g[2 * i], g[2 * i + 1]);
-              store_piece_tma(st, &maps.d, w, (int32_t)col0, (int32_t)row0);
+              store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(g[16 * h + i]);
-                store_piece_tma(st, &maps.d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
+                store_piece_tma(st, &map_d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
               }
             }
           }
@@ -521,10 +550,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         }
       }
     }
-    if constexpr (kEpi == kEpiLinearOperands) {              // error path: copies that nothing has waited for
-#pragma unroll
-      for (int k = 0; k < 2; ++k) if (ops[k].pending) ops[k].drain(os.bar + k);
-    }
+    if constexpr (kEpi == kEpiLinearWide) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (lane == 0) bulk_store_wait_all();                    // shared memory stays until the TMA unit has read it
   }
 
@@ -723,8 +749,8 @@ struct DenseOperand {
 };
 
 template <bool kAMn, bool kBMn, int kEpi>
-static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const DenseMaps& maps, DenseParams p, cudaStream_t st) {
-  using Cfg = DenseCfg<kEpi == kEpiLinearOperands>;
+static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const CUtensorMap& map_d, DenseParams p, cudaStream_t st, const CUtensorMap& map_z = {}) {
+  using Cfg = DenseCfg<kEpi>;
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ma, mb;
   if (kAMn) { if (int32_t rc = make_map(&ma, dt, 2, a.p, p.M, p.K, a.ld * 2, 64, 64, "A (MN-major)")) return rc; }
@@ -752,11 +778,11 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap_enabled(kLaunchGemm) ? 2 : 1;
-  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, maps, p));
+  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_z, p));
   return METIS_OK;
 }
 
-// pieces of 32 rows x 64 bytes that the epilogue stores or loads
+// pieces of 32 rows x 64 bytes that the epilogue stores
 static int32_t map_bf16(CUtensorMap* map, const void* d, int64_t ld, int64_t M, int64_t N, const char* what) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, d, N, M, ld * 2, 32, 32, what, 64);
 }
@@ -766,13 +792,13 @@ static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M
                          void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st) {
   DenseParams p = {};
   p.M = M; p.N = N; p.K = K; p.status = status; p.c = c; p.ldc = ldc;
-  DenseMaps maps = {};
+  CUtensorMap md = {};
   if (d_f32) {
-    if (int32_t rc = make_map(&maps.d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
-    return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, maps, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, maps, p, st);
+    if (int32_t rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
+    return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, md, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, md, p, st);
   }
-  if (int32_t rc = map_bf16(&maps.d, d, ldd, M, N, "D")) return rc;
-  return a.mn ? launch_dense<true, true, kEpiSum>(a, b, maps, p, st) : launch_dense<false, true, kEpiSum>(a, b, maps, p, st);
+  if (int32_t rc = map_bf16(&md, d, ldd, M, N, "D")) return rc;
+  return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, p, st);
 }
 
 // Whether a product of M tokens goes to the kernels for few of them (dense_small.cu).
@@ -813,19 +839,18 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   p.M = a->M; p.N = a->N; p.K = a->K; p.status = a->status;
   p.bias = a->bias; p.bias_f32 = a->bias_dtype == METIS_DTYPE_F32; p.act = a->activation;
   auto wide = [](const void* t, int64_t ld) { return t && aligned16(t) && ld % 8 == 0; };
-  p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_tma = wide(a->gate, a->ldgate);
-  p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_tma = wide(a->residual, a->ldr);
-  p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_tma = wide(a->y, a->ldy);
-  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_tma = wide(a->z, a->ldz);
+  p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_wide = wide(a->gate, a->ldgate);
+  p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_wide = wide(a->residual, a->ldr);
+  p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_wide = wide(a->y, a->ldy);
+  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_wide = wide(a->z, a->ldz);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
   if (few_tokens(a->M, a->N, a->K)) return launch_dense_small(a->x, a->ldx, a->w, false, a->ldw, p, st);
-  DenseMaps maps = {};
-  if (p.d_tma) if (int32_t rc = map_bf16(&maps.d, a->y, a->ldy, a->M, a->N, "y")) return rc;
-  if (p.z_tma) if (int32_t rc = map_bf16(&maps.z, a->z, a->ldz, a->M, a->N, "z")) return rc;
-  if (p.gate_tma) if (int32_t rc = map_bf16(&maps.gate, a->gate, a->ldgate, a->M, a->N, "gate")) return rc;
-  if (p.residual_tma) if (int32_t rc = map_bf16(&maps.residual, a->residual, a->ldr, a->M, a->N, "residual")) return rc;
   const DenseOperand x = {a->x, a->ldx, false}, w = {a->w, a->ldw, false};
-  return a->gate || a->residual ? launch_dense<false, false, kEpiLinearOperands>(x, w, maps, p, st) : launch_dense<false, false, kEpiLinear>(x, w, maps, p, st);
+  CUtensorMap md = {}, mz = {};
+  if (p.d_wide) if (int32_t rc = map_bf16(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
+  if (p.z_wide) if (int32_t rc = map_bf16(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
+  if (a->gate || a->residual || a->z) return launch_dense<false, false, kEpiLinearWide>(x, w, md, p, st, mz);
+  return launch_dense<false, false, kEpiLinear>(x, w, md, p, st);
 }
 
 constexpr int kPointwiseGroups = 64;
@@ -896,7 +921,7 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (!a_mn_major && few_tokens(M, N, K)) {
     DenseParams p = {};
     p.M = M; p.N = N; p.K = K; p.status = status;
-    p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_tma = 1;
+    p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_wide = 1;
     return launch_dense_small(a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
   }
   return dense_sum({a, lda, a_mn_major != 0}, {b, ldb, true}, M, N, K, nullptr, 0, d, false, ldd, status, reinterpret_cast<cudaStream_t>(stream));
@@ -944,7 +969,7 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + ceil_div(a->M * 4, 16) * 16);
   p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
   const DenseOperand h = {a->h, a->ldh, false}, w = {a->w, a->ldw, false};
-  const DenseMaps none = {};
+  const CUtensorMap none = {};
   if (a->M <= kFewRows) {
     if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
   } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, p, st)) return rc;
@@ -987,11 +1012,11 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   for (int64_t v0 = 0; v0 < a->V; v0 += columns) {
     const int64_t n = a->V - v0 < columns ? a->V - v0 : columns;
     const bool last = v0 + n == a->V;
-    DenseMaps maps = {};
+    CUtensorMap mg = {};
     p.N = n;
     p.col0 = v0;
-    if (int32_t rc = map_bf16(&maps.d, g, columns, a->M, n, "G")) return rc;
-    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, maps, p, st)) return rc;
+    if (int32_t rc = map_bf16(&mg, g, columns, a->M, n, "G")) return rc;
+    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
     if (dh) {
       if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
                                  last ? dh : acc, !last, last ? lddh : a->K, a->status, st)) return rc;

@@ -217,8 +217,8 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       const int e = e0 + k * step;
       const int64_t n = n0 + 8 * (e & ((1 << shift) - 1)), m = m0 + (e >> shift);
       if (e < tokens << shift && n < p.N) {
-        if (p.gate) load_row8(p.gate + m * p.ldgate + n, p.gate_tma, p.N - n, gate[k]);
-        if (p.residual) load_row8(p.residual + m * p.ldr + n, p.residual_tma, p.N - n, residual[k]);
+        if (p.gate) load_row8(p.gate + m * p.ldgate + n, p.gate_wide, p.N - n, gate[k]);
+        if (p.residual) load_row8(p.residual + m * p.ldr + n, p.residual_wide, p.N - n, residual[k]);
       }
     }
 #pragma unroll
@@ -248,7 +248,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         for (int i = 0; i < 8; ++i)
           if (i < left) v[i] += p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + n + i) : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + n + i));
       }
-      if (p.z) store_row8(p.z + m * p.ldz + n, p.z_tma, left, v);
+      if (p.z) store_row8(p.z + m * p.ldz + n, p.z_wide, left, v);
       activate_all(p.act, v);
       if (p.gate) {
 #pragma unroll
@@ -258,7 +258,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[2 * i] += bf16_lo(residual[k][i]); v[2 * i + 1] += bf16_hi(residual[k][i]); }
       }
-      store_row8(p.d + m * p.ldd + n, p.d_tma, left, v);
+      store_row8(p.d + m * p.ldd + n, p.d_wide, left, v);
     }
   }
   __syncwarp();
