@@ -32,6 +32,23 @@ struct DenseParams {
   const float* c;  int64_t ldc;
 };
 
+// Products of few tokens (dense_small.cu).
+struct SmallShape {
+  int32_t rows;                                            // weight rows of a tile
+  int32_t bn;                                              // tokens of a tile, a multiple of 16
+  int32_t kb;                                              // blocks of 64 along the contraction to a stage
+  int32_t stages, stage_bytes;
+  int32_t splits, blocks_per_split;
+};
+struct SmallPlan {
+  SmallShape sh;
+  float us;
+};
+SmallPlan plan_dense_small(int64_t M, int64_t N, int64_t K, bool w_mn);
+int32_t launch_dense_small(const SmallShape& sh, const void* t, int64_t ldt, const void* w, bool w_mn, int64_t ldw, const DenseParams& p, cudaStream_t st);
+int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int64_t ldw, const DenseParams& p, cudaStream_t st);
+int64_t small_stats_slots(int64_t V);
+
 #ifdef __CUDACC__
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

@@ -18,23 +18,27 @@
 
 namespace metis {
 
-enum DenseEpilogue { kEpiLinear, kEpiLinearWide, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
+enum DenseEpilogue { kEpiLinear, kEpiLinearWide, kEpiLinearOdd, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
 
 template <int kEpi> struct DenseCfg {
-  static constexpr bool kWide = kEpi == kEpiLinearWide;
+  static constexpr bool kOperands = kEpi == kEpiLinearWide || kEpi == kEpiLinearOdd;
   static constexpr int kParts = 2;                         // epilogue warps for each 32-lane quarter of tensor memory
-  static constexpr int kStages = kWide ? 5 : 6;
+  static constexpr int kStages = kOperands ? 5 : 6;
   static constexpr int kHalfBytes = 128 * 128;             // 128 rows x 64 elements of A or of B
   static constexpr int kBoxBytes = 64 * 128;               // one MN-major box: 64 contraction rows x 64 elements
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kEpilogueWarps = 4 * kParts;
   static constexpr int kChunks = 8 / kParts;               // of 32 columns, that a warp takes of a tile
   static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-  static constexpr int kBuffers = kWide ? 4 : 2;           // of 32 rows x 64 bytes, for each epilogue warp
-  static constexpr int kStagingBytes = kEpilogueWarps * kBuffers * 2048;
+  // for each epilogue warp: buffers of 32 rows x 64 bytes for what is stored, then two for the pieces of the operands
+  static constexpr int kStores = kEpi == kEpiLinearOdd ? 1 : 2;
+  static constexpr int kPieceBytes = kEpi == kEpiLinearOdd ? 32 * 80 : 2048;
+  static constexpr int kWarpBytes = kStores * 2048 + (kOperands ? 2 * kPieceBytes : 0);
+  static constexpr int kStagingBytes = kEpilogueWarps * kWarpBytes;
   static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 };
-static_assert(DenseCfg<kEpiLinear>::kSmemBytes <= 227 * 1024 && DenseCfg<kEpiLinearWide>::kSmemBytes <= 227 * 1024);
+static_assert(DenseCfg<kEpiLinearOdd>::kWarpBytes % 512 == 0, "the swizzle of a stored piece counts from 512 bytes");
+static_assert(DenseCfg<kEpiLinear>::kSmemBytes <= 227 * 1024 && DenseCfg<kEpiLinearWide>::kSmemBytes <= 227 * 1024 && DenseCfg<kEpiLinearOdd>::kSmemBytes <= 227 * 1024);
 
 // ---- epilogue pieces ----------------------------------------------------------------------------------------
 
@@ -58,9 +62,10 @@ struct Staging {
 };
 
 // 32 rows x 64 bytes, one row per lane (four 16-byte pieces), through shared memory to the tensor at (row0, x): 64-byte swizzle.
+template <int kStores = 2>
 __device__ __forceinline__ void store_piece_tma(Staging& st, const CUtensorMap* map, const uint32_t (&w)[16], int32_t x, int32_t row0) {
   const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
-  uint8_t* buf = st.next();
+  uint8_t* buf = kStores == 2 ? st.next() : st.idle();
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
@@ -80,10 +85,17 @@ __device__ __forceinline__ void store_piece_rows(Staging& st, __nv_bfloat16* out
     *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
   __syncwarp();
   const bool live = col0 + lane < N;
-  const int rows = M - row0 < 32 ? (int)(M - row0) : 32;
-  for (int r = 0; r < rows; ++r) {
-    const uint8_t* at = buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2;
-    if (live) out[(row0 + r) * ld + col0 + lane] = *reinterpret_cast<const __nv_bfloat16*>(at);
+  unsigned short* to = reinterpret_cast<unsigned short*>(out) + row0 * ld + col0 + lane;
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 8) {                     // eight rows on their way at a time
+    unsigned short v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + i;
+      v[i] = *reinterpret_cast<const unsigned short*>(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (live && row0 + r0 + i < M) to[(r0 + i) * ld] = v[i];
   }
   __syncwarp();
 }
@@ -128,40 +140,75 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p,
   }
 }
 
-// An operand of the epilogue, [M, N] bf16.  Its pieces of 32 rows x 64 bytes come into a buffer of the warp's by asynchronous copies (four
-// lanes a row: whole sectors), the next one on its way while the last one is worked on; each fetch is a group of copies, empty or not.
-struct EpilogueOperand {
+// An operand of the epilogue, [M, N] bf16.  Its pieces of 32 rows x 64 bytes come into a buffer of the warp's by asynchronous copies, the
+// next one on its way while the last one is worked on; each fetch is a group of copies, empty or not.
+//   rows of whole 16-byte pieces: four lanes a row, so that a copy takes whole sectors; the ragged end of a row is load_piece_rows'
+//   any others (kOdd): the aligned 16 bytes that hold them, five a row since a row may begin anywhere in them, shifted when they are taken (what
+//     lies beside the piece in them belongs to the same allocation and is not used).  Without it every piece waits for four rounds of
+//     loads: 8192 x 8961 x 1536 with silu, gate and residual 840 us, by 4-byte copies 574, 8960 columns 199.
+template <bool kOdd> struct EpilogueOperand {
   const __nv_bfloat16* src;                                // null: there is none
   int64_t ld;
   bool wide;                                               // 16-byte aligned rows
   uint8_t* buf;
   __device__ __forceinline__ void fetch(bool valid, int64_t col0, int64_t row0, int64_t M, int64_t N) {
     __syncwarp();                                          // every lane has read what the buffer held
-    if (src && wide && valid && col0 + 32 <= N) {
-      const int lane = threadIdx.x & 31;
-      const __nv_bfloat16* at = src + (row0 + (lane >> 2)) * ld + col0 + (lane & 3) * 8;
-      const uint32_t to = smem_u32(buf);
+    const int lane = threadIdx.x & 31;
+    const uint32_t to = smem_u32(buf);
+    if constexpr (kOdd) {
+      if (src && valid) {
+        const int bytes = N - col0 < 32 ? 2 * (int)(N - col0) : 64, rows = M - row0 < 32 ? (int)(M - row0) : 32;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + (lane >> 2);
-        if (row0 + r < M)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)), "l"(at + 8 * i * ld) : "memory");
+        for (int i = 0; i < 5; ++i) {
+          const int at = i * 32 + lane, r = at / 5, k = at - r * 5;
+          const uintptr_t first = reinterpret_cast<uintptr_t>(src + (row0 + r) * ld + col0);
+          if (r < rows && 16 * k < bytes + (int)(first & 15))
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + at * 16), "l"((first & ~(uintptr_t)15) + 16 * k) : "memory");
+        }
+      }
+    } else {
+      if (src && wide && valid && col0 + 32 <= N) {
+        const __nv_bfloat16* at = src + (row0 + (lane >> 2)) * ld + col0 + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2);
+          if (row0 + r < M)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)), "l"(at + 8 * i * ld) : "memory");
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   // this lane's 32 elements of its row, of the piece that was fetched two groups ago
-  __device__ __forceinline__ void take(uint32_t (&w)[16]) {
-    const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  __device__ __forceinline__ void take(uint32_t (&w)[16], int64_t col0, int64_t row0) {
+    const int lane = threadIdx.x & 31;
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
+    if constexpr (kOdd) {
+      const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src + (row0 + lane) * ld + col0) & 15);
+      uint32_t x[20];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint4 t = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((k ^ swz) << 4));
-      w[4 * k] = t.x; w[4 * k + 1] = t.y; w[4 * k + 2] = t.z; w[4 * k + 3] = t.w;
+      for (int k = 0; k < 5; ++k) {
+        const uint4 t = *reinterpret_cast<const uint4*>(buf + lane * 80 + 16 * k);
+        x[4 * k] = t.x; x[4 * k + 1] = t.y; x[4 * k + 2] = t.z; x[4 * k + 3] = t.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 18; ++k) x[k] = (off & 8) ? x[k + 2] : x[k];
+#pragma unroll
+      for (int k = 0; k < 17; ++k) x[k] = (off & 4) ? x[k + 1] : x[k];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) w[k] = __funnelshift_r(x[k], x[k + 1], (off & 2) * 8);
+    } else {
+      const int swz = (lane >> 1) & 3;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 t = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((k ^ swz) << 4));
+        w[4 * k] = t.x; w[4 * k + 1] = t.y; w[4 * k + 2] = t.z; w[4 * k + 3] = t.w;
+      }
     }
   }
 };
+
 // The output alone: bias and activation, a store through the TMA unit.
 __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const uint32_t (&r)[32], int64_t row0, int64_t col0) {
   float v[32];
@@ -185,9 +232,10 @@ struct PieceAt {
   bool valid;
   int64_t row0, col0;
 };
-__device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, EpilogueOperand& gate,
-                                                  EpilogueOperand& residual, const uint32_t (&r)[32],
-                                                  int64_t row0, int64_t col0, const PieceAt& next) {
+template <bool kOdd>
+__device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, EpilogueOperand<kOdd>& gate,
+                                                  EpilogueOperand<kOdd>& residual, const uint32_t (&r)[32], int64_t row0, int64_t col0, const PieceAt& next) {
+  constexpr int kStores = kOdd ? 1 : 2;
   const bool full = col0 + 32 <= p.N;
   float v[32];
 #pragma unroll
@@ -197,19 +245,19 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   if (p.z) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (p.z_wide) store_piece_tma(st, map_z, w, (int32_t)col0, (int32_t)row0);
+    if (p.z_wide) store_piece_tma<kStores>(st, map_z, w, (int32_t)col0, (int32_t)row0);
     else store_piece_rows(st, p.z, p.ldz, w, col0, row0, p.M, p.N);
   }
   activate_all(p.act, v);
   if (gate.src) {
-    if (gate.wide && full) gate.take(w);
+    if (kOdd || (gate.wide && full)) gate.take(w, col0, row0);
     else load_piece_rows(st, gate.src, gate.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
   }
   gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
   if (residual.src) {
-    if (residual.wide && full) residual.take(w);
+    if (kOdd || (residual.wide && full)) residual.take(w, col0, row0);
     else load_piece_rows(st, residual.src, residual.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
@@ -217,7 +265,7 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-  if (p.d_wide) store_piece_tma(st, map_d, w, (int32_t)col0, (int32_t)row0);
+  if (p.d_wide) store_piece_tma<kStores>(st, map_d, w, (int32_t)col0, (int32_t)row0);
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
 
@@ -408,9 +456,10 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const int q = warp & 3;
     const int part = (warp - 2) >> 2;
     const uint32_t empty_leader = map_to_cta(smem_u32(acc_empty), 0);
-    Staging st{staging + (warp - 2) * (Cfg::kStagingBytes / Cfg::kEpilogueWarps)};
+    Staging st{staging + (warp - 2) * Cfg::kWarpBytes};
     // operands of the epilogue; `ahead` is the piece whose copies are on their way
-    EpilogueOperand gate = {p.gate, p.ldgate, p.gate_wide != 0, st.base + 4096}, residual = {p.residual, p.ldr, p.residual_wide != 0, st.base + 6144};
+    EpilogueOperand<kEpi == kEpiLinearOdd> gate = {p.gate, p.ldgate, p.gate_wide != 0, st.base + Cfg::kStores * 2048},
+                                           residual = {p.residual, p.ldr, p.residual_wide != 0, gate.buf + Cfg::kPieceBytes};
     PieceAt ahead = {false, 0, 0};
     auto first_piece = [&](int64_t t) {                      // this warp's first piece of tile t
       int64_t tm = 0, tn = 0;
@@ -444,7 +493,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           }
         }
       }
-      if constexpr (kEpi == kEpiLinearWide) {
+      if constexpr (Cfg::kOperands) {
         if (rows && n0 < p.N && !ahead.valid) {
           gate.fetch(true, n0, row0, p.M, p.N);
           residual.fetch(true, n0, row0, p.M, p.N);
@@ -461,7 +510,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       float picked = 0.0f;
       bool found = false;
       // the next chunk of the accumulator is read while this one is worked on, where the registers allow it
-      constexpr bool kAhead = kEpi != kEpiLinearWide;
+      constexpr bool kAhead = !Cfg::kOperands;
       uint32_t r[kAhead ? 2 : 1][32];
       if (kAhead) tc_load32(t_row, r[0]);
 #pragma unroll
@@ -481,7 +530,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           const int64_t at = hit - col0;                   // the target's place in this chunk
           const bool here = at >= 0 && at < 32;
           if constexpr (kEpi == kEpiLinear) linear_chunk(p, st, &map_d, v, row0, col0);
-          if constexpr (kEpi == kEpiLinearWide) {
+          if constexpr (Cfg::kOperands) {
             PieceAt next = {ch + 1 < Cfg::kChunks && col0 + 32 < p.N, row0, col0 + 32};
             if (!next.valid) next = ahead = first_piece(tile + num_pairs);
             linear_wide_chunk(p, st, &map_d, &map_z, gate, residual, v, row0, col0, next);
@@ -550,7 +599,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         }
       }
     }
-    if constexpr (kEpi == kEpiLinearWide) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (Cfg::kOperands) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (lane == 0) bulk_store_wait_all();                    // shared memory stays until the TMA unit has read it
   }
 
@@ -641,9 +690,57 @@ head_sum_kernel(const float* __restrict__ nll, const int64_t* __restrict__ targe
 
 // ---- backward of the epilogue -----------------------------------------------------------------------------------
 
-// dz = dy * gate * act'(z), dgate = dy * act(z), and column sums of dz before its rounding.  A warp's lane has kVec columns of a row,
-// the block's eight warps take eight rows at a time; a block owns 32 * kVec columns and every gridDim.y-th group of rows.
-template <int kAct, int kVec>
+// Eight consecutive elements at any address (of which `left` are in the row): the one or two aligned 16 bytes that hold them, shifted.  What
+// lies beside the row in them belongs to the same allocation and is not used.
+template <bool kWide> __device__ __forceinline__ void load8_any(const __nv_bfloat16* at, int64_t left, float (&v)[8]) {
+  if constexpr (kWide) {
+    Load8<__nv_bfloat16>::load(at, v);
+  } else {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+    const uint32_t off = (uint32_t)(a & 15);
+    const int64_t bytes = 2 * (left < 8 ? left : 8);
+    const uint4* p = reinterpret_cast<const uint4*>(a & ~(uintptr_t)15);
+    const uint4 lo = __ldg(p);
+    uint4 hi = make_uint4(0u, 0u, 0u, 0u);
+    if (off + bytes > 16) hi = __ldg(p + 1);
+    uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) x[k] = (off & 8) ? x[k + 2] : x[k];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) x[k] = (off & 4) ? x[k + 1] : x[k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = __funnelshift_r(x[k], x[k + 1], (off & 2) * 8);
+      v[2 * k] = bf16_lo(w);
+      v[2 * k + 1] = bf16_hi(w);
+    }
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) { return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])); }
+// The eight elements of every lane, 256 together, to a run of `count` elements at any address: through the warp's buffer, laid out there as the
+// run lies to 16 bytes, so that all but its two ends leave as whole 16 bytes.
+__device__ __forceinline__ void store_run(__nv_bfloat16* run, int count, unsigned short* buf, const float (&v)[8]) {
+  const int lane = threadIdx.x & 31, off = (int)(reinterpret_cast<uintptr_t>(run) & 15) >> 1;
+  const uint4 q = pack8(v);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) buf[off + lane * 8 + i] = (unsigned short)(w[i >> 1] >> ((i & 1) * 16));
+  __syncwarp();
+  unsigned short* to = reinterpret_cast<unsigned short*>(run) - off;
+  for (int k = lane; k * 8 < off + count; k += 32) {
+    if (k * 8 >= off && k * 8 + 8 <= off + count) {
+      *reinterpret_cast<uint4*>(to + k * 8) = *reinterpret_cast<const uint4*>(buf + k * 8);
+    } else {
+      for (int i = k * 8; i < k * 8 + 8; ++i) if (i >= off && i < off + count) to[i] = buf[i];
+    }
+  }
+}
+
+// dz = dy * gate * act'(z), dgate = dy * act(z), and column sums of dz before its rounding.  A warp's lane has eight columns of a row, the
+// block's eight warps take eight rows at a time; a block owns 256 columns and every gridDim.y-th group of rows.  dz has 16-byte aligned
+// rows; kWide: all the others do too, and N is a multiple of 8.  Bound by memory: 8192 x 8960 with gate 126 us, 5.8 TB/s.
+template <int kAct, bool kWide>
 __global__ void __launch_bounds__(256)
 linear_pointwise_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, const __nv_bfloat16* __restrict__ z, int64_t ldz,
                         const __nv_bfloat16* __restrict__ gate, int64_t ldgate, int64_t M, int64_t N,
@@ -651,62 +748,52 @@ linear_pointwise_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, cons
                         float* __restrict__ sums) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * kVec;
-  float acc[kVec];
+  const int64_t col0 = (int64_t)blockIdx.x * 256, col = col0 + lane * 8, left = N - col;
+  const int count = N - col0 < 256 ? (int)(N - col0) : 256;
+  __shared__ __align__(16) unsigned short s_run[8][264];
+  float acc[8];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
-  auto load = [](const __nv_bfloat16* at, float (&v)[kVec]) {
-    if constexpr (kVec == 8) Load8<__nv_bfloat16>::load(at, v);
-    else v[0] = __bfloat162float(__ldg(at));
-  };
-  auto store = [](__nv_bfloat16* at, const float (&v)[kVec]) {
-    if constexpr (kVec == 8) *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    else *at = __float2bfloat16_rn(v[0]);
-  };
-  if (col < N) {
-    for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < M; row += (int64_t)gridDim.y * 8) {
-      float d[kVec], a[kVec], out[kVec];
-      load(dy + row * lddy + col, d);
+  for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+  for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < M; row += (int64_t)gridDim.y * 8) {
+    float d[8], a[8], out[8];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) { a[i] = 1.0f; out[i] = d[i]; }
-      if (kAct != METIS_ACT_NONE || dgate) {
-        float zv[kVec];
-        load(z + row * ldz + col, zv);
+    for (int i = 0; i < 8; ++i) { d[i] = 0.0f; a[i] = 1.0f; }
+    if (left > 0) {
+      float zv[8], g[8];
+      load8_any<kWide>(dy + row * lddy + col, left, d);
+      if (kAct != METIS_ACT_NONE || dgate) load8_any<kWide>(z + row * ldz + col, left, zv);
+      if (gate) load8_any<kWide>(gate + row * ldgate + col, left, g);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+      for (int i = 0; i < 8; ++i) {
+        out[i] = d[i];
+        if (kAct != METIS_ACT_NONE || dgate) {
           float slope;
           activate_both<kAct>(zv[i], a[i], slope);
-          out[i] = d[i] * slope;
+          out[i] *= slope;
         }
+        if (gate) out[i] *= g[i];
+        a[i] *= d[i];
+        acc[i] += out[i];
       }
-      if (gate) {
-        float g[kVec];
-        load(gate + row * ldgate + col, g);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) out[i] *= g[i];
+      if (dz) {
+        __nv_bfloat16* to = dz + row * lddz + col;
+        if (kWide || left >= 8) *reinterpret_cast<uint4*>(to) = pack8(out);
+        else for (int i = 0; i < left; ++i) to[i] = __float2bfloat16_rn(out[i]);
       }
-      if (dgate) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) a[i] *= d[i];
-        store(dgate + row * lddg + col, a);
-      }
-      if (dz) store(dz + row * lddz + col, out);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) acc[i] += out[i];
+      if (kWide && dgate) *reinterpret_cast<uint4*>(dgate + row * lddg + col) = pack8(a);
     }
+    if (!kWide && dgate) store_run(dgate + row * lddg + col0, count, s_run[warp], a);
   }
   if (sums) {
-    __shared__ float s_sum[8][32 * kVec];
+    __shared__ float s_sum[8][256];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) s_sum[warp][lane * kVec + i] = acc[i];
+    for (int i = 0; i < 8; ++i) s_sum[warp][lane * 8 + i] = acc[i];
     __syncthreads();
-    for (int c = threadIdx.x; c < 32 * kVec; c += 256) {
-      float t = s_sum[0][c];
+    const int c = threadIdx.x;
+    float t = s_sum[0][c];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) t += s_sum[w][c];
-      const int64_t at = (int64_t)blockIdx.x * 32 * kVec + c;
-      if (at < N) sums[(int64_t)blockIdx.y * N + at] = t;
-    }
+    for (int w = 1; w < 8; ++w) t += s_sum[w][c];
+    if (col0 + c < N) sums[(int64_t)blockIdx.y * N + col0 + c] = t;
   }
 }
 
@@ -724,11 +811,6 @@ linear_bias_kernel(const float* __restrict__ sums, int groups, int64_t N, T* __r
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
-
-// dense_small.cu
-int32_t launch_dense_small(const void* t, int64_t ldt, const void* w, bool w_mn, int64_t ldw, const DenseParams& p, cudaStream_t st);
-int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int64_t ldw, const DenseParams& p, cudaStream_t st);
-int64_t small_stats_slots(int64_t V);
 
 static int32_t check_rows(const void* p, int64_t ld, int64_t cols, const char* what) {
   if (!p) return fail(METIS_ERR_BAD_ARGUMENT, "%s is null", what);
@@ -801,12 +883,21 @@ static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M
   return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, p, st);
 }
 
-// Whether a product of M tokens goes to the kernels for few of them (dense_small.cu).
-static bool few_tokens(int64_t M, int64_t N, int64_t K) {
+// Whether a product goes to the kernel for few tokens, with the shape it takes there: by a model of both.  A round of 256 x 256 tiles takes
+// 0.29 us for each stage of the contraction, and its start, end and launch 7.5 us; a quarter of the pairs or less of them busy is what it
+// loses by (3584 x 18944: 92 us for 1 to 256 tokens).
+static bool few_tokens(int64_t M, int64_t N, int64_t K, bool w_mn, SmallShape* sh) {
+  if (M > 2048) return false;
+  const SmallPlan plan = plan_dense_small(M, N, K, w_mn);
+  *sh = plan.sh;
+  const int64_t pairs = device_sm_count() / 2, rounds = ceil_div(ceil_div(M, 256) * ceil_div(N, 256), pairs > 0 ? pairs : 1);
+  const float tiles_us = 0.29f * (float)(rounds * ceil_div(K, 64)), memory_us = (float)(2 * N * K) / 5.5e6f;
+  const float pair_us = 7.5f + (tiles_us > memory_us ? tiles_us : memory_us);
 #ifdef METIS_TIMING_KNOBS
   if (const char* e = getenv("METIS_DEV_DENSE_SMALL")) return atoi(e) != 0;
+  if (getenv("METIS_DEV_DENSE_PRINT")) fprintf(stderr, "M %lld N %lld K %lld: small %.1f (rows %d bn %d kb %d splits %d stages %d) pair %.1f\n", (long long)M, (long long)N, (long long)K, plan.us, plan.sh.rows, plan.sh.bn, plan.sh.kb, plan.sh.splits, plan.sh.stages, pair_us);
 #endif
-  return M <= 128;
+  return plan.us < pair_us;
 }
 
 // Columns of the vocabulary that the backward pass takes at a time: their gradients G [M, columns] in bf16 go through memory.
@@ -833,6 +924,9 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   if (int32_t rc = check_rows(a->x, a->ldx, a->K, "x")) return rc;
   if (int32_t rc = check_rows(a->w, a->ldw, a->K, "w")) return rc;
   if (!a->y) return fail(METIS_ERR_BAD_ARGUMENT, "y is null");
+  const uintptr_t odd = reinterpret_cast<uintptr_t>(a->y) | reinterpret_cast<uintptr_t>(a->z) | reinterpret_cast<uintptr_t>(a->gate) | reinterpret_cast<uintptr_t>(a->residual);
+  if ((odd & 1u) || (reinterpret_cast<uintptr_t>(a->bias) & (a->bias_dtype == METIS_DTYPE_F32 ? 3u : 1u)))
+    return fail(METIS_ERR_BAD_ALIGNMENT, "a tensor is not aligned to its elements");
   if (a->ldy < a->N || (a->z && a->ldz < a->N) || (a->gate && a->ldgate < a->N) || (a->residual && a->ldr < a->N))
     return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
   DenseParams p = {};
@@ -844,11 +938,13 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_wide = wide(a->y, a->ldy);
   p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_wide = wide(a->z, a->ldz);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
-  if (few_tokens(a->M, a->N, a->K)) return launch_dense_small(a->x, a->ldx, a->w, false, a->ldw, p, st);
+  SmallShape sh;
+  if (few_tokens(a->M, a->N, a->K, false, &sh)) return launch_dense_small(sh, a->x, a->ldx, a->w, false, a->ldw, p, st);
   const DenseOperand x = {a->x, a->ldx, false}, w = {a->w, a->ldw, false};
   CUtensorMap md = {}, mz = {};
   if (p.d_wide) if (int32_t rc = map_bf16(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
   if (p.z_wide) if (int32_t rc = map_bf16(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
+  if ((a->gate && !p.gate_wide) || (a->residual && !p.residual_wide)) return launch_dense<false, false, kEpiLinearOdd>(x, w, md, p, st, mz);
   if (a->gate || a->residual || a->z) return launch_dense<false, false, kEpiLinearWide>(x, w, md, p, st, mz);
   return launch_dense<false, false, kEpiLinear>(x, w, md, p, st);
 }
@@ -860,14 +956,14 @@ extern "C" int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N) 
 }
 
 template <int kAct>
-static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool vec, dim3 grid, float* sums) {
+static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool wide, dim3 grid, float* sums) {
   auto launch = [&](auto kern) {
     return launch_overlapped(kLaunchStream, kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(a->stream),
                              static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __nv_bfloat16*>(a->z), a->ldz,
                              static_cast<const __nv_bfloat16*>(a->gate), a->ldgate, a->M, a->N, static_cast<__nv_bfloat16*>(a->dz), a->lddz,
                              static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
   };
-  METIS_CUDA_OK(vec ? launch(linear_pointwise_kernel<kAct, 8>) : launch(linear_pointwise_kernel<kAct, 1>));
+  METIS_CUDA_OK(wide ? launch(linear_pointwise_kernel<kAct, true>) : launch(linear_pointwise_kernel<kAct, false>));
   return METIS_OK;
 }
 
@@ -883,9 +979,12 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
     return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
   if (a->dbias && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_linear_pointwise_workspace_bytes(a->M, a->N)))
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
-  auto wide = [](const void* t, int64_t ld) { return !t || (aligned16(t) && ld % 8 == 0); };
-  const bool vec = a->N % 8 == 0 && wide(a->dy, a->lddy) && wide(a->z, a->ldz) && wide(a->gate, a->ldgate) && wide(a->dz, a->lddz) && wide(a->dgate, a->lddg);
-  const int64_t columns = ceil_div(a->N, vec ? 256 : 32);
+  auto rows16 = [](const void* t, int64_t ld) { return !t || (aligned16(t) && ld % 8 == 0); };
+  if (!rows16(a->dz, a->lddz)) return fail(METIS_ERR_BAD_ALIGNMENT, "dz must be 16-byte aligned with a leading dimension that is a multiple of 8");
+  for (const void* t : {a->dy, a->z, a->gate, static_cast<const void*>(a->dgate)})
+    if (reinterpret_cast<uintptr_t>(t) & 1u) return fail(METIS_ERR_BAD_ALIGNMENT, "tensors must be 2-byte aligned");
+  const bool wide = a->N % 8 == 0 && rows16(a->dy, a->lddy) && rows16(a->z, a->ldz) && rows16(a->gate, a->ldgate) && rows16(a->dgate, a->lddg);
+  const int64_t columns = ceil_div(a->N, 256);
   // with sums no more groups of rows than the workspace has; else about 16 blocks for each SM
   int64_t groups = ceil_div(a->M, 8), most = ceil_div((int64_t)device_sm_count() * 16, columns);
   if (a->dbias && most > kPointwiseGroups) most = kPointwiseGroups;
@@ -895,10 +994,10 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   const dim3 grid((unsigned)columns, (unsigned)groups);
   int32_t rc = METIS_OK;
   switch (a->activation) {
-    case METIS_ACT_SILU: rc = launch_pointwise<METIS_ACT_SILU>(a, vec, grid, sums); break;
-    case METIS_ACT_GELU: rc = launch_pointwise<METIS_ACT_GELU>(a, vec, grid, sums); break;
-    case METIS_ACT_GELU_TANH: rc = launch_pointwise<METIS_ACT_GELU_TANH>(a, vec, grid, sums); break;
-    default: rc = launch_pointwise<METIS_ACT_NONE>(a, vec, grid, sums);
+    case METIS_ACT_SILU: rc = launch_pointwise<METIS_ACT_SILU>(a, wide, grid, sums); break;
+    case METIS_ACT_GELU: rc = launch_pointwise<METIS_ACT_GELU>(a, wide, grid, sums); break;
+    case METIS_ACT_GELU_TANH: rc = launch_pointwise<METIS_ACT_GELU_TANH>(a, wide, grid, sums); break;
+    default: rc = launch_pointwise<METIS_ACT_NONE>(a, wide, grid, sums);
   }
   if (rc || !a->dbias) return rc;
   const dim3 blocks((unsigned)ceil_div(a->N, 256));
@@ -918,11 +1017,12 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (int32_t rc = check_rows(a, lda, a_mn_major ? M : K, "a")) return rc;
   if (int32_t rc = check_rows(b, ldb, N, "b")) return rc;
   if (int32_t rc = check_rows(d, ldd, N, "d")) return rc;
-  if (!a_mn_major && few_tokens(M, N, K)) {
+  SmallShape sh;
+  if (!a_mn_major && few_tokens(M, N, K, true, &sh)) {
     DenseParams p = {};
     p.M = M; p.N = N; p.K = K; p.status = status;
     p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_wide = 1;
-    return launch_dense_small(a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
+    return launch_dense_small(sh, a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
   }
   return dense_sum({a, lda, a_mn_major != 0}, {b, ldb, true}, M, N, K, nullptr, 0, d, false, ldd, status, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -123,7 +123,9 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
   operand(w, rw);
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = rw.rows;
-  LinearResult out{empty_like_options(x, shape, at::kBFloat16), keep_z ? empty_like_options(x, shape, at::kBFloat16) : Tensor()};
+  // (z is nobody else's: rows of whole 16-byte pieces)
+  const int64_t z_pitch = (rw.rows + 7) / 8 * 8;
+  LinearResult out{empty_like_options(x, shape, at::kBFloat16), keep_z ? empty_like_options(x, {rx.rows, z_pitch}, at::kBFloat16) : Tensor()};
   if (rx.rows == 0) return out;
   metis_linear_args a = {};
   a.M = rx.rows; a.N = rw.rows; a.K = rx.cols;
@@ -134,7 +136,7 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
   if (gate.defined()) { a.gate = gate.data_ptr(); a.ldgate = Rows(gate).ld; }
   if (residual.defined()) { a.residual = residual.data_ptr(); a.ldr = Rows(residual).ld; }
   a.y = out.y.data_ptr(); a.ldy = a.N;
-  a.z = ptr(out.z); a.ldz = a.N;
+  a.z = ptr(out.z); a.ldz = z_pitch;
   a.stream = stream_of(x);
   check(lib.metis_linear(&a), "metis_linear");
   launched += 1;
@@ -208,7 +210,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           a.M = M; a.N = N;
           a.dy = dy.data_ptr(); a.lddy = rdy.ld;
           a.activation = (int32_t)act;
-          if (saved[3].defined()) { a.z = saved[3].data_ptr(); a.ldz = N; }
+          if (saved[3].defined()) { a.z = saved[3].data_ptr(); a.ldz = saved[3].size(1); }
           if (saved[2].defined()) { a.gate = saved[2].data_ptr(); a.ldgate = Rows(saved[2]).ld; }
           if (write_dz) {
             const int64_t pitch = (N + 7) / 8 * 8;

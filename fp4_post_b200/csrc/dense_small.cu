@@ -8,22 +8,17 @@
 //   stats    (the head's losses) a CTA takes an even part of the vocabulary, in units of 32 rows, tile after tile with two accumulators;
 //            every epilogue lane keeps running statistics for each token of the rows it sees and the lanes are merged at the end.
 //
-// Roles: warp 0 loads, warp 1 issues, the others drain tensor memory.  No copy is multicast; every wait is bounded.
+// Roles: warp 0 loads, warp 1 issues, warps 2 and up drain tensor memory.  No copy is multicast; every wait is bounded.
 #include "dense.cuh"
 #include "pair.cuh"
 
+#include <atomic>
+
 namespace metis {
 
-constexpr int kSmallThreads = 192;
+constexpr int kSmallThreads = 384;                       // loader, issuer, eight that drain tensor memory; the epilogue is everybody's
 // Shared memory of a CTA: two fit an SM, so that clusters of any size find room; one where all CTAs run at once and leave none idle.
 constexpr int kSmallBudget = 100 * 1024, kSmallBudgetAlone = 200 * 1024;
-
-struct SmallShape {
-  int32_t rows;                                            // weight rows of a tile
-  int32_t bn;                                              // tokens of a tile, a multiple of 16
-  int32_t stages, stage_bytes;
-  int32_t splits, iters_per_split;
-};
 
 // Barriers, tensor memory and the abort flag behind the pipeline's stages.
 struct SmallBars {
@@ -72,8 +67,14 @@ __device__ __forceinline__ float4 load_cluster_f32x4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// Eight elements of a row of a bf16 operand as words (vec: 16-byte aligned rows); those past the end of the row are zero.
-__device__ __forceinline__ void load_row8(const __nv_bfloat16* src, bool vec, int64_t left, uint32_t (&w)[4]) {
+__device__ __forceinline__ float load_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+// Eight elements of a row of a bf16 operand as words: together (vec: 16-byte aligned rows), or `apart` from one another; those past the end
+// of the row are zero.
+__device__ __forceinline__ void load_row8(const __nv_bfloat16* src, bool vec, int apart, int64_t left, uint32_t (&w)[4]) {
   if (vec && left >= 8) {
     const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
     w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
@@ -81,17 +82,17 @@ __device__ __forceinline__ void load_row8(const __nv_bfloat16* src, bool vec, in
     const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = 2 * i < left ? __ldg(s + 2 * i) : 0, hi = 2 * i + 1 < left ? __ldg(s + 2 * i + 1) : 0;
+      const uint32_t lo = 2 * i * apart < left ? __ldg(s + 2 * i * apart) : 0, hi = (2 * i + 1) * apart < left ? __ldg(s + (2 * i + 1) * apart) : 0;
       w[i] = lo | (hi << 16);
     }
   }
 }
-__device__ __forceinline__ void store_row8(__nv_bfloat16* dst, bool vec, int64_t left, const float (&v)[8]) {
+__device__ __forceinline__ void store_row8(__nv_bfloat16* dst, bool vec, int apart, int64_t left, const float (&v)[8]) {
   if (vec && left >= 8) {
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < left) dst[i] = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 8; ++i) if (i * apart < left) dst[i * apart] = __float2bfloat16_rn(v[i]);
   }
 }
 
@@ -120,9 +121,12 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   const int rank = sh.splits > 1 ? (int)cluster_ctarank() : 0;
   const int64_t tile = blockIdx.x / sh.splits;
   const int64_t n0 = tile * sh.rows, m0 = (int64_t)blockIdx.y * sh.bn;
-  const int iters_all = (int)((p.K + 63) / 64);
-  const int it0 = rank * sh.iters_per_split;
-  const int iters = iters_all - it0 < sh.iters_per_split ? iters_all - it0 : sh.iters_per_split;      // at least one: the host sees to it
+  // this CTA's blocks of 64 along the contraction, `kb` of them to a stage (at least one: the host sees to it)
+  const int blocks_all = (int)((p.K + 63) / 64);
+  const int block0 = rank * sh.blocks_per_split;
+  const int blocks = blocks_all - block0 < sh.blocks_per_split ? blocks_all - block0 : sh.blocks_per_split;
+  const int block_bytes = token_bytes + sh.rows * 128;
+  const int iters = (blocks + sh.kb - 1) / sh.kb;
   const uint32_t tmem_cols = small_tmem_cols(sh.bn);
   small_setup(bars, sh.stages, tmem_cols, 1);
   const uint32_t tmem_base = *bars.tmem_slot;
@@ -138,15 +142,19 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         break;
       }
       if (elect_one()) {
-        const uint32_t st = base + stage * sh.stage_bytes, sw = st + token_bytes, bar = smem_u32(&bars.full[stage]);
-        const int32_t k0 = (it0 + it) * 64;
-        mbar_expect_tx_addr(bar, (uint32_t)sh.stage_bytes);
-        if (kWMn) {
-          for (int r = 0; r < sh.rows; r += 64) tma_load_2d_addr(sw + r * 128, &map_w, (int32_t)n0 + r, k0, bar);
-        } else {
-          tma_load_2d_addr(sw, &map_w, k0, (int32_t)n0, bar);
+        const uint32_t bar = smem_u32(&bars.full[stage]);
+        const int n_blocks = blocks - it * sh.kb < sh.kb ? blocks - it * sh.kb : sh.kb;
+        mbar_expect_tx_addr(bar, (uint32_t)(n_blocks * block_bytes));
+        for (int b = 0; b < n_blocks; ++b) {
+          const uint32_t st = base + stage * sh.stage_bytes + b * block_bytes, sw = st + token_bytes;
+          const int32_t k0 = (block0 + it * sh.kb + b) * 64;
+          if (kWMn) {
+            for (int r = 0; r < sh.rows; r += 64) tma_load_2d_addr(sw + r * 128, &map_w, (int32_t)n0 + r, k0, bar);
+          } else {
+            tma_load_2d_addr(sw, &map_w, k0, (int32_t)n0, bar);
+          }
+          tma_load_2d_addr(st, &map_t, k0, (int32_t)m0, bar);
         }
-        tma_load_2d_addr(st, &map_t, k0, (int32_t)m0, bar);
       }
       if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
     }
@@ -164,8 +172,11 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t st = base + stage * sh.stage_bytes;
-        small_mma<kWMn>(tmem_base, st + token_bytes, st, idesc, it == 0);
+        const int n_blocks = blocks - it * sh.kb < sh.kb ? blocks - it * sh.kb : sh.kb;
+        for (int b = 0; b < n_blocks; ++b) {
+          const uint32_t st = base + stage * sh.stage_bytes + b * block_bytes;
+          small_mma<kWMn>(tmem_base, st + token_bytes, st, idesc, it == 0 && b == 0);
+        }
         tc_commit(&bars.empty[stage]);
         if (it == iters - 1) tc_commit(bars.acc_full);
       }
@@ -178,7 +189,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       while (!mbar_try(bars.drain, 0) && global_ns() - t0 < kWaitLimitNs) {}
     }
     __syncwarp();
-  } else {
+  } else if (warp < 10) {
     const int q = warp & 3;
     if (!mbar_wait(bars.acc_full, 0, bars.abort_flag)) {
       if (lane == 0) report(p.status, bars.abort_flag, METIS_DEV_TIMEOUT_MMA);
@@ -187,7 +198,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16);
       if (q * 32 < sh.rows) {
-        for (int c0 = 0; c0 < sh.bn && m0 + c0 < p.M; c0 += 32) {
+        for (int c0 = ((warp - 2) >> 2) * 32; c0 < sh.bn && m0 + c0 < p.M; c0 += 64) {
           uint32_t r[32];
           tc_load32(t_row + c0, r);
           tc_wait_ld(r);
@@ -203,10 +214,13 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   small_free(tmem_base, tmem_cols);
   if (sh.splits > 1) cluster_sync_all();                   // the partial sums of every CTA are in place
 
-  // Items of eight weight rows of one token, the CTAs of the cluster in turn; a thread has the epilogue's operands of kFly items in
-  // flight before it uses them (one element at a time, 64 tokens of the silu and gate of 18944 rows: 56 us for the product; 35 so).
+  // Items of eight elements of one token, the CTAs of the cluster in turn; a thread has the epilogue's operands of kFly items in
+  // flight before it uses them (one element at a time, 64 tokens of the silu and gate of 18944 rows: 56 us for the product; 29 so).
+  // The eight lie together where rows are 16-byte aligned, else an item apart, so that neighbouring lanes have neighbouring elements.
   const int tokens = p.M - m0 < sh.bn ? (int)(p.M - m0) : sh.bn;
   const int shift = sh.rows == 128 ? 4 : sh.rows == 64 ? 3 : 2;        // log2 of the items of a token
+  const bool wide = p.d_wide && (!p.z || p.z_wide) && (!p.gate || p.gate_wide) && (!p.residual || p.residual_wide);
+  const int apart = wide ? 1 : 1 << shift, first = wide ? 8 : 1;
   const uint32_t mine = smem_u32(partial);
   constexpr int kFly = 4;
   const int step = sh.splits * kSmallThreads;
@@ -215,40 +229,42 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
       const int e = e0 + k * step;
-      const int64_t n = n0 + 8 * (e & ((1 << shift) - 1)), m = m0 + (e >> shift);
+      const int64_t n = n0 + first * (e & ((1 << shift) - 1)), m = m0 + (e >> shift);
       if (e < tokens << shift && n < p.N) {
-        if (p.gate) load_row8(p.gate + m * p.ldgate + n, p.gate_wide, p.N - n, gate[k]);
-        if (p.residual) load_row8(p.residual + m * p.ldr + n, p.residual_wide, p.N - n, residual[k]);
+        if (p.gate) load_row8(p.gate + m * p.ldgate + n, wide, apart, p.N - n, gate[k]);
+        if (p.residual) load_row8(p.residual + m * p.ldr + n, wide, apart, p.N - n, residual[k]);
       }
     }
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
       const int e = e0 + k * step;
-      const int r = 8 * (e & ((1 << shift) - 1)), t = e >> shift;
+      const int r = first * (e & ((1 << shift) - 1)), t = e >> shift;
       const int64_t n = n0 + r, m = m0 + t, left = p.N - n;
       if (e >= tokens << shift || left <= 0) continue;
       float v[8];
-      if (sh.splits > 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        const uint32_t at = mine + (t * 128 + r) * 4;
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      const uint32_t at = mine + (t * 128 + r) * 4;
 #pragma unroll 4
-        for (int s = 0; s < sh.splits; ++s) {
-          const uint32_t from = map_to_cta(at, s);
+      for (int s = 0; s < sh.splits; ++s) {
+        const uint32_t from = sh.splits > 1 ? map_to_cta(at, s) : at;
+        if (wide) {
           const float4 a = load_cluster_f32x4(from), b = load_cluster_f32x4(from + 16);
           v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
           v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += load_cluster_f32(from + i * apart * 4);
         }
-      } else {
-        const float4 a = *reinterpret_cast<const float4*>(partial + t * 128 + r), b = *reinterpret_cast<const float4*>(partial + t * 128 + r + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
       }
       if (p.bias) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < left) v[i] += p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + n + i) : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + n + i));
+        for (int i = 0; i < 8; ++i) {
+          const int64_t c = n + i * apart;
+          if (i * apart < left) v[i] += p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + c) : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + c));
+        }
       }
-      if (p.z) store_row8(p.z + m * p.ldz + n, p.z_wide, left, v);
+      if (p.z) store_row8(p.z + m * p.ldz + n, wide, apart, left, v);
       activate_all(p.act, v);
       if (p.gate) {
 #pragma unroll
@@ -258,7 +274,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[2 * i] += bf16_lo(residual[k][i]); v[2 * i + 1] += bf16_hi(residual[k][i]); }
       }
-      store_row8(p.d + m * p.ldd + n, p.d_wide, left, v);
+      store_row8(p.d + m * p.ldd + n, wide, apart, left, v);
     }
   }
   __syncwarp();
@@ -437,37 +453,95 @@ dense_small_stats_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
 
 // ---- host side ------------------------------------------------------------------------------------------------
 
-// Tile rows and splits of a product of N weight rows: the grid whose busiest SM reads least.  A split has four stages at least (the cluster's
-// meeting costs as much as their load).
-static SmallShape small_linear_shape(int64_t M, int64_t N, int64_t K, bool w_mn) {
-  SmallShape best = {};
-  const int64_t iters = ceil_div(K, 64), sms = device_sm_count();
-  const int bn = M >= 128 ? 128 : (int)(ceil_div(M, 16) * 16);
-  const int64_t token_tiles = ceil_div(M, bn);
-  int64_t best_cost = INT64_MAX;
-  for (int rows = 128; rows >= (w_mn ? 64 : 32); rows >>= 1) {
-    for (int splits = 1; splits <= 8; ++splits) {
-      const int64_t per = ceil_div(iters, splits);
-      if (splits > 1 && (per < 4 || ceil_div(iters, per) != splits)) continue;
-      const int64_t ctas = ceil_div(N, rows) * splits * token_tiles;
-      const int64_t cost = ceil_div(ctas, sms) * per * (rows + bn) + (splits > 1 ? 4 * (128 + bn) : 0);
-      if (cost < best_cost) {
-        best_cost = cost;
-        best.rows = rows; best.splits = splits; best.iters_per_split = (int)per;
+// Clusters of `splits` CTAs with `smem` bytes each that run at once on the current device, asked once.
+static int resident_clusters(int splits, int which, const void* kern, int smem) {
+  static std::atomic<int> known[64][9][2][2];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  std::atomic<int>& slot = known[dev][splits][which & 1][which >> 1];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)splits);
+    cfg.blockDim = dim3(kSmallThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallBudgetAlone) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    slot.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Shape of a product, and its time in us by the model that chooses it.  A stage takes an SM 0.25 us at least (the round through its two
+// barriers), its bytes come at 108 GB/s an SM and 10 TB/s over all of them, the weight from memory at 5.5 TB/s; around that 4.2 us, 13 ns
+// for each token of a tile and 0.15 ns for each element (drain and epilogue), where a cluster meets 1.5 us and 10 ns a
+// token more, and 4 us for every further round of CTAs.  Measured against the model, us, by rows of a
+// tile, blocks to a stage, splits: 1 x 3584 x 18944 26.4 (128, 2, 4), 27.8 (64, 4, 4), 81 (32, 1, 1); 64 x 3584 x 18944 30.1 (128, 2, 4), 34.0
+// (128, 1, 5); 256 x 3584 x 3584 21.1 (128, 1, 4), 30.2 (32, 1, 1); 256 x 1536 x 1536 14.0 (64, 1, 4), 16.2 (64, 1, 2); 1 x 18944 x 3584 24.5
+// (128, 2, 1), 25.3 (64, 4, 1).
+SmallPlan plan_dense_small(int64_t M, int64_t N, int64_t K, bool w_mn) {
+  SmallPlan best = {};
+  best.us = 1e30f;
+  const int64_t blocks = ceil_div(K, 64), sms = device_sm_count();
+  const int64_t token_tiles = ceil_div(M, 256);
+  const int bn = (int)(ceil_div(ceil_div(M, token_tiles), 16) * 16);
+  const void* kern = w_mn ? reinterpret_cast<const void*>(dense_small_kernel<true>) : reinterpret_cast<const void*>(dense_small_kernel<false>);
+  const float memory_us = (float)(2 * N * K) / 5.5e6f;
+  for (int alone = 0; alone < 2; ++alone) {
+    const int budget = alone ? kSmallBudgetAlone : kSmallBudget;
+    for (int rows = 128; rows >= (w_mn ? 64 : 32); rows >>= 1) {
+      const int block_bytes = (rows + bn) * 128;
+      int kb = 4;                                          // a stage of up to 48 KiB, four of them at least
+      while (kb > 1 && (kb * block_bytes > 48 * 1024 || 4 * kb * block_bytes > budget - 2048 - (128 - rows) * 128)) kb >>= 1;
+      const int stage_bytes = kb * block_bytes;
+      int stages = (budget - 2048 - (128 - rows) * 128) / stage_bytes;
+      if (stages > 24) stages = 24;
+      if (stages < 3 || 2048 + bn * 512 > budget) continue;
+      for (int splits = 1; splits <= 8; ++splits) {
+        const int64_t per = ceil_div(blocks, splits);
+        if (splits > 1 && (per < 4 || ceil_div(blocks, per) != splits)) continue;
+        const int64_t clusters = ceil_div(N, rows) * token_tiles, at_once = resident_clusters(splits, alone + 2 * w_mn, kern, budget);
+        const int64_t rounds = ceil_div(clusters, at_once), ctas = (clusters < at_once ? clusters : at_once) * splits;
+        const float sharing = ctas > sms ? (float)ctas / (float)sms : 1.0f;
+        float block_us = sharing * (float)block_bytes / 108e3f;
+        const float all_us = (float)block_bytes * (float)ctas / 10e6f, trip_us = 0.25f / (float)kb;
+        if (block_us < all_us) block_us = all_us;
+        if (block_us < trip_us) block_us = trip_us;
+        const float feed_us = (float)(rounds * per) * block_us;
+        const float us = (feed_us > memory_us ? feed_us : memory_us) + 4.0f * (float)(rounds - 1) + 4.2f + 0.013f * (float)bn + 0.00015f * (float)(rows * bn) + (splits > 1 ? 1.5f + 0.01f * (float)bn : 0.0f);
+        if (us < best.us) {
+          best.us = us;
+          best.sh = SmallShape{rows, bn, kb, stages, stage_bytes, splits, (int)per};
+        }
       }
     }
   }
-  best.bn = bn;
-  best.stage_bytes = (best.rows + bn) * 128;
-  const int budget = best.splits <= 2 && ceil_div(N, best.rows) * best.splits * token_tiles <= sms ? kSmallBudgetAlone : kSmallBudget;
-  best.stages = (budget - 2048 - (128 - best.rows) * 128) / best.stage_bytes;
-  if (best.stages > 24) best.stages = 24;
+#ifdef METIS_TIMING_KNOBS
+  if (const char* e = getenv("METIS_DEV_SMALL_SHAPE")) {       // rows,kb,splits,alone
+    int r, kb, sp, al;
+    if (sscanf(e, "%d,%d,%d,%d", &r, &kb, &sp, &al) == 4) {
+      const int stage_bytes = kb * (r + bn) * 128;
+      int stages = ((al ? kSmallBudgetAlone : kSmallBudget) - 2048 - (128 - r) * 128) / stage_bytes;
+      if (stages > 24) stages = 24;
+      const int64_t per = ceil_div(blocks, sp);
+      if (stages >= 2 && ceil_div(blocks, per) == sp) best.sh = SmallShape{r, bn, kb, stages, stage_bytes, sp, (int)per};
+    }
+  }
+#endif
   return best;
 }
 
 // d = epilogue(T W^T) for tokens t [M, K] and a weight w [N, K] (or [K, N])
-int32_t launch_dense_small(const void* t, int64_t ldt, const void* w, bool w_mn, int64_t ldw, const DenseParams& p, cudaStream_t st) {
-  const SmallShape sh = small_linear_shape(p.M, p.N, p.K, w_mn);
+int32_t launch_dense_small(const SmallShape& sh, const void* t, int64_t ldt, const void* w, bool w_mn, int64_t ldw, const DenseParams& p, cudaStream_t st) {
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mt, mw;
   if (int32_t rc = make_map(&mt, dt, 2, t, p.K, p.M, ldt * 2, 64, sh.bn, "tokens")) return rc;

@@ -475,7 +475,7 @@ int32_t metis_linear(const metis_linear_args* args);
 /*
  * Gradients through that epilogue: dz = bf16(dy * gate * act'(z)), dgate = bf16(dy * act(z)), dbias = sum over rows of
  * dy * gate * act'(z) in fp32, rounded once.  Each output may be null; gate null: 1.  z is not read where neither the
- * activation nor dgate needs it.  The workspace is for dbias alone.
+ * activation nor dgate needs it.  dz has 16-byte aligned rows.  The workspace is for dbias alone.
  */
 typedef struct metis_linear_pointwise_args {
   int64_t M, N;

@@ -39,7 +39,9 @@ def test_linear_refuses_bad_parts_of_the_epilogue(L, p):
     assert L.metis_linear(linear_args(p, x=p + 2)) == -3
     assert L.metis_linear(linear_args(p, w=p + 8)) == -3
     assert L.metis_linear(linear_args(p, bias=p, bias_dtype=7)) == -1
+    assert L.metis_linear(linear_args(p, y=p + 1)) == -3 and L.metis_linear(linear_args(p, bias=p + 2, bias_dtype=1)) == -3
     for name, ld in (("gate", "ldgate"), ("residual", "ldr"), ("z", "ldz")):
+        assert L.metis_linear(linear_args(p, **{name: p + 1, ld: 24})) == -3
         assert L.metis_linear(linear_args(p, **{name: p, ld: 23})) == -1
 
 
@@ -53,6 +55,7 @@ def test_pointwise_refuses(L, p):
     assert call(M=0) == -2 and call(N=-1) == -2 and call(dy=None) == -1 and call(dz=None) == -1 and call(z=None) == -1
     assert call(activation=9) == -1 and call(lddy=8) == -1 and call(lddz=8) == -1 and call(gate=p, ldgate=8) == -1 and call(dgate=p, lddg=2) == -1
     assert call(dbias=p, dbias_dtype=5) == -1
+    assert call(dz=p + 2) == -3 and call(lddz=28) == -3 and call(dy=p + 1) == -3          # dz is an operand of the products behind it
     assert call(dbias=p, dbias_dtype=0) == -4                                        # no workspace
     assert call(dbias=p, dbias_dtype=0, workspace=p, workspace_bytes=16) == -4
     assert call(dbias=p, dbias_dtype=0, workspace=p + 4, workspace_bytes=1 << 30) == -4
