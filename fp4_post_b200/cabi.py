@@ -44,7 +44,7 @@ EXPORTS = (
     "metis_bf16_panel_gemm_workspace_bytes", "metis_bf16_panel_gemm",
     "metis_lowrank_dts_workspace_bytes", "metis_lowrank_dts", "metis_lowrank_dts_mean", "metis_lowrank_du_workspace_bytes", "metis_lowrank_du",
     "metis_rope_pair", "metis_silu_mul",
-    "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product",
+    "metis_dense_launches", "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product",
     "metis_head_loss_workspace_bytes", "metis_head_loss", "metis_head_sum", "metis_head_backward_workspace_bytes", "metis_head_backward",
 )
 
@@ -186,6 +186,8 @@ def lib() -> C.CDLL:
     L.metis_rope_pair.restype = i32
     L.metis_silu_mul.argtypes = [vp, vp, vp, i64, vp]
     L.metis_silu_mul.restype = i32
+    L.metis_dense_launches.argtypes = []
+    L.metis_dense_launches.restype = i64
     L.metis_linear.argtypes = [C.POINTER(LinearArgs)]
     L.metis_linear.restype = i32
     L.metis_linear_pointwise_workspace_bytes.argtypes = [i64, i64]
@@ -253,11 +255,6 @@ def dense_host():
     if _dense_lib is None or _dense_lib is not _lib:
         _bind_dense()
     return _dense
-
-
-def dense_launches() -> int:
-    """Kernels that dense.py's calls have launched since import."""
-    return 0 if _dense is None else _dense.launches()
 
 
 def check(rc: int, what: str) -> None:

@@ -4,6 +4,9 @@
 
 #include "gemm_common.cuh"
 
+#include <atomic>
+#include <utility>
+
 namespace metis {
 
 struct DenseParams {
@@ -19,11 +22,14 @@ struct DenseParams {
   __nv_bfloat16* z;               int64_t ldz;     int32_t z_wide;
   // head: logits l = scale * (A B^T); columns of the vocabulary [0, N) of this launch are [col0, col0 + N) of all
   const int64_t* target;  int64_t ignore;
+  const int32_t* row_of;                                   // the rows that are not ignored, one after the other (null: all rows, as they lie)
+  const int32_t* live;  int32_t live_is_k;                 // their number, in place of M, or of K where the rows are contracted (null: neither)
+  int64_t stats_ld;
   int64_t vocab;  int64_t col0;
   float scale, scale_log2e;                                // 1 / temperature, and that times log2(e)
   float weight_scale;                                      // scale, with the sign of the loss
-  float2* stats;                                           // [slots, M]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum)
-  float* stats_e;                                          // [slots, M]: sum of 2^(..) (l log2(e) - maximum), or null
+  float2* stats;                                           // [slots, stats_ld]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum)
+  float* stats_e;                                          // [slots, stats_ld]: sum of 2^(..) (l log2(e) - maximum), or null
   float* picked;                                           // [M]: logit of the target
   const float* lse;                                        // [M]
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss: gout[row * stride] times *inv_count (null: 1)
@@ -31,6 +37,8 @@ struct DenseParams {
   // sum of pieces: fp32 addend
   const float* c;  int64_t ldc;
 };
+
+extern std::atomic<int64_t> dense_launches;                // kernels launched by the entry points of these two files
 
 // Products of few tokens (dense_small.cu).
 struct SmallShape {
@@ -51,7 +59,21 @@ int64_t small_stats_slots(int64_t V);
 
 #ifdef __CUDACC__
 
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_counted(int launch_class, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+  dense_launches.fetch_add(1, std::memory_order_relaxed);
+  return launch_overlapped(launch_class, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// A count that the kernel before wrote, read behind grid_dependency_wait().  Through a const __restrict__ pointer, or by __ldg, the compiler may
+// take a load for one of memory that nobody writes and move it in front of that wait.
+__device__ __forceinline__ int32_t load_count(const int32_t* p) {
+  int32_t n;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(n) : "l"(p) : "memory");
+  return n;
+}
 
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;

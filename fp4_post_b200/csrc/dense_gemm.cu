@@ -18,6 +18,8 @@
 
 namespace metis {
 
+std::atomic<int64_t> dense_launches{0};
+
 enum DenseEpilogue { kEpiLinear, kEpiLinearWide, kEpiLinearOdd, kEpiStats, kEpiStatsEntropy, kEpiGrad, kEpiSum, kEpiSumF32 };
 
 template <int kEpi> struct DenseCfg {
@@ -112,7 +114,7 @@ __device__ __forceinline__ void load_piece_rows(Staging& st, const __nv_bfloat16
   for (int r0 = 0; r0 < 32; r0 += 8) {
     unsigned short v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = live && row0 + r0 + i < M ? __ldg(s + (r0 + i) * ld) : (unsigned short)0;
+    for (int i = 0; i < 8; ++i) v[i] = live && row0 + r0 + i < M ? s[(r0 + i) * ld] : (unsigned short)0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = r0 + i;
@@ -132,11 +134,11 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const DenseParams& p,
   if (p.bias_f32) {
     const float* b = static_cast<const float*>(p.bias) + col0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += __ldg(b + i);
+    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += b[i];
   } else {
     const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.bias) + col0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += __bfloat162float(__ldg(b + i));
+    for (int i = 0; i < 32; ++i) if (full || col0 + i < p.N) v[i] += __bfloat162float(b[i]);
   }
 }
 
@@ -332,10 +334,6 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   const uint32_t cta = cluster_ctarank();                  // 0 = leader
   const int64_t pair = blockIdx.x >> 1;
   const int64_t num_pairs = gridDim.x >> 1;
-  const int64_t tiles_m = (p.M + 255) / 256;
-  const int64_t tiles_n = (p.N + BN - 1) / BN;
-  const int64_t num_tiles = tiles_m * tiles_n;
-  const int iters = (int)((p.K + 63) / 64);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -355,6 +353,18 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_dependency_wait();                                  // everything above touches shared and tensor memory only
+
+  // (scalars of their own: a changed copy of the parameters was read back unchanged)
+  int64_t M = p.M, K = p.K;
+  if (p.live) {
+    const int64_t n = load_count(p.live);
+    if (p.live_is_k) K = n;
+    else M = n;
+  }
+  const int64_t tiles_m = (M + 255) / 256;
+  const int64_t tiles_n = (p.N + BN - 1) / BN;
+  const int64_t num_tiles = tiles_m * tiles_n;
+  const int iters = (int)((K + 63) / 64);                // 0 where no row is left: the sums are zeros
 
   if (warp == 0) {
     // ===== TMA producer (both CTAs): every copy reports to the leader's barrier =====
@@ -400,7 +410,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     grid_launch_dependents();                                // the last loads of this CTA are on their way: let the next kernel's CTAs in
   } else if (warp == 1) {
     // ===== tensor-core issuer (leader only) =====
-    if (cta == 0) {
+    if (cta == 0 && iters > 0) {
       int stage = 0;
       uint32_t phase = 0, local_tile = 0;
       bool ok = true, issued = false;
@@ -465,7 +475,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       int64_t tm = 0, tn = 0;
       if (t < num_tiles) tile_coords(t, tiles_m, tiles_n, p.band, tm, tn);
       PieceAt at = {t < num_tiles, tm * 256 + cta * 128 + q * 32, tn * BN + part * (32 * Cfg::kChunks)};
-      at.valid = at.valid && at.row0 < p.M && at.col0 < p.N;
+      at.valid = at.valid && at.row0 < M && at.col0 < p.N;
       return at;
     };
     uint32_t local_tile = 0;
@@ -476,31 +486,35 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const int64_t row0 = tm * 256 + cta * 128 + q * 32;
       const int64_t row = row0 + lane;
       const int64_t n0 = tn * BN + part * (32 * Cfg::kChunks);
-      const bool rows = row0 < p.M;                        // warp-uniform: the tile's rows of this warp are not all past the end
+      // warp-uniform: there are rows of this warp in the tile; the logits' gradient has zeros up to the next multiple of 64, what a stage of the
+      // contraction over the rows reads
+      const bool rows = row0 < (kEpi == kEpiGrad ? (M + 63) / 64 * 64 : M);
       int64_t hit = -1;                                    // the target's column in this launch
       float lse2 = 0.0f, weight = 0.0f;
       bool dead = true;
       if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy || kEpi == kEpiGrad) {
-        if (row < p.M) {
-          const int64_t t = __ldg(p.target + row);
+        if (row < M) {
+          const int64_t given = p.row_of ? p.row_of[row] : row;
+          const int64_t t = p.target[given];
           if (t != p.ignore && t >= 0 && t < p.vocab) hit = t - p.col0;
           if constexpr (kEpi == kEpiGrad) {
             dead = t == p.ignore;
-            lse2 = __ldg(p.lse + row) * kLog2e;
-            weight = __ldg(p.gout + row * p.gout_stride) * p.weight_scale;
-            if (p.inv_count) weight *= __ldg(p.inv_count);
+            lse2 = p.lse[given] * kLog2e;
+            weight = p.gout[given * p.gout_stride] * p.weight_scale;
+            if (p.inv_count) weight *= *p.inv_count;
             if (t < 0 || t >= p.vocab) weight = NAN;       // (a target outside the vocabulary; ignored rows are dead)
           }
         }
       }
       if constexpr (Cfg::kOperands) {
         if (rows && n0 < p.N && !ahead.valid) {
-          gate.fetch(true, n0, row0, p.M, p.N);
-          residual.fetch(true, n0, row0, p.M, p.N);
+          gate.fetch(true, n0, row0, M, p.N);
+          residual.fetch(true, n0, row0, M, p.N);
         }
         ahead.valid = false;
       }
-      if (!mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
+      const bool sums = iters > 0;
+      if (sums && !mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
         if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_MMA);
         break;
       }
@@ -512,18 +526,23 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       // the next chunk of the accumulator is read while this one is worked on, where the registers allow it
       constexpr bool kAhead = !Cfg::kOperands;
       uint32_t r[kAhead ? 2 : 1][32];
-      if (kAhead) tc_load32(t_row, r[0]);
+      if (kAhead && sums) tc_load32(t_row, r[0]);
 #pragma unroll
       for (int ch = 0; ch < Cfg::kChunks; ++ch) {
         uint32_t(&v)[32] = r[kAhead ? ch & 1 : 0];
-        if (!kAhead) tc_load32(t_row + ch * 32, v);
-        tc_wait_ld(v);
-        if (ch < Cfg::kChunks - 1) {
-          if (kAhead) tc_load32(t_row + (ch + 1) * 32, r[kAhead ? (ch + 1) & 1 : 0]);
+        if (sums) {
+          if (!kAhead) tc_load32(t_row + ch * 32, v);
+          tc_wait_ld(v);
+          if (ch < Cfg::kChunks - 1) {
+            if (kAhead) tc_load32(t_row + (ch + 1) * 32, r[kAhead ? (ch + 1) & 1 : 0]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_leader + buf * 8);
+          }
         } else {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(empty_leader + buf * 8);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0u;
         }
         const int64_t col0 = n0 + ch * 32;
         if (rows && col0 < p.N) {
@@ -561,7 +580,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             float g[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(v[i]);
-            if (p.c && row < p.M) {
+            if (p.c && row < M) {
               const float* c = p.c + row * p.ldc + col0;
               if (col0 + 32 <= p.N) {
 #pragma unroll
@@ -591,8 +610,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         }
       }
       if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
-        if (row < p.M) {
-          const int64_t slot = (tn * 2 + part) * p.M + row;
+        if (row < M) {
+          const int64_t slot = (tn * 2 + part) * p.stats_ld + row;
           p.stats[slot] = make_float2(stats.m, stats.s);
           if constexpr (kEpi == kEpiStatsEntropy) p.stats_e[slot] = stats.e;
           if (found) p.picked[row] = picked;
@@ -618,15 +637,17 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 // neighbouring rows).  A block takes 32 rows; its eight warps take the slots in turn and are merged in a fixed order.
 template <bool kEntropy>
 __global__ void __launch_bounds__(256)
-head_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ stats_e, const float* __restrict__ picked,
-                 const int64_t* __restrict__ target, int64_t ignore, int64_t vocab, int64_t M, int slots,
-                 float sign, float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ entropy) {
+head_rows_kernel(const float2* stats, const float* stats_e, const float* picked,
+                 const int64_t* target, int64_t ignore, int64_t vocab, int64_t M, const int32_t* row_of,
+                 const int32_t* live, int slots,
+                 float sign, float* nll, float* lse, float* entropy) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * 32 + lane;
   __shared__ RowStats s_part[8][32];
   RowStats a = {-INFINITY, 0.0f, 0.0f};
-  if (row < M) {
+  const int64_t rows = live ? load_count(live) : M;
+  if (row < rows) {
     constexpr int kFly = 8;                                // loads in flight
     for (int s0 = warp; s0 < slots; s0 += 8 * kFly) {
       float2 v[kFly];
@@ -647,23 +668,99 @@ head_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ sta
   }
   s_part[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && row < M) {
+  if (warp == 0 && row < rows) {
 #pragma unroll
     for (int w = 1; w < 8; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
     const float all = fmaf(a.m, kLn2, logf(a.s));
-    const int64_t t = target[row];
-    lse[row] = all;
-    nll[row] = t == ignore ? 0.0f : (t < 0 || t >= vocab) ? NAN : sign * (all - picked[row]);
+    const int64_t given = row_of ? row_of[row] : row, t = target[given];
+    lse[given] = all;
+    nll[given] = t == ignore ? 0.0f : (t < 0 || t >= vocab) ? NAN : sign * (all - picked[row]);
     // H = log s - sum p (l - m): p = 2^(l - m) / s, l - m in units of log2
-    if constexpr (kEntropy) entropy[row] = logf(a.s) - kLn2 * (a.e / a.s);
+    if constexpr (kEntropy) entropy[given] = t == ignore ? 0.0f : logf(a.s) - kLn2 * (a.e / a.s);
+  }
+}
+
+// ---- rows that are not ignored -----------------------------------------------------------------------------------
+// A third of the tokens of a training batch and more are prompt or padding.  Where the products behind are long enough (kPackFlops), the
+// others are brought together first: 8192 rows, a third ignored, 151936 x 1536 with gradients 11.6 ms, 8.0 so.
+
+// row_of[i] = the i-th row that is not ignored, place_of[m] = its i or -1, *live = their number; zeros for the losses of the others.  One block,
+// in the order of the rows.
+__global__ void __launch_bounds__(1024)
+head_index_kernel(const int64_t* target, int64_t ignore, int64_t M, int32_t* row_of, int32_t* place_of,
+                  int32_t* live, float* nll, float* entropy) {
+  grid_dependency_wait();
+  __shared__ int s_warp[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = 0;
+  for (int64_t m0 = 0, it = 0; m0 < M; m0 += 1024, ++it) {
+    const int64_t m = m0 + threadIdx.x;
+    const bool on = m < M && target[m] != ignore;
+    const uint32_t mask = __ballot_sync(0xffffffffu, on);
+    int* counts = s_warp[it & 1];
+    if (lane == 0) counts[warp] = __popc(mask);
+    __syncthreads();
+    int total = counts[lane], mine = lane < warp ? total : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    const int place = before + mine + __popc(mask & ((1u << lane) - 1u));
+    if (m < M) {
+      place_of[m] = on ? place : -1;
+      if (on) {
+        row_of[place] = (int32_t)m;
+      } else {
+        if (nll) nll[m] = 0.0f;
+        if (entropy) entropy[m] = 0.0f;
+      }
+    }
+    before += total;
+  }
+  if (threadIdx.x == 0) *live = before;
+}
+
+// packed[i] = h[row_of[i]], and zeros up to the next multiple of 64 (what a stage of the contraction over the rows reads); rows of 16-byte pieces
+__global__ void __launch_bounds__(256)
+head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, const int32_t* row_of, const int32_t* live,
+                   __nv_bfloat16* packed) {
+  grid_dependency_wait();
+  const int64_t n = load_count(live), end = (n + 63) / 64 * 64 < M ? (n + 63) / 64 * 64 : M;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += (int64_t)gridDim.x * 8) {
+    uint4* to = reinterpret_cast<uint4*>(packed) + i * pieces;
+    if (i < n) {
+      const uint4* from = reinterpret_cast<const uint4*>(h + row_of[i] * ldh);
+#pragma unroll 4
+      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = from[k];
+    } else {
+      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
+
+// dh[m] = packed[place_of[m]], zeros for the rows that are ignored
+__global__ void __launch_bounds__(256)
+head_scatter_kernel(const __nv_bfloat16* packed, int64_t M, int pieces, const int32_t* place_of, __nv_bfloat16* dh, int64_t lddh) {
+  grid_dependency_wait();
+  for (int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += (int64_t)gridDim.x * 8) {
+    const int64_t i = place_of[m];
+    uint4* to = reinterpret_cast<uint4*>(dh + m * lddh);
+    if (i >= 0) {
+      const uint4* from = reinterpret_cast<const uint4*>(packed) + i * pieces;
+#pragma unroll 4
+      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = from[k];
+    } else {
+      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = make_uint4(0u, 0u, 0u, 0u);
+    }
   }
 }
 
 // loss = sum of nll, or that over the number of rows that are not ignored; inv_count = 1 / that number (1 for the sum).  One block,
 // fixed order.
 __global__ void __launch_bounds__(1024)
-head_sum_kernel(const float* __restrict__ nll, const int64_t* __restrict__ target, int64_t ignore, int64_t M, int mean,
-                float* __restrict__ loss, float* __restrict__ inv_count) {
+head_sum_kernel(const float* nll, const int64_t* target, int64_t ignore, int64_t M, int mean,
+                float* loss, float* inv_count) {
   grid_dependency_wait();
   __shared__ double s_sum[32];
   __shared__ unsigned long long s_count[32];
@@ -694,15 +791,17 @@ head_sum_kernel(const float* __restrict__ nll, const int64_t* __restrict__ targe
 // lies beside the row in them belongs to the same allocation and is not used.
 template <bool kWide> __device__ __forceinline__ void load8_any(const __nv_bfloat16* at, int64_t left, float (&v)[8]) {
   if constexpr (kWide) {
-    Load8<__nv_bfloat16>::load(at, v);
+    const uint4 w = *reinterpret_cast<const uint4*>(at);
+    v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+    v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
   } else {
     const uintptr_t a = reinterpret_cast<uintptr_t>(at);
     const uint32_t off = (uint32_t)(a & 15);
     const int64_t bytes = 2 * (left < 8 ? left : 8);
     const uint4* p = reinterpret_cast<const uint4*>(a & ~(uintptr_t)15);
-    const uint4 lo = __ldg(p);
+    const uint4 lo = p[0];
     uint4 hi = make_uint4(0u, 0u, 0u, 0u);
-    if (off + bytes > 16) hi = __ldg(p + 1);
+    if (off + bytes > 16) hi = p[1];
     uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
     for (int k = 0; k < 6; ++k) x[k] = (off & 8) ? x[k + 2] : x[k];
@@ -742,10 +841,10 @@ __device__ __forceinline__ void store_run(__nv_bfloat16* run, int count, unsigne
 // rows; kWide: all the others do too, and N is a multiple of 8.  Bound by memory: 8192 x 8960 with gate 126 us, 5.8 TB/s.
 template <int kAct, bool kWide>
 __global__ void __launch_bounds__(256)
-linear_pointwise_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, const __nv_bfloat16* __restrict__ z, int64_t ldz,
-                        const __nv_bfloat16* __restrict__ gate, int64_t ldgate, int64_t M, int64_t N,
-                        __nv_bfloat16* __restrict__ dz, int64_t lddz, __nv_bfloat16* __restrict__ dgate, int64_t lddg,
-                        float* __restrict__ sums) {
+linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* z, int64_t ldz,
+                        const __nv_bfloat16* gate, int64_t ldgate, int64_t M, int64_t N,
+                        __nv_bfloat16* dz, int64_t lddz, __nv_bfloat16* dgate, int64_t lddg,
+                        float* sums) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t col0 = (int64_t)blockIdx.x * 256, col = col0 + lane * 8, left = N - col;
@@ -799,7 +898,7 @@ linear_pointwise_kernel(const __nv_bfloat16* __restrict__ dy, int64_t lddy, cons
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-linear_bias_kernel(const float* __restrict__ sums, int groups, int64_t N, T* __restrict__ out) {
+linear_bias_kernel(const float* sums, int groups, int64_t N, T* out) {
   grid_dependency_wait();
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (c >= N) return;
@@ -861,6 +960,7 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap_enabled(kLaunchGemm) ? 2 : 1;
   METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_z, p));
+  dense_launches.fetch_add(1, std::memory_order_relaxed);
   return METIS_OK;
 }
 
@@ -871,8 +971,9 @@ static int32_t map_bf16(CUtensorMap* map, const void* d, int64_t ld, int64_t M, 
 
 // D (bf16 or fp32) = A B^T + C, gradients: (A K-major, B MN-major) or (both MN-major)
 static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M, int64_t N, int64_t K, const float* c, int64_t ldc,
-                         void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st) {
+                         void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st, const int32_t* live = nullptr) {
   DenseParams p = {};
+  p.live = live; p.live_is_k = a.mn;                       // (rows that are not ignored: the output's, or those a weight's gradient sums over)
   p.M = M; p.N = N; p.K = K; p.status = status; p.c = c; p.ldc = ldc;
   CUtensorMap md = {};
   if (d_f32) {
@@ -912,6 +1013,8 @@ static int64_t piece_columns(int64_t M, int64_t V) {
 }  // namespace metis
 
 using namespace metis;
+
+extern "C" int64_t metis_dense_launches(void) { return dense_launches.load(std::memory_order_relaxed); }
 
 extern "C" int32_t metis_linear(const metis_linear_args* a) {
   if (!a) return fail(METIS_ERR_BAD_ARGUMENT, "args is null");
@@ -958,7 +1061,7 @@ extern "C" int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N) 
 template <int kAct>
 static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool wide, dim3 grid, float* sums) {
   auto launch = [&](auto kern) {
-    return launch_overlapped(kLaunchStream, kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(a->stream),
+    return launch_counted(kLaunchStream, kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(a->stream),
                              static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __nv_bfloat16*>(a->z), a->ldz,
                              static_cast<const __nv_bfloat16*>(a->gate), a->ldgate, a->M, a->N, static_cast<__nv_bfloat16*>(a->dz), a->lddz,
                              static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
@@ -1003,9 +1106,9 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   const dim3 blocks((unsigned)ceil_div(a->N, 256));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
   if (a->dbias_dtype == METIS_DTYPE_BF16)
-    METIS_CUDA_OK(launch_overlapped(kLaunchShort, linear_bias_kernel<__nv_bfloat16>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<__nv_bfloat16*>(a->dbias)));
+    METIS_CUDA_OK(launch_counted(kLaunchShort, linear_bias_kernel<__nv_bfloat16>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<__nv_bfloat16*>(a->dbias)));
   else
-    METIS_CUDA_OK(launch_overlapped(kLaunchShort, linear_bias_kernel<float>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<float*>(a->dbias)));
+    METIS_CUDA_OK(launch_counted(kLaunchShort, linear_bias_kernel<float>, blocks, dim3(256), 0, st, (const float*)sums, (int)groups, a->N, static_cast<float*>(a->dbias)));
   return METIS_OK;
 }
 
@@ -1041,20 +1144,54 @@ static int32_t check_head(const metis_head_args* a) {
   if (!a->target || !a->lse) return fail(METIS_ERR_BAD_ARGUMENT, "target or lse is null");
   return METIS_OK;
 }
-static DenseParams head_params(const metis_head_args* a) {
+constexpr int64_t kFewRows = 64;                           // rows of a head that the weight's read bounds
+static int64_t head_slots(int64_t M, int64_t V) { return M <= kFewRows ? small_stats_slots(V) : 2 * ceil_div(V, 256); }
+
+// Packing the rows that are not ignored takes 6 us and the time of two passes over h, on either side, whether there are any or none; from
+// 10^12 operations of one product on (0.7 ms) that is 1 to 2 % of the call.
+constexpr double kPackFlops = 1e12;
+struct HeadPack {
+  bool on;
+  int32_t *live, *row_of, *place_of;
+  __nv_bfloat16* h;
+  int64_t bytes;
+};
+static HeadPack head_pack(int64_t M, int64_t V, int64_t K, void* at) {
+  HeadPack k = {};
+  k.on = 2.0 * (double)M * (double)V * (double)K >= kPackFlops && M > kFewRows;
+  if (!k.on) return k;
+  const int64_t index = ceil_div(M * 4, 256) * 256;
+  char* b = static_cast<char*>(at);
+  k.live = reinterpret_cast<int32_t*>(b);
+  k.row_of = reinterpret_cast<int32_t*>(b + 256);
+  k.place_of = reinterpret_cast<int32_t*>(b + 256 + index);
+  k.h = reinterpret_cast<__nv_bfloat16*>(b + 256 + 2 * index);
+  k.bytes = 256 + 2 * index + ceil_div(2 * M * K, 256) * 256;
+  return k;
+}
+static DenseParams head_params(const metis_head_args* a, const HeadPack& pack) {
   DenseParams p = {};
+  if (pack.on) { p.row_of = pack.row_of; p.live = pack.live; }
   p.M = a->M; p.N = a->V; p.K = a->K; p.status = a->status;
   p.target = a->target; p.ignore = a->ignore_index; p.vocab = a->V;
   p.weight_scale = a->negate ? -a->scale : a->scale;
   p.scale = a->scale; p.scale_log2e = a->scale * 1.4426950408889634f;
   return p;
 }
-constexpr int64_t kFewRows = 64;                           // rows of a head that the weight's read bounds
-static int64_t head_slots(int64_t M, int64_t V) { return M <= kFewRows ? small_stats_slots(V) : 2 * ceil_div(V, 256); }
+static unsigned row_blocks(int64_t rows) {
+  const int64_t blocks = ceil_div(rows, 8), most = (int64_t)device_sm_count() * 8;
+  return (unsigned)(blocks < most ? blocks : most);
+}
+static int32_t pack_rows(const metis_head_args* a, const HeadPack& k, float* nll, float* entropy, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchShort, head_index_kernel, dim3(1), dim3(1024), 0, st, a->target, a->ignore_index, a->M, k.row_of, k.place_of, k.live, nll, entropy));
+  METIS_CUDA_OK(launch_counted(kLaunchStream, head_gather_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M,
+                                  (int)(a->K / 8), (const int32_t*)k.row_of, (const int32_t*)k.live, k.h));
+  return METIS_OK;
+}
 
 extern "C" int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
-  return ceil_div(M * 4, 16) * 16 + head_slots(M, V) * M * (entropy ? 12 : 8);
+  return head_pack(M, V, K, nullptr).bytes + ceil_div(M * 4, 16) * 16 + head_slots(M, V) * M * (entropy ? 12 : 8);
 }
 
 extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) {
@@ -1063,34 +1200,37 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_loss_workspace_bytes(a->M, a->V, a->K, entropy != nullptr))
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
-  DenseParams p = head_params(a);
+  const HeadPack pack = head_pack(a->M, a->V, a->K, a->workspace);
+  DenseParams p = head_params(a, pack);
   const int64_t slots = head_slots(a->M, a->V);
-  p.picked = static_cast<float*>(a->workspace);
-  p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + ceil_div(a->M * 4, 16) * 16);
+  p.picked = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pack.bytes);
+  p.stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(p.picked) + ceil_div(a->M * 4, 16) * 16);
   p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
-  const DenseOperand h = {a->h, a->ldh, false}, w = {a->w, a->ldw, false};
+  p.stats_ld = a->M;
+  if (pack.on) if (int32_t rc = pack_rows(a, pack, nll, entropy, st)) return rc;
+  const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false}, w = {a->w, a->ldw, false};
   const CUtensorMap none = {};
   if (a->M <= kFewRows) {
     if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
   } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, p, st)) return rc;
   const dim3 blocks((unsigned)ceil_div(a->M, 32));
   auto rows = entropy ? head_rows_kernel<true> : head_rows_kernel<false>;
-  METIS_CUDA_OK(launch_overlapped(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
-                                  a->target, a->ignore_index, a->V, a->M, (int)slots, a->negate ? -1.0f : 1.0f, nll, a->lse, entropy));
+  METIS_CUDA_OK(launch_counted(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
+                                  a->target, a->ignore_index, a->V, a->M, p.row_of, p.live, (int)slots, a->negate ? -1.0f : 1.0f, nll, a->lse, entropy));
   return METIS_OK;
 }
 
 extern "C" int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_index, int64_t M, int32_t mean, float* loss, float* inv_count, void* stream) {
   if (int32_t rc = check_extent(M, "M")) return rc;
   if (!nll || !target || !loss || !inv_count) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
-  METIS_CUDA_OK(launch_overlapped(kLaunchShort, head_sum_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), nll, target, ignore_index, M, (int)(mean != 0), loss, inv_count));
+  METIS_CUDA_OK(launch_counted(kLaunchShort, head_sum_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), nll, target, ignore_index, M, (int)(mean != 0), loss, inv_count));
   return METIS_OK;
 }
 
 extern "C" int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
   const int64_t columns = piece_columns(M, V);
-  return ceil_div(2 * M * columns, 256) * 256 + (columns < V ? 4 * M * K : 0);
+  return head_pack(M, V, K, nullptr).bytes + ceil_div(2 * M * columns, 256) * 256 + (columns < V ? 4 * M * K : 0);
 }
 
 extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* gout, int32_t gout_stride, const float* inv_count,
@@ -1103,11 +1243,14 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_backward_workspace_bytes(a->M, a->V, a->K))
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  const HeadPack pack = head_pack(a->M, a->V, a->K, a->workspace);
   const int64_t columns = piece_columns(a->M, a->V);
-  __nv_bfloat16* g = static_cast<__nv_bfloat16*>(a->workspace);
-  float* acc = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + ceil_div(2 * a->M * columns, 256) * 256);
+  __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(a->workspace) + pack.bytes);
+  float* acc = reinterpret_cast<float*>(reinterpret_cast<char*>(g) + ceil_div(2 * a->M * columns, 256) * 256);
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a->w);
-  DenseParams p = head_params(a);
+  if (pack.on) if (int32_t rc = pack_rows(a, pack, nullptr, nullptr, st)) return rc;
+  const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false};
+  DenseParams p = head_params(a, pack);
   p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride; p.inv_count = inv_count;
   for (int64_t v0 = 0; v0 < a->V; v0 += columns) {
     const int64_t n = a->V - v0 < columns ? a->V - v0 : columns;
@@ -1116,15 +1259,20 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
     p.N = n;
     p.col0 = v0;
     if (int32_t rc = map_bf16(&mg, g, columns, a->M, n, "G")) return rc;
-    if (int32_t rc = launch_dense<false, false, kEpiGrad>({a->h, a->ldh, false}, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
-    if (dh) {
-      if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
-                                 last ? dh : acc, !last, last ? lddh : a->K, a->status, st)) return rc;
-    }
+    if (int32_t rc = launch_dense<false, false, kEpiGrad>(h, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
     if (dw) {
-      if (int32_t rc = dense_sum({g, columns, true}, {a->h, a->ldh, true}, n, a->K, a->M, nullptr, 0,
-                                 static_cast<__nv_bfloat16*>(dw) + v0 * lddw, false, lddw, a->status, st)) return rc;
+      if (int32_t rc = dense_sum({g, columns, true}, {h.p, h.ld, true}, n, a->K, a->M, nullptr, 0,
+                                 static_cast<__nv_bfloat16*>(dw) + v0 * lddw, false, lddw, a->status, st, p.live)) return rc;
+    }
+    if (dh) {
+      // (packed rows: the last piece's product ends in the place of h, which nothing reads any more)
+      void* out = !last ? static_cast<void*>(acc) : pack.on ? static_cast<void*>(pack.h) : dh;
+      if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
+                                 out, !last, last && !pack.on ? lddh : a->K, a->status, st, p.live)) return rc;
     }
   }
+  if (dh && pack.on)
+    METIS_CUDA_OK(launch_counted(kLaunchStream, head_scatter_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, (const __nv_bfloat16*)pack.h, a->M, (int)(a->K / 8),
+                                    (const int32_t*)pack.place_of, static_cast<__nv_bfloat16*>(dh), lddh));
   return METIS_OK;
 }

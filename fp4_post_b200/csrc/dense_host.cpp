@@ -18,7 +18,6 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <atomic>
 #include <string.h>
 
 #include "../../include/metis_nvfp4.h"
@@ -34,8 +33,6 @@ struct Entries {
   METIS_DENSE_ENTRIES(X)
 #undef X
 } lib;
-
-std::atomic<int64_t> launched{0};
 
 struct NoGil {
   PyThreadState* state = PyEval_SaveThread();
@@ -139,7 +136,6 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
   a.z = ptr(out.z); a.ldz = z_pitch;
   a.stream = stream_of(x);
   check(lib.metis_linear(&a), "metis_linear");
-  launched += 1;
   return out;
 }
 
@@ -148,7 +144,6 @@ Tensor product(const Tensor& a, const Rows& ra, bool mn, const Tensor& b, const 
   const int64_t M = mn ? ra.cols : ra.rows, K = mn ? ra.rows : ra.cols;
   const Tensor d = empty_like_options(b, {M, rb.cols}, at::kBFloat16);
   check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, d.data_ptr(), rb.cols, nullptr, stream_of(b)), "metis_bf16_product");
-  launched += 1;
   return d;
 }
 
@@ -231,7 +226,6 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           }
           a.stream = stream_of(dy);
           check(lib.metis_linear_pointwise(&a), "metis_linear_pointwise");
-          launched += need_b ? 2 : 1;
         }
         if (need_x) {
           Rows rw(saved[1]);
@@ -283,13 +277,11 @@ HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, 
   const Tensor ws = scratch(h, lib.metis_head_loss_workspace_bytes(a.M, a.V, a.K, entropy));
   a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
   check(lib.metis_head_loss(&a, ptr<float>(each), ptr<float>(r.entropy)), "metis_head_loss");
-  launched += 2;
   r.out = each;
   if (form == kSum || form == kMean) {
     r.out = empty_like_options(h, {}, at::kFloat);
     r.inv_count = empty_like_options(h, {1}, at::kFloat);
     check(lib.metis_head_sum(ptr<float>(each), a.target, ignore, M, form == kMean, ptr<float>(r.out), ptr<float>(r.inv_count), a.stream), "metis_head_sum");
-    launched += 1;
   }
   return r;
 }
@@ -326,7 +318,6 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
       const Tensor ws = scratch(h, lib.metis_head_backward_workspace_bytes(a.M, a.V, a.K));
       a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
       check(lib.metis_head_backward(&a, ptr<float>(g), each, ptr<float>(saved[4]), ptr(out[0]), a.K, ptr(out[1]), a.K), "metis_head_backward");
-      launched += 1 + need_h + need_w;
     }
     return once(std::move(out));
   }
@@ -426,9 +417,6 @@ PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// kernels launched by these calls so far
-PyObject* launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(launched.load()); }
-
 // name, address: binds an entry point; returns whether this module has a use for it
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 2) {
@@ -446,7 +434,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(linear), METHOD(head), METHOD(launches), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(linear), METHOD(head), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "metis_dense", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

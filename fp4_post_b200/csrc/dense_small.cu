@@ -12,8 +12,6 @@
 #include "dense.cuh"
 #include "pair.cuh"
 
-#include <atomic>
-
 namespace metis {
 
 constexpr int kSmallThreads = 384;                       // loader, issuer, eight that drain tensor memory; the epilogue is everybody's
@@ -76,13 +74,13 @@ __device__ __forceinline__ float load_cluster_f32(uint32_t addr) {
 // of the row are zero.
 __device__ __forceinline__ void load_row8(const __nv_bfloat16* src, bool vec, int apart, int64_t left, uint32_t (&w)[4]) {
   if (vec && left >= 8) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
+    const uint4 q = *reinterpret_cast<const uint4*>(src);
     w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
   } else {
     const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = 2 * i * apart < left ? __ldg(s + 2 * i * apart) : 0, hi = (2 * i + 1) * apart < left ? __ldg(s + (2 * i + 1) * apart) : 0;
+      const uint32_t lo = 2 * i * apart < left ? s[2 * i * apart] : 0, hi = (2 * i + 1) * apart < left ? s[(2 * i + 1) * apart] : 0;
       w[i] = lo | (hi << 16);
     }
   }
@@ -261,7 +259,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int64_t c = n + i * apart;
-          if (i * apart < left) v[i] += p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + c) : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + c));
+          if (i * apart < left) v[i] += p.bias_f32 ? static_cast<const float*>(p.bias)[c] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[c]);
         }
       }
       if (p.z) store_row8(p.z + m * p.ldz + n, wide, apart, left, v);
@@ -387,7 +385,7 @@ dense_small_stats_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     const int64_t token = m0 + c0 + lane;                  // lane l looks after the target of token l
     int64_t target = -1;
     if (token < p.M && c0 < sh.bn) {
-      const int64_t t = __ldg(p.target + token);
+      const int64_t t = p.target[token];
       if (t != p.ignore && t >= 0 && t < p.vocab) target = t;
     }
     float m[32], s[32], e[32];
@@ -441,7 +439,7 @@ dense_small_stats_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
       }
     }
     if (token < p.M && c0 < sh.bn) {
-      const int64_t slot = ((int64_t)blockIdx.x * 4 + q) * p.M + token;
+      const int64_t slot = ((int64_t)blockIdx.x * 4 + q) * p.stats_ld + token;
       p.stats[slot] = make_float2(a[0].m, a[0].s);
       if constexpr (kEntropy) p.stats_e[slot] = a[0].e;
     }
@@ -566,6 +564,7 @@ int32_t launch_dense_small(const SmallShape& sh, const void* t, int64_t ldt, con
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, mw, mt, p, sh));
+  dense_launches.fetch_add(1, std::memory_order_relaxed);
   return METIS_OK;
 }
 
@@ -590,7 +589,7 @@ int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int6
   auto kern = p.stats_e ? (wide ? dense_small_stats_kernel<true, 8> : dense_small_stats_kernel<true, 4>)
                         : (wide ? dense_small_stats_kernel<false, 8> : dense_small_stats_kernel<false, 4>);
   METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  METIS_CUDA_OK(launch_overlapped(kLaunchGemm, kern, dim3((unsigned)(small_stats_slots(p.N) / 4)), dim3(wide ? 320 : 192), (size_t)smem, st, mw, mt, p, sh));
+  METIS_CUDA_OK(launch_counted(kLaunchGemm, kern, dim3((unsigned)(small_stats_slots(p.N) / 4)), dim3(wide ? 320 : 192), (size_t)smem, st, mw, mt, p, sh));
   return METIS_OK;
 }
 

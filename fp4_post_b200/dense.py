@@ -128,6 +128,6 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor
                    ignore_index: int = -100):
     """log softmax(hidden @ weight.T / temperature) at the given token ids, fp32, shaped like ids; 0 where ids is ignore_index.
 
-    With entropy=True also the entropy of each row's distribution (ignored rows included), which carries no gradient."""
+    With entropy=True also the entropy of each row's distribution (0 likewise), which carries no gradient."""
     out = _head(hidden, weight, ids, ignore_index, temperature, _LOGPROBS, entropy)
     return out if entropy else out[0]

@@ -450,6 +450,9 @@ int32_t metis_silu_mul(const void* gate, const void* up, void* out, int64_t n, v
 
 /* ---- products that stay in bf16: linear layer with its epilogue -------------------------------------------- */
 
+/* Kernels that the entry points below have launched in this process. */
+int64_t metis_dense_launches(void);
+
 /*
  * y = act(x W^T + bias) * gate + residual, x [M, K], W [N, K], y [M, N], all bf16, sums in fp32, one rounding at the end.
  * bias (bf16 or fp32 [N]), gate and residual ([M, N]) may be null; z, where given, receives bf16(x W^T + bias), from which
@@ -504,7 +507,8 @@ int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const
 /*
  * l = scale * h W^T [M, V] with h [M, K] and W [V, K] in bf16; l is formed tile by tile in fp32 and not stored.
  * metis_head_loss: lse[m] = log sum_j exp l[m][j]; nll[m] = lse[m] - l[m][target[m]], 0 where target[m] = ignore_index, NaN
- * where it is no other index of the vocabulary; entropy (optional) = lse - sum_j p l.  h and w as x and w of metis_linear.
+ * where it is no other index of the vocabulary; entropy (optional) = lse - sum_j p l, 0 where target[m] = ignore_index.  h and w as x and w of metis_linear.
+ * lse of ignored rows is not set.
  */
 typedef struct metis_head_args {
   int64_t M, V, K;

@@ -171,7 +171,7 @@ def head64(h, w, t, temperature, ignore_index=-100):
     logp = torch.log_softmax(logits, dim=1)
     live = t != ignore_index
     picked = logp.gather(1, torch.where(live, t, 0)[:, None])[:, 0]
-    return torch.where(live, picked, 0.0), -(logp.exp() * logp).sum(dim=1), logits
+    return torch.where(live, picked, 0.0), torch.where(live, -(logp.exp() * logp).sum(dim=1), 0.0), logits
 
 
 def head_inputs(M, V, K, ignored=0.2, seed=0, size=2.0):
@@ -249,6 +249,49 @@ def test_gradients_over_several_pieces_of_the_vocabulary(monkeypatch):
     exact = torch.autograd.grad(-logp.sum(), (h64, w64))
     for a, e in zip(got, exact):
         assert rel(a, e) <= 2 * STEP
+
+
+@pytest.mark.parametrize("ignored", [0.0, 0.4, 1.0])
+def test_rows_that_are_brought_together(ignored):
+    # a product of 10^12 operations: the rows that are not ignored are packed before it
+    M, V, K = 4129, 131100, 1024
+    h, w, t = head_inputs(M, V, K, ignored)
+    if ignored == 1.0:
+        t[:] = -100
+    live = t != -100
+    h[~live] = float("nan")
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    logp, ent = dense.token_logprobs(h, w, t, entropy=True, temperature=1.5)
+    g = normal(M, seed=9, dtype=torch.float32)
+    dh, dw = torch.autograd.grad(logp, (h, w), g)
+    assert not logp[~live].any() and not ent[~live].any() and not dh[~live].any()
+    loss = dense.linear_cross_entropy(h, w, t)
+    dh2, dw2 = torch.autograd.grad(loss, (h, w))
+    if ignored == 1.0:
+        assert not dw.any() and torch.isnan(loss) and not dh2.any() and not dw2.any()
+        return
+    h64, w64 = h[live].detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    want, want_ent, logits = head64(h64, w64, t[live], 1.5)
+    with torch.no_grad():
+        tol = (K * 2.0 ** -23 * (h64[:64].abs() @ w64.abs().t()).max() / 1.5 + 2.0 ** -20 * (1 + logits.abs().max())).item()
+    assert (logp[live].double() - want).abs().max() <= 2 * tol
+    assert (ent[live].double() - want_ent).abs().max() <= (2 + 2 * math.log(V)) * tol
+    exact = torch.autograd.grad(want, (h64, w64), g[live].double())
+    check_head_gradients((dh[live], dw), exact, h64, w64, logits.detach(), g[live], t[live], 1.5, tol)
+    want = torch.nn.functional.cross_entropy(h64 @ w64.t(), t[live])
+    assert abs(float(loss.detach()) - float(want.detach())) <= 2 * tol
+    exact = torch.autograd.grad(want, (h64, w64))
+    assert rel(dh2[live], exact[0]) <= 2 * STEP and rel(dw2, exact[1]) <= 2 * STEP
+
+
+def test_launches_are_counted():
+    from fp4_post_b200 import ops
+    h, w, t = head_inputs(100, 500, 64)
+    before = ops.launch_count()
+    dense.token_logprobs(h, w, t)
+    dense.linear(h, w)
+    assert ops.launch_count() - before == 3
 
 
 def test_rows_that_are_ignored():
