@@ -30,7 +30,7 @@ struct DenseParams {
   float weight_scale;                                      // scale, with the sign of the loss
   float2* stats;                                           // [slots, stats_ld]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum)
   float* stats_e;                                          // [slots, stats_ld]: sum of 2^(..) (l log2(e) - maximum), or null
-  float* picked;                                           // [M]: logit of the target
+  float* picked;                                           // [M]: logit of the target times log2(e), as the statistics have it
   const float* lse;                                        // [M]
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss: gout[row * stride] times *inv_count (null: 1)
   const float* inv_count;

@@ -558,7 +558,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
             if (here) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (at == i) picked = __uint_as_float(v[i]) * p.scale;
+              for (int i = 0; i < 32; ++i) if (at == i) picked = __uint_as_float(v[i]) * p.scale_log2e;
               found = true;
             }
           }
@@ -633,50 +633,127 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 
 // ---- statistics of the pieces into losses ---------------------------------------------------------------------
 
-// nll, lse and entropy of each row from the statistics of its `slots` pieces (slots of a row lie M apart: neighbouring threads read
-// neighbouring rows).  A block takes 32 rows; its eight warps take the slots in turn and are merged in a fixed order.
-template <bool kEntropy>
+// nll, lse and entropy of each row from the statistics of its `slots` pieces (slots of a row lie M apart).  The tensor core cuts what it adds
+// up to instead of rounding it (16 products of a row at a time: 2e-6 of a logit at K = 3584), which shows in the target's logit, the largest
+// of its row if the model knows anything.  So that one is formed again in fp32, and takes its place in the row's sums as well: log-probabilities
+// of 16 rows of 3584 are 2.9e-7 from 64 bits instead of 2.2e-6.
+//   kRows = 32  a block takes 32 rows: its eight warps take the slots in turn, neighbouring lanes neighbouring rows
+//   kRows = 1   few rows: a block takes one, its threads the slots
+struct HeadRows {
+  const float2* stats;  const float* stats_e;  const float* picked;
+  const __nv_bfloat16* h;  int64_t ldh;                    // rows as the statistics have them (packed or not)
+  const __nv_bfloat16* w;  int64_t ldw;
+  const int64_t* target;  int64_t ignore, vocab, M;
+  const int32_t* row_of;  const int32_t* live;
+  int32_t pieces, slots;                                   // 16-byte pieces of a row of h; slots
+  float scale, scale_log2e, sign;
+  float* nll;  float* lse;  float* entropy;
+};
+
+__device__ __forceinline__ float dot8(uint4 a, uint4 b, float c) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = fmaf(bf16_hi(x[i]), bf16_hi(y[i]), fmaf(bf16_lo(x[i]), bf16_lo(y[i]), c));
+  return c;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <bool kEntropy, int kRows>
 __global__ void __launch_bounds__(256)
-head_rows_kernel(const float2* stats, const float* stats_e, const float* picked,
-                 const int64_t* target, int64_t ignore, int64_t vocab, int64_t M, const int32_t* row_of,
-                 const int32_t* live, int slots,
-                 float sign, float* nll, float* lse, float* entropy) {
+head_rows_kernel(const HeadRows p) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
   __shared__ RowStats s_part[8][32];
+  __shared__ float s_dot[32];
+  const int64_t rows = p.live ? load_count(p.live) : p.M, row0 = (int64_t)blockIdx.x * kRows;
+  if (row0 >= rows) return;
+  // the row's target, or -1 where none is to be looked up
+  auto target_of = [&](int64_t row) {
+    const int64_t t = p.target[p.row_of ? p.row_of[row] : row];
+    return t != p.ignore && t >= 0 && t < p.vocab ? t : (int64_t)-1;
+  };
+  constexpr int kDots = kRows == 32 ? 4 : 1;               // rows of a warp, side by side
+  float dot[kDots];
+  const uint4 *hp[kDots], *wp[kDots];
+#pragma unroll
+  for (int i = 0; i < kDots; ++i) {
+    const int64_t row = kRows == 32 ? row0 + warp * 4 + i : row0, t = row < rows ? target_of(row) : -1;
+    dot[i] = 0.0f;
+    hp[i] = reinterpret_cast<const uint4*>(p.h + (t < 0 ? 0 : row) * p.ldh);
+    wp[i] = reinterpret_cast<const uint4*>(p.w + (t < 0 ? 0 : t) * p.ldw);
+  }
+#pragma unroll 2
+  for (int k = kRows == 32 ? lane : (int)threadIdx.x; k < p.pieces; k += kRows == 32 ? 32 : 256) {
+#pragma unroll
+    for (int i = 0; i < kDots; ++i) dot[i] = dot8(hp[i][k], wp[i][k], dot[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kDots; ++i) {
+    dot[i] = warp_sum(dot[i]);
+    if (lane == 0) s_dot[warp * kDots + i] = dot[i];
+  }
+
   RowStats a = {-INFINITY, 0.0f, 0.0f};
-  const int64_t rows = live ? load_count(live) : M;
+  const int64_t row = kRows == 32 ? row0 + lane : row0;
   if (row < rows) {
-    constexpr int kFly = 8;                                // loads in flight
-    for (int s0 = warp; s0 < slots; s0 += 8 * kFly) {
+    constexpr int kFly = 8, kStep = kRows == 32 ? 8 : 256;  // loads in flight
+    for (int s0 = kRows == 32 ? warp : (int)threadIdx.x; s0 < p.slots; s0 += kStep * kFly) {
       float2 v[kFly];
       float e[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
-        const int s = s0 + 8 * i;
+        const int s = s0 + kStep * i;
         v[i] = make_float2(-INFINITY, 0.0f);
         e[i] = 0.0f;
-        if (s < slots) {
-          v[i] = stats[(int64_t)s * M + row];
-          if constexpr (kEntropy) e[i] = stats_e[(int64_t)s * M + row];
+        if (s < p.slots) {
+          v[i] = p.stats[(int64_t)s * p.M + row];
+          if constexpr (kEntropy) e[i] = p.stats_e[(int64_t)s * p.M + row];
         }
       }
 #pragma unroll
       for (int i = 0; i < kFly; ++i) stats_merge<kEntropy>(a, RowStats{v[i].x, v[i].y, e[i]});
     }
   }
+  if constexpr (kRows == 1) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      RowStats b;
+      b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+      b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+      b.e = kEntropy ? __shfl_xor_sync(0xffffffffu, a.e, o) : 0.0f;
+      if (lane & o) { const RowStats t = a; a = b; b = t; }            // the same order on both sides
+      stats_merge<kEntropy>(a, b);
+    }
+  }
   s_part[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && row < rows) {
+  if (warp == 0 && row < rows && (kRows == 32 || lane == 0)) {
 #pragma unroll
     for (int w = 1; w < 8; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
+    const int64_t given = p.row_of ? p.row_of[row] : row, t = p.target[given];
+    const bool ignored = t == p.ignore, inside = t >= 0 && t < p.vocab;
+    float logit = 0.0f;
+    if (!ignored && inside) {
+      if constexpr (kRows == 32) {
+        logit = s_dot[lane];
+      } else {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) logit += s_dot[w];
+      }
+      const float base = stats_base(a.m), was = fmaxf(p.picked[row] - base, -1e30f), is = fmaxf(logit * p.scale_log2e - base, -1e30f);
+      const float xw = exp2_fast(was), xi = exp2_fast(is);
+      a.s += xi - xw;
+      if constexpr (kEntropy) a.e += fmaf(xi, is, -xw * was);
+    }
     const float all = fmaf(a.m, kLn2, logf(a.s));
-    const int64_t given = row_of ? row_of[row] : row, t = target[given];
-    lse[given] = all;
-    nll[given] = t == ignore ? 0.0f : (t < 0 || t >= vocab) ? NAN : sign * (all - picked[row]);
+    p.lse[given] = all;
+    p.nll[given] = ignored ? 0.0f : !inside ? NAN : p.sign * (all - logit * p.scale);
     // H = log s - sum p (l - m): p = 2^(l - m) / s, l - m in units of log2
-    if constexpr (kEntropy) entropy[given] = t == ignore ? 0.0f : logf(a.s) - kLn2 * (a.e / a.s);
+    if constexpr (kEntropy) p.entropy[given] = ignored ? 0.0f : logf(a.s) - kLn2 * (a.e / a.s);
   }
 }
 
@@ -1213,10 +1290,16 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   if (a->M <= kFewRows) {
     if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
   } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, p, st)) return rc;
-  const dim3 blocks((unsigned)ceil_div(a->M, 32));
-  auto rows = entropy ? head_rows_kernel<true> : head_rows_kernel<false>;
-  METIS_CUDA_OK(launch_counted(kLaunchShort, rows, blocks, dim3(256), 0, st, (const float2*)p.stats, (const float*)p.stats_e, (const float*)p.picked,
-                                  a->target, a->ignore_index, a->V, a->M, p.row_of, p.live, (int)slots, a->negate ? -1.0f : 1.0f, nll, a->lse, entropy));
+  HeadRows r = {};
+  r.stats = p.stats; r.stats_e = p.stats_e; r.picked = p.picked;
+  r.h = static_cast<const __nv_bfloat16*>(h.p); r.ldh = h.ld; r.w = static_cast<const __nv_bfloat16*>(a->w); r.ldw = a->ldw;
+  r.target = a->target; r.ignore = a->ignore_index; r.vocab = a->V; r.M = a->M; r.row_of = p.row_of; r.live = p.live;
+  r.pieces = (int32_t)(a->K / 8); r.slots = (int32_t)slots;
+  r.scale = p.scale; r.scale_log2e = p.scale_log2e; r.sign = a->negate ? -1.0f : 1.0f;
+  r.nll = nll; r.lse = a->lse; r.entropy = entropy;
+  const bool few = a->M <= kFewRows;
+  auto rows = few ? (entropy ? head_rows_kernel<true, 1> : head_rows_kernel<false, 1>) : (entropy ? head_rows_kernel<true, 32> : head_rows_kernel<false, 32>);
+  METIS_CUDA_OK(launch_counted(kLaunchShort, rows, dim3((unsigned)ceil_div(a->M, few ? 1 : 32)), dim3(256), 0, st, r));
   return METIS_OK;
 }
 

@@ -418,7 +418,7 @@ dense_small_stats_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         float l = 0.0f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) if (i == who) l = __uint_as_float(r[i]);
-        if (lane == at) p.picked[m0 + c0 + who] = l * p.scale;
+        if (lane == at) p.picked[m0 + c0 + who] = l * p.scale_log2e;
       }
     }
     // lanes into one: after five steps lane l has the statistics of token l, half of the tokens leaving at each
