@@ -44,7 +44,7 @@ EXPORTS = (
     "metis_bf16_panel_gemm_workspace_bytes", "metis_bf16_panel_gemm",
     "metis_lowrank_dts_workspace_bytes", "metis_lowrank_dts", "metis_lowrank_dts_mean", "metis_lowrank_du_workspace_bytes", "metis_lowrank_du",
     "metis_rope_pair", "metis_silu_mul",
-    "metis_dense_launches", "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product",
+    "metis_dense_launches", "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product_workspace_bytes", "metis_bf16_product",
     "metis_head_loss_workspace_bytes", "metis_head_loss", "metis_head_sum", "metis_head_backward_workspace_bytes", "metis_head_backward",
 )
 
@@ -194,7 +194,9 @@ def lib() -> C.CDLL:
     L.metis_linear_pointwise_workspace_bytes.restype = i64
     L.metis_linear_pointwise.argtypes = [C.POINTER(LinearPointwiseArgs)]
     L.metis_linear_pointwise.restype = i32
-    L.metis_bf16_product.argtypes = [vp, i32, i64, vp, i64, i64, i64, i64, vp, i64, vp, vp]
+    L.metis_bf16_product_workspace_bytes.argtypes = [i64, i64, i64, i32]
+    L.metis_bf16_product_workspace_bytes.restype = i64
+    L.metis_bf16_product.argtypes = [vp, i32, i64, vp, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp]
     L.metis_bf16_product.restype = i32
     L.metis_head_loss_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.metis_head_loss_workspace_bytes.restype = i64

@@ -34,11 +34,25 @@ struct DenseParams {
   const float* lse;                                        // [M]
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss: gout[row * stride] times *inv_count (null: 1)
   const float* inv_count;
-  // sum of pieces: fp32 addend
+  // sum of pieces: fp32 addend.  With `splits` > 1 each split of the contraction has sums of its own, [splits, split_rows, N]
   const float* c;  int64_t ldc;
+  int32_t splits, iters_per_split;
+  int64_t split_rows;
 };
 
 extern std::atomic<int64_t> dense_launches;                // kernels launched by the entry points of these two files
+
+// Lets a kernel take `bytes` of shared memory, asked once for each device (`done`: a bit for each that has it).
+static inline cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // Products of few tokens (dense_small.cu).
 struct SmallShape {
@@ -147,6 +161,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 w = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&w);
 }
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) { return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])); }
 
 // Running softmax statistics of one row: m, the maximum of the logits seen (times log2 e), s, the sum of 2^(l - m), and e, the
 // sum of 2^(l - m) (l - m).  m starts at -infinity; base() replaces it there, so that no difference of two infinities is formed.

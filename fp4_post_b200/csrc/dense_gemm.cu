@@ -363,8 +363,10 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   }
   const int64_t tiles_m = (M + 255) / 256;
   const int64_t tiles_n = (p.N + BN - 1) / BN;
-  const int64_t num_tiles = tiles_m * tiles_n;
-  const int iters = (int)((K + 63) / 64);                // 0 where no row is left: the sums are zeros
+  const int iters_all = (int)((K + 63) / 64);              // 0 where no row is left: the sums are zeros
+  // a unit of work: a tile, or one split of the contraction of a tile (all tiles of a split, then the next: units that run together share operands)
+  constexpr bool kSplit = kEpi == kEpiSumF32;
+  const int64_t tiles = tiles_m * tiles_n, num_tiles = kSplit ? tiles * p.splits : tiles;
 
   if (warp == 0) {
     // ===== TMA producer (both CTAs): every copy reports to the leader's barrier =====
@@ -376,7 +378,9 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const uint32_t full_leader = map_to_cta(full_local, 0);
     for (int64_t tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       int64_t tm, tn;
-      tile_coords(tile, tiles_m, tiles_n, p.band, tm, tn);
+      const int split = kSplit ? (int)(tile / tiles) : 0, it0 = kSplit ? split * p.iters_per_split : 0;
+      const int iters = kSplit && iters_all - it0 > p.iters_per_split ? p.iters_per_split : iters_all - it0;
+      tile_coords(kSplit ? tile - split * tiles : tile, tiles_m, tiles_n, p.band, tm, tn);
       const int32_t m0 = (int32_t)(tm * 256 + cta * 128);             // this CTA's rows of A
       const int32_t n0 = (int32_t)(tn * BN + cta * 128);              // this CTA's rows of B
       for (int it = 0; it < iters; ++it) {
@@ -388,7 +392,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
         const uint32_t sb = sa + Cfg::kHalfBytes;
         const uint32_t bar = full_leader + stage * 8;
-        const int32_t k0 = it * 64;
+        const int32_t k0 = (it0 + it) * 64;
         if (elect_one()) {
           if (cta == 0) mbar_expect_tx_addr(full_local + stage * 8, 2 * Cfg::kStageBytes);
           if (kAMn) {
@@ -410,7 +414,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     grid_launch_dependents();                                // the last loads of this CTA are on their way: let the next kernel's CTAs in
   } else if (warp == 1) {
     // ===== tensor-core issuer (leader only) =====
-    if (cta == 0 && iters > 0) {
+    if (cta == 0 && iters_all > 0) {
       int stage = 0;
       uint32_t phase = 0, local_tile = 0;
       bool ok = true, issued = false;
@@ -431,6 +435,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           }
         }
         tc_fence_after();
+        const int it0 = kSplit ? (int)(tile / tiles) * p.iters_per_split : 0;
+        const int iters = kSplit && iters_all - it0 > p.iters_per_split ? p.iters_per_split : iters_all - it0;
         const uint32_t d_tmem = tmem_base + buf * BN;
         for (int it = 0; it < iters; ++it) {
           ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[stage], phase, abort_flag));
@@ -481,7 +487,9 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     uint32_t local_tile = 0;
     for (int64_t tile = pair; tile < num_tiles; tile += num_pairs, ++local_tile) {
       int64_t tm, tn;
-      tile_coords(tile, tiles_m, tiles_n, p.band, tm, tn);
+      const int64_t split = kSplit ? tile / tiles : 0;
+      tile_coords(kSplit ? tile - split * tiles : tile, tiles_m, tiles_n, p.band, tm, tn);
+      const int64_t out0 = kSplit ? split * p.split_rows : 0;              // this split's first row of the sums
       const uint32_t buf = local_tile & 1u;
       const int64_t row0 = tm * 256 + cta * 128 + q * 32;
       const int64_t row = row0 + lane;
@@ -513,7 +521,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         }
         ahead.valid = false;
       }
-      const bool sums = iters > 0;
+      const bool sums = iters_all > 0;
       if (sums && !mbar_wait_cluster(&acc_full[buf], (local_tile >> 1) & 1u, abort_flag)) {
         if (lane == 0) report(p.status, abort_flag, METIS_DEV_TIMEOUT_MMA);
         break;
@@ -581,7 +589,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(v[i]);
             if (p.c && row < M) {
-              const float* c = p.c + row * p.ldc + col0;
+              const float* c = p.c + (out0 + row) * p.ldc + col0;
               if (col0 + 32 <= p.N) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -603,7 +611,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
               for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(g[16 * h + i]);
-                store_piece_tma(st, &map_d, w, (int32_t)col0 + 16 * h, (int32_t)row0);
+                store_piece_tma(st, &map_d, w, (int32_t)col0 + 16 * h, (int32_t)(out0 + row0));
               }
             }
           }
@@ -637,8 +645,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 // up to instead of rounding it (16 products of a row at a time: 2e-6 of a logit at K = 3584), which shows in the target's logit, the largest
 // of its row if the model knows anything.  So that one is formed again in fp32, and takes its place in the row's sums as well: log-probabilities
 // of 16 rows of 3584 are 2.9e-7 from 64 bits instead of 2.2e-6.
-//   kRows = 32  a block takes 32 rows: its eight warps take the slots in turn, neighbouring lanes neighbouring rows
-//   kRows = 1   few rows: a block takes one, its threads the slots
+//   kRows = 32  a block of 32 warps takes 32 rows: its warps take the slots in turn, neighbouring lanes neighbouring rows
+//   kRows = 1   few rows: a block of 8 warps takes one, its threads the slots
 struct HeadRows {
   const float2* stats;  const float* stats_e;  const float* picked;
   const __nv_bfloat16* h;  int64_t ldh;                    // rows as the statistics have them (packed or not)
@@ -663,11 +671,12 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 template <bool kEntropy, int kRows>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRows == 32 ? 1024 : 256)
 head_rows_kernel(const HeadRows p) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __shared__ RowStats s_part[8][32];
+  constexpr int kWarps = kRows == 32 ? 32 : 8;
+  __shared__ RowStats s_part[kWarps][32];
   __shared__ float s_dot[32];
   const int64_t rows = p.live ? load_count(p.live) : p.M, row0 = (int64_t)blockIdx.x * kRows;
   if (row0 >= rows) return;
@@ -676,31 +685,23 @@ head_rows_kernel(const HeadRows p) {
     const int64_t t = p.target[p.row_of ? p.row_of[row] : row];
     return t != p.ignore && t >= 0 && t < p.vocab ? t : (int64_t)-1;
   };
-  constexpr int kDots = kRows == 32 ? 4 : 1;               // rows of a warp, side by side
-  float dot[kDots];
-  const uint4 *hp[kDots], *wp[kDots];
-#pragma unroll
-  for (int i = 0; i < kDots; ++i) {
-    const int64_t row = kRows == 32 ? row0 + warp * 4 + i : row0, t = row < rows ? target_of(row) : -1;
-    dot[i] = 0.0f;
-    hp[i] = reinterpret_cast<const uint4*>(p.h + (t < 0 ? 0 : row) * p.ldh);
-    wp[i] = reinterpret_cast<const uint4*>(p.w + (t < 0 ? 0 : t) * p.ldw);
-  }
-#pragma unroll 2
-  for (int k = kRows == 32 ? lane : (int)threadIdx.x; k < p.pieces; k += kRows == 32 ? 32 : 256) {
-#pragma unroll
-    for (int i = 0; i < kDots; ++i) dot[i] = dot8(hp[i][k], wp[i][k], dot[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < kDots; ++i) {
-    dot[i] = warp_sum(dot[i]);
-    if (lane == 0) s_dot[warp * kDots + i] = dot[i];
+  // a warp has a row, or a part of the block's
+  {
+    const int64_t row = kRows == 32 ? row0 + warp : row0, t = row < rows ? target_of(row) : -1;
+    float dot = 0.0f;
+    if (t >= 0) {
+      const uint4 *hp = reinterpret_cast<const uint4*>(p.h + row * p.ldh), *wp = reinterpret_cast<const uint4*>(p.w + t * p.ldw);
+#pragma unroll 4
+      for (int k = kRows == 32 ? lane : (int)threadIdx.x; k < p.pieces; k += kRows == 32 ? 32 : 256) dot = dot8(hp[k], wp[k], dot);
+    }
+    dot = warp_sum(dot);
+    if (lane == 0) s_dot[warp] = dot;
   }
 
   RowStats a = {-INFINITY, 0.0f, 0.0f};
   const int64_t row = kRows == 32 ? row0 + lane : row0;
   if (row < rows) {
-    constexpr int kFly = 8, kStep = kRows == 32 ? 8 : 256;  // loads in flight
+    constexpr int kFly = 8, kStep = kRows == 32 ? kWarps : 256;         // loads in flight
     for (int s0 = kRows == 32 ? warp : (int)threadIdx.x; s0 < p.slots; s0 += kStep * kFly) {
       float2 v[kFly];
       float e[kFly];
@@ -732,8 +733,7 @@ head_rows_kernel(const HeadRows p) {
   s_part[warp][lane] = a;
   __syncthreads();
   if (warp == 0 && row < rows && (kRows == 32 || lane == 0)) {
-#pragma unroll
-    for (int w = 1; w < 8; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
+    for (int w = 1; w < kWarps; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
     const int64_t given = p.row_of ? p.row_of[row] : row, t = p.target[given];
     const bool ignored = t == p.ignore, inside = t >= 0 && t < p.vocab;
     float logit = 0.0f;
@@ -816,20 +816,25 @@ head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, c
   }
 }
 
-// dh[m] = packed[place_of[m]], zeros for the rows that are ignored
+// d[m] = the sum over the splits of row place_of[m] of the sums (m itself where there is no place_of), in bf16; zeros for a place of -1.  A thread takes eight
+// columns of a row.
 __global__ void __launch_bounds__(256)
-head_scatter_kernel(const __nv_bfloat16* packed, int64_t M, int pieces, const int32_t* place_of, __nv_bfloat16* dh, int64_t lddh) {
+finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M, int pieces, const int32_t* place_of, __nv_bfloat16* d, int64_t ldd) {
   grid_dependency_wait();
-  for (int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += (int64_t)gridDim.x * 8) {
-    const int64_t i = place_of[m];
-    uint4* to = reinterpret_cast<uint4*>(dh + m * lddh);
+  const int64_t ld = 8 * (int64_t)pieces, total = M * pieces;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+    const int64_t m = e / pieces, k = e - m * pieces, i = place_of ? place_of[m] : m;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (i >= 0) {
-      const uint4* from = reinterpret_cast<const uint4*>(packed) + i * pieces;
 #pragma unroll 4
-      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = from[k];
-    } else {
-      for (int k = threadIdx.x & 31; k < pieces; k += 32) to[k] = make_uint4(0u, 0u, 0u, 0u);
+      for (int s = 0; s < splits; ++s) {
+        const float4* at = reinterpret_cast<const float4*>(sums + (s * split_rows + i) * ld + 8 * k);
+        const float4 x = at[0], y = at[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
     }
+    reinterpret_cast<uint4*>(d + m * ldd)[k] = pack8(v);
   }
 }
 
@@ -892,7 +897,6 @@ template <bool kWide> __device__ __forceinline__ void load8_any(const __nv_bfloa
     }
   }
 }
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) { return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])); }
 // The eight elements of every lane, 256 together, to a run of `count` elements at any address: through the warp's buffer, laid out there as the
 // run lies to 16 bytes, so that all but its two ends leave as whole 16 bytes.
 __device__ __forceinline__ void store_run(__nv_bfloat16* run, int count, unsigned short* buf, const float (&v)[8]) {
@@ -1000,6 +1004,12 @@ static int32_t check_extent(int64_t n, const char* what) {
   return METIS_OK;
 }
 
+// blocks of eight warps for so many warps' work
+static unsigned row_blocks(int64_t warps) {
+  const int64_t blocks = ceil_div(warps, 8), most = (int64_t)device_sm_count() * 8;
+  return (unsigned)(blocks < most ? blocks : most);
+}
+
 struct DenseOperand {
   const void* p;
   int64_t ld;
@@ -1016,12 +1026,15 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   if (kBMn) { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.N, p.K, b.ld * 2, 64, 64, "B (MN-major)")) return rc; }
   else      { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.K, p.N, b.ld * 2, 64, 128, "B (K-major)")) return rc; }
   p.band = 8;
-  const int64_t tiles = ceil_div(p.M, 256) * ceil_div(p.N, 256);
+  if (p.splits < 1) p.splits = 1;
+  if (p.splits == 1) p.iters_per_split = INT32_MAX;
+  const int64_t tiles = ceil_div(p.M, 256) * ceil_div(p.N, 256) * p.splits;
   int64_t pairs = device_sm_count() / 2;
   if (pairs > tiles) pairs = tiles;
-  pairs = ceil_div(tiles, ceil_div(tiles, pairs));         // the fewest that finish in the same number of rounds
+  if (!p.live) pairs = ceil_div(tiles, ceil_div(tiles, pairs));        // the fewest that finish in the same number of rounds
   auto kern = dense_gemm_pair_kernel<kAMn, kBMn, kEpi>;
-  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
+  static std::atomic<uint64_t> done{0};
+  METIS_CUDA_OK(allow_shared(reinterpret_cast<const void*>(kern), Cfg::kSmemBytes, done));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
   cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
@@ -1046,19 +1059,47 @@ static int32_t map_bf16(CUtensorMap* map, const void* d, int64_t ld, int64_t M, 
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, d, N, M, ld * 2, 32, 32, what, 64);
 }
 
-// D (bf16 or fp32) = A B^T + C, gradients: (A K-major, B MN-major) or (both MN-major)
-static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M, int64_t N, int64_t K, const float* c, int64_t ldc,
-                         void* d, bool d_f32, int64_t ldd, int32_t* status, cudaStream_t st, const int32_t* live = nullptr) {
+// D = A B^T for gradients: (A K-major, B MN-major), or (both MN-major).  In bf16; or `sums`, fp32 [splits, split_rows, N] with split_rows = M in
+// whole tiles, added to what they hold where `add` is set, and finish_sums behind them.
+struct Splits {
+  int32_t splits, iters_per_split;
+  int64_t rows, bytes;                                     // of the sums
+};
+static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M, int64_t N, int64_t K, void* d, int64_t ldd, int32_t* status, cudaStream_t st,
+                         const int32_t* live = nullptr, const Splits* sp = nullptr, float* sums = nullptr, bool add = false) {
   DenseParams p = {};
   p.live = live; p.live_is_k = a.mn;                       // (rows that are not ignored: the output's, or those a weight's gradient sums over)
-  p.M = M; p.N = N; p.K = K; p.status = status; p.c = c; p.ldc = ldc;
+  p.M = M; p.N = N; p.K = K; p.status = status;
   CUtensorMap md = {};
-  if (d_f32) {
-    if (int32_t rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, d, N, M, ldd * 4, 16, 32, "D", 64)) return rc;
+  if (sums) {
+    p.splits = sp->splits; p.iters_per_split = sp->iters_per_split; p.split_rows = sp->rows;
+    p.c = add ? sums : nullptr; p.ldc = N;
+    if (int32_t rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, sums, N, sp->splits * sp->rows, N * 4, 16, 32, "sums", 64)) return rc;
     return a.mn ? launch_dense<true, true, kEpiSumF32>(a, b, md, p, st) : launch_dense<false, true, kEpiSumF32>(a, b, md, p, st);
   }
   if (int32_t rc = map_bf16(&md, d, ldd, M, N, "D")) return rc;
   return a.mn ? launch_dense<true, true, kEpiSum>(a, b, md, p, st) : launch_dense<false, true, kEpiSum>(a, b, md, p, st);
+}
+
+// Splits of the contraction: what fills the rounds of pairs, weighed against the sums' way through memory (0.29 us for a stage of a round, 5
+// TB/s; fewer than 8 stages to a split are not worth its start).  Loss's input gradient, us, one / so many: 1021 x 1000 over 32003 224 / 69 (4),
+// 2048 x 1536 over 75968 374 / 268 (3).
+static Splits plan_splits(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256), iters = ceil_div(K, 64), pairs = device_sm_count() > 1 ? device_sm_count() / 2 : 74;
+  Splits best = {1, (int32_t)iters, ceil_div(M, 256) * 256, 0};
+  float best_us = 0.29f * (float)(ceil_div(tiles, pairs) * iters) * 0.95f;
+  for (int s = 2; s <= 16; ++s) {
+    const int64_t per = ceil_div(iters, s);
+    if (per < 8 || ceil_div(iters, per) != s) continue;
+    const float us = 0.29f * (float)(ceil_div(tiles * s, pairs) * per) + 5.0f + (float)(8 * s * best.rows * N) / 5e6f;
+    if (us < best_us) {
+      best_us = us;
+      best.splits = s;
+      best.iters_per_split = (int32_t)per;
+    }
+  }
+  best.bytes = best.splits * best.rows * N * 4;
+  return best;
 }
 
 // Whether a product goes to the kernel for few tokens, with the shape it takes there: by a model of both.  A round of 256 x 256 tiles takes
@@ -1068,8 +1109,9 @@ static bool few_tokens(int64_t M, int64_t N, int64_t K, bool w_mn, SmallShape* s
   if (M > 2048) return false;
   const SmallPlan plan = plan_dense_small(M, N, K, w_mn);
   *sh = plan.sh;
-  const int64_t pairs = device_sm_count() / 2, rounds = ceil_div(ceil_div(M, 256) * ceil_div(N, 256), pairs > 0 ? pairs : 1);
-  const float tiles_us = 0.29f * (float)(rounds * ceil_div(K, 64)), memory_us = (float)(2 * N * K) / 5.5e6f;
+  const int64_t pairs = device_sm_count() > 1 ? device_sm_count() / 2 : 1, tiles = ceil_div(M, 256) * ceil_div(N, 256), rounds = ceil_div(tiles, pairs);
+  const float busy = tiles < pairs ? (float)tiles / (float)pairs : 1.0f;             // (the weight comes to the pairs that have a tile)
+  const float tiles_us = 0.29f * (float)(rounds * ceil_div(K, 64)), memory_us = (float)(2 * N * K) / (5.5e6f * busy);
   const float pair_us = 7.5f + (tiles_us > memory_us ? tiles_us : memory_us);
 #ifdef METIS_TIMING_KNOBS
   if (const char* e = getenv("METIS_DEV_DENSE_SMALL")) return atoi(e) != 0;
@@ -1189,14 +1231,28 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   return METIS_OK;
 }
 
+static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64_t N, const int32_t* place_of, __nv_bfloat16* d, int64_t ldd, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchStream, finish_sums_kernel, dim3(row_blocks(ceil_div(M * N, 256))), dim3(256), 0, st, sums, (int)sp.splits, sp.rows, M, (int)(N / 8), place_of, d, ldd));
+  return METIS_OK;
+}
+
+extern "C" int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  SmallShape sh;
+  if (!a_mn_major && few_tokens(M, N, K, true, &sh)) return 0;
+  const Splits sp = plan_splits(M, N, K);
+  return sp.splits > 1 ? sp.bytes : 0;
+}
+
 extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
-                                      void* d, int64_t ldd, int32_t* status, void* stream) {
+                                      void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   if (int32_t rc = check_extent(M, "M")) return rc;
   if (int32_t rc = check_extent(N, "N")) return rc;
   if (int32_t rc = check_extent(K, "K")) return rc;
   if (int32_t rc = check_rows(a, lda, a_mn_major ? M : K, "a")) return rc;
   if (int32_t rc = check_rows(b, ldb, N, "b")) return rc;
   if (int32_t rc = check_rows(d, ldd, N, "d")) return rc;
+  if (N % 8 != 0) return fail(METIS_ERR_BAD_SHAPE, "N = %lld must be a multiple of 8", (long long)N);
   SmallShape sh;
   if (!a_mn_major && few_tokens(M, N, K, true, &sh)) {
     DenseParams p = {};
@@ -1204,7 +1260,14 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
     p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_wide = 1;
     return launch_dense_small(sh, a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
   }
-  return dense_sum({a, lda, a_mn_major != 0}, {b, ldb, true}, M, N, K, nullptr, 0, d, false, ldd, status, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const Splits sp = plan_splits(M, N, K);
+  const DenseOperand oa = {a, lda, a_mn_major != 0}, ob = {b, ldb, true};
+  if (sp.splits == 1) return dense_sum(oa, ob, M, N, K, d, ldd, status, st);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < sp.bytes) return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
+  float* sums = static_cast<float*>(workspace);
+  if (int32_t rc = dense_sum(oa, ob, M, N, K, nullptr, 0, status, st, nullptr, &sp, sums)) return rc;
+  return finish_sums(sums, sp, M, N, nullptr, static_cast<__nv_bfloat16*>(d), ldd, st);
 }
 
 // ---- head ---------------------------------------------------------------------------------------------------------
@@ -1255,10 +1318,6 @@ static DenseParams head_params(const metis_head_args* a, const HeadPack& pack) {
   p.scale = a->scale; p.scale_log2e = a->scale * 1.4426950408889634f;
   return p;
 }
-static unsigned row_blocks(int64_t rows) {
-  const int64_t blocks = ceil_div(rows, 8), most = (int64_t)device_sm_count() * 8;
-  return (unsigned)(blocks < most ? blocks : most);
-}
 static int32_t pack_rows(const metis_head_args* a, const HeadPack& k, float* nll, float* entropy, cudaStream_t st) {
   METIS_CUDA_OK(launch_counted(kLaunchShort, head_index_kernel, dim3(1), dim3(1024), 0, st, a->target, a->ignore_index, a->M, k.row_of, k.place_of, k.live, nll, entropy));
   METIS_CUDA_OK(launch_counted(kLaunchStream, head_gather_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M,
@@ -1299,7 +1358,7 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   r.nll = nll; r.lse = a->lse; r.entropy = entropy;
   const bool few = a->M <= kFewRows;
   auto rows = few ? (entropy ? head_rows_kernel<true, 1> : head_rows_kernel<false, 1>) : (entropy ? head_rows_kernel<true, 32> : head_rows_kernel<false, 32>);
-  METIS_CUDA_OK(launch_counted(kLaunchShort, rows, dim3((unsigned)ceil_div(a->M, few ? 1 : 32)), dim3(256), 0, st, r));
+  METIS_CUDA_OK(launch_counted(kLaunchShort, rows, dim3((unsigned)ceil_div(a->M, few ? 1 : 32)), dim3(few ? 256 : 1024), 0, st, r));
   return METIS_OK;
 }
 
@@ -1310,10 +1369,32 @@ extern "C" int32_t metis_head_sum(const float* nll, const int64_t* target, int64
   return METIS_OK;
 }
 
+// What the backward pass keeps: packed rows, the gradients G of a piece's logits, and the sums of dh over pieces and splits (none where one
+// product makes it in its place).
+struct HeadBackward {
+  HeadPack pack;
+  int64_t columns;
+  Splits sp;
+  __nv_bfloat16* g;
+  float* sums;
+  int64_t bytes;
+};
+static HeadBackward plan_head_backward(int64_t M, int64_t V, int64_t K, void* at) {
+  HeadBackward b = {};
+  b.pack = head_pack(M, V, K, at);
+  b.columns = piece_columns(M, V);
+  b.sp = plan_splits(M, K, b.columns < V ? b.columns : V);
+  const bool summed = b.pack.on || b.columns < V || b.sp.splits > 1;
+  const int64_t g_bytes = ceil_div(2 * M * b.columns, 256) * 256;
+  b.g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(at) + b.pack.bytes);
+  b.sums = summed ? reinterpret_cast<float*>(reinterpret_cast<char*>(b.g) + g_bytes) : nullptr;
+  b.bytes = b.pack.bytes + g_bytes + (summed ? b.sp.bytes : 0);
+  return b;
+}
+
 extern "C" int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
-  const int64_t columns = piece_columns(M, V);
-  return head_pack(M, V, K, nullptr).bytes + ceil_div(2 * M * columns, 256) * 256 + (columns < V ? 4 * M * K : 0);
+  return plan_head_backward(M, V, K, nullptr).bytes;
 }
 
 extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* gout, int32_t gout_stride, const float* inv_count,
@@ -1326,36 +1407,31 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_backward_workspace_bytes(a->M, a->V, a->K))
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
-  const HeadPack pack = head_pack(a->M, a->V, a->K, a->workspace);
-  const int64_t columns = piece_columns(a->M, a->V);
-  __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(a->workspace) + pack.bytes);
-  float* acc = reinterpret_cast<float*>(reinterpret_cast<char*>(g) + ceil_div(2 * a->M * columns, 256) * 256);
+  const HeadBackward b = plan_head_backward(a->M, a->V, a->K, a->workspace);
+  const HeadPack& pack = b.pack;
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a->w);
   if (pack.on) if (int32_t rc = pack_rows(a, pack, nullptr, nullptr, st)) return rc;
   const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false};
   DenseParams p = head_params(a, pack);
   p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride; p.inv_count = inv_count;
-  for (int64_t v0 = 0; v0 < a->V; v0 += columns) {
-    const int64_t n = a->V - v0 < columns ? a->V - v0 : columns;
-    const bool last = v0 + n == a->V;
+  for (int64_t v0 = 0; v0 < a->V; v0 += b.columns) {
+    const int64_t n = a->V - v0 < b.columns ? a->V - v0 : b.columns;
     CUtensorMap mg = {};
     p.N = n;
     p.col0 = v0;
-    if (int32_t rc = map_bf16(&mg, g, columns, a->M, n, "G")) return rc;
+    if (int32_t rc = map_bf16(&mg, b.g, b.columns, a->M, n, "G")) return rc;
     if (int32_t rc = launch_dense<false, false, kEpiGrad>(h, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
     if (dw) {
-      if (int32_t rc = dense_sum({g, columns, true}, {h.p, h.ld, true}, n, a->K, a->M, nullptr, 0,
-                                 static_cast<__nv_bfloat16*>(dw) + v0 * lddw, false, lddw, a->status, st, p.live)) return rc;
+      if (int32_t rc = dense_sum({b.g, b.columns, true}, {h.p, h.ld, true}, n, a->K, a->M, static_cast<__nv_bfloat16*>(dw) + v0 * lddw, lddw, a->status, st, p.live)) return rc;
     }
     if (dh) {
-      // (packed rows: the last piece's product ends in the place of h, which nothing reads any more)
-      void* out = !last ? static_cast<void*>(acc) : pack.on ? static_cast<void*>(pack.h) : dh;
-      if (int32_t rc = dense_sum({g, columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, v0 ? acc : nullptr, a->K,
-                                 out, !last, last && !pack.on ? lddh : a->K, a->status, st, p.live)) return rc;
+      // a shorter last piece has no more splits than the others; those that it leaves out keep what they hold
+      const int64_t stages = ceil_div(n, 64);
+      Splits sp = b.sp;
+      sp.splits = (int32_t)ceil_div(stages, sp.iters_per_split);
+      if (int32_t rc = dense_sum({b.g, b.columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, b.sums ? nullptr : dh, lddh, a->status, st, p.live, &sp, b.sums, v0 > 0)) return rc;
     }
   }
-  if (dh && pack.on)
-    METIS_CUDA_OK(launch_counted(kLaunchStream, head_scatter_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, (const __nv_bfloat16*)pack.h, a->M, (int)(a->K / 8),
-                                    (const int32_t*)pack.place_of, static_cast<__nv_bfloat16*>(dh), lddh));
+  if (dh && b.sums) return finish_sums(b.sums, b.sp, a->M, a->K, pack.on ? pack.place_of : nullptr, static_cast<__nv_bfloat16*>(dh), lddh, st);
   return METIS_OK;
 }

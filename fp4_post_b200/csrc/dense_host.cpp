@@ -26,7 +26,7 @@ namespace {
 
 #define METIS_DENSE_ENTRIES(X)                                                                                             \
   X(metis_last_error_string) X(metis_linear) X(metis_linear_pointwise) X(metis_linear_pointwise_workspace_bytes)          \
-  X(metis_bf16_product) X(metis_head_loss) X(metis_head_loss_workspace_bytes) X(metis_head_sum) X(metis_head_backward)    \
+  X(metis_bf16_product) X(metis_bf16_product_workspace_bytes) X(metis_head_loss) X(metis_head_loss_workspace_bytes) X(metis_head_sum) X(metis_head_backward)    \
   X(metis_head_backward_workspace_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -143,7 +143,9 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
 Tensor product(const Tensor& a, const Rows& ra, bool mn, const Tensor& b, const Rows& rb) {
   const int64_t M = mn ? ra.cols : ra.rows, K = mn ? ra.rows : ra.cols;
   const Tensor d = empty_like_options(b, {M, rb.cols}, at::kBFloat16);
-  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, d.data_ptr(), rb.cols, nullptr, stream_of(b)), "metis_bf16_product");
+  const int64_t bytes = lib.metis_bf16_product_workspace_bytes(M, rb.cols, K, mn);
+  const Tensor ws = bytes > 0 ? scratch(b, bytes) : Tensor();
+  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, d.data_ptr(), rb.cols, ptr(ws), bytes, nullptr, stream_of(b)), "metis_bf16_product");
   return d;
 }
 

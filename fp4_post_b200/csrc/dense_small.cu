@@ -16,7 +16,7 @@ namespace metis {
 
 constexpr int kSmallThreads = 384;                       // loader, issuer, eight that drain tensor memory; the epilogue is everybody's
 // Shared memory of a CTA: two fit an SM, so that clusters of any size find room; one where all CTAs run at once and leave none idle.
-constexpr int kSmallBudget = 100 * 1024, kSmallBudgetAlone = 200 * 1024;
+constexpr int kSmallBudget = 100 * 1024, kSmallBudgetAlone = 200 * 1024, kStatsBudget = 200 * 1024;
 
 // Barriers, tensor memory and the abort flag behind the pipeline's stages.
 struct SmallBars {
@@ -479,22 +479,21 @@ static int resident_clusters(int splits, int which, const void* kern, int smem) 
   return n;
 }
 
-// Shape of a product, and its time in us by the model that chooses it.  A stage takes an SM 0.25 us at least (the round through its two
-// barriers), its bytes come at 108 GB/s an SM and 10 TB/s over all of them, the weight from memory at 5.5 TB/s; around that 4.2 us, 13 ns
-// for each token of a tile and 0.15 ns for each element (drain and epilogue), where a cluster meets 1.5 us and 10 ns a
-// token more, and 4 us for every further round of CTAs.  Measured against the model, us, by rows of a
-// tile, blocks to a stage, splits: 1 x 3584 x 18944 26.4 (128, 2, 4), 27.8 (64, 4, 4), 81 (32, 1, 1); 64 x 3584 x 18944 30.1 (128, 2, 4), 34.0
-// (128, 1, 5); 256 x 3584 x 3584 21.1 (128, 1, 4), 30.2 (32, 1, 1); 256 x 1536 x 1536 14.0 (64, 1, 4), 16.2 (64, 1, 2); 1 x 18944 x 3584 24.5
-// (128, 2, 1), 25.3 (64, 4, 1).
+// Shape of a product, and its time in us by the model that chooses it.  A block's two copies take an SM 0.23 us at least, however small; its
+// bytes come at 108 GB/s an SM and 10 TB/s over all of them, the weight from memory at 5.5 TB/s.  Around that 4.2 us, 13 ns for each token of a
+// tile and 0.15 ns for each element (drain and epilogue), 1.5 us and 10 ns a token more where a cluster meets, and 4 us for every further
+// round of CTAs.  Measured, us, by rows of a tile, blocks to a stage, splits: 1 x 3584 x 18944 26.4 (128, 2, 4), 27.8 (64, 4, 4), 35 (128, 1, 3),
+// 47 (32, 4, 1); 64 x 3584 x 18944 30.1 (128, 2, 4), 34.0 (128, 1, 5); 256 x 3584 x 3584 21.1 (128, 1, 4), 30.2 (32, 1, 1); 256 x 1536 x 1536
+// 14.0 (64, 1, 4), 16.2 (64, 1, 2); 1 x 18944 x 3584 24.5 (128, 2, 1), 25.3 (64, 4, 1).
 SmallPlan plan_dense_small(int64_t M, int64_t N, int64_t K, bool w_mn) {
   SmallPlan best = {};
-  best.us = 1e30f;
+  float best_rank = 1e30f;
   const int64_t blocks = ceil_div(K, 64), sms = device_sm_count();
   const int64_t token_tiles = ceil_div(M, 256);
   const int bn = (int)(ceil_div(ceil_div(M, token_tiles), 16) * 16);
   const void* kern = w_mn ? reinterpret_cast<const void*>(dense_small_kernel<true>) : reinterpret_cast<const void*>(dense_small_kernel<false>);
   const float memory_us = (float)(2 * N * K) / 5.5e6f;
-  for (int alone = 0; alone < 2; ++alone) {
+  for (int alone = 1; alone >= 0; --alone) {               // (deeper pipelines first, where the model sees no difference)
     const int budget = alone ? kSmallBudgetAlone : kSmallBudget;
     for (int rows = 128; rows >= (w_mn ? 64 : 32); rows >>= 1) {
       const int block_bytes = (rows + bn) * 128;
@@ -511,12 +510,15 @@ SmallPlan plan_dense_small(int64_t M, int64_t N, int64_t K, bool w_mn) {
         const int64_t rounds = ceil_div(clusters, at_once), ctas = (clusters < at_once ? clusters : at_once) * splits;
         const float sharing = ctas > sms ? (float)ctas / (float)sms : 1.0f;
         float block_us = sharing * (float)block_bytes / 108e3f;
-        const float all_us = (float)block_bytes * (float)ctas / 10e6f, trip_us = 0.25f / (float)kb;
+        const float all_us = (float)block_bytes * (float)ctas / 10e6f, trip_us = 0.23f;
         if (block_us < all_us) block_us = all_us;
         if (block_us < trip_us) block_us = trip_us;
         const float feed_us = (float)(rounds * per) * block_us;
-        const float us = (feed_us > memory_us ? feed_us : memory_us) + 4.0f * (float)(rounds - 1) + 4.2f + 0.013f * (float)bn + 0.00015f * (float)(rows * bn) + (splits > 1 ? 1.5f + 0.01f * (float)bn : 0.0f);
-        if (us < best.us) {
+        const float rest = 4.0f * (float)(rounds - 1) + 4.2f + 0.013f * (float)bn + 0.00015f * (float)(rows * bn) + (splits > 1 ? 1.5f + 0.01f * (float)bn : 0.0f);
+        const bool bound = feed_us < memory_us;            // by memory: of such shapes the one that feeds faster
+        const float us = (bound ? memory_us : feed_us) + rest, rank = us + 0.3f * (bound ? feed_us : memory_us);
+        if (rank < best_rank) {
+          best_rank = rank;
           best.us = us;
           best.sh = SmallShape{rows, bn, kb, stages, stage_bytes, splits, (int)per};
         }
@@ -548,7 +550,8 @@ int32_t launch_dense_small(const SmallShape& sh, const void* t, int64_t ldt, con
   const int pipe = sh.stages * sh.stage_bytes + (128 - sh.rows) * 128, sums = sh.bn * 512;
   const int smem = 2048 + (pipe > sums ? pipe : sums);
   auto kern = w_mn ? dense_small_kernel<true> : dense_small_kernel<false>;
-  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done[2];
+  METIS_CUDA_OK(allow_shared(reinterpret_cast<const void*>(kern), kSmallBudgetAlone, done[w_mn]));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ceil_div(p.N, sh.rows) * sh.splits), (unsigned)ceil_div(p.M, sh.bn), 1);
   cfg.blockDim = dim3(kSmallThreads, 1, 1);
@@ -579,7 +582,7 @@ int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int6
   sh.rows = 128;
   sh.bn = (int)(ceil_div(p.M, 16) * 16);
   sh.stage_bytes = (sh.rows + sh.bn) * 128;
-  sh.stages = 200 * 1024 / sh.stage_bytes;
+  sh.stages = kStatsBudget / sh.stage_bytes;
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mt, mw;
   if (int32_t rc = make_map(&mt, dt, 2, h, p.K, p.M, ldh * 2, 64, sh.bn, "h")) return rc;
@@ -588,7 +591,8 @@ int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int6
   const bool wide = sh.bn > 32;
   auto kern = p.stats_e ? (wide ? dense_small_stats_kernel<true, 8> : dense_small_stats_kernel<true, 4>)
                         : (wide ? dense_small_stats_kernel<false, 8> : dense_small_stats_kernel<false, 4>);
-  METIS_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done[4];
+  METIS_CUDA_OK(allow_shared(reinterpret_cast<const void*>(kern), 2048 + kStatsBudget, done[2 * wide + (p.stats_e != nullptr)]));
   METIS_CUDA_OK(launch_counted(kLaunchGemm, kern, dim3((unsigned)(small_stats_slots(p.N) / 4)), dim3(wide ? 320 : 192), (size_t)smem, st, mw, mt, p, sh));
   return METIS_OK;
 }

@@ -497,10 +497,12 @@ int32_t metis_linear_pointwise(const metis_linear_pointwise_args* args);
 
 /*
  * D [M, N] = A B^T in bf16, sums in fp32: b is [K, N], a is [M, K] (a_mn_major = 0: an input's gradient, dz W) or [K, M]
- * (1: a weight's, dz^T x).  All three have 16-byte aligned rows.
+ * (1: a weight's, dz^T x).  All three have 16-byte aligned rows, N is a multiple of 8.  A product of few tiles is split along K:
+ * its workspace holds the splits' sums in fp32, added in a fixed order.
  */
+int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major);
 int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
-                           int64_t K, void* d, int64_t ldd, int32_t* status, void* stream);
+                           int64_t K, void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- head: losses over the vocabulary without the logits ----------------------------------------------------- */
 
@@ -531,7 +533,7 @@ int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_i
 /*
  * dh [M, K] = G W and dw [V, K] = G^T h (bf16, either may be null) with G[m][j] = scale * g_m (softmax(l)[m][j] - [j = target[m]]),
  * g_m = gout[m * gout_stride] * (inv_count ? *inv_count : 1), 0 where target[m] = ignore_index.  The logits are formed
- * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, dh's sum over the pieces in fp32.
+ * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, dh's sums in fp32.
  */
 int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K);
 int32_t metis_head_backward(const metis_head_args* args, const float* gout, int32_t gout_stride, const float* inv_count,

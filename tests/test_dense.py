@@ -63,10 +63,12 @@ def test_pointwise_refuses(L, p):
 
 
 def test_product_refuses(L, p):
-    call = lambda a=p, mn=0, lda=16, b=p, ldb=24, M=4, N=24, K=16, d=p, ldd=24: L.metis_bf16_product(a, mn, lda, b, ldb, M, N, K, d, ldd, None, None)
+    call = lambda a=p, mn=0, lda=16, b=p, ldb=24, M=4, N=24, K=16, d=p, ldd=24: L.metis_bf16_product(a, mn, lda, b, ldb, M, N, K, d, ldd, None, 0, None, None)
     assert call(M=0) == -2 and call(K=0) == -2 and call(N=1 << 31) == -7
     assert call(a=None) == -1 and call(b=None) == -1 and call(d=None) == -1
     assert call(lda=8) == -3 and call(ldb=20) == -3 and call(ldd=12) == -3 and call(a=p + 4) == -3 and call(mn=1, lda=2) == -3
+    assert call(N=23) == -2                                                           # rows of whole 16-byte pieces
+    assert call(M=2100, K=100000, lda=100000) == -4 and L.metis_bf16_product_workspace_bytes(2100, 24, 100000, 0) > 0      # split: no workspace
 
 
 def test_head_refuses(L, p):
