@@ -670,7 +670,7 @@ def run_decoder_step(args):
         cfg = type(cfg)(**{**cfg.__dict__, "layers": args.layers})          # a shallower stack for quick runs
     torch.manual_seed(0)
     with torch.device(dev):
-        model = Decoder(cfg, fuse_norms=not args.no_fused_norm).to(torch.bfloat16)
+        model = Decoder(cfg, fuse_norms=not args.no_fused_norm, fuse_dense=args.fuse_dense).to(torch.bfloat16)
     margs = MetisArgs(forward_svd_rank=r, activation_lowrank_svd=r, backward_lowrank_svd=r)
     margs.device = dev
     exact_svd = torch.linalg.svd
@@ -753,7 +753,8 @@ def run_decoder_step(args):
                           "tokens_per_s": tokens / ms * 1e3, "metis_linear_tflops": lin / ms / 1e9,
                           "share_of_device_time_in_library_kernels": share, "device_ms_of_one_eager_step": round(total / 1e3, 1),
                           "top_kernels_of_one_eager_step": top_kernels, "launch_mode": mode,
-                          "fused_norms": not args.no_fused_norm, "data": "synthetic token ids, random weights"}), flush=True)
+                          "fused_norms": not args.no_fused_norm, "fused_dense": args.fuse_dense,
+                          "peak_memory_gb": round(torch.cuda.max_memory_allocated() / 1e9, 1), "data": "synthetic token ids, random weights"}), flush=True)
     if world > 1:
         if isinstance(runner, GraphedStep):
             runner.release()
@@ -819,6 +820,7 @@ def main():
                     help="stack this many Metis layers (the headline is 1): with several GPUs the gradient all-reduce "
                          "of layer k then runs beside the backward of layer k-1")
     ap.add_argument("--no-graph", action="store_true", help="decoder steps: issue from Python instead of one CUDA graph")
+    ap.add_argument("--fuse-dense", action="store_true", help="decoder steps: the head's loss without its logits (dense.py) instead of lm_head and torch's cross entropy")
     ap.add_argument("--no-fused-norm", action="store_true", help="decoder steps: plain RMSNorm modules instead of the fused norm -> quantizer entry")
     ap.add_argument("--rows", type=int, default=16384)
     ap.add_argument("--cols", type=int, default=4096)

@@ -12,6 +12,10 @@ is not a model zoo.
 With `fuse_norms=True` the two RMSNorms of a block hand their output to the projection group that
 follows already quantized (RMSNorm.forward_quantized): one pass over the hidden state computes the
 normalised tensor and its column mean, the next quantizes it for all projections of the group.
+
+With `fuse_dense=True` what stays in bf16 runs on dense.py: the loss and `token_logprobs` take the head without its logits in
+memory, and a projection that is no Metis layer (target_modules of replace_linear_with_metis leaves it out) has its activation, the
+product with `up` and the residual in its own kernel.
 """
 from __future__ import annotations
 
@@ -22,7 +26,7 @@ import torch.nn.functional as Fn
 from torch import nn
 from torch.autograd import forward_ad
 
-from fp4_post_b200 import ops
+from fp4_post_b200 import dense, ops
 from fp4_post_b200.Metis.Metis.bitlinear import forward_group
 from fp4_post_b200.Metis.models.llama import RMSNorm
 
@@ -75,16 +79,34 @@ def _table_of(t: torch.Tensor, T: int, D: int) -> bool:
     return t.dim() >= 2 and t.shape[-2:] == (T, D) and t.numel() == T * D
 
 
+def _dense_weight(weight: torch.Tensor, *tensors) -> bool:
+    """Whether dense.py takes this weight with these tensors: bf16 on one CUDA device, an inner size that 8 divides."""
+    return weight.shape[1] % 8 == 0 and all(t.is_cuda and t.dtype == torch.bfloat16 and t.device == weight.device for t in (weight, *tensors))
+
+
+def _project(module: nn.Module, x: torch.Tensor, fuse: bool, *, activation=None, gate=None, residual=None):
+    """activation(module(x)) * gate + residual, in one kernel where the module is a plain linear layer in bf16."""
+    if fuse and type(module) is nn.Linear and _dense_weight(module.weight, x, *(t for t in (gate, residual, module.bias) if t is not None)):
+        return dense.linear(x, module.weight, module.bias, activation=activation, gate=gate, residual=residual)
+    y = module(x)
+    if activation == "silu":
+        y = Fn.silu(y)
+    if gate is not None:
+        y = y * gate
+    return y if residual is None else residual + y
+
+
 class Attention(nn.Module):
-    def __init__(self, cfg: DecoderConfig):
+    def __init__(self, cfg: DecoderConfig, fuse_dense: bool = False):
         super().__init__()
         self.cfg = cfg
+        self.fuse_dense = fuse_dense
         self.q_proj = nn.Linear(cfg.hidden, cfg.heads * cfg.head_dim, bias=cfg.qkv_bias)
         self.k_proj = nn.Linear(cfg.hidden, cfg.kv_heads * cfg.head_dim, bias=cfg.qkv_bias)
         self.v_proj = nn.Linear(cfg.hidden, cfg.kv_heads * cfg.head_dim, bias=cfg.qkv_bias)
         self.o_proj = nn.Linear(cfg.heads * cfg.head_dim, cfg.hidden, bias=False)
 
-    def forward(self, h, cos, sin):
+    def forward(self, h, cos, sin, residual=None):
         B, T, _ = h.shape
         c = self.cfg
         q, k, v = forward_group((self.q_proj, self.k_proj, self.v_proj), h)     # one shared activation, three branches
@@ -96,31 +118,37 @@ class Attention(nn.Module):
         else:
             q, k = _rope(q.transpose(1, 2), cos, sin), _rope(k.transpose(1, 2), cos, sin)
         a = Fn.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        return self.o_proj(a.transpose(1, 2).reshape(B, T, c.heads * c.head_dim))
+        return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, c.heads * c.head_dim), self.fuse_dense, residual=residual)
 
 
 class MLP(nn.Module):
-    def __init__(self, cfg: DecoderConfig):
+    def __init__(self, cfg: DecoderConfig, fuse_dense: bool = False):
         super().__init__()
+        self.fuse_dense = fuse_dense
         self.gate_proj = nn.Linear(cfg.hidden, cfg.ffn, bias=False)
         self.up_proj = nn.Linear(cfg.hidden, cfg.ffn, bias=False)
         self.down_proj = nn.Linear(cfg.ffn, cfg.hidden, bias=False)
 
-    def forward(self, h):
-        gate, up = forward_group((self.gate_proj, self.up_proj), h)
-        if gate.shape == up.shape and gate.numel() % 8 == 0 and _native(gate, up):
-            return self.down_proj(ops.silu_mul(gate, up))
-        return self.down_proj(Fn.silu(gate) * up)
+    def forward(self, h, residual=None):
+        if self.fuse_dense and type(self.gate_proj) is nn.Linear:
+            act = _project(self.gate_proj, h, True, activation="silu", gate=self.up_proj(h))
+        else:
+            gate, up = forward_group((self.gate_proj, self.up_proj), h)
+            if gate.shape == up.shape and gate.numel() % 8 == 0 and _native(gate, up):
+                act = ops.silu_mul(gate, up)
+            else:
+                act = Fn.silu(gate) * up
+        return _project(self.down_proj, act, self.fuse_dense, residual=residual)
 
 
 class Block(nn.Module):
-    def __init__(self, cfg: DecoderConfig, fuse_norms: bool):
+    def __init__(self, cfg: DecoderConfig, fuse_norms: bool, fuse_dense: bool = False):
         super().__init__()
         self.fuse_norms = fuse_norms
         self.input_layernorm = RMSNorm(cfg.hidden, cfg.eps)
-        self.self_attn = Attention(cfg)
+        self.self_attn = Attention(cfg, fuse_dense)
         self.post_attention_layernorm = RMSNorm(cfg.hidden, cfg.eps)
-        self.mlp = MLP(cfg)
+        self.mlp = MLP(cfg, fuse_dense)
 
     def _normed(self, norm, x, first_of_group):
         group = getattr(first_of_group, "activation_group", None)
@@ -129,16 +157,17 @@ class Block(nn.Module):
         return norm(x)
 
     def forward(self, x, cos, sin):
-        x = x + self.self_attn(self._normed(self.input_layernorm, x, self.self_attn.q_proj), cos, sin)
-        return x + self.mlp(self._normed(self.post_attention_layernorm, x, self.mlp.gate_proj))
+        x = self.self_attn(self._normed(self.input_layernorm, x, self.self_attn.q_proj), cos, sin, x)
+        return self.mlp(self._normed(self.post_attention_layernorm, x, self.mlp.gate_proj), x)
 
 
 class Decoder(nn.Module):
-    def __init__(self, cfg: DecoderConfig, fuse_norms: bool = True):
+    def __init__(self, cfg: DecoderConfig, fuse_norms: bool = True, fuse_dense: bool = False):
         super().__init__()
         self.cfg = cfg
+        self.fuse_dense = fuse_dense
         self.embed_tokens = nn.Embedding(cfg.vocab, cfg.hidden)
-        self.layers = nn.ModuleList(Block(cfg, fuse_norms) for _ in range(cfg.layers))
+        self.layers = nn.ModuleList(Block(cfg, fuse_norms, fuse_dense) for _ in range(cfg.layers))
         self.norm = RMSNorm(cfg.hidden, cfg.eps)
         self.lm_head = nn.Linear(cfg.hidden, cfg.vocab, bias=False)      # stays bf16: not in the reference's target list
 
@@ -149,14 +178,37 @@ class Decoder(nn.Module):
         ang = torch.cat((ang, ang), dim=-1)
         return ang.cos().to(dtype)[None, None], ang.sin().to(dtype)[None, None]
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+    def hidden(self, ids: torch.Tensor) -> torch.Tensor:
+        """What the head reads: the normalised hidden states [B, T, hidden]."""
         x = self.embed_tokens(ids)
         cos, sin = self.rotary(ids.shape[1], ids.device, x.dtype)
         for blk in self.layers:
             x = blk(x, cos, sin)
-        return self.lm_head(self.norm(x))
+        return self.norm(x)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return self.lm_head(self.hidden(ids))
+
+    def _fused_head(self, hidden: torch.Tensor) -> bool:
+        return self.fuse_dense and type(self.lm_head) is nn.Linear and _dense_weight(self.lm_head.weight, hidden)
 
     def loss(self, ids: torch.Tensor) -> torch.Tensor:
         """Next-token cross entropy on the given ids."""
-        logits = self.forward(ids)
+        hidden = self.hidden(ids)
+        if self._fused_head(hidden):
+            target = Fn.pad(ids[:, 1:], (0, 1), value=-100)                  # the last position of a row has no next token
+            return dense.linear_cross_entropy(hidden, self.lm_head.weight, target)
+        logits = self.lm_head(hidden)
         return Fn.cross_entropy(logits[:, :-1].reshape(-1, logits.shape[-1]).float(), ids[:, 1:].reshape(-1))
+
+    def token_logprobs(self, ids: torch.Tensor, temperature: float = 1.0, entropy: bool = False):
+        """Log-probabilities of each row's tokens behind the first, fp32 [B, T - 1] (and the entropies of their distributions, without
+        gradient): what a policy-gradient step takes of the policy and of its reference."""
+        hidden = self.hidden(ids)
+        if self._fused_head(hidden):
+            target = Fn.pad(ids[:, 1:], (0, 1), value=-100)
+            out = dense.token_logprobs(hidden, self.lm_head.weight, target, temperature=temperature, entropy=entropy)
+            return (out[0][:, :-1], out[1][:, :-1]) if entropy else out[:, :-1]
+        logp = torch.log_softmax(self.lm_head(hidden)[:, :-1].float() / temperature, dim=-1)
+        picked = logp.gather(-1, ids[:, 1:, None])[..., 0]
+        return (picked, -(logp.detach().exp() * logp.detach()).sum(dim=-1)) if entropy else picked

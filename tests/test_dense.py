@@ -105,3 +105,20 @@ def test_cpu_tensors_are_refused(built_library):
         dense.linear_cross_entropy(x, w, t, reduction="average")
     with pytest.raises(ValueError, match="activation"):
         dense.linear(x, w, activation="relu6")
+
+
+def test_the_decoder_with_fused_dense_layers_is_the_plain_one_on_the_cpu():
+    from fp4_post_b200.decoder import Decoder, DecoderConfig
+    cfg = DecoderConfig(hidden=64, layers=2, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=97)
+    torch.manual_seed(0)
+    plain = Decoder(cfg)
+    fused = Decoder(cfg, fuse_dense=True)
+    fused.load_state_dict(plain.state_dict())
+    ids = torch.randint(0, cfg.vocab, (2, 12))
+    assert torch.equal(plain(ids), fused(ids)) and torch.equal(plain.loss(ids), fused.loss(ids))
+    logp, entropy = plain.token_logprobs(ids, temperature=0.8, entropy=True)
+    assert logp.shape == entropy.shape == (2, 11)
+    want = torch.log_softmax(plain(ids)[:, :-1] / 0.8, dim=-1)
+    torch.testing.assert_close(logp, want.gather(-1, ids[:, 1:, None])[..., 0])
+    torch.testing.assert_close(entropy, -(want.exp() * want).sum(-1))
+    torch.testing.assert_close(-plain.token_logprobs(ids).mean(), plain.loss(ids))

@@ -374,3 +374,244 @@ def test_what_the_calls_refuse():
         with pytest.raises(error):
             call()
             raise AssertionError(f"case {i} was not refused")
+
+
+# ---- how the calls are made -----------------------------------------------------------------------------------
+
+def train_step(x, w, b, g, r, head, t, dy):
+    """Everything together: a gated layer, a layer onto a residual, the loss, and all gradients."""
+    h = dense.linear(x, w, b, activation="silu", gate=g)
+    h = dense.linear(h, w, residual=r)
+    loss = dense.linear_cross_entropy(h, head, t, temperature=0.9)
+    logp, ent = dense.token_logprobs(h, head, t, entropy=True)
+    grads = torch.autograd.grad((loss, logp), (x, w, b, g, r, head), (None, dy))
+    return (loss.detach(), logp.detach(), ent, *grads)
+
+
+def train_inputs(seed, M=300, K=256, V=1003):
+    x, w, b = normal(M, K, seed=seed), normal(K, K, scale=K ** -0.5, seed=seed + 1), normal(K, seed=seed + 2)
+    g, r, head = normal(M, K, seed=seed + 3), normal(M, K, seed=seed + 4), normal(V, K, scale=K ** -0.5, seed=seed + 5)
+    t = torch.randint(0, V, (M,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+    t[3::7] = -100
+    return [v.requires_grad_(True) for v in (x, w, b, g, r, head)] + [t, normal(M, seed=seed + 6, dtype=torch.float32)]
+
+
+def test_calls_together_and_again_give_the_same_bits():
+    inputs = train_inputs(1)
+    want = train_step(*inputs)
+    for _ in range(3):
+        assert all(torch.equal(a, c) for a, c in zip(train_step(*inputs), want))
+    # against torch in 64 bits: bf16 between the calls (h is rounded twice, and its gradients), so the norm of the whole goes by six roundings
+    d = [v.detach().double().requires_grad_(True) for v in inputs[:6]]
+    t, dy = inputs[6:]
+    h = linear64(d[0], d[1], d[2], "silu", d[3], None)
+    h = linear64(h, d[1], None, None, None, d[4])
+    loss = torch.nn.functional.cross_entropy(h @ d[5].t() / 0.9, t)
+    logp, ent, _ = head64(h, d[5], t, 1.0)
+    exact = torch.autograd.grad((loss, logp), d, (None, dy.double()))
+    assert rel(want[0], loss.detach()) <= 6 * STEP and rel(want[1], logp.detach()) <= 6 * STEP and rel(want[2], ent.detach()) <= 6 * STEP
+    for a, e in zip(want[3:], exact):
+        assert rel(a, e) <= 6 * STEP
+
+
+def test_on_another_stream_and_from_several_threads():
+    import threading
+    inputs = train_inputs(2)
+    want = train_step(*inputs)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(st):
+            for _ in range(10):
+                got = train_step(*inputs)
+                if not all(torch.equal(a, c) for a, c in zip(got, want)):
+                    wrong.append(1)
+    work()
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not wrong
+
+
+@pytest.mark.parametrize("M,V", [(300, 1003), (16, 5000), (2500, 300)])
+def test_captured_in_graphs_that_are_replayed_in_turn(M, V):
+    first, second = train_inputs(3, M=M, V=V), train_inputs(4, M=M, V=V)
+    static = [train_inputs(5, M=M, V=V) for _ in range(2)]
+    graphs, outs = [], []
+    for s in static:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            train_step(*s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(train_step(*s))
+        graphs.append(graph)
+    for inputs in (first, second, first):
+        want = train_step(*inputs)
+        for s, graph in zip(static, graphs):
+            with torch.no_grad():
+                for a, c in zip(s, inputs):
+                    a.copy_(c)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_backward_twice_and_a_graph_of_the_gradients():
+    x, w = normal(40, 64).requires_grad_(True), normal(48, 64, seed=1).requires_grad_(True)
+    y = dense.linear(x, w, activation="gelu")
+    dy = normal(40, 48, seed=2)
+    a = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    c = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+    t = torch.zeros(40, dtype=torch.int64, device="cuda")
+    for out in (dense.linear(x, w, activation="gelu").float().sum(), dense.linear_cross_entropy(x, w, t)):
+        gx, = torch.autograd.grad(out, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            gx.float().sum().backward()
+    # a saved tensor that was changed in between is noticed
+    y = dense.linear(x, w)
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+
+
+def test_offsets_beyond_32_bits():
+    M, N, K = 70001, 32776, 8                                # 2.3 * 10^9 elements in y, gate and residual
+    x, w = normal(M, K), normal(N, K, seed=1)
+    g = normal(1, N, seed=2).expand(M, N).contiguous()
+    y = dense.linear(x, w, activation="silu", gate=g, residual=g)
+    rows = torch.tensor([0, 1, 35000, 65535, 65537, 69999, 70000], device="cuda")
+    want = linear64(x[rows].double(), w.double(), None, "silu", g[rows].double(), g[rows].double())
+    err = (y[rows].double() - want).abs()
+    assert (err <= STEP * want.abs() + 2.0 ** -16 * (1 + g[rows].double().abs())).all()
+    del y, g
+    # (a vocabulary of 131080 rows and 20000 tokens: 2.6 * 10^9 logits)
+    M, V, K = 20000, 131080, 8
+    h, w, t = head_inputs(M, V, K)
+    h.requires_grad_(True)
+    loss = dense.linear_cross_entropy(h, w, t, reduction="sum")
+    dh, = torch.autograd.grad(loss, h)
+    rows = torch.arange(M - 300, M, device="cuda")
+    h64 = h.detach()[rows].double().requires_grad_(True)
+    logp, _, _ = head64(h64, w.double(), t[rows], 1.0)
+    exact, = torch.autograd.grad(-logp.sum(), h64)
+    assert rel(dh[rows], exact) <= 2 * STEP
+    each = dense.token_logprobs(h, w, t)
+    assert (each[rows].double() - logp).abs().max() <= 1e-4
+
+
+def test_gradients_against_differences():
+    """Central differences of the calls themselves, along random directions; steps that bf16 represents.  The loss is smooth, so that the difference over
+    2 d is off by its third derivative (d^2 / 6 of it) and by the outputs' roundings over d."""
+    M, N, K = 32, 40, 64
+    x, w, t = normal(M, K), normal(N, K, scale=0.25, seed=1), torch.arange(M, device="cuda") % N
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    gx, gw = torch.autograd.grad(dense.linear_cross_entropy(x, w, t, reduction="sum"), (x, w))
+    for leaf, grad, other in ((x, gx, w), (w, gw, x)):
+        direction = torch.randint(-1, 2, leaf.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).bfloat16()
+        d = 2.0 ** -5
+        moved = [(leaf.detach() + s * d * direction) for s in (1, -1)]
+        real = [(m.double() - leaf.detach().double()) for m in moved]      # what bf16 made of the step
+        f = [float(dense.linear_cross_entropy(*((m, other) if leaf is x else (other, m)), t, reduction="sum").double()) for m in moved]
+        along = float((grad.double() * (real[0] - real[1])).sum())
+        scale = float((grad.double().abs() * (real[0] - real[1]).abs()).sum())
+        assert abs((f[0] - f[1]) - along) <= 0.02 * scale + 1e-3
+
+
+# ---- the decoder ------------------------------------------------------------------------------------------------
+
+@pytest.fixture()
+def decoders():
+    from fp4_post_b200.decoder import Decoder, DecoderConfig
+    cfg = DecoderConfig(hidden=256, layers=2, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1003)
+    torch.manual_seed(0)
+    plain = Decoder(cfg, fuse_norms=False).cuda().bfloat16()
+    fused = Decoder(cfg, fuse_norms=False, fuse_dense=True).cuda().bfloat16()
+    fused.load_state_dict(plain.state_dict())
+    return plain, fused, torch.randint(0, cfg.vocab, (3, 65), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+
+
+def test_the_decoder_calls_them(decoders):
+    from fp4_post_b200 import ops
+    plain, fused, ids = decoders
+    want, before = plain.loss(ids), ops.launch_count()
+    loss = fused.loss(ids)
+    # per block the o, gate and down projections, then the head: statistics, rows, mean
+    assert ops.launch_count() - before == 2 * 3 + 3
+    assert rel(loss.detach(), want.detach().double()) <= 2e-3
+    want.backward()
+    loss.backward()
+    for (name, a), (_, c) in zip(fused.named_parameters(), plain.named_parameters()):
+        # both sides round every tensor between their kernels to bf16, the plain one more of them (the logits among them)
+        assert rel(a.grad, c.grad.double()) <= 0.05, name
+    with torch.no_grad():
+        logp, ent = fused.token_logprobs(ids, temperature=0.7, entropy=True)
+        logp_p, ent_p = plain.token_logprobs(ids, temperature=0.7, entropy=True)
+        # (the plain logits are rounded to bf16: 2^-8 of their size, at most 4 here, on either side of the difference)
+        assert logp.shape == (3, 64) and (logp - logp_p).abs().max() <= 0.1 and (ent - ent_p).abs().max() <= 0.1
+        assert torch.equal(logp, fused.token_logprobs(ids, temperature=0.7))
+        assert rel(-fused.token_logprobs(ids).mean(), loss.detach().double()) <= 1e-6
+
+
+def metis_decoder(fuse_dense, targets):
+    import fp4_post_b200
+    fp4_post_b200.install_reference_aliases()
+    from fp4_post_b200.decoder import Decoder, DecoderConfig
+    from grpo.grpo import MetisArgs, replace_linear_with_metis
+    cfg = DecoderConfig(hidden=256, layers=2, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1003)
+    torch.manual_seed(0)
+    model = Decoder(cfg, fuse_dense=fuse_dense).cuda().bfloat16()
+    args = MetisArgs(forward_svd_rank=32, activation_lowrank_svd=32, backward_lowrank_svd=32)
+    args.device = "cuda"
+    args.q_backward_input = args.q_backward_weight = args.q_backward_outputgrad = "nvfp4e2m1bnosr"
+    replace_linear_with_metis(model, dtype=torch.bfloat16, metis_args=args, target_modules=targets, compute_dtype=torch.bfloat16)
+    return model, torch.randint(0, cfg.vocab, (2, 64), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+
+
+def test_the_decoder_with_metis_layers_and_fused_dense_steps_as_a_graph():
+    from fp4_post_b200.graphs import GraphedStep
+    model, ids = metis_decoder(True, None)
+    params = list(model.parameters())
+
+    def step():
+        for p in params:
+            p.grad = None
+        loss = model.loss(ids)
+        loss.backward()
+        return loss
+    want = float(step().detach())
+    grads = [p.grad.clone() for p in params]
+    runner = GraphedStep(step, warmup=1)
+    loss = runner()
+    torch.cuda.synchronize()
+    assert float(loss.detach()) == want                     # round to nearest throughout: the same kernels, the same bits
+    for p, g in zip(params, grads):
+        assert torch.equal(p.grad, g)
+    runner.release()
+
+
+def test_the_decoder_with_some_projections_left_in_bf16():
+    """o, gate and down stay plain layers beside Metis ones: fused, they are what they were but for the roundings between their kernels."""
+    targets = ["q_proj", "k_proj", "v_proj", "up_proj"]
+    (fused, ids), (plain, _) = metis_decoder(True, targets), metis_decoder(False, targets)
+    plain.load_state_dict(fused.state_dict())
+    a, c = fused.loss(ids), plain.loss(ids)
+    assert rel(a.detach(), c.detach().double()) <= 5e-3
+    a.backward()
+    c.backward()
+    for (name, p), (_, q) in zip(fused.named_parameters(), plain.named_parameters()):
+        # (NVFP4 gradients: a rounding of an activation can move an element of a block by a step, an eighth of its size or more)
+        assert torch.isfinite(p.grad).all() and (float(q.grad.double().norm()) < 1e-6 or rel(p.grad, q.grad.double()) <= 0.35), name
