@@ -63,6 +63,24 @@ struct Staging {
   }
 };
 
+// Two such pieces of two tensors at once: one wait for the buffers, one fence.
+__device__ __forceinline__ void store_two_tma(Staging& st, const CUtensorMap* map0, const uint32_t (&w0)[16], const CUtensorMap* map1, const uint32_t (&w1)[16],
+                                              int32_t x, int32_t row0) {
+  const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  uint8_t* buf = st.idle();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w0[4 * k], w0[4 * k + 1], w0[4 * k + 2], w0[4 * k + 3]);
+    *reinterpret_cast<uint4*>(buf + 2048 + lane * 64 + ((k ^ swz) << 4)) = make_uint4(w1[4 * k], w1[4 * k + 1], w1[4 * k + 2], w1[4 * k + 3]);
+  }
+  fence_async_shared();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map0, smem_u32(buf), x, row0);
+    tma_store_2d(map1, smem_u32(buf) + 2048, x, row0);
+  }
+}
+
 // 32 rows x 64 bytes, one row per lane (four 16-byte pieces), through shared memory to the tensor at (row0, x): 64-byte swizzle.
 template <int kStores = 2>
 __device__ __forceinline__ void store_piece_tma(Staging& st, const CUtensorMap* map, const uint32_t (&w)[16], int32_t x, int32_t row0) {
@@ -225,11 +243,12 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
 
-// With z, gate or residual: several tensors of the output's size pass by.  What is read comes by asynchronous copies of the load/store unit
-// a piece ahead; what is written leaves by the TMA unit.  Tried, 8192 x 8960 x 1536, us, plain 150 to 158: silu, gate and z / gate and residual by
-// this form 211 / 188 (five stages in place of six pay for the buffers); loads into registers where they are used 238 / 220; loads by the
-// TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores by the load/store
-// unit 235 / 188.  `next`: the piece that this warp takes after this one.
+// With z, gate or residual: several tensors of the output's size pass by, and a warp's chain of waits for a piece is what bounds the layer
+// (the tensor pipe is busy 0.53 of the time, 0.95 without them).  What is read comes by asynchronous copies of the load/store unit a piece
+// ahead; what is written leaves by the TMA unit, both tensors behind one fence.  Tried, 8192 x 8960 x 1536, us, plain 150 to 158: silu, gate and z /
+// gate and residual by this form 204 / 187 (five stages in place of six pay for the buffers); loads into registers where they are used 238 /
+// 220; loads by the TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores
+// by the load/store unit 235 / 188.  `next`: the piece that this warp takes after this one.
 struct PieceAt {
   bool valid;
   int64_t row0, col0;
@@ -242,13 +261,16 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-  uint32_t w[16];
+  uint32_t w[16], zw[16];
   if (p.bias) add_bias32(v, p, col0, full);
+  const bool two = !kOdd && p.z && p.z_wide && p.d_wide;   // z and the output leave together
   if (p.z) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (p.z_wide) store_piece_tma<kStores>(st, map_z, w, (int32_t)col0, (int32_t)row0);
-    else store_piece_rows(st, p.z, p.ldz, w, col0, row0, p.M, p.N);
+    for (int i = 0; i < 16; ++i) zw[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    if (!two) {
+      if (p.z_wide) store_piece_tma<kStores>(st, map_z, zw, (int32_t)col0, (int32_t)row0);
+      else store_piece_rows(st, p.z, p.ldz, zw, col0, row0, p.M, p.N);
+    }
   }
   activate_all(p.act, v);
   if (gate.src) {
@@ -267,7 +289,8 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-  if (p.d_wide) store_piece_tma<kStores>(st, map_d, w, (int32_t)col0, (int32_t)row0);
+  if (two) store_two_tma(st, map_z, zw, map_d, w, (int32_t)col0, (int32_t)row0);
+  else if (p.d_wide) store_piece_tma<kStores>(st, map_d, w, (int32_t)col0, (int32_t)row0);
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
 
@@ -535,7 +558,9 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       constexpr bool kAhead = !Cfg::kOperands;
       uint32_t r[kAhead ? 2 : 1][32];
       if (kAhead && sums) tc_load32(t_row, r[0]);
-#pragma unroll
+      // (a piece with operands is some 600 instructions, several times that with the activations it may have: four copies of it leave the
+      // instruction cache)
+#pragma unroll(Cfg::kOperands ? 1 : Cfg::kChunks)
       for (int ch = 0; ch < Cfg::kChunks; ++ch) {
         uint32_t(&v)[32] = r[kAhead ? ch & 1 : 0];
         if (sums) {
@@ -1025,7 +1050,7 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   else      { if (int32_t rc = make_map(&ma, dt, 2, a.p, p.K, p.M, a.ld * 2, 64, 128, "A (K-major)")) return rc; }
   if (kBMn) { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.N, p.K, b.ld * 2, 64, 64, "B (MN-major)")) return rc; }
   else      { if (int32_t rc = make_map(&mb, dt, 2, b.p, p.K, p.N, b.ld * 2, 64, 128, "B (K-major)")) return rc; }
-  p.band = 8;
+  p.band = 16;                                             // (4, 8, 16, 32: loss of 2048 tokens over 151936 x 1536 774, 770, 755, 746 us; linear layers the same)
   if (p.splits < 1) p.splits = 1;
   if (p.splits == 1) p.iters_per_split = INT32_MAX;
   const int64_t tiles = ceil_div(p.M, 256) * ceil_div(p.N, 256) * p.splits;
@@ -1120,7 +1145,8 @@ static bool few_tokens(int64_t M, int64_t N, int64_t K, bool w_mn, SmallShape* s
   return plan.us < pair_us;
 }
 
-// Columns of the vocabulary that the backward pass takes at a time: their gradients G [M, columns] in bf16 go through memory.
+// Columns of the vocabulary that the backward pass takes at a time: their gradients G [M, columns] in bf16 go through memory.  Loss and
+// gradients of 8192 x 151936 x 1536 with pieces of 256 MiB 12.9 ms, of 512 12.3, of 1024 12.3, whole 12.2.
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 static int64_t piece_columns(int64_t M, int64_t V) {
   int64_t columns = kPieceBytes / (2 * M) / 256 * 256;
