@@ -32,7 +32,7 @@ struct DenseParams {
   float* stats_e;                                          // [slots, stats_ld]: sum of 2^(..) (l log2(e) - maximum), or null
   float* picked;                                           // [M]: logit of the target times log2(e), as the statistics have it
   const float* lse;                                        // [M]
-  const float* gout;  int32_t gout_stride;                 // gradient of each row's loss: gout[row * stride] times *inv_count (null: 1)
+  const float* gout;  int32_t gout_stride;                 // gradient of each row's loss (stride 1), or of all, times *inv_count (null: 1)
   const float* inv_count;
   // sum of pieces: fp32 addend.  With `splits` > 1 each split of the contraction has sums of its own, [splits, split_rows, N]
   const float* c;  int64_t ldc;
@@ -88,6 +88,8 @@ __device__ __forceinline__ int32_t load_count(const int32_t* p) {
   asm volatile("ld.global.b32 %0, [%1];" : "=r"(n) : "l"(p) : "memory");
   return n;
 }
+
+__device__ __forceinline__ float common_weight(const float* gout, const float* inv_count, float scale) { return *gout * (inv_count ? *inv_count : 1.0f) * scale; }
 
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;

@@ -507,6 +507,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       at.valid = at.valid && at.row0 < M && at.col0 < p.N;
       return at;
     };
+    const float alpha = kEpi == kEpiSum && p.gout ? common_weight(p.gout, p.inv_count, p.weight_scale) : 1.0f;
     uint32_t local_tile = 0;
     for (int64_t tile = pair; tile < num_tiles; tile += num_pairs, ++local_tile) {
       int64_t tm, tn;
@@ -531,8 +532,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           if constexpr (kEpi == kEpiGrad) {
             dead = t == p.ignore;
             lse2 = p.lse[given] * kLog2e;
-            weight = p.gout[given * p.gout_stride] * p.weight_scale;
-            if (p.inv_count) weight *= *p.inv_count;
+            // (one gradient for all rows: it multiplies the products, not G, whose common factor bf16 would round)
+            weight = p.gout_stride ? p.gout[given] * p.weight_scale : p.weight_scale < 0.0f ? -1.0f : 1.0f;
             if (t < 0 || t >= p.vocab) weight = NAN;       // (a target outside the vocabulary; ignored rows are dead)
           }
         }
@@ -612,8 +613,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           if constexpr (kEpi == kEpiSum || kEpi == kEpiSumF32) {
             float g[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(v[i]);
-            if (p.c && row < M) {
+            for (int i = 0; i < 32; ++i) g[i] = kEpi == kEpiSum ? __uint_as_float(v[i]) * alpha : __uint_as_float(v[i]);
+            if (kEpi == kEpiSumF32 && p.c && row < M) {
               const float* c = p.c + (out0 + row) * p.ldc + col0;
               if (col0 + 32 <= p.N) {
 #pragma unroll
@@ -841,11 +842,13 @@ head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, c
   }
 }
 
-// d[m] = the sum over the splits of row place_of[m] of the sums (m itself where there is no place_of), in bf16; zeros for a place of -1.  A thread takes eight
+// d[m] = alpha times the sum over the splits of row place_of[m] of the sums (m itself where there is no place_of), in bf16; zeros for a place of -1.  A thread takes eight
 // columns of a row.
 __global__ void __launch_bounds__(256)
-finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M, int pieces, const int32_t* place_of, __nv_bfloat16* d, int64_t ldd) {
+finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M, int pieces, const int32_t* place_of, const float* gout, const float* inv_count,
+                   float scale, __nv_bfloat16* d, int64_t ldd) {
   grid_dependency_wait();
+  const float alpha = gout ? common_weight(gout, inv_count, scale) : 1.0f;
   const int64_t ld = 8 * (int64_t)pieces, total = M * pieces;
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
     const int64_t m = e / pieces, k = e - m * pieces, i = place_of ? place_of[m] : m;
@@ -859,6 +862,8 @@ finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M,
         v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
       }
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= alpha;
     reinterpret_cast<uint4*>(d + m * ldd)[k] = pack8(v);
   }
 }
@@ -888,7 +893,7 @@ head_sum_kernel(const float* nll, const int64_t* target, int64_t ignore, int64_t
   if (threadIdx.x == 0) {
     for (int w = 1; w < 32; ++w) { sum += s_sum[w]; count += s_count[w]; }
     *loss = (float)(mean ? sum / (double)count : sum);     // (no row at all: 0 / 0, as torch has it)
-    *inv_count = mean ? (float)(1.0 / (double)count) : 1.0f;
+    *inv_count = !mean ? 1.0f : count ? (float)(1.0 / (double)count) : 0.0f;       // (then there is no gradient either)
   }
 }
 
@@ -1086,13 +1091,19 @@ static int32_t map_bf16(CUtensorMap* map, const void* d, int64_t ld, int64_t M, 
 
 // D = A B^T for gradients: (A K-major, B MN-major), or (both MN-major).  In bf16; or `sums`, fp32 [splits, split_rows, N] with split_rows = M in
 // whole tiles, added to what they hold where `add` is set, and finish_sums behind them.
+struct CommonWeight {                                      // what a bf16 D is multiplied by: scale * *gout * (inv_count ? *inv_count : 1); nothing where gout is null
+  const float* gout = nullptr;
+  const float* inv_count = nullptr;
+  float scale = 1.0f;
+};
 struct Splits {
   int32_t splits, iters_per_split;
   int64_t rows, bytes;                                     // of the sums
 };
 static int32_t dense_sum(const DenseOperand& a, const DenseOperand& b, int64_t M, int64_t N, int64_t K, void* d, int64_t ldd, int32_t* status, cudaStream_t st,
-                         const int32_t* live = nullptr, const Splits* sp = nullptr, float* sums = nullptr, bool add = false) {
+                         const int32_t* live = nullptr, const Splits* sp = nullptr, float* sums = nullptr, bool add = false, const CommonWeight& weight = {}) {
   DenseParams p = {};
+  p.gout = weight.gout; p.inv_count = weight.inv_count; p.weight_scale = weight.scale;
   p.live = live; p.live_is_k = a.mn;                       // (rows that are not ignored: the output's, or those a weight's gradient sums over)
   p.M = M; p.N = N; p.K = K; p.status = status;
   CUtensorMap md = {};
@@ -1257,8 +1268,8 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   return METIS_OK;
 }
 
-static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64_t N, const int32_t* place_of, __nv_bfloat16* d, int64_t ldd, cudaStream_t st) {
-  METIS_CUDA_OK(launch_counted(kLaunchStream, finish_sums_kernel, dim3(row_blocks(ceil_div(M * N, 256))), dim3(256), 0, st, sums, (int)sp.splits, sp.rows, M, (int)(N / 8), place_of, d, ldd));
+static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64_t N, const int32_t* place_of, const CommonWeight& weight, __nv_bfloat16* d, int64_t ldd, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchStream, finish_sums_kernel, dim3(row_blocks(ceil_div(M * N, 256))), dim3(256), 0, st, sums, (int)sp.splits, sp.rows, M, (int)(N / 8), place_of, weight.gout, weight.inv_count, weight.scale, d, ldd));
   return METIS_OK;
 }
 
@@ -1293,7 +1304,7 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (!workspace || !aligned16(workspace) || workspace_bytes < sp.bytes) return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   float* sums = static_cast<float*>(workspace);
   if (int32_t rc = dense_sum(oa, ob, M, N, K, nullptr, 0, status, st, nullptr, &sp, sums)) return rc;
-  return finish_sums(sums, sp, M, N, nullptr, static_cast<__nv_bfloat16*>(d), ldd, st);
+  return finish_sums(sums, sp, M, N, nullptr, {}, static_cast<__nv_bfloat16*>(d), ldd, st);
 }
 
 // ---- head ---------------------------------------------------------------------------------------------------------
@@ -1427,6 +1438,7 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
                                        void* dh, int64_t lddh, void* dw, int64_t lddw) {
   if (int32_t rc = check_head(a)) return rc;
   if (!gout || (!dh && !dw)) return fail(METIS_ERR_BAD_ARGUMENT, "gout is null, or nothing is asked for");
+  if (gout_stride && inv_count) return fail(METIS_ERR_BAD_ARGUMENT, "inv_count belongs to one gradient for all rows");
   if (gout_stride != 0 && gout_stride != 1) return fail(METIS_ERR_BAD_ARGUMENT, "gout_stride must be 0 or 1");
   if (dh) if (int32_t rc = check_rows(dh, lddh, a->K, "dh")) return rc;
   if (dw) if (int32_t rc = check_rows(dw, lddw, a->K, "dw")) return rc;
@@ -1439,7 +1451,8 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   if (pack.on) if (int32_t rc = pack_rows(a, pack, nullptr, nullptr, st)) return rc;
   const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false};
   DenseParams p = head_params(a, pack);
-  p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride; p.inv_count = inv_count;
+  p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride;
+  const CommonWeight weight = gout_stride ? CommonWeight{} : CommonWeight{gout, inv_count, a->scale};
   for (int64_t v0 = 0; v0 < a->V; v0 += b.columns) {
     const int64_t n = a->V - v0 < b.columns ? a->V - v0 : b.columns;
     CUtensorMap mg = {};
@@ -1448,16 +1461,17 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
     if (int32_t rc = map_bf16(&mg, b.g, b.columns, a->M, n, "G")) return rc;
     if (int32_t rc = launch_dense<false, false, kEpiGrad>(h, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
     if (dw) {
-      if (int32_t rc = dense_sum({b.g, b.columns, true}, {h.p, h.ld, true}, n, a->K, a->M, static_cast<__nv_bfloat16*>(dw) + v0 * lddw, lddw, a->status, st, p.live)) return rc;
+      if (int32_t rc = dense_sum({b.g, b.columns, true}, {h.p, h.ld, true}, n, a->K, a->M, static_cast<__nv_bfloat16*>(dw) + v0 * lddw, lddw, a->status, st, p.live,
+                                 nullptr, nullptr, false, weight)) return rc;
     }
     if (dh) {
       // a shorter last piece has no more splits than the others; those that it leaves out keep what they hold
       const int64_t stages = ceil_div(n, 64);
       Splits sp = b.sp;
       sp.splits = (int32_t)ceil_div(stages, sp.iters_per_split);
-      if (int32_t rc = dense_sum({b.g, b.columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, b.sums ? nullptr : dh, lddh, a->status, st, p.live, &sp, b.sums, v0 > 0)) return rc;
+      if (int32_t rc = dense_sum({b.g, b.columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, b.sums ? nullptr : dh, lddh, a->status, st, p.live, &sp, b.sums, v0 > 0, weight)) return rc;
     }
   }
-  if (dh && b.sums) return finish_sums(b.sums, b.sp, a->M, a->K, pack.on ? pack.place_of : nullptr, static_cast<__nv_bfloat16*>(dh), lddh, st);
+  if (dh && b.sums) return finish_sums(b.sums, b.sp, a->M, a->K, pack.on ? pack.place_of : nullptr, weight, static_cast<__nv_bfloat16*>(dh), lddh, st);
   return METIS_OK;
 }

@@ -527,12 +527,14 @@ typedef struct metis_head_args {
 } metis_head_args;
 int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy);
 int32_t metis_head_loss(const metis_head_args* args, float* nll, float* entropy);
-/* loss = sum of nll, over the number of rows that are not ignored where mean is set; *inv_count = 1 over that number, or 1. */
+/* loss = sum of nll, over the number of rows that are not ignored where mean is set; *inv_count = 1 over that number (0 where
+ * there is none), or 1. */
 int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_index, int64_t M, int32_t mean, float* loss,
                        float* inv_count, void* stream);
 /*
  * dh [M, K] = G W and dw [V, K] = G^T h (bf16, either may be null) with G[m][j] = scale * g_m (softmax(l)[m][j] - [j = target[m]]),
- * g_m = gout[m * gout_stride] * (inv_count ? *inv_count : 1), 0 where target[m] = ignore_index.  The logits are formed
+ * g_m = gout[m] (gout_stride 1; inv_count is null) or *gout * (inv_count ? *inv_count : 1) (gout_stride 0), 0 where
+ * target[m] = ignore_index.  The logits are formed
  * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, dh's sums in fp32.
  */
 int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K);

@@ -86,6 +86,7 @@ def test_head_refuses(L, p):
     assert L.metis_head_loss(args(), None, None) == -1
     assert L.metis_head_backward(args(), None, 0, None, p, 16, p, 16) == -1
     assert L.metis_head_backward(args(), p, 2, None, p, 16, p, 16) == -1
+    assert L.metis_head_backward(args(), p, 1, p, p, 16, p, 16) == -1                # a mean has one gradient for all rows
     assert L.metis_head_backward(args(), p, 0, None, None, 16, None, 16) == -1       # nothing asked for
     assert L.metis_head_backward(args(), p, 0, None, p, 8, p, 16) == -3 and L.metis_head_backward(args(), p, 0, None, p, 16, p + 2, 16) == -3
     assert L.metis_head_sum(None, p, -100, 4, 1, p, p, None) == -1 and L.metis_head_sum(p, p, -100, 0, 1, p, p, None) == -2

@@ -236,6 +236,23 @@ def test_losses_over_many_tiles():
     check_head(700, 40003, 128)
 
 
+def test_the_common_factor_of_a_mean_is_not_rounded():
+    # 1 / 1021 is not a bf16 number: in the logits' gradient it would move every gradient by the same 2^-9 or so
+    h, w, t = head_inputs(1021, 3001, 128, ignored=0.0, size=0.5)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    h64, w64 = h.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    logp, _, _ = head64(h64, w64, t, 1.0)
+    for factor in (1.0, 1.0 / 3.0):
+        dh, dw = torch.autograd.grad(dense.linear_cross_entropy(h, w, t), (h, w), torch.tensor(factor, device="cuda"))
+        eh, ew = torch.autograd.grad(-logp.mean(), (h64, w64), torch.tensor(factor, device="cuda", dtype=torch.float64), retain_graph=True)
+        for a, e in ((dh, eh), (dw, ew)):
+            # The best factor between the two is 1, but for what independent roundings of 10^5 elements leave on average, and for one that is not
+            # independent: the target's element of the logits' gradient is p - 1, and where p is less than half of bf16's step below 1 (2^-9, as
+            # nearly everywhere here, p being about 1 / 3001) it is rounded to -1, too far from 0 by p.
+            assert abs(float((a.double() * e).sum() / (e * e).sum()) - 1.0) <= STEP / 16 + float(logp.detach().exp().mean())
+
+
 def test_gradients_over_several_pieces_of_the_vocabulary(monkeypatch):
     # 65536 rows take the vocabulary in pieces of 4096 columns: 9001 of them are three
     M, V, K = 65536, 9001, 16
