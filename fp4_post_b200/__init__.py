@@ -2,6 +2,7 @@
 
     fp4_post_b200.cabi     ctypes binding of include/metis_nvfp4.h
     fp4_post_b200.ops      tensor-level wrappers (quantize, RMSNorm->quantize, GEMM, ...)
+    fp4_post_b200.dense    bf16 linear layers, cross entropy and token log-probabilities
     fp4_post_b200.Metis    host-side mirror of the reference's Metis package
     fp4_post_b200.grpo     MetisArgs / replace_linear_with_metis
 
