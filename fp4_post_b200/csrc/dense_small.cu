@@ -488,7 +488,7 @@ static int resident_clusters(int splits, int which, const void* kern, int smem) 
 SmallPlan plan_dense_small(int64_t M, int64_t N, int64_t K, bool w_mn) {
   SmallPlan best = {};
   float best_rank = 1e30f;
-  const int64_t blocks = ceil_div(K, 64), sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  const int64_t blocks = ceil_div(K, 64), sms = device_sm_count();
   const int64_t token_tiles = ceil_div(M, 256);
   const int bn = (int)(ceil_div(ceil_div(M, token_tiles), 16) * 16);
   const void* kern = w_mn ? reinterpret_cast<const void*>(dense_small_kernel<true>) : reinterpret_cast<const void*>(dense_small_kernel<false>);
@@ -572,7 +572,7 @@ int32_t launch_dense_small(const SmallShape& sh, const void* t, int64_t ldt, con
 }
 
 int64_t small_stats_slots(int64_t V) {
-  const int64_t units = ceil_div(V, 32), sms = device_sm_count() > 0 ? device_sm_count() : 148;
+  const int64_t units = ceil_div(V, 32), sms = device_sm_count();
   return 4 * (units < sms ? units : sms);
 }
 
