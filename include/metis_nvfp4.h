@@ -457,7 +457,8 @@ int64_t metis_dense_launches(void);
  * y = act(x W^T + bias) * gate + residual, x [M, K], W [N, K], y [M, N], all bf16, sums in fp32, one rounding at the end.
  * bias (bf16 or fp32 [N]), gate and residual ([M, N]) may be null; z, where given, receives bf16(x W^T + bias), from which
  * metis_linear_pointwise forms the gradients.  x and w: 16-byte aligned rows (leading dimensions multiples of 8), K a
- * multiple of 8; the others any, 16-byte aligned rows being the fast ones.  What nn.Linear and the elementwise kernels behind
+ * multiple of 8; the others any, 16-byte aligned rows being the fast ones (rows that begin elsewhere are read by the aligned 16
+ * bytes that hold them: up to 14 bytes beside a tensor are read, and not used; device allocations are whole 256 bytes).  What nn.Linear and the elementwise kernels behind
  * it do for a projection that replace_linear_with_metis leaves as it is (src/grpo/grpo.py:119-196, target_modules).
  */
 typedef struct metis_linear_args {
