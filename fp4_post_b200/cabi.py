@@ -76,7 +76,7 @@ class LinearArgs(C.Structure):
         ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
         ("bias", C.c_void_p), ("bias_dtype", C.c_int32), ("activation", C.c_int32),
         ("gate", C.c_void_p), ("ldgate", C.c_int64), ("residual", C.c_void_p), ("ldr", C.c_int64),
-        ("y", C.c_void_p), ("ldy", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64),
+        ("y", C.c_void_p), ("ldy", C.c_int64), ("act", C.c_void_p), ("ldact", C.c_int64), ("slope", C.c_void_p), ("ldslope", C.c_int64),
         ("status", C.c_void_p), ("stream", C.c_void_p),
     ]
 
@@ -85,9 +85,10 @@ class LinearPointwiseArgs(C.Structure):
     """struct metis_linear_pointwise_args"""
     _fields_ = [
         ("M", C.c_int64), ("N", C.c_int64),
-        ("dy", C.c_void_p), ("lddy", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64),
+        ("dy", C.c_void_p), ("lddy", C.c_int64), ("act", C.c_void_p), ("ldact", C.c_int64), ("slope", C.c_void_p), ("ldslope", C.c_int64),
+        ("gate", C.c_void_p), ("ldgate", C.c_int64),
         ("dz", C.c_void_p), ("lddz", C.c_int64), ("dgate", C.c_void_p), ("lddg", C.c_int64),
-        ("dbias", C.c_void_p), ("dbias_dtype", C.c_int32), ("activation", C.c_int32),
+        ("dbias", C.c_void_p), ("dbias_dtype", C.c_int32), ("reserved", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("stream", C.c_void_p),
     ]
 

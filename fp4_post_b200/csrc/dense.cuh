@@ -4,6 +4,8 @@
 
 #include "gemm_common.cuh"
 
+#include <cuda_fp16.h>
+
 #include <atomic>
 #include <utility>
 
@@ -13,13 +15,14 @@ struct DenseParams {
   int64_t M, N, K;
   int32_t* status;
   int32_t band;                                            // row tiles per band of the tile order
-  // linear layer: d = act(A B^T + bias) * gate + residual, and z, what act was applied to
+  // linear layer: d = act(z) * gate + residual with z = A B^T + bias; for the gradients act(z) in bf16 and act'(z) as half_slopes has it
   const void* bias;  int32_t bias_f32;
   int32_t act;
   const __nv_bfloat16* gate;      int64_t ldgate;  int32_t gate_wide;       // *_wide: rows of 16-byte pieces
   const __nv_bfloat16* residual;  int64_t ldr;     int32_t residual_wide;
   __nv_bfloat16* d;               int64_t ldd;     int32_t d_wide;
-  __nv_bfloat16* z;               int64_t ldz;     int32_t z_wide;
+  __nv_bfloat16* act_out;         int64_t ldact;                            // (both of 16-byte rows)
+  uint32_t* slope;                int64_t ldslope;                          // (in elements of 16 bits)
   // head: logits l = scale * (A B^T); columns of the vocabulary [0, N) of this launch are [col0, col0 + N) of all
   const int64_t* target;  int64_t ignore;
   const int32_t* row_of;                                   // the rows that are not ignored, one after the other (null: all rows, as they lie)
@@ -145,6 +148,28 @@ template <int kAct> __device__ __forceinline__ void activate_both(float z, float
     a = z * p;
     slope = fmaf(a * (1.0f - p), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), p);
   }
+}
+// What a backward pass needs of z.  act' lies in [-0.13, 1.13], so 16 bits with ten of mantissa hold it: in fp16, times 2^15 (the values lie
+// below 37100, and down to 2^-29 none loses bits).  An error of 2^-12 at most; from z in bf16 the slope has one of |z act''| 2^-9, and the
+// gradients of x and W, which round dz to bf16, are then 1.7 times as far from the exact ones as their own last rounding puts them; 1.4 so.
+constexpr float kSlopeScale = 32768.0f;
+__device__ __forceinline__ uint32_t half_slopes(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo * kSlopeScale, hi * kSlopeScale);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int kAct, int kN> __device__ __forceinline__ void activate_both_of(float (&v)[kN], uint32_t (&slopes)[kN / 2]) {
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    float s[2];
+    activate_both<kAct>(v[2 * i], v[2 * i], s[0]);
+    activate_both<kAct>(v[2 * i + 1], v[2 * i + 1], s[1]);
+    slopes[i] = half_slopes(s[0], s[1]);
+  }
+}
+template <int kN> __device__ __forceinline__ void activate_both_all(int act, float (&v)[kN], uint32_t (&slopes)[kN / 2]) {
+  if (act == METIS_ACT_SILU) activate_both_of<METIS_ACT_SILU>(v, slopes);
+  else if (act == METIS_ACT_GELU) activate_both_of<METIS_ACT_GELU>(v, slopes);
+  else activate_both_of<METIS_ACT_GELU_TANH>(v, slopes);
 }
 template <int kN> __device__ __forceinline__ void activate_all(int act, float (&v)[kN]) {
   if (act == METIS_ACT_SILU) {

@@ -81,6 +81,27 @@ __device__ __forceinline__ void store_two_tma(Staging& st, const CUtensorMap* ma
   }
 }
 
+// Three, the third in a buffer of the caller's.
+__device__ __forceinline__ void store_three_tma(Staging& st, uint8_t* third, const CUtensorMap* map0, const uint32_t (&w0)[16], const CUtensorMap* map1,
+                                                const uint32_t (&w1)[16], const CUtensorMap* map2, const uint32_t (&w2)[16], int32_t x, int32_t row0) {
+  const int lane = threadIdx.x & 31, swz = (lane >> 1) & 3;
+  uint8_t* buf = st.idle();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int at = lane * 64 + ((k ^ swz) << 4);
+    *reinterpret_cast<uint4*>(buf + at) = make_uint4(w0[4 * k], w0[4 * k + 1], w0[4 * k + 2], w0[4 * k + 3]);
+    *reinterpret_cast<uint4*>(buf + 2048 + at) = make_uint4(w1[4 * k], w1[4 * k + 1], w1[4 * k + 2], w1[4 * k + 3]);
+    *reinterpret_cast<uint4*>(third + at) = make_uint4(w2[4 * k], w2[4 * k + 1], w2[4 * k + 2], w2[4 * k + 3]);
+  }
+  fence_async_shared();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map0, smem_u32(buf), x, row0);
+    tma_store_2d(map1, smem_u32(buf) + 2048, x, row0);
+    tma_store_2d(map2, smem_u32(third), x, row0);
+  }
+}
+
 // 32 rows x 64 bytes, one row per lane (four 16-byte pieces), through shared memory to the tensor at (row0, x): 64-byte swizzle.
 template <int kStores = 2>
 __device__ __forceinline__ void store_piece_tma(Staging& st, const CUtensorMap* map, const uint32_t (&w)[16], int32_t x, int32_t row0) {
@@ -244,36 +265,39 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
 
-// With z, gate or residual: several tensors of the output's size pass by, and a warp's chain of waits for a piece is what bounds the layer
-// (the tensor pipe is busy 0.53 of the time, 0.95 without them).  What is read comes by asynchronous copies of the load/store unit a piece
-// ahead; what is written leaves by the TMA unit, both tensors behind one fence.  Tried, 8192 x 8960 x 1536, us, plain 150 to 158: silu, gate and z /
-// gate and residual by this form 204 / 187 (five stages in place of six pay for the buffers); loads into registers where they are used 238 /
-// 220; loads by the TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores
-// by the load/store unit 235 / 188.  `next`: the piece that this warp takes after this one.
+// With gate, residual, or what the gradients need: several tensors of the output's size pass by, and each adds its time to the layer's
+// (the tensor pipe is busy 0.53 of the time with two, 0.95 without).  What is read comes by asynchronous copies of the load/store unit a piece
+// ahead; what is written leaves by the TMA unit, all of it behind one fence where there are buffers for it (without a residual its buffer is
+// the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 210, and slopes 230, and act(z) 250 (272 with a wait and a
+// fence for the output alone), gate and residual 189, all of them 285 (five stages in place of six pay for the buffers).  Tried with two
+// outputs, silu and gate / gate and residual, 204 / 187 by this form: loads into registers where they are used 238 / 220; loads by the TMA
+// unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores by the load/store
+// unit 235 / 188.  `next`: the piece that this warp takes after this one.
 struct PieceAt {
   bool valid;
   int64_t row0, col0;
 };
 template <bool kOdd>
-__device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_z, EpilogueOperand<kOdd>& gate,
+__device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging& st, const CUtensorMap* map_d, const CUtensorMap* map_s, const CUtensorMap* map_a, EpilogueOperand<kOdd>& gate,
                                                   EpilogueOperand<kOdd>& residual, const uint32_t (&r)[32], int64_t row0, int64_t col0, const PieceAt& next) {
   constexpr int kStores = kOdd ? 1 : 2;
   const bool full = col0 + 32 <= p.N;
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-  uint32_t w[16], zw[16];
+  uint32_t w[16], slopes[16], act[16];
   if (p.bias) add_bias32(v, p, col0, full);
-  const bool two = !kOdd && p.z && p.z_wide && p.d_wide;   // z and the output leave together
-  if (p.z) {
+  if (p.slope) activate_both_all(p.act, v, slopes);
+  else activate_all(p.act, v);
+  if (p.act_out) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zw[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (!two) {
-      if (p.z_wide) store_piece_tma<kStores>(st, map_z, zw, (int32_t)col0, (int32_t)row0);
-      else store_piece_rows(st, p.z, p.ldz, zw, col0, row0, p.M, p.N);
-    }
+    for (int i = 0; i < 16; ++i) act[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
   }
-  activate_all(p.act, v);
+  const bool together = !kOdd && p.d_wide && !(p.slope && p.act_out && residual.src);
+  if (!together) {
+    if (p.slope) store_piece_tma<kStores>(st, map_s, slopes, (int32_t)col0, (int32_t)row0);
+    if (p.act_out) store_piece_tma<kStores>(st, map_a, act, (int32_t)col0, (int32_t)row0);
+  }
   if (gate.src) {
     if (kOdd || (gate.wide && full)) gate.take(w, col0, row0);
     else load_piece_rows(st, gate.src, gate.ld, col0, row0, p.M, p.N, w);
@@ -290,7 +314,9 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-  if (two) store_two_tma(st, map_z, zw, map_d, w, (int32_t)col0, (int32_t)row0);
+  if (together && p.slope && p.act_out) store_three_tma(st, residual.buf, map_s, slopes, map_a, act, map_d, w, (int32_t)col0, (int32_t)row0);
+  else if (together && p.slope) store_two_tma(st, map_s, slopes, map_d, w, (int32_t)col0, (int32_t)row0);
+  else if (together && p.act_out) store_two_tma(st, map_a, act, map_d, w, (int32_t)col0, (int32_t)row0);
   else if (p.d_wide) store_piece_tma<kStores>(st, map_d, w, (int32_t)col0, (int32_t)row0);
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
 }
@@ -335,7 +361,7 @@ __device__ __forceinline__ void stats_chunk(const DenseParams& p, RowStats& a, c
 template <bool kAMn, bool kBMn, int kEpi>
 __global__ void __launch_bounds__(DenseCfg<kEpi>::kThreads, 1)
 dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
-                       const __grid_constant__ CUtensorMap map_z, const DenseParams p) {
+                       const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_act, const DenseParams p) {
   using Cfg = DenseCfg<kEpi>;
   constexpr int kStages = Cfg::kStages;
   constexpr int BN = 256;
@@ -587,7 +613,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           if constexpr (Cfg::kOperands) {
             PieceAt next = {ch + 1 < Cfg::kChunks && col0 + 32 < p.N, row0, col0 + 32};
             if (!next.valid) next = ahead = first_piece(tile + num_pairs);
-            linear_wide_chunk(p, st, &map_d, &map_z, gate, residual, v, row0, col0, next);
+            linear_wide_chunk(p, st, &map_d, &map_s, &map_act, gate, residual, v, row0, col0, next);
           }
           if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
             stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
@@ -948,12 +974,12 @@ __device__ __forceinline__ void store_run(__nv_bfloat16* run, int count, unsigne
   }
 }
 
-// dz = dy * gate * act'(z), dgate = dy * act(z), and column sums of dz before its rounding.  A warp's lane has eight columns of a row, the
-// block's eight warps take eight rows at a time; a block owns 256 columns and every gridDim.y-th group of rows.  dz has 16-byte aligned
-// rows; kWide: all the others do too, and N is a multiple of 8.  Bound by memory: 8192 x 8960 with gate 126 us, 5.8 TB/s.
-template <int kAct, bool kWide>
+// dz = dy * gate * slope, dgate = dy * act, and column sums of dz before its rounding.  A warp's lane has eight columns of a row, the
+// block's eight warps take eight rows at a time; a block owns 256 columns and every gridDim.y-th group of rows.  dz, slope and act have
+// 16-byte aligned rows; kWide: all the others do too, and N is a multiple of 8.  Bound by memory: 8192 x 8960 with gate 145 us, 6.1 TB/s.
+template <bool kWide>
 __global__ void __launch_bounds__(256)
-linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat16* z, int64_t ldz,
+linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __half* slope, int64_t lds, const __nv_bfloat16* act, int64_t lda,
                         const __nv_bfloat16* gate, int64_t ldgate, int64_t M, int64_t N,
                         __nv_bfloat16* dz, int64_t lddz, __nv_bfloat16* dgate, int64_t lddg,
                         float* sums) {
@@ -968,20 +994,18 @@ linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __nv_bfloat
   for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < M; row += (int64_t)gridDim.y * 8) {
     float d[8], a[8], out[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { d[i] = 0.0f; a[i] = 1.0f; }
+    for (int i = 0; i < 8; ++i) { d[i] = 0.0f; a[i] = 0.0f; }
     if (left > 0) {
-      float zv[8], g[8];
+      float g[8];
+      uint4 s;
       load8_any<kWide>(dy + row * lddy + col, left, d);
-      if (kAct != METIS_ACT_NONE || dgate) load8_any<kWide>(z + row * ldz + col, left, zv);
+      if (slope) s = *reinterpret_cast<const uint4*>(slope + row * lds + col);
+      if (dgate) load8_any<true>(act + row * lda + col, left, a);
       if (gate) load8_any<kWide>(gate + row * ldgate + col, left, g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         out[i] = d[i];
-        if (kAct != METIS_ACT_NONE || dgate) {
-          float slope;
-          activate_both<kAct>(zv[i], a[i], slope);
-          out[i] *= slope;
-        }
+        if (slope) out[i] *= (1.0f / kSlopeScale) * __half2float(reinterpret_cast<const __half*>(&s)[i]);
         if (gate) out[i] *= g[i];
         a[i] *= d[i];
         acc[i] += out[i];
@@ -1048,7 +1072,7 @@ struct DenseOperand {
 };
 
 template <bool kAMn, bool kBMn, int kEpi>
-static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const CUtensorMap& map_d, DenseParams p, cudaStream_t st, const CUtensorMap& map_z = {}) {
+static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const CUtensorMap& map_d, DenseParams p, cudaStream_t st, const CUtensorMap& map_s = {}, const CUtensorMap& map_act = {}) {
   using Cfg = DenseCfg<kEpi>;
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ma, mb;
@@ -1080,7 +1104,7 @@ static int32_t launch_dense(const DenseOperand& a, const DenseOperand& b, const 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap_enabled(kLaunchGemm) ? 2 : 1;
-  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_z, p));
+  METIS_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, ma, mb, map_d, map_s, map_act, p));
   dense_launches.fetch_add(1, std::memory_order_relaxed);
   return METIS_OK;
 }
@@ -1184,10 +1208,13 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   if (int32_t rc = check_rows(a->x, a->ldx, a->K, "x")) return rc;
   if (int32_t rc = check_rows(a->w, a->ldw, a->K, "w")) return rc;
   if (!a->y) return fail(METIS_ERR_BAD_ARGUMENT, "y is null");
-  const uintptr_t odd = reinterpret_cast<uintptr_t>(a->y) | reinterpret_cast<uintptr_t>(a->z) | reinterpret_cast<uintptr_t>(a->gate) | reinterpret_cast<uintptr_t>(a->residual);
+  if (a->slope && a->activation == METIS_ACT_NONE) return fail(METIS_ERR_BAD_ARGUMENT, "slope is given without an activation");
+  if (a->act) if (int32_t rc = check_rows(a->act, a->ldact, a->N, "act")) return rc;
+  if (a->slope) if (int32_t rc = check_rows(a->slope, a->ldslope, a->N, "slope")) return rc;
+  const uintptr_t odd = reinterpret_cast<uintptr_t>(a->y) | reinterpret_cast<uintptr_t>(a->gate) | reinterpret_cast<uintptr_t>(a->residual);
   if ((odd & 1u) || (reinterpret_cast<uintptr_t>(a->bias) & (a->bias_dtype == METIS_DTYPE_F32 ? 3u : 1u)))
     return fail(METIS_ERR_BAD_ALIGNMENT, "a tensor is not aligned to its elements");
-  if (a->ldy < a->N || (a->z && a->ldz < a->N) || (a->gate && a->ldgate < a->N) || (a->residual && a->ldr < a->N))
+  if (a->ldy < a->N || (a->gate && a->ldgate < a->N) || (a->residual && a->ldr < a->N))
     return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
   DenseParams p = {};
   p.M = a->M; p.N = a->N; p.K = a->K; p.status = a->status;
@@ -1196,16 +1223,18 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   p.gate = static_cast<const __nv_bfloat16*>(a->gate); p.ldgate = a->ldgate; p.gate_wide = wide(a->gate, a->ldgate);
   p.residual = static_cast<const __nv_bfloat16*>(a->residual); p.ldr = a->ldr; p.residual_wide = wide(a->residual, a->ldr);
   p.d = static_cast<__nv_bfloat16*>(a->y); p.ldd = a->ldy; p.d_wide = wide(a->y, a->ldy);
-  p.z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ldz; p.z_wide = wide(a->z, a->ldz);
+  p.act_out = static_cast<__nv_bfloat16*>(a->act); p.ldact = a->ldact;
+  p.slope = static_cast<uint32_t*>(a->slope); p.ldslope = a->ldslope;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
   SmallShape sh;
   if (few_tokens(a->M, a->N, a->K, false, &sh)) return launch_dense_small(sh, a->x, a->ldx, a->w, false, a->ldw, p, st);
   const DenseOperand x = {a->x, a->ldx, false}, w = {a->w, a->ldw, false};
-  CUtensorMap md = {}, mz = {};
+  CUtensorMap md = {}, ms = {}, ma = {};
   if (p.d_wide) if (int32_t rc = map_bf16(&md, a->y, a->ldy, a->M, a->N, "y")) return rc;
-  if (p.z_wide) if (int32_t rc = map_bf16(&mz, a->z, a->ldz, a->M, a->N, "z")) return rc;
-  if ((a->gate && !p.gate_wide) || (a->residual && !p.residual_wide)) return launch_dense<false, false, kEpiLinearOdd>(x, w, md, p, st, mz);
-  if (a->gate || a->residual || a->z) return launch_dense<false, false, kEpiLinearWide>(x, w, md, p, st, mz);
+  if (a->slope) if (int32_t rc = map_bf16(&ms, a->slope, a->ldslope, a->M, a->N, "slope")) return rc;        // (16 bits are 16 bits)
+  if (a->act) if (int32_t rc = map_bf16(&ma, a->act, a->ldact, a->M, a->N, "act")) return rc;
+  if ((a->gate && !p.gate_wide) || (a->residual && !p.residual_wide)) return launch_dense<false, false, kEpiLinearOdd>(x, w, md, p, st, ms, ma);
+  if (a->gate || a->residual || a->slope || a->act) return launch_dense<false, false, kEpiLinearWide>(x, w, md, p, st, ms, ma);
   return launch_dense<false, false, kEpiLinear>(x, w, md, p, st);
 }
 
@@ -1215,15 +1244,15 @@ extern "C" int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N) 
   return kPointwiseGroups * N * (int64_t)sizeof(float);
 }
 
-template <int kAct>
 static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool wide, dim3 grid, float* sums) {
   auto launch = [&](auto kern) {
     return launch_counted(kLaunchStream, kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(a->stream),
-                             static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __nv_bfloat16*>(a->z), a->ldz,
+                             static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __half*>(a->slope), a->ldslope,
+                             static_cast<const __nv_bfloat16*>(a->act), a->ldact,
                              static_cast<const __nv_bfloat16*>(a->gate), a->ldgate, a->M, a->N, static_cast<__nv_bfloat16*>(a->dz), a->lddz,
                              static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
   };
-  METIS_CUDA_OK(wide ? launch(linear_pointwise_kernel<kAct, true>) : launch(linear_pointwise_kernel<kAct, false>));
+  METIS_CUDA_OK(wide ? launch(linear_pointwise_kernel<true>) : launch(linear_pointwise_kernel<false>));
   return METIS_OK;
 }
 
@@ -1232,18 +1261,19 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   if (int32_t rc = check_extent(a->M, "M")) return rc;
   if (int32_t rc = check_extent(a->N, "N")) return rc;
   if (!a->dy || (!a->dz && !a->dgate && !a->dbias)) return fail(METIS_ERR_BAD_ARGUMENT, "dy is null, or nothing is asked for");
-  if (a->activation < METIS_ACT_NONE || a->activation > METIS_ACT_GELU_TANH) return fail(METIS_ERR_BAD_ARGUMENT, "unknown activation %d", a->activation);
-  if ((a->activation != METIS_ACT_NONE || a->dgate) && !a->z) return fail(METIS_ERR_BAD_ARGUMENT, "z is null");
+  if (a->dgate && !a->act) return fail(METIS_ERR_BAD_ARGUMENT, "act is null");
+  if (a->act) if (int32_t rc = check_rows(a->act, a->ldact, a->N, "act")) return rc;
+  if (a->slope) if (int32_t rc = check_rows(a->slope, a->ldslope, a->N, "slope")) return rc;
   if (a->dbias && a->dbias_dtype != METIS_DTYPE_BF16 && a->dbias_dtype != METIS_DTYPE_F32) return fail(METIS_ERR_BAD_ARGUMENT, "unknown dbias_dtype %d", a->dbias_dtype);
-  if (a->lddy < a->N || (a->z && a->ldz < a->N) || (a->gate && a->ldgate < a->N) || (a->dz && a->lddz < a->N) || (a->dgate && a->lddg < a->N))
+  if (a->lddy < a->N || (a->gate && a->ldgate < a->N) || (a->dz && a->lddz < a->N) || (a->dgate && a->lddg < a->N))
     return fail(METIS_ERR_BAD_ARGUMENT, "a leading dimension is smaller than N = %lld", (long long)a->N);
   if (a->dbias && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_linear_pointwise_workspace_bytes(a->M, a->N)))
     return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   auto rows16 = [](const void* t, int64_t ld) { return !t || (aligned16(t) && ld % 8 == 0); };
   if (!rows16(a->dz, a->lddz)) return fail(METIS_ERR_BAD_ALIGNMENT, "dz must be 16-byte aligned with a leading dimension that is a multiple of 8");
-  for (const void* t : {a->dy, a->z, a->gate, static_cast<const void*>(a->dgate)})
+  for (const void* t : {a->dy, a->gate, static_cast<const void*>(a->dgate)})
     if (reinterpret_cast<uintptr_t>(t) & 1u) return fail(METIS_ERR_BAD_ALIGNMENT, "tensors must be 2-byte aligned");
-  const bool wide = a->N % 8 == 0 && rows16(a->dy, a->lddy) && rows16(a->z, a->ldz) && rows16(a->gate, a->ldgate) && rows16(a->dgate, a->lddg);
+  const bool wide = a->N % 8 == 0 && rows16(a->dy, a->lddy) && rows16(a->gate, a->ldgate) && rows16(a->dgate, a->lddg);
   const int64_t columns = ceil_div(a->N, 256);
   // with sums no more groups of rows than the workspace has; else about 16 blocks for each SM
   int64_t groups = ceil_div(a->M, 8), most = ceil_div((int64_t)device_sm_count() * 16, columns);
@@ -1252,13 +1282,7 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   if (groups > 65535) groups = 65535;
   float* sums = a->dbias ? static_cast<float*>(a->workspace) : nullptr;
   const dim3 grid((unsigned)columns, (unsigned)groups);
-  int32_t rc = METIS_OK;
-  switch (a->activation) {
-    case METIS_ACT_SILU: rc = launch_pointwise<METIS_ACT_SILU>(a, wide, grid, sums); break;
-    case METIS_ACT_GELU: rc = launch_pointwise<METIS_ACT_GELU>(a, wide, grid, sums); break;
-    case METIS_ACT_GELU_TANH: rc = launch_pointwise<METIS_ACT_GELU_TANH>(a, wide, grid, sums); break;
-    default: rc = launch_pointwise<METIS_ACT_NONE>(a, wide, grid, sums);
-  }
+  const int32_t rc = launch_pointwise(a, wide, grid, sums);
   if (rc || !a->dbias) return rc;
   const dim3 blocks((unsigned)ceil_div(a->N, 256));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);

@@ -111,18 +111,19 @@ variable_list once(variable_list grads) {
 
 // ---- linear -------------------------------------------------------------------------------------------------------
 
-struct LinearResult { Tensor y, z; };
+struct LinearResult { Tensor y, act, slope; };
 
-LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& gate, const Tensor& residual, int64_t act, bool keep_z) {
+LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& gate, const Tensor& residual, int64_t act, bool keep_act, bool keep_slope) {
   c10::OptionalDeviceGuard guard(x.device());
   Rows rx(x), rw(w);
   operand(x, rx);
   operand(w, rw);
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = rw.rows;
-  // (z is nobody else's: rows of whole 16-byte pieces)
-  const int64_t z_pitch = (rw.rows + 7) / 8 * 8;
-  LinearResult out{empty_like_options(x, shape, at::kBFloat16), keep_z ? empty_like_options(x, {rx.rows, z_pitch}, at::kBFloat16) : Tensor()};
+  // (what the gradients need is nobody else's: rows of whole 16-byte pieces)
+  const int64_t pitch = (rw.rows + 7) / 8 * 8;
+  LinearResult out{empty_like_options(x, shape, at::kBFloat16), keep_act ? empty_like_options(x, {rx.rows, pitch}, at::kBFloat16) : Tensor(),
+                   keep_slope ? empty_like_options(x, {rx.rows, pitch}, at::kHalf) : Tensor()};
   if (rx.rows == 0) return out;
   metis_linear_args a = {};
   a.M = rx.rows; a.N = rw.rows; a.K = rx.cols;
@@ -133,7 +134,8 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
   if (gate.defined()) { a.gate = gate.data_ptr(); a.ldgate = Rows(gate).ld; }
   if (residual.defined()) { a.residual = residual.data_ptr(); a.ldr = Rows(residual).ld; }
   a.y = out.y.data_ptr(); a.ldy = a.N;
-  a.z = ptr(out.z); a.ldz = z_pitch;
+  a.act = ptr(out.act); a.ldact = pitch;
+  a.slope = ptr(out.slope); a.ldslope = pitch;
   a.stream = stream_of(x);
   check(lib.metis_linear(&a), "metis_linear");
   return out;
@@ -155,8 +157,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const Tensor b = bias.value_or(Tensor()), g = gate.value_or(Tensor());
     const bool through = x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad());
     const bool gated = g.defined() && g.requires_grad();
-    const LinearResult out = linear_forward(x, weight, b, g, residual.value_or(Tensor()), act, gated || (act != METIS_ACT_NONE && through));
-    ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), x.requires_grad() ? weight : Tensor(), through ? g : Tensor(), out.z});
+    const LinearResult out = linear_forward(x, weight, b, g, residual.value_or(Tensor()), act, gated, act != METIS_ACT_NONE && through);
+    ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), x.requires_grad() ? weight : Tensor(), through ? g : Tensor(), out.act, out.slope});
     ctx->saved_data["s"] = std::vector<int64_t>{act, bias.has_value(), gate.has_value(), residual.has_value(),
                                                 b.defined() && b.scalar_type() == at::kFloat, weight.size(0), weight.size(1)};
     ctx->saved_data["x"] = x.sizes().vec();
@@ -206,8 +208,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           metis_linear_pointwise_args a = {};
           a.M = M; a.N = N;
           a.dy = dy.data_ptr(); a.lddy = rdy.ld;
-          a.activation = (int32_t)act;
-          if (saved[3].defined()) { a.z = saved[3].data_ptr(); a.ldz = saved[3].size(1); }
+          if (saved[3].defined()) { a.act = saved[3].data_ptr(); a.ldact = saved[3].size(1); }
+          if (saved[4].defined()) { a.slope = saved[4].data_ptr(); a.ldslope = saved[4].size(1); }
           if (saved[2].defined()) { a.gate = saved[2].data_ptr(); a.ldgate = Rows(saved[2]).ld; }
           if (write_dz) {
             const int64_t pitch = (N + 7) / 8 * 8;
@@ -365,7 +367,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
       y = LinearFunction::apply(x, w, given(bias), given(gate), given(residual), act);
     } else {
-      y = linear_forward(x, w, bias, gate, residual, act, false).y;
+      y = linear_forward(x, w, bias, gate, residual, act, false, false).y;
     }
   }
   return THPVariable_Wrap(y);

@@ -85,13 +85,17 @@ __device__ __forceinline__ void load_row8(const __nv_bfloat16* src, bool vec, in
     }
   }
 }
-__device__ __forceinline__ void store_row8(__nv_bfloat16* dst, bool vec, int apart, int64_t left, const float (&v)[8]) {
+__device__ __forceinline__ void store_words8(unsigned short* dst, bool vec, int apart, int64_t left, const uint32_t (&w)[4]) {
   if (vec && left >= 8) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i * apart < left) dst[i * apart] = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 8; ++i) if (i * apart < left) dst[i * apart] = (unsigned short)(w[i >> 1] >> ((i & 1) * 16));
   }
+}
+__device__ __forceinline__ void store_row8(__nv_bfloat16* dst, bool vec, int apart, int64_t left, const float (&v)[8]) {
+  const uint32_t w[4] = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+  store_words8(reinterpret_cast<unsigned short*>(dst), vec, apart, left, w);
 }
 
 // One stage's MMAs: D[128 weight rows, bn tokens] += weights [128, 64] tokens [bn, 64]^T.  A tile of fewer than 128 rows reads what lies
@@ -217,7 +221,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   // The eight lie together where rows are 16-byte aligned, else an item apart, so that neighbouring lanes have neighbouring elements.
   const int tokens = p.M - m0 < sh.bn ? (int)(p.M - m0) : sh.bn;
   const int shift = sh.rows == 128 ? 4 : sh.rows == 64 ? 3 : 2;        // log2 of the items of a token
-  const bool wide = p.d_wide && (!p.z || p.z_wide) && (!p.gate || p.gate_wide) && (!p.residual || p.residual_wide);
+  const bool wide = p.d_wide && (!p.gate || p.gate_wide) && (!p.residual || p.residual_wide);
   const int apart = wide ? 1 : 1 << shift, first = wide ? 8 : 1;
   const uint32_t mine = smem_u32(partial);
   constexpr int kFly = 4;
@@ -262,8 +266,14 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           if (i * apart < left) v[i] += p.bias_f32 ? static_cast<const float*>(p.bias)[c] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[c]);
         }
       }
-      if (p.z) store_row8(p.z + m * p.ldz + n, wide, apart, left, v);
-      activate_all(p.act, v);
+      if (p.slope) {
+        uint32_t slopes[4];
+        activate_both_all(p.act, v, slopes);
+        store_words8(reinterpret_cast<unsigned short*>(p.slope) + m * p.ldslope + n, wide, apart, left, slopes);
+      } else {
+        activate_all(p.act, v);
+      }
+      if (p.act_out) store_row8(p.act_out + m * p.ldact + n, wide, apart, left, v);
       if (p.gate) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[2 * i] *= bf16_lo(gate[k][i]); v[2 * i + 1] *= bf16_hi(gate[k][i]); }

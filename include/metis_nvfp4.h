@@ -454,12 +454,14 @@ int32_t metis_silu_mul(const void* gate, const void* up, void* out, int64_t n, v
 int64_t metis_dense_launches(void);
 
 /*
- * y = act(x W^T + bias) * gate + residual, x [M, K], W [N, K], y [M, N], all bf16, sums in fp32, one rounding at the end.
- * bias (bf16 or fp32 [N]), gate and residual ([M, N]) may be null; z, where given, receives bf16(x W^T + bias), from which
- * metis_linear_pointwise forms the gradients.  x and w: 16-byte aligned rows (leading dimensions multiples of 8), K a
- * multiple of 8; the others any, 16-byte aligned rows being the fast ones (rows that begin elsewhere are read by the aligned 16
- * bytes that hold them: up to 14 bytes beside a tensor are read, and not used; device allocations are whole 256 bytes).  What nn.Linear and the elementwise kernels behind
- * it do for a projection that replace_linear_with_metis leaves as it is (src/grpo/grpo.py:119-196, target_modules).
+ * y = act(z) * gate + residual with z = x W^T + bias, x [M, K], W [N, K], y [M, N], all bf16, sums in fp32, one rounding at
+ * the end.  bias (bf16 or fp32 [N]), gate and residual ([M, N]) may be null.  For metis_linear_pointwise, each optional:
+ * act [M, N] receives bf16(act(z)), what the gate's gradient needs; slope [M, N] receives fp16(2^15 act'(z)), what the others
+ * need where there is an activation (16 bits of z itself would cost the gradients as much again as their own rounding).
+ * x, w, act and slope: 16-byte aligned rows (leading dimensions multiples of 8), K a multiple of 8; the others any, 16-byte
+ * aligned rows being the fast ones (rows that begin elsewhere are read by the aligned 16 bytes that hold them: up to 14 bytes
+ * beside a tensor are read, and not used; device allocations are whole 256 bytes).  What nn.Linear and the elementwise kernels
+ * behind it do for a projection that replace_linear_with_metis leaves as it is (src/grpo/grpo.py:119-196, target_modules).
  */
 typedef struct metis_linear_args {
   int64_t M, N, K;
@@ -470,7 +472,8 @@ typedef struct metis_linear_args {
   const void* gate;      int64_t ldgate;
   const void* residual;  int64_t ldr;
   void* y;  int64_t ldy;
-  void* z;  int64_t ldz;
+  void* act;    int64_t ldact;
+  void* slope;  int64_t ldslope;
   int32_t* status;          /* optional device int32: 0, or a METIS_DEV_* code */
   void* stream;
 } metis_linear_args;
@@ -478,18 +481,19 @@ int32_t metis_linear(const metis_linear_args* args);
 
 /*
  * Gradients through that epilogue: dz = bf16(dy * gate * act'(z)), dgate = bf16(dy * act(z)), dbias = sum over rows of
- * dy * gate * act'(z) in fp32, rounded once.  Each output may be null; gate null: 1.  z is not read where neither the
- * activation nor dgate needs it.  dz has 16-byte aligned rows.  The workspace is for dbias alone.
+ * dy * gate * act'(z) in fp32, rounded once.  Each output may be null; gate null: 1; slope null: 1 (no activation).  act is read
+ * for dgate alone.  dz, act and slope have 16-byte aligned rows.  The workspace is for dbias alone.
  */
 typedef struct metis_linear_pointwise_args {
   int64_t M, N;
   const void* dy;    int64_t lddy;
-  const void* z;     int64_t ldz;
+  const void* act;   int64_t ldact;
+  const void* slope; int64_t ldslope;
   const void* gate;  int64_t ldgate;
   void* dz;     int64_t lddz;
   void* dgate;  int64_t lddg;
   void* dbias;  int32_t dbias_dtype;
-  int32_t activation;
+  int32_t reserved;
   void* workspace;  int64_t workspace_bytes;
   void* stream;
 } metis_linear_pointwise_args;

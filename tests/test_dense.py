@@ -40,26 +40,31 @@ def test_linear_refuses_bad_parts_of_the_epilogue(L, p):
     assert L.metis_linear(linear_args(p, w=p + 8)) == -3
     assert L.metis_linear(linear_args(p, bias=p, bias_dtype=7)) == -1
     assert L.metis_linear(linear_args(p, y=p + 1)) == -3 and L.metis_linear(linear_args(p, bias=p + 2, bias_dtype=1)) == -3
-    for name, ld in (("gate", "ldgate"), ("residual", "ldr"), ("z", "ldz")):
+    for name, ld in (("gate", "ldgate"), ("residual", "ldr")):
         assert L.metis_linear(linear_args(p, **{name: p + 1, ld: 24})) == -3
         assert L.metis_linear(linear_args(p, **{name: p, ld: 23})) == -1
+    for name, ld in (("act", "ldact"), ("slope", "ldslope")):                         # rows of 16-byte pieces
+        for at, pitch in ((p + 2, 24), (p + 8, 24), (p, 16), (p, 28)):
+            assert L.metis_linear(linear_args(p, activation=1, **{name: at, ld: pitch})) == -3
+    assert L.metis_linear(linear_args(p, activation=0, slope=p, ldslope=24)) == -1    # nothing that has a slope
 
 
 def test_pointwise_refuses(L, p):
     def call(**changes):
-        a = cabi.LinearPointwiseArgs(M=4, N=24, dy=p, lddy=24, z=p, ldz=24, dz=p, lddz=24, activation=1)
+        a = cabi.LinearPointwiseArgs(M=4, N=24, dy=p, lddy=24, act=p, ldact=24, slope=p, ldslope=24, dz=p, lddz=24)
         for k, v in changes.items():
             setattr(a, k, v)
         return L.metis_linear_pointwise(a)
     assert L.metis_linear_pointwise(None) == -1
-    assert call(M=0) == -2 and call(N=-1) == -2 and call(dy=None) == -1 and call(dz=None) == -1 and call(z=None) == -1
-    assert call(activation=9) == -1 and call(lddy=8) == -1 and call(lddz=8) == -1 and call(gate=p, ldgate=8) == -1 and call(dgate=p, lddg=2) == -1
+    assert call(M=0) == -2 and call(N=-1) == -2 and call(dy=None) == -1 and call(dz=None) == -1
+    assert call(act=p + 2) == -3 and call(ldact=20) == -3 and call(slope=p + 8) == -3 and call(ldslope=16) == -3
+    assert call(lddy=8) == -1 and call(lddz=8) == -1 and call(gate=p, ldgate=8) == -1 and call(dgate=p, lddg=2) == -1
     assert call(dbias=p, dbias_dtype=5) == -1
     assert call(dz=p + 2) == -3 and call(lddz=28) == -3 and call(dy=p + 1) == -3          # dz is an operand of the products behind it
     assert call(dbias=p, dbias_dtype=0) == -4                                        # no workspace
     assert call(dbias=p, dbias_dtype=0, workspace=p, workspace_bytes=16) == -4
     assert call(dbias=p, dbias_dtype=0, workspace=p + 4, workspace_bytes=1 << 30) == -4
-    assert call(activation=0, z=None, dgate=p, lddg=24) == -1                        # the gate's gradient needs z
+    assert call(act=None, dgate=p, lddg=24) == -1                                    # the gate's gradient needs act(z)
 
 
 def test_product_refuses(L, p):

@@ -2,7 +2,7 @@
 
 Tolerances count roundings: a bf16 output is off by at most half a step, 2^-8 of its value; sums of K products in fp32 by at most
 K 2^-23 of the sum of their magnitudes (each addition rounds or cuts at 2^-23 of what it adds up to); gradients that pass through a bf16
-intermediate (dz, the logits' gradient, the z that act' is taken at) by 2^-8 for each, independent from element to element, so that the
+intermediate (dz, the logits' gradient, act(z) where the gate has a gradient) by 2^-8 for each, independent from element to element, so that the
 2-norm of a product's error is that part of its norm."""
 import math
 
@@ -81,7 +81,7 @@ def check_linear(M, N, K, act=None, bias=None, gate=False, residual=False, grad=
         exact = torch.autograd.grad(want, [t for t in copies if t is not None], dy.double().reshape(-1, N))
         for t, got, ref in zip(leaves, grads, exact):
             assert got.shape == t.shape and got.dtype == t.dtype
-            # its own rounding, that of dz and that of z
+            # its own rounding, that of dz or act(z), and less than another of the slope's
             assert rel(got.reshape(ref.shape), ref) <= 3 * STEP, (tuple(t.shape), rel(got.reshape(ref.shape), ref))
         if residual:
             assert torch.equal(grads[-1], dy)
@@ -129,6 +129,44 @@ def test_linear_of_no_rows():
     assert y.shape == (0, 24)
     gx, gw, gb, gr = torch.autograd.grad(y, (x, w, b, r), torch.empty_like(y))
     assert gx.shape == x.shape and gr.shape == r.shape and not gw.any() and not gb.any()
+
+
+def test_linear_gradients_take_two_roundings():
+    """Roundings of one type that fall independently add by squares: a gradient that rounds an intermediate to bf16 (dz, act(z)) and then
+    itself is sqrt(2) = 1.41 times as far from the exact one as bf16 has to be.  Slopes in 16 bits with ten of mantissa add 1/64 of that square; a
+    z in bf16 instead would take the erf form's to 1.6."""
+    for act in ("silu", "gelu", "gelu_tanh"):
+        for M, N, K in ((512, 1000, 192), (24, 1001, 192)):                               # CTA pairs; few tokens and odd rows
+            x, w, dy, g = normal(M, K), normal(N, K, scale=K ** -0.5, seed=1), normal(M, N, seed=2), normal(M, N, seed=3)
+            for gate in (None, g):
+                leaves = [t.clone().requires_grad_(True) for t in (x, w) + ((gate,) if gate is not None else ())]
+                y = dense.linear(*leaves[:2], activation=act, gate=leaves[2] if gate is not None else None)
+                got = torch.autograd.grad(y, leaves, dy)
+                copies = [t.detach().double().requires_grad_(True) for t in leaves]
+                out = act64(act, copies[0] @ copies[1].t())
+                exact = torch.autograd.grad(out * copies[2] if gate is not None else out, copies, dy.double())
+                for a, e in zip(got, exact):
+                    off, least = (a.double() - e).norm(), (e.bfloat16().double() - e).norm()
+                    assert off <= 1.5 * least, (act, M, gate is not None, float(off / least))
+
+
+def test_linear_slopes_of_far_values():
+    """Where the slope is small it keeps its relative accuracy: fp16 with 2^15 in front is normal down to 2^-29 (silu at z = -22)."""
+    for M in (8, 512):
+        z = torch.linspace(-20, -10, M, device="cuda", dtype=torch.float64).bfloat16()
+        x = torch.zeros(M, 8, device="cuda", dtype=torch.bfloat16)
+        x[:, 0] = z
+        w = torch.zeros(264, 8, device="cuda", dtype=torch.bfloat16)
+        w[:, 0] = 1
+        x.requires_grad_(True)
+        dy = torch.zeros(M, 264, device="cuda", dtype=torch.bfloat16)
+        dy[:, 7] = 1
+        got, = torch.autograd.grad(dense.linear(x, w, activation="silu"), x, dy)
+        z = z.double()
+        p = torch.sigmoid(z)
+        want = p * (1 + z * (1 - p))
+        # two roundings to bf16, one to fp16; 1 + z (1 - p) and the logistic function in fp32: a few parts in 2^20
+        assert ((got[:, 0].double() - want) / want).abs().max() <= 2 * 2.0 ** -8 + 2.0 ** -11
 
 
 def test_linear_gradients_of_some_inputs_only():
