@@ -635,7 +635,17 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : pack_bf16(g[2 * i], g[2 * i + 1]);
-            store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+            if (p.two_parts) {
+              uint32_t low[16];                            // (what is left of an infinity is nothing)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float a = g[2 * i] - bf16_lo(w[i]), c = g[2 * i + 1] - bf16_hi(w[i]);
+                low[i] = dead ? 0u : pack_bf16(fabsf(a) < INFINITY ? a : 0.0f, fabsf(c) < INFINITY ? c : 0.0f);
+              }
+              store_two_tma(st, &map_d, w, &map_s, low, (int32_t)col0, (int32_t)row0);
+            } else {
+              store_piece_tma(st, &map_d, w, (int32_t)col0, (int32_t)row0);
+            }
           }
           if constexpr (kEpi == kEpiSum || kEpi == kEpiSumF32) {
             float g[32];
@@ -869,10 +879,20 @@ head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, c
   }
 }
 
-// d[m] = alpha times the sum over the splits of row place_of[m] of the sums (m itself where there is no place_of), in bf16; zeros for a place of -1.  A thread takes eight
-// columns of a row.
+// The rows of h twice, `half` apart and zeros between: what a gradient of two parts is contracted with.
 __global__ void __launch_bounds__(256)
-finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M, int pieces, const int32_t* place_of, const float* gout, const float* inv_count,
+head_stack_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int half, int pieces, __nv_bfloat16* out) {
+  grid_dependency_wait();
+  for (int e = blockIdx.x * 256 + threadIdx.x; e < 2 * half * pieces; e += gridDim.x * 256) {
+    const int i = e / pieces, k = e - i * pieces, m = i < half ? i : i - half;
+    reinterpret_cast<uint4*>(out)[e] = m < M ? reinterpret_cast<const uint4*>(h + m * ldh)[k] : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// d[m] = alpha times the sum over the splits of row place_of[m] of the sums (m itself where there is no place_of) and of the row `half` behind
+// it (0: none), in bf16; zeros for a place of -1.  A thread takes eight columns of a row.
+__global__ void __launch_bounds__(256)
+finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M, int pieces, const int32_t* place_of, int64_t half, const float* gout, const float* inv_count,
                    float scale, __nv_bfloat16* d, int64_t ldd) {
   grid_dependency_wait();
   const float alpha = gout ? common_weight(gout, inv_count, scale) : 1.0f;
@@ -887,6 +907,11 @@ finish_sums_kernel(const float* sums, int splits, int64_t split_rows, int64_t M,
         const float4 x = at[0], y = at[1];
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
         v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+        if (half) {
+          const float4 z = at[half * (ld / 4)], u = at[half * (ld / 4) + 1];
+          v[0] += z.x; v[1] += z.y; v[2] += z.z; v[3] += z.w;
+          v[4] += u.x; v[5] += u.y; v[6] += u.z; v[7] += u.w;
+        }
       }
     }
 #pragma unroll
@@ -1293,8 +1318,8 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   return METIS_OK;
 }
 
-static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64_t N, const int32_t* place_of, const CommonWeight& weight, __nv_bfloat16* d, int64_t ldd, cudaStream_t st) {
-  METIS_CUDA_OK(launch_counted(kLaunchStream, finish_sums_kernel, dim3(row_blocks(ceil_div(M * N, 256))), dim3(256), 0, st, sums, (int)sp.splits, sp.rows, M, (int)(N / 8), place_of, weight.gout, weight.inv_count, weight.scale, d, ldd));
+static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64_t N, const int32_t* place_of, int64_t half, const CommonWeight& weight, __nv_bfloat16* d, int64_t ldd, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchStream, finish_sums_kernel, dim3(row_blocks(ceil_div(M * N, 256))), dim3(256), 0, st, sums, (int)sp.splits, sp.rows, M, (int)(N / 8), place_of, half, weight.gout, weight.inv_count, weight.scale, d, ldd));
   return METIS_OK;
 }
 
@@ -1329,7 +1354,7 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (!workspace || !aligned16(workspace) || workspace_bytes < sp.bytes) return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   float* sums = static_cast<float*>(workspace);
   if (int32_t rc = dense_sum(oa, ob, M, N, K, nullptr, 0, status, st, nullptr, &sp, sums)) return rc;
-  return finish_sums(sums, sp, M, N, nullptr, {}, static_cast<__nv_bfloat16*>(d), ldd, st);
+  return finish_sums(sums, sp, M, N, nullptr, 0, {}, static_cast<__nv_bfloat16*>(d), ldd, st);
 }
 
 // ---- head ---------------------------------------------------------------------------------------------------------
@@ -1437,20 +1462,29 @@ struct HeadBackward {
   HeadPack pack;
   int64_t columns;
   Splits sp;
-  __nv_bfloat16* g;
+  __nv_bfloat16 *g, *stacked;                              // stacked: h twice, for G in two parts
   float* sums;
+  int64_t half;                                            // rows from one part of G to the other; 0: it has one
   int64_t bytes;
 };
+// Up to so many rows G goes as two bf16 numbers, its value and what that leaves, one below the other; they are 17 bits of it, and the gradients
+// have their own rounding alone.  In one number a row's target, most of the row, is rounded once: over few rows that falls anywhere
+// up to 2^-8 of the gradient (2 rows of 1472 over 4931: 1.7 times as far off as the gradient's own rounding; over many it averages to 1.4).  Tiles
+// have 256 rows, so the second part costs a stage of the contraction over the rows and G's bytes.
+constexpr int64_t kTwoPartRows = 128;
 static HeadBackward plan_head_backward(int64_t M, int64_t V, int64_t K, void* at) {
   HeadBackward b = {};
   b.pack = head_pack(M, V, K, at);
-  b.columns = piece_columns(M, V);
-  b.sp = plan_splits(M, K, b.columns < V ? b.columns : V);
-  const bool summed = b.pack.on || b.columns < V || b.sp.splits > 1;
-  const int64_t g_bytes = ceil_div(2 * M * b.columns, 256) * 256;
+  b.half = M <= kTwoPartRows && !b.pack.on ? ceil_div(M, 8) * 8 : 0;
+  const int64_t rows = b.half ? 2 * b.half : M;
+  b.columns = piece_columns(rows, V);
+  b.sp = plan_splits(rows, K, b.columns < V ? b.columns : V);
+  const bool summed = b.half || b.pack.on || b.columns < V || b.sp.splits > 1;
+  const int64_t g_bytes = ceil_div(2 * rows * b.columns, 256) * 256, sum_bytes = summed ? ceil_div(b.sp.bytes, 256) * 256 : 0;
   b.g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(at) + b.pack.bytes);
   b.sums = summed ? reinterpret_cast<float*>(reinterpret_cast<char*>(b.g) + g_bytes) : nullptr;
-  b.bytes = b.pack.bytes + g_bytes + (summed ? b.sp.bytes : 0);
+  b.stacked = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(b.g) + g_bytes + sum_bytes);
+  b.bytes = b.pack.bytes + g_bytes + sum_bytes + (b.half ? 2 * rows * K : 0);
   return b;
 }
 
@@ -1477,16 +1511,23 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false};
   DenseParams p = head_params(a, pack);
   p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride;
+  p.two_parts = b.half > 0;
+  const int64_t rows = b.half ? 2 * b.half : a->M;         // of G
+  const DenseOperand of_dw = {b.half ? b.stacked : h.p, b.half ? a->K : h.ld, true};
+  if (b.half && dw)
+    METIS_CUDA_OK(launch_counted(kLaunchStream, head_stack_kernel, dim3(row_blocks(rows)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M, (int)b.half,
+                                 (int)(a->K / 8), b.stacked));
   const CommonWeight weight = gout_stride ? CommonWeight{} : CommonWeight{gout, inv_count, a->scale};
   for (int64_t v0 = 0; v0 < a->V; v0 += b.columns) {
     const int64_t n = a->V - v0 < b.columns ? a->V - v0 : b.columns;
-    CUtensorMap mg = {};
+    CUtensorMap mg = {}, ml = {};
     p.N = n;
     p.col0 = v0;
-    if (int32_t rc = map_bf16(&mg, b.g, b.columns, a->M, n, "G")) return rc;
-    if (int32_t rc = launch_dense<false, false, kEpiGrad>(h, {w + v0 * a->ldw, a->ldw, false}, mg, p, st)) return rc;
+    if (int32_t rc = map_bf16(&mg, b.g, b.columns, b.half ? b.half : a->M, n, "G")) return rc;
+    if (b.half) if (int32_t rc = map_bf16(&ml, b.g + b.half * b.columns, b.columns, b.half, n, "G")) return rc;
+    if (int32_t rc = launch_dense<false, false, kEpiGrad>(h, {w + v0 * a->ldw, a->ldw, false}, mg, p, st, ml)) return rc;
     if (dw) {
-      if (int32_t rc = dense_sum({b.g, b.columns, true}, {h.p, h.ld, true}, n, a->K, a->M, static_cast<__nv_bfloat16*>(dw) + v0 * lddw, lddw, a->status, st, p.live,
+      if (int32_t rc = dense_sum({b.g, b.columns, true}, of_dw, n, a->K, rows, static_cast<__nv_bfloat16*>(dw) + v0 * lddw, lddw, a->status, st, p.live,
                                  nullptr, nullptr, false, weight)) return rc;
     }
     if (dh) {
@@ -1494,9 +1535,9 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
       const int64_t stages = ceil_div(n, 64);
       Splits sp = b.sp;
       sp.splits = (int32_t)ceil_div(stages, sp.iters_per_split);
-      if (int32_t rc = dense_sum({b.g, b.columns, false}, {w + v0 * a->ldw, a->ldw, true}, a->M, a->K, n, b.sums ? nullptr : dh, lddh, a->status, st, p.live, &sp, b.sums, v0 > 0, weight)) return rc;
+      if (int32_t rc = dense_sum({b.g, b.columns, false}, {w + v0 * a->ldw, a->ldw, true}, rows, a->K, n, b.sums ? nullptr : dh, lddh, a->status, st, p.live, &sp, b.sums, v0 > 0, weight)) return rc;
     }
   }
-  if (dh && b.sums) return finish_sums(b.sums, b.sp, a->M, a->K, pack.on ? pack.place_of : nullptr, weight, static_cast<__nv_bfloat16*>(dh), lddh, st);
+  if (dh && b.sums) return finish_sums(b.sums, b.sp, a->M, a->K, pack.on ? pack.place_of : nullptr, b.half, weight, static_cast<__nv_bfloat16*>(dh), lddh, st);
   return METIS_OK;
 }

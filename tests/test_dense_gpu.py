@@ -263,6 +263,33 @@ def check_head(M, V, K, temperature=1.0, seed=0, ignored=0.2):
     check_head_gradients(back, exact, h64, w64, logits.detach(), g, t, temperature, tol)
 
 
+@pytest.mark.parametrize("M,V,K", [(1, 97, 64), (2, 4931, 1472), (54, 3225, 104), (64, 513, 72), (128, 700, 136), (129, 700, 136), (300, 1000, 264)])
+def test_roundings_of_the_heads_gradients(M, V, K):
+    """Up to 128 rows the logits' gradient goes as two bf16 numbers: the gradients have their own rounding, with 2^-9 of it from the second
+    number's.  Above that it goes as one: two roundings, which add by squares, sqrt(2)."""
+    h, w, t = head_inputs(M, V, K)
+    copies = [x.double().requires_grad_(True) for x in (h, w)]
+    leaves = [x.requires_grad_(True) for x in (h, w)]
+    g = normal(M, seed=7, dtype=torch.float32)
+    logp, _, logits = head64(*copies, t, 0.7)
+    for got, want, upstream in ((dense.token_logprobs(h, w, t, temperature=0.7), logp, g),
+                                (dense.linear_cross_entropy(h, w, t, temperature=0.7), -logp.sum() / (t != -100).sum(), torch.tensor(0.7, device="cuda"))):
+        grads = torch.autograd.grad(got, leaves, upstream)
+        exact = torch.autograd.grad(want, copies, upstream.double(), retain_graph=True)
+        for a, e in zip(grads, exact):
+            off, least = (a.double() - e).norm(), (e.bfloat16().double() - e).norm()
+            assert off <= (1.02 if M <= 128 else 1.5) * least, float(off / least)
+
+
+def test_ignored_rows_take_nothing_of_their_gradient():
+    h, w, t = head_inputs(70, 130, 64, 0.4)
+    leaves = [x.requires_grad_(True) for x in (h, w)]
+    g = normal(70, seed=9, dtype=torch.float32)
+    bad = torch.where(t == -100, float("nan"), g)
+    got = [torch.autograd.grad(dense.linear_cross_entropy(h, w, t, reduction="none"), leaves, x) for x in (g, bad)]
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and not got[0][0][t == -100].any()
+
+
 @pytest.mark.parametrize("M,V,K", [(1, 2, 8), (1, 97, 64), (3, 1, 8), (24, 97, 64), (16, 4099, 256), (33, 256, 72), (128, 257, 64), (129, 1000, 128), (257, 513, 1000),
                                    (300, 5003, 96), (1021, 777, 40), (2, 30001, 64), (64, 6000, 3584)])
 def test_losses_and_their_gradients(M, V, K):
