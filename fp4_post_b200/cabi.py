@@ -88,7 +88,7 @@ class LinearPointwiseArgs(C.Structure):
         ("dy", C.c_void_p), ("lddy", C.c_int64), ("act", C.c_void_p), ("ldact", C.c_int64), ("slope", C.c_void_p), ("ldslope", C.c_int64),
         ("gate", C.c_void_p), ("ldgate", C.c_int64),
         ("dz", C.c_void_p), ("lddz", C.c_int64), ("dgate", C.c_void_p), ("lddg", C.c_int64),
-        ("dbias", C.c_void_p), ("dbias_dtype", C.c_int32), ("reserved", C.c_int32),
+        ("dbias", C.c_void_p), ("dbias_dtype", C.c_int32), ("half", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("stream", C.c_void_p),
     ]
 
@@ -195,9 +195,9 @@ def lib() -> C.CDLL:
     L.metis_linear_pointwise_workspace_bytes.restype = i64
     L.metis_linear_pointwise.argtypes = [C.POINTER(LinearPointwiseArgs)]
     L.metis_linear_pointwise.restype = i32
-    L.metis_bf16_product_workspace_bytes.argtypes = [i64, i64, i64, i32]
+    L.metis_bf16_product_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
     L.metis_bf16_product_workspace_bytes.restype = i64
-    L.metis_bf16_product.argtypes = [vp, i32, i64, vp, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp]
+    L.metis_bf16_product.argtypes = [vp, i32, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp]
     L.metis_bf16_product.restype = i32
     L.metis_head_loss_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.metis_head_loss_workspace_bytes.restype = i64

@@ -37,7 +37,7 @@ struct DenseParams {
   const float* lse;                                        // [M]
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss (stride 1), or of all, times *inv_count (null: 1)
   const float* inv_count;
-  int32_t two_parts;                                       // the logits' gradient leaves as two bf16 numbers, by maps of their own
+  int32_t half, half_rows;                                 // rows in two parts of bf16, so far apart (0: one part), and how many of each are rows
   // sum of pieces: fp32 addend.  With `splits` > 1 each split of the contraction has sums of its own, [splits, split_rows, N]
   const float* c;  int64_t ldc;
   int32_t splits, iters_per_split;

@@ -635,7 +635,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = dead ? 0u : pack_bf16(g[2 * i], g[2 * i + 1]);
-            if (p.two_parts) {
+            if (p.half) {
               uint32_t low[16];                            // (what is left of an infinity is nothing)
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -879,13 +879,13 @@ head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, c
   }
 }
 
-// The rows of h twice, `half` apart and zeros between: what a gradient of two parts is contracted with.
+// The rows of x twice, `half` apart and zeros between: what a gradient of two parts is contracted with.
 __global__ void __launch_bounds__(256)
-head_stack_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int half, int pieces, __nv_bfloat16* out) {
+stack_rows_kernel(const __nv_bfloat16* x, int64_t ldx, int64_t M, int64_t half, int64_t pieces, __nv_bfloat16* out) {
   grid_dependency_wait();
-  for (int e = blockIdx.x * 256 + threadIdx.x; e < 2 * half * pieces; e += gridDim.x * 256) {
-    const int i = e / pieces, k = e - i * pieces, m = i < half ? i : i - half;
-    reinterpret_cast<uint4*>(out)[e] = m < M ? reinterpret_cast<const uint4*>(h + m * ldh)[k] : make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < 2 * half * pieces; e += (int64_t)gridDim.x * 256) {
+    const int64_t i = e / pieces, k = e - i * pieces, m = i < half ? i : i - half;
+    reinterpret_cast<uint4*>(out)[e] = m < M ? reinterpret_cast<const uint4*>(x + m * ldx)[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -1006,7 +1006,7 @@ template <bool kWide>
 __global__ void __launch_bounds__(256)
 linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __half* slope, int64_t lds, const __nv_bfloat16* act, int64_t lda,
                         const __nv_bfloat16* gate, int64_t ldgate, int64_t M, int64_t N,
-                        __nv_bfloat16* dz, int64_t lddz, __nv_bfloat16* dgate, int64_t lddg,
+                        __nv_bfloat16* dz, int64_t lddz, int64_t half, __nv_bfloat16* dgate, int64_t lddg,
                         float* sums) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1016,11 +1016,11 @@ linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __half* slo
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-  for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < M; row += (int64_t)gridDim.y * 8) {
+  for (int64_t row = (int64_t)blockIdx.y * 8 + warp; row < (half ? half : M); row += (int64_t)gridDim.y * 8) {
     float d[8], a[8], out[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { d[i] = 0.0f; a[i] = 0.0f; }
-    if (left > 0) {
+    for (int i = 0; i < 8; ++i) { d[i] = 0.0f; a[i] = 0.0f; out[i] = 0.0f; }
+    if (left > 0 && row < M) {
       float g[8];
       uint4 s;
       load8_any<kWide>(dy + row * lddy + col, left, d);
@@ -1035,14 +1035,23 @@ linear_pointwise_kernel(const __nv_bfloat16* dy, int64_t lddy, const __half* slo
         a[i] *= d[i];
         acc[i] += out[i];
       }
-      if (dz) {
-        __nv_bfloat16* to = dz + row * lddz + col;
-        if (kWide || left >= 8) *reinterpret_cast<uint4*>(to) = pack8(out);
-        else for (int i = 0; i < left; ++i) to[i] = __float2bfloat16_rn(out[i]);
-      }
-      if (kWide && dgate) *reinterpret_cast<uint4*>(dgate + row * lddg + col) = pack8(a);
     }
-    if (!kWide && dgate) store_run(dgate + row * lddg + col0, count, s_run[warp], a);
+    if (left > 0) {
+      for (int part = 0; dz && part < (half ? 2 : 1); ++part) {
+        __nv_bfloat16* to = dz + (part * half + row) * lddz + col;
+        const uint4 q = pack8(out);
+        if (kWide || left >= 8) *reinterpret_cast<uint4*>(to) = q;
+        else for (int i = 0; i < left; ++i) to[i] = __float2bfloat16_rn(out[i]);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                      // what the first part leaves (of an infinity nothing)
+          const float r = out[i] - (i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]));
+          out[i] = fabsf(r) < INFINITY ? r : 0.0f;
+        }
+      }
+      if (kWide && dgate && row < M) *reinterpret_cast<uint4*>(dgate + row * lddg + col) = pack8(a);
+    }
+    if (!kWide && dgate && row < M) store_run(dgate + row * lddg + col0, count, s_run[warp], a);
   }
   if (sums) {
     __shared__ float s_sum[8][256];
@@ -1263,6 +1272,8 @@ extern "C" int32_t metis_linear(const metis_linear_args* a) {
   return launch_dense<false, false, kEpiLinear>(x, w, md, p, st);
 }
 
+static bool half_ok(int32_t half, int64_t rows) { return half % 8 == 0 && half >= rows && half <= METIS_TWO_PART_ROWS; }
+
 constexpr int kPointwiseGroups = 64;
 extern "C" int64_t metis_linear_pointwise_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
@@ -1275,7 +1286,7 @@ static int32_t launch_pointwise(const metis_linear_pointwise_args* a, bool wide,
                              static_cast<const __nv_bfloat16*>(a->dy), a->lddy, static_cast<const __half*>(a->slope), a->ldslope,
                              static_cast<const __nv_bfloat16*>(a->act), a->ldact,
                              static_cast<const __nv_bfloat16*>(a->gate), a->ldgate, a->M, a->N, static_cast<__nv_bfloat16*>(a->dz), a->lddz,
-                             static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
+                             (int64_t)(a->dz ? a->half : 0), static_cast<__nv_bfloat16*>(a->dgate), a->lddg, sums);
   };
   METIS_CUDA_OK(wide ? launch(linear_pointwise_kernel<true>) : launch(linear_pointwise_kernel<false>));
   return METIS_OK;
@@ -1299,9 +1310,10 @@ extern "C" int32_t metis_linear_pointwise(const metis_linear_pointwise_args* a) 
   for (const void* t : {a->dy, a->gate, static_cast<const void*>(a->dgate)})
     if (reinterpret_cast<uintptr_t>(t) & 1u) return fail(METIS_ERR_BAD_ALIGNMENT, "tensors must be 2-byte aligned");
   const bool wide = a->N % 8 == 0 && rows16(a->dy, a->lddy) && rows16(a->gate, a->ldgate) && rows16(a->dgate, a->lddg);
+  if (a->half && !half_ok(a->half, a->M)) return fail(METIS_ERR_BAD_ARGUMENT, "half = %d must be a multiple of 8 from M = %lld to 128", a->half, (long long)a->M);
   const int64_t columns = ceil_div(a->N, 256);
   // with sums no more groups of rows than the workspace has; else about 16 blocks for each SM
-  int64_t groups = ceil_div(a->M, 8), most = ceil_div((int64_t)device_sm_count() * 16, columns);
+  int64_t groups = ceil_div(a->half ? a->half : a->M, 8), most = ceil_div((int64_t)device_sm_count() * 16, columns);
   if (a->dbias && most > kPointwiseGroups) most = kPointwiseGroups;
   if (groups > most) groups = most;
   if (groups > 65535) groups = 65535;
@@ -1323,16 +1335,22 @@ static int32_t finish_sums(const float* sums, const Splits& sp, int64_t M, int64
   return METIS_OK;
 }
 
-extern "C" int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+extern "C" int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major, int32_t half) {
+  if (M <= 0 || N <= 0 || K <= 0 || half < 0) return 0;
+  if (half) (a_mn_major ? K : M) = 2 * half;
   SmallShape sh;
   if (!a_mn_major && few_tokens(M, N, K, true, &sh)) return 0;
   const Splits sp = plan_splits(M, N, K);
-  return sp.splits > 1 ? sp.bytes : 0;
+  return (sp.splits > 1 || (half && !a_mn_major) ? sp.bytes : 0) + (half && a_mn_major ? 4 * (int64_t)half * N : 0);
+}
+
+static int32_t stack_rows(const __nv_bfloat16* x, int64_t ldx, int64_t M, int64_t half, int64_t K, __nv_bfloat16* out, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchStream, stack_rows_kernel, dim3(row_blocks(ceil_div(2 * half * (K / 8), 32))), dim3(256), 0, st, x, ldx, M, half, K / 8, out));
+  return METIS_OK;
 }
 
 extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
-                                      void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+                                      int32_t half, void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   if (int32_t rc = check_extent(M, "M")) return rc;
   if (int32_t rc = check_extent(N, "N")) return rc;
   if (int32_t rc = check_extent(K, "K")) return rc;
@@ -1340,21 +1358,34 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   if (int32_t rc = check_rows(b, ldb, N, "b")) return rc;
   if (int32_t rc = check_rows(d, ldd, N, "d")) return rc;
   if (N % 8 != 0) return fail(METIS_ERR_BAD_SHAPE, "N = %lld must be a multiple of 8", (long long)N);
+  if (half && !half_ok(half, a_mn_major ? K : M)) return fail(METIS_ERR_BAD_ARGUMENT, "half = %d must be a multiple of 8 from the rows' number to 128", half);
+  const int64_t rows = a_mn_major ? K : M;
+  if (half) (a_mn_major ? K : M) = 2 * half;
   SmallShape sh;
   if (!a_mn_major && few_tokens(M, N, K, true, &sh)) {
     DenseParams p = {};
     p.M = M; p.N = N; p.K = K; p.status = status;
+    p.half = half; p.half_rows = (int32_t)(half ? rows : 0);
     p.d = static_cast<__nv_bfloat16*>(d); p.ldd = ldd; p.d_wide = 1;
     return launch_dense_small(sh, a, lda, b, true, ldb, p, reinterpret_cast<cudaStream_t>(stream));
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const Splits sp = plan_splits(M, N, K);
-  const DenseOperand oa = {a, lda, a_mn_major != 0}, ob = {b, ldb, true};
-  if (sp.splits == 1) return dense_sum(oa, ob, M, N, K, d, ldd, status, st);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < sp.bytes) return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
+  const DenseOperand oa = {a, lda, a_mn_major != 0};
+  DenseOperand ob = {b, ldb, true};
+  const bool summed = sp.splits > 1 || (half && !a_mn_major);
+  const int64_t sum_bytes = summed ? sp.bytes : 0, stack_bytes = half && a_mn_major ? 4 * (int64_t)half * N : 0;
+  if (sum_bytes + stack_bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < sum_bytes + stack_bytes))
+    return fail(METIS_ERR_WORKSPACE, "workspace too small or misaligned");
   float* sums = static_cast<float*>(workspace);
+  if (stack_bytes) {
+    __nv_bfloat16* stacked = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(workspace) + sum_bytes);
+    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(b), ldb, rows, half, N, stacked, st)) return rc;
+    ob = {stacked, N, true};
+  }
+  if (!summed) return dense_sum(oa, ob, M, N, K, d, ldd, status, st);
   if (int32_t rc = dense_sum(oa, ob, M, N, K, nullptr, 0, status, st, nullptr, &sp, sums)) return rc;
-  return finish_sums(sums, sp, M, N, nullptr, 0, {}, static_cast<__nv_bfloat16*>(d), ldd, st);
+  return finish_sums(sums, sp, a_mn_major ? M : rows, N, nullptr, a_mn_major ? 0 : half, {}, static_cast<__nv_bfloat16*>(d), ldd, st);
 }
 
 // ---- head ---------------------------------------------------------------------------------------------------------
@@ -1467,15 +1498,11 @@ struct HeadBackward {
   int64_t half;                                            // rows from one part of G to the other; 0: it has one
   int64_t bytes;
 };
-// Up to so many rows G goes as two bf16 numbers, its value and what that leaves, one below the other; they are 17 bits of it, and the gradients
-// have their own rounding alone.  In one number a row's target, most of the row, is rounded once: over few rows that falls anywhere
-// up to 2^-8 of the gradient (2 rows of 1472 over 4931: 1.7 times as far off as the gradient's own rounding; over many it averages to 1.4).  Tiles
-// have 256 rows, so the second part costs a stage of the contraction over the rows and G's bytes.
-constexpr int64_t kTwoPartRows = 128;
+
 static HeadBackward plan_head_backward(int64_t M, int64_t V, int64_t K, void* at) {
   HeadBackward b = {};
   b.pack = head_pack(M, V, K, at);
-  b.half = M <= kTwoPartRows && !b.pack.on ? ceil_div(M, 8) * 8 : 0;
+  b.half = M <= METIS_TWO_PART_ROWS && !b.pack.on ? ceil_div(M, 8) * 8 : 0;      // G in two parts, see metis_bf16_product
   const int64_t rows = b.half ? 2 * b.half : M;
   b.columns = piece_columns(rows, V);
   b.sp = plan_splits(rows, K, b.columns < V ? b.columns : V);
@@ -1511,12 +1538,11 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   const DenseOperand h = {pack.on ? pack.h : a->h, pack.on ? a->K : a->ldh, false};
   DenseParams p = head_params(a, pack);
   p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride;
-  p.two_parts = b.half > 0;
+  p.half = (int32_t)b.half;
   const int64_t rows = b.half ? 2 * b.half : a->M;         // of G
   const DenseOperand of_dw = {b.half ? b.stacked : h.p, b.half ? a->K : h.ld, true};
   if (b.half && dw)
-    METIS_CUDA_OK(launch_counted(kLaunchStream, head_stack_kernel, dim3(row_blocks(rows)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M, (int)b.half,
-                                 (int)(a->K / 8), b.stacked));
+    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M, b.half, a->K, b.stacked, st)) return rc;
   const CommonWeight weight = gout_stride ? CommonWeight{} : CommonWeight{gout, inv_count, a->scale};
   for (int64_t v0 = 0; v0 < a->V; v0 += b.columns) {
     const int64_t n = a->V - v0 < b.columns ? a->V - v0 : b.columns;

@@ -142,12 +142,12 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
 }
 
 // a b, or a^T b with `mn`, for matrices of 16-byte aligned rows
-Tensor product(const Tensor& a, const Rows& ra, bool mn, const Tensor& b, const Rows& rb) {
+Tensor product(const Tensor& a, const Rows& ra, bool mn, int32_t half, const Tensor& b, const Rows& rb) {
   const int64_t M = mn ? ra.cols : ra.rows, K = mn ? ra.rows : ra.cols;
   const Tensor d = empty_like_options(b, {M, rb.cols}, at::kBFloat16);
-  const int64_t bytes = lib.metis_bf16_product_workspace_bytes(M, rb.cols, K, mn);
+  const int64_t bytes = lib.metis_bf16_product_workspace_bytes(M, rb.cols, K, mn, half);
   const Tensor ws = bytes > 0 ? scratch(b, bytes) : Tensor();
-  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, d.data_ptr(), rb.cols, ptr(ws), bytes, nullptr, stream_of(b)), "metis_bf16_product");
+  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, half, d.data_ptr(), rb.cols, ptr(ws), bytes, nullptr, stream_of(b)), "metis_bf16_product");
   return d;
 }
 
@@ -204,6 +204,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         Rows rdz = rdy;
         const bool write_dz = product_wanted && (epilogue || !operand(dy, rdz));
         Tensor dz = dy;
+        const int32_t half = product_wanted && epilogue && M <= METIS_TWO_PART_ROWS ? (int32_t)(M + 7) / 8 * 8 : 0;      // (dy as it is has one part)
         if (write_dz || need_b || need_gate) {
           metis_linear_pointwise_args a = {};
           a.M = M; a.N = N;
@@ -213,7 +214,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           if (saved[2].defined()) { a.gate = saved[2].data_ptr(); a.ldgate = Rows(saved[2]).ld; }
           if (write_dz) {
             const int64_t pitch = (N + 7) / 8 * 8;
-            dz = empty_like_options(dy, {M, pitch}, at::kBFloat16);
+            dz = empty_like_options(dy, {half ? 2 * half : M, pitch}, at::kBFloat16);
+            a.half = half;
             rdz.rows = M; rdz.cols = N; rdz.ld = pitch;
             a.dz = dz.data_ptr(); a.lddz = pitch;
           }
@@ -234,12 +236,12 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         if (need_x) {
           Rows rw(saved[1]);
           operand(saved[1], rw);
-          out[0] = product(dz, rdz, false, saved[1], rw).view(x_shape);
+          out[0] = product(dz, rdz, false, half, saved[1], rw).view(x_shape);
         }
         if (need_w) {
           Rows rx(saved[0]);
           operand(saved[0], rx);
-          out[1] = product(dz, rdz, true, saved[0], rx);
+          out[1] = product(dz, rdz, true, half, saved[0], rx);
         }
       }
     }

@@ -219,7 +219,7 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   // Items of eight elements of one token, the CTAs of the cluster in turn; a thread has the epilogue's operands of kFly items in
   // flight before it uses them (one element at a time, 64 tokens of the silu and gate of 18944 rows: 56 us for the product; 29 so).
   // The eight lie together where rows are 16-byte aligned, else an item apart, so that neighbouring lanes have neighbouring elements.
-  const int tokens = p.M - m0 < sh.bn ? (int)(p.M - m0) : sh.bn;
+  const int tokens = p.half ? p.half_rows : p.M - m0 < sh.bn ? (int)(p.M - m0) : sh.bn;       // (two parts are one tile)
   const int shift = sh.rows == 128 ? 4 : sh.rows == 64 ? 3 : 2;        // log2 of the items of a token
   const bool wide = p.d_wide && (!p.gate || p.gate_wide) && (!p.residual || p.residual_wide);
   const int apart = wide ? 1 : 1 << shift, first = wide ? 8 : 1;
@@ -257,6 +257,11 @@ dense_small_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += load_cluster_f32(from + i * apart * 4);
+        }
+        if (p.half) {                                      // (a product: rows of 16-byte pieces)
+          const float4 a = load_cluster_f32x4(from + p.half * 512), b = load_cluster_f32x4(from + p.half * 512 + 16);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
       }
       if (p.bias) {

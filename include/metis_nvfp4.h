@@ -483,6 +483,7 @@ int32_t metis_linear(const metis_linear_args* args);
  * Gradients through that epilogue: dz = bf16(dy * gate * act'(z)), dgate = bf16(dy * act(z)), dbias = sum over rows of
  * dy * gate * act'(z) in fp32, rounded once.  Each output may be null; gate null: 1; slope null: 1 (no activation).  act is read
  * for dgate alone.  dz, act and slope have 16-byte aligned rows.  The workspace is for dbias alone.
+ * half > 0 (see metis_bf16_product): dz is [2 half, N], its rows in two parts, zeros in the rows from M to half of both.
  */
 typedef struct metis_linear_pointwise_args {
   int64_t M, N;
@@ -493,7 +494,7 @@ typedef struct metis_linear_pointwise_args {
   void* dz;     int64_t lddz;
   void* dgate;  int64_t lddg;
   void* dbias;  int32_t dbias_dtype;
-  int32_t reserved;
+  int32_t half;
   void* workspace;  int64_t workspace_bytes;
   void* stream;
 } metis_linear_pointwise_args;
@@ -504,10 +505,17 @@ int32_t metis_linear_pointwise(const metis_linear_pointwise_args* args);
  * D [M, N] = A B^T in bf16, sums in fp32: b is [K, N], a is [M, K] (a_mn_major = 0: an input's gradient, dz W) or [K, M]
  * (1: a weight's, dz^T x).  All three have 16-byte aligned rows, N is a multiple of 8.  A product of few tiles is split along K:
  * its workspace holds the splits' sums in fp32, added in a fixed order.
+ *
+ * half > 0, for few rows (dz's M or, MN-major, its K; a multiple of 8 from that number to METIS_TWO_PART_ROWS): a's row m is the sum
+ * of two bf16 numbers, its rows m and half + m, what the first leaves; zeros from the last row to half in both.  They hold 17 bits, and
+ * the product has its own rounding alone.  One number leaves an error of as much again, which for few rows does not
+ * average: up to 1.7 times the product's own (2 rows of 1472 over 4931 columns), 1.4 for many.  Tiles are of more rows than that, and the other
+ * operand's bytes are what bounds them: the second part costs next to nothing.
  */
-int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major);
+#define METIS_TWO_PART_ROWS 128
+int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t a_mn_major, int32_t half);
 int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N,
-                           int64_t K, void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+                           int64_t K, int32_t half, void* d, int64_t ldd, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- head: losses over the vocabulary without the logits ----------------------------------------------------- */
 

@@ -59,7 +59,7 @@ def test_pointwise_refuses(L, p):
     assert call(M=0) == -2 and call(N=-1) == -2 and call(dy=None) == -1 and call(dz=None) == -1
     assert call(act=p + 2) == -3 and call(ldact=20) == -3 and call(slope=p + 8) == -3 and call(ldslope=16) == -3
     assert call(lddy=8) == -1 and call(lddz=8) == -1 and call(gate=p, ldgate=8) == -1 and call(dgate=p, lddg=2) == -1
-    assert call(dbias=p, dbias_dtype=5) == -1
+    assert call(dbias=p, dbias_dtype=5) == -1 and call(half=4) == -1 and call(half=-8) == -1 and call(half=136) == -1 and call(M=9, half=8) == -1
     assert call(dz=p + 2) == -3 and call(lddz=28) == -3 and call(dy=p + 1) == -3          # dz is an operand of the products behind it
     assert call(dbias=p, dbias_dtype=0) == -4                                        # no workspace
     assert call(dbias=p, dbias_dtype=0, workspace=p, workspace_bytes=16) == -4
@@ -68,12 +68,16 @@ def test_pointwise_refuses(L, p):
 
 
 def test_product_refuses(L, p):
-    call = lambda a=p, mn=0, lda=16, b=p, ldb=24, M=4, N=24, K=16, d=p, ldd=24: L.metis_bf16_product(a, mn, lda, b, ldb, M, N, K, d, ldd, None, 0, None, None)
+    call = lambda a=p, mn=0, lda=16, b=p, ldb=24, M=4, N=24, K=16, half=0, d=p, ldd=24: L.metis_bf16_product(a, mn, lda, b, ldb, M, N, K, half, d, ldd, None, 0, None, None)
     assert call(M=0) == -2 and call(K=0) == -2 and call(N=1 << 31) == -7
     assert call(a=None) == -1 and call(b=None) == -1 and call(d=None) == -1
     assert call(lda=8) == -3 and call(ldb=20) == -3 and call(ldd=12) == -3 and call(a=p + 4) == -3 and call(mn=1, lda=2) == -3
     assert call(N=23) == -2                                                           # rows of whole 16-byte pieces
-    assert call(M=2100, K=100000, lda=100000) == -4 and L.metis_bf16_product_workspace_bytes(2100, 24, 100000, 0) > 0      # split: no workspace
+    assert call(M=2100, K=100000, lda=100000) == -4 and L.metis_bf16_product_workspace_bytes(2100, 24, 100000, 0, 0) > 0   # split: no workspace
+    for half in (-8, 4, 12, 136):                                                    # two parts: a multiple of 8 from the rows' number to 128
+        assert call(half=half) == -1 and call(mn=1, half=half) == -1
+    assert call(M=17, half=16) == -1 and call(mn=1, K=24, half=16) == -1
+    assert call(mn=1, M=16, K=8, half=8) == -4 and L.metis_bf16_product_workspace_bytes(16, 24, 8, 1, 8) > 0        # the other operand's rows twice
 
 
 def test_head_refuses(L, p):

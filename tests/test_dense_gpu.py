@@ -131,23 +131,27 @@ def test_linear_of_no_rows():
     assert gx.shape == x.shape and gr.shape == r.shape and not gw.any() and not gb.any()
 
 
-def test_linear_gradients_take_two_roundings():
-    """Roundings of one type that fall independently add by squares: a gradient that rounds an intermediate to bf16 (dz, act(z)) and then
-    itself is sqrt(2) = 1.41 times as far from the exact one as bf16 has to be.  Slopes in 16 bits with ten of mantissa add 1/64 of that square; a
-    z in bf16 instead would take the erf form's to 1.6."""
+@pytest.mark.parametrize("M,N,K", [(1, 473, 344), (7, 33, 8), (24, 1001, 192), (64, 2000, 520), (65, 130, 64), (128, 515, 264), (129, 515, 264), (512, 1000, 192)])
+def test_roundings_of_the_gradients(M, N, K):
+    """Roundings of one type that fall independently add by squares.  Up to 128 rows dz goes as two bf16 numbers: dx and dW have their own
+    rounding, with the slope's, an eighth of that (1.01; over as few as 56 elements the two may agree by a third, 1.05), and 2^-9 of it from the second
+    number.  Above that dz is rounded: sqrt(2) and the slope's, 1.42.  The gate's gradient has act(z) in bf16 and its own, which fall anywhere
+    where there are few.  (z in bf16 would take the erf form's dx to 1.6.)"""
     for act in ("silu", "gelu", "gelu_tanh"):
-        for M, N, K in ((512, 1000, 192), (24, 1001, 192)):                               # CTA pairs; few tokens and odd rows
-            x, w, dy, g = normal(M, K), normal(N, K, scale=K ** -0.5, seed=1), normal(M, N, seed=2), normal(M, N, seed=3)
-            for gate in (None, g):
-                leaves = [t.clone().requires_grad_(True) for t in (x, w) + ((gate,) if gate is not None else ())]
-                y = dense.linear(*leaves[:2], activation=act, gate=leaves[2] if gate is not None else None)
-                got = torch.autograd.grad(y, leaves, dy)
-                copies = [t.detach().double().requires_grad_(True) for t in leaves]
-                out = act64(act, copies[0] @ copies[1].t())
-                exact = torch.autograd.grad(out * copies[2] if gate is not None else out, copies, dy.double())
-                for a, e in zip(got, exact):
-                    off, least = (a.double() - e).norm(), (e.bfloat16().double() - e).norm()
-                    assert off <= 1.5 * least, (act, M, gate is not None, float(off / least))
+        x, w, dy, g = normal(M, K), normal(N, K, scale=K ** -0.5, seed=1), normal(M, N, seed=2), normal(M, N, seed=3)
+        for gate in (None, g):
+            leaves = [t.clone().requires_grad_(True) for t in (x, w) + ((gate,) if gate is not None else ())]
+            y = dense.linear(*leaves[:2], activation=act, gate=leaves[2] if gate is not None else None)
+            got = torch.autograd.grad(y, leaves, dy)
+            copies = [t.detach().double().requires_grad_(True) for t in leaves]
+            out = act64(act, copies[0] @ copies[1].t())
+            exact = torch.autograd.grad(out * copies[2] if gate is not None else out, copies, dy.double())
+            for i, (a, e) in enumerate(zip(got, exact)):
+                off, least = (a.double() - e).norm(), (e.bfloat16().double() - e).norm()
+                if i < 2 or M * N >= 10000:
+                    assert off <= (1.1 if M <= 128 and i < 2 else 1.5) * least, (act, i, float(off / least))
+                else:
+                    assert ((a.double() - e).abs() <= 2.01 * STEP * e.abs() + 2.0 ** -18).all()          # (act(z) from z in fp32, of sums of K products)
 
 
 def test_linear_slopes_of_far_values():
