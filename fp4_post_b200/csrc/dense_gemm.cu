@@ -268,8 +268,9 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
 // With gate, residual, or what the gradients need: several tensors of the output's size pass by, and each adds its time to the layer's
 // (the tensor pipe is busy 0.53 of the time with two, 0.95 without).  What is read comes by asynchronous copies of the load/store unit a piece
 // ahead; what is written leaves by the TMA unit, all of it behind one fence where there are buffers for it (without a residual its buffer is
-// the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 210, and slopes 230, and act(z) 250 (272 with a wait and a
-// fence for the output alone), gate and residual 189, all of them 285 (five stages in place of six pay for the buffers).  Tried with two
+// the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 200, and slopes and act(z) 232 (270 with a wait and
+// a fence for the output alone, and the next copies ahead of it), gate and residual 192, all of them 257.  (Five stages in place of six pay for the
+// buffers: 156 plain.)  Tried with two
 // outputs, silu and gate / gate and residual, 204 / 187 by this form: loads into registers where they are used 238 / 220; loads by the TMA
 // unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores by the load/store
 // unit 235 / 188.  `next`: the piece that this warp takes after this one.
@@ -293,6 +294,9 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
 #pragma unroll
     for (int i = 0; i < 16; ++i) act[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
   }
+  // the stores' fence waits for copies on their way as well: with three outputs they start behind it (silu, gate, slopes and act(z) 256 -> 232
+  // us), without they are wanted early (gate and residual 190, behind it 195 to 208)
+  const bool late = p.slope && p.act_out;
   const bool together = !kOdd && p.d_wide && !(p.slope && p.act_out && residual.src);
   if (!together) {
     if (p.slope) store_piece_tma<kStores>(st, map_s, slopes, (int32_t)col0, (int32_t)row0);
@@ -304,14 +308,14 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
   }
-  gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
+  if (!late) gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
   if (residual.src) {
     if (kOdd || (residual.wide && full)) residual.take(w, col0, row0);
     else load_piece_rows(st, residual.src, residual.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }
   }
-  residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
+  if (!late) residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
   if (together && p.slope && p.act_out) store_three_tma(st, residual.buf, map_s, slopes, map_a, act, map_d, w, (int32_t)col0, (int32_t)row0);
@@ -319,6 +323,10 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
   else if (together && p.act_out) store_two_tma(st, map_a, act, map_d, w, (int32_t)col0, (int32_t)row0);
   else if (p.d_wide) store_piece_tma<kStores>(st, map_d, w, (int32_t)col0, (int32_t)row0);
   else store_piece_rows(st, p.d, p.ldd, w, col0, row0, p.M, p.N);
+  if (late) {
+    gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
+    residual.fetch(next.valid, next.col0, next.row0, p.M, p.N);
+  }
 }
 
 // The statistics of this lane's row take 32 more logits: maximum of the chunk, then one exponential per element.
