@@ -60,7 +60,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x [..., K], weight [N, K] (the layout of nn.Linear), bias [N] in bf16 or fp32; gate and residual are shaped like the output
     [..., N] (no broadcasting).  activation: None, "silu", "gelu" (erf form) or "gelu_tanh".  A SwiGLU block is
     linear(linear(h, w_gate, activation="silu", gate=linear(h, w_up)), w_down, residual=x).
-    Differentiable once in all tensors; the backward pass keeps bf16(x @ weight.T + bias)."""
+    Differentiable once in all tensors; the backward pass keeps the activation's slopes in 16 bits, and
+    act(..) in bf16 where the gate has a gradient."""
     try:
         code = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

@@ -154,6 +154,26 @@ def test_roundings_of_the_gradients(M, N, K):
                     assert ((a.double() - e).abs() <= 2.01 * STEP * e.abs() + 2.0 ** -18).all()          # (act(z) from z in fp32, of sums of K products)
 
 
+@pytest.mark.parametrize("N", [776, 771])
+@pytest.mark.parametrize("gate,residual", [(True, False), (True, True), (False, True), (False, False)])
+def test_linear_of_many_rows_and_what_its_gradients_keep(N, gate, residual):
+    # 2100 rows: the CTA pairs, whatever the shape; 771: rows that 16 bytes do not divide
+    check_linear(2100, N, 136, "silu", torch.bfloat16, gate, residual, seed=N)
+    check_linear(2100, N, 72, None, None, gate, residual, seed=N + 1)
+
+
+def test_linear_of_many_rows_and_shifted_operands():
+    M, N, K = 2100, 776, 72
+    x, w, dy = normal(M, K), normal(N, K, scale=K ** -0.5, seed=1), normal(M, N, seed=2)
+    g, r = (normal(M, N + 3, seed=s)[:, 1:1 + N] for s in (3, 4))
+    def run(*extra):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, *extra)]
+        y = dense.linear(*leaves[:2], activation="gelu", gate=leaves[2], residual=leaves[3])
+        return (y, *torch.autograd.grad(y, leaves, dy))
+    # the same sums by another epilogue: an element may fall on the other side of a rounding, one step, and few do
+    assert all(rel(a.double(), b.double()) <= STEP for a, b in zip(run(g, r), run(g.contiguous(), r.contiguous())))
+
+
 def test_linear_slopes_of_far_values():
     """Where the slope is small it keeps its relative accuracy: fp16 with 2^15 in front is normal down to 2^-29 (silu at z = -22)."""
     for M in (8, 512):
