@@ -221,10 +221,11 @@ template <bool kOdd> struct EpilogueOperand {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // this lane's 32 elements of its row, of the piece that was fetched two groups ago
-  __device__ __forceinline__ void take(uint32_t (&w)[16], int64_t col0, int64_t row0) {
+  // this lane's 32 elements of its row, of the piece that was fetched two groups ago, or in the last group
+  __device__ __forceinline__ void take(uint32_t (&w)[16], int64_t col0, int64_t row0, bool last) {
     const int lane = threadIdx.x & 31;
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (last) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
     if constexpr (kOdd) {
       const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(src + (row0 + lane) * ld + col0) & 15);
@@ -266,14 +267,14 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
 }
 
 // With gate, residual, or what the gradients need: several tensors of the output's size pass by, and each adds its time to the layer's
-// (the tensor pipe is busy 0.53 of the time with two, 0.95 without).  What is read comes by asynchronous copies of the load/store unit a piece
-// ahead; what is written leaves by the TMA unit, all of it behind one fence where there are buffers for it (without a residual its buffer is
-// the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 200, and slopes and act(z) 232 (270 with a wait and
-// a fence for the output alone, and the next copies ahead of it), gate and residual 192, all of them 257.  (Five stages in place of six pay for the
-// buffers: 156 plain.)  Tried with two
-// outputs, silu and gate / gate and residual, 204 / 187 by this form: loads into registers where they are used 238 / 220; loads by the TMA
-// unit, which queue behind the tiles' own, 209 / -; 16 warps of 96 registers 258 / 269, with four stages 275 / 236; stores by the load/store
-// unit 235 / 188.  `next`: the piece that this warp takes after this one.
+// (the tensor pipe is busy 0.59 of the time with four of them, 0.95 with the output alone).  What is read comes by asynchronous copies of the
+// load/store unit a piece ahead; what is written leaves by the TMA unit, all of it behind one fence where there are buffers for it (without
+// a residual its buffer is the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 200, and slopes and act(z)
+// 232 (270 with a wait and a fence for the output alone, and the next copies ahead of it), gate and residual 192, all of them 257; five
+// stages in place of six, for the buffers' sake, cost a plain layer 4.  It is a warp's chain that takes the time, not the bytes: one row of
+// the gate for all takes as long.  Tried with two outputs (silu, gate, one tensor for the gradients / gate and residual, 204 / 187 by this
+// form): loads into registers where they are used 238 / 220; loads by the TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96
+// registers 258 / 269, with four stages 275 / 236; stores by the load/store unit 235 / 188.  `next`: the piece that this warp takes after this one.
 struct PieceAt {
   bool valid;
   int64_t row0, col0;
@@ -303,14 +304,14 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
     if (p.act_out) store_piece_tma<kStores>(st, map_a, act, (int32_t)col0, (int32_t)row0);
   }
   if (gate.src) {
-    if (kOdd || (gate.wide && full)) gate.take(w, col0, row0);
+    if (kOdd || (gate.wide && full)) gate.take(w, col0, row0, false);
     else load_piece_rows(st, gate.src, gate.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] *= bf16_lo(w[i]); v[2 * i + 1] *= bf16_hi(w[i]); }
   }
   if (!late) gate.fetch(next.valid, next.col0, next.row0, p.M, p.N);
   if (residual.src) {
-    if (kOdd || (residual.wide && full)) residual.take(w, col0, row0);
+    if (kOdd || (residual.wide && full)) residual.take(w, col0, row0, late);        // (late: no group of the gate lies behind it)
     else load_piece_rows(st, residual.src, residual.ld, col0, row0, p.M, p.N, w);
 #pragma unroll
     for (int i = 0; i < 16; ++i) { v[2 * i] += bf16_lo(w[i]); v[2 * i + 1] += bf16_hi(w[i]); }

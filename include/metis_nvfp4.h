@@ -548,7 +548,8 @@ int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_i
  * dh [M, K] = G W and dw [V, K] = G^T h (bf16, either may be null) with G[m][j] = scale * g_m (softmax(l)[m][j] - [j = target[m]]),
  * g_m = gout[m] (gout_stride 1; inv_count is null) or *gout * (inv_count ? *inv_count : 1) (gout_stride 0), 0 where
  * target[m] = ignore_index.  The logits are formed
- * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, dh's sums in fp32.
+ * again piece by piece of the vocabulary; a piece's G goes through the workspace in bf16, in two parts up to METIS_TWO_PART_ROWS
+ * rows (see metis_bf16_product), dh's sums in fp32.  *gout multiplies the products in fp32.
  */
 int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K);
 int32_t metis_head_backward(const metis_head_args* args, const float* gout, int32_t gout_stride, const float* inv_count,
