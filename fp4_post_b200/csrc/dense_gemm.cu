@@ -270,7 +270,7 @@ __device__ __forceinline__ void linear_chunk(const DenseParams& p, Staging& st, 
 // (the tensor pipe is busy 0.59 of the time with four of them, 0.95 with the output alone).  What is read comes by asynchronous copies of the
 // load/store unit a piece ahead; what is written leaves by the TMA unit, all of it behind one fence where there are buffers for it (without
 // a residual its buffer is the third).  8192 x 8960 x 1536, us: plain 152, silu with slopes 184, silu and gate 200, and slopes and act(z)
-// 232 (270 with a wait and a fence for the output alone, and the next copies ahead of it), gate and residual 192, all of them 257; five
+// 224 (240 warm; 270 with a wait and a fence for the output alone), gate and residual 192, all of them 248 (272 warm); five
 // stages in place of six, for the buffers' sake, cost a plain layer 4.  It is a warp's chain that takes the time, not the bytes: one row of
 // the gate for all takes as long.  Tried with two outputs (silu, gate, one tensor for the gradients / gate and residual, 204 / 187 by this
 // form): loads into registers where they are used 238 / 220; loads by the TMA unit, which queue behind the tiles' own, 209 / -; 16 warps of 96
@@ -295,8 +295,8 @@ __device__ __forceinline__ void linear_wide_chunk(const DenseParams& p, Staging&
 #pragma unroll
     for (int i = 0; i < 16; ++i) act[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
   }
-  // the stores' fence waits for copies on their way as well: with three outputs they start behind it (silu, gate, slopes and act(z) 256 -> 232
-  // us), without they are wanted early (gate and residual 190, behind it 195 to 208)
+  // the stores' fence waits for copies on their way as well: with three outputs they start behind it (silu, gate, slopes and act(z) 228 -> 224
+  // us, 250 -> 240 warm), without they are wanted early (gate and residual 188, behind it 192)
   const bool late = p.slope && p.act_out;
   const bool together = !kOdd && p.d_wide && !(p.slope && p.act_out && residual.src);
   if (!together) {
