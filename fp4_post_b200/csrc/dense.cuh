@@ -31,9 +31,8 @@ struct DenseParams {
   int64_t vocab;  int64_t col0;
   float scale, scale_log2e;                                // 1 / temperature, and that times log2(e)
   float weight_scale;                                      // scale, with the sign of the loss
-  float2* stats;                                           // [slots, stats_ld]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum)
+  float2* stats;                                           // [slots, stats_ld]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum), the target's l left out
   float* stats_e;                                          // [slots, stats_ld]: sum of 2^(..) (l log2(e) - maximum), or null
-  float* picked;                                           // [M]: logit of the target times log2(e), as the statistics have it
   const float* lse;                                        // [M]
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss (stride 1), or of all, times *inv_count (null: 1)
   const float* inv_count;
@@ -197,6 +196,7 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) { return make_uint4(
 struct RowStats {
   float m, s, e;
 };
+constexpr uint32_t kMinusInfinity = 0xff800000u;         // (a logit that adds nothing)
 __device__ __forceinline__ float stats_base(float m) { return m == -INFINITY ? 0.0f : m; }
 // b into a
 template <bool kEntropy> __device__ __forceinline__ void stats_merge(RowStats& a, const RowStats& b) {

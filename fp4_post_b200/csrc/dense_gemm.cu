@@ -3,8 +3,8 @@
 //   D [M, N] = A B^T, A [M, K] and B [N, K], either operand stored with the contraction in its rows instead (MN-major: the
 //   gradients read their operands as they lie, nothing is transposed in memory), and behind it
 //     linear   act(D + bias) * gate + residual in bf16, and the value in front of act where a backward pass will want it
-//     stats    for each row the maximum of the logits and the sum of their exponentials over this tile's columns, the entropy's
-//              sum, and the target's logit: the logits themselves are never stored
+//     stats    for each row the maximum of the logits and the sum of their exponentials over this tile's columns, and the entropy's
+//              sum, all without the target's: the logits themselves are never stored
 //     grad     the logits' gradient (softmax - one-hot) times the row's weight, in bf16: the operand of the two products behind it
 //     sum      D, or D plus an fp32 addend, in bf16 or fp32: gradients, summed over pieces of the vocabulary
 //
@@ -589,8 +589,6 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * (32 * Cfg::kChunks);
       RowStats stats = {-INFINITY, 0.0f, 0.0f};
-      float picked = 0.0f;
-      bool found = false;
       // the next chunk of the accumulator is read while this one is worked on, where the registers allow it
       constexpr bool kAhead = !Cfg::kOperands;
       uint32_t r[kAhead ? 2 : 1][32];
@@ -625,12 +623,11 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             linear_wide_chunk(p, st, &map_d, &map_s, &map_act, gate, residual, v, row0, col0, next);
           }
           if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy) {
-            stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
-            if (here) {
+            if (here) {                                    // (head_rows_kernel adds the target's)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (at == i) picked = __uint_as_float(v[i]) * p.scale_log2e;
-              found = true;
+              for (int i = 0; i < 32; ++i) if (at == i) v[i] = kMinusInfinity;
             }
+            stats_chunk<kEpi == kEpiStatsEntropy>(p, stats, v, col0);
           }
           if constexpr (kEpi == kEpiGrad) {
             float g[32];
@@ -694,7 +691,6 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           const int64_t slot = (tn * 2 + part) * p.stats_ld + row;
           p.stats[slot] = make_float2(stats.m, stats.s);
           if constexpr (kEpi == kEpiStatsEntropy) p.stats_e[slot] = stats.e;
-          if (found) p.picked[row] = picked;
         }
       }
     }
@@ -715,12 +711,14 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 
 // nll, lse and entropy of each row from the statistics of its `slots` pieces (slots of a row lie M apart).  The tensor core cuts what it adds
 // up to instead of rounding it (16 products of a row at a time: 2e-6 of a logit at K = 3584), which shows in the target's logit, the largest
-// of its row if the model knows anything.  So that one is formed again in fp32, and takes its place in the row's sums as well: log-probabilities
-// of 16 rows of 3584 are 2.9e-7 from 64 bits instead of 2.2e-6.
+// of its row if the model knows anything.  So the pieces leave it out, and it is formed here, in fp32: log-probabilities of 16 rows of 3584 are
+// 2.9e-7 from 64 bits instead of 2.2e-6.  With R, the others' sum, relative to the larger of the target's logit t and their maximum:
+//   t the largest   -log p = log(1 + R), log1p: for a token the model is sure of (1 - p of 1e-6) as many bits of it as of any, and never negative
+//   otherwise       -log p = log(R + 2^d) - d ln 2, d = t less their maximum; R is 1 at least and d negative
 //   kRows = 32  a block of 32 warps takes 32 rows: its warps take the slots in turn, neighbouring lanes neighbouring rows
 //   kRows = 1   few rows: a block of 8 warps takes one, its threads the slots
 struct HeadRows {
-  const float2* stats;  const float* stats_e;  const float* picked;
+  const float2* stats;  const float* stats_e;
   const __nv_bfloat16* h;  int64_t ldh;                    // rows as the statistics have them (packed or not)
   const __nv_bfloat16* w;  int64_t ldw;
   const int64_t* target;  int64_t ignore, vocab, M;
@@ -808,24 +806,27 @@ head_rows_kernel(const HeadRows p) {
     for (int w = 1; w < kWarps; ++w) stats_merge<kEntropy>(a, s_part[w][lane]);
     const int64_t given = p.row_of ? p.row_of[row] : row, t = p.target[given];
     const bool ignored = t == p.ignore, inside = t >= 0 && t < p.vocab;
-    float logit = 0.0f;
+    float nll = NAN, log_sum;
     if (!ignored && inside) {
+      float l2 = 0.0f;                                     // the target's logit, times log2 e
       if constexpr (kRows == 32) {
-        logit = s_dot[lane];
+        l2 = s_dot[lane];
       } else {
 #pragma unroll
-        for (int w = 0; w < 8; ++w) logit += s_dot[w];
+        for (int w = 0; w < 8; ++w) l2 += s_dot[w];
       }
-      const float base = stats_base(a.m), was = fmaxf(p.picked[row] - base, -1e30f), is = fmaxf(logit * p.scale_log2e - base, -1e30f);
-      const float xw = exp2_fast(was), xi = exp2_fast(is);
-      a.s += xi - xw;
-      if constexpr (kEntropy) a.e += fmaf(xi, is, -xw * was);
+      l2 *= p.scale_log2e;
+      const float base = stats_base(fmaxf(a.m, l2)), rest = a.s * exp2_fast(a.m - base), d = l2 - base;
+      log_sum = d == 0.0f ? log1pf(rest) : logf(rest + exp2_fast(d));
+      nll = log_sum - kLn2 * d;
+      stats_merge<kEntropy>(a, RowStats{l2, 1.0f, 0.0f});
+    } else {
+      log_sum = logf(a.s);
     }
-    const float all = fmaf(a.m, kLn2, logf(a.s));
-    p.lse[given] = all;
-    p.nll[given] = ignored ? 0.0f : !inside ? NAN : p.sign * (all - logit * p.scale);
+    p.lse[given] = fmaf(a.m, kLn2, log_sum);
+    p.nll[given] = ignored ? 0.0f : p.sign * nll;
     // H = log s - sum p (l - m): p = 2^(l - m) / s, l - m in units of log2
-    if constexpr (kEntropy) p.entropy[given] = ignored ? 0.0f : logf(a.s) - kLn2 * (a.e / a.s);
+    if constexpr (kEntropy) p.entropy[given] = ignored ? 0.0f : log_sum - kLn2 * (a.e / a.s);
   }
 }
 
@@ -1454,7 +1455,7 @@ static int32_t pack_rows(const metis_head_args* a, const HeadPack& k, float* nll
 
 extern "C" int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy) {
   if (M <= 0 || V <= 0 || K <= 0) return 0;
-  return head_pack(M, V, K, nullptr).bytes + ceil_div(M * 4, 16) * 16 + head_slots(M, V) * M * (entropy ? 12 : 8);
+  return head_pack(M, V, K, nullptr).bytes + head_slots(M, V) * M * (entropy ? 12 : 8);
 }
 
 extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) {
@@ -1466,8 +1467,7 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   const HeadPack pack = head_pack(a->M, a->V, a->K, a->workspace);
   DenseParams p = head_params(a, pack);
   const int64_t slots = head_slots(a->M, a->V);
-  p.picked = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pack.bytes);
-  p.stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(p.picked) + ceil_div(a->M * 4, 16) * 16);
+  p.stats = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + pack.bytes);
   p.stats_e = entropy ? reinterpret_cast<float*>(p.stats + slots * a->M) : nullptr;
   p.stats_ld = a->M;
   if (pack.on) if (int32_t rc = pack_rows(a, pack, nll, entropy, st)) return rc;
@@ -1477,7 +1477,7 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
     if (int32_t rc = launch_dense_small_stats(a->h, a->ldh, a->w, a->ldw, p, st)) return rc;
   } else if (int32_t rc = entropy ? launch_dense<false, false, kEpiStatsEntropy>(h, w, none, p, st) : launch_dense<false, false, kEpiStats>(h, w, none, p, st)) return rc;
   HeadRows r = {};
-  r.stats = p.stats; r.stats_e = p.stats_e; r.picked = p.picked;
+  r.stats = p.stats; r.stats_e = p.stats_e;
   r.h = static_cast<const __nv_bfloat16*>(h.p); r.ldh = h.ld; r.w = static_cast<const __nv_bfloat16*>(a->w); r.ldw = a->ldw;
   r.target = a->target; r.ignore = a->ignore_index; r.vocab = a->V; r.M = a->M; r.row_of = p.row_of; r.live = p.live;
   r.pieces = (int32_t)(a->K / 8); r.slots = (int32_t)slots;

@@ -420,20 +420,18 @@ dense_small_stats_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_addr(smem_u32(&bars.acc_empty[buf]));
-      if (first + q < u1 && row < p.N) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) stats_add<kEntropy>(__uint_as_float(r[i]) * p.scale_log2e, m[i], s[i], e[i]);
-      }
-      // targets among these 32 rows: seldom any
+      // targets among these 32 rows, seldom any: left out (head_rows_kernel adds them)
       uint32_t hits = __ballot_sync(0xffffffffu, first + q < u1 && (target >> 5) == first + q);
       while (hits) {
         const int who = __ffs(hits) - 1;
         hits &= hits - 1;
-        const int at = (int)(__shfl_sync(0xffffffffu, target, who) & 31);
-        float l = 0.0f;
+        const bool at = (int)(__shfl_sync(0xffffffffu, target, who) & 31) == lane;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) if (i == who) l = __uint_as_float(r[i]);
-        if (lane == at) p.picked[m0 + c0 + who] = l * p.scale_log2e;
+        for (int i = 0; i < 32; ++i) if (i == who && at) r[i] = kMinusInfinity;
+      }
+      if (first + q < u1 && row < p.N) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) stats_add<kEntropy>(__uint_as_float(r[i]) * p.scale_log2e, m[i], s[i], e[i]);
       }
     }
     // lanes into one: after five steps lane l has the statistics of token l, half of the tokens leaving at each
@@ -591,7 +589,7 @@ int64_t small_stats_slots(int64_t V) {
   return 4 * (units < sms ? units : sms);
 }
 
-// p.stats, p.stats_e and p.picked of up to 64 tokens h [M, K] against a vocabulary w [V, K]: small_stats_slots(V) slots
+// p.stats and p.stats_e of up to 64 tokens h [M, K] against a vocabulary w [V, K]: small_stats_slots(V) slots
 int32_t launch_dense_small_stats(const void* h, int64_t ldh, const void* w, int64_t ldw, const DenseParams& p, cudaStream_t st) {
   SmallShape sh = {};
   sh.rows = 128;

@@ -1,0 +1,87 @@
+"""The bf16 products and the head's losses (fp4_post_b200/dense.py) where an answer is easily lost: tokens that the model is sure of,
+ignored rows that hold anything, derivatives and traces that the native calls cannot follow, waits that run out, saved tensors that come back
+laid out otherwise.  The plain sides are torch in 64 bits.  A bf16 rounding is off by at most 2^-8 of the value (STEP)."""
+import math
+
+import pytest
+import torch
+
+from fp4_post_b200 import dense
+
+pytestmark = pytest.mark.gpu
+STEP = 2.0 ** -8
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib(built_library):
+    return built_library
+
+
+def normal(*shape, scale=1.0, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+# ---- tokens that the model is sure of -------------------------------------------------------------------------------
+
+def sure_rows(M, V, K, temperature, seed=0):
+    """Hidden states that lean on their token's row of the head so far that 1 - p of the target runs from 0.3 down to 1e-6, row by row."""
+    w = normal(V, K, scale=K ** -0.5, seed=seed)
+    t = torch.randperm(V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed + 1))[:M]
+    wt = w[t].double()
+    direction = wt / (wt * wt).sum(dim=1, keepdim=True)                  # one unit of it is one unit of the target's logit
+    want = 10.0 ** torch.linspace(math.log10(0.3), -6.0, M, device="cuda", dtype=torch.float64)
+    # (the others' logits are some hundredths of it: their sum is about V)
+    reach = temperature * (math.log(V) + torch.log((1 - want) / want))
+    return (direction * reach[:, None]).bfloat16(), w, t
+
+
+def exact_head(h, w, t, temperature):
+    """log p of the target and 1 - p of it, without cancellation, and the logits, in 64 bits."""
+    logits = h.double() @ w.double().t() / temperature
+    others = logits.scatter(1, t[:, None], -math.inf)
+    picked = logits.gather(1, t[:, None])[:, 0]
+    odds = torch.logsumexp(others, dim=1) - picked                       # log((1 - p) / p)
+    return -torch.nn.functional.softplus(odds), torch.sigmoid(odds), logits
+
+
+def logit_error(h, w, logits, temperature, K):
+    """What a logit is off by: sums of K products at 2^-23 of their magnitudes, its scaling and the logarithm's at 2^-23 each."""
+    return K * 2.0 ** -23 * float((h.double().abs() @ w.double().abs().t()).max()) / temperature + 2.0 ** -21 * (1 + float(logits.abs().max()))
+
+
+SURE = [(1, 97, 64), (9, 1003, 3584), (64, 1003, 256), (100, 1003, 3584), (200, 1003, 3584), (300, 2500, 512)]
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.6, 1.7])
+@pytest.mark.parametrize("M,V,K", SURE)
+def test_log_probabilities_of_sure_tokens(M, V, K, temperature):
+    """-log p = log(1 + (1 - p) / p) has the relative error of the odds, which is twice a logit's error, and of their sum, V additions of
+    2^-24 at the most; it is never negative, so no log-probability is positive."""
+    h, w, t = sure_rows(M, V, K, temperature)
+    want, _, logits = exact_head(h, w, t, temperature)
+    off = 2 * logit_error(h, w, logits, temperature, K) + V * 2.0 ** -24
+    got, entropy = dense.token_logprobs(h, w, t, temperature=temperature, entropy=True)
+    assert (got <= 0).all() and (entropy >= 0).all()
+    assert ((got.double() - want).abs() <= 1.1 * off * want.abs()).all()
+    loss = dense.linear_cross_entropy(h, w, t, temperature=temperature, reduction="none")
+    assert torch.equal(loss, -got)
+    # the entropy: (1 - p) / p times the others' distances, of which only the logits' differences are off
+    logp = torch.log_softmax(logits, dim=1)
+    exact = -(logp.exp() * logp).sum(dim=1)
+    assert ((entropy.double() - exact).abs() <= 1.1 * (2 * off + 2.0 ** -20) * exact + 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("M", [6, 70])
+def test_a_target_of_infinite_logit_or_alone_in_its_vocabulary(M):
+    h, w, t = normal(M, 64), normal(90, 64, seed=1), torch.arange(M, device="cuda")
+    got = dense.token_logprobs(h, w[:1], torch.zeros_like(t), entropy=True)
+    assert not got[0].any() and not got[1].any()                         # p = 1
+    w[t[2]] = 0
+    w[t[2], 0] = float("inf")
+    h[:, 0] = h[:, 0].abs() + 1
+    got = dense.token_logprobs(h, w, t)
+    assert torch.isnan(got[2]) and torch.isnan(got).all()                # infinity less infinity, as a subtracted maximum has it
+    w[t[2], 0] = -float("inf")
+    got = dense.token_logprobs(h, w, t)
+    assert got[2] == -float("inf") and torch.isfinite(got[:2]).all() and torch.isfinite(got[3:]).all()
