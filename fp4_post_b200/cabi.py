@@ -46,6 +46,7 @@ EXPORTS = (
     "metis_rope_pair", "metis_silu_mul",
     "metis_dense_launches", "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product_workspace_bytes", "metis_bf16_product",
     "metis_head_loss_workspace_bytes", "metis_head_loss", "metis_head_sum", "metis_head_backward_workspace_bytes", "metis_head_backward",
+    "metis_head_loss_keep", "metis_head_backward_kept",
 )
 
 
@@ -203,12 +204,16 @@ def lib() -> C.CDLL:
     L.metis_head_loss_workspace_bytes.restype = i64
     L.metis_head_loss.argtypes = [C.POINTER(HeadArgs), vp, vp]
     L.metis_head_loss.restype = i32
+    L.metis_head_loss_keep.argtypes = [C.POINTER(HeadArgs), vp, vp, vp]
+    L.metis_head_loss_keep.restype = i32
     L.metis_head_sum.argtypes = [vp, vp, i64, i64, i32, vp, vp, vp]
     L.metis_head_sum.restype = i32
     L.metis_head_backward_workspace_bytes.argtypes = [i64, i64, i64]
     L.metis_head_backward_workspace_bytes.restype = i64
     L.metis_head_backward.argtypes = [C.POINTER(HeadArgs), vp, i32, vp, vp, i64, vp, i64]
     L.metis_head_backward.restype = i32
+    L.metis_head_backward_kept.argtypes = [C.POINTER(HeadArgs), vp, vp, i32, vp, vp, i64, vp, i64]
+    L.metis_head_backward_kept.restype = i32
     _lib = L
     return L
 

@@ -34,6 +34,7 @@ struct DenseParams {
   float2* stats;                                           // [slots, stats_ld]: maximum of l log2(e) and sum of 2^(l log2(e) - maximum), the target's l left out
   float* stats_e;                                          // [slots, stats_ld]: sum of 2^(..) (l log2(e) - maximum), or null
   const float* lse;                                        // [M]
+  const float* target_logp;                                // [M]: the target's log-probability
   const float* gout;  int32_t gout_stride;                 // gradient of each row's loss (stride 1), or of all, times *inv_count (null: 1)
   const float* inv_count;
   int32_t half, half_rows;                                 // rows in two parts of bf16, so far apart (0: one part), and how many of each are rows

@@ -558,7 +558,7 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       // contraction over the rows reads
       const bool rows = row0 < (kEpi == kEpiGrad ? (M + 63) / 64 * 64 : M);
       int64_t hit = -1;                                    // the target's column in this launch
-      float lse2 = 0.0f, weight = 0.0f;
+      float lse2 = 0.0f, weight = 0.0f, at_target = 0.0f;
       bool dead = true;
       if constexpr (kEpi == kEpiStats || kEpi == kEpiStatsEntropy || kEpi == kEpiGrad) {
         if (row < M) {
@@ -571,6 +571,9 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             // (one gradient for all rows: it multiplies the products, not G, whose common factor bf16 would round)
             weight = p.gout_stride ? p.gout[given] * p.weight_scale : p.weight_scale < 0.0f ? -1.0f : 1.0f;
             if (t < 0 || t >= p.vocab) weight = NAN;       // (a target outside the vocabulary; ignored rows are dead)
+            // The target's p - 1 from its log-probability, as the forward pass kept it: from this logit, which the tensor core cuts, and the one-hot
+            // it would be off by 2e-6 of the logit, for a token that the model is sure of more than there is of it.
+            if (hit >= n0 && hit < n0 + 32 * Cfg::kChunks) at_target = expm1f(p.target_logp[given]) * weight;
           }
         }
       }
@@ -634,9 +637,8 @@ dense_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
             for (int i = 0; i < 32; ++i) g[i] = exp2_fast(fmaf(__uint_as_float(v[i]), p.scale_log2e, -lse2)) * weight;
             if (here) {
-              // the one-hot's place: (p - 1) weight
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (at == i) g[i] -= weight;
+              for (int i = 0; i < 32; ++i) if (at == i) g[i] = at_target;
             }
             uint32_t w[16];
 #pragma unroll
@@ -725,7 +727,7 @@ struct HeadRows {
   const int32_t* row_of;  const int32_t* live;
   int32_t pieces, slots;                                   // 16-byte pieces of a row of h; slots
   float scale, scale_log2e, sign;
-  float* nll;  float* lse;  float* entropy;
+  float* nll;  float* lse;  float* entropy;  float* target_logp;      // the last two may be null
 };
 
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float c) {
@@ -825,8 +827,27 @@ head_rows_kernel(const HeadRows p) {
     }
     p.lse[given] = fmaf(a.m, kLn2, log_sum);
     p.nll[given] = ignored ? 0.0f : p.sign * nll;
+    if (p.target_logp) p.target_logp[given] = -nll;
     // H = log s - sum p (l - m): p = 2^(l - m) / s, l - m in units of log2
     if constexpr (kEntropy) p.entropy[given] = ignored ? 0.0f : log_sum - kLn2 * (a.e / a.s);
+  }
+}
+
+// The same from lse alone, for a backward pass that was not given what the forward pass had: to 2^-24 of the logit.  A warp has a row.
+__global__ void __launch_bounds__(256)
+head_target_kernel(const __nv_bfloat16* h, int64_t ldh, const __nv_bfloat16* w, int64_t ldw, const int64_t* target, int64_t ignore, int64_t vocab, int64_t M,
+                   int pieces, float scale, const float* lse, float* target_logp) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < M; row += (int64_t)gridDim.x * 8) {
+    const int64_t t = target[row];
+    if (t == ignore || t < 0 || t >= vocab) continue;
+    const uint4 *hp = reinterpret_cast<const uint4*>(h + row * ldh), *wp = reinterpret_cast<const uint4*>(w + t * ldw);
+    float dot = 0.0f;
+#pragma unroll 4
+    for (int k = lane; k < pieces; k += 32) dot = dot8(hp[k], wp[k], dot);
+    dot = warp_sum(dot);
+    if (lane == 0) target_logp[row] = fmaf(dot, scale, -lse[row]);
   }
 }
 
@@ -1458,7 +1479,9 @@ extern "C" int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t
   return head_pack(M, V, K, nullptr).bytes + head_slots(M, V) * M * (entropy ? 12 : 8);
 }
 
-extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) {
+extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* entropy) { return metis_head_loss_keep(a, nll, entropy, nullptr); }
+
+extern "C" int32_t metis_head_loss_keep(const metis_head_args* a, float* nll, float* entropy, float* target_logp) {
   if (int32_t rc = check_head(a)) return rc;
   if (!nll) return fail(METIS_ERR_BAD_ARGUMENT, "nll is null");
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < metis_head_loss_workspace_bytes(a->M, a->V, a->K, entropy != nullptr))
@@ -1482,7 +1505,7 @@ extern "C" int32_t metis_head_loss(const metis_head_args* a, float* nll, float* 
   r.target = a->target; r.ignore = a->ignore_index; r.vocab = a->V; r.M = a->M; r.row_of = p.row_of; r.live = p.live;
   r.pieces = (int32_t)(a->K / 8); r.slots = (int32_t)slots;
   r.scale = p.scale; r.scale_log2e = p.scale_log2e; r.sign = a->negate ? -1.0f : 1.0f;
-  r.nll = nll; r.lse = a->lse; r.entropy = entropy;
+  r.nll = nll; r.lse = a->lse; r.entropy = entropy; r.target_logp = target_logp;
   const bool few = a->M <= kFewRows;
   auto rows = few ? (entropy ? head_rows_kernel<true, 1> : head_rows_kernel<false, 1>) : (entropy ? head_rows_kernel<true, 32> : head_rows_kernel<false, 32>);
   METIS_CUDA_OK(launch_counted(kLaunchShort, rows, dim3((unsigned)ceil_div(a->M, few ? 1 : 32)), dim3(few ? 256 : 1024), 0, st, r));
@@ -1504,6 +1527,7 @@ struct HeadBackward {
   Splits sp;
   __nv_bfloat16 *g, *stacked;                              // stacked: h twice, for G in two parts
   float* sums;
+  float* target_logp;                                      // where the call brings none
   int64_t half;                                            // rows from one part of G to the other; 0: it has one
   int64_t bytes;
 };
@@ -1520,7 +1544,9 @@ static HeadBackward plan_head_backward(int64_t M, int64_t V, int64_t K, void* at
   b.g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(at) + b.pack.bytes);
   b.sums = summed ? reinterpret_cast<float*>(reinterpret_cast<char*>(b.g) + g_bytes) : nullptr;
   b.stacked = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(b.g) + g_bytes + sum_bytes);
-  b.bytes = b.pack.bytes + g_bytes + sum_bytes + (b.half ? 2 * rows * K : 0);
+  const int64_t stacked_bytes = b.half ? 2 * rows * K : 0;
+  b.target_logp = reinterpret_cast<float*>(reinterpret_cast<char*>(b.stacked) + stacked_bytes);
+  b.bytes = b.pack.bytes + g_bytes + sum_bytes + stacked_bytes + 4 * M;
   return b;
 }
 
@@ -1531,6 +1557,11 @@ extern "C" int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int
 
 extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* gout, int32_t gout_stride, const float* inv_count,
                                        void* dh, int64_t lddh, void* dw, int64_t lddw) {
+  return metis_head_backward_kept(a, nullptr, gout, gout_stride, inv_count, dh, lddh, dw, lddw);
+}
+
+extern "C" int32_t metis_head_backward_kept(const metis_head_args* a, const float* target_logp, const float* gout, int32_t gout_stride, const float* inv_count,
+                                            void* dh, int64_t lddh, void* dw, int64_t lddw) {
   if (int32_t rc = check_head(a)) return rc;
   if (!gout || (!dh && !dw)) return fail(METIS_ERR_BAD_ARGUMENT, "gout is null, or nothing is asked for");
   if (gout_stride && inv_count) return fail(METIS_ERR_BAD_ARGUMENT, "inv_count belongs to one gradient for all rows");
@@ -1548,6 +1579,10 @@ extern "C" int32_t metis_head_backward(const metis_head_args* a, const float* go
   DenseParams p = head_params(a, pack);
   p.lse = a->lse; p.gout = gout; p.gout_stride = gout_stride;
   p.half = (int32_t)b.half;
+  p.target_logp = target_logp ? target_logp : b.target_logp;
+  if (!target_logp)
+    METIS_CUDA_OK(launch_counted(kLaunchStream, head_target_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, w, a->ldw, a->target,
+                                 a->ignore_index, a->V, a->M, (int)(a->K / 8), a->scale, (const float*)a->lse, b.target_logp));
   const int64_t rows = b.half ? 2 * b.half : a->M;         // of G
   const DenseOperand of_dw = {b.half ? b.stacked : h.p, b.half ? a->K : h.ld, true};
   if (b.half && dw)

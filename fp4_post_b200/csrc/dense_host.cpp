@@ -26,7 +26,7 @@ namespace {
 
 #define METIS_DENSE_ENTRIES(X)                                                                                             \
   X(metis_last_error_string) X(metis_linear) X(metis_linear_pointwise) X(metis_linear_pointwise_workspace_bytes)          \
-  X(metis_bf16_product) X(metis_bf16_product_workspace_bytes) X(metis_head_loss) X(metis_head_loss_workspace_bytes) X(metis_head_sum) X(metis_head_backward)    \
+  X(metis_bf16_product) X(metis_bf16_product_workspace_bytes) X(metis_head_loss_keep) X(metis_head_loss_workspace_bytes) X(metis_head_sum) X(metis_head_backward_kept) \
   X(metis_head_backward_workspace_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -253,7 +253,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 
 enum HeadForm { kEach, kSum, kMean, kLogprobs };
 
-struct HeadResult { Tensor out, lse, entropy, inv_count; };
+struct HeadResult { Tensor out, lse, logp, entropy, inv_count; };
 
 metis_head_args head_args(const Tensor& h, const Tensor& w, const Tensor& target, const Tensor& lse, int64_t ignore, double scale, int64_t form) {
   Rows rh(h), rw(w);
@@ -272,17 +272,18 @@ metis_head_args head_args(const Tensor& h, const Tensor& w, const Tensor& target
   return a;
 }
 
-HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy) {
+HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy, bool keep) {
   c10::OptionalDeviceGuard guard(h.device());
   const int64_t M = target.numel();
   HeadResult r;
   Tensor each = empty_like_options(h, target.sizes(), at::kFloat);
   r.lse = empty_like_options(h, {M}, at::kFloat);
+  if (keep) r.logp = empty_like_options(h, {M}, at::kFloat);         // (the output is the caller's, who may change it)
   if (entropy) r.entropy = empty_like_options(h, target.sizes(), at::kFloat);
   metis_head_args a = head_args(h, w, target, r.lse, ignore, scale, form);
   const Tensor ws = scratch(h, lib.metis_head_loss_workspace_bytes(a.M, a.V, a.K, entropy));
   a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
-  check(lib.metis_head_loss(&a, ptr<float>(each), ptr<float>(r.entropy)), "metis_head_loss");
+  check(lib.metis_head_loss_keep(&a, ptr<float>(each), ptr<float>(r.entropy), ptr<float>(r.logp)), "metis_head_loss_keep");
   r.out = each;
   if (form == kSum || form == kMean) {
     r.out = empty_like_options(h, {}, at::kFloat);
@@ -294,9 +295,9 @@ HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, 
 
 struct HeadFunction : torch::autograd::Function<HeadFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy) {
-    const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy);
+    const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({h, w, target, r.lse, r.inv_count});
+    ctx->save_for_backward({h, w, target, r.lse, r.logp, r.inv_count});
     ctx->saved_data["o"] = std::vector<int64_t>{ignore, form};
     ctx->saved_data["s"] = scale;
     if (!entropy) return {r.out};
@@ -323,7 +324,7 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
       if (need_w) out[1] = empty_like_options(h, w.sizes(), at::kBFloat16);
       const Tensor ws = scratch(h, lib.metis_head_backward_workspace_bytes(a.M, a.V, a.K));
       a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
-      check(lib.metis_head_backward(&a, ptr<float>(g), each, ptr<float>(saved[4]), ptr(out[0]), a.K, ptr(out[1]), a.K), "metis_head_backward");
+      check(lib.metis_head_backward_kept(&a, ptr<float>(saved[4]), ptr<float>(g), each, ptr<float>(saved[5]), ptr(out[0]), a.K, ptr(out[1]), a.K), "metis_head_backward_kept");
     }
     return once(std::move(out));
   }
@@ -407,7 +408,7 @@ PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       out = r[0];
       if (entropy) ent = r[1];
     } else {
-      const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy != 0);
+      const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy != 0, false);
       out = r.out;
       ent = r.entropy;
     }

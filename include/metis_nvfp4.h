@@ -540,6 +540,9 @@ typedef struct metis_head_args {
 } metis_head_args;
 int64_t metis_head_loss_workspace_bytes(int64_t M, int64_t V, int64_t K, int32_t entropy);
 int32_t metis_head_loss(const metis_head_args* args, float* nll, float* entropy);
+/* The same, with what metis_head_backward_kept takes: target_logp [M] (may be null), the target's log-probability, to 2^-24 of the smaller of
+ * itself and the logits however near 0 it is.  Not set for ignored rows. */
+int32_t metis_head_loss_keep(const metis_head_args* args, float* nll, float* entropy, float* target_logp);
 /* loss = sum of nll, over the number of rows that are not ignored where mean is set; *inv_count = 1 over that number (0 where
  * there is none), or 1. */
 int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_index, int64_t M, int32_t mean, float* loss,
@@ -554,6 +557,10 @@ int32_t metis_head_sum(const float* nll, const int64_t* target, int64_t ignore_i
 int64_t metis_head_backward_workspace_bytes(int64_t M, int64_t V, int64_t K);
 int32_t metis_head_backward(const metis_head_args* args, const float* gout, int32_t gout_stride, const float* inv_count,
                             void* dh, int64_t lddh, void* dw, int64_t lddw);
+/* The same with the target's log-probabilities of metis_head_loss_keep (null: formed from lse again, where softmax(l)[m][target] - 1 is off by 2^-23
+ * of the logit, which for a token of p near 1 may be all of it). */
+int32_t metis_head_backward_kept(const metis_head_args* args, const float* target_logp, const float* gout, int32_t gout_stride, const float* inv_count,
+                                 void* dh, int64_t lddh, void* dw, int64_t lddw);
 
 #ifdef __cplusplus
 }

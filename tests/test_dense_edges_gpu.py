@@ -85,3 +85,63 @@ def test_a_target_of_infinite_logit_or_alone_in_its_vocabulary(M):
     w[t[2], 0] = -float("inf")
     got = dense.token_logprobs(h, w, t)
     assert got[2] == -float("inf") and torch.isfinite(got[:2]).all() and torch.isfinite(got[3:]).all()
+
+
+def exact_logit_gradient(h, w, t, temperature):
+    """softmax - one-hot over the temperature, the target's element without cancellation, in 64 bits."""
+    logp, miss, logits = exact_head(h, w, t, temperature)
+    return torch.softmax(logits, dim=1).scatter(1, t[:, None], -miss[:, None]) / temperature, miss, logits
+
+
+def check_sure_gradients(got, G, h, w, M, off):
+    """Every element of G has the relative error of its logits, and its rounding to bf16 (above 128 rows once, below in two numbers), the
+    gradient its own: by elements, since a row of dh and of dw may be of any size."""
+    g_off = off + (STEP if M > 128 else STEP * STEP)
+    for a, want, reach in ((got[0], G @ w, G.abs() @ w.abs()), (got[1], G.t() @ h, G.abs().t() @ h.abs())):
+        assert a.dtype == torch.bfloat16 and a.shape == want.shape
+        assert ((a.double() - want).abs() <= STEP * want.abs() + 1.1 * g_off * reach).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.6])
+@pytest.mark.parametrize("M,V,K", SURE)
+def test_gradients_of_sure_tokens(M, V, K, temperature):
+    """What a row adds is (1 - p) times a vector of its own size: each row weighed by 1 / (1 - p), all of them count alike in dw."""
+    h, w, t = sure_rows(M, V, K, temperature)
+    G, miss, logits = exact_logit_gradient(h, w, t, temperature)
+    off = 2 * logit_error(h, w, logits, temperature, K) + V * 2.0 ** -24
+    leaves = [h.requires_grad_(True), w.requires_grad_(True)]
+    up = (1 / miss).float()
+    h64, w64 = h.detach().double(), w.detach().double()
+    for out, sign in ((dense.linear_cross_entropy(h, w, t, temperature=temperature, reduction="none"), 1.0), (dense.token_logprobs(h, w, t, temperature=temperature), -1.0)):
+        with torch.no_grad():
+            out.mul_(2)                                                  # the output is the caller's, to change as it likes
+        check_sure_gradients(torch.autograd.grad(out, leaves, up), sign * up.double()[:, None] * G, h64, w64, M, off)
+    loss = dense.linear_cross_entropy(h, w, t, temperature=temperature)
+    check_sure_gradients(torch.autograd.grad(loss, leaves), G / M, h64, w64, M, off)
+
+
+@pytest.mark.parametrize("M", [20, 300])
+def test_the_c_call_without_kept_log_probabilities(M):
+    """metis_head_backward forms the target's log-probability from lse: off by 2^-22 of the logits beside the kept one's error."""
+    from fp4_post_b200 import cabi
+    V, K = 777, 256
+    L = cabi.lib()
+    h, w, t = sure_rows(M, V, K, 1.0)
+    t[1::5] = -100
+    live = t != -100
+    G, _, logits = exact_logit_gradient(h, w, t.clamp(min=0), 1.0)
+    G[~live] = 0
+    lse, nll, g = (torch.empty(M, device="cuda") for _ in range(3))
+    g.fill_(1.0)
+    ws = torch.empty(max(L.metis_head_loss_workspace_bytes(M, V, K, 0), L.metis_head_backward_workspace_bytes(M, V, K)), dtype=torch.uint8, device="cuda")
+    a = cabi.HeadArgs(M=M, V=V, K=K, h=h.data_ptr(), ldh=K, w=w.data_ptr(), ldw=K, target=t.data_ptr(), ignore_index=-100, scale=1.0, lse=lse.data_ptr(),
+                      workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+    assert L.metis_head_loss(a, nll.data_ptr(), None) == 0
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    assert L.metis_head_backward(a, g.data_ptr(), 1, None, dh.data_ptr(), K, dw.data_ptr(), K) == 0
+    off = logit_error(h, w, logits, 1.0, K)
+    h64, w64 = h.double(), w.double()
+    one = torch.zeros_like(G).scatter(1, t.clamp(min=0)[:, None], 2.0 ** -21 * float(logits.abs().max())) * live[:, None]
+    for got, want, reach, extra in ((dh, G @ w64, G.abs() @ w64.abs(), one @ w64.abs()), (dw, G.t() @ h64, G.abs().t() @ h64.abs(), one.t() @ h64.abs())):
+        assert ((got.double() - want).abs() <= STEP * want.abs() + 1.1 * (2 * off + V * 2.0 ** -24 + STEP) * reach + extra).all()
+    assert not dh[~live].any()
