@@ -910,13 +910,14 @@ head_gather_kernel(const __nv_bfloat16* h, int64_t ldh, int64_t M, int pieces, c
   }
 }
 
-// The rows of x twice, `half` apart and zeros between: what a gradient of two parts is contracted with.
+// The rows of x `parts` times, `half` apart and zeros between: what a gradient of two parts is contracted with.  With `target`, zeros in the rows
+// that are ignored: their gradient is 0, but 0 times what they may hold (a NaN of the padding) is not.
 __global__ void __launch_bounds__(256)
-stack_rows_kernel(const __nv_bfloat16* x, int64_t ldx, int64_t M, int64_t half, int64_t pieces, __nv_bfloat16* out) {
+stack_rows_kernel(const __nv_bfloat16* x, int64_t ldx, int64_t M, int parts, int64_t half, int64_t pieces, const int64_t* target, int64_t ignore, __nv_bfloat16* out) {
   grid_dependency_wait();
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < 2 * half * pieces; e += (int64_t)gridDim.x * 256) {
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < parts * half * pieces; e += (int64_t)gridDim.x * 256) {
     const int64_t i = e / pieces, k = e - i * pieces, m = i < half ? i : i - half;
-    reinterpret_cast<uint4*>(out)[e] = m < M ? reinterpret_cast<const uint4*>(x + m * ldx)[k] : make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(out)[e] = m < M && !(target && target[m] == ignore) ? reinterpret_cast<const uint4*>(x + m * ldx)[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -1375,8 +1376,8 @@ extern "C" int64_t metis_bf16_product_workspace_bytes(int64_t M, int64_t N, int6
   return (sp.splits > 1 || (half && !a_mn_major) ? sp.bytes : 0) + (half && a_mn_major ? 4 * (int64_t)half * N : 0);
 }
 
-static int32_t stack_rows(const __nv_bfloat16* x, int64_t ldx, int64_t M, int64_t half, int64_t K, __nv_bfloat16* out, cudaStream_t st) {
-  METIS_CUDA_OK(launch_counted(kLaunchStream, stack_rows_kernel, dim3(row_blocks(ceil_div(2 * half * (K / 8), 32))), dim3(256), 0, st, x, ldx, M, half, K / 8, out));
+static int32_t stack_rows(const __nv_bfloat16* x, int64_t ldx, int64_t M, int parts, int64_t half, int64_t K, const int64_t* target, int64_t ignore, __nv_bfloat16* out, cudaStream_t st) {
+  METIS_CUDA_OK(launch_counted(kLaunchStream, stack_rows_kernel, dim3(row_blocks(ceil_div(parts * half * (K / 8), 32))), dim3(256), 0, st, x, ldx, M, parts, half, K / 8, target, ignore, out));
   return METIS_OK;
 }
 
@@ -1411,7 +1412,7 @@ extern "C" int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t
   float* sums = static_cast<float*>(workspace);
   if (stack_bytes) {
     __nv_bfloat16* stacked = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(workspace) + sum_bytes);
-    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(b), ldb, rows, half, N, stacked, st)) return rc;
+    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(b), ldb, rows, 2, half, N, nullptr, 0, stacked, st)) return rc;
     ob = {stacked, N, true};
   }
   if (!summed) return dense_sum(oa, ob, M, N, K, d, ldd, status, st);
@@ -1525,7 +1526,7 @@ struct HeadBackward {
   HeadPack pack;
   int64_t columns;
   Splits sp;
-  __nv_bfloat16 *g, *stacked;                              // stacked: h twice, for G in two parts
+  __nv_bfloat16 *g, *stacked;                              // stacked: h as dw contracts it with G, twice for two parts
   float* sums;
   float* target_logp;                                      // where the call brings none
   int64_t half;                                            // rows from one part of G to the other; 0: it has one
@@ -1544,7 +1545,7 @@ static HeadBackward plan_head_backward(int64_t M, int64_t V, int64_t K, void* at
   b.g = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(at) + b.pack.bytes);
   b.sums = summed ? reinterpret_cast<float*>(reinterpret_cast<char*>(b.g) + g_bytes) : nullptr;
   b.stacked = reinterpret_cast<__nv_bfloat16*>(reinterpret_cast<char*>(b.g) + g_bytes + sum_bytes);
-  const int64_t stacked_bytes = b.half ? 2 * rows * K : 0;
+  const int64_t stacked_bytes = b.pack.on ? 0 : 2 * rows * K;
   b.target_logp = reinterpret_cast<float*>(reinterpret_cast<char*>(b.stacked) + stacked_bytes);
   b.bytes = b.pack.bytes + g_bytes + sum_bytes + stacked_bytes + 4 * M;
   return b;
@@ -1584,9 +1585,9 @@ extern "C" int32_t metis_head_backward_kept(const metis_head_args* a, const floa
     METIS_CUDA_OK(launch_counted(kLaunchStream, head_target_kernel, dim3(row_blocks(a->M)), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a->h), a->ldh, w, a->ldw, a->target,
                                  a->ignore_index, a->V, a->M, (int)(a->K / 8), a->scale, (const float*)a->lse, b.target_logp));
   const int64_t rows = b.half ? 2 * b.half : a->M;         // of G
-  const DenseOperand of_dw = {b.half ? b.stacked : h.p, b.half ? a->K : h.ld, true};
-  if (b.half && dw)
-    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M, b.half, a->K, b.stacked, st)) return rc;
+  const DenseOperand of_dw = {pack.on ? pack.h : b.stacked, a->K, true};
+  if (!pack.on && dw)
+    if (int32_t rc = stack_rows(static_cast<const __nv_bfloat16*>(a->h), a->ldh, a->M, b.half ? 2 : 1, b.half ? b.half : a->M, a->K, a->target, a->ignore_index, b.stacked, st)) return rc;
   const CommonWeight weight = gout_stride ? CommonWeight{} : CommonWeight{gout, inv_count, a->scale};
   for (int64_t v0 = 0; v0 < a->V; v0 += b.columns) {
     const int64_t n = a->V - v0 < b.columns ? a->V - v0 : b.columns;

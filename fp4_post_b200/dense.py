@@ -116,7 +116,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
     hidden [..., K] and weight [V, K] bf16, target [...] int64 or int32.  The logits are formed tile by tile in fp32 and folded
     into each row's maximum and sum; the backward pass forms them again, piece by piece of the vocabulary, and differentiates
-    hidden and weight (once).  A target that is neither ignore_index nor in the vocabulary makes its loss NaN.  The mean over no
+    hidden and weight (once).  A row whose target is ignore_index adds nothing, whatever it holds.  A target that is neither ignore_index nor in the vocabulary makes its loss NaN.  The mean over no
     row at all is NaN, as torch has it."""
     try:
         form = _FORMS[reduction]

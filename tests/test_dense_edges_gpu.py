@@ -145,3 +145,29 @@ def test_the_c_call_without_kept_log_probabilities(M):
     for got, want, reach, extra in ((dh, G @ w64, G.abs() @ w64.abs(), one @ w64.abs()), (dw, G.t() @ h64, G.abs().t() @ h64.abs(), one.t() @ h64.abs())):
         assert ((got.double() - want).abs() <= STEP * want.abs() + 1.1 * (2 * off + V * 2.0 ** -24 + STEP) * reach + extra).all()
     assert not dh[~live].any()
+
+
+# ---- ignored rows --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("M,V,K", [(1, 97, 64), (20, 97, 64), (64, 300, 136), (100, 513, 64), (128, 300, 64), (129, 300, 64), (700, 1003, 128), (4129, 131100, 1024)])
+def test_ignored_rows_may_hold_anything(M, V, K):
+    """The same bits as with zeros there, on either side of every rule of size (the last is long enough for the rows to be packed)."""
+    h, w = normal(M, K), normal(V, K, scale=K ** -0.5, seed=1)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    t = torch.randint(0, V, (M,), device="cuda", generator=gen)
+    off = torch.rand(M, device="cuda", generator=gen) < 0.4
+    off[0] = True
+    t[off] = -100
+    bad = h.clone()
+    bad[off] = torch.tensor([float("nan"), float("inf"), -float("inf"), 3.3e38], device="cuda").bfloat16()[torch.arange(int(off.sum()) * K, device="cuda") % 4].view(-1, K)
+    h[off] = 0
+    g = normal(M, seed=9, dtype=torch.float32)
+    w.requires_grad_(True)
+    got = []
+    for x in (h, bad):
+        x.requires_grad_(True)
+        loss = dense.linear_cross_entropy(x, w, t, reduction="sum")
+        logp, ent = dense.token_logprobs(x, w, t, entropy=True)
+        got.append((loss.detach(), logp.detach(), ent, *torch.autograd.grad(loss, (x, w)), *torch.autograd.grad(logp, (x, w), g), *torch.autograd.grad(dense.linear_cross_entropy(x, w, t), w)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
