@@ -10,12 +10,14 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <string.h>
@@ -339,6 +341,20 @@ bool tensor_or_none(PyObject* o, Tensor* t) {
   return true;
 }
 
+// What torch records of its own operations and these calls do not show it: their answers would come without their derivative, or as constants
+// of the trace, and nobody would know.  (Wrappers of function transforms have no data to read, and raise where it is read.)
+void check_followed(std::initializer_list<const Tensor*> tensors) {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !(Modes::any_modes_set() && (Modes::get_mode(Mode::PROXY) || Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::FUNCTIONAL))),
+              "the bf16 products cannot be traced: they are no operations of torch");
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(!t->_fw_grad(0).defined(), "the bf16 products have no forward-mode derivative");
+    TORCH_CHECK(!t->unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python), "the bf16 products take no tensor subclass that dispatches by itself");
+  }
+}
+
 // x, weight, bias or None, gate or None, residual or None, activation -> the output, or None where dense.py has to look at the arguments first
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -352,6 +368,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!tensor_or_none(args[0], &x) || !tensor_or_none(args[1], &w) || !tensor_or_none(args[2], &bias) || !tensor_or_none(args[3], &gate) ||
       !tensor_or_none(args[4], &residual) || !x.defined() || !w.defined())
     Py_RETURN_NONE;
+  check_followed({&x, &w, &bias, &gate, &residual});
   if (!plain(x, x, at::kBFloat16) || !plain(w, x, at::kBFloat16) || w.dim() != 2 || x.dim() < 1) Py_RETURN_NONE;
   Rows rx(x), rw(w);
   if (!operand(x, rx) || !operand(w, rw) || rx.cols != rw.cols || rw.rows == 0 || rw.cols == 0 || rw.cols % 8 != 0) Py_RETURN_NONE;
@@ -395,6 +412,7 @@ PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (entropy < 0) return nullptr;
   if (!tensor_or_none(args[0], &h) || !tensor_or_none(args[1], &w) || !tensor_or_none(args[2], &target) || !h.defined() || !w.defined() || !target.defined())
     Py_RETURN_NONE;
+  check_followed({&h, &w, &target});
   if (!plain(h, h, at::kBFloat16) || !plain(w, h, at::kBFloat16) || !plain(target, h, at::kLong) || w.dim() != 2 || h.dim() < 1) Py_RETURN_NONE;
   Rows rh(h), rw(w);
   if (!operand(h, rh) || !operand(w, rw) || rh.cols != rw.cols || rw.rows == 0 || rw.cols == 0 || rw.cols % 8 != 0 || rh.rows == 0) Py_RETURN_NONE;

@@ -62,16 +62,20 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return x * cos + torch.cat((-x2, x1), dim=-1) * sin
 
 
-def _native(*tensors) -> bool:
-    """Inference on plain bf16 CUDA tensors: the elementwise pieces run as one launch each, with the same roundings.  Whatever
-    has to see the torch operations gets them: autograd, forward-mode derivatives (which no_grad leaves on), vmap and the
-    other function transforms, tensor subclasses, dispatch modes, tracing."""
+def _plain(*tensors) -> bool:
+    """Plain bf16 CUDA tensors of one device that only autograd follows: the library's own calls may take them.  Whatever has to see the
+    torch operations gets them: forward-mode derivatives (which no_grad leaves on), vmap and the other function transforms, tensor subclasses,
+    dispatch modes, tracing."""
     first = tensors[0]
-    return (not torch.is_grad_enabled()
-            and all(type(t) in (torch.Tensor, nn.Parameter) and t.is_cuda and t.dtype == torch.bfloat16 and t.device == first.device
-                    and t.numel() > 0 and forward_ad.unpack_dual(t).tangent is None for t in tensors)
+    return (not torch.jit.is_tracing() and not torch.compiler.is_compiling()
             and torch._C._functorch.peek_interpreter_stack() is None and torch._C._len_torch_dispatch_stack() == 0
-            and not torch.compiler.is_compiling() and not torch.jit.is_tracing())
+            and all(type(t) in (torch.Tensor, nn.Parameter) and t.is_cuda and t.dtype == torch.bfloat16 and t.device == first.device
+                    and t.numel() > 0 and forward_ad.unpack_dual(t).tangent is None for t in tensors))
+
+
+def _native(*tensors) -> bool:
+    """Inference on such tensors: the elementwise pieces run as one launch each, with the same roundings."""
+    return not torch.is_grad_enabled() and _plain(*tensors)
 
 
 def _table_of(t: torch.Tensor, T: int, D: int) -> bool:
@@ -80,8 +84,8 @@ def _table_of(t: torch.Tensor, T: int, D: int) -> bool:
 
 
 def _dense_weight(weight: torch.Tensor, *tensors) -> bool:
-    """Whether dense.py takes this weight with these tensors: bf16 on one CUDA device, an inner size that 8 divides."""
-    return weight.shape[1] % 8 == 0 and all(t.is_cuda and t.dtype == torch.bfloat16 and t.device == weight.device for t in (weight, *tensors))
+    """Whether dense.py takes this weight with these tensors: plain ones, an inner size that 8 divides."""
+    return _plain(weight, *tensors) and weight.shape[1] % 8 == 0
 
 
 def _project(module: nn.Module, x: torch.Tensor, fuse: bool, *, activation=None, gate=None, residual=None):

@@ -10,6 +10,7 @@ nothing here computes on the CPU.  Operands are bfloat16, sums and softmax stati
 have any pitch that 16 bytes divide (others are copied first).  A call runs on the current stream of its tensors' device and can be
 captured in a CUDA graph.  The calls and their gradients are native (csrc/dense_host.cpp); what is here is what they refuse, and the
 copies of tensors that the kernels cannot read as they lie.
+They are no operations of torch: forward-mode derivatives, function transforms, traces and tensor subclasses that dispatch are refused.
 The reference leaves all of this to torch (nn.Linear, F.cross_entropy and TRL's selective log-softmax around src/grpo/grpo.py:199-215).
 """
 from __future__ import annotations
@@ -116,8 +117,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
     hidden [..., K] and weight [V, K] bf16, target [...] int64 or int32.  The logits are formed tile by tile in fp32 and folded
     into each row's maximum and sum; the backward pass forms them again, piece by piece of the vocabulary, and differentiates
-    hidden and weight (once).  A row whose target is ignore_index adds nothing, whatever it holds.  A target that is neither ignore_index nor in the vocabulary makes its loss NaN.  The mean over no
-    row at all is NaN, as torch has it."""
+    hidden and weight (once).  A row whose target is ignore_index adds nothing, whatever it holds.  A target that is neither
+    ignore_index nor in the vocabulary makes its loss NaN.  The mean over no row at all is NaN, as torch has it."""
     try:
         form = _FORMS[reduction]
     except (KeyError, TypeError):

@@ -35,3 +35,35 @@ def test_the_head_with_kept_log_probabilities_refuses_what_it_does_without(L, p)
     assert L.metis_head_backward_kept(head_args(p), p, None, 0, None, p, 16, p, 16) == -1
     assert L.metis_head_backward_kept(head_args(p), p, p, 1, p, p, 16, p, 16) == -1
     assert L.metis_head_backward_kept(head_args(p), p, p, 0, None, None, 16, None, 16) == -1
+
+
+def test_what_torch_would_not_see_is_refused(built_library):
+    """Forward-mode derivatives and traces: the calls would return without a tangent, or as a constant of the trace."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, y = torch.zeros(4, 16), torch.zeros(24, 16), torch.zeros(24), torch.zeros(4, 24)
+    x, w, b, y = (t.bfloat16() for t in (x, w, b, y))
+    t = torch.zeros(4, dtype=torch.int64)
+    calls = [lambda x, w, b, y: dense.linear(x, w, b, gate=y, residual=y), lambda x, w, b, y: dense.linear_cross_entropy(x, w, t), lambda x, w, b, y: dense.token_logprobs(x, w, t)]
+    for call in calls:
+        for i in range(2):
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(*(forward_ad.make_dual(v, torch.ones_like(v)) if j == i else v for j, v in enumerate((x, w, b, y))))
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (x, w, b, y), check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(call)(x, w, b, y)
+    for kind in ("bias", "gate", "residual"):
+        v = dict(bias=b, gate=y, residual=y)[kind]
+        with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            dense.linear(x, w, **{kind: forward_ad.make_dual(v, torch.ones_like(v))})
+
+    class Logged(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with pytest.raises(RuntimeError, match="subclass"):
+        dense.linear(torch.Tensor._make_subclass(Logged, x), w)
+    # outside of all that they are refused as before
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        dense.linear(x, w)

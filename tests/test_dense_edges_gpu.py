@@ -171,3 +171,49 @@ def test_ignored_rows_may_hold_anything(M, V, K):
         got.append((loss.detach(), logp.detach(), ent, *torch.autograd.grad(loss, (x, w)), *torch.autograd.grad(logp, (x, w), g), *torch.autograd.grad(dense.linear_cross_entropy(x, w, t), w)))
     for a, b in zip(*got):
         assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+# ---- the decoder where torch has to see the operations ---------------------------------------------------------------
+
+@pytest.fixture()
+def decoders():
+    from fp4_post_b200.decoder import Decoder, DecoderConfig
+    cfg = DecoderConfig(hidden=256, layers=2, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1003)
+    torch.manual_seed(0)
+    plain = Decoder(cfg, fuse_norms=False).cuda().bfloat16()
+    fused = Decoder(cfg, fuse_norms=False, fuse_dense=True).cuda().bfloat16()
+    fused.load_state_dict(plain.state_dict())
+    return plain, fused, torch.randint(0, cfg.vocab, (3, 65), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+
+
+def mlp(model):
+    return lambda h: model.layers[0].mlp(h)
+
+
+@pytest.mark.parametrize("record", [False, True])
+def test_forward_mode_derivatives_pass_through_the_fused_decoder(decoders, record):
+    from torch.autograd import forward_ad
+    plain, fused, ids = decoders
+    h, dh = normal(3, 65, 256), normal(3, 65, 256, seed=1)
+    got = []
+    for model in (plain, fused):
+        model.hidden = lambda ids: forward_ad.make_dual(h, dh)
+        with forward_ad.dual_level(), torch.set_grad_enabled(record):
+            outs = (model.layers[0].mlp(forward_ad.make_dual(h, dh)), model.loss(ids), model.token_logprobs(ids))
+            got.append([t for out in outs for t in forward_ad.unpack_dual(out)])
+    for a, b in zip(*got):
+        assert a is not None and torch.equal(a, b)
+
+
+def test_traces_and_transforms_of_the_fused_decoder_are_those_of_the_plain_one(decoders):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    plain, fused, _ = decoders
+    h, other = normal(3, 65, 256), normal(3, 65, 256, seed=1)
+    with torch.no_grad():
+        traced = torch.jit.trace(fused.layers[0].mlp, (h,), check_trace=False)
+        as_graph = make_fx(mlp(fused))(h)
+    want = plain.layers[0].mlp(other).detach()             # (with gradients on: silu and product are torch's, as those of a trace are)
+    assert torch.equal(traced(other), want) and torch.equal(as_graph(other), want)
+    assert torch.equal(torch.vmap(mlp(fused))(torch.stack((other, h))), torch.vmap(mlp(plain))(torch.stack((other, h))))
+    grads = [torch.func.grad(lambda x: mlp(m)(x).float().sum())(other) for m in (plain, fused)]
+    assert torch.equal(*grads)
