@@ -88,6 +88,15 @@ def _dense_weight(weight: torch.Tensor, *tensors) -> bool:
     return _plain(weight, *tensors) and weight.shape[1] % 8 == 0
 
 
+def _bare(module: nn.Module, kind: type) -> bool:
+    """Whether calling the module is no more than calling kind.forward: nothing derived, no hook of its own or of all modules, no forward put in
+    its place."""
+    g = nn.modules.module
+    return (type(module) is kind and "forward" not in vars(module)
+            and not any((module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks, g._global_forward_hooks,
+                         g._global_forward_pre_hooks, g._global_backward_hooks, g._global_backward_pre_hooks)))
+
+
 def _project(module: nn.Module, x: torch.Tensor, fuse: bool, *, activation=None, gate=None, residual=None):
     """activation(module(x)) * gate + residual, in one kernel where the module is a plain linear layer in bf16."""
     if fuse and type(module) is nn.Linear and _dense_weight(module.weight, x, *(t for t in (gate, residual, module.bias) if t is not None)):
@@ -149,6 +158,7 @@ class Block(nn.Module):
     def __init__(self, cfg: DecoderConfig, fuse_norms: bool, fuse_dense: bool = False):
         super().__init__()
         self.fuse_norms = fuse_norms
+        self.fuse_dense = fuse_dense
         self.input_layernorm = RMSNorm(cfg.hidden, cfg.eps)
         self.self_attn = Attention(cfg, fuse_dense)
         self.post_attention_layernorm = RMSNorm(cfg.hidden, cfg.eps)
@@ -161,8 +171,12 @@ class Block(nn.Module):
         return norm(x)
 
     def forward(self, x, cos, sin):
-        x = self.self_attn(self._normed(self.input_layernorm, x, self.self_attn.q_proj), cos, sin, x)
-        return self.mlp(self._normed(self.post_attention_layernorm, x, self.mlp.gate_proj), x)
+        # (the residual goes into a branch's last projection where nobody can see the branch by itself, or has put another module there)
+        attn, mlp = self.self_attn, self.mlp
+        h = self._normed(self.input_layernorm, x, attn.q_proj)
+        x = attn(h, cos, sin, x) if self.fuse_dense and _bare(attn, Attention) else x + attn(h, cos, sin)
+        h = self._normed(self.post_attention_layernorm, x, mlp.gate_proj)
+        return mlp(h, x) if self.fuse_dense and _bare(mlp, MLP) else x + mlp(h)
 
 
 class Decoder(nn.Module):
@@ -193,26 +207,34 @@ class Decoder(nn.Module):
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         return self.lm_head(self.hidden(ids))
 
-    def _fused_head(self, hidden: torch.Tensor) -> bool:
-        return self.fuse_dense and type(self.lm_head) is nn.Linear and _dense_weight(self.lm_head.weight, hidden)
+    def _fused_head(self) -> bool:
+        """Whether the head may be taken without its logits: they come from this class's forward, and from nothing put in its place."""
+        return self.fuse_dense and type(self).forward is Decoder.forward and "forward" not in vars(self) and type(self.lm_head) is nn.Linear
 
     def loss(self, ids: torch.Tensor) -> torch.Tensor:
         """Next-token cross entropy on the given ids."""
-        hidden = self.hidden(ids)
-        if self._fused_head(hidden):
-            target = Fn.pad(ids[:, 1:], (0, 1), value=-100)                  # the last position of a row has no next token
-            return dense.linear_cross_entropy(hidden, self.lm_head.weight, target)
-        logits = self.lm_head(hidden)
+        if self._fused_head():
+            hidden = self.hidden(ids)
+            if _dense_weight(self.lm_head.weight, hidden):
+                target = Fn.pad(ids[:, 1:], (0, 1), value=-100)              # the last position of a row has no next token
+                return dense.linear_cross_entropy(hidden, self.lm_head.weight, target)
+            logits = self.lm_head(hidden)
+        else:
+            logits = self.forward(ids)
         return Fn.cross_entropy(logits[:, :-1].reshape(-1, logits.shape[-1]).float(), ids[:, 1:].reshape(-1))
 
     def token_logprobs(self, ids: torch.Tensor, temperature: float = 1.0, entropy: bool = False):
         """Log-probabilities of each row's tokens behind the first, fp32 [B, T - 1] (and the entropies of their distributions, without
         gradient): what a policy-gradient step takes of the policy and of its reference."""
-        hidden = self.hidden(ids)
-        if self._fused_head(hidden):
-            target = Fn.pad(ids[:, 1:], (0, 1), value=-100)
-            out = dense.token_logprobs(hidden, self.lm_head.weight, target, temperature=temperature, entropy=entropy)
-            return (out[0][:, :-1], out[1][:, :-1]) if entropy else out[:, :-1]
-        logp = torch.log_softmax(self.lm_head(hidden)[:, :-1].float() / temperature, dim=-1)
+        if self._fused_head():
+            hidden = self.hidden(ids)
+            if _dense_weight(self.lm_head.weight, hidden):
+                target = Fn.pad(ids[:, 1:], (0, 1), value=-100)
+                out = dense.token_logprobs(hidden, self.lm_head.weight, target, temperature=temperature, entropy=entropy)
+                return (out[0][:, :-1], out[1][:, :-1]) if entropy else out[:, :-1]
+            logits = self.lm_head(hidden)
+        else:
+            logits = self.forward(ids)
+        logp = torch.log_softmax(logits[:, :-1].float() / temperature, dim=-1)
         picked = logp.gather(-1, ids[:, 1:, None])[..., 0]
         return (picked, -(logp.detach().exp() * logp.detach()).sum(dim=-1)) if entropy else picked

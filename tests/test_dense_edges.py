@@ -67,3 +67,76 @@ def test_what_torch_would_not_see_is_refused(built_library):
     # outside of all that they are refused as before
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         dense.linear(x, w)
+
+
+# ---- the decoder ---------------------------------------------------------------------------------------------------
+
+def tiny(**options):
+    from fp4_post_b200.decoder import Decoder, DecoderConfig
+    torch.manual_seed(0)
+    model = Decoder(DecoderConfig(hidden=64, layers=2, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=97), **options)
+    return model, torch.randint(0, 97, (2, 12))
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_hooks_see_the_branches_of_a_block_without_the_residual(fuse):
+    model, ids = tiny(fuse_dense=fuse)
+    want = model(ids)
+    block, seen = model.layers[0], {}
+    handles = [m.register_forward_hook(lambda m, args, out, name=name: seen.update({name: (len(args), out)})) for name, m in (("attn", block.self_attn), ("mlp", block.mlp))]
+    x = model.embed_tokens(ids)
+    cos, sin = model.rotary(ids.shape[1], ids.device, x.dtype)
+    out = block(x, cos, sin)
+    for handle in handles:
+        handle.remove()
+    (n_attn, a), (n_mlp, b) = seen["attn"], seen["mlp"]
+    assert n_attn == 3 and n_mlp == 1
+    h = x + block.self_attn(block.input_layernorm(x), cos, sin)
+    assert torch.equal(a, block.self_attn(block.input_layernorm(x), cos, sin)) and torch.equal(b, block.mlp(block.post_attention_layernorm(h)))
+    assert torch.equal(out, x + a + b) and torch.equal(model(ids), want)
+    seen.clear()
+    with torch.nn.modules.module.register_module_forward_hook(lambda m, args, out: seen.update({id(m): out})):
+        block(x, cos, sin)
+    assert torch.equal(seen[id(block.self_attn)], a) and torch.equal(seen[id(block.mlp)], b)
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_modules_put_in_the_place_of_a_blocks_own(fuse):
+    model, ids = tiny(fuse_dense=fuse)
+    want, block = model(ids), model.layers[1]
+
+    class Twice(torch.nn.Module):                           # what stood there, through the arguments that it takes
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def __getattr__(self, name):
+            return getattr(super().__getattr__("inner"), name) if name != "inner" else super().__getattr__(name)
+
+        def forward(self, *args):
+            assert len(args) in (1, 3)
+            return self.inner(*args)
+    block.self_attn, block.mlp = Twice(block.self_attn), Twice(block.mlp)
+    assert torch.equal(model(ids), want)
+    inner = model.layers[0].mlp.forward
+    model.layers[0].mlp.forward = lambda h: inner(h)        # a forward of the instance's own
+    assert torch.equal(model(ids), want)
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_the_loss_is_that_of_an_overridden_forward(fuse):
+    from fp4_post_b200.decoder import Decoder
+
+    class Cold(Decoder):
+        def forward(self, ids):
+            return super().forward(ids) * 0.5
+    model, ids = tiny(fuse_dense=fuse)
+    want = torch.nn.functional.cross_entropy(0.5 * model(ids)[:, :-1].reshape(-1, 97), ids[:, 1:].reshape(-1))
+    plain = model.loss(ids)
+    model.__class__ = Cold
+    assert torch.equal(model.loss(ids), want) and not torch.equal(want, plain)
+    torch.testing.assert_close(-model.token_logprobs(ids).mean(), want)
+    model.__class__ = Decoder
+    forward = model.forward
+    model.forward = lambda ids: forward(ids) * 0.5
+    assert torch.equal(model.loss(ids), want)
