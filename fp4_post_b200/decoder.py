@@ -98,8 +98,8 @@ def _bare(module: nn.Module, kind: type) -> bool:
 
 
 def _project(module: nn.Module, x: torch.Tensor, fuse: bool, *, activation=None, gate=None, residual=None):
-    """activation(module(x)) * gate + residual, in one kernel where the module is a plain linear layer in bf16."""
-    if fuse and type(module) is nn.Linear and _dense_weight(module.weight, x, *(t for t in (gate, residual, module.bias) if t is not None)):
+    """activation(module(x)) * gate + residual, in one kernel where the module is a plain linear layer in bf16, its weight what its forward takes."""
+    if fuse and _bare(module, nn.Linear) and _dense_weight(module.weight, x, *(t for t in (gate, residual, module.bias) if t is not None)):
         return dense.linear(x, module.weight, module.bias, activation=activation, gate=gate, residual=residual)
     y = module(x)
     if activation == "silu":
@@ -143,7 +143,7 @@ class MLP(nn.Module):
         self.down_proj = nn.Linear(cfg.ffn, cfg.hidden, bias=False)
 
     def forward(self, h, residual=None):
-        if self.fuse_dense and type(self.gate_proj) is nn.Linear:
+        if self.fuse_dense and _bare(self.gate_proj, nn.Linear):
             act = _project(self.gate_proj, h, True, activation="silu", gate=self.up_proj(h))
         else:
             gate, up = forward_group((self.gate_proj, self.up_proj), h)
@@ -209,7 +209,7 @@ class Decoder(nn.Module):
 
     def _fused_head(self) -> bool:
         """Whether the head may be taken without its logits: they come from this class's forward, and from nothing put in its place."""
-        return self.fuse_dense and type(self).forward is Decoder.forward and "forward" not in vars(self) and type(self.lm_head) is nn.Linear
+        return self.fuse_dense and type(self).forward is Decoder.forward and "forward" not in vars(self) and _bare(self.lm_head, nn.Linear)
 
     def loss(self, ids: torch.Tensor) -> torch.Tensor:
         """Next-token cross entropy on the given ids."""

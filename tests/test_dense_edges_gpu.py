@@ -217,3 +217,46 @@ def test_traces_and_transforms_of_the_fused_decoder_are_those_of_the_plain_one(d
     assert torch.equal(torch.vmap(mlp(fused))(torch.stack((other, h))), torch.vmap(mlp(plain))(torch.stack((other, h))))
     grads = [torch.func.grad(lambda x: mlp(m)(x).float().sum())(other) for m in (plain, fused)]
     assert torch.equal(*grads)
+
+
+def test_hooks_of_plain_layers_run_in_the_fused_decoder(decoders):
+    plain, fused, ids = decoders
+    ran = {}
+    names = ["self_attn.o_proj", "mlp.gate_proj", "mlp.down_proj", "lm_head"]
+
+    def layers(model):
+        return [model.layers[0].get_submodule(n) if n != "lm_head" else model.lm_head for n in names]
+    for model in (plain, fused):
+        for name, m in zip(names, layers(model)):
+            m.register_forward_hook(lambda m, args, out, key=(model, name): (ran.update({key: 1 + ran.get(key, 0)}), 1.25 * out)[1])
+            m.register_full_backward_hook(lambda m, gi, go, key=(model, name, "backward"): ran.update({key: 1 + ran.get(key, 0)}))
+    want, loss = plain.loss(ids), fused.loss(ids)
+    want.backward()
+    loss.backward()
+    plain.token_logprobs(ids), fused.token_logprobs(ids)
+    for name in names:
+        assert ran[plain, name] == ran[fused, name] == 2 and ran[plain, name, "backward"] == ran[fused, name, "backward"] == 1
+    # (the second block of the fused one runs on dense.py: roundings between its kernels, as in the decoder's own comparison)
+    assert abs(float(loss.detach()) - float(want.detach())) <= 2e-3 * float(want.detach())
+
+
+def test_a_weight_that_a_hook_makes_is_the_one_that_is_used(decoders):
+    """weight_norm keeps the layer's type and puts its weight together in a hook in front of forward."""
+    plain, fused, ids = decoders
+    for model in (plain, fused):
+        for m in (model.layers[0].mlp.gate_proj, model.layers[1].self_attn.o_proj, model.lm_head):
+            torch.nn.utils.weight_norm(m)
+            with torch.no_grad():
+                m.weight_g.mul_(3)                          # (the weight of the last forward pass is stale now)
+    with torch.no_grad():
+        for model in (plain, fused):
+            model.layers[0].mlp.down_proj.weight.zero_()    # (nothing on dense.py stays between the two that rounds apart)
+            model.layers[1].mlp.down_proj.weight.zero_()
+            model.layers[0].self_attn.o_proj.weight.zero_()
+        assert torch.equal(plain.loss(ids), fused.loss(ids))
+        assert torch.equal(plain.token_logprobs(ids), fused.token_logprobs(ids))
+        for model in (plain, fused):
+            model.layers[0].mlp.down_proj.weight.copy_(torch.eye(256, 512))
+        h = normal(2, 5, 256)
+        a, b = plain.layers[0].mlp(h), fused.layers[0].mlp(h)
+        assert a.any() and torch.equal(a, b)                # one product by 1: no rounding of the down projection's
