@@ -111,11 +111,20 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// The caller's status word, for the launches of the backward pass: no saved variable, so that the caller may set it back to 0 in between.
+void keep_status(AutogradContext* ctx, const Tensor& status) {
+  if (status.defined()) ctx->saved_data["status"] = status;
+}
+Tensor kept_status(AutogradContext* ctx) {
+  const auto it = ctx->saved_data.find("status");
+  return it == ctx->saved_data.end() ? Tensor() : it->second.toTensor();
+}
+
 // ---- linear -------------------------------------------------------------------------------------------------------
 
 struct LinearResult { Tensor y, act, slope; };
 
-LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& gate, const Tensor& residual, int64_t act, bool keep_act, bool keep_slope) {
+LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& gate, const Tensor& residual, int64_t act, bool keep_act, bool keep_slope, const Tensor& status) {
   c10::OptionalDeviceGuard guard(x.device());
   Rows rx(x), rw(w);
   operand(x, rx);
@@ -138,37 +147,39 @@ LinearResult linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias
   a.y = out.y.data_ptr(); a.ldy = a.N;
   a.act = ptr(out.act); a.ldact = pitch;
   a.slope = ptr(out.slope); a.ldslope = pitch;
+  a.status = ptr<int32_t>(status);
   a.stream = stream_of(x);
   check(lib.metis_linear(&a), "metis_linear");
   return out;
 }
 
 // a b, or a^T b with `mn`, for matrices of 16-byte aligned rows
-Tensor product(const Tensor& a, const Rows& ra, bool mn, int32_t half, const Tensor& b, const Rows& rb) {
+Tensor product(const Tensor& a, const Rows& ra, bool mn, int32_t half, const Tensor& b, const Rows& rb, const Tensor& status) {
   const int64_t M = mn ? ra.cols : ra.rows, K = mn ? ra.rows : ra.cols;
   const Tensor d = empty_like_options(b, {M, rb.cols}, at::kBFloat16);
   const int64_t bytes = lib.metis_bf16_product_workspace_bytes(M, rb.cols, K, mn, half);
   const Tensor ws = bytes > 0 ? scratch(b, bytes) : Tensor();
-  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, half, d.data_ptr(), rb.cols, ptr(ws), bytes, nullptr, stream_of(b)), "metis_bf16_product");
+  check(lib.metis_bf16_product(a.data_ptr(), mn, ra.ld, b.data_ptr(), rb.ld, M, rb.cols, K, half, d.data_ptr(), rb.cols, ptr(ws), bytes, ptr<int32_t>(status), stream_of(b)), "metis_bf16_product");
   return d;
 }
 
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, const std::optional<Tensor>& gate,
-                        const std::optional<Tensor>& residual, int64_t act) {
+                        const std::optional<Tensor>& residual, int64_t act, const Tensor* status) {
     const Tensor b = bias.value_or(Tensor()), g = gate.value_or(Tensor());
     const bool through = x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad());
     const bool gated = g.defined() && g.requires_grad();
-    const LinearResult out = linear_forward(x, weight, b, g, residual.value_or(Tensor()), act, gated, act != METIS_ACT_NONE && through);
+    const LinearResult out = linear_forward(x, weight, b, g, residual.value_or(Tensor()), act, gated, act != METIS_ACT_NONE && through, *status);
     ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), x.requires_grad() ? weight : Tensor(), through ? g : Tensor(), out.act, out.slope});
     ctx->saved_data["s"] = std::vector<int64_t>{act, bias.has_value(), gate.has_value(), residual.has_value(),
                                                 b.defined() && b.scalar_type() == at::kFloat, weight.size(0), weight.size(1)};
     ctx->saved_data["x"] = x.sizes().vec();
+    keep_status(ctx, *status);
     return out.y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(6);
+    variable_list out(7);
     if (!grads[0].defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
     const std::vector<int64_t> o = ctx->saved_data["s"].toIntVector(), x_shape = ctx->saved_data["x"].toIntVector();
@@ -206,6 +217,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         Rows rdz = rdy;
         const bool write_dz = product_wanted && (epilogue || !operand(dy, rdz));
         Tensor dz = dy;
+        const Tensor status = kept_status(ctx);
         const int32_t half = product_wanted && epilogue && M <= METIS_TWO_PART_ROWS ? (int32_t)(M + 7) / 8 * 8 : 0;      // (dy as it is has one part)
         if (write_dz || need_b || need_gate) {
           metis_linear_pointwise_args a = {};
@@ -238,12 +250,12 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         if (need_x) {
           Rows rw(saved[1]);
           operand(saved[1], rw);
-          out[0] = product(dz, rdz, false, half, saved[1], rw).view(x_shape);
+          out[0] = product(dz, rdz, false, half, saved[1], rw, status).view(x_shape);
         }
         if (need_w) {
           Rows rx(saved[0]);
           operand(saved[0], rx);
-          out[1] = product(dz, rdz, true, half, saved[0], rx);
+          out[1] = product(dz, rdz, true, half, saved[0], rx, status);
         }
       }
     }
@@ -257,7 +269,7 @@ enum HeadForm { kEach, kSum, kMean, kLogprobs };
 
 struct HeadResult { Tensor out, lse, logp, entropy, inv_count; };
 
-metis_head_args head_args(const Tensor& h, const Tensor& w, const Tensor& target, const Tensor& lse, int64_t ignore, double scale, int64_t form) {
+metis_head_args head_args(const Tensor& h, const Tensor& w, const Tensor& target, const Tensor& lse, int64_t ignore, double scale, int64_t form, const Tensor& status) {
   Rows rh(h), rw(w);
   operand(h, rh);
   operand(w, rw);
@@ -270,11 +282,12 @@ metis_head_args head_args(const Tensor& h, const Tensor& w, const Tensor& target
   a.scale = (float)scale;
   a.negate = form == kLogprobs;
   a.lse = ptr<float>(lse);
+  a.status = ptr<int32_t>(status);
   a.stream = stream_of(h);
   return a;
 }
 
-HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy, bool keep) {
+HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy, bool keep, const Tensor& status) {
   c10::OptionalDeviceGuard guard(h.device());
   const int64_t M = target.numel();
   HeadResult r;
@@ -282,7 +295,7 @@ HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, 
   r.lse = empty_like_options(h, {M}, at::kFloat);
   if (keep) r.logp = empty_like_options(h, {M}, at::kFloat);         // (the output is the caller's, who may change it)
   if (entropy) r.entropy = empty_like_options(h, target.sizes(), at::kFloat);
-  metis_head_args a = head_args(h, w, target, r.lse, ignore, scale, form);
+  metis_head_args a = head_args(h, w, target, r.lse, ignore, scale, form, status);
   const Tensor ws = scratch(h, lib.metis_head_loss_workspace_bytes(a.M, a.V, a.K, entropy));
   a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
   check(lib.metis_head_loss_keep(&a, ptr<float>(each), ptr<float>(r.entropy), ptr<float>(r.logp)), "metis_head_loss_keep");
@@ -296,19 +309,21 @@ HeadResult head_forward(const Tensor& h, const Tensor& w, const Tensor& target, 
 }
 
 struct HeadFunction : torch::autograd::Function<HeadFunction> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy) {
-    const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy, true);
+  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, double scale, int64_t form, bool entropy,
+                               const Tensor* status) {
+    const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy, true, *status);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({h, w, target, r.lse, r.logp, r.inv_count});
     ctx->saved_data["o"] = std::vector<int64_t>{ignore, form};
     ctx->saved_data["s"] = scale;
+    keep_status(ctx, *status);
     if (!entropy) return {r.out};
     ctx->mark_non_differentiable({r.entropy});
     return {r.out, r.entropy};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(7);
+    variable_list out(8);
     if (!grads[0].defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
     const std::vector<int64_t> o = ctx->saved_data["o"].toIntVector();
@@ -318,7 +333,7 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
       at::AutoGradMode off(false);
       const Tensor &h = saved[0], &w = saved[1];
       c10::OptionalDeviceGuard guard(h.device());
-      metis_head_args a = head_args(h, w, saved[2], saved[3], o[0], ctx->saved_data["s"].toDouble(), o[1]);
+      metis_head_args a = head_args(h, w, saved[2], saved[3], o[0], ctx->saved_data["s"].toDouble(), o[1], kept_status(ctx));
       Tensor g = grads[0].reshape({-1});
       const bool each = g.numel() > 1 && g.stride(0) != 0;         // else one value for all rows
       if (each) g = g.contiguous();
@@ -341,6 +356,10 @@ bool tensor_or_none(PyObject* o, Tensor* t) {
   return true;
 }
 
+bool status_word(const Tensor& status, const Tensor& like) {
+  return !status.defined() || (plain(status, like, at::kInt) && status.numel() == 1);
+}
+
 // What torch records of its own operations and these calls do not show it: their answers would come without their derivative, or as constants
 // of the trace, and nobody would know.  (Wrappers of function transforms have no data to read, and raise where it is read.)
 void check_followed(std::initializer_list<const Tensor*> tensors) {
@@ -355,18 +374,18 @@ void check_followed(std::initializer_list<const Tensor*> tensors) {
   }
 }
 
-// x, weight, bias or None, gate or None, residual or None, activation -> the output, or None where dense.py has to look at the arguments first
+// x, weight, bias or None, gate or None, residual or None, activation, status or None -> the output, or None where dense.py has to look at the arguments first
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  Tensor x, w, bias, gate, residual;
-  if (nargs != 6 || !PyLong_Check(args[5])) {
-    PyErr_SetString(PyExc_TypeError, "linear: five tensors and an activation");
+  Tensor x, w, bias, gate, residual, status;
+  if (nargs != 7 || !PyLong_Check(args[5])) {
+    PyErr_SetString(PyExc_TypeError, "linear: five tensors, an activation and a status word");
     return nullptr;
   }
   const int64_t act = PyLong_AsLongLong(args[5]);
   if (act == -1 && PyErr_Occurred()) return nullptr;
   if (!tensor_or_none(args[0], &x) || !tensor_or_none(args[1], &w) || !tensor_or_none(args[2], &bias) || !tensor_or_none(args[3], &gate) ||
-      !tensor_or_none(args[4], &residual) || !x.defined() || !w.defined())
+      !tensor_or_none(args[4], &residual) || !tensor_or_none(args[6], &status) || !x.defined() || !w.defined())
     Py_RETURN_NONE;
   check_followed({&x, &w, &bias, &gate, &residual});
   if (!plain(x, x, at::kBFloat16) || !plain(w, x, at::kBFloat16) || w.dim() != 2 || x.dim() < 1) Py_RETURN_NONE;
@@ -379,27 +398,28 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!plain(*t, x, at::kBFloat16) || t->dim() != x.dim() || t->size(-1) != rw.rows || !Rows(*t).ok) Py_RETURN_NONE;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) if (t->size(i) != x.size(i)) Py_RETURN_NONE;
   }
+  if (!status_word(status, x)) Py_RETURN_NONE;
   Tensor y;
   {
     NoGil free_;
     const auto records = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     if (c10::GradMode::is_enabled() && (records(x) || records(w) || records(bias) || records(gate) || records(residual))) {
       const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-      y = LinearFunction::apply(x, w, given(bias), given(gate), given(residual), act);
+      y = LinearFunction::apply(x, w, given(bias), given(gate), given(residual), act, &status);
     } else {
-      y = linear_forward(x, w, bias, gate, residual, act, false, false).y;
+      y = linear_forward(x, w, bias, gate, residual, act, false, false, status).y;
     }
   }
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
-// hidden, weight, target (int64), ignore_index, scale, form, entropy -> (output, entropies or None), or None as above
+// hidden, weight, target (int64), ignore_index, scale, form, entropy, status or None -> (output, entropies or None), or None as above
 PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  Tensor h, w, target;
-  if (nargs != 7) {
-    PyErr_SetString(PyExc_TypeError, "head: hidden, weight, target, ignore_index, scale, form, entropy");
+  Tensor h, w, target, status;
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "head: hidden, weight, target, ignore_index, scale, form, entropy, status");
     return nullptr;
   }
   const int64_t ignore = PyLong_AsLongLong(args[3]);
@@ -410,7 +430,7 @@ PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (form == -1 && PyErr_Occurred()) return nullptr;
   const int entropy = PyObject_IsTrue(args[6]);
   if (entropy < 0) return nullptr;
-  if (!tensor_or_none(args[0], &h) || !tensor_or_none(args[1], &w) || !tensor_or_none(args[2], &target) || !h.defined() || !w.defined() || !target.defined())
+  if (!tensor_or_none(args[0], &h) || !tensor_or_none(args[1], &w) || !tensor_or_none(args[2], &target) || !tensor_or_none(args[7], &status) || !h.defined() || !w.defined() || !target.defined())
     Py_RETURN_NONE;
   check_followed({&h, &w, &target});
   if (!plain(h, h, at::kBFloat16) || !plain(w, h, at::kBFloat16) || !plain(target, h, at::kLong) || w.dim() != 2 || h.dim() < 1) Py_RETURN_NONE;
@@ -418,15 +438,16 @@ PyObject* head(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!operand(h, rh) || !operand(w, rw) || rh.cols != rw.cols || rw.rows == 0 || rw.cols == 0 || rw.cols % 8 != 0 || rh.rows == 0) Py_RETURN_NONE;
   if (!target.is_contiguous() || target.dim() != h.dim() - 1) Py_RETURN_NONE;
   for (int64_t i = 0; i < target.dim(); ++i) if (target.size(i) != h.size(i)) Py_RETURN_NONE;
+  if (!status_word(status, h)) Py_RETURN_NONE;
   Tensor out, ent;
   {
     NoGil free_;
     if (c10::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) {
-      const variable_list r = HeadFunction::apply(h, w, target, ignore, scale, form, entropy != 0);
+      const variable_list r = HeadFunction::apply(h, w, target, ignore, scale, form, entropy != 0, &status);
       out = r[0];
       if (entropy) ent = r[1];
     } else {
-      const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy != 0, false);
+      const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy != 0, false, status);
       out = r.out;
       ent = r.entropy;
     }

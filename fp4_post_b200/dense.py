@@ -10,6 +10,9 @@ nothing here computes on the CPU.  Operands are bfloat16, sums and softmax stati
 have any pitch that 16 bytes divide (others are copied first).  A call runs on the current stream of its tensors' device and can be
 captured in a CUDA graph.  The calls and their gradients are native (csrc/dense_host.cpp); what is here is what they refuse, and the
 copies of tensors that the kernels cannot read as they lie.
+Every wait of the kernels is bounded; one that runs out (0.4 s: a GPU that another process holds) ends the kernel and leaves its outputs as they are.
+status, an int32 tensor of one element on the same device that holds 0, receives a positive METIS_DEV_* code then, from the call or from its
+backward pass: read it where a step's results are read.
 They are no operations of torch: forward-mode derivatives, function transforms, traces and tensor subclasses that dispatch are refused.
 The reference leaves all of this to torch (nn.Linear, F.cross_entropy and TRL's selective log-softmax around src/grpo/grpo.py:199-215).
 """
@@ -46,6 +49,13 @@ def _check_product(x, weight, what: str) -> None:
         raise ValueError(f"weight {tuple(weight.shape)}: the inner size must be a positive multiple of 8")
 
 
+def _check_status(status, device: torch.device) -> None:
+    if status is not None:
+        _check(status, "status", device, (torch.int32,))
+        if status.numel() != 1:
+            raise ValueError(f"status must have one element, not {status.numel()}")
+
+
 def _readable(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """t with contiguous elements on an address that 16 bytes divide."""
     if t is None:
@@ -55,7 +65,7 @@ def _readable(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
-           gate: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+           gate: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x @ weight.T + bias) * gate + residual, rounded to bf16 once.
 
     x [..., K], weight [N, K] (the layout of nn.Linear), bias [N] in bf16 or fp32; gate and residual are shaped like the output
@@ -68,7 +78,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     except (KeyError, TypeError):
         raise ValueError(f"activation must be None, 'silu', 'gelu' or 'gelu_tanh', not {activation!r}") from None
     host = cabi.dense_host()
-    out = host.linear(x, weight, bias, gate, residual, code)
+    out = host.linear(x, weight, bias, gate, residual, code, status)
     if out is not None:
         return out
     _check_product(x, weight, "x")
@@ -82,37 +92,39 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
             _check(t, name, x.device)
             if tuple(t.shape) != shape:
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, not that of the output, {shape}")
-    out = host.linear(*(_readable(t) for t in (x, weight, bias, gate, residual)), code)
+    _check_status(status, x.device)
+    out = host.linear(*(_readable(t) for t in (x, weight, bias, gate, residual)), code, status)
     if out is None:
         raise RuntimeError("linear cannot read these tensors")
     return out
 
 
-def _head(hidden, weight, target, ignore_index, temperature, form, entropy):
+def _head(hidden, weight, target, ignore_index, temperature, form, entropy, status):
     scale = 1.0 / temperature if temperature else 0.0
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"temperature must be positive and finite, not {temperature}")
     host = cabi.dense_host()
-    out = host.head(hidden, weight, target, ignore_index, scale, form, entropy)
+    out = host.head(hidden, weight, target, ignore_index, scale, form, entropy, status)
     if out is not None:
         return out
     _check_product(hidden, weight, "hidden")
     _check(target, "target", hidden.device, (torch.int64, torch.int32))
     if target.shape != hidden.shape[:-1]:
         raise ValueError(f"targets have shape {tuple(target.shape)}, hidden states {tuple(hidden.shape)}")
+    _check_status(status, hidden.device)
     if target.numel() == 0:
         # nothing to do, but the graph stays connected: the gradients are zeros
         rows = hidden.sum(dim=-1, dtype=torch.float32) + (weight[:1].float() * 0.0).sum()
         out = rows if form in (_FORMS["none"], _LOGPROBS) else rows.sum() / (0.0 if form == _FORMS["mean"] else 1.0)
         return out, rows.detach()
-    out = host.head(_readable(hidden), _readable(weight), target.to(torch.int64).contiguous(), ignore_index, scale, form, entropy)
+    out = host.head(_readable(hidden), _readable(weight), target.to(torch.int64).contiguous(), ignore_index, scale, form, entropy, status)
     if out is None:
         raise RuntimeError("the head's losses cannot read these tensors")
     return out
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
-                         reduction: str = "mean", temperature: float = 1.0) -> torch.Tensor:
+                         reduction: str = "mean", temperature: float = 1.0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """F.cross_entropy(hidden @ weight.T / temperature, target, ignore_index=..., reduction=...) in fp32 without the logits.
 
     hidden [..., K] and weight [V, K] bf16, target [...] int64 or int32.  The logits are formed tile by tile in fp32 and folded
@@ -123,13 +135,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         form = _FORMS[reduction]
     except (KeyError, TypeError):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}") from None
-    return _head(hidden, weight, target, ignore_index, temperature, form, False)[0]
+    return _head(hidden, weight, target, ignore_index, temperature, form, False, status)[0]
 
 
 def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor, *, temperature: float = 1.0, entropy: bool = False,
-                   ignore_index: int = -100):
+                   ignore_index: int = -100, status: Optional[torch.Tensor] = None):
     """log softmax(hidden @ weight.T / temperature) at the given token ids, fp32, shaped like ids; 0 where ids is ignore_index.
 
     With entropy=True also the entropy of each row's distribution (0 likewise), which carries no gradient."""
-    out = _head(hidden, weight, ids, ignore_index, temperature, _LOGPROBS, entropy)
+    out = _head(hidden, weight, ids, ignore_index, temperature, _LOGPROBS, entropy, status)
     return out if entropy else out[0]

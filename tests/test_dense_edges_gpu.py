@@ -260,3 +260,79 @@ def test_a_weight_that_a_hook_makes_is_the_one_that_is_used(decoders):
         h = normal(2, 5, 256)
         a, b = plain.layers[0].mlp(h), fused.layers[0].mlp(h)
         assert a.any() and torch.equal(a, b)                # one product by 1: no rounding of the down projection's
+
+
+# ---- the status word -------------------------------------------------------------------------------------------------
+
+def calls_with(status, M):
+    """Every call with a status word, and its backward pass."""
+    x, w, y = normal(M, 64), normal(104, 64, scale=0.125, seed=1), normal(M, 104, seed=2)
+    t = torch.arange(M, device="cuda") % 104
+    for v in (x, w, y):
+        v.requires_grad_(True)
+    out = dense.linear(x, w, activation="silu", gate=y, status=status)
+    torch.autograd.grad(out, (x, w, y), normal(M, 104, seed=3))
+    torch.autograd.grad(dense.linear_cross_entropy(x, w, t, status=status), (x, w))
+    logp, _ = dense.token_logprobs(x, w, t, entropy=True, status=status)
+    torch.autograd.grad(logp.sum(), (x, w))
+    with torch.no_grad():
+        dense.linear(x, w, status=status)
+        dense.linear(x[:, ::2].repeat(1, 2), w.t().contiguous().t(), status=status)      # (copied before it is read)
+        dense.linear_cross_entropy(x, w, t.int(), status=status)
+
+
+@pytest.fixture()
+def entries():
+    """Entry points bound to functions that note the status they are given and go on to the library."""
+    import ctypes as C
+    from fp4_post_b200 import cabi
+    L, host, seen, keep = cabi.lib(), cabi.dense_host(), [], []
+
+    def put(name, types, status):
+        real = getattr(L, name)
+
+        def noted(*args):
+            seen.append((name, status(args)))
+            return real(*args)
+        keep.append(C.CFUNCTYPE(C.c_int32, *types)(noted))
+        assert host.bind(name, C.cast(keep[-1], C.c_void_p).value)
+    vp, i32, i64, of_args = C.c_void_p, C.c_int32, C.c_int64, lambda a: a[0].contents.status
+    put("metis_linear", [C.POINTER(cabi.LinearArgs)], of_args)
+    put("metis_bf16_product", [vp, i32, i64, vp, i64, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp], lambda a: a[13])
+    put("metis_head_loss_keep", [C.POINTER(cabi.HeadArgs), vp, vp, vp], of_args)
+    put("metis_head_backward_kept", [C.POINTER(cabi.HeadArgs), vp, vp, i32, vp, vp, i64, vp, i64], of_args)
+    yield seen
+    for name in ("metis_linear", "metis_bf16_product", "metis_head_loss_keep", "metis_head_backward_kept"):
+        host.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
+
+
+@pytest.mark.parametrize("M", [40, 300])
+def test_every_launch_that_waits_has_the_callers_status_word(entries, M):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    calls_with(status, M)
+    torch.cuda.synchronize()
+    assert {at for _, at in entries} == {status.data_ptr()} and {n for n, _ in entries} == {"metis_linear", "metis_bf16_product", "metis_head_loss_keep", "metis_head_backward_kept"}
+    assert status.item() == 0
+    entries.clear()
+    calls_with(None, M)
+    assert entries and {at for _, at in entries} == {None}
+
+
+def test_the_status_word_may_be_set_back_between_forward_and_backward():
+    status = torch.zeros((), dtype=torch.int32, device="cuda")
+    x, w = normal(40, 64).requires_grad_(True), normal(48, 64, seed=1)
+    out = dense.linear(x, w, activation="gelu", status=status)
+    status.zero_()
+    torch.autograd.grad(out, x, normal(40, 48, seed=2))
+    assert status.item() == 0
+
+
+def test_bad_status_words_are_refused():
+    x, w, t = normal(4, 64), normal(24, 64, seed=1), torch.zeros(4, dtype=torch.int64, device="cuda")
+    calls = [lambda s: dense.linear(x, w, status=s), lambda s: dense.linear_cross_entropy(x, w, t, status=s), lambda s: dense.token_logprobs(x, w, t, status=s),
+             lambda s: dense.token_logprobs(x[:0], w, t[:0], status=s)]
+    for call in calls:
+        for bad, error in ((torch.zeros(1, dtype=torch.int32), ValueError), (torch.zeros(2, dtype=torch.int32, device="cuda"), ValueError),
+                           (torch.zeros(0, dtype=torch.int32, device="cuda"), ValueError), (torch.zeros(1, dtype=torch.int64, device="cuda"), TypeError), (0, TypeError)):
+            with pytest.raises(error):
+                call(bad)
