@@ -1432,6 +1432,7 @@ static int32_t check_head(const metis_head_args* a) {
   if (int32_t rc = check_rows(a->w, a->ldw, a->K, "w")) return rc;
   if (a->negate != 0 && a->negate != 1) return fail(METIS_ERR_BAD_ARGUMENT, "negate must be 0 or 1");
   if (!a->target || !a->lse) return fail(METIS_ERR_BAD_ARGUMENT, "target or lse is null");
+  if (!(a->scale > 0.0f && a->scale <= 0x1p127f)) return fail(METIS_ERR_BAD_ARGUMENT, "scale = %g must be positive, and at most 2^127: 1.44 times it is finite", (double)a->scale);
   return METIS_OK;
 }
 constexpr int64_t kFewRows = 64;                           // rows of a head that the weight's read bounds

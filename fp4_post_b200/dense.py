@@ -101,8 +101,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 def _head(hidden, weight, target, ignore_index, temperature, form, entropy, status):
     scale = 1.0 / temperature if temperature else 0.0
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, not {temperature}")
+    if not 2.0 ** -149 <= scale <= 2.0 ** 127:             # (the kernels have it, and 1.44 times it, in 32 bits)
+        raise ValueError(f"temperature must be positive and finite, and so must 1 / temperature in 32 bits, not {temperature}")
     host = cabi.dense_host()
     out = host.head(hidden, weight, target, ignore_index, scale, form, entropy, status)
     if out is not None:

@@ -37,6 +37,18 @@ def test_the_head_with_kept_log_probabilities_refuses_what_it_does_without(L, p)
     assert L.metis_head_backward_kept(head_args(p), p, p, 0, None, None, 16, None, 16) == -1
 
 
+def test_temperatures_that_32_bits_cannot_divide_by_are_refused(L, p):
+    x, w, t = torch.zeros(4, 16).bfloat16(), torch.zeros(24, 16).bfloat16(), torch.zeros(4, dtype=torch.int64)
+    for temperature in (0.0, -1.0, float("inf"), float("nan"), 1e-39, 1e-300, 5e-324, 1e46, 1e300):
+        with pytest.raises(ValueError, match="temperature"):
+            dense.linear_cross_entropy(x, w, t, temperature=temperature)
+        with pytest.raises(ValueError, match="temperature"):
+            dense.token_logprobs(x, w, t, temperature=temperature)
+    for scale in (0.0, -1.0, float("inf"), float("nan"), 3e38):
+        assert L.metis_head_loss(head_args(p, scale=scale), p, None) == -1
+        assert L.metis_head_backward(head_args(p, scale=scale), p, 0, None, p, 16, p, 16) == -1
+
+
 def test_what_torch_would_not_see_is_refused(built_library):
     """Forward-mode derivatives and traces: the calls would return without a tangent, or as a constant of the trace."""
     from torch.autograd import forward_ad

@@ -87,6 +87,18 @@ def test_a_target_of_infinite_logit_or_alone_in_its_vocabulary(M):
     assert got[2] == -float("inf") and torch.isfinite(got[:2]).all() and torch.isfinite(got[3:]).all()
 
 
+@pytest.mark.parametrize("M", [6, 70])
+def test_the_hottest_and_the_coldest_temperatures(M):
+    h, w, t = normal(M, 64), normal(90, 64, seed=1), torch.arange(M, device="cuda")
+    for temperature in (1e30, 1e38, 1e44):                  # all tokens alike
+        got, entropy = dense.token_logprobs(h, w, t, temperature=temperature, entropy=True)
+        assert (got + math.log(90)).abs().max() <= 1e-5 and (entropy - math.log(90)).abs().max() <= 1e-5
+    best = (h.double() @ w.double().t()).argmax(dim=1)
+    for temperature in (1e-4, 1e-20):                       # one takes it all (none is within 16 times 1e-4 of it, but for one row in a thousand)
+        got = dense.token_logprobs(h, w, best, temperature=temperature)
+        assert float((got > -1e-6).float().mean()) >= 0.98
+
+
 def exact_logit_gradient(h, w, t, temperature):
     """softmax - one-hot over the temperature, the target's element without cancellation, in 64 bits."""
     logp, miss, logits = exact_head(h, w, t, temperature)
