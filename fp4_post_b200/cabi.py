@@ -265,6 +265,11 @@ def dense_host():
     return _dense
 
 
+def dense_launches() -> int:
+    """Kernels that the bf16 products have launched: none before the library is loaded, which a count does not do."""
+    return 0 if _lib is None else _lib.metis_dense_launches()
+
+
 def check(rc: int, what: str) -> None:
     """Turn a non-zero status into a Python exception, with the library's own message.
 

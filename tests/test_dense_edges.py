@@ -81,6 +81,13 @@ def test_what_torch_would_not_see_is_refused(built_library):
         dense.linear(x, w)
 
 
+def test_launches_are_counted_without_the_library(monkeypatch, tmp_path):
+    from fp4_post_b200 import ops
+    monkeypatch.setattr(cabi, "_lib", None)
+    monkeypatch.setattr(cabi, "LIB_PATH", tmp_path / "none.so")
+    assert ops.launch_count() == sum(ops.LAUNCHES.values())
+
+
 # ---- the decoder ---------------------------------------------------------------------------------------------------
 
 def tiny(**options):
