@@ -54,12 +54,20 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _cxx_runtime(cxx: str) -> list[str]:
+    """Links the shared C++ runtime, the one that torch has loaded.  A compiler installed beside the system's may find the static one alone, and a
+    module with streams of its own ends the process where it puts a number into a message."""
+    found = subprocess.run([cxx, "-print-file-name=libstdc++.so.6"], stdout=subprocess.PIPE, text=True).stdout.strip()
+    return [found] if Path(found).is_absolute() and Path(found).exists() else []
+
+
 def _host_command(source: Path = HOST_SOURCE, target: Path = HOST_PATH, libraries: tuple = ()) -> list[str]:
     import torch
     root = Path(torch.__file__).resolve().parent
     include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], Path(_nvcc()).resolve().parent.parent / "include"]
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *(f"-I{p}" for p in include), str(source), "-o", str(target), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", *libraries]
+    cxx = os.environ.get("CXX", "g++")
+    return [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{p}" for p in include), str(source), "-o", str(target), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", *libraries, *_cxx_runtime(cxx)]
 
 
 def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False) -> Path:
@@ -84,7 +92,7 @@ def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     hosts = []
     for source, target, libraries in ((HOST_SOURCE, HOST_PATH, ()), (DENSE_SOURCE, DENSE_PATH, ("-lc10_cuda",))):
-        if not timing_knobs and (force or _stale(target, [source, PKG.parent / "include" / "metis_nvfp4.h"])):
+        if not timing_knobs and (force or _stale(target, [source, PKG.parent / "include" / "metis_nvfp4.h", Path(__file__)])):
             hosts.append((source, subprocess.Popen(_host_command(source, target, libraries), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = []
     for src, p in procs:

@@ -88,6 +88,19 @@ def test_launches_are_counted_without_the_library(monkeypatch, tmp_path):
     assert ops.launch_count() == sum(ops.LAUNCHES.values())
 
 
+def test_the_native_modules_put_numbers_into_messages(tmp_path):
+    """Beside torch: with a C++ runtime of its own such a module ends the process (hence one of its own here)."""
+    import subprocess
+    import sys
+    from fp4_post_b200 import build
+    source, target = tmp_path / "numbers.cpp", tmp_path / "numbers.so"
+    source.write_text('#include <sstream>\n#include <string>\n'
+                      'extern "C" const char* say(long n) { static std::string s; std::ostringstream o; o << "status " << n << " " << 1.5; s = o.str(); return s.c_str(); }\n')
+    subprocess.run(build._host_command(source, target), check=True)
+    code = f"import torch, ctypes; f = ctypes.CDLL({str(target)!r}).say; f.restype = ctypes.c_char_p; f.argtypes = [ctypes.c_long]; print(f(-7).decode())"
+    assert subprocess.run([sys.executable, "-c", code], check=True, stdout=subprocess.PIPE, text=True).stdout.strip() == "status -7 1.5"
+
+
 # ---- the decoder ---------------------------------------------------------------------------------------------------
 
 def tiny(**options):

@@ -274,6 +274,29 @@ def test_a_weight_that_a_hook_makes_is_the_one_that_is_used(decoders):
         assert a.any() and torch.equal(a, b)                # one product by 1: no rounding of the down projection's
 
 
+# ---- errors of the library ---------------------------------------------------------------------------------------------
+
+def test_errors_of_the_library_are_raised_with_their_number():
+    """In the call and, on a thread of autograd's, in its backward pass."""
+    import ctypes as C
+    from fp4_post_b200 import cabi
+    L, host = cabi.lib(), cabi.dense_host()
+    x, w, t = normal(40, 64).requires_grad_(True), normal(48, 64, seed=1).requires_grad_(True), torch.arange(40, device="cuda")
+    calls = {"metis_linear": lambda: dense.linear(x, w), "metis_head_loss_keep": lambda: dense.linear_cross_entropy(x, w, t),
+             "metis_linear_pointwise": lambda: torch.autograd.grad(dense.linear(x, w, activation="silu"), x, normal(40, 48)),
+             "metis_bf16_product": lambda: torch.autograd.grad(dense.linear(x, w), x, normal(40, 48)),
+             "metis_head_backward_kept": lambda: torch.autograd.grad(dense.linear_cross_entropy(x, w, t), x)}
+    for name, call in calls.items():
+        refuse = C.CFUNCTYPE(C.c_int32)(lambda: -7)
+        assert host.bind(name, C.cast(refuse, C.c_void_p).value)
+        try:
+            with pytest.raises(RuntimeError, match=f"{name}: status -7"):
+                call()
+        finally:
+            host.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
+        call()
+
+
 # ---- the status word -------------------------------------------------------------------------------------------------
 
 def calls_with(status, M):
