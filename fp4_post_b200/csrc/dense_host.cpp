@@ -64,6 +64,7 @@ bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr
 struct Rows {
   int64_t rows = 0, cols = 0, ld = 0;
   bool ok = false;
+  Rows() = default;
   explicit Rows(const Tensor& t) {
     if (t.dim() < 1) return;
     cols = t.size(-1);
@@ -86,16 +87,21 @@ bool operand(const Tensor& t, Rows& r) {
 bool plain(const Tensor& t, const Tensor& like, at::ScalarType type) {
   return t.is_cuda() && t.scalar_type() == type && t.device() == like.device() && t.layout() == at::kStrided && !t.is_neg() && !t.is_conj();
 }
-// t as a matrix of 16-byte aligned rows, copied if it has to be
-Tensor as_operand(const Tensor& t, int64_t cols, Rows& r) {
-  Tensor m = t.reshape({-1, cols});
-  r = Rows(m);
-  if (!operand(m, r)) {
-    m = m.clone(at::MemoryFormat::Contiguous);
-    r = Rows(m);
-    TORCH_CHECK(operand(m, r), "rows of ", cols, " elements cannot be read");
-  }
-  return m;
+// t as rows that the TMA unit reads, copied if it has to be
+Tensor as_operand(const Tensor& t, Rows& r) {
+  r = Rows(t);
+  if (operand(t, r)) return t;
+  const Tensor c = t.clone(at::MemoryFormat::Contiguous);
+  r = Rows(c);
+  TORCH_CHECK(operand(c, r), "rows of ", r.cols, " elements cannot be read");
+  return c;
+}
+
+// A tensor that was saved is what it was, but a hook of saved tensors may have laid it out otherwise, and has to be asked whether it gave back
+// the same at all: the kernels read what they are pointed at.
+const Tensor& given_back(const Tensor& t, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes) {
+  TORCH_CHECK(plain(t, like, type) && t.sizes() == sizes, "a saved tensor came back as ", t.toString(), " of shape ", t.sizes(), " on ", t.device());
+  return t;
 }
 
 // Gradients are formed by kernels that record nothing: one that is asked for with a graph of its own raises when it is differentiated.
@@ -181,7 +187,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(7);
     if (!grads[0].defined()) return out;
-    const variable_list saved = ctx->get_saved_variables();
+    variable_list saved = ctx->get_saved_variables();
     const std::vector<int64_t> o = ctx->saved_data["s"].toIntVector(), x_shape = ctx->saved_data["x"].toIntVector();
     const int64_t act = o[0], N = o[5], K = o[6];
     // (the edges are those of the tensors that were given)
@@ -212,6 +218,16 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           dy = dy.contiguous();
           rdy = Rows(dy);
         }
+        const int64_t kept_pitch = (N + 7) / 8 * 8;
+        Rows rx, rw, rgate, ract, rslope;
+        if (saved[0].defined()) saved[0] = as_operand(given_back(saved[0], dy, at::kBFloat16, x_shape), rx);
+        if (saved[1].defined()) saved[1] = as_operand(given_back(saved[1], dy, at::kBFloat16, {N, K}), rw);
+        if (saved[2].defined()) {
+          rgate = Rows(given_back(saved[2], dy, at::kBFloat16, dy_shaped.sizes()));
+          if (!rgate.ok) rgate = Rows(saved[2] = saved[2].contiguous());
+        }
+        if (saved[3].defined()) saved[3] = as_operand(given_back(saved[3], dy, at::kBFloat16, {M, kept_pitch}), ract);
+        if (saved[4].defined()) saved[4] = as_operand(given_back(saved[4], dy, at::kHalf, {M, kept_pitch}), rslope);
         // dz is dy itself where nothing changes it and its rows can be read as they lie
         const bool product_wanted = need_x || need_w, epilogue = act != METIS_ACT_NONE || saved[2].defined();
         Rows rdz = rdy;
@@ -223,9 +239,9 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           metis_linear_pointwise_args a = {};
           a.M = M; a.N = N;
           a.dy = dy.data_ptr(); a.lddy = rdy.ld;
-          if (saved[3].defined()) { a.act = saved[3].data_ptr(); a.ldact = saved[3].size(1); }
-          if (saved[4].defined()) { a.slope = saved[4].data_ptr(); a.ldslope = saved[4].size(1); }
-          if (saved[2].defined()) { a.gate = saved[2].data_ptr(); a.ldgate = Rows(saved[2]).ld; }
+          if (saved[3].defined()) { a.act = saved[3].data_ptr(); a.ldact = ract.ld; }
+          if (saved[4].defined()) { a.slope = saved[4].data_ptr(); a.ldslope = rslope.ld; }
+          if (saved[2].defined()) { a.gate = saved[2].data_ptr(); a.ldgate = rgate.ld; }
           if (write_dz) {
             const int64_t pitch = (N + 7) / 8 * 8;
             dz = empty_like_options(dy, {half ? 2 * half : M, pitch}, at::kBFloat16);
@@ -247,16 +263,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
           a.stream = stream_of(dy);
           check(lib.metis_linear_pointwise(&a), "metis_linear_pointwise");
         }
-        if (need_x) {
-          Rows rw(saved[1]);
-          operand(saved[1], rw);
-          out[0] = product(dz, rdz, false, half, saved[1], rw, status).view(x_shape);
-        }
-        if (need_w) {
-          Rows rx(saved[0]);
-          operand(saved[0], rx);
-          out[1] = product(dz, rdz, true, half, saved[0], rx, status);
-        }
+        if (need_x) out[0] = product(dz, rdz, false, half, saved[1], rw, status).view(x_shape);
+        if (need_w) out[1] = product(dz, rdz, true, half, saved[0], rx, status);
       }
     }
     return once(std::move(out));
@@ -314,7 +322,8 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
     const HeadResult r = head_forward(h, w, target, ignore, scale, form, entropy, true, *status);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({h, w, target, r.lse, r.logp, r.inv_count});
-    ctx->saved_data["o"] = std::vector<int64_t>{ignore, form};
+    ctx->saved_data["o"] = std::vector<int64_t>{ignore, form, w.size(0), w.size(1)};
+    ctx->saved_data["h"] = h.sizes().vec();
     ctx->saved_data["s"] = scale;
     keep_status(ctx, *status);
     if (!entropy) return {r.out};
@@ -331,9 +340,15 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
     if (!need_h && !need_w) return out;
     {
       at::AutoGradMode off(false);
-      const Tensor &h = saved[0], &w = saved[1];
-      c10::OptionalDeviceGuard guard(h.device());
-      metis_head_args a = head_args(h, w, saved[2], saved[3], o[0], ctx->saved_data["s"].toDouble(), o[1], kept_status(ctx));
+      const std::vector<int64_t> h_shape = ctx->saved_data["h"].toIntVector();
+      const Tensor& dout = grads[0];                        // (on the device of the forward pass: the engine sees to it)
+      c10::OptionalDeviceGuard guard(dout.device());
+      Rows rh, rw;
+      const Tensor h = as_operand(given_back(saved[0], dout, at::kBFloat16, h_shape), rh), w = as_operand(given_back(saved[1], dout, at::kBFloat16, {o[2], o[3]}), rw);
+      const Tensor target = given_back(saved[2], dout, at::kLong, at::IntArrayRef(h_shape).slice(0, h_shape.size() - 1)).contiguous();
+      const Tensor lse = given_back(saved[3], dout, at::kFloat, {target.numel()}).contiguous(), logp = given_back(saved[4], dout, at::kFloat, {target.numel()}).contiguous();
+      const Tensor inv_count = saved[5].defined() ? given_back(saved[5], dout, at::kFloat, {1}) : Tensor();
+      metis_head_args a = head_args(h, w, target, lse, o[0], ctx->saved_data["s"].toDouble(), o[1], kept_status(ctx));
       Tensor g = grads[0].reshape({-1});
       const bool each = g.numel() > 1 && g.stride(0) != 0;         // else one value for all rows
       if (each) g = g.contiguous();
@@ -341,7 +356,7 @@ struct HeadFunction : torch::autograd::Function<HeadFunction> {
       if (need_w) out[1] = empty_like_options(h, w.sizes(), at::kBFloat16);
       const Tensor ws = scratch(h, lib.metis_head_backward_workspace_bytes(a.M, a.V, a.K));
       a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel();
-      check(lib.metis_head_backward_kept(&a, ptr<float>(saved[4]), ptr<float>(g), each, ptr<float>(saved[5]), ptr(out[0]), a.K, ptr(out[1]), a.K), "metis_head_backward_kept");
+      check(lib.metis_head_backward_kept(&a, ptr<float>(logp), ptr<float>(g), each, ptr<float>(inv_count), ptr(out[0]), a.K, ptr(out[1]), a.K), "metis_head_backward_kept");
     }
     return once(std::move(out));
   }

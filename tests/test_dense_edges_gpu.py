@@ -371,3 +371,62 @@ def test_bad_status_words_are_refused():
                            (torch.zeros(0, dtype=torch.int32, device="cuda"), ValueError), (torch.zeros(1, dtype=torch.int64, device="cuda"), TypeError), (0, TypeError)):
             with pytest.raises(error):
                 call(bad)
+
+
+# ---- saved tensors ---------------------------------------------------------------------------------------------------
+
+def otherwise(t):
+    """The same values the other way round in memory."""
+    if t.dim() == 0:
+        return t.clone()
+    if t.dim() == 1:
+        return torch.stack((t, t), dim=1)[:, 0]
+    return t.transpose(0, -1).contiguous().transpose(0, -1)
+
+
+def misaligned(t):
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+    return flat.copy_(t.reshape(-1)).view(t.shape)
+
+
+@pytest.mark.parametrize("M,N", [(40, 96), (40, 97), (300, 97), (1, 96)])
+def test_saved_tensors_that_come_back_laid_out_otherwise(M, N):
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    K = 64
+    x, w, b, g, r = normal(M, K), normal(N, K, scale=0.125, seed=1), normal(N, seed=2), normal(M, N, seed=3), normal(M, N, seed=4)
+    t, dy, dl = torch.arange(M, device="cuda") % N, normal(M, N, seed=5), normal(M, seed=6, dtype=torch.float32)
+    t[M // 2] = -100
+    leaves = [v.requires_grad_(True) for v in (x, w, b, g, r)]
+
+    def step():
+        y = dense.linear(x, w, b, activation="gelu", gate=g, residual=r)
+        z = dense.linear(x, w)
+        return (*torch.autograd.grad(y, leaves, dy), *torch.autograd.grad(z, (x, w), dy), *torch.autograd.grad(dense.linear_cross_entropy(x, w, t), (x, w)),
+                *torch.autograd.grad(dense.token_logprobs(x, w, t), (x, w), dl))
+    want = step()
+    for hooks in (saved_tensors_hooks(lambda v: v, otherwise), saved_tensors_hooks(lambda v: v, misaligned), saved_tensors_hooks(otherwise, lambda v: v), save_on_cpu(pin_memory=True)):
+        with hooks:
+            got = step()
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+    for spoil in (lambda v: v.cpu(), lambda v: v.float() if v.dtype != torch.float32 else v.double(), lambda v: v[:0]):
+        with saved_tensors_hooks(lambda v: v, spoil), pytest.raises(RuntimeError, match="saved tensor"):
+            torch.autograd.grad(dense.linear(x, w, activation="silu", gate=g), (x, w, g), dy)
+        with saved_tensors_hooks(lambda v: v, spoil), pytest.raises(RuntimeError, match="saved tensor"):
+            torch.autograd.grad(dense.token_logprobs(x, w, t), (x, w), dl)
+
+
+def test_under_activation_checkpoints():
+    from torch.utils.checkpoint import checkpoint
+    x, w, u, head = normal(50, 64), normal(96, 64, scale=0.125, seed=1), normal(64, 96, scale=0.1, seed=2), normal(101, 64, scale=0.125, seed=3)
+    t = torch.arange(50, device="cuda")
+    leaves = [v.requires_grad_(True) for v in (x, w, u, head)]
+
+    def run(x, w, u, head):
+        h = dense.linear(dense.linear(x, w, activation="silu", gate=dense.linear(x, w)), u, residual=x)
+        return dense.linear_cross_entropy(h, head, t)
+    want = torch.autograd.grad(run(*leaves), leaves)
+    for reentrant in (False, True):
+        for v in leaves:
+            v.grad = None
+        checkpoint(run, *leaves, use_reentrant=reentrant).backward()
+        assert all(torch.equal(v.grad, c) for v, c in zip(leaves, want))
