@@ -106,7 +106,7 @@ __device__ __forceinline__ float logistic(float u) { return rcp_approx(1.0f + ex
 
 // The normal distribution's function.  For a = |z| it is exp(-a^2 / 2) g(a) on the left, where g(a) = exp(a^2 / 2) erfc(a / sqrt 2) / 2
 // falls like 1 / a: a polynomial in t = 1 / (1 + 0.3 a) without a constant term, fitted for least relative error over a in [0, 13.5] (where
-// the value leaves fp32): 1.3e-7 by itself, 7e-7 in fp32 up to a = 3 and 8e-6 at the end, where a^2 is rounded.  16 instructions against the
+// the value leaves fp32): 1.6e-7 by itself, 7e-7 in fp32 up to a = 3 and 8e-6 at the end, where a^2 is rounded.  16 instructions against the
 // 40 of normcdff, which kept the tensor core waiting: 8192 x 8960 x 1536 with gelu 505 us.
 __device__ __forceinline__ float normal_cdf(float z) {
   const float a = fabsf(z), t = rcp_approx(fmaf(0.3f, a, 1.0f));
@@ -151,7 +151,7 @@ template <int kAct> __device__ __forceinline__ void activate_both(float z, float
   }
 }
 // What a backward pass needs of z.  act' lies in [-0.13, 1.13], so 16 bits with ten of mantissa hold it: in fp16, times 2^15 (the values lie
-// below 37100, and down to 2^-29 none loses bits).  An error of 2^-12 at most; from z in bf16 the slope has one of |z act''| 2^-9, and the
+// below 37100, and down to 2^-29 none loses bits).  An error of 2^-11 of the slope at most, an eighth of bf16's; from z in bf16 the slope has one of |z act''| 2^-9, and the
 // gradients of x and W, which round dz to bf16, are then 1.7 times as far from the exact ones as their own last rounding puts them; 1.4 so.
 constexpr float kSlopeScale = 32768.0f;
 __device__ __forceinline__ uint32_t half_slopes(float lo, float hi) {

@@ -14,8 +14,9 @@ follows already quantized (RMSNorm.forward_quantized): one pass over the hidden 
 normalised tensor and its column mean, the next quantizes it for all projections of the group.
 
 With `fuse_dense=True` what stays in bf16 runs on dense.py: the loss and `token_logprobs` take the head without its logits in
-memory, and a projection that is no Metis layer (target_modules of replace_linear_with_metis leaves it out) has its activation, the
-product with `up` and the residual in its own kernel.
+memory, and where o, gate and down are no Metis layers (target_modules of replace_linear_with_metis leaves them out) they have the
+activation, the product with `up` and the residual in their own kernels.  q/k/v and up, which nothing follows, stay torch's.
+A layer that has hooks is called like any module, and whatever has to see torch's operations gets them.
 """
 from __future__ import annotations
 

@@ -8,12 +8,14 @@
 All three run on tcgen05 kernels of this library (csrc/dense_gemm.cu, csrc/dense_small.cu for few tokens) and need CUDA tensors;
 nothing here computes on the CPU.  Operands are bfloat16, sums and softmax statistics fp32.  The inner size is a multiple of 8; rows may
 have any pitch that 16 bytes divide (others are copied first).  A call runs on the current stream of its tensors' device and can be
-captured in a CUDA graph.  The calls and their gradients are native (csrc/dense_host.cpp); what is here is what they refuse, and the
-copies of tensors that the kernels cannot read as they lie.
-Every wait of the kernels is bounded; one that runs out (0.4 s: a GPU that another process holds) ends the kernel and leaves its outputs as they are.
-status, an int32 tensor of one element on the same device that holds 0, receives a positive METIS_DEV_* code then, from the call or from its
-backward pass: read it where a step's results are read.
-They are no operations of torch: forward-mode derivatives, function transforms, traces and tensor subclasses that dispatch are refused.
+captured in a CUDA graph (a backward pass too, while no eager graph of the same leaves is kept: see graphs.py).  The calls and their
+gradients are native (csrc/dense_host.cpp); what is here is what they refuse, and the copies of tensors that the kernels cannot read as
+they lie.  They are no operations of torch: forward-mode derivatives, function transforms, traces and tensor subclasses that dispatch by
+themselves are refused.
+
+Every wait of the kernels is bounded; one that runs out (0.4 s: a GPU that another process holds) ends the kernel and leaves its outputs
+as they are.  status, an int32 tensor of one element on the same device that holds 0, receives a positive METIS_DEV_* code then, from the
+call or from its backward pass: read it where a step's results are read.
 The reference leaves all of this to torch (nn.Linear, F.cross_entropy and TRL's selective log-softmax around src/grpo/grpo.py:199-215).
 """
 from __future__ import annotations
@@ -71,8 +73,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x [..., K], weight [N, K] (the layout of nn.Linear), bias [N] in bf16 or fp32; gate and residual are shaped like the output
     [..., N] (no broadcasting).  activation: None, "silu", "gelu" (erf form) or "gelu_tanh".  A SwiGLU block is
     linear(linear(h, w_gate, activation="silu", gate=linear(h, w_up)), w_down, residual=x).
-    Differentiable once in all tensors; the backward pass keeps the activation's slopes in 16 bits, and
-    act(..) in bf16 where the gate has a gradient."""
+    Differentiable once in all tensors.  Besides their own rounding the gradients have those of what they are made of: the activation's slopes
+    in fp16 (2^-11), act(..) in bf16 for the gate's, and above 128 rows dz, the output's gradient taken through the epilogue, in bf16 (up to
+    128 rows in two bf16 numbers): 2.4e-3 of a gradient's norm in place of 1.7e-3."""
     try:
         code = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
@@ -129,7 +132,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
     hidden [..., K] and weight [V, K] bf16, target [...] int64 or int32.  The logits are formed tile by tile in fp32 and folded
     into each row's maximum and sum; the backward pass forms them again, piece by piece of the vocabulary, and differentiates
-    hidden and weight (once).  A row whose target is ignore_index adds nothing, whatever it holds.  A target that is neither
+    hidden and weight (once).  The gradients are rounded to bf16; so is, above 128 rows, the logits' gradient that they are made of (up to 128 in
+    two bf16 numbers): 1.9e-3 to 2.4e-3 of their norm in place of 1.7e-3.  A row whose target is ignore_index adds nothing, whatever it holds.  A target that is neither
     ignore_index nor in the vocabulary makes its loss NaN.  The mean over no row at all is NaN, as torch has it."""
     try:
         form = _FORMS[reduction]
@@ -142,6 +146,7 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor
                    ignore_index: int = -100, status: Optional[torch.Tensor] = None):
     """log softmax(hidden @ weight.T / temperature) at the given token ids, fp32, shaped like ids; 0 where ids is ignore_index.
 
+    Never positive, and as exact for a token that the model is sure of (1 - p of 1e-6) as for any.  Gradients as those of linear_cross_entropy.
     With entropy=True also the entropy of each row's distribution (0 likewise), which carries no gradient."""
     out = _head(hidden, weight, ids, ignore_index, temperature, _LOGPROBS, entropy, status)
     return out if entropy else out[0]

@@ -523,7 +523,7 @@ int32_t metis_bf16_product(const void* a, int32_t a_mn_major, int64_t lda, const
  * l = scale * h W^T [M, V] with h [M, K] and W [V, K] in bf16, scale positive, up to 2^127; l is formed tile by tile in fp32 and not stored.
  * metis_head_loss: lse[m] = log sum_j exp l[m][j]; nll[m] = lse[m] - l[m][target[m]], 0 where target[m] = ignore_index, NaN
  * where it is no other index of the vocabulary; entropy (optional) = lse - sum_j p l, 0 where target[m] = ignore_index.  h and w as x and w of metis_linear.
- * lse of ignored rows is not set.
+ * lse of ignored rows is not set, and what they hold in h adds nothing to any result.
  */
 typedef struct metis_head_args {
   int64_t M, V, K;
