@@ -274,6 +274,20 @@ def test_a_weight_that_a_hook_makes_is_the_one_that_is_used(decoders):
         assert a.any() and torch.equal(a, b)                # one product by 1: no rounding of the down projection's
 
 
+def test_function_transforms_are_refused():
+    x, w, b, t = normal(3, 40, 64), normal(48, 64, seed=1), normal(3, 48, seed=2), torch.arange(40, device="cuda")
+    calls = [(lambda v: dense.linear(v, w), x), (lambda v: dense.linear(x[0], w, v), b), (lambda v: dense.linear(x[0], w, residual=v), normal(3, 40, 48)),
+             (lambda v: dense.linear(x[0], v), normal(3, 48, 64)), (lambda v: dense.token_logprobs(v, w, t), x), (lambda v: dense.token_logprobs(x[0], w, v), t.expand(3, 40).contiguous())]
+    for call, batch in calls:
+        with pytest.raises(RuntimeError):
+            torch.vmap(call)(batch)
+        if batch.is_floating_point():
+            with pytest.raises(RuntimeError):
+                torch.func.grad(lambda v: call(v).float().sum())(batch[0])
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(call, (batch[0],), (batch[0],))
+
+
 # ---- errors of the library ---------------------------------------------------------------------------------------------
 
 def test_errors_of_the_library_are_raised_with_their_number():
