@@ -2,8 +2,8 @@
 
     python -m fp4_post_b200.build        # or: from fp4_post_b200.build import build; build()
 
-Output: fp4_post_b200/_lib/libmetis_nvfp4.so, and cabi.HOST_PATH and cabi.DENSE_PATH, the native parts of the tensor-level wrappers
-and of dense.py (g++ against the installed torch and Python, whose versions are in their names).  nvcc cross-compiles without a GPU.
+Output: fp4_post_b200/_lib/libmetis_nvfp4.so, and cabi.HOST_PATH, cabi.DENSE_PATH and cabi.ROLLOUT_PATH, the native parts of the
+tensor-level wrappers, of dense.py and of rollout.py (g++ against the installed torch and Python, whose versions are in their names).  nvcc cross-compiles without a GPU.
 
     python -m fp4_post_b200.build --timing-knobs
 
@@ -22,7 +22,7 @@ import sys
 import sysconfig
 from pathlib import Path
 
-from .cabi import DENSE_PATH, HOST_PATH
+from .cabi import DENSE_PATH, HOST_PATH, ROLLOUT_PATH
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -31,7 +31,9 @@ LIB = OUT_DIR / "libmetis_nvfp4.so"
 KNOBS_LIB = OUT_DIR / "libmetis_nvfp4_knobs.so"
 HOST_SOURCE = CSRC / "host_ops.cpp"
 DENSE_SOURCE = CSRC / "dense_host.cpp"
-SOURCES = ["api.cu", "quantize.cu", "rmsnorm_quant.cu", "dequantize.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "lowrank_bwd.cu", "decoder_ops.cu", "dense_gemm.cu", "dense_small.cu"]
+ROLLOUT_SOURCE = CSRC / "rollout_host.cpp"
+SOURCES = ["api.cu", "quantize.cu", "rmsnorm_quant.cu", "dequantize.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "lowrank_bwd.cu", "decoder_ops.cu", "dense_gemm.cu", "dense_small.cu",
+           "rotary.cu", "paged_cache.cu", "paged_attention.cu", "sample.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
@@ -91,7 +93,8 @@ def build(force: bool = False, verbose: bool = False, timing_knobs: bool = False
                 print(" ".join(cmd), file=sys.stderr)
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     hosts = []
-    for source, target, libraries in ((HOST_SOURCE, HOST_PATH, ()), (DENSE_SOURCE, DENSE_PATH, ("-lc10_cuda",))):
+    for source, target, libraries in ((HOST_SOURCE, HOST_PATH, ()), (DENSE_SOURCE, DENSE_PATH, ("-lc10_cuda",)),
+                                      (ROLLOUT_SOURCE, ROLLOUT_PATH, ("-lc10_cuda",))):
         if not timing_knobs and (force or _stale(target, [source, PKG.parent / "include" / "metis_nvfp4.h", Path(__file__)])):
             hosts.append((source, subprocess.Popen(_host_command(source, target, libraries), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = []

@@ -16,9 +16,10 @@ import torch                # the native wrappers below link against it: it has 
 # loads it and build.py makes one for each.
 HOST_PATH = Path(__file__).resolve().parent / "_lib" / f"metis_host-{sysconfig.get_config_var('SOABI')}-torch-{torch.__version__}.so"
 DENSE_PATH = HOST_PATH.with_name(HOST_PATH.name.replace("metis_host", "metis_dense", 1))
+ROLLOUT_PATH = HOST_PATH.with_name(HOST_PATH.name.replace("metis_host", "metis_rollout", 1))
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmetis_nvfp4.so"
 
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_E4M3 = 0, 1, 2
 SF_ROWMAJOR, SF_MMA = 0, 1
 ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
 Q_TRANSPOSE, Q_STOCHASTIC, Q_OFFSET_ON_DEVICE, Q_HADAMARD = 1, 2, 4, 8
@@ -31,6 +32,8 @@ STATUS_TEXT = {
     -5: "CUDA error", -6: "unsupported", -7: "too large",
     1: "device timeout waiting for TMA data", 2: "device timeout waiting for the tensor core",
     3: "device timeout waiting for the accumulator hand-off",
+    16: "not enough free pages", 17: "a sequence that the cache does not have", 18: "a sequence longer than its table, or a negative count",
+    19: "the same sequence twice in one call", 20: "a fork's destination that is not empty",
 }
 
 EXPORTS = (
@@ -47,6 +50,8 @@ EXPORTS = (
     "metis_dense_launches", "metis_linear", "metis_linear_pointwise_workspace_bytes", "metis_linear_pointwise", "metis_bf16_product_workspace_bytes", "metis_bf16_product",
     "metis_head_loss_workspace_bytes", "metis_head_loss", "metis_head_sum", "metis_head_backward_workspace_bytes", "metis_head_backward",
     "metis_head_loss_keep", "metis_head_backward_kept",
+    "metis_rollout_launches", "metis_rotary", "metis_cache_check", "metis_cache_append", "metis_cache_attend_workspace_bytes", "metis_cache_attend",
+    "metis_cache_workspace_bytes", "metis_cache_reserve", "metis_cache_fork", "metis_cache_free", "metis_cache_compact", "metis_sample",
 )
 
 
@@ -105,11 +110,65 @@ class HeadArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    """struct metis_rotary_args"""
+    _fields_ = [
+        ("tokens", C.c_int64), ("inner", C.c_int64),
+        ("heads_q", C.c_int32), ("heads_k", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("dtype", C.c_int32), ("positions_64", C.c_int32),
+        ("turns", C.c_void_p), ("magnitude", C.c_float), ("reserved", C.c_int32), ("positions", C.c_void_p),
+        ("q", C.c_void_p), ("q_outer", C.c_int64), ("q_token", C.c_int64), ("q_head", C.c_int64),
+        ("k", C.c_void_p), ("k_outer", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class CacheArgs(C.Structure):
+    """struct metis_cache"""
+    _fields_ = [
+        ("pool", C.c_void_p), ("pages", C.c_int64),
+        ("layers", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("tables", C.c_void_p), ("sequences", C.c_int64), ("width", C.c_int64), ("lengths", C.c_void_p), ("refs", C.c_void_p),
+        ("scales", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class AppendArgs(C.Structure):
+    """struct metis_append_args"""
+    _fields_ = [
+        ("tokens", C.c_int64), ("layer", C.c_int32), ("heads_q", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32),
+        ("turns", C.c_void_p), ("magnitude", C.c_float), ("index_64", C.c_int32), ("slots", C.c_void_p), ("positions", C.c_void_p),
+        ("q", C.c_void_p), ("q_token", C.c_int64), ("q_head", C.c_int64), ("k", C.c_void_p), ("k_token", C.c_int64), ("k_head", C.c_int64),
+        ("v", C.c_void_p), ("v_token", C.c_int64), ("v_head", C.c_int64), ("q_out", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class AttendArgs(C.Structure):
+    """struct metis_attend_args"""
+    _fields_ = [
+        ("rows", C.c_int64), ("layer", C.c_int32), ("heads_q", C.c_int32), ("slots", C.c_void_p), ("slots_64", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
+class SampleArgs(C.Structure):
+    """struct metis_sample_args"""
+    _fields_ = [
+        ("rows", C.c_int64), ("vocab", C.c_int64), ("logits", C.c_void_p), ("ld", C.c_int64), ("dtype", C.c_int32), ("u_64", C.c_int32), ("u", C.c_void_p),
+        ("top_p", C.c_double), ("temperature", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32), ("reserved", C.c_int32),
+        ("temperature_rows", C.c_void_p), ("top_p_rows", C.c_void_p), ("min_p_rows", C.c_void_p), ("top_k_rows", C.c_void_p),
+        ("token", C.c_void_p), ("logprob", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
 _lib = None
 _host = None
 _host_lib = None            # the library whose entry points _host has
 _dense = None
 _dense_lib = None
+_rollout = None
+_rollout_lib = None
 
 
 class MetisLibraryError(RuntimeError):
@@ -214,6 +273,25 @@ def lib() -> C.CDLL:
     L.metis_head_backward.restype = i32
     L.metis_head_backward_kept.argtypes = [C.POINTER(HeadArgs), vp, vp, i32, vp, vp, i64, vp, i64]
     L.metis_head_backward_kept.restype = i32
+    L.metis_rollout_launches.argtypes = []
+    L.metis_rollout_launches.restype = i64
+    cache = C.POINTER(CacheArgs)
+    L.metis_rotary.argtypes = [C.POINTER(RotaryArgs)]
+    L.metis_cache_check.argtypes = [cache]
+    L.metis_cache_append.argtypes = [cache, C.POINTER(AppendArgs)]
+    L.metis_cache_attend_workspace_bytes.argtypes = [cache, i64, i32]
+    L.metis_cache_attend.argtypes = [cache, C.POINTER(AttendArgs)]
+    L.metis_cache_workspace_bytes.argtypes = [cache, i64]
+    L.metis_cache_reserve.argtypes = [cache, vp, vp, i64, i32, i64, vp, i64, vp]
+    L.metis_cache_fork.argtypes = [cache, vp, vp, i32, i64, i32, vp, i64, vp]
+    L.metis_cache_free.argtypes = [cache, vp, i32, i64, vp]
+    L.metis_cache_compact.argtypes = [cache, vp, vp, i64, vp]
+    L.metis_sample.argtypes = [C.POINTER(SampleArgs)]
+    for name in ("metis_cache_attend_workspace_bytes", "metis_cache_workspace_bytes"):
+        getattr(L, name).restype = i64
+    for name in ("metis_rotary", "metis_cache_check", "metis_cache_append", "metis_cache_attend", "metis_cache_reserve", "metis_cache_fork", "metis_cache_free",
+                 "metis_cache_compact", "metis_sample"):
+        getattr(L, name).restype = i32
     _lib = L
     return L
 
@@ -250,6 +328,15 @@ def _bind_dense() -> None:
     _dense_lib = L
 
 
+def _bind_rollout() -> None:
+    global _rollout, _rollout_lib
+    L = lib()
+    if _rollout is None:
+        _rollout = _native("metis_rollout", ROLLOUT_PATH)
+    _bind(_rollout, L)
+    _rollout_lib = L
+
+
 def host():
     """The native part of the wrappers in ops.py (csrc/host_ops.cpp), with the entry points of lib(): allocations and call in one; every
     function returns (status, tensors...).  Callers of the C entry points alone do without it."""
@@ -263,6 +350,18 @@ def dense_host():
     if _dense_lib is None or _dense_lib is not _lib:
         _bind_dense()
     return _dense
+
+
+def rollout_host():
+    """The native part of rollout.py (csrc/rollout_host.cpp), with the entry points of lib()."""
+    if _rollout_lib is None or _rollout_lib is not _lib:
+        _bind_rollout()
+    return _rollout
+
+
+def rollout_launches() -> int:
+    """Kernels that the calls of rollout.py have launched: none before the library is loaded, which a count does not do."""
+    return 0 if _lib is None else _lib.metis_rollout_launches()
 
 
 def dense_launches() -> int:

@@ -1,0 +1,579 @@
+// Attention of one new token for each row over a paged key-value cache, split over the keys of all rows and joined.
+//
+//   s_j = scale q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j
+//
+// Every key and value is read once and meets the few query heads of its key-value head (6 or 7 in this repository's decoders): 14 flops for each
+// byte, which memory bounds as long as the tensor core does them (fp32 units alone would take as long as the memory).  Tiles are of 16 keys.  The keys
+// are the rows of the matrix product and the query heads its columns, S^T = K Q^T and O^T = V^T P^T: eight columns hold a whole group, where the
+// usual orientation would pad the group to 16 rows and do twice the work; and mma.sync it is, because a tile of 128 rows has nothing to
+// put into the other columns that a tcgen05 product would have.
+//
+// A warp owns its tiles: it brings them by asynchronous copies into its own ring of shared memory (no barrier with other warps), keeps its own running
+// maximum, sum and output in registers, and the warps of a block are joined when their row ends.  The flattened list of all tiles of all (row, key-value
+// head) pairs is cut into equal parts, one for each block that the GPU holds at once, whatever the lengths are (they are on the device): a block
+// finds its part by the sum of the lengths.  A pair that one block covers is finished there; of one that several cover, each writes its maximum, sum
+// and output to the workspace, and a second launch joins them in order.
+//
+// p goes into its product as two bf16 numbers (off by 2^-15 together: the first is less than 2^-7 of p below it, the second rounds that by 2^-8 of
+// itself), or one fp16 number (2^-12, with e4m3): the rounding of the output, 2^-9 on the average, is the only one that counts.  Statistics and sums
+// are fp32.
+#include "rollout.cuh"
+
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+namespace metis {
+namespace {
+
+constexpr int kTile = 16;                 // keys of a tile
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxRows = 1024;            // of one launch: their lengths are summed in shared memory
+constexpr int kMinTiles = kWarps;         // of a block's part, so that each warp has one
+
+struct AttendParams {
+  const __nv_bfloat16* q;
+  int64_t q_row, q_head;
+  __nv_bfloat16* out;
+  float* lse;
+  const void* slots;
+  bool slots_64;
+  int32_t rows, heads_q, group, chunks;   // chunks: pieces of a group that a block takes at once, each a unit of work beside others
+  const int32_t* lengths;
+  const int32_t* tables;
+  int64_t sequences, width, pages, page_bytes;
+  int32_t kv_heads, page_size, head_dim;
+  const char* keys;                       // of the layer, on page 0
+  int64_t values_off;                     // bytes from keys to values
+  const float* scales;                    // [2, kv_heads], or null
+  float scale;                            // times log2(e)
+  float* part_o;                          // [2 blocks, 8 NT, D]
+  float2* part_ml;                        // [2 blocks, 8 NT]
+  int4* join;                             // [blocks]: row, key-value head and chunk, last block
+};
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes, or zeros where `bytes` is 0 (the source is not read then)
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void matrices(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void matrices_transposed(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+template <bool kHalf>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kHalf)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two e4m3 -> two fp16, exactly
+__device__ __forceinline__ uint32_t widen(uint32_t two) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((uint16_t)two));
+  return d;
+}
+__device__ __forceinline__ uint32_t bits(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+
+// Rows of a tile in shared memory: 16-byte pieces exchanged by the row, so that eight rows' pieces of one column lie in eight different
+// groups of banks (rows of 64 bytes lie two to a line of 128).
+template <int kRowBytes> __device__ __forceinline__ int piece_at(int row, int piece) {
+  if constexpr (kRowBytes == 64) return row * 64 + ((piece ^ (row >> 1)) & 3) * 16;
+  else return row * kRowBytes + ((piece & ~7) | ((piece ^ row) & 7)) * 16;
+}
+
+template <int D, int NT, bool kE4m3> struct Plan {
+  static constexpr int kItem = kE4m3 ? 1 : 2;
+  static constexpr int kRowBytes = D * kItem;
+  static constexpr int kPartBytes = kTile * kRowBytes;                  // keys, or values, of a tile
+  static constexpr int kStages = kE4m3 ? 6 : 3;
+  static constexpr int kWarpBytes = kStages * 2 * kPartBytes;           // >= 8 NT D fp32, which is what a warp leaves there at the end of a row
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kPieces = kRowBytes / 16;
+  static_assert(8 * NT * D * 4 <= kWarpBytes, "a warp's output goes where its tiles were");
+};
+
+template <int D, int NT, bool kE4m3>
+__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) {
+  using L = Plan<D, NT, kE4m3>;
+  extern __shared__ __align__(128) char ring[];
+  __shared__ int64_t before[kMaxRows + 1];           // tiles of the rows in front, for one key-value head
+  __shared__ int64_t warp_sums[kWarps];
+  __shared__ float2 warp_ml[kWarps][8 * NT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  grid_dependency_wait();
+
+  // ---- this block's part of the tiles ----
+  auto row_slot = [&](int row) -> int64_t {
+    const int64_t slot = p.slots ? load_index(p.slots, p.slots_64, row) : row;
+    return slot >= 0 && slot < p.sequences ? slot : -1;
+  };
+  auto row_length = [&](int64_t slot) -> int64_t {
+    if (slot < 0) return 0;
+    const int64_t length = p.lengths[slot], most = p.width * p.page_size;
+    return length < 0 ? 0 : length < most ? length : most;
+  };
+  for (int base = 0; base < p.rows; base += kThreads) {
+    const int row = base + threadIdx.x;
+    int64_t tiles = row < p.rows ? (row_length(row_slot(row)) + kTile - 1) / kTile : 0, all;
+    const int64_t ahead = base ? before[base] : 0;
+    const int64_t mine = ahead + block_exclusive<kThreads>(tiles, warp_sums, all);
+    if (row < p.rows) {
+      before[row] = mine;
+      if (row == p.rows - 1) before[p.rows] = mine + tiles;
+    }
+    if (threadIdx.x == kThreads - 1 && base + kThreads < p.rows) before[base + kThreads] = mine + tiles;
+    __syncthreads();
+  }
+  const int heads = p.kv_heads * p.chunks;                               // units of work beside one another on the same row
+  const int64_t total = before[p.rows] * heads;
+  const int64_t parts = min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+  const int64_t cta = blockIdx.x;
+  // rows without keys
+  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    if (before[row + 1] != before[row]) continue;
+    for (int i = threadIdx.x; i < p.heads_q * p.head_dim; i += kThreads) p.out[(int64_t)row * p.heads_q * p.head_dim + i] = __float2bfloat16_rn(0.0f);
+    if (p.lse) for (int i = threadIdx.x; i < p.heads_q; i += kThreads) p.lse[(int64_t)row * p.heads_q + i] = -CUDART_INF_F;
+  }
+  if (threadIdx.x == 0) p.join[cta] = make_int4(-1, 0, 0, 0);
+  if (cta >= parts) return;
+  int64_t at = cta * total / parts;
+  const int64_t end = (cta + 1) * total / parts;
+
+  char* const mine = ring + warp * L::kWarpBytes;
+  const uint32_t mine_at = smem_address(mine);
+  while (at < end) {
+    // the row that the tile belongs to: the last one that begins at or before it (rows without tiles begin where the next one does)
+    int lo = 0, hi = p.rows;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] * heads <= at) lo = mid; else hi = mid;
+    }
+    const int row = lo;
+    const int64_t row_tiles = before[row + 1] - before[row], inside = at - before[row] * heads;
+    const int unit = (int)(inside / row_tiles), head = unit / p.chunks, chunk = unit - head * p.chunks;
+    const int64_t begin = inside - unit * row_tiles, stop = min(row_tiles, begin + (end - at));
+    const int64_t slot = row_slot(row), length = row_length(slot);
+    const int first_head = head * p.group + chunk * 8 * NT, live = min(8 * NT, p.group - chunk * 8 * NT);
+    const float k_scale = p.scales ? p.scales[head] : 1.0f, v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
+
+    // ---- queries as the columns of a product: of step i, elements 16 i + 2 t and + 8 of head g (e4m3: in the order in which the keys come) ----
+    uint32_t q[NT][D / 16][2];
+    float q_scale[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool there = n * 8 + g < live;
+      const __nv_bfloat16* x = p.q + (int64_t)row * p.q_row + (int64_t)(first_head + n * 8 + g) * p.q_head;
+      float biggest = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int e = i * 16 + (kE4m3 ? 4 * t + 2 * j : 2 * t + 8 * j);
+          q[n][i][j] = there && e < p.head_dim ? *reinterpret_cast<const uint32_t*>(x + e) : 0u;
+          if constexpr (kE4m3) biggest = fmaxf(biggest, fmaxf(fabsf(bf16_lo(q[n][i][j])), fabsf(bf16_hi(q[n][i][j]))));
+        }
+      q_scale[n] = 1.0f;
+      if constexpr (kE4m3) {
+        // fp16 holds a row of bf16 exactly where it is brought to [1, 2) by a power of two; what lies 2^14 below the row's largest element
+        // loses bits that are 2^-25 of that one.  (Infinite and NaN rows stay what they are.)
+        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 1));
+        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 2));
+        const int e = min(max((int)((__float_as_uint(biggest) >> 23) & 255u), 2), 252);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) q[n][i][j] = bits(__floats2half2_rn(bf16_lo(q[n][i][j]) * down, bf16_hi(q[n][i][j]) * down));
+        q_scale[n] = __uint_as_float((uint32_t)e << 23);
+      }
+    }
+    // what scores of the columns 2 t and 2 t + 1 are multiplied by
+    float s_scale[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s_scale[n][j] = p.scale * k_scale * (kE4m3 ? __shfl_sync(0xffffffffu, q_scale[n], (2 * t + j) * 4) : 1.0f);
+
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+      m[n][0] = m[n][1] = -CUDART_INF_F;
+      l[n][0] = l[n][1] = 0.0f;
+    }
+
+    // ---- the warp's tiles: begin + warp, and every fourth from there ----
+    const int64_t first = begin + warp;
+    const int mine_count = first < stop ? (int)((stop - first + kWarps - 1) / kWarps) : 0;
+    const int page_tiles = p.page_size / kTile;
+    const int32_t* table = p.tables + slot * p.width;
+    const int64_t head_off = (int64_t)head * p.page_size * p.head_dim * L::kItem;
+    const int row_bytes = p.head_dim * L::kItem;
+    int32_t page = -1;                    // of the lane's tile among the 32 that are looked up at once
+    int fetched = 0;                      // tiles whose copies have been issued
+    uint32_t absent = 0;                  // bit i: the tile i before the last fetched one lies on no page of the pool
+    auto fetch = [&]() {
+      if (fetched < mine_count) {
+        if ((fetched & 31) == 0) {
+          const int64_t tile = first + (int64_t)(fetched + lane) * kWarps;
+          page = tile < stop ? table[tile / page_tiles] : -1;
+        }
+        const int32_t pg = __shfl_sync(0xffffffffu, page, fetched & 31);
+        const int64_t tile = first + (int64_t)fetched * kWarps;
+        const bool good = pg >= 0 && pg < p.pages;
+        absent = absent << 1 | (good ? 0u : 1u);
+        const int keys = good ? (int)min((int64_t)kTile, length - tile * kTile) : 0;
+        const char* from = p.keys + (good ? (int64_t)pg * p.page_bytes + head_off + (tile % page_tiles) * kTile * row_bytes : 0);
+        const uint32_t to = mine_at + (uint32_t)(fetched % L::kStages) * 2 * L::kPartBytes;
+#pragma unroll
+        for (int i = 0; i < kTile * L::kPieces / 32; ++i) {
+          const int piece = i * 32 + lane, r = piece / L::kPieces, c = piece % L::kPieces;
+          const bool in = r < keys && c * 16 < row_bytes;
+          const char* src = from + (in ? r * row_bytes + c * 16 : 0);
+          const uint32_t dst = to + piece_at<L::kRowBytes>(r, c);
+          if (!kE4m3 || row_bytes % 16 == 0) {
+            copy16(dst, src, in ? 16 : 0);
+            copy16(dst + L::kPartBytes, src + p.values_off, in ? 16 : 0);
+          } else {
+            // (rows of an odd number of 8 bytes begin on 8 bytes alone)
+            const bool both = in && c * 16 + 8 < row_bytes;
+            copy8(dst, src, in ? 8 : 0);
+            copy8(dst + 8, src + (both ? 8 : 0), both ? 8 : 0);
+            copy8(dst + L::kPartBytes, src + p.values_off, in ? 8 : 0);
+            copy8(dst + L::kPartBytes + 8, src + (both ? 8 : 0) + p.values_off, both ? 8 : 0);
+          }
+        }
+        ++fetched;
+      }
+      copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) fetch();
+
+    for (int done = 0; done < mine_count; ++done) {
+      copies_wait<L::kStages - 2>();
+      __syncwarp();                        // every lane's copies of this tile are there, and the tile before it has been read by all
+      fetch();
+      const uint32_t kt = mine_at + (uint32_t)(done % L::kStages) * 2 * L::kPartBytes, vt = kt + L::kPartBytes;
+      const int64_t tile = first + (int64_t)done * kWarps;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+      if constexpr (!kE4m3) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t a[4];
+          matrices(kt + piece_at<L::kRowBytes>(lane & 15, 2 * i + (lane >> 4)), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) multiply<false>(s[n], a, q[n][i][0], q[n][i][1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2) {
+          uint32_t r[4];
+          matrices(kt + piece_at<L::kRowBytes>(lane & 15, i + (lane >> 4)), r);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a[4] = {widen(r[2 * j]), widen(r[2 * j + 1]), widen(r[2 * j] >> 16), widen(r[2 * j + 1] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) multiply<true>(s[n], a, q[n][i + j][0], q[n][i + j][1]);
+          }
+        }
+      }
+      // ---- softmax: column 2 t + j, keys g and g + 8 ----
+      const int64_t left = (absent >> (fetched - 1 - done)) & 1u ? 0 : length - tile * kTile;
+      const bool in0 = g < left, in1 = g + 8 < left;
+      uint32_t hi[NT][2], lo_[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float pr[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x0 = in0 ? s[n][j] * s_scale[n][j] : -CUDART_INF_F, x1 = in1 ? s[n][2 + j] * s_scale[n][j] : -CUDART_INF_F;
+          float top = fmaxf(x0, x1);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float now = fmaxf(m[n][j], top), from = now == -CUDART_INF_F ? 0.0f : now;
+          const float keep = exp2_fast(m[n][j] - from);
+          pr[j] = exp2_fast(x0 - from);
+          pr[2 + j] = exp2_fast(x1 - from);
+          m[n][j] = now;
+          l[n][j] = l[n][j] * keep + (pr[j] + pr[2 + j]);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][j] *= keep;
+            o[n][i][2 + j] *= keep;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (kE4m3) {
+            hi[n][r] = transpose8(bits(__floats2half2_rn(pr[2 * r], pr[2 * r + 1])));
+          } else {
+            // the first part is the largest bf16 below p, so that the second one is positive: zero or negative, it would make NaN of an infinite value
+            const uint32_t w = __byte_perm(max(__float_as_uint(pr[2 * r]), 1u) - 1u, max(__float_as_uint(pr[2 * r + 1]), 1u) - 1u, 0x7632);
+            hi[n][r] = transpose8(w);
+            lo_[n][r] = transpose8(bits(__floats2bfloat162_rn(pr[2 * r] - bf16_lo(w), pr[2 * r + 1] - bf16_hi(w))));
+          }
+        }
+      }
+      // ---- values ----
+      if constexpr (!kE4m3) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t a[4];
+          matrices_transposed(vt + piece_at<L::kRowBytes>((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            multiply<false>(o[n][i], a, hi[n][0], hi[n][1]);
+            multiply<false>(o[n][i], a, lo_[n][0], lo_[n][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2) {
+          uint32_t r[4];                   // pairs of elements 16 i + 2 g of keys 2 t, 2 t + 1 and 8 more; the same of 16 (i + 1)
+          matrices_transposed(vt + piece_at<L::kRowBytes>(lane & 15, i + (lane >> 4)), r);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x = __byte_perm(r[2 * j], 0, 0x3120), y = __byte_perm(r[2 * j + 1], 0, 0x3120);
+            const uint32_t a[4] = {widen(x), widen(x >> 16), widen(y), widen(y >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) multiply<true>(o[n][i + j], a, hi[n][0], hi[n][1]);
+          }
+        }
+      }
+    }
+    copies_wait<0>();
+    __syncwarp();
+
+    // ---- join the warps; element of o[n][i]: c0, c1 of row g, c2, c3 of row g + 8 of the output's 16 i, columns 2 t, 2 t + 1 ----
+    float* const left_o = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = l[n][j];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int column = n * 8 + 2 * t + j;
+        if (g == 0) warp_ml[warp][column] = make_float2(m[n][j], sum);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int e0 = i * 16 + (kE4m3 ? 2 * g : g), e1 = i * 16 + (kE4m3 ? 2 * g + 1 : g + 8);
+          left_o[column * D + e0] = o[n][i][j];
+          left_o[column * D + e1] = o[n][i][2 + j];
+        }
+      }
+    __syncthreads();
+    const bool whole = begin == 0 && stop == row_tiles;
+    const int64_t place = (cta * 2 + (begin == 0 ? 1 : 0)) * 8 * NT;
+    for (int i = threadIdx.x; i < live * D; i += kThreads) {
+      const int column = i / D, e = i - column * D;
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][column].x);
+      const float from = top == -CUDART_INF_F ? 0.0f : top;
+      float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = warp_ml[w][column];
+        const float f = exp2_fast(ml.x - from);
+        sum += ml.y * f;
+        acc += reinterpret_cast<const float*>(ring + w * L::kWarpBytes)[i] * f;
+      }
+      if (whole) {
+        const int64_t to = (int64_t)row * p.heads_q + first_head + column;
+        if (e < p.head_dim) p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(acc, sum) * v_scale);
+        if (e == 0 && p.lse) p.lse[to] = (from + log2f(sum)) * 0.69314718055994531f;
+      } else {
+        p.part_o[(place + column) * D + e] = acc;
+        if (e == 0) p.part_ml[place + column] = make_float2(top, sum);
+      }
+    }
+    if (!whole && begin > 0 && threadIdx.x == 0) {
+      // the block whose part ends in the middle of the row's first piece leaves the joining to the next one
+      const int64_t start = before[row] * heads + unit * row_tiles, last = start + row_tiles - 1;
+      const int64_t c0 = ((start + 1) * parts - 1) / total, c1 = ((last + 1) * parts - 1) / total;
+      if (c0 == cta - 1) p.join[cta] = make_int4(row, unit, (int)c1, 0);
+    }
+    __syncthreads();                       // the ring is free again
+    at += stop - begin;
+  }
+}
+
+// Joins the pieces of a row that several blocks wrote: block x those of which the second piece is block x's, for one query head of the group.  A
+// warp takes every eighth piece, a lane D / 32 elements.
+template <int D, int NT>
+__global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
+  constexpr int E = D / 32;
+  __shared__ float acc_of[8][D];
+  __shared__ float2 ml_of[8];
+  grid_dependency_wait();
+  const int4 job = p.join[blockIdx.x];
+  if (job.x < 0) return;
+  const int head = job.y / p.chunks, chunk = job.y - head * p.chunks, column = blockIdx.y;
+  if (chunk * 8 * NT + column >= p.group) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = (int64_t)blockIdx.x - 1;
+  const int pieces = (int)(job.z - c0) + 1;
+  auto place = [&](int i) { return ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
+  float top = -CUDART_INF_F;
+  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float from = top == -CUDART_INF_F ? 0.0f : top;
+  float acc[E], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+  for (int i = warp; i < pieces; i += 8) {
+    const int64_t at = place(i);
+    const float2 ml = p.part_ml[at];
+    const float f = exp2_fast(ml.x - from);
+    sum += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += p.part_o[at * D + e * 32 + lane] * f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc_of[warp][e * 32 + lane] = acc[e];
+  if (lane == 0) ml_of[warp] = make_float2(0.0f, sum);
+  __syncthreads();
+  const int64_t to = (int64_t)job.x * p.heads_q + head * p.group + chunk * 8 * NT + column;
+  const float v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
+  float all = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) all += ml_of[w].y;
+  for (int e = threadIdx.x; e < p.head_dim; e += 256) {
+    float a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) a += acc_of[w][e];
+    p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(a, all) * v_scale);
+  }
+  if (threadIdx.x == 0 && p.lse) p.lse[to] = (from + log2f(all)) * 0.69314718055994531f;
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+// Columns of eight that a block takes at once: the whole group up to 32 heads (16 of 256 elements: registers), in pieces beyond.
+int column_tiles(int group, int D) {
+  const int nt = group <= 8 ? 1 : group <= 16 ? 2 : 4;
+  return D == 256 && nt > 2 ? 2 : nt;
+}
+
+template <int D, int NT, bool kE4m3>
+struct Launch {
+  using L = Plan<D, NT, kE4m3>;
+  static int64_t workspace(int64_t blocks) { return blocks * (16 + 16 * NT * (8 + D * 4)); }
+  // as many as the GPU holds at once
+  static int32_t blocks(int64_t* n) {
+    if (const cudaError_t e = allow_smem<&attend_kernel<D, NT, kE4m3>>(L::kSmem); e != cudaSuccess) return fail(METIS_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
+    *n = (int64_t)device_sm_count() * resident_ctas(reinterpret_cast<const void*>(attend_kernel<D, NT, kE4m3>), kThreads, L::kSmem);
+    return METIS_OK;
+  }
+  static int32_t run(AttendParams p, void* ws, int64_t ws_bytes, cudaStream_t st) {
+    int64_t n = 0;
+    if (const int32_t rc = blocks(&n)) return rc;
+    if (ws_bytes < workspace(n)) return fail(METIS_ERR_WORKSPACE, "the workspace has %lld bytes, %lld are needed", (long long)ws_bytes, (long long)workspace(n));
+    char* w = static_cast<char*>(ws);
+    p.join = reinterpret_cast<int4*>(w);
+    p.part_ml = reinterpret_cast<float2*>(w + n * 16);
+    p.part_o = reinterpret_cast<float*>(w + n * (16 + 16 * NT * 8));
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, attend_kernel<D, NT, kE4m3>, dim3((unsigned)n), dim3(kThreads), L::kSmem, st, p));
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT>, dim3((unsigned)n, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
+    count_rollout_launches(2);
+    return METIS_OK;
+  }
+};
+
+// f(Launch<...>()) of the kernel for these sizes
+template <typename F>
+int32_t with_kernel(int head_dim, int group, bool e4m3, const F& f) {
+  const int D = padded_dim(head_dim), nt = column_tiles(group, D);
+  if (D == 64)  return nt == 1 ? (e4m3 ? f(Launch<64, 1, true>()) : f(Launch<64, 1, false>())) : nt == 2 ? (e4m3 ? f(Launch<64, 2, true>()) : f(Launch<64, 2, false>()))
+                                                                                              : (e4m3 ? f(Launch<64, 4, true>()) : f(Launch<64, 4, false>()));
+  if (D == 128) return nt == 1 ? (e4m3 ? f(Launch<128, 1, true>()) : f(Launch<128, 1, false>())) : nt == 2 ? (e4m3 ? f(Launch<128, 2, true>()) : f(Launch<128, 2, false>()))
+                                                                                                : (e4m3 ? f(Launch<128, 4, true>()) : f(Launch<128, 4, false>()));
+  return nt == 1 ? (e4m3 ? f(Launch<256, 1, true>()) : f(Launch<256, 1, false>())) : (e4m3 ? f(Launch<256, 2, true>()) : f(Launch<256, 2, false>()));
+}
+
+}  // namespace
+}  // namespace metis
+
+using namespace metis;
+
+extern "C" int64_t metis_cache_attend_workspace_bytes(const metis_cache* c, int64_t rows, int32_t heads_q) {
+  if (!c || rows <= 0 || c->kv_heads <= 0 || heads_q <= 0 || c->head_dim <= 0 || c->head_dim > 256) return 0;
+  int64_t bytes = 0;
+  const int32_t rc = with_kernel(c->head_dim, heads_q / c->kv_heads, c->dtype == METIS_DTYPE_E4M3, [&](auto kernel) {
+    int64_t n = 0;
+    const int32_t failed = kernel.blocks(&n);
+    bytes = kernel.workspace(n);
+    return failed;
+  });
+  return rc ? 0 : bytes;
+}
+
+extern "C" int32_t metis_cache_attend(const metis_cache* cache, const metis_attend_args* a) {
+  CacheView c;
+  if (const int32_t rc = check_cache(cache, &c)) return rc;
+  if (!a || !a->q || !a->out || !a->workspace) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
+  if (a->rows <= 0 || a->heads_q <= 0 || a->heads_q % c.kv_heads != 0 || a->layer < 0 || a->layer >= c.layers)
+    return fail(METIS_ERR_BAD_SHAPE, "rows must be positive, heads_q a multiple of kv_heads and the layer one of the cache");
+  if (a->q_row % 2 != 0 || a->q_head % 2 != 0 || (reinterpret_cast<uintptr_t>(a->q) & 3) || !aligned16(a->workspace))
+    return fail(METIS_ERR_BAD_ALIGNMENT, "rows of q must be 4-byte aligned and the workspace 16");
+  const int group = a->heads_q / c.kv_heads, nt = column_tiles(group, padded_dim(c.head_dim));
+  const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;
+  const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  // more rows than one launch counts go in several, one after the other: they share the workspace
+  for (int64_t row = 0; row < a->rows; row += kMaxRows) {
+    AttendParams p = {};
+    p.rows = (int32_t)min((int64_t)kMaxRows, a->rows - row);
+    p.q = static_cast<const __nv_bfloat16*>(a->q) + row * a->q_row; p.q_row = a->q_row; p.q_head = a->q_head;
+    p.out = static_cast<__nv_bfloat16*>(a->out) + row * a->heads_q * c.head_dim;
+    p.lse = a->lse ? a->lse + row * a->heads_q : nullptr;
+    p.slots = a->slots ? static_cast<const char*>(a->slots) + row * (a->slots_64 ? 8 : 4) : nullptr;
+    p.slots_64 = a->slots_64 != 0;
+    p.heads_q = a->heads_q; p.group = group; p.chunks = (group + 8 * nt - 1) / (8 * nt);
+    p.lengths = c.lengths; p.tables = c.tables; p.sequences = c.sequences; p.width = c.width;
+    if (!a->slots && row > 0) {              // row i of the launch is sequence row + i
+      p.lengths += row; p.tables += row * c.width; p.sequences = c.sequences > row ? c.sequences - row : 0;
+    }
+    p.pages = c.pages; p.page_bytes = c.page_bytes; p.kv_heads = c.kv_heads; p.page_size = c.page_size; p.head_dim = c.head_dim;
+    p.keys = c.pool + a->layer * 2 * part;
+    p.values_off = part;
+    p.scales = cache->scales ? cache->scales + (int64_t)a->layer * 2 * c.kv_heads : nullptr;
+    p.scale = a->scale * 1.4426950408889634f;
+    const int32_t rc = with_kernel(c.head_dim, group, c.item == 1, [&](auto kernel) { return kernel.run(p, a->workspace, a->workspace_bytes, st); });
+    if (rc != METIS_OK) return rc;
+  }
+  return METIS_OK;
+}

@@ -1,0 +1,81 @@
+// What the kernels of a rollout share: indices of either width, the cache's addresses, sums over a block.
+#pragma once
+
+#include <atomic>
+
+#include "common.cuh"
+
+namespace metis {
+
+void count_rollout_launches(int n);
+
+// The cache as the kernels see it: metis_cache, checked.
+struct CacheView {
+  char* pool;
+  int64_t page_bytes;       // of one page, all layers
+  int64_t pages;
+  int32_t* tables;
+  int64_t sequences, width;
+  int32_t* lengths;
+  int32_t* refs;
+  int32_t* status;
+  int32_t layers, kv_heads, page_size, head_dim, item;      // item: bytes of an element
+};
+int32_t check_cache(const metis_cache* c, CacheView* view);
+
+#ifdef __CUDACC__
+
+// Lets a kernel take `bytes` of shared memory, asked once for each device.
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+__device__ __forceinline__ int64_t load_index(const void* p, bool wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
+}
+
+// Sums over the block of `kThreads` threads: what the threads before this one have, that with its own, and all.  Integers, or doubles in a
+// fixed order; what one thread gets up to itself is bit for bit what the next one has before itself.  `warp_sums` has room for one value
+// per warp; all threads call it.
+template <typename T> struct Scan { T before, upto, all; };
+template <int kThreads, typename T>
+__device__ __forceinline__ Scan<T> block_scan(T v, T* warp_sums) {
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  T sum = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T from = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += from;
+  }
+  __syncthreads();                                   // (warp_sums may still be read from the call before)
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  T ahead = T(0), all = T(0);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) ahead = all;
+    all += warp_sums[w];
+  }
+  const T left = __shfl_up_sync(0xffffffffu, sum, 1);
+  return {lane == 0 ? ahead : ahead + left, ahead + sum, all};
+}
+template <int kThreads, typename T>
+__device__ __forceinline__ T block_exclusive(T v, T* warp_sums, T& total) {
+  const Scan<T> s = block_scan<kThreads>(v, warp_sums);
+  total = s.all;
+  return s.before;
+}
+
+#endif
+
+}  // namespace metis

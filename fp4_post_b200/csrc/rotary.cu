@@ -1,0 +1,388 @@
+// Rotary positions, and the same with the keys and values written into a paged cache.
+//
+// A pair (a, b) of a head at position p goes to m (a cos - b sin, b cos + a sin) of the angle 2 pi p f, f a frequency in turns per position.  f is held
+// as a 64-bit fraction of a turn: p f modulo 1 is then one integer product whose high bits are thrown away, exact to p 2^-65 turns at any
+// position, and the angle never needs a range reduction (fp32 products of positions and frequencies are off by p 2^-24, a whole radian at 2^24).
+// No table of cosines is kept or read: a block forms those of its tokens once, in shared memory, and uses them for all heads.
+//
+// Bound by memory: every element is read and written once.  A thread holds the cosines of one unit (16 bytes of each half, or 16 bytes of
+// neighbouring pairs) in registers and takes it through the heads of its token; of few tokens, heads are spread over the block instead.
+#include "rollout.cuh"
+
+#include <cuda_fp16.h>
+
+namespace metis {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RotaryShape {
+  int32_t heads_q, heads_k, head_dim, rotary_dim;
+  int32_t units, rotary_units;        // of a head: all, and those that turn
+  int32_t head_lanes, block_tokens;   // threads that share a token's heads, tokens of a block
+  float magnitude, sign;              // what cosines and sines are multiplied by; the direction
+};
+
+template <typename T> struct Vec;
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int kWide = 8;
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+    v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
+    uint4 w;
+    __nv_bfloat162 t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w.x = *reinterpret_cast<uint32_t*>(&t[0]); w.y = *reinterpret_cast<uint32_t*>(&t[1]);
+    w.z = *reinterpret_cast<uint32_t*>(&t[2]); w.w = *reinterpret_cast<uint32_t*>(&t[3]);
+    *reinterpret_cast<uint4*>(p) = w;
+  }
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+};
+template <> struct Vec<float> {
+  static constexpr int kWide = 4;
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
+    const float4 w = *reinterpret_cast<const float4*>(p);
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+
+// cos and sin of the pair of frequency `turn` at a position: the angle in half turns, in [-1, 1)
+__device__ __forceinline__ float2 cos_sin(uint64_t turn, int64_t position, const RotaryShape& s) {
+  const uint64_t part = turn * (uint64_t)position;
+  float sn, cs;
+  sincospif((float)(int32_t)(part >> 32) * 0x1p-31f, &sn, &cs);
+  return make_float2(cs * s.magnitude, sn * s.magnitude * s.sign);
+}
+
+// One unit of a head: the two pieces of W elements (half layout), one piece of W elements (neighbouring pairs; c[] by pairs), or W elements that
+// are copied.  kPair: W = 1, the elements of one pair.
+template <typename T, int W, bool kInterleaved, typename Put>
+__device__ __forceinline__ void turn_unit(const T* x, int unit, const float2 (&c)[W], const RotaryShape& s, bool turns, const Put& put) {
+  if constexpr (W == 1) {
+    if (!turns) {
+      put.one(s.rotary_dim + unit - s.rotary_units, Vec<T>::one(x + s.rotary_dim + unit - s.rotary_units));
+      return;
+    }
+    const int i = kInterleaved ? 2 * unit : unit, j = kInterleaved ? 2 * unit + 1 : unit + s.rotary_dim / 2;
+    const float a = Vec<T>::one(x + i), b = Vec<T>::one(x + j);
+    put.one(i, fmaf(a, c[0].x, -b * c[0].y));
+    put.one(j, fmaf(b, c[0].x, a * c[0].y));
+  } else {
+    float a[W];
+    if (!turns) {
+      const int at = s.rotary_dim + (unit - s.rotary_units) * W;
+      Vec<T>::load(x + at, a);
+      put.wide(at, a);
+    } else if constexpr (kInterleaved) {
+      Vec<T>::load(x + unit * W, a);
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        const float u = a[i], v = a[i + 1];
+        a[i] = fmaf(u, c[i / 2].x, -v * c[i / 2].y);
+        a[i + 1] = fmaf(v, c[i / 2].x, u * c[i / 2].y);
+      }
+      put.wide(unit * W, a);
+    } else {
+      float b[W];
+      const int at = unit * W, bt = at + s.rotary_dim / 2;
+      Vec<T>::load(x + at, a);
+      Vec<T>::load(x + bt, b);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float u = a[i], v = b[i];
+        a[i] = fmaf(u, c[i].x, -v * c[i].y);
+        b[i] = fmaf(v, c[i].x, u * c[i].y);
+      }
+      put.wide(at, a);
+      put.wide(bt, b);
+    }
+  }
+}
+
+// pairs of a unit
+template <int W, bool kInterleaved> __host__ __device__ constexpr int unit_pairs() { return W == 1 ? 1 : kInterleaved ? W / 2 : W; }
+
+// The cosines of this thread's unit, out of the block's table of its tokens.
+template <int W, bool kInterleaved>
+__device__ __forceinline__ void unit_table(const float2* table, int token, int unit, int pairs, bool turns, float2 (&c)[W]) {
+  constexpr int P = unit_pairs<W, kInterleaved>();
+#pragma unroll
+  for (int i = 0; i < P; ++i) c[i] = turns ? table[token * pairs + unit * P + i] : make_float2(1.0f, 0.0f);
+}
+
+template <typename T> struct PutDense {
+  T* out;
+  __device__ __forceinline__ void one(int i, float v) const { Vec<T>::put(out + i, v); }
+  __device__ __forceinline__ void wide(int i, const float (&v)[Vec<T>::kWide]) const { Vec<T>::store(out + i, v); }
+};
+
+struct RotaryTensors {
+  const void* positions;
+  int64_t tokens, inner;
+  const uint64_t* turns;
+  const void *q, *k;
+  int64_t q_outer, q_token, q_head, k_outer, k_token, k_head;
+  void *q_out, *k_out;
+  bool positions_64;
+};
+
+template <typename T, int W, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryTensors t, const RotaryShape s) {
+  extern __shared__ float2 table[];
+  grid_dependency_wait();
+  const int pairs = s.rotary_dim / 2;
+  const int64_t first = (int64_t)blockIdx.x * s.block_tokens;
+  const int here = (int)min((int64_t)s.block_tokens, t.tokens - first);
+  for (int i = threadIdx.x; i < here * pairs; i += kThreads) {
+    const int token = i / pairs;
+    const int64_t at = first + token;
+    table[i] = cos_sin(t.turns[i - token * pairs], t.positions ? load_index(t.positions, t.positions_64, at) : at % t.inner, s);
+  }
+  __syncthreads();
+  const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
+  const int lane = rest % s.head_lanes, token = rest / s.head_lanes;
+  if (token >= here) return;
+  const bool turns = unit < s.rotary_units;
+  float2 c[W];
+  unit_table<W, kInterleaved>(table, token, unit, pairs, turns, c);
+  const int64_t at = first + token, outer = at / t.inner, inner = at - outer * t.inner;
+  const T* q = static_cast<const T*>(t.q) + outer * t.q_outer + inner * t.q_token;
+  T* q_out = static_cast<T*>(t.q_out) + at * s.heads_q * s.head_dim;
+#pragma unroll 4
+  for (int h = lane; h < s.heads_q; h += s.head_lanes)
+    turn_unit<T, W, kInterleaved>(q + h * t.q_head, unit, c, s, turns, PutDense<T>{q_out + (int64_t)h * s.head_dim});
+  if (s.heads_k == 0) return;
+  const T* k = static_cast<const T*>(t.k) + outer * t.k_outer + inner * t.k_token;
+  T* k_out = static_cast<T*>(t.k_out) + at * s.heads_k * s.head_dim;
+#pragma unroll 4
+  for (int h = lane; h < s.heads_k; h += s.head_lanes)
+    turn_unit<T, W, kInterleaved>(k + h * t.k_head, unit, c, s, turns, PutDense<T>{k_out + (int64_t)h * s.head_dim});
+}
+
+// ---- append -------------------------------------------------------------------------------------------------------
+
+struct AppendTensors {
+  CacheView cache;
+  char* layer_pool;                 // the layer's keys on page 0
+  const float* scales;              // [2, kv_heads] of the layer, or null
+  const void *slots, *positions;
+  int64_t tokens;
+  const uint64_t* turns;            // null: nothing turns
+  const __nv_bfloat16 *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  __nv_bfloat16* q_out;
+  bool slots_64, positions_64;
+};
+
+// Elements of the cache: bf16 as they are, e4m3 as x / scale rounded to nearest and saturated (NaN stays NaN).  The quotient is the IEEE one:
+// a product with a reciprocal is off by up to one bit of fp32, which at a border of the format is a step of 2^-3.
+template <bool kE4m3> struct PutCache;
+template <> struct PutCache<false> {
+  __nv_bfloat16* out;
+  float scale;
+  __device__ __forceinline__ void one(int i, float v) const { out[i] = __float2bfloat16_rn(v); }
+  __device__ __forceinline__ void wide(int i, const float (&v)[8]) const { Vec<__nv_bfloat16>::store(out + i, v); }
+};
+template <> struct PutCache<true> {
+  uint8_t* out;
+  float scale;
+  __device__ __forceinline__ void one(int i, float v) const { out[i] = float_to_e4m3(__fdiv_rn(v, scale)); }
+  __device__ __forceinline__ void wide(int i, const float (&v)[8]) const {
+    uint32_t w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[4 * j], scale), __fdiv_rn(v[4 * j + 1], scale)), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[4 * j + 2], scale), __fdiv_rn(v[4 * j + 3], scale)), __NV_SATFINITE, __NV_E4M3);
+      w[j] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(w[0], w[1]);
+  }
+};
+
+// One block takes tokens, and the heads of q, k and v of each, as rotary_kernel does.  What a token goes to is looked up once, by one thread.
+template <int W, bool kInterleaved, bool kE4m3>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendTensors t, const RotaryShape s) {
+  extern __shared__ float2 table[];
+  __shared__ int64_t token_at[kThreads];             // bytes from layer_pool to the token's row in the keys of head 0, -1: nowhere, -2: no sequence
+  __shared__ int64_t token_position[kThreads];
+  grid_dependency_wait();
+  const CacheView& c = t.cache;
+  const int pairs = s.rotary_dim / 2;
+  const int64_t first = (int64_t)blockIdx.x * s.block_tokens;
+  const int here = (int)min((int64_t)s.block_tokens, t.tokens - first);
+  if ((int)threadIdx.x < here) {
+    const int64_t i = first + threadIdx.x, slot = t.slots ? load_index(t.slots, t.slots_64, i) : i;
+    int64_t position = t.positions ? load_index(t.positions, t.positions_64, i) : 0, at = -2;
+    if (slot >= 0 && slot < c.sequences) {
+      const int64_t length = c.lengths[slot];
+      if (!t.positions) position = length - 1;
+      at = -1;
+      if (position >= 0 && position < length && position < c.width * c.page_size) {
+        const int64_t page = c.tables[slot * c.width + position / c.page_size];
+        if (page >= 0 && page < c.pages) at = page * c.page_bytes + (position % c.page_size) * c.head_dim * c.item;
+      }
+    }
+    token_at[threadIdx.x] = at;
+    token_position[threadIdx.x] = position;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < here * pairs; i += kThreads) {
+    const int token = i / pairs;
+    table[i] = cos_sin(t.turns[i - token * pairs], token_position[token], s);
+  }
+  __syncthreads();
+  const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
+  const int lane = rest % s.head_lanes, token = rest / s.head_lanes;
+  if (token >= here) return;
+  const bool turns = unit < s.rotary_units;
+  float2 cs[W];
+  unit_table<W, kInterleaved>(table, token, unit, pairs, turns, cs);
+  const int64_t i = first + token, at = token_at[token];
+  if (s.heads_q > 0) {
+    const __nv_bfloat16* q = t.q + i * t.q_token;
+    __nv_bfloat16* q_out = t.q_out + i * s.heads_q * s.head_dim;
+    if (at == -2) {
+      // (zeros whatever the row holds)
+      for (int h = lane; h < s.heads_q; h += s.head_lanes)
+        for (int e = unit; e < s.head_dim; e += s.units) q_out[(int64_t)h * s.head_dim + e] = __float2bfloat16_rn(0.0f);
+    } else {
+#pragma unroll 4
+      for (int h = lane; h < s.heads_q; h += s.head_lanes)
+        turn_unit<__nv_bfloat16, W, kInterleaved>(q + h * t.q_head, unit, cs, s, turns, PutDense<__nv_bfloat16>{q_out + (int64_t)h * s.head_dim});
+    }
+  }
+  if (at < 0) return;
+  char* const row = t.layer_pool + at;
+  const int64_t head_bytes = (int64_t)c.page_size * c.head_dim * c.item, values = c.kv_heads * head_bytes;
+  using Out = std::conditional_t<kE4m3, uint8_t, __nv_bfloat16>;
+  const __nv_bfloat16 *k = t.k + i * t.k_token, *v = t.v + i * t.v_token;
+  for (int h = lane; h < c.kv_heads; h += s.head_lanes)
+    turn_unit<__nv_bfloat16, W, kInterleaved>(k + h * t.k_head, unit, cs, s, turns,
+                                              PutCache<kE4m3>{reinterpret_cast<Out*>(row + h * head_bytes), kE4m3 ? t.scales[h] : 1.0f});
+  // values are copied, in the units of the keys (a pair that would be turned by nothing)
+#pragma unroll
+  for (int j = 0; j < W; ++j) cs[j] = make_float2(1.0f, 0.0f);
+  for (int h = lane; h < c.kv_heads; h += s.head_lanes) {
+    const __nv_bfloat16* x = v + h * t.v_head;
+    const PutCache<kE4m3> put{reinterpret_cast<Out*>(row + values + h * head_bytes), kE4m3 ? t.scales[c.kv_heads + h] : 1.0f};
+    if constexpr (W == 1) {
+      for (int e = unit; e < s.head_dim; e += s.units) put.one(e, Vec<__nv_bfloat16>::one(x + e));
+    } else {
+      for (int e = unit; e < s.head_dim / W; e += s.units) {
+        float a[W];
+        Vec<__nv_bfloat16>::load(x + e * W, a);
+        put.wide(e * W, a);
+      }
+    }
+  }
+}
+
+// Threads by unit, lane of heads and token.  A thread takes four heads or more by the same cosines, unless that leaves the GPU with less than 512
+// threads on each SM: then the heads are spread.
+RotaryShape rotary_shape(int64_t tokens, int heads_q, int heads_k, int head_dim, int rotary_dim, bool interleaved, int wide) {
+  RotaryShape s = {};
+  s.heads_q = heads_q; s.heads_k = heads_k; s.head_dim = head_dim; s.rotary_dim = rotary_dim;
+  s.rotary_units = wide == 1 ? rotary_dim / 2 : interleaved ? rotary_dim / wide : rotary_dim / 2 / wide;
+  s.units = s.rotary_units + (head_dim - rotary_dim) / wide;
+  const int rest = kThreads / s.units, heads = heads_q > heads_k ? heads_q : heads_k;
+  const int64_t enough = (int64_t)device_sm_count() * 512;
+  int lanes = 1;
+  while (lanes * 2 <= rest && lanes < heads && (lanes * 8 <= heads || tokens * s.units * lanes < enough)) lanes *= 2;
+  s.head_lanes = lanes;
+  s.block_tokens = rest / lanes;
+  // the table of a block's cosines stays below the shared memory that every launch has
+  const int most = 40960 / (int)sizeof(float2) / (rotary_dim / 2 > 0 ? rotary_dim / 2 : 1);
+  if (s.block_tokens > most) s.block_tokens = most;
+  return s;
+}
+
+bool multiple(std::initializer_list<int64_t> v, int64_t n) {
+  for (const int64_t x : v) if (x % n != 0) return false;
+  return true;
+}
+
+template <typename T, int W>
+cudaError_t launch_rotary(bool interleaved, const RotaryTensors& t, const RotaryShape& s, cudaStream_t st) {
+  const int64_t blocks = ceil_div(t.tokens, s.block_tokens);
+  const size_t smem = (size_t)s.block_tokens * (s.rotary_dim / 2) * sizeof(float2);
+  return launch_overlapped(kLaunchShort, interleaved ? rotary_kernel<T, W, true> : rotary_kernel<T, W, false>, dim3((unsigned)blocks), dim3(kThreads), smem, st, t, s);
+}
+
+template <int W, bool kInterleaved>
+cudaError_t launch_append(bool e4m3, const AppendTensors& t, const RotaryShape& s, cudaStream_t st) {
+  const int64_t blocks = ceil_div(t.tokens, s.block_tokens);
+  const size_t smem = (size_t)s.block_tokens * (s.rotary_dim / 2) * sizeof(float2);
+  return launch_overlapped(kLaunchShort, e4m3 ? append_kernel<W, kInterleaved, true> : append_kernel<W, kInterleaved, false>, dim3((unsigned)blocks), dim3(kThreads), smem, st, t, s);
+}
+
+}  // namespace
+}  // namespace metis
+
+using namespace metis;
+
+extern "C" int32_t metis_rotary(const metis_rotary_args* a) {
+  if (!a || !a->q || !a->q_out || !a->turns || (a->heads_k > 0 && (!a->k || !a->k_out))) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
+  if (a->dtype != METIS_DTYPE_BF16 && a->dtype != METIS_DTYPE_F32) return fail(METIS_ERR_BAD_ARGUMENT, "dtype must be bf16 or fp32");
+  if (a->tokens <= 0 || a->inner <= 0 || a->heads_q <= 0 || a->heads_k < 0 || a->head_dim <= 0 || a->head_dim > 256 || a->head_dim % 8 != 0)
+    return fail(METIS_ERR_BAD_SHAPE, "tokens and heads must be positive and head_dim a multiple of 8 up to 256");
+  if (a->rotary_dim <= 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 2 != 0)
+    return fail(METIS_ERR_BAD_SHAPE, "rotary_dim must be even and at most head_dim");
+  const int item = a->dtype == METIS_DTYPE_BF16 ? 2 : 4, wide = 16 / item;
+  // 16 bytes at a time where the pairs, the tensors' rows and addresses allow it, element by element elsewhere
+  const bool vectors = (a->interleaved ? a->rotary_dim : a->rotary_dim / 2) % wide == 0 && multiple({a->q_outer, a->q_token, a->q_head}, wide) &&
+                       (a->heads_k == 0 || multiple({a->k_outer, a->k_token, a->k_head}, wide)) && aligned16(a->q) && aligned16(a->q_out) &&
+                       aligned16(a->k) && aligned16(a->k_out);
+  RotaryShape s = rotary_shape(a->tokens, a->heads_q, a->heads_k, a->head_dim, a->rotary_dim, a->interleaved != 0, vectors ? wide : 1);
+  s.magnitude = a->magnitude;
+  s.sign = a->inverse ? -1.0f : 1.0f;
+  if (ceil_div(a->tokens, s.block_tokens) >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
+  const RotaryTensors t = {a->positions, a->tokens, a->inner, a->turns, a->q, a->k, a->q_outer, a->q_token, a->q_head, a->k_outer, a->k_token, a->k_head,
+                           a->q_out, a->k_out, a->positions_64 != 0};
+  const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  const bool in = a->interleaved != 0;
+  if (item == 2) METIS_CUDA_OK((vectors ? launch_rotary<__nv_bfloat16, 8>(in, t, s, st) : launch_rotary<__nv_bfloat16, 1>(in, t, s, st)));
+  else           METIS_CUDA_OK((vectors ? launch_rotary<float, 4>(in, t, s, st) : launch_rotary<float, 1>(in, t, s, st)));
+  count_rollout_launches(1);
+  return METIS_OK;
+}
+
+extern "C" int32_t metis_cache_append(const metis_cache* cache, const metis_append_args* a) {
+  AppendTensors t = {};
+  if (const int32_t rc = check_cache(cache, &t.cache)) return rc;
+  const CacheView& c = t.cache;
+  if (!a || !a->k || !a->v || (a->heads_q > 0 && (!a->q || !a->q_out))) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
+  if (a->tokens <= 0 || a->heads_q < 0 || a->layer < 0 || a->layer >= c.layers) return fail(METIS_ERR_BAD_SHAPE, "tokens must be positive and the layer one of the cache");
+  if (a->turns && (a->rotary_dim <= 0 || a->rotary_dim > c.head_dim || a->rotary_dim % 2 != 0)) return fail(METIS_ERR_BAD_SHAPE, "rotary_dim must be even and at most head_dim");
+  if (!multiple({a->k_token, a->k_head, a->v_token, a->v_head}, 8) || (a->heads_q > 0 && !multiple({a->q_token, a->q_head}, 8)))
+    return fail(METIS_ERR_BAD_ALIGNMENT, "strides must be multiples of 8 elements");
+  if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q) || !aligned16(a->q_out)) return fail(METIS_ERR_BAD_ALIGNMENT, "tensors must be 16-byte aligned");
+  const int rotary = a->turns ? a->rotary_dim : 0;
+  const bool in = a->interleaved != 0 && rotary > 0, vectors = (in ? rotary : rotary / 2) % 8 == 0;
+  RotaryShape s = rotary_shape(a->tokens, a->heads_q, c.kv_heads, c.head_dim, rotary, in, vectors ? 8 : 1);
+  s.heads_q = a->heads_q;
+  s.magnitude = a->magnitude;
+  s.sign = 1.0f;
+  if (ceil_div(a->tokens, s.block_tokens) >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
+  const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;       // keys, or values, of one layer on a page
+  t.layer_pool = c.pool + a->layer * 2 * part;
+  t.scales = cache->scales ? cache->scales + (int64_t)a->layer * 2 * c.kv_heads : nullptr;
+  t.slots = a->slots; t.positions = a->positions; t.tokens = a->tokens; t.turns = a->turns;
+  t.q = static_cast<const __nv_bfloat16*>(a->q); t.k = static_cast<const __nv_bfloat16*>(a->k); t.v = static_cast<const __nv_bfloat16*>(a->v);
+  t.q_token = a->q_token; t.q_head = a->q_head; t.k_token = a->k_token; t.k_head = a->k_head; t.v_token = a->v_token; t.v_head = a->v_head;
+  t.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+  t.slots_64 = (a->index_64 & 1) != 0; t.positions_64 = (a->index_64 & 2) != 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  const bool e4m3 = c.item == 1;
+  if (vectors) METIS_CUDA_OK((in ? launch_append<8, true>(e4m3, t, s, st) : launch_append<8, false>(e4m3, t, s, st)));
+  else         METIS_CUDA_OK((in ? launch_append<1, true>(e4m3, t, s, st) : launch_append<1, false>(e4m3, t, s, st)));
+  count_rollout_launches(1);
+  return METIS_OK;
+}

@@ -23,7 +23,7 @@ LAUNCHES = {"quantize": 0, "rmsnorm_quantize": 0, "dequantize": 0, "col_mean": 0
 
 
 def launch_count() -> int:
-    return sum(LAUNCHES.values()) + cabi.dense_launches()          # (dense.py's are counted where they are made)
+    return sum(LAUNCHES.values()) + cabi.dense_launches() + cabi.rollout_launches()          # (dense.py's and rollout.py's are counted where they are made)
 
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:

@@ -52,6 +52,7 @@ extern "C" {
 /* element types of dense operands */
 #define METIS_DTYPE_BF16 0
 #define METIS_DTYPE_F32  1
+#define METIS_DTYPE_E4M3 2  /* pages of a key-value cache only */
 
 /* activations of metis_linear */
 #define METIS_ACT_NONE      0
@@ -561,6 +562,153 @@ int32_t metis_head_backward(const metis_head_args* args, const float* gout, int3
  * of the logit, which for a token of p near 1 may be all of it). */
 int32_t metis_head_backward_kept(const metis_head_args* args, const float* target_logp, const float* gout, int32_t gout_stride, const float* inv_count,
                                  void* dh, int64_t lddh, void* dw, int64_t lddw);
+
+/* ---- rollout: rotary positions, a paged key-value cache with attention over it, sampling --------------------------- */
+
+/* Kernels that the entry points below have launched in this process. */
+int64_t metis_rollout_launches(void);
+
+/*
+ * Rotary positions of x [tokens, heads, head_dim] for up to two tensors (queries and keys; k may be null) in one launch:
+ * of the first rotary_dim elements of a head the pair i, (i, rotary_dim/2 + i) or with `interleaved` (2i, 2i + 1), is turned by the
+ * angle 2 pi position turns[i] / 2^64 and multiplied by `magnitude`; the others are copied.  turns[i] is the pair's frequency as a
+ * fraction of a turn per position, in units of 2^-64: the product with a position is exact modulo a whole turn, so that an angle is as
+ * exact at position 2^31 as at 1.  inverse: by minus the angle (what a gradient takes).  Computed in fp32, rounded once.
+ * Token t of `tokens` is (t / inner, t % inner) under the two token strides; strides in elements, the last dimension dense.  positions:
+ * one for each token (int32, or int64 with positions_64), or null: t % inner.  Outputs are contiguous.  dtype bf16 or fp32.  What the
+ * reference leaves to the attention of its models (src/Metis/models/llama.py, or the Hugging Face model around its layers).
+ */
+typedef struct metis_rotary_args {
+  int64_t tokens, inner;
+  int32_t heads_q, heads_k, head_dim, rotary_dim;
+  int32_t interleaved, inverse, dtype, positions_64;
+  const uint64_t* turns;    /* [rotary_dim / 2] on the device */
+  float magnitude;
+  int32_t reserved;
+  const void* positions;
+  const void* q;  int64_t q_outer, q_token, q_head;
+  const void* k;  int64_t k_outer, k_token, k_head;
+  void* q_out;
+  void* k_out;
+  void* stream;
+} metis_rotary_args;
+int32_t metis_rotary(const metis_rotary_args* args);
+
+/*
+ * A key-value cache in pages.  pool [pages, layers, 2 (keys, values), kv_heads, page_size, head_dim] in bf16 or e4m3, 16-byte aligned;
+ * tables [sequences, width] int32, the pages of each sequence in order (-1 behind them); lengths [sequences] and refs [pages] int32 (how
+ * many tables hold a page: 0 is a free one); scales fp32 [layers, 2, kv_heads], what an e4m3 element is multiplied by (null with bf16).
+ * page_size is a multiple of 16, head_dim of 8 up to 256.  Everything is on the device, so that a decode step with its bookkeeping can
+ * be captured.  status (int32, required): a call that cannot be done leaves everything as it is and puts its METIS_CACHE_* code there, unless there
+ * is one already.  Indices on the device are checked there: a page number outside the pool is read as an absent one.
+ */
+#define METIS_CACHE_NO_PAGES  16  /* not enough free pages */
+#define METIS_CACHE_BAD_SLOT  17  /* a sequence that the cache does not have */
+#define METIS_CACHE_TOO_LONG  18  /* longer than `width` pages, or a negative count */
+#define METIS_CACHE_TWICE     19  /* the same sequence twice in one call */
+#define METIS_CACHE_NOT_EMPTY 20  /* a fork's destination that has a length */
+typedef struct metis_cache {
+  void* pool;
+  int64_t pages;
+  int32_t layers, kv_heads, page_size, head_dim, dtype, reserved;
+  int32_t* tables;
+  int64_t sequences, width;
+  int32_t* lengths;
+  int32_t* refs;
+  const float* scales;
+  int32_t* status;
+} metis_cache;
+/* Whether the calls below take this cache: its sizes and pointers, nothing on the device. */
+int32_t metis_cache_check(const metis_cache* cache);
+
+/*
+ * Rotary positions of q and k (turns null: none) and k and v written into the pages, in one launch.  Token i belongs to sequence slots[i]
+ * (null: i) at positions[i] (null: its last one, lengths - 1).  A token whose sequence or position the cache does not have is not written, and its
+ * q_out is zeros where it is the sequence that is missing.  q [tokens, heads_q, head_dim] may be null; strides in elements, multiples of 8; bf16.
+ * e4m3: round to nearest of x / scale, saturating.  Two tokens of one call for the same place: one of them is there afterwards.
+ */
+typedef struct metis_append_args {
+  int64_t tokens;
+  int32_t layer, heads_q, rotary_dim, interleaved;
+  const uint64_t* turns;
+  float magnitude;
+  int32_t index_64;         /* bit 0: slots are int64, bit 1: positions */
+  const void* slots;
+  const void* positions;
+  const void* q;  int64_t q_token, q_head;
+  const void* k;  int64_t k_token, k_head;
+  const void* v;  int64_t v_token, v_head;
+  void* q_out;              /* [tokens, heads_q, head_dim] */
+  void* stream;
+} metis_append_args;
+int32_t metis_cache_append(const metis_cache* cache, const metis_append_args* args);
+
+/*
+ * Attention of one new token for each row: out[i] = softmax(scale q[i] K^T) V over the lengths[s] keys of sequence s = slots[i] (null: i),
+ * head h of heads_q on key-value head h / (heads_q / kv_heads).  q and out bf16 [rows, heads_q, head_dim] (q with strides in elements, multiples
+ * of 2; out contiguous), lse (may be null) fp32 [rows, heads_q]: log of the sum of exp(scale q k).  No keys, or a sequence that the cache does not
+ * have: zeros and -inf.  Work is split over all keys of all rows in equal parts whatever the lengths, parts of one row are joined in a second launch.
+ */
+typedef struct metis_attend_args {
+  int64_t rows;
+  int32_t layer, heads_q;
+  const void* slots;
+  int32_t slots_64;
+  float scale;
+  const void* q;  int64_t q_row, q_head;
+  void* out;
+  float* lse;
+  void* workspace;  int64_t workspace_bytes;
+  void* stream;
+} metis_attend_args;
+int64_t metis_cache_attend_workspace_bytes(const metis_cache* cache, int64_t rows, int32_t heads_q);
+int32_t metis_cache_attend(const metis_cache* cache, const metis_attend_args* args);
+
+/*
+ * Bookkeeping.  Free pages are taken lowest first, in the order of the call's sequences, so that results do not depend on the schedule.
+ * Indices are int32 or (index_64) int64 on the device; a negative sequence stands for none.
+ *   reserve  lengthens sequence slots[i] by counts[i] (counts null: by count), with pages of their own for what does not fit the last one
+ *   fork     makes sequence dst[i] (an empty one) the same as src[i] was before the call: with `share` whole pages are held by both, and what the last
+ *            page is filled with is copied; without, every page is copied
+ *   free     empties sequences; a page that no table holds any more is free.  A sequence given twice is emptied once.
+ *   compact  moves the pages that are held to the front of the pool: page k of those at or above their number n goes to the k-th free one
+ *            below it.  *live = n.
+ */
+int64_t metis_cache_workspace_bytes(const metis_cache* cache, int64_t n);
+int32_t metis_cache_reserve(const metis_cache* cache, const void* slots, const void* counts, int64_t count, int32_t index_64, int64_t n,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+int32_t metis_cache_fork(const metis_cache* cache, const void* src, const void* dst, int32_t index_64, int64_t n, int32_t share,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+int32_t metis_cache_free(const metis_cache* cache, const void* slots, int32_t index_64, int64_t n, void* stream);
+int32_t metis_cache_compact(const metis_cache* cache, int32_t* live, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One token for each row of logits [rows, vocab] (bf16 or fp32, row stride ld), by the row's random number u in [0, 1).  With
+ * w = exp((x - max x) (1 / temperature)) in fp32 and the tokens ordered by logit, the largest first, equal ones by index: the first top_k
+ * (0: all); of them the shortest front whose weights are at least top_p of theirs; of them those with w >= min_p; always the first.  The token is
+ * the first one, by index, up to which the weights of the kept ones exceed u times their total.  Sums of weights in 64 bits.  temperature 0: the
+ * first of the order.  -inf and NaN are never taken; a row that has nothing else gives -1, and so does one whose u or parameters are
+ * outside their ranges.  logprob (may be null) fp32: log softmax(x / temperature) of the token over the whole row (temperature 0: of x), NaN beside -1.
+ * The *_rows pointers (may be null) hold one value for each row in place of the scalar: fp32, top_k int32.
+ */
+typedef struct metis_sample_args {
+  int64_t rows, vocab;
+  const void* logits;  int64_t ld;
+  int32_t dtype, u_64;      /* u_64: u is fp64, else fp32 */
+  const void* u;
+  double top_p;
+  float temperature, min_p;
+  int32_t top_k, reserved;
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int32_t* top_k_rows;
+  int64_t* token;
+  float* logprob;
+  void* stream;
+} metis_sample_args;
+#define METIS_SAMPLE_MAX_VOCAB 393216
+int32_t metis_sample(const metis_sample_args* args);
 
 #ifdef __cplusplus
 }
