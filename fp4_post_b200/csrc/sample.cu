@@ -4,14 +4,17 @@
 //   top-k keeps the first k of the order; top-p the shortest front of those whose weights are at least p of theirs; min-p those with w >= min_p.
 //   Each keeps a front of the order, so that what is kept is "x above a cut, and the first n of those that equal it".
 //
-// A cluster of up to eight blocks takes a row: it is read once from memory, 16 bytes at a time, and stays in shared memory in fp32 for all passes.  Nothing is
-// sorted: a cut is found by histograms of 2048 bins, first of (max - x) / T in steps of 1/64, then of the bits of the logits in the bin where
-// the cut lies until one value is left (one more level for bf16, two or three for fp32).
+// A cluster of up to eight blocks takes a row: it is read once from memory, 16 bytes at a time, and stays in shared memory (bf16 as 16-bit keys in the order of the
+// values, fp32 as it is) for all passes.  Nothing is sorted; a cut is found by histograms:
+//   bf16  The bins are the values themselves, from the largest one on: 4095 of them, those below 2^-8 in magnitude together in one.  That is every logit
+//         within +-256.  A pass counts, five instructions and an addition in shared memory an element; a bin's weight is its count times the
+//         weight of its value, so that one histogram serves top-k, top-p and the sum of all.  (A cut in the bin of small values or behind the last one goes the other way.)
+//   fp32  2048 bins, first of (max - x) / T in steps of 1/64, then of the bits of the logits in the bin where the cut lies until one value is left.
 //
 // Whether a token is in or out goes by sums over up to all the vocabulary, and an fp32 sum would move borders with the order of its terms.  Here the
-// sums have 64 bits: a bin's weights lie within a factor of 2^(1/44), all 24 bits of each are multiples of one unit, and the bin adds them as
-// whole numbers (two of at most 14 bits: 20000 of those fit 32 bits), exactly and in any order; bins, threads and blocks are added as doubles in
-// a fixed order.  So a token does not depend on the schedule, and two programs that take the same weights find the same one.
+// sums have 64 bits: counts times weights; or, of fp32, a bin's weights lie within a factor of 2^(1/44), all 24 bits of each are multiples of one unit, and the
+// bin adds them as whole numbers (two of at most 14 bits: 49664 of those fit 32 bits), exactly and in any order; bins, threads and blocks are
+// added as doubles in a fixed order.  So a token does not depend on the schedule, and two programs that take the same weights find the same one.
 #include "rollout.cuh"
 
 #include <cooperative_groups.h>
@@ -23,7 +26,8 @@ namespace metis {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;                        // of a histogram of weights: two words each
+constexpr int kValues = 2 * kBins;                 // of a histogram of counts: one
 constexpr int kMaxCluster = 8;
 constexpr float kStep = 64.0f;                     // bins for a factor of e
 constexpr int kLowBits = 13;
@@ -31,8 +35,7 @@ constexpr int kLowBits = 13;
 struct SampleParams {
   const void* logits;
   int64_t ld;
-  int32_t vocab, each;                             // each: elements of a thread, odd (their reads then meet no bank twice)
-  int32_t dtype;
+  int32_t vocab, each;                             // each: elements of a thread, an odd number of words (their reads then meet no bank twice)
   bool u_64;
   const void* u;
   double top_p;
@@ -45,59 +48,124 @@ struct SampleParams {
 };
 
 struct Found { double above, inside; int32_t bin; };      // weight before the bin where the target is met, and in it
+struct Cut { float at; bool found; double ties; };        // kept are those above `at` and the first `ties` that equal it
 
 struct Shared {
   double sums[kThreads / 32];
   int64_t counts[kThreads / 32];
-  double gathered[2][kMaxCluster];
+  double gathered[2][kMaxCluster][2];
   Found found;
+  Cut cut[2];                                      // of top-k, of top-p
+  double share;                                    // weight of what top-k keeps
   uint32_t low, high;                              // keys in the bin, of this block
-  float maxima[kThreads / 32];
-  uint32_t* lows;                                  // the two histograms, [kBins] each
-  uint32_t* highs;
+  uint32_t maxima[kThreads / 32];
+  uint32_t bins[2 * kBins];
 };
 
 // The same order as the numbers', as whole numbers; bf16 in 16 bits.
-__device__ __forceinline__ uint32_t key_of(float x, int drop) {
+template <int kDrop> __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x);
-  return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> drop;
+  return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> kDrop;
 }
-__device__ __forceinline__ float value_of(uint32_t key, int drop) {
-  const bool positive = (key << drop) >> 31;
-  const uint32_t b = (key << drop) | (!positive && drop ? (1u << drop) - 1u : 0u);
-  return __uint_as_float(positive ? b & 0x7fffffffu : ~b);
+template <int kDrop> __device__ __forceinline__ float value_of(uint32_t key) {
+  const uint32_t k = key << kDrop;
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~(k | ((1u << kDrop) - 1u)));
 }
 
+// Elements in shared memory: fp32, or the 16-bit keys of bf16.
+template <typename T> struct Store;
+template <> struct Store<float> {
+  static constexpr int kDrop = 0, kWord = 1;        // elements of a 32-bit word
+  using Element = float;
+  static __device__ __forceinline__ float at(const float* x, int i) { return x[i]; }
+  template <typename F> static __device__ __forceinline__ void word(const float* x, int w, const F& f) { f(w, x[w]); }
+  static __device__ __forceinline__ float clean(float v) { return v == v ? v + 0.0f : -CUDART_INF_F; }
+};
+template <> struct Store<__nv_bfloat16> {
+  static constexpr int kDrop = 16, kWord = 2;
+  using Element = uint16_t;
+  static __device__ __forceinline__ float at(const uint16_t* x, int i) { return value_of<16>(x[i]); }
+  // two bf16 -> two keys: NaN as -inf (the maximum with it), -0 as 0, then negative ones with all bits turned and the others with the sign
+  static __device__ __forceinline__ uint32_t keys(uint32_t two) {
+    const uint32_t lowest = 0xff80ff80u, none = 0u;
+    __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&lowest));
+    v = __hadd2_rn(v, *reinterpret_cast<const __nv_bfloat162*>(&none));
+    const uint32_t w = *reinterpret_cast<uint32_t*>(&v), s = w & 0x80008000u;
+    return w ^ ((s - (s >> 15)) | 0x80008000u);
+  }
+};
+constexpr uint32_t kLowest16 = 0x007fu;            // the key of -inf
+constexpr int kAbove = 0xbb80, kBelow = 0x447f;    // the keys of 2^-8 and -2^-8
+
 // The cluster's blocks on one row.
+template <typename T>
 struct Row {
+  using S = Store<T>;
+  using E = typename S::Element;
   cg::cluster_group cluster;
   Shared& sh;
-  const float* x;                                  // this block's logits; -inf behind the last
+  const E* x;                                      // this block's logits; -inf behind the last
   int blocks, rank, held;                          // held: elements of x
   float top, inverse;                              // the largest logit, 1/T
-  int drop;
   int turn = 0;
 
   __device__ float weight(float v) const { return v == top ? 1.0f : expf(__fmul_rn(__fsub_rn(v, top), inverse)); }
 
-  // One value of each block to all; two buffers in turn, so that one barrier does for both writing and reading.
-  __device__ const double* gather(double v) {
+  // f(x) of each of the block's elements, 16 bytes at a time
+  template <typename F> __device__ __forceinline__ void each(const F& f) const {
+    constexpr int kWide = 16 / (int)sizeof(E);
+    for (int i = threadIdx.x; i < held / kWide; i += kThreads) {
+      const uint4 w = reinterpret_cast<const uint4*>(x)[i];
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(E) == 4) f(__uint_as_float(v[j]));
+        else { f(value_of<16>(v[j] & 0xffffu)); f(value_of<16>(v[j] >> 16)); }
+      }
+    }
+  }
+  template <typename F> __device__ __forceinline__ void each_key(const F& f) const {
+    for (int i = threadIdx.x; i < held / 8; i += kThreads) {
+      const uint4 w = reinterpret_cast<const uint4*>(x)[i];
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { f(v[j] & 0xffffu); f(v[j] >> 16); }
+    }
+  }
+
+  // Two values of each block to all; two buffers in turn, so that one barrier does for both writing and reading.
+  __device__ const double (*gather(double a, double b = 0.0))[2] {
     turn ^= 1;
-    if (threadIdx.x < (unsigned)blocks) cluster.map_shared_rank(&sh, threadIdx.x)->gathered[turn][rank] = v;
+    if (threadIdx.x < (unsigned)blocks) {
+      double* to = cluster.map_shared_rank(&sh, threadIdx.x)->gathered[turn][rank];
+      to[0] = a;
+      to[1] = b;
+    }
     cluster.sync();
     return sh.gathered[turn];
   }
   // What the blocks before this one have, and all.
   __device__ double ahead(double v, double& all) {
-    const double* g = gather(v);
+    const double (*g)[2] = gather(v);
     double before = 0.0;
     all = 0.0;
     for (int r = 0; r < blocks; ++r) {
       if (r == rank) before = all;
-      all += g[r];
+      all += g[r][0];
     }
     return before;
   }
+  __device__ double sum_of(double mine) {
+    double all;
+    ahead(block_scan<kThreads>(mine, sh.sums).all, all);
+    return all;
+  }
+  __device__ void clear() {
+    for (int i = threadIdx.x; i < 2 * kBins; i += kThreads) sh.bins[i] = 0u;
+    __syncthreads();
+  }
+
+  // ---- histograms of weights (fp32; bf16 where the values' bins do not have the cut) ----
 
   __device__ int bin_of(float v) const {
     const float d = __fmul_rn(__fmul_rn(__fsub_rn(top, v), inverse), kStep);
@@ -108,34 +176,32 @@ struct Row {
   __device__ static int unit_of(int bin) { return bin == kBins - 1 ? -72 : (int)floorf(-(float)(bin + 1) * (1.44269504f / kStep)) - 2 - 24; }
   __device__ static uint32_t whole(float w, int unit) { return (uint32_t)(w * __uint_as_float((uint32_t)(127 - unit) << 23)); }
 
-  __device__ void clear() {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.lows[i] = sh.highs[i] = 0u;
-    __syncthreads();
-  }
   template <bool kMass> __device__ void add(int bin, float v, int unit) {
     if constexpr (kMass) {
       const uint32_t m = whole(weight(v), unit);
-      atomicAdd(&sh.lows[bin], m & ((1u << kLowBits) - 1u));
-      atomicAdd(&sh.highs[bin], m >> kLowBits);
+      atomicAdd(&sh.bins[bin], m & ((1u << kLowBits) - 1u));
+      atomicAdd(&sh.bins[kBins + bin], m >> kLowBits);
     } else {
-      atomicAdd(&sh.lows[bin], 1u);
+      atomicAdd(&sh.bins[bin], 1u);
     }
   }
-  // Where the bins' sums, in order, reach the target; false if they do not.  units: the bins' unit, or their own where it is 1.
+  // Where the bins' sums, in order, reach the target; false if they do not.  unit: the bins', or their own where it is 1.
   template <bool kMass> __device__ bool reach(double target, int unit, Found& out) {
-    __syncthreads();
     cluster.sync();
+    constexpr int kMost = kBins / kThreads;
     const int slice = kBins / blocks, mine = slice > kThreads ? slice / kThreads : 1;
-    double v[kBins / kThreads], sum = 0.0;
-    for (int i = 0; i < mine; ++i) {
+    double v[kMost], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
       const int local = threadIdx.x * mine + i;
       v[i] = 0.0;
-      if (local >= slice) continue;
+      if (i >= mine || local >= slice) continue;
       const int bin = rank * slice + local;
       uint64_t low = 0, high = 0;
       for (int r = 0; r < blocks; ++r) {
-        low += cluster.map_shared_rank(sh.lows, r)[bin];
-        if (kMass) high += cluster.map_shared_rank(sh.highs, r)[bin];
+        const Shared* peer = cluster.map_shared_rank(&sh, r);
+        low += peer->bins[bin];
+        if (kMass) high += peer->bins[kBins + bin];
       }
       const uint64_t m = low + (high << kLowBits);
       if (m) v[i] = kMass ? ldexp((double)m, unit == 1 ? unit_of(bin) : unit) : (double)m;
@@ -147,17 +213,15 @@ struct Row {
     if (all < target) return false;                // the same for all blocks
     const double before = base + s.before, upto = base + s.upto;
     if (before < target && target <= upto) {
-      double above = before;
-      int hit = -1;
-      for (int i = 0; i < mine; ++i) {
-        if (v[i] == 0.0) continue;
-        if (hit >= 0) {
-          above += v[hit];
-        }
-        hit = i;
-        if (target <= above + v[i]) break;
+      Found f = {before, 0.0, 0};
+      double next = before;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i) {
+        // (the last one that has anything, where rounding keeps the sum below the target)
+        if (v[i] == 0.0 || (f.inside > 0.0 && target <= next)) continue;
+        f = {next, v[i], rank * slice + (int)threadIdx.x * mine + i};
+        next += v[i];
       }
-      const Found f = {above, v[hit], rank * slice + (int)threadIdx.x * mine + hit};
       for (int r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->found = f;
     }
     cluster.sync();
@@ -167,44 +231,45 @@ struct Row {
 
   // The cut of the elements above `floor`: `at` such that the weights (or the number) of those above it are below the target and with those that equal
   // it are not; what is above, and how many equal it.  False if all of them do not reach the target.
-  template <bool kMass> __device__ bool cut(double target, float floor, float& at, double& above, double& ties) {
+  template <bool kMass> __device__ __noinline__ bool cut(double target, float floor, float& at, double& above, double& ties) {
     clear();
-    for (int i = threadIdx.x; i < held; i += kThreads)
-      if (x[i] > floor) {
-        const int bin = bin_of(x[i]);
-        add<kMass>(bin, x[i], kMass ? unit_of(bin) : 0);
+    each([&](float v) {
+      if (v > floor) {
+        const int bin = bin_of(v);
+        add<kMass>(bin, v, kMass ? unit_of(bin) : 0);
       }
+    });
+    if (threadIdx.x == 0) { sh.low = 0xffffffffu; sh.high = 0u; }
     Found f;
     if (!reach<kMass>(target, 1, f)) return false;
     above = f.above;
     const int bin = f.bin, unit = unit_of(bin);
     // the bin's smallest and largest keys
-    if (threadIdx.x == 0) { sh.low = 0xffffffffu; sh.high = 0u; }
-    __syncthreads();
     uint32_t low = 0xffffffffu, high = 0u;
-    for (int i = threadIdx.x; i < held; i += kThreads)
-      if (x[i] > floor && bin_of(x[i]) == bin) {
-        const uint32_t k = key_of(x[i], drop);
+    each([&](float v) {
+      if (v > floor && bin_of(v) == bin) {
+        const uint32_t k = key_of<S::kDrop>(v);
         low = min(low, k);
         high = max(high, k);
       }
+    });
     low = __reduce_min_sync(0xffffffffu, low);
     high = __reduce_max_sync(0xffffffffu, high);
     if ((threadIdx.x & 31) == 0) { atomicMin(&sh.low, low); atomicMax(&sh.high, high); }
     __syncthreads();
-    const double* g = gather((double)sh.low);
-    for (int r = 0; r < blocks; ++r) low = min(low, (uint32_t)g[r]);
-    g = gather((double)sh.high);
-    for (int r = 0; r < blocks; ++r) high = max(high, (uint32_t)g[r]);
+    const double (*g)[2] = gather((double)sh.low, (double)sh.high);
+    for (int r = 0; r < blocks; ++r) {
+      low = min(low, (uint32_t)g[r][0]);
+      high = max(high, (uint32_t)g[r][1]);
+    }
     while (true) {
       const uint32_t span = high - low;
       const int shift = max(0, 21 - __clz(span));          // (span >> shift) < 2048
       clear();
-      for (int i = threadIdx.x; i < held; i += kThreads)
-        if (x[i] > floor && bin_of(x[i]) == bin) {
-          const uint32_t k = key_of(x[i], drop);
-          if (k >= low && k <= high) add<kMass>((int)((high - k) >> shift), x[i], unit);
-        }
+      each([&](float v) {
+        const uint32_t k = key_of<S::kDrop>(v);
+        if (k >= low && k <= high && v > floor && bin_of(v) == bin) add<kMass>((int)((high - k) >> shift), v, unit);
+      });
       // (a target that rounding puts in front of the bin's first element, or behind its last, is met by that one)
       Found next;
       if (!reach<kMass>(fmax(fmin(target - above, f.inside), 1e-300), unit, next)) return false;
@@ -214,66 +279,228 @@ struct Row {
       if (shift == 0) break;
       low = max(low, high - ((1u << shift) - 1u));
     }
-    at = value_of(high, drop);
+    at = value_of<S::kDrop>(high);
     ties = kMass ? rint(f.inside / ldexp((double)whole(weight(at), unit), unit)) : f.inside;
+    return true;
+  }
+
+  // of those that equal the cut, as many as have less than the target in front of them
+  __device__ double ties_below(double target, double before, float at, double limit) const {
+    const double w = (double)weight(at);
+    double n = w > 0.0 ? fmax(1.0, ceil((target - before) / w)) : limit;
+    while (n < limit && before + n * w < target) n += 1.0;
+    while (n > 1.0 && before + (n - 1.0) * w >= target) n -= 1.0;
+    return fmin(n, limit);
+  }
+
+  // Top-k and top-p by these histograms.  all_weights: of the whole row.
+  __device__ __noinline__ Cut by_weights(int64_t k, int64_t vocab, double top_p, double all_weights) {
+    Cut c = {-CUDART_INF_F, false, 0.0};
+    double above = 0.0;
+    if (k > 0 && k < vocab) {
+      float at;
+      double equal;
+      if (cut<false>((double)k, -CUDART_INF_F, at, above, equal)) c = {at, true, (double)k - above};       // (else there are not so many)
+    }
+    if (top_p < 1.0) {
+      double total = all_weights, over = 0.0;
+      if (c.found) {
+        double sum = 0.0;
+        each([&](float v) { if (v > c.at) sum += (double)weight(v); });
+        over = sum_of(sum);
+        total = over + c.ties * (double)weight(c.at);
+      }
+      const double target = fmax(top_p * total, 1e-300);                  // (the first one is always kept)
+      float at;
+      double before, equal;
+      if (cut<true>(target, c.at, at, before, equal)) c = {at, true, ties_below(target, before, at, equal)};
+      else if (c.found) c.ties = ties_below(target, over, c.at, c.ties);  // all that are above the cut of top-k, and some that equal it
+    }
+    return c;
+  }
+
+  // ---- the histogram of values (bf16) ----
+
+  // Bins in the order of the values: bin 0 is the largest one's.  With d its distance to that one in keys, small = the bin of all that are below 2^-8 in magnitude
+  // (if the largest is not below those) and gap = how many keys that bin swallows:
+  //   keys above: d;   in it: small;   below: d - gap
+  struct Values { int top, small, gap; bool has_small; };
+  __device__ static Values values(int top) {
+    if (top >= kAbove) return {top, top - kAbove + 1, kAbove - kBelow - 2, true};
+    if (top > kBelow) return {top, 0, top - kBelow - 1, true};
+    return {top, 0, 0, false};
+  }
+
+  // The same cut from counts; false where it lies in a bin of several values.  all_weights: of the row.
+  __device__ bool by_values(int64_t k, double top_p, Cut& c, double& all_weights) {
+    const Values b = values((int)key_of<16>(top));
+    clear();
+    double extra = 0.0;                            // weights in the bins of several values: the small ones', and behind them the last one's
+    double extra_small = 0.0;
+    each_key([&](uint32_t key) {
+      const int d = b.top - (int)key;
+      const int bin = min(max(min(d, b.small), d - b.gap), kValues - 1);
+      if (key == kLowest16) return;
+      atomicAdd(&sh.bins[bin], 1u);
+      if (bin == kValues - 1) extra += (double)weight(value_of<16>(key));
+      else if (b.has_small && bin == b.small) extra_small += (double)weight(value_of<16>(key));
+    });
+    // (sums of nothing, mostly)
+    double rest = 0.0, small = 0.0;
+    if (__syncthreads_or(extra != 0.0 || extra_small != 0.0)) {
+      rest = block_scan<kThreads>(extra, sh.sums).all;
+      small = block_scan<kThreads>(extra_small, sh.sums).all;
+    }
+    {
+      const double (*g)[2] = gather(rest, small);  // (and the counts are there)
+      rest = small = 0.0;
+      for (int r = 0; r < blocks; ++r) { rest += g[r][0]; small += g[r][1]; }
+    }
+    // a thread has neighbouring bins: counts and weights, and what is before them
+    constexpr int kMost = kValues / kThreads;
+    const int slice = kValues / blocks, mine = slice / kThreads > 0 ? slice / kThreads : 1;
+    const bool active = (int)threadIdx.x * mine < slice;
+    const int first = rank * slice + (int)threadIdx.x * mine;
+    uint32_t n[kMost];
+    double count = 0.0, mass = 0.0;
+    auto several = [&](int bin) { return bin == kValues - 1 || (b.has_small && bin == b.small); };
+    auto value = [&](int bin) { return value_of<16>((uint32_t)(b.top - bin - (bin > b.small ? b.gap : 0))); };
+    auto bin_mass = [&](int bin, uint32_t m) { return m == 0 ? 0.0 : bin == kValues - 1 ? rest : several(bin) ? small : (double)m * (double)weight(value(bin)); };
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      n[i] = 0;
+      if (i >= mine || !active) continue;
+      for (int r = 0; r < blocks; ++r) n[i] += cluster.map_shared_rank(&sh, r)->bins[first + i];
+    }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      if (n[i] == 0) continue;
+      count += (double)n[i];
+      mass += bin_mass(first + i, n[i]);
+    }
+    const Scan<double> sc = block_scan<kThreads>(count, sh.sums), sm = block_scan<kThreads>(mass, sh.sums);
+    const double (*g)[2] = gather(sc.all, sm.all);
+    double before_count = 0.0, before_mass = 0.0, all_count = 0.0;
+    all_weights = 0.0;
+    for (int r = 0; r < blocks; ++r) {
+      if (r == rank) { before_count = all_count; before_mass = all_weights; }
+      all_count += g[r][0];
+      all_weights += g[r][1];
+    }
+    const double upto_count = before_count + sc.upto, upto_mass = before_mass + sm.upto;
+    before_count += sc.before;
+    before_mass += sm.before;
+    // (ties of -1: the cut lies in a bin of several values)
+    c = {-CUDART_INF_F, false, 0.0};
+    double total = all_weights;
+    if (k > 0 && (double)k < all_count) {
+      const double want = (double)k;
+      if (before_count < want && want <= upto_count) {
+        Cut found = {0.0f, true, -1.0};
+        double ahead_n = before_count, ahead_m = before_mass, share = 0.0;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+          if (n[i] == 0) continue;
+          if (ahead_n < want && want <= ahead_n + (double)n[i] && !several(first + i)) {
+            found = {value(first + i), true, want - ahead_n};
+            share = ahead_m + found.ties * (double)weight(found.at);
+          }
+          ahead_n += (double)n[i];
+          ahead_m += bin_mass(first + i, n[i]);
+        }
+        for (int r = 0; r < blocks; ++r) {
+          Shared* peer = cluster.map_shared_rank(&sh, r);
+          peer->cut[0] = found;
+          peer->share = share;
+        }
+      }
+      cluster.sync();
+      c = sh.cut[0];
+      if (c.ties < 0.0) return false;
+      total = sh.share;
+    }
+    if (top_p < 1.0) {
+      const double target = fmax(top_p * total, 1e-300);                  // (the first one is always kept)
+      if (before_mass < target && target <= upto_mass) {
+        Cut found = {0.0f, true, -1.0};
+        double ahead_m = before_mass;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) {
+          // (the last one that has anything, where rounding keeps the sum below the target)
+          if (n[i] == 0 || !open) continue;
+          const double m = bin_mass(first + i, n[i]);
+          if (m == 0.0) continue;
+          found = {value(first + i), true, several(first + i) ? -1.0 : ties_below(target, ahead_m, value(first + i), (double)n[i])};
+          open = ahead_m + m < target;
+          ahead_m += m;
+        }
+        if (c.found && found.ties >= 0.0 && (found.at < c.at || (found.at == c.at && found.ties > c.ties))) found = c;
+        for (int r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->cut[1] = found;
+      }
+      cluster.sync();
+      c = sh.cut[1];
+      if (c.ties < 0.0) return false;
+    }
     return true;
   }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
-  extern __shared__ __align__(16) float dynamic[];
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+  using S = Store<T>;
+  using E = typename S::Element;
+  extern __shared__ __align__(16) char dynamic[];
   __shared__ Shared sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t row = blockIdx.x / blocks;
   const int held = p.each * kThreads, first = rank * held, here = max(0, min(held, p.vocab - first));
-  float* x = dynamic + 2 * kBins;
-  if (threadIdx.x == 0) {
-    sh.lows = reinterpret_cast<uint32_t*>(dynamic);
-    sh.highs = reinterpret_cast<uint32_t*>(dynamic) + kBins;
-  }
+  E* x = reinterpret_cast<E*>(dynamic);
   cluster.barrier_arrive();                        // (a block is written to by the others once all have begun)
   grid_dependency_wait();
 
   // ---- the row; NaN and what is behind it as -inf, -0 as 0 ----
-  float top = -CUDART_INF_F;
   const T* from = static_cast<const T*>(p.logits) + row * p.ld + first;
-  auto take = [&](float v) {
-    v = v == v ? v + 0.0f : -CUDART_INF_F;
-    top = fmaxf(top, v);
-    return v;
-  };
-  constexpr int kWide = 16 / sizeof(T);
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
-    done = here / kWide * kWide;
+  constexpr int kWide = 16 / (int)sizeof(T);
+  const int wide = (reinterpret_cast<uintptr_t>(from) & 15) == 0 ? here / kWide : 0;
+  uint32_t best = 0;                               // the largest key
 #pragma unroll 4
-    for (int i = threadIdx.x * kWide; i < done; i += kThreads * kWide) {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(from + i));
-      float4* to = reinterpret_cast<float4*>(x + i);
-      if constexpr (sizeof(T) == 2) {
-        to[0] = make_float4(take(bf16_lo(w.x)), take(bf16_hi(w.x)), take(bf16_lo(w.y)), take(bf16_hi(w.y)));
-        to[1] = make_float4(take(bf16_lo(w.z)), take(bf16_hi(w.z)), take(bf16_lo(w.w)), take(bf16_hi(w.w)));
-      } else {
-        to[0] = make_float4(take(__uint_as_float(w.x)), take(__uint_as_float(w.y)), take(__uint_as_float(w.z)), take(__uint_as_float(w.w)));
-      }
+  for (int i = threadIdx.x; i < wide; i += kThreads) {
+    uint4 w = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+    if constexpr (sizeof(T) == 2) {
+      w = make_uint4(S::keys(w.x), S::keys(w.y), S::keys(w.z), S::keys(w.w));
+      best = __vmaxu2(best, __vmaxu2(__vmaxu2(w.x, w.y), __vmaxu2(w.z, w.w)));
+    } else {
+      const float4 v = make_float4(S::clean(__uint_as_float(w.x)), S::clean(__uint_as_float(w.y)), S::clean(__uint_as_float(w.z)), S::clean(__uint_as_float(w.w)));
+      w = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+      best = max(best, key_of<0>(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
+    }
+    reinterpret_cast<uint4*>(x)[i] = w;
+  }
+  if constexpr (sizeof(T) == 2) best = max(best & 0xffffu, best >> 16);
+  for (int i = wide * kWide + threadIdx.x; i < held; i += kThreads) {
+    if constexpr (sizeof(T) == 2) {
+      x[i] = (E)(i < here ? S::keys(reinterpret_cast<const uint16_t*>(from)[i]) & 0xffffu : kLowest16);
+      best = max(best, (uint32_t)x[i]);
+    } else {
+      x[i] = i < here ? S::clean(from[i]) : -CUDART_INF_F;
+      best = max(best, key_of<0>(x[i]));
     }
   }
-  for (int i = done + threadIdx.x; i < held; i += kThreads) x[i] = i < here ? take((float)from[i]) : -CUDART_INF_F;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) sh.maxima[threadIdx.x >> 5] = top;
+  best = __reduce_max_sync(0xffffffffu, best);
+  if ((threadIdx.x & 31) == 0) sh.maxima[threadIdx.x >> 5] = best;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, sh.maxima[w]);
+  for (int w = 0; w < kThreads / 32; ++w) best = max(best, sh.maxima[w]);
 
   cluster.barrier_wait();
-  Row r{cluster, sh, x, blocks, rank, held, 0.0f, 0.0f, sizeof(T) == 2 ? 16 : 0};
+  Row<T> r{cluster, sh, x, blocks, rank, held, 0.0f, 0.0f};
   {
-    const double* g = r.gather((double)top);
-    for (int i = 0; i < blocks; ++i) top = fmaxf(top, (float)g[i]);
+    const double (*g)[2] = r.gather((double)best);
+    for (int i = 0; i < blocks; ++i) best = max(best, (uint32_t)g[i][0]);
   }
+  const float top = value_of<S::kDrop>(best);
   const float t = p.temperature_rows ? p.temperature_rows[row] : p.temperature, min_p = p.min_p_rows ? p.min_p_rows[row] : p.min_p;
   const double top_p = p.top_p_rows ? (double)p.top_p_rows[row] : p.top_p;
   int64_t k = p.top_k_rows ? p.top_k_rows[row] : p.top_k;
@@ -293,104 +520,80 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   r.top = top;
   r.inverse = __fdiv_rn(1.0f, heat);
 
-  // ---- all weights, for the log-probability and where nothing but a share of all is asked for ----
-  const int mine = threadIdx.x * p.each;
+  // ---- the cut, and the weight of all ----
+  Cut cut = {-CUDART_INF_F, false, 0.0};
   double all_weights = 0.0;
-  if (p.logprob || (top_p < 1.0 && k == 0)) {
+  const bool filtered = k != 1 && ((k > 0 && k < p.vocab) || top_p < 1.0), everything = k == 0 && !filtered && min_p == 0.0f;
+  bool settled = !filtered, counted = false;
+  if constexpr (sizeof(T) == 2)
+    if (filtered) {
+      settled = r.by_values(k, top_p, cut, all_weights);
+      counted = true;
+    }
+  if (!counted && !everything && (p.logprob || (filtered && top_p < 1.0))) {
     double sum = 0.0;
-    for (int i = mine; i < mine + p.each; ++i) sum += (double)r.weight(x[i]);
-    const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
-    r.ahead(s.all, all_weights);
+    r.each([&](float v) { sum += (double)r.weight(v); });
+    all_weights = r.sum_of(sum);
   }
+  if (!settled) cut = r.by_weights(k, p.vocab, top_p, all_weights);
+  if (k == 1) cut = {top, true, 1.0};
 
-  // ---- the cut: kept are those above `at` and the first `ties` that equal it ----
-  float at = -CUDART_INF_F;
-  double ties = 0.0;
-  double above;
-  if (k == 1) {
-    at = top;
-    ties = 1.0;
-  } else if (k > 0 && k < p.vocab) {
-    float c;
-    double equal;
-    if (r.cut<false>((double)k, -CUDART_INF_F, c, above, equal)) {       // (else there are not so many)
-      at = c;
-      ties = (double)k - above;
-    }
-  }
-  if (top_p < 1.0 && k != 1) {
-    double total = all_weights;
-    if (k > 0) {
-      double sum = 0.0;
-      for (int i = mine; i < mine + p.each; ++i) if (x[i] > at) sum += (double)r.weight(x[i]);
-      const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
-      r.ahead(s.all, total);
-      above = total;
-      if (at > -CUDART_INF_F) total += ties * (double)r.weight(at);
-    }
-    const double target = fmax(top_p * total, 1e-300);            // (the first one is always kept)
-    float c;
-    double equal, before = 0.0;
-    double limit = ties;
-    bool found = r.cut<true>(target, at, c, before, equal);
-    if (found) {
-      at = c;
-      limit = equal;
-    } else {
-      before = above;                              // all that are above the cut of top-k, and some that equal it
-      found = k > 0 && at > -CUDART_INF_F;
-    }
-    if (found) {
-      // of those that equal the cut, as many as have less than the target in front of them
-      const double w = (double)r.weight(at);
-      double n = w > 0.0 ? fmax(1.0, ceil((target - before) / w)) : limit;
-      while (n < limit && before + n * w < target) n += 1.0;
-      while (n > 1.0 && before + (n - 1.0) * w >= target) n -= 1.0;
-      ties = fmin(n, limit);
-    }
-  }
-
-  // ---- which of the equal ones this thread's first is ----
-  double rank_of = 0.0;
-  if (at > -CUDART_INF_F) {
-    int64_t equal = 0;
-    for (int i = mine; i < mine + p.each; ++i) equal += x[i] == at;
-    const Scan<int64_t> s = block_scan<kThreads>(equal, sh.counts);
-    double none;
-    rank_of = r.ahead((double)s.all, none) + (double)s.before;
-  }
-  // ---- the kept weights in order of their indices ----
-  auto walk = [&](const auto& keep) {
-    double nth = rank_of;
-    for (int i = mine; i < mine + p.each; ++i) {
-      const float v = x[i];
-      if (v < at || v == -CUDART_INF_F) continue;
-      if (v == at) {
-        nth += 1.0;
-        if (nth > ties) continue;
+  // ---- the kept weights of this thread's elements, in order of their indices ----
+  const uint32_t lowest = max(key_of<S::kDrop>(cut.at), key_of<S::kDrop>(-CUDART_INF_F) + 1u);     // keys from here on
+  const uint32_t tie = cut.found ? key_of<S::kDrop>(cut.at) : 0u;
+  const int words = p.each / S::kWord, from_word = threadIdx.x * words;
+  auto walk = [&](const auto& f) {                 // f(index, key) of each that is not below the cut
+    for (int w = from_word; w < from_word + words; ++w) {
+      const uint32_t v = reinterpret_cast<const uint32_t*>(x)[w];
+      if constexpr (sizeof(E) == 4) {
+        const uint32_t key = key_of<0>(__uint_as_float(v));
+        if (key >= lowest && !f(w, key)) return;
+      } else {
+        if ((v & 0xffffu) >= lowest && !f(2 * w, v & 0xffffu)) return;
+        if ((v >> 16) >= lowest && !f(2 * w + 1, v >> 16)) return;
       }
-      const float w = r.weight(v);
-      if (w >= min_p && w > 0.0f && !keep(i, w)) break;
     }
   };
+  auto kept_weight = [&](uint32_t key) {
+    const float w = r.weight(value_of<S::kDrop>(key));
+    return w >= min_p ? (double)w : 0.0;
+  };
   double sum = 0.0;
-  walk([&](int, float w) { sum += (double)w; return true; });
+  int64_t equal = 0;
+  walk([&](int, uint32_t key) {
+    if (key == tie) ++equal; else sum += kept_weight(key);
+    return true;
+  });
+  double nth = 0.0;                                // ties before this thread's
+  if (cut.found) {
+    const Scan<int64_t> s = block_scan<kThreads>(equal, sh.counts);
+    double none;
+    nth = r.ahead((double)s.all, none) + (double)s.before;
+    sum += fmin(fmax(cut.ties - nth, 0.0), (double)equal) * kept_weight(tie);
+  }
   const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
   double total;
   const double base = r.ahead(s.all, total);
+  if (everything) all_weights = total;
   double mark = u * total;
   if (mark >= total) mark = __longlong_as_double(__double_as_longlong(total) - 1);      // (rounded up: the last one)
-  const double before = base + s.before;
-  if (before <= mark && mark < base + s.upto) {
-    double acc = before;
+  double acc = base + s.before;
+  if (acc <= mark && mark < base + s.upto) {
     int token = -1;
-    walk([&](int i, float w) {
-      acc += (double)w;
+    walk([&](int i, uint32_t key) {
+      if (key == tie) {
+        nth += 1.0;
+        if (nth > cut.ties) return true;
+      }
+      const double w = kept_weight(key);
+      if (w == 0.0) return true;
+      acc += w;
       token = i;
       return acc <= mark;
     });
+    const float v = S::kDrop ? value_of<S::kDrop>((uint32_t)x[token]) : (float)x[token];
     p.token[row] = first + token;
-    if (p.logprob) p.logprob[row] = (float)((x[token] == top ? 0.0 : ((double)x[token] - (double)top) / (double)heat) - log(all_weights));
+    if (p.logprob) p.logprob[row] = (float)((v == top ? 0.0 : ((double)v - (double)top) / (double)heat) - log(all_weights));
   }
   cluster.sync();                                  // nobody leaves while another block may read what it has
 }
@@ -405,24 +608,24 @@ extern "C" int32_t metis_sample(const metis_sample_args* a) {
   if (a->dtype != METIS_DTYPE_BF16 && a->dtype != METIS_DTYPE_F32) return fail(METIS_ERR_BAD_ARGUMENT, "logits must be bf16 or fp32");
   if (a->rows <= 0 || a->vocab <= 0 || (a->rows > 1 && a->ld < a->vocab)) return fail(METIS_ERR_BAD_SHAPE, "rows and vocab must be positive, rows of logits apart");
   if (a->vocab > METIS_SAMPLE_MAX_VOCAB) return fail(METIS_ERR_TOO_LARGE, "vocabularies have at most %d entries", METIS_SAMPLE_MAX_VOCAB);
+  const bool half = a->dtype == METIS_DTYPE_BF16;
   // A block for each 8192 entries up to eight of them: fewer entries for each are sooner done, more blocks wait longer for one another.
   int blocks = 1;
   while (blocks < kMaxCluster && a->vocab > (int64_t)blocks * 8192) blocks *= 2;
-  int64_t each = ceil_div(ceil_div(a->vocab, blocks), kThreads);
-  each |= 1;
+  const int word = half ? 2 : 1;
+  const int64_t each = (ceil_div(ceil_div(a->vocab, blocks), (int64_t)kThreads * word) | 1) * word;
   if (a->rows * blocks >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more rows than one launch takes");
   SampleParams p = {};
-  p.logits = a->logits; p.ld = a->ld; p.vocab = (int32_t)a->vocab; p.each = (int32_t)each; p.dtype = a->dtype; p.u_64 = a->u_64 != 0; p.u = a->u;
+  p.logits = a->logits; p.ld = a->ld; p.vocab = (int32_t)a->vocab; p.each = (int32_t)each; p.u_64 = a->u_64 != 0; p.u = a->u;
   p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
   p.temperature_rows = a->temperature_rows; p.top_p_rows = a->top_p_rows; p.min_p_rows = a->min_p_rows; p.top_k_rows = a->top_k_rows;
   p.token = a->token; p.logprob = a->logprob;
-  constexpr int kMostSmem = (2 * kBins + (METIS_SAMPLE_MAX_VOCAB / kMaxCluster / kThreads + 1) * kThreads) * 4;
-  const bool half = a->dtype == METIS_DTYPE_BF16;
+  constexpr int kMostSmem = (METIS_SAMPLE_MAX_VOCAB / kMaxCluster / kThreads + 1) * kThreads * 4;
   METIS_CUDA_OK(half ? allow_smem<&sample_kernel<__nv_bfloat16>>(kMostSmem) : allow_smem<&sample_kernel<float>>(kMostSmem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a->rows * blocks));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(2 * kBins + each * kThreads) * 4;
+  cfg.dynamicSmemBytes = (size_t)each * kThreads * (half ? 2 : 4);
   cfg.stream = static_cast<cudaStream_t>(a->stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

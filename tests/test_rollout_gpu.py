@@ -822,6 +822,21 @@ def test_sample_what_may_not_be_taken(dtype, vocab):
     assert token[0] == -1 and token[1] == -1 and token[4] == 17 and token[7] == vocab - 1 and token[8] == 1
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sample_cuts_among_small_and_far_values(dtype):
+    """Cuts among logits of tiny magnitude (subnormal ones too), far below the largest, and around huge ones."""
+    n = 6000
+    tiny = torch.ldexp(torch.randn(n, device=DEV, generator=gen(20)), torch.randint(-140, -6, (n,), device=DEV, generator=gen(21)))
+    rows = [tiny, tiny - 0.0, torch.where(torch.arange(n, device=DEV) % 50 == 0, tiny + 3.0, tiny), -tiny.abs(), normal(n, seed=22, scale=300.0, dtype=torch.float32),
+            normal(n, seed=23, scale=1e30, dtype=torch.float32), torch.where(torch.arange(n, device=DEV) == 77, 1000.0, tiny), normal(n, seed=24, scale=1e-30, dtype=torch.float32)]
+    x = torch.stack(rows).to(dtype)
+    x[1, ::2] = 0.0
+    x[1, 1::4] = -0.0
+    u = torch.rand(8, device=DEV, generator=gen(25))
+    for kw in (dict(), dict(top_k=100), dict(top_p=0.5), dict(top_k=3000, top_p=0.4), dict(temperature=100.0, top_p=0.9), dict(temperature=1e3, top_k=40), dict(temperature=1e31, top_p=0.3), dict(temperature=0.01, top_k=70, top_p=0.99)):
+        check_samples(x, u, **kw)
+
+
 def test_sample_at_the_ends_of_u():
     x = normal(6, 1000, seed=4)
     u = torch.tensor([0.0, 1 - 2.0 ** -24, 1 - 2.0 ** -53, 2.0 ** -60, 0.5, 0.25], device=DEV, dtype=torch.float64)
