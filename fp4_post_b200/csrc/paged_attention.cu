@@ -25,11 +25,13 @@
 namespace metis {
 namespace {
 
-constexpr int kTile = 16;                 // keys of a tile
+constexpr int kRows = 16;                 // keys of one product, which lie on one page
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxRows = 1024;            // of one launch: their lengths are summed in shared memory
 constexpr int kMinTiles = kWarps;         // of a block's part, so that each warp has one
+constexpr float kNone = -3e38f;           // the maximum of no scores: finite, so that a score of -inf weighs nothing behind it
+constexpr float kSlack = 8.0f;            // weights may be up to 2^8 before the maximum they are relative to is moved
 
 struct AttendParams {
   const __nv_bfloat16* q;
@@ -97,26 +99,39 @@ __device__ __forceinline__ uint32_t bits(__nv_bfloat162 v) { return *reinterpret
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
 // Rows of a tile in shared memory: 16-byte pieces exchanged by the row, so that eight rows' pieces of one column lie in eight different
-// groups of banks (rows of 64 bytes lie two to a line of 128).
-template <int kRowBytes> __device__ __forceinline__ int piece_at(int row, int piece) {
-  if constexpr (kRowBytes == 64) return row * 64 + ((piece ^ (row >> 1)) & 3) * 16;
-  else return row * kRowBytes + ((piece & ~7) | ((piece ^ row) & 7)) * 16;
+// groups of banks (rows of 64 bytes lie two to a line of 128).  A lane's row and the low bit of its piece are fixed and the even rest is a constant of
+// the unrolled loop, which comes in by one exclusive or.
+template <int kRowBytes> __device__ __forceinline__ uint32_t piece_base(int row, int piece) {
+  if constexpr (kRowBytes == 64) return row * 64 + (((piece ^ (row >> 1)) & 3) << 4);
+  else return row * kRowBytes + ((piece & ~7) << 4) + (((piece ^ row) & 7) << 4);
+}
+template <int kRowBytes> __device__ __forceinline__ uint32_t piece_next(uint32_t base, int even) {
+  constexpr int kMask = kRowBytes == 64 ? 3 : 7;
+  return (base ^ ((even & kMask) << 4)) + ((even & ~kMask) << 4);
 }
 
 template <int D, int NT, bool kE4m3> struct Plan {
   static constexpr int kItem = kE4m3 ? 1 : 2;
   static constexpr int kRowBytes = D * kItem;
-  static constexpr int kPartBytes = kTile * kRowBytes;                  // keys, or values, of a tile
-  static constexpr int kStages = kE4m3 ? 6 : 3;
-  static constexpr int kWarpBytes = kStages * 2 * kPartBytes;           // >= 8 NT D fp32, which is what a warp leaves there at the end of a row
+  static constexpr int kPartBytes = kRows * kRowBytes;                  // keys, or values, of 16 tokens
+  static constexpr int MT = kE4m3 ? 2 : 1;                              // times 16 keys in a tile: 8-bit ones bring half the bytes for the same softmax
+  static constexpr int kTile = kRows * MT;
+  static constexpr int kTileBytes = 2 * MT * kPartBytes;
+  // Two tiles in the ring: one is worked on while the other comes.  Three blocks of an SM have 12 of them on their way, 96 KB, more than the latency of
+  // the memory at its full rate asks for; a third tile would cost one of the blocks.
+  static constexpr int kStages = 2;
+  static constexpr int kWarpBytes = kStages * kTileBytes;               // >= 8 NT D fp32, which is what a warp leaves there at the end of a row
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kPieces = kRowBytes / 16;
+  static constexpr int kHeld = D / 16 * NT * 6;                         // registers of output and queries
+  static constexpr int kBlocks = kHeld <= 48 ? 3 : kHeld <= 96 ? 2 : 1;
   static_assert(8 * NT * D * 4 <= kWarpBytes, "a warp's output goes where its tiles were");
 };
 
 template <int D, int NT, bool kE4m3>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_kernel(const AttendParams p) {
   using L = Plan<D, NT, kE4m3>;
+  constexpr int MT = L::MT;
   extern __shared__ __align__(128) char ring[];
   __shared__ int64_t before[kMaxRows + 1];           // tiles of the rows in front, for one key-value head
   __shared__ int64_t warp_sums[kWarps];
@@ -136,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) 
   };
   for (int base = 0; base < p.rows; base += kThreads) {
     const int row = base + threadIdx.x;
-    int64_t tiles = row < p.rows ? (row_length(row_slot(row)) + kTile - 1) / kTile : 0, all;
+    int64_t tiles = row < p.rows ? (row_length(row_slot(row)) + L::kTile - 1) / L::kTile : 0, all;
     const int64_t ahead = base ? before[base] : 0;
     const int64_t mine = ahead + block_exclusive<kThreads>(tiles, warp_sums, all);
     if (row < p.rows) {
@@ -223,49 +238,72 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) 
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
-      m[n][0] = m[n][1] = -CUDART_INF_F;
+      m[n][0] = m[n][1] = kNone;
       l[n][0] = l[n][1] = 0.0f;
     }
 
     // ---- the warp's tiles: begin + warp, and every fourth from there ----
-    const int64_t first = begin + warp;
-    const int mine_count = first < stop ? (int)((stop - first + kWarps - 1) / kWarps) : 0;
-    const int page_tiles = p.page_size / kTile;
+    const int first = (int)begin + warp, tiles_end = (int)stop, keys_all = (int)length;
+    const int mine_count = first < tiles_end ? (tiles_end - first + kWarps - 1) / kWarps : 0;
+    const int page_rows = p.page_size / kRows;                            // times 16 keys on a page
     const int32_t* table = p.tables + slot * p.width;
-    const int64_t head_off = (int64_t)head * p.page_size * p.head_dim * L::kItem;
     const int row_bytes = p.head_dim * L::kItem;
-    int32_t page = -1;                    // of the lane's tile among the 32 that are looked up at once
-    int fetched = 0;                      // tiles whose copies have been issued
-    uint32_t absent = 0;                  // bit i: the tile i before the last fetched one lies on no page of the pool
+    const char* const head_keys = p.keys + (int64_t)head * p.page_size * row_bytes;
+    const bool exact = p.head_dim == D;
+    // copies: lane's row and piece of the first of a part's 512-byte steps (all further ones by constants where the head has D elements)
+    constexpr int kStepRows = 32 / L::kPieces;
+    const uint32_t copy_base = piece_base<L::kRowBytes>(lane / L::kPieces, lane % L::kPieces);
+    int32_t page = -1, piece_on_page = 0;  // of the lane's 16 keys among the 32 times 16 that are looked up at once
+    int fetched = 0;                       // tiles whose copies have been issued
+    uint32_t absent = 0;                   // bit i: the 16 keys i before the last fetched ones lie on no page of the pool
     auto fetch = [&]() {
       if (fetched < mine_count) {
-        if ((fetched & 31) == 0) {
-          const int64_t tile = first + (int64_t)(fetched + lane) * kWarps;
-          page = tile < stop ? table[tile / page_tiles] : -1;
+        if ((fetched * MT & 31) == 0) {
+          const int which = (first + (fetched + lane / MT) * kWarps) * MT + lane % MT;
+          const bool in = which * kRows < keys_all && which < tiles_end * MT;
+          page = in ? table[which / page_rows] : -1;
+          piece_on_page = which % page_rows;
         }
-        const int32_t pg = __shfl_sync(0xffffffffu, page, fetched & 31);
-        const int64_t tile = first + (int64_t)fetched * kWarps;
-        const bool good = pg >= 0 && pg < p.pages;
-        absent = absent << 1 | (good ? 0u : 1u);
-        const int keys = good ? (int)min((int64_t)kTile, length - tile * kTile) : 0;
-        const char* from = p.keys + (good ? (int64_t)pg * p.page_bytes + head_off + (tile % page_tiles) * kTile * row_bytes : 0);
-        const uint32_t to = mine_at + (uint32_t)(fetched % L::kStages) * 2 * L::kPartBytes;
 #pragma unroll
-        for (int i = 0; i < kTile * L::kPieces / 32; ++i) {
-          const int piece = i * 32 + lane, r = piece / L::kPieces, c = piece % L::kPieces;
-          const bool in = r < keys && c * 16 < row_bytes;
-          const char* src = from + (in ? r * row_bytes + c * 16 : 0);
-          const uint32_t dst = to + piece_at<L::kRowBytes>(r, c);
-          if (!kE4m3 || row_bytes % 16 == 0) {
-            copy16(dst, src, in ? 16 : 0);
-            copy16(dst + L::kPartBytes, src + p.values_off, in ? 16 : 0);
+        for (int part = 0; part < MT; ++part) {
+          const int from_lane = (fetched * MT + part) & 31;
+          const int32_t pg = __shfl_sync(0xffffffffu, page, from_lane);
+          const int at_page = __shfl_sync(0xffffffffu, piece_on_page, from_lane);
+          const bool good = pg >= 0 && pg < p.pages;
+          absent = absent << 1 | (good ? 0u : 1u);
+          const int keys = good ? min(kRows, keys_all - ((first + fetched * kWarps) * MT + part) * kRows) : 0;
+          const char* from = good ? head_keys + (int64_t)pg * p.page_bytes + at_page * (kRows * row_bytes) : p.keys;
+          const uint32_t to = mine_at + (uint32_t)(fetched % L::kStages) * L::kTileBytes + part * 2 * L::kPartBytes;
+          if (exact && keys == kRows) {
+            const char* src = from + lane * 16;
+            const char* src_v = src + p.values_off;
+#pragma unroll
+            for (int i = 0; i < L::kPartBytes / 512; ++i) {
+              // (a step's first row is a multiple of the rows of a step: its bits and the lane's do not meet)
+              constexpr int kMask = L::kRowBytes == 64 ? 0 : 7;
+              const uint32_t dst = to + ((copy_base ^ ((i * kStepRows & kMask) << 4)) + i * 512);
+              copy16(dst, src + i * 512, 16);
+              copy16(dst + L::kPartBytes, src_v + i * 512, 16);
+            }
           } else {
-            // (rows of an odd number of 8 bytes begin on 8 bytes alone)
-            const bool both = in && c * 16 + 8 < row_bytes;
-            copy8(dst, src, in ? 8 : 0);
-            copy8(dst + 8, src + (both ? 8 : 0), both ? 8 : 0);
-            copy8(dst + L::kPartBytes, src + p.values_off, in ? 8 : 0);
-            copy8(dst + L::kPartBytes + 8, src + (both ? 8 : 0) + p.values_off, both ? 8 : 0);
+#pragma unroll 1
+            for (int i = 0; i < L::kPartBytes / 512; ++i) {
+              const int piece = i * 32 + lane, r = piece / L::kPieces, c = piece % L::kPieces;
+              const bool in = r < keys && c * 16 < row_bytes;
+              const char* src = from + (in ? r * row_bytes + c * 16 : 0);
+              const uint32_t dst = to + piece_base<L::kRowBytes>(r, c);
+              if (!kE4m3 || row_bytes % 16 == 0) {
+                copy16(dst, src, in ? 16 : 0);
+                copy16(dst + L::kPartBytes, src + p.values_off, in ? 16 : 0);
+              } else {
+                // (rows of an odd number of 8 bytes begin on 8 bytes alone)
+                const bool both = in && c * 16 + 8 < row_bytes;
+                copy8(dst, src, in ? 8 : 0);
+                copy8(dst + 8, src + (both ? 8 : 0), both ? 8 : 0);
+                copy8(dst + L::kPartBytes, src + p.values_off, in ? 8 : 0);
+                copy8(dst + L::kPartBytes + 8, src + (both ? 8 : 0) + p.values_off, both ? 8 : 0);
+              }
+            }
           }
         }
         ++fetched;
@@ -275,97 +313,143 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) 
 #pragma unroll
     for (int i = 0; i < L::kStages - 1; ++i) fetch();
 
+    const uint32_t k_base = piece_base<L::kRowBytes>(lane & 15, lane >> 4);
+    const uint32_t v_base = kE4m3 ? k_base : piece_base<L::kRowBytes>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
     for (int done = 0; done < mine_count; ++done) {
-      copies_wait<L::kStages - 2>();
-      __syncwarp();                        // every lane's copies of this tile are there, and the tile before it has been read by all
+      __syncwarp();                        // the tile before this one has been read by all lanes
       fetch();
-      const uint32_t kt = mine_at + (uint32_t)(done % L::kStages) * 2 * L::kPartBytes, vt = kt + L::kPartBytes;
-      const int64_t tile = first + (int64_t)done * kWarps;
-      float s[NT][4];
+      copies_wait<L::kStages - 1>();
+      __syncwarp();                        // every lane's copies of this tile are there
+      const uint32_t tile_at = mine_at + (uint32_t)(done % L::kStages) * L::kTileBytes;
+      // ---- scores: keys g and g + 8 of each 16, columns 2 t and 2 t + 1 ----
+      constexpr int kChains = MT * NT == 1 ? 2 : 1;                       // (a single sum would wait for each of its products)
+      float s[MT][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-      if constexpr (!kE4m3) {
+      for (int u = 0; u < MT; ++u) {
+        float sums[kChains][NT][4];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t a[4];
-          matrices(kt + piece_at<L::kRowBytes>(lane & 15, 2 * i + (lane >> 4)), a);
+        for (int c = 0; c < kChains; ++c)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) multiply<false>(s[n], a, q[n][i][0], q[n][i][1]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 16; i += 2) {
-          uint32_t r[4];
-          matrices(kt + piece_at<L::kRowBytes>(lane & 15, i + (lane >> 4)), r);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t a[4] = {widen(r[2 * j]), widen(r[2 * j + 1]), widen(r[2 * j] >> 16), widen(r[2 * j + 1] >> 16)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) multiply<true>(s[n], a, q[n][i + j][0], q[n][i + j][1]);
-          }
-        }
-      }
-      // ---- softmax: column 2 t + j, keys g and g + 8 ----
-      const int64_t left = (absent >> (fetched - 1 - done)) & 1u ? 0 : length - tile * kTile;
-      const bool in0 = g < left, in1 = g + 8 < left;
-      uint32_t hi[NT][2], lo_[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float pr[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float x0 = in0 ? s[n][j] * s_scale[n][j] : -CUDART_INF_F, x1 = in1 ? s[n][2 + j] * s_scale[n][j] : -CUDART_INF_F;
-          float top = fmaxf(x0, x1);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float now = fmaxf(m[n][j], top), from = now == -CUDART_INF_F ? 0.0f : now;
-          const float keep = exp2_fast(m[n][j] - from);
-          pr[j] = exp2_fast(x0 - from);
-          pr[2 + j] = exp2_fast(x1 - from);
-          m[n][j] = now;
-          l[n][j] = l[n][j] * keep + (pr[j] + pr[2 + j]);
+          for (int n = 0; n < NT; ++n) sums[c][n][0] = sums[c][n][1] = sums[c][n][2] = sums[c][n][3] = 0.0f;
+        const uint32_t kt = tile_at + u * 2 * L::kPartBytes + k_base;
+        if constexpr (!kE4m3) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            o[n][i][j] *= keep;
-            o[n][i][2 + j] *= keep;
+            uint32_t a[4];
+            matrices(piece_next<L::kRowBytes>(kt, 2 * i), a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) multiply<false>(sums[i % kChains][n], a, q[n][i][0], q[n][i][1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2) {
+            uint32_t r[4];
+            matrices(piece_next<L::kRowBytes>(kt, i), r);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t a[4] = {widen(r[2 * j]), widen(r[2 * j + 1]), widen(r[2 * j] >> 16), widen(r[2 * j + 1] >> 16)};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) multiply<true>(sums[j % kChains][n], a, q[n][i + j][0], q[n][i + j][1]);
+            }
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if constexpr (kE4m3) {
-            hi[n][r] = transpose8(bits(__floats2half2_rn(pr[2 * r], pr[2 * r + 1])));
-          } else {
-            // the first part is the largest bf16 below p, so that the second one is positive: zero or negative, it would make NaN of an infinite value
-            const uint32_t w = __byte_perm(max(__float_as_uint(pr[2 * r]), 1u) - 1u, max(__float_as_uint(pr[2 * r + 1]), 1u) - 1u, 0x7632);
-            hi[n][r] = transpose8(w);
-            lo_[n][r] = transpose8(bits(__floats2bfloat162_rn(pr[2 * r] - bf16_lo(w), pr[2 * r + 1] - bf16_hi(w))));
-          }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][n][e] = (kChains == 2 ? sums[0][n][e] + sums[kChains - 1][n][e] : sums[0][n][e]) * s_scale[n][e & 1];
+      }
+      // ---- keys behind the last one, and on no page, weigh nothing ----
+      const int left = keys_all - (first + done * kWarps) * L::kTile;
+      const uint32_t gone = absent >> ((fetched - 1 - done) * MT);
+      if (left < L::kTile || (gone & ((1u << MT) - 1u))) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+          const int live_keys = (gone >> (MT - 1 - u)) & 1u ? 0 : left - u * kRows;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (g + (e >> 1) * 8 >= live_keys) s[u][n][e] = -CUDART_INF_F;
         }
       }
-      // ---- values ----
-      if constexpr (!kE4m3) {
+      // ---- softmax: the maximum that weights are relative to moves when one of them would pass 2^8, and the sums with it ----
+      bool over = false;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t a[4];
-          matrices_transposed(vt + piece_at<L::kRowBytes>((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)), a);
+      for (int u = 0; u < MT; ++u)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            multiply<false>(o[n][i], a, hi[n][0], hi[n][1]);
-            multiply<false>(o[n][i], a, lo_[n][0], lo_[n][1]);
-          }
-        }
-      } else {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < D / 16; i += 2) {
-          uint32_t r[4];                   // pairs of elements 16 i + 2 g of keys 2 t, 2 t + 1 and 8 more; the same of 16 (i + 1)
-          matrices_transposed(vt + piece_at<L::kRowBytes>(lane & 15, i + (lane >> 4)), r);
+          for (int e = 0; e < 4; ++e) over |= s[u][n][e] - m[n][e & 1] > kSlack;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t x = __byte_perm(r[2 * j], 0, 0x3120), y = __byte_perm(r[2 * j + 1], 0, 0x3120);
-            const uint32_t a[4] = {widen(x), widen(x >> 16), widen(y), widen(y >> 16)};
+            float top = m[n][j];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) multiply<true>(o[n][i + j], a, hi[n][0], hi[n][1]);
+            for (int u = 0; u < MT; ++u) top = fmaxf(top, fmaxf(s[u][n][j], s[u][n][2 + j]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float keep = exp2_fast(m[n][j] - top);
+            m[n][j] = top;
+            l[n][j] *= keep;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[n][i][j] *= keep;
+              o[n][i][2 + j] *= keep;
+            }
+          }
+      }
+      // ---- weights, as the columns of the other product ----
+#pragma unroll
+      for (int u = 0; u < MT; ++u) {
+        uint32_t hi[NT][2], lo_[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pr[e] = exp2_fast(s[u][n][e] - m[n][e & 1]);
+            l[n][e & 1] += pr[e];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (kE4m3) {
+              hi[n][r] = transpose8(bits(__floats2half2_rn(pr[2 * r], pr[2 * r + 1])));
+            } else {
+              // the first part is the largest bf16 below p, so that the second one is positive: zero or negative, it would make NaN of an infinite value
+              const uint32_t w = __byte_perm(max(__float_as_uint(pr[2 * r]), 1u) - 1u, max(__float_as_uint(pr[2 * r + 1]), 1u) - 1u, 0x7632);
+              hi[n][r] = transpose8(w);
+              lo_[n][r] = transpose8(bits(__floats2bfloat162_rn(pr[2 * r] - bf16_lo(w), pr[2 * r + 1] - bf16_hi(w))));
+            }
+          }
+        }
+        // ---- values ----
+        const uint32_t vt = tile_at + (u * 2 + 1) * L::kPartBytes + v_base;
+        if constexpr (!kE4m3) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t a[4];
+            matrices_transposed(piece_next<L::kRowBytes>(vt, 2 * i), a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              multiply<false>(o[n][i], a, hi[n][0], hi[n][1]);
+              multiply<false>(o[n][i], a, lo_[n][0], lo_[n][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2) {
+            uint32_t r[4];                 // pairs of elements 16 i + 2 g of keys 2 t, 2 t + 1 and 8 more; the same of 16 (i + 1)
+            matrices_transposed(piece_next<L::kRowBytes>(vt, i), r);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t x = __byte_perm(r[2 * j], 0, 0x3120), y = __byte_perm(r[2 * j + 1], 0, 0x3120);
+              const uint32_t a[4] = {widen(x), widen(x >> 16), widen(y), widen(y >> 16)};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) multiply<true>(o[n][i + j], a, hi[n][0], hi[n][1]);
+            }
           }
         }
       }
@@ -397,22 +481,21 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) 
     const int64_t place = (cta * 2 + (begin == 0 ? 1 : 0)) * 8 * NT;
     for (int i = threadIdx.x; i < live * D; i += kThreads) {
       const int column = i / D, e = i - column * D;
-      float top = -CUDART_INF_F;
+      float top = kNone;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][column].x);
-      const float from = top == -CUDART_INF_F ? 0.0f : top;
       float sum = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float2 ml = warp_ml[w][column];
-        const float f = exp2_fast(ml.x - from);
+        const float f = exp2_fast(ml.x - top);
         sum += ml.y * f;
         acc += reinterpret_cast<const float*>(ring + w * L::kWarpBytes)[i] * f;
       }
       if (whole) {
         const int64_t to = (int64_t)row * p.heads_q + first_head + column;
         if (e < p.head_dim) p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(acc, sum) * v_scale);
-        if (e == 0 && p.lse) p.lse[to] = (from + log2f(sum)) * 0.69314718055994531f;
+        if (e == 0 && p.lse) p.lse[to] = (top + log2f(sum)) * 0.69314718055994531f;
       } else {
         p.part_o[(place + column) * D + e] = acc;
         if (e == 0) p.part_ml[place + column] = make_float2(top, sum);
@@ -445,11 +528,10 @@ __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
   const int64_t c0 = (int64_t)blockIdx.x - 1;
   const int pieces = (int)(job.z - c0) + 1;
   auto place = [&](int i) { return ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
-  float top = -CUDART_INF_F;
+  float top = kNone;
   for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float from = top == -CUDART_INF_F ? 0.0f : top;
   float acc[E], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
@@ -457,7 +539,7 @@ __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
   for (int i = warp; i < pieces; i += 8) {
     const int64_t at = place(i);
     const float2 ml = p.part_ml[at];
-    const float f = exp2_fast(ml.x - from);
+    const float f = exp2_fast(ml.x - top);
     sum += ml.y * f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += p.part_o[at * D + e * 32 + lane] * f;
@@ -477,7 +559,7 @@ __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
     for (int w = 0; w < 8; ++w) a += acc_of[w][e];
     p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(a, all) * v_scale);
   }
-  if (threadIdx.x == 0 && p.lse) p.lse[to] = (from + log2f(all)) * 0.69314718055994531f;
+  if (threadIdx.x == 0 && p.lse) p.lse[to] = (top + log2f(all)) * 0.69314718055994531f;
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
