@@ -28,8 +28,12 @@ namespace {
 constexpr int kRows = 16;                 // keys of one product, which lie on one page
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxRows = 1024;            // of one launch: their lengths are summed in shared memory
-constexpr int kMinTiles = kWarps;         // of a block's part, so that each warp has one
+constexpr int kMaxRows = 512;             // of one launch: their sequences and lengths are kept in shared memory
+constexpr int64_t kMaxTiles = (int64_t)1 << 30;      // of one launch and one head
+constexpr int kMinTiles = 8;              // of a part: two for each warp
+// What beginning and ending a row costs a block, in tiles: parts are equal in tiles and this for each row.  A batch of 256 rows of 1 to 2047 keys took
+// 85 us where short rows were counted by their tiles alone, 75 with 4, 57 with 16, 56 with 20 to 32; few long rows do not change.
+constexpr int kBegin = 20;
 constexpr float kNone = -3e38f;           // the maximum of no scores: finite, so that a score of -inf weighs nothing behind it
 constexpr float kSlack = 8.0f;            // weights may be up to 2^8 before the maximum they are relative to is moved
 
@@ -51,7 +55,10 @@ struct AttendParams {
   float scale;                            // times log2(e)
   float* part_o;                          // [2 blocks, 8 NT, D]
   float2* part_ml;                        // [2 blocks, 8 NT]
-  int4* join;                             // [blocks]: row, key-value head and chunk, last block
+  // What the second launch joins: row, unit (key-value head and chunk), first and last block.  One place for each unit of each row where those are no more
+  // than blocks, else one for each block: that of the second piece.
+  int4* join;
+  bool by_unit;
 };
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -133,36 +140,32 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
   using L = Plan<D, NT, kE4m3>;
   constexpr int MT = L::MT;
   extern __shared__ __align__(128) char ring[];
-  __shared__ int64_t before[kMaxRows + 1];           // tiles of the rows in front, for one key-value head
-  __shared__ int64_t warp_sums[kWarps];
+  __shared__ int32_t before[kMaxRows + 1];           // cost of the rows in front, for one key-value head: kBegin and their tiles
+  __shared__ int32_t slot_of[kMaxRows], length_of[kMaxRows];
+  __shared__ int32_t warp_sums[kWarps];
   __shared__ float2 warp_ml[kWarps][8 * NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   grid_dependency_wait();
 
   // ---- this block's part of the tiles ----
-  auto row_slot = [&](int row) -> int64_t {
-    const int64_t slot = p.slots ? load_index(p.slots, p.slots_64, row) : row;
-    return slot >= 0 && slot < p.sequences ? slot : -1;
-  };
-  auto row_length = [&](int64_t slot) -> int64_t {
-    if (slot < 0) return 0;
-    const int64_t length = p.lengths[slot], most = p.width * p.page_size;
-    return length < 0 ? 0 : length < most ? length : most;
-  };
   for (int base = 0; base < p.rows; base += kThreads) {
     const int row = base + threadIdx.x;
-    int64_t tiles = row < p.rows ? (row_length(row_slot(row)) + L::kTile - 1) / L::kTile : 0, all;
-    const int64_t ahead = base ? before[base] : 0;
-    const int64_t mine = ahead + block_exclusive<kThreads>(tiles, warp_sums, all);
+    int32_t length = 0;
     if (row < p.rows) {
-      before[row] = mine;
-      if (row == p.rows - 1) before[p.rows] = mine + tiles;
+      const int64_t slot = p.slots ? load_index(p.slots, p.slots_64, row) : row;
+      const bool known = slot >= 0 && slot < p.sequences;
+      if (known) length = min(max(p.lengths[slot], 0), (int32_t)(p.width * p.page_size));
+      slot_of[row] = known ? (int32_t)slot : -1;
+      length_of[row] = length;
     }
-    if (threadIdx.x == kThreads - 1 && base + kThreads < p.rows) before[base + kThreads] = mine + tiles;
+    const int32_t ahead = base ? before[base] : 0;
+    const Scan<int32_t> s = block_scan<kThreads>(length ? (length + L::kTile - 1) / L::kTile + kBegin : 0, warp_sums);
+    if (row <= p.rows) before[row] = ahead + s.before;
+    if (threadIdx.x == kThreads - 1 && row < p.rows) before[row + 1] = ahead + s.upto;
     __syncthreads();
   }
   const int heads = p.kv_heads * p.chunks;                               // units of work beside one another on the same row
-  const int64_t total = before[p.rows] * heads;
+  const int64_t total = (int64_t)before[p.rows] * heads;
   const int64_t parts = min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
   const int64_t cta = blockIdx.x;
   // rows without keys
@@ -170,8 +173,9 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     if (before[row + 1] != before[row]) continue;
     for (int i = threadIdx.x; i < p.heads_q * p.head_dim; i += kThreads) p.out[(int64_t)row * p.heads_q * p.head_dim + i] = __float2bfloat16_rn(0.0f);
     if (p.lse) for (int i = threadIdx.x; i < p.heads_q; i += kThreads) p.lse[(int64_t)row * p.heads_q + i] = -CUDART_INF_F;
+    if (p.by_unit) for (int i = threadIdx.x; i < heads; i += kThreads) p.join[row * heads + i] = make_int4(-1, 0, 0, 0);
   }
-  if (threadIdx.x == 0) p.join[cta] = make_int4(-1, 0, 0, 0);
+  if (!p.by_unit && threadIdx.x == 0) p.join[cta] = make_int4(-1, 0, 0, 0);
   if (cta >= parts) return;
   int64_t at = cta * total / parts;
   const int64_t end = (cta + 1) * total / parts;
@@ -183,13 +187,18 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     int lo = 0, hi = p.rows;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (before[mid] * heads <= at) lo = mid; else hi = mid;
+      if ((int64_t)before[mid] * heads <= at) lo = mid; else hi = mid;
     }
     const int row = lo;
-    const int64_t row_tiles = before[row + 1] - before[row], inside = at - before[row] * heads;
-    const int unit = (int)(inside / row_tiles), head = unit / p.chunks, chunk = unit - head * p.chunks;
-    const int64_t begin = inside - unit * row_tiles, stop = min(row_tiles, begin + (end - at));
-    const int64_t slot = row_slot(row), length = row_length(slot);
+    const int row_cost = before[row + 1] - before[row], row_tiles = row_cost - kBegin;
+    const int64_t inside = at - (int64_t)before[row] * heads;
+    const int unit = (int)(inside / row_cost), head = unit / p.chunks, chunk = unit - head * p.chunks;
+    // this block's tiles of the unit; its first kBegin places stand for none
+    const int here = (int)(inside - (int64_t)unit * row_cost);
+    const int begin = max(here - kBegin, 0), stop = (int)min((int64_t)row_tiles, here - kBegin + (end - at));
+    at += stop > begin ? stop + kBegin - here : end - at;
+    if (stop <= begin) continue;           // (the part ends before the unit's first tile)
+    const int64_t slot = slot_of[row];
     const int first_head = head * p.group + chunk * 8 * NT, live = min(8 * NT, p.group - chunk * 8 * NT);
     const float k_scale = p.scales ? p.scales[head] : 1.0f, v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
 
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     }
 
     // ---- the warp's tiles: begin + warp, and every fourth from there ----
-    const int first = (int)begin + warp, tiles_end = (int)stop, keys_all = (int)length;
+    const int first = begin + warp, tiles_end = stop, keys_all = length_of[row];
     const int mine_count = first < tiles_end ? (tiles_end - first + kWarps - 1) / kWarps : 0;
     const int page_rows = p.page_size / kRows;                            // times 16 keys on a page
     const int32_t* table = p.tables + slot * p.width;
@@ -501,19 +510,17 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
         if (e == 0) p.part_ml[place + column] = make_float2(top, sum);
       }
     }
-    if (!whole && begin > 0 && threadIdx.x == 0) {
-      // the block whose part ends in the middle of the row's first piece leaves the joining to the next one
-      const int64_t start = before[row] * heads + unit * row_tiles, last = start + row_tiles - 1;
+    if (threadIdx.x == 0 && (p.by_unit ? begin == 0 : begin > 0)) {
+      const int64_t start = (int64_t)before[row] * heads + (int64_t)unit * row_cost + kBegin, last = start + row_tiles - 1;
       const int64_t c0 = ((start + 1) * parts - 1) / total, c1 = ((last + 1) * parts - 1) / total;
-      if (c0 == cta - 1) p.join[cta] = make_int4(row, unit, (int)c1, 0);
+      if (p.by_unit) p.join[row * heads + unit] = make_int4(whole ? -1 : row, unit, (int)c0, (int)c1);
+      else if (c0 == cta - 1) p.join[cta] = make_int4(row, unit, (int)c0, (int)c1);
     }
     __syncthreads();                       // the ring is free again
-    at += stop - begin;
   }
 }
 
-// Joins the pieces of a row that several blocks wrote: block x those of which the second piece is block x's, for one query head of the group.  A
-// warp takes every eighth piece, a lane D / 32 elements.
+// Joins the pieces of a unit that several blocks wrote, for one query head of the group.  A warp takes every eighth piece, a lane D / 32 elements.
 template <int D, int NT>
 __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
   constexpr int E = D / 32;
@@ -525,8 +532,8 @@ __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
   const int head = job.y / p.chunks, chunk = job.y - head * p.chunks, column = blockIdx.y;
   if (chunk * 8 * NT + column >= p.group) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c0 = (int64_t)blockIdx.x - 1;
-  const int pieces = (int)(job.z - c0) + 1;
+  const int64_t c0 = job.z;
+  const int pieces = job.w - job.z + 1;
   auto place = [&](int i) { return ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
   float top = kNone;
   for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
@@ -585,12 +592,15 @@ struct Launch {
     int64_t n = 0;
     if (const int32_t rc = blocks(&n)) return rc;
     if (ws_bytes < workspace(n)) return fail(METIS_ERR_WORKSPACE, "the workspace has %lld bytes, %lld are needed", (long long)ws_bytes, (long long)workspace(n));
+    const int64_t units = (int64_t)p.rows * p.kv_heads * p.chunks;
+    p.by_unit = units <= n;
     char* w = static_cast<char*>(ws);
     p.join = reinterpret_cast<int4*>(w);
     p.part_ml = reinterpret_cast<float2*>(w + n * 16);
     p.part_o = reinterpret_cast<float*>(w + n * (16 + 16 * NT * 8));
     METIS_CUDA_OK(launch_overlapped(kLaunchShort, attend_kernel<D, NT, kE4m3>, dim3((unsigned)n), dim3(kThreads), L::kSmem, st, p));
-    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT>, dim3((unsigned)n, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
+    const int64_t joins = p.by_unit ? units : n;
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT>, dim3((unsigned)joins, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
     count_rollout_launches(2);
     return METIS_OK;
   }
@@ -636,9 +646,10 @@ extern "C" int32_t metis_cache_attend(const metis_cache* cache, const metis_atte
   const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;
   const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   // more rows than one launch counts go in several, one after the other: they share the workspace
-  for (int64_t row = 0; row < a->rows; row += kMaxRows) {
+  const int64_t row_tiles = c.width * c.page_size / kRows, most = kMaxTiles / row_tiles < kMaxRows ? kMaxTiles / row_tiles : kMaxRows;
+  for (int64_t row = 0; row < a->rows; row += most) {
     AttendParams p = {};
-    p.rows = (int32_t)min((int64_t)kMaxRows, a->rows - row);
+    p.rows = (int32_t)min(most, a->rows - row);
     p.q = static_cast<const __nv_bfloat16*>(a->q) + row * a->q_row; p.q_row = a->q_row; p.q_head = a->q_head;
     p.out = static_cast<__nv_bfloat16*>(a->out) + row * a->heads_q * c.head_dim;
     p.lse = a->lse ? a->lse + row * a->heads_q : nullptr;
