@@ -288,15 +288,51 @@ __global__ void __launch_bounds__(256) free_kernel(const CacheView c, const void
 
 enum MoveKind { kFork, kCompact };
 
+// Rows of kRun moves in a row of the plan's list, as pieces of V (16 bytes, or 8 where the rows of 8-bit elements end on half a piece): the filled rows
+// of a page lie in `places`, one for each layer, key or value and head, and are taken as one list, so that all threads have work whatever a page is filled with.
+// A block takes kBatch pieces a thread, all of its loads before its first store; what a prompt's group of answers copies is read once for kRun of them.
+constexpr int kBatch = 8, kRun = 4;
+template <typename V>
+__device__ __forceinline__ void move_rows(const CacheView& c, const Move* moves, int count, int place_bytes, int places, int part) {
+  const int row = c.head_dim * c.item;
+  V v[kBatch];
+  int32_t at_from = -1, at_filled = -1;
+#pragma unroll 1
+  for (int m = 0; m < count; ++m) {
+    const Move mv = moves[m];
+    if (mv.from < 0 || mv.from >= c.pages) continue;       // (a table that named no page)
+    const int in_place = mv.filled * row / (int)sizeof(V), all = in_place * places;
+    int at = part * kBatch * kMoveThreads + (int)threadIdx.x;
+    if (at >= all) continue;
+    int place = at / in_place, inside = at - place * in_place;
+    const int step_places = kMoveThreads / in_place, step_inside = kMoveThreads - step_places * in_place;
+    const bool fresh = mv.from != at_from || mv.filled != at_filled;
+    const char* from = c.pool + mv.from * c.page_bytes;
+    char* to = c.pool + mv.to * c.page_bytes;
+    int off[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      off[i] = at < all ? place * place_bytes + inside * (int)sizeof(V) : -1;
+      if (fresh && at < all) v[i] = *reinterpret_cast<const V*>(from + off[i]);
+      at += kMoveThreads;
+      place += step_places;
+      inside += step_inside;
+      if (inside >= in_place) { inside -= in_place; ++place; }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (off[i] >= 0) *reinterpret_cast<V*>(to + off[i]) = v[i];
+    at_from = mv.from;
+    at_filled = mv.filled;
+  }
+}
+
 // The plan's moves, and what goes with them: of a fork with shared pages the tables' rows and one more holder for each page; of a compaction the
-// pages' new numbers in all tables, and their holders.  A warp takes rows of one (page, layer, key or value, head) of up to 4 KB, all of its
-// loads before the first store.
+// pages' new numbers in all tables, and their holders.
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, const Work w, MoveKind kind, int64_t n) {
   grid_dependency_wait();
   const int32_t moves = w.header->moves;
   if (moves < 0) return;
-  const int64_t warps = (int64_t)gridDim.x * (kMoveThreads / 32), warp = (int64_t)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
   const int64_t threads = (int64_t)gridDim.x * kMoveThreads, thread = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x;
   if (kind == kFork) {
     for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
@@ -324,28 +360,16 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, c
         if (p >= 0 && p < c.pages) c.tables[i] = w.renumbered[p];
       }
   }
-  // Rows of a head lie behind one another: a page is kv_heads * 2 * layers pieces of page_size rows, one piece where it is full.
-  const int64_t row = (int64_t)c.head_dim * c.item, piece = row * c.page_size, pieces = c.page_bytes / piece;
-  constexpr int kBatch = 8;
-  constexpr int64_t kGrain = kBatch * 512;                 // bytes a warp takes at once
-  const int64_t grains = (piece + kGrain - 1) / kGrain, jobs = (int64_t)moves * pieces * grains;
-  for (int64_t j = warp; j < jobs; j += warps) {
-    const int64_t m = j / (pieces * grains), rest = j - m * pieces * grains, which = rest / grains, grain = rest - which * grains;
-    const Move mv = w.moves[m];
-    if (mv.from < 0 || mv.from >= c.pages) continue;       // (a table that named no page)
-    const int64_t filled = mv.filled * row;
-    const char* from = c.pool + mv.from * c.page_bytes + which * piece + grain * kGrain;
-    char* to = c.pool + mv.to * c.page_bytes + which * piece + grain * kGrain;
-    const int64_t left = filled - grain * kGrain;
-    uint4 v[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (i * 512 + lane * 16 + 8 < left) v[i] = *reinterpret_cast<const uint4*>(from + i * 512 + lane * 16);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (i * 512 + lane * 16 + 8 < left) *reinterpret_cast<uint4*>(to + i * 512 + lane * 16) = v[i];
-    // (rows of 8-bit elements may end on half a piece)
-    if (left % 16 == 8 && left < kGrain && left > 0 && lane == 0) *reinterpret_cast<uint2*>(to + left - 8) = *reinterpret_cast<const uint2*>(from + left - 8);
+  const int row = c.head_dim * c.item, piece = row * c.page_size, pieces = (int)(c.page_bytes / piece);
+  const int unit = row % 16 == 0 ? 16 : 8;
+  const int parts = (int)((c.page_bytes / unit + kBatch * kMoveThreads - 1) / (kBatch * kMoveThreads));      // of a full page
+  const int run = kind == kFork ? kRun : 1;
+  const int64_t runs = (moves + run - 1) / run;
+  for (int64_t j = blockIdx.x; j < runs * parts; j += gridDim.x) {
+    const int64_t r = j / parts;
+    const int part = (int)(j - r * parts), count = (int)min((int64_t)run, moves - r * run);
+    if (unit == 16) move_rows<uint4>(c, w.moves + r * run, count, piece, pieces, part);
+    else            move_rows<uint2>(c, w.moves + r * run, count, piece, pieces, part);
   }
 }
 
@@ -379,6 +403,7 @@ int32_t check_cache(const metis_cache* c, CacheView* v) {
   if (c->page_size <= 0 || c->page_size % 16 != 0) return fail(METIS_ERR_BAD_SHAPE, "page_size must be a multiple of 16");
   if (c->head_dim <= 0 || c->head_dim > 256 || c->head_dim % 8 != 0) return fail(METIS_ERR_BAD_SHAPE, "head_dim must be a multiple of 8 up to 256");
   if (c->width > (((int64_t)1 << 31) - 1) / c->page_size) return fail(METIS_ERR_TOO_LARGE, "lengths are 32-bit numbers");
+  if ((int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim >= (int64_t)1 << 30) return fail(METIS_ERR_TOO_LARGE, "a page of all layers has less than 2^30 elements");
   if (!aligned16(c->pool)) return fail(METIS_ERR_BAD_ALIGNMENT, "the pool must be 16-byte aligned");
   *v = {static_cast<char*>(c->pool), (int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim * item, c->pages, c->tables, c->sequences, c->width, c->lengths,
         c->refs, c->status, c->layers, c->kv_heads, c->page_size, c->head_dim, item};

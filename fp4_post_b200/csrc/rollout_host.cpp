@@ -232,8 +232,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
       TORCH_CHECK(saved[0].defined() && saved[0].numel() == tokens, "the saved positions came back as something else");
       positions = indices(saved[0], "saved positions", any.device(), tokens);
     }
+    const Tensor other = gq.defined() && gk.defined() ? gk : Tensor();
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-    const variable_list r = RotaryFunction::apply(any, gq.defined() && gk.defined() ? given(gk) : std::nullopt, given(positions), &by, o[2] == 0);
+    const variable_list r = c10::GradMode::is_enabled() ? RotaryFunction::apply(any, given(other), given(positions), &by, o[2] == 0) : turned(any, other, positions, by, o[2] == 0);
     out[0] = gq.defined() ? r[0] : Tensor();
     if (gk.defined()) out[1] = gq.defined() ? r[1] : r[0];
     return out;

@@ -9,7 +9,7 @@
 // neighbouring pairs) in registers and takes it through the heads of its token; of few tokens, heads are spread over the block instead.
 #include "rollout.cuh"
 
-#include <cuda_fp16.h>
+#include <type_traits>
 
 namespace metis {
 namespace {
@@ -19,7 +19,8 @@ constexpr int kThreads = 256;
 struct RotaryShape {
   int32_t heads_q, heads_k, head_dim, rotary_dim;
   int32_t units, rotary_units;        // of a head: all, and those that turn
-  int32_t head_lanes, block_tokens;   // threads that share a token's heads, tokens of a block
+  int32_t head_lanes, block_tokens;   // threads that share a token's heads, tokens that a block takes at once
+  int32_t span;                       // and in all, one group of block_tokens after the other
   float magnitude, sign;              // what cosines and sines are multiplied by; the direction
 };
 
@@ -135,12 +136,12 @@ struct RotaryTensors {
 };
 
 template <typename T, int W, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryTensors t, const RotaryShape s) {
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryTensors t, const RotaryShape s) {
   extern __shared__ float2 table[];
   grid_dependency_wait();
   const int pairs = s.rotary_dim / 2;
-  const int64_t first = (int64_t)blockIdx.x * s.block_tokens;
-  const int here = (int)min((int64_t)s.block_tokens, t.tokens - first);
+  const int64_t first = (int64_t)blockIdx.x * s.span;
+  const int here = (int)min((int64_t)s.span, t.tokens - first);
   for (int i = threadIdx.x; i < here * pairs; i += kThreads) {
     const int token = i / pairs;
     const int64_t at = first + token;
@@ -148,23 +149,24 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryTensors t,
   }
   __syncthreads();
   const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
-  const int lane = rest % s.head_lanes, token = rest / s.head_lanes;
-  if (token >= here) return;
+  const int lane = rest % s.head_lanes;
   const bool turns = unit < s.rotary_units;
-  float2 c[W];
-  unit_table<W, kInterleaved>(table, token, unit, pairs, turns, c);
-  const int64_t at = first + token, outer = at / t.inner, inner = at - outer * t.inner;
-  const T* q = static_cast<const T*>(t.q) + outer * t.q_outer + inner * t.q_token;
-  T* q_out = static_cast<T*>(t.q_out) + at * s.heads_q * s.head_dim;
-#pragma unroll 4
-  for (int h = lane; h < s.heads_q; h += s.head_lanes)
-    turn_unit<T, W, kInterleaved>(q + h * t.q_head, unit, c, s, turns, PutDense<T>{q_out + (int64_t)h * s.head_dim});
-  if (s.heads_k == 0) return;
-  const T* k = static_cast<const T*>(t.k) + outer * t.k_outer + inner * t.k_token;
-  T* k_out = static_cast<T*>(t.k_out) + at * s.heads_k * s.head_dim;
-#pragma unroll 4
-  for (int h = lane; h < s.heads_k; h += s.head_lanes)
-    turn_unit<T, W, kInterleaved>(k + h * t.k_head, unit, c, s, turns, PutDense<T>{k_out + (int64_t)h * s.head_dim});
+  if (rest >= s.head_lanes * s.block_tokens) return;
+  for (int token = rest / s.head_lanes; token < here; token += s.block_tokens) {
+    float2 c[W];
+    unit_table<W, kInterleaved>(table, token, unit, pairs, turns, c);
+    const int64_t at = first + token, outer = at / t.inner, inner = at - outer * t.inner;
+    const T* q = static_cast<const T*>(t.q) + outer * t.q_outer + inner * t.q_token;
+    T* q_out = static_cast<T*>(t.q_out) + at * s.heads_q * s.head_dim;
+#pragma unroll 8
+    for (int h = lane; h < s.heads_q; h += s.head_lanes)
+      turn_unit<T, W, kInterleaved>(q + h * t.q_head, unit, c, s, turns, PutDense<T>{q_out + (int64_t)h * s.head_dim});
+    if (s.heads_k == 0) continue;
+    const T* k = static_cast<const T*>(t.k) + outer * t.k_outer + inner * t.k_token;
+    T* k_out = static_cast<T*>(t.k_out) + at * s.heads_k * s.head_dim;
+    for (int h = lane; h < s.heads_k; h += s.head_lanes)
+      turn_unit<T, W, kInterleaved>(k + h * t.k_head, unit, c, s, turns, PutDense<T>{k_out + (int64_t)h * s.head_dim});
+  }
 }
 
 // ---- append -------------------------------------------------------------------------------------------------------
@@ -209,17 +211,17 @@ template <> struct PutCache<true> {
 
 // One block takes tokens, and the heads of q, k and v of each, as rotary_kernel does.  What a token goes to is looked up once, by one thread.
 template <int W, bool kInterleaved, bool kE4m3>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendTensors t, const RotaryShape s) {
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendTensors t, const RotaryShape s) {
   extern __shared__ float2 table[];
-  __shared__ int64_t token_at[kThreads];             // bytes from layer_pool to the token's row in the keys of head 0, -1: nowhere, -2: no sequence
-  __shared__ int64_t token_position[kThreads];
+  int64_t* const token_at = reinterpret_cast<int64_t*>(table + s.span * (s.rotary_dim / 2));      // bytes from layer_pool to the token's row in the keys of head 0, -1: nowhere, -2: no sequence
+  int64_t* const token_position = token_at + s.span;
   grid_dependency_wait();
   const CacheView& c = t.cache;
   const int pairs = s.rotary_dim / 2;
-  const int64_t first = (int64_t)blockIdx.x * s.block_tokens;
-  const int here = (int)min((int64_t)s.block_tokens, t.tokens - first);
-  if ((int)threadIdx.x < here) {
-    const int64_t i = first + threadIdx.x, slot = t.slots ? load_index(t.slots, t.slots_64, i) : i;
+  const int64_t first = (int64_t)blockIdx.x * s.span;
+  const int here = (int)min((int64_t)s.span, t.tokens - first);
+  for (int n = threadIdx.x; n < here; n += kThreads) {
+    const int64_t i = first + n, slot = t.slots ? load_index(t.slots, t.slots_64, i) : i;
     int64_t position = t.positions ? load_index(t.positions, t.positions_64, i) : 0, at = -2;
     if (slot >= 0 && slot < c.sequences) {
       const int64_t length = c.lengths[slot];
@@ -230,8 +232,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendTensors t,
         if (page >= 0 && page < c.pages) at = page * c.page_bytes + (position % c.page_size) * c.head_dim * c.item;
       }
     }
-    token_at[threadIdx.x] = at;
-    token_position[threadIdx.x] = position;
+    token_at[n] = at;
+    token_position[n] = position;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < here * pairs; i += kThreads) {
@@ -240,46 +242,49 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendTensors t,
   }
   __syncthreads();
   const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
-  const int lane = rest % s.head_lanes, token = rest / s.head_lanes;
-  if (token >= here) return;
+  const int lane = rest % s.head_lanes;
   const bool turns = unit < s.rotary_units;
-  float2 cs[W];
-  unit_table<W, kInterleaved>(table, token, unit, pairs, turns, cs);
-  const int64_t i = first + token, at = token_at[token];
-  if (s.heads_q > 0) {
-    const __nv_bfloat16* q = t.q + i * t.q_token;
+  if (rest >= s.head_lanes * s.block_tokens) return;
+  using Out = std::conditional_t<kE4m3, uint8_t, __nv_bfloat16>;
+  const int64_t head_bytes = (int64_t)c.page_size * c.head_dim * c.item, values = c.kv_heads * head_bytes;
+  for (int token = rest / s.head_lanes; token < here; token += s.block_tokens) {
+    float2 cs[W];
+    unit_table<W, kInterleaved>(table, token, unit, pairs, turns, cs);
+    const int64_t i = first + token, at = token_at[token];
     __nv_bfloat16* q_out = t.q_out + i * s.heads_q * s.head_dim;
     if (at == -2) {
       // (zeros whatever the row holds)
-      for (int h = lane; h < s.heads_q; h += s.head_lanes)
-        for (int e = unit; e < s.head_dim; e += s.units) q_out[(int64_t)h * s.head_dim + e] = __float2bfloat16_rn(0.0f);
-    } else {
-#pragma unroll 4
-      for (int h = lane; h < s.heads_q; h += s.head_lanes)
-        turn_unit<__nv_bfloat16, W, kInterleaved>(q + h * t.q_head, unit, cs, s, turns, PutDense<__nv_bfloat16>{q_out + (int64_t)h * s.head_dim});
+      for (int h = lane; h < s.heads_q; h += s.head_lanes) {
+        if constexpr (W > 1) {
+          const float zeros[W] = {};
+          for (int e = unit; e < s.head_dim / W; e += s.units) Vec<__nv_bfloat16>::store(q_out + (int64_t)h * s.head_dim + e * W, zeros);
+        } else {
+          for (int e = unit; e < s.head_dim; e += s.units) q_out[(int64_t)h * s.head_dim + e] = __float2bfloat16_rn(0.0f);
+        }
+      }
+      continue;
     }
-  }
-  if (at < 0) return;
-  char* const row = t.layer_pool + at;
-  const int64_t head_bytes = (int64_t)c.page_size * c.head_dim * c.item, values = c.kv_heads * head_bytes;
-  using Out = std::conditional_t<kE4m3, uint8_t, __nv_bfloat16>;
-  const __nv_bfloat16 *k = t.k + i * t.k_token, *v = t.v + i * t.v_token;
-  for (int h = lane; h < c.kv_heads; h += s.head_lanes)
-    turn_unit<__nv_bfloat16, W, kInterleaved>(k + h * t.k_head, unit, cs, s, turns,
-                                              PutCache<kE4m3>{reinterpret_cast<Out*>(row + h * head_bytes), kE4m3 ? t.scales[h] : 1.0f});
-  // values are copied, in the units of the keys (a pair that would be turned by nothing)
-#pragma unroll
-  for (int j = 0; j < W; ++j) cs[j] = make_float2(1.0f, 0.0f);
-  for (int h = lane; h < c.kv_heads; h += s.head_lanes) {
-    const __nv_bfloat16* x = v + h * t.v_head;
-    const PutCache<kE4m3> put{reinterpret_cast<Out*>(row + values + h * head_bytes), kE4m3 ? t.scales[c.kv_heads + h] : 1.0f};
-    if constexpr (W == 1) {
-      for (int e = unit; e < s.head_dim; e += s.units) put.one(e, Vec<__nv_bfloat16>::one(x + e));
-    } else {
-      for (int e = unit; e < s.head_dim / W; e += s.units) {
-        float a[W];
-        Vec<__nv_bfloat16>::load(x + e * W, a);
-        put.wide(e * W, a);
+    const __nv_bfloat16* q = t.q + i * t.q_token;
+#pragma unroll 8
+    for (int h = lane; h < s.heads_q; h += s.head_lanes)
+      turn_unit<__nv_bfloat16, W, kInterleaved>(q + h * t.q_head, unit, cs, s, turns, PutDense<__nv_bfloat16>{q_out + (int64_t)h * s.head_dim});
+    if (at < 0) continue;
+    char* const row = t.layer_pool + at;
+    const __nv_bfloat16 *k = t.k + i * t.k_token, *v = t.v + i * t.v_token;
+    for (int h = lane; h < c.kv_heads; h += s.head_lanes)
+      turn_unit<__nv_bfloat16, W, kInterleaved>(k + h * t.k_head, unit, cs, s, turns,
+                                                PutCache<kE4m3>{reinterpret_cast<Out*>(row + h * head_bytes), kE4m3 ? t.scales[h] : 1.0f});
+    for (int h = lane; h < c.kv_heads; h += s.head_lanes) {
+      const __nv_bfloat16* x = v + h * t.v_head;
+      const PutCache<kE4m3> put{reinterpret_cast<Out*>(row + values + h * head_bytes), kE4m3 ? t.scales[c.kv_heads + h] : 1.0f};
+      if constexpr (W == 1) {
+        for (int e = unit; e < s.head_dim; e += s.units) put.one(e, Vec<__nv_bfloat16>::one(x + e));
+      } else {
+        for (int e = unit; e < s.head_dim / W; e += s.units) {
+          float a[W];
+          Vec<__nv_bfloat16>::load(x + e * W, a);
+          put.wide(e * W, a);
+        }
       }
     }
   }
@@ -298,10 +303,19 @@ RotaryShape rotary_shape(int64_t tokens, int heads_q, int heads_k, int head_dim,
   while (lanes * 2 <= rest && lanes < heads && (lanes * 8 <= heads || tokens * s.units * lanes < enough)) lanes *= 2;
   s.head_lanes = lanes;
   s.block_tokens = rest / lanes;
-  // the table of a block's cosines stays below the shared memory that every launch has
-  const int most = 40960 / (int)sizeof(float2) / (rotary_dim / 2 > 0 ? rotary_dim / 2 : 1);
-  if (s.block_tokens > most) s.block_tokens = most;
   return s;
+}
+
+// How many tokens a block takes in all: one wave of blocks where their tables of cosines (and what else a token needs) allow it.  1024 blocks of 8 tokens
+// were 1.4 waves, and 8192 tokens of 28 + 4 heads took 27.6 us.
+int32_t set_span(RotaryShape& s, int64_t tokens, const void* kernel, int token_bytes) {
+  const int bytes = s.rotary_dim / 2 * (int)sizeof(float2) + token_bytes;
+  const int64_t most = bytes > 0 ? 40960 / bytes : 1 << 20;
+  const int64_t resident = (int64_t)device_sm_count() * resident_ctas(kernel, kThreads, 16384);
+  int64_t span = ceil_div(ceil_div(tokens, resident), s.block_tokens) * s.block_tokens;
+  if (span > most) span = most;
+  s.span = (int32_t)span;
+  return (int32_t)span * bytes;
 }
 
 bool multiple(std::initializer_list<int64_t> v, int64_t n) {
@@ -309,18 +323,18 @@ bool multiple(std::initializer_list<int64_t> v, int64_t n) {
   return true;
 }
 
-template <typename T, int W>
-cudaError_t launch_rotary(bool interleaved, const RotaryTensors& t, const RotaryShape& s, cudaStream_t st) {
-  const int64_t blocks = ceil_div(t.tokens, s.block_tokens);
-  const size_t smem = (size_t)s.block_tokens * (s.rotary_dim / 2) * sizeof(float2);
-  return launch_overlapped(kLaunchShort, interleaved ? rotary_kernel<T, W, true> : rotary_kernel<T, W, false>, dim3((unsigned)blocks), dim3(kThreads), smem, st, t, s);
+template <typename T, int W, bool kInterleaved>
+cudaError_t launch_rotary(const RotaryTensors& t, RotaryShape s, cudaStream_t st) {
+  const auto kernel = rotary_kernel<T, W, kInterleaved>;
+  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 0);
+  return launch_overlapped(kLaunchShort, kernel, dim3((unsigned)ceil_div(t.tokens, s.span)), dim3(kThreads), (size_t)smem, st, t, s);
 }
 
-template <int W, bool kInterleaved>
-cudaError_t launch_append(bool e4m3, const AppendTensors& t, const RotaryShape& s, cudaStream_t st) {
-  const int64_t blocks = ceil_div(t.tokens, s.block_tokens);
-  const size_t smem = (size_t)s.block_tokens * (s.rotary_dim / 2) * sizeof(float2);
-  return launch_overlapped(kLaunchShort, e4m3 ? append_kernel<W, kInterleaved, true> : append_kernel<W, kInterleaved, false>, dim3((unsigned)blocks), dim3(kThreads), smem, st, t, s);
+template <int W, bool kInterleaved, bool kE4m3>
+cudaError_t launch_append(const AppendTensors& t, RotaryShape s, cudaStream_t st) {
+  const auto kernel = append_kernel<W, kInterleaved, kE4m3>;
+  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 16);
+  return launch_overlapped(kLaunchShort, kernel, dim3((unsigned)ceil_div(t.tokens, s.span)), dim3(kThreads), (size_t)smem, st, t, s);
 }
 
 }  // namespace
@@ -343,13 +357,19 @@ extern "C" int32_t metis_rotary(const metis_rotary_args* a) {
   RotaryShape s = rotary_shape(a->tokens, a->heads_q, a->heads_k, a->head_dim, a->rotary_dim, a->interleaved != 0, vectors ? wide : 1);
   s.magnitude = a->magnitude;
   s.sign = a->inverse ? -1.0f : 1.0f;
-  if (ceil_div(a->tokens, s.block_tokens) >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
+  if (a->tokens >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
   const RotaryTensors t = {a->positions, a->tokens, a->inner, a->turns, a->q, a->k, a->q_outer, a->q_token, a->q_head, a->k_outer, a->k_token, a->k_head,
                            a->q_out, a->k_out, a->positions_64 != 0};
   const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   const bool in = a->interleaved != 0;
-  if (item == 2) METIS_CUDA_OK((vectors ? launch_rotary<__nv_bfloat16, 8>(in, t, s, st) : launch_rotary<__nv_bfloat16, 1>(in, t, s, st)));
-  else           METIS_CUDA_OK((vectors ? launch_rotary<float, 4>(in, t, s, st) : launch_rotary<float, 1>(in, t, s, st)));
+  const auto by_layout = [&](auto element, auto width) {
+    using T = decltype(element);
+    constexpr int W = decltype(width)::value;
+    return in ? launch_rotary<T, W, true>(t, s, st) : launch_rotary<T, W, false>(t, s, st);
+  };
+  using One = std::integral_constant<int, 1>;
+  if (item == 2) METIS_CUDA_OK((vectors ? by_layout(__nv_bfloat16(), std::integral_constant<int, 8>()) : by_layout(__nv_bfloat16(), One())));
+  else           METIS_CUDA_OK((vectors ? by_layout(0.0f, std::integral_constant<int, 4>()) : by_layout(0.0f, One())));
   count_rollout_launches(1);
   return METIS_OK;
 }
@@ -370,7 +390,7 @@ extern "C" int32_t metis_cache_append(const metis_cache* cache, const metis_appe
   s.heads_q = a->heads_q;
   s.magnitude = a->magnitude;
   s.sign = 1.0f;
-  if (ceil_div(a->tokens, s.block_tokens) >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
+  if (a->tokens >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more tokens than one launch takes");
   const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;       // keys, or values, of one layer on a page
   t.layer_pool = c.pool + a->layer * 2 * part;
   t.scales = cache->scales ? cache->scales + (int64_t)a->layer * 2 * c.kv_heads : nullptr;
@@ -381,8 +401,12 @@ extern "C" int32_t metis_cache_append(const metis_cache* cache, const metis_appe
   t.slots_64 = (a->index_64 & 1) != 0; t.positions_64 = (a->index_64 & 2) != 0;
   const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   const bool e4m3 = c.item == 1;
-  if (vectors) METIS_CUDA_OK((in ? launch_append<8, true>(e4m3, t, s, st) : launch_append<8, false>(e4m3, t, s, st)));
-  else         METIS_CUDA_OK((in ? launch_append<1, true>(e4m3, t, s, st) : launch_append<1, false>(e4m3, t, s, st)));
+  const auto by_layout = [&](auto width) {
+    constexpr int W = decltype(width)::value;
+    return in ? (e4m3 ? launch_append<W, true, true>(t, s, st) : launch_append<W, true, false>(t, s, st))
+              : (e4m3 ? launch_append<W, false, true>(t, s, st) : launch_append<W, false, false>(t, s, st));
+  };
+  METIS_CUDA_OK((vectors ? by_layout(std::integral_constant<int, 8>()) : by_layout(std::integral_constant<int, 1>())));
   count_rollout_launches(1);
   return METIS_OK;
 }
