@@ -69,6 +69,30 @@ __device__ __forceinline__ Scan<T> block_scan(T v, T* warp_sums) {
   const T left = __shfl_up_sync(0xffffffffu, sum, 1);
   return {lane == 0 ? ahead : ahead + left, ahead + sum, all};
 }
+// Two at once, between the same barriers.
+template <int kThreads, typename T>
+__device__ __forceinline__ void block_scan_two(T a, T b, T* sums_a, T* sums_b, Scan<T>& of_a, Scan<T>& of_b) {
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T from_a = __shfl_up_sync(0xffffffffu, a, o), from_b = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) { a += from_a; b += from_b; }
+  }
+  __syncthreads();
+  if (lane == 31) { sums_a[warp] = a; sums_b[warp] = b; }
+  __syncthreads();
+  T ahead_a = T(0), ahead_b = T(0), all_a = T(0), all_b = T(0);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) { ahead_a = all_a; ahead_b = all_b; }
+    all_a += sums_a[w];
+    all_b += sums_b[w];
+  }
+  const T left_a = __shfl_up_sync(0xffffffffu, a, 1), left_b = __shfl_up_sync(0xffffffffu, b, 1);
+  of_a = {lane == 0 ? ahead_a : ahead_a + left_a, ahead_a + a, all_a};
+  of_b = {lane == 0 ? ahead_b : ahead_b + left_b, ahead_b + b, all_b};
+}
 template <int kThreads, typename T>
 __device__ __forceinline__ T block_exclusive(T v, T* warp_sums, T& total) {
   const Scan<T> s = block_scan<kThreads>(v, warp_sums);

@@ -4,8 +4,7 @@
 //   top-k keeps the first k of the order; top-p the shortest front of those whose weights are at least p of theirs; min-p those with w >= min_p.
 //   Each keeps a front of the order, so that what is kept is "x above a cut, and the first n of those that equal it".
 //
-// A cluster of up to eight blocks takes a row: it is read once from memory, 16 bytes at a time, and stays in shared memory (bf16 as 16-bit keys in the order of the
-// values, fp32 as it is) for all passes.  Nothing is sorted; a cut is found by histograms:
+// A cluster of up to eight blocks takes a row: it is read once from memory, 16 bytes at a time, and stays in shared memory (in its type) for all passes.  Nothing is sorted; a cut is found by histograms:
 //   bf16  The bins are the values themselves, from the largest one on: 4095 of them, those below 2^-8 in magnitude together in one.  That is every logit
 //         within +-256.  A pass counts, five instructions and an addition in shared memory an element; a bin's weight is its count times the
 //         weight of its value, so that one histogram serves top-k, top-p and the sum of all.  (A cut in the bin of small values or behind the last one goes the other way.)
@@ -51,8 +50,7 @@ struct Found { double above, inside; int32_t bin; };      // weight before the b
 struct Cut { float at; bool found; double ties; };        // kept are those above `at` and the first `ties` that equal it
 
 struct Shared {
-  double sums[kThreads / 32];
-  int64_t counts[kThreads / 32];
+  double sums[kThreads / 32], more_sums[kThreads / 32];
   double gathered[2][kMaxCluster][2];
   Found found;
   Cut cut[2];                                      // of top-k, of top-p
@@ -72,25 +70,25 @@ template <int kDrop> __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~(k | ((1u << kDrop) - 1u)));
 }
 
-// Elements in shared memory: fp32, or the 16-bit keys of bf16.
+// Elements in shared memory, in the type of the logits: NaN as -inf, -0 as 0.
 template <typename T> struct Store;
 template <> struct Store<float> {
-  static constexpr int kDrop = 0, kWord = 1;        // elements of a 32-bit word
-  using Element = float;
-  static __device__ __forceinline__ float at(const float* x, int i) { return x[i]; }
-  template <typename F> static __device__ __forceinline__ void word(const float* x, int w, const F& f) { f(w, x[w]); }
+  static constexpr int kDrop = 0, kWord = 1;        // bits that keys go without, elements of a 32-bit word
   static __device__ __forceinline__ float clean(float v) { return v == v ? v + 0.0f : -CUDART_INF_F; }
+  static __device__ __forceinline__ uint32_t clean(uint32_t w) { return __float_as_uint(clean(__uint_as_float(w))); }
+  static __device__ __forceinline__ float value(uint32_t w, int) { return __uint_as_float(w); }
 };
 template <> struct Store<__nv_bfloat16> {
   static constexpr int kDrop = 16, kWord = 2;
-  using Element = uint16_t;
-  static __device__ __forceinline__ float at(const uint16_t* x, int i) { return value_of<16>(x[i]); }
-  // two bf16 -> two keys: NaN as -inf (the maximum with it), -0 as 0, then negative ones with all bits turned and the others with the sign
-  static __device__ __forceinline__ uint32_t keys(uint32_t two) {
-    const uint32_t lowest = 0xff80ff80u, none = 0u;
-    __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&lowest));
-    v = __hadd2_rn(v, *reinterpret_cast<const __nv_bfloat162*>(&none));
-    const uint32_t w = *reinterpret_cast<uint32_t*>(&v), s = w & 0x80008000u;
+  static __device__ __forceinline__ uint32_t clean(uint32_t two) {
+    const uint32_t lowest = 0xff80ff80u, none = 0u;                       // (the maximum of NaN and a number is the number)
+    const __nv_bfloat162 v = __hadd2_rn(__hmax2(*reinterpret_cast<__nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&lowest)), *reinterpret_cast<const __nv_bfloat162*>(&none));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float value(uint32_t w, int half) { return half ? bf16_hi(w) : bf16_lo(w); }
+  // two keys: negative ones with all bits turned, the others with the sign
+  static __device__ __forceinline__ uint32_t keys(uint32_t w) {
+    const uint32_t s = w & 0x80008000u;
     return w ^ ((s - (s >> 15)) | 0x80008000u);
   }
 };
@@ -101,36 +99,28 @@ constexpr int kAbove = 0xbb80, kBelow = 0x447f;    // the keys of 2^-8 and -2^-8
 template <typename T>
 struct Row {
   using S = Store<T>;
-  using E = typename S::Element;
   cg::cluster_group cluster;
   Shared& sh;
-  const E* x;                                      // this block's logits; -inf behind the last
+  const uint32_t* x;                               // this block's logits; -inf behind the last
   int blocks, rank, held;                          // held: elements of x
   float top, inverse;                              // the largest logit, 1/T
   int turn = 0;
 
   __device__ float weight(float v) const { return v == top ? 1.0f : expf(__fmul_rn(__fsub_rn(v, top), inverse)); }
 
-  // f(x) of each of the block's elements, 16 bytes at a time
-  template <typename F> __device__ __forceinline__ void each(const F& f) const {
-    constexpr int kWide = 16 / (int)sizeof(E);
-    for (int i = threadIdx.x; i < held / kWide; i += kThreads) {
+  // f(word) of each of the block's words, 16 bytes at a time
+  template <typename F> __device__ __forceinline__ void each_word(const F& f) const {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < held / S::kWord / 4; i += kThreads) {
       const uint4 w = reinterpret_cast<const uint4*>(x)[i];
-      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(E) == 4) f(__uint_as_float(v[j]));
-        else { f(value_of<16>(v[j] & 0xffffu)); f(value_of<16>(v[j] >> 16)); }
-      }
+      f(w.x); f(w.y); f(w.z); f(w.w);
     }
   }
-  template <typename F> __device__ __forceinline__ void each_key(const F& f) const {
-    for (int i = threadIdx.x; i < held / 8; i += kThreads) {
-      const uint4 w = reinterpret_cast<const uint4*>(x)[i];
-      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  template <typename F> __device__ __forceinline__ void each(const F& f) const {
+    each_word([&](uint32_t w) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { f(v[j] & 0xffffu); f(v[j] >> 16); }
-    }
+      for (int h = 0; h < S::kWord; ++h) f(S::value(w, h));
+    });
   }
 
   // Two values of each block to all; two buffers in turn, so that one barrier does for both writing and reading.
@@ -165,6 +155,26 @@ struct Row {
     __syncthreads();
   }
 
+  // One word of all blocks' histograms, summed (all loads before the first addition: one from a peer takes some 700 cycles).
+  __device__ uint32_t of_all(int word) const {
+    uint32_t v[kMaxCluster], sum = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) v[r] = r < blocks ? cluster.map_shared_rank(&sh, r)->bins[word] : 0u;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) sum += v[r];
+    return sum;
+  }
+
+  __device__ uint64_t of_all_wide(int word) const {
+    uint32_t v[kMaxCluster];
+    uint64_t sum = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) v[r] = r < blocks ? cluster.map_shared_rank(&sh, r)->bins[word] : 0u;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) sum += v[r];
+    return sum;
+  }
+
   // ---- histograms of weights (fp32; bf16 where the values' bins do not have the cut) ----
 
   __device__ int bin_of(float v) const {
@@ -197,13 +207,10 @@ struct Row {
       v[i] = 0.0;
       if (i >= mine || local >= slice) continue;
       const int bin = rank * slice + local;
-      uint64_t low = 0, high = 0;
-      for (int r = 0; r < blocks; ++r) {
-        const Shared* peer = cluster.map_shared_rank(&sh, r);
-        low += peer->bins[bin];
-        if (kMass) high += peer->bins[kBins + bin];
-      }
-      const uint64_t m = low + (high << kLowBits);
+      // (each block's word is below 2^29.6, and eight of them below 2^32 only where they are counts)
+      uint64_t m;
+      if constexpr (kMass) m = of_all_wide(bin) + (of_all_wide(kBins + bin) << kLowBits);
+      else m = of_all(bin);
       if (m) v[i] = kMass ? ldexp((double)m, unit == 1 ? unit_of(bin) : unit) : (double)m;
       sum += v[i];
     }
@@ -337,13 +344,18 @@ struct Row {
     clear();
     double extra = 0.0;                            // weights in the bins of several values: the small ones', and behind them the last one's
     double extra_small = 0.0;
-    each_key([&](uint32_t key) {
-      const int d = b.top - (int)key;
-      const int bin = min(max(min(d, b.small), d - b.gap), kValues - 1);
-      if (key == kLowest16) return;
-      atomicAdd(&sh.bins[bin], 1u);
-      if (bin == kValues - 1) extra += (double)weight(value_of<16>(key));
-      else if (b.has_small && bin == b.small) extra_small += (double)weight(value_of<16>(key));
+    const int small_bin = b.has_small ? b.small : -1;
+    each_word([&](uint32_t w) {
+      const uint32_t two = S::keys(w);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = (int)(h ? two >> 16 : two & 0xffffu), d = b.top - key;
+        const int bin = min(max(min(d, b.small), d - b.gap), kValues - 1);
+        if (key == (int)kLowest16) continue;
+        atomicAdd(&sh.bins[bin], 1u);
+        if (bin == kValues - 1) extra += (double)weight(S::value(w, h));
+        else if (bin == small_bin) extra_small += (double)weight(S::value(w, h));
+      }
     });
     // (sums of nothing, mostly)
     double rest = 0.0, small = 0.0;
@@ -370,7 +382,7 @@ struct Row {
     for (int i = 0; i < kMost; ++i) {
       n[i] = 0;
       if (i >= mine || !active) continue;
-      for (int r = 0; r < blocks; ++r) n[i] += cluster.map_shared_rank(&sh, r)->bins[first + i];
+      n[i] = of_all(first + i);
     }
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
@@ -378,7 +390,8 @@ struct Row {
       count += (double)n[i];
       mass += bin_mass(first + i, n[i]);
     }
-    const Scan<double> sc = block_scan<kThreads>(count, sh.sums), sm = block_scan<kThreads>(mass, sh.sums);
+    Scan<double> sc, sm;
+    block_scan_two<kThreads>(count, mass, sh.sums, sh.more_sums, sc, sm);
     const double (*g)[2] = gather(sc.all, sm.all);
     double before_count = 0.0, before_mass = 0.0, all_count = 0.0;
     all_weights = 0.0;
@@ -449,45 +462,54 @@ struct Row {
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
   using S = Store<T>;
-  using E = typename S::Element;
-  extern __shared__ __align__(16) char dynamic[];
+  extern __shared__ __align__(16) uint32_t x[];
   __shared__ Shared sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t row = blockIdx.x / blocks;
   const int held = p.each * kThreads, first = rank * held, here = max(0, min(held, p.vocab - first));
-  E* x = reinterpret_cast<E*>(dynamic);
   cluster.barrier_arrive();                        // (a block is written to by the others once all have begun)
   grid_dependency_wait();
+
+  const float t = p.temperature_rows ? p.temperature_rows[row] : p.temperature, min_p = p.min_p_rows ? p.min_p_rows[row] : p.min_p;
+  const double top_p = p.top_p_rows ? (double)p.top_p_rows[row] : p.top_p;
+  int64_t k = p.top_k_rows ? p.top_k_rows[row] : p.top_k;
+  const double u = p.u_64 ? static_cast<const double*>(p.u)[row] : (double)static_cast<const float*>(p.u)[row];
 
   // ---- the row; NaN and what is behind it as -inf, -0 as 0 ----
   const T* from = static_cast<const T*>(p.logits) + row * p.ld + first;
   constexpr int kWide = 16 / (int)sizeof(T);
   const int wide = (reinterpret_cast<uintptr_t>(from) & 15) == 0 ? here / kWide : 0;
-  uint32_t best = 0;                               // the largest key
+  float most = -CUDART_INF_F;
+  uint32_t most_two = 0xff80ff80u;                 // of the even elements, of the odd ones
+  auto track = [&](uint32_t w) {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&most_two), *reinterpret_cast<__nv_bfloat162*>(&w));
+      most_two = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      most = fmaxf(most, __uint_as_float(w));
+    }
+  };
 #pragma unroll 4
   for (int i = threadIdx.x; i < wide; i += kThreads) {
-    uint4 w = __ldcs(reinterpret_cast<const uint4*>(from) + i);
-    if constexpr (sizeof(T) == 2) {
-      w = make_uint4(S::keys(w.x), S::keys(w.y), S::keys(w.z), S::keys(w.w));
-      best = __vmaxu2(best, __vmaxu2(__vmaxu2(w.x, w.y), __vmaxu2(w.z, w.w)));
-    } else {
-      const float4 v = make_float4(S::clean(__uint_as_float(w.x)), S::clean(__uint_as_float(w.y)), S::clean(__uint_as_float(w.z)), S::clean(__uint_as_float(w.w)));
-      w = make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
-      best = max(best, key_of<0>(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
-    }
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+    const uint4 w = make_uint4(S::clean(v.x), S::clean(v.y), S::clean(v.z), S::clean(v.w));
+    track(w.x); track(w.y); track(w.z); track(w.w);
     reinterpret_cast<uint4*>(x)[i] = w;
   }
-  if constexpr (sizeof(T) == 2) best = max(best & 0xffffu, best >> 16);
   for (int i = wide * kWide + threadIdx.x; i < held; i += kThreads) {
     if constexpr (sizeof(T) == 2) {
-      x[i] = (E)(i < here ? S::keys(reinterpret_cast<const uint16_t*>(from)[i]) & 0xffffu : kLowest16);
-      best = max(best, (uint32_t)x[i]);
+      const uint32_t w = S::clean(i < here ? 0xff800000u | reinterpret_cast<const uint16_t*>(from)[i] : 0xff80ff80u);
+      track(w);
+      reinterpret_cast<uint16_t*>(x)[i] = (uint16_t)w;
     } else {
-      x[i] = i < here ? S::clean(from[i]) : -CUDART_INF_F;
-      best = max(best, key_of<0>(x[i]));
+      const uint32_t w = i < here ? S::clean(__float_as_uint(from[i])) : 0xff800000u;
+      track(w);
+      x[i] = w;
     }
   }
+  if constexpr (sizeof(T) == 2) most = fmaxf(bf16_lo(most_two), bf16_hi(most_two));
+  uint32_t best = key_of<S::kDrop>(most);          // the largest key
   best = __reduce_max_sync(0xffffffffu, best);
   if ((threadIdx.x & 31) == 0) sh.maxima[threadIdx.x >> 5] = best;
   __syncthreads();
@@ -501,10 +523,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     for (int i = 0; i < blocks; ++i) best = max(best, (uint32_t)g[i][0]);
   }
   const float top = value_of<S::kDrop>(best);
-  const float t = p.temperature_rows ? p.temperature_rows[row] : p.temperature, min_p = p.min_p_rows ? p.min_p_rows[row] : p.min_p;
-  const double top_p = p.top_p_rows ? (double)p.top_p_rows[row] : p.top_p;
-  int64_t k = p.top_k_rows ? p.top_k_rows[row] : p.top_k;
-  const double u = p.u_64 ? static_cast<const double*>(p.u)[row] : (double)static_cast<const float*>(p.u)[row];
   const bool fine = (t == 0.0f || (t >= 0x1p-126f && t <= 3.4028235e38f)) && top_p >= 0.0 && min_p >= 0.0f && min_p <= 1.0f && k >= 0 && u >= 0.0 && u < 1.0 &&
                     top > -CUDART_INF_F;
   if (!fine) {                                     // (for all blocks of the cluster)
@@ -539,61 +557,88 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   if (k == 1) cut = {top, true, 1.0};
 
   // ---- the kept weights of this thread's elements, in order of their indices ----
-  const uint32_t lowest = max(key_of<S::kDrop>(cut.at), key_of<S::kDrop>(-CUDART_INF_F) + 1u);     // keys from here on
-  const uint32_t tie = cut.found ? key_of<S::kDrop>(cut.at) : 0u;
+  const float from_value = cut.found ? cut.at : sizeof(T) == 2 ? -0x1.fep127f : -3.4028235e38f;  // (the lowest finite one: -inf is never kept)
   const int words = p.each / S::kWord, from_word = threadIdx.x * words;
-  auto walk = [&](const auto& f) {                 // f(index, key) of each that is not below the cut
+  auto walk = [&](const auto& f) {                 // f(index, value) of each that is not below the cut
+    __nv_bfloat162 from_two = __float2bfloat162_rn(from_value);
     for (int w = from_word; w < from_word + words; ++w) {
-      const uint32_t v = reinterpret_cast<const uint32_t*>(x)[w];
-      if constexpr (sizeof(E) == 4) {
-        const uint32_t key = key_of<0>(__uint_as_float(v));
-        if (key >= lowest && !f(w, key)) return;
+      uint32_t v = x[w];
+      if constexpr (sizeof(T) == 4) {
+        if (__uint_as_float(v) >= from_value && !f(w, __uint_as_float(v))) return;
       } else {
-        if ((v & 0xffffu) >= lowest && !f(2 * w, v & 0xffffu)) return;
-        if ((v >> 16) >= lowest && !f(2 * w + 1, v >> 16)) return;
+        const uint32_t in = __hge2_mask(*reinterpret_cast<__nv_bfloat162*>(&v), from_two);
+        if (in == 0u) continue;
+        if ((in & 0xffffu) && !f(2 * w, bf16_lo(v))) return;
+        if ((in >> 16) && !f(2 * w + 1, bf16_hi(v))) return;
       }
     }
   };
-  auto kept_weight = [&](uint32_t key) {
-    const float w = r.weight(value_of<S::kDrop>(key));
+  auto kept_weight = [&](float v) {
+    const float w = r.weight(v);
     return w >= min_p ? (double)w : 0.0;
   };
+  // those above the cut, summed, and those that equal it, counted; all lanes go the same way
   double sum = 0.0;
-  int64_t equal = 0;
-  walk([&](int, uint32_t key) {
-    if (key == tie) ++equal; else sum += kept_weight(key);
-    return true;
-  });
-  double nth = 0.0;                                // ties before this thread's
-  if (cut.found) {
-    const Scan<int64_t> s = block_scan<kThreads>(equal, sh.counts);
-    double none;
-    nth = r.ahead((double)s.all, none) + (double)s.before;
-    sum += fmin(fmax(cut.ties - nth, 0.0), (double)equal) * kept_weight(tie);
+  int32_t equal = 0;
+#pragma unroll 4
+  for (int w = from_word; w < from_word + words; ++w) {
+    const uint32_t v = x[w];
+    bool in = false;
+#pragma unroll
+    for (int h = 0; h < S::kWord; ++h) in |= S::value(v, h) >= from_value;
+    if (!__any_sync(0xffffffffu, in)) continue;
+#pragma unroll
+    for (int h = 0; h < S::kWord; ++h) {
+      const float value = S::value(v, h);
+      const bool tie = cut.found && value == cut.at;
+      equal += tie;
+      sum += value >= from_value && !tie ? kept_weight(value) : 0.0;
+    }
   }
-  const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
-  double total;
-  const double base = r.ahead(s.all, total);
+  // Which block has the mark goes by the blocks' sums, the same numbers in all of them; there, a thread by its own.
+  double nth = 0.0, kept_ties = 0.0;               // ties before this thread's, and how many of its own are kept
+  const double tie_weight = cut.found ? kept_weight(cut.at) : 0.0;
+  Scan<double> se, ss;
+  block_scan_two<kThreads>((double)equal, sum, sh.sums, sh.more_sums, se, ss);
+  double total = 0.0, base = 0.0, upto = 0.0;
+  {
+    const double (*g)[2] = r.gather(se.all, ss.all);
+    double ties_before = 0.0;
+    for (int i = 0; i < blocks; ++i) {
+      if (i == rank) { base = total; nth = ties_before + se.before; }
+      total += g[i][1] + fmin(fmax(cut.ties - ties_before, 0.0), g[i][0]) * tie_weight;
+      ties_before += g[i][0];
+      if (i == rank) upto = total;
+    }
+  }
   if (everything) all_weights = total;
   double mark = u * total;
   if (mark >= total) mark = __longlong_as_double(__double_as_longlong(total) - 1);      // (rounded up: the last one)
-  double acc = base + s.before;
-  if (acc <= mark && mark < base + s.upto) {
-    int token = -1;
-    walk([&](int i, uint32_t key) {
-      if (key == tie) {
-        nth += 1.0;
-        if (nth > cut.ties) return true;
-      }
-      const double w = kept_weight(key);
-      if (w == 0.0) return true;
-      acc += w;
-      token = i;
-      return acc <= mark;
-    });
-    const float v = S::kDrop ? value_of<S::kDrop>((uint32_t)x[token]) : (float)x[token];
-    p.token[row] = first + token;
-    if (p.logprob) p.logprob[row] = (float)((v == top ? 0.0 : ((double)v - (double)top) / (double)heat) - log(all_weights));
+  if (base <= mark && mark < upto) {               // (one block of the cluster)
+    kept_ties = fmin(fmax(cut.ties - nth, 0.0), (double)equal);
+    sum += kept_ties * tie_weight;
+    const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
+    mark -= base;
+    if (mark >= s.all) mark = __longlong_as_double(__double_as_longlong(s.all) - 1);    // (the sums of threads and of blocks are rounded apart)
+    if (s.before <= mark && mark < s.upto) {
+      double acc = s.before;
+      int token = -1;
+      float chosen = 0.0f;
+      walk([&](int i, float v) {
+        if (cut.found && v == cut.at) {
+          nth += 1.0;
+          if (nth > cut.ties) return true;
+        }
+        const double w = kept_weight(v);
+        if (w == 0.0) return true;
+        acc += w;
+        token = i;
+        chosen = v;
+        return acc <= mark;
+      });
+      p.token[row] = first + token;
+      if (p.logprob) p.logprob[row] = (float)((chosen == top ? 0.0 : ((double)chosen - (double)top) / (double)heat) - log(all_weights));
+    }
   }
   cluster.sync();                                  // nobody leaves while another block may read what it has
 }
@@ -609,9 +654,10 @@ extern "C" int32_t metis_sample(const metis_sample_args* a) {
   if (a->rows <= 0 || a->vocab <= 0 || (a->rows > 1 && a->ld < a->vocab)) return fail(METIS_ERR_BAD_SHAPE, "rows and vocab must be positive, rows of logits apart");
   if (a->vocab > METIS_SAMPLE_MAX_VOCAB) return fail(METIS_ERR_TOO_LARGE, "vocabularies have at most %d entries", METIS_SAMPLE_MAX_VOCAB);
   const bool half = a->dtype == METIS_DTYPE_BF16;
-  // A block for each 8192 entries up to eight of them: fewer entries for each are sooner done, more blocks wait longer for one another.
+  // A block for each 8192 entries up to eight of them while the GPU holds all rows at once (two blocks an SM); of more rows fewer and larger ones, of up to
+  // 96 KB each: few are sooner done, more blocks wait longer for one another.
   int blocks = 1;
-  while (blocks < kMaxCluster && a->vocab > (int64_t)blocks * 8192) blocks *= 2;
+  while (blocks < kMaxCluster && a->vocab > (int64_t)blocks * 8192 && (a->rows * blocks * 2 <= (int64_t)device_sm_count() * 2 || a->vocab > (int64_t)blocks * (half ? 49152 : 24576))) blocks *= 2;
   const int word = half ? 2 : 1;
   const int64_t each = (ceil_div(ceil_div(a->vocab, blocks), (int64_t)kThreads * word) | 1) * word;
   if (a->rows * blocks >= ((int64_t)1 << 31)) return fail(METIS_ERR_TOO_LARGE, "more rows than one launch takes");
