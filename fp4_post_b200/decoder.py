@@ -17,17 +17,22 @@ With `fuse_dense=True` what stays in bf16 runs on dense.py: the loss and `token_
 memory, and where o, gate and down are no Metis layers (target_modules of replace_linear_with_metis leaves them out) they have the
 activation, the product with `up` and the residual in their own kernels.  q/k/v and up, which nothing follows, stay torch's.
 A layer that has hooks is called like any module, and whatever has to see torch's operations gets them.
+
+With `fuse_rotary=True` queries and keys are turned by one kernel of rollout.py, forward and backward, with angles in fp32 in place of bf16 tables.
+`Decoder.generate` is the rollout: prompts are prefilled once, their pages forked for a group of answers each, and a decode step appends to
+the paged cache, attends over it and samples on kernels of that module, eagerly or as one CUDA graph.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn.functional as Fn
 from torch import nn
 from torch.autograd import forward_ad
 
-from fp4_post_b200 import dense, ops
+from fp4_post_b200 import dense, ops, rollout
 from fp4_post_b200.Metis.Metis.bitlinear import forward_group
 from fp4_post_b200.Metis.models.llama import RMSNorm
 
@@ -44,6 +49,9 @@ class DecoderConfig:
     rope_theta: float = 1e6
     eps: float = 1e-6
     qkv_bias: bool = True            # Qwen2: biases on q/k/v only
+    rope_scaling: Optional[dict] = None      # see rollout.rotary_frequencies
+    rotary_dim: Optional[int] = None         # elements of a head that turn (all)
+    rope_interleaved: bool = False           # pairs of neighbours in place of halves
 
     def linear_flops_per_token(self, rank: int) -> int:
         """Algorithmic forward flops of the Metis projections per token: 2 N K + 2 r (K + N) each."""
@@ -63,14 +71,26 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return x * cos + torch.cat((-x2, x1), dim=-1) * sin
 
 
-def _plain(*tensors) -> bool:
-    """Plain bf16 CUDA tensors of one device that only autograd follows: the library's own calls may take them.  Whatever has to see the
+def _rope_part(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """The same where pairs are neighbours, or a part of the head turns: the tables' width."""
+    front, rest = x[..., :cos.shape[-1]], x[..., cos.shape[-1]:]
+    if interleaved:
+        turned = torch.stack((-front[..., 1::2], front[..., ::2]), dim=-1).flatten(-2)
+        front = front * cos + turned * sin
+    else:
+        front = _rope(front, cos, sin)
+    return torch.cat((front, rest), dim=-1)
+
+
+def _plain(*tensors, dtypes=(torch.bfloat16,)) -> bool:
+    """Plain CUDA tensors of one device and type (bf16) that only autograd follows: the library's own calls may take them.  Whatever has to see the
     torch operations gets them: forward-mode derivatives (which no_grad leaves on), vmap and the other function transforms, tensor subclasses,
     dispatch modes, tracing."""
     first = tensors[0]
     return (not torch.jit.is_tracing() and not torch.compiler.is_compiling()
             and torch._C._functorch.peek_interpreter_stack() is None and torch._C._len_torch_dispatch_stack() == 0
-            and all(type(t) in (torch.Tensor, nn.Parameter) and t.is_cuda and t.dtype == torch.bfloat16 and t.device == first.device
+            and first.dtype in dtypes
+            and all(type(t) in (torch.Tensor, nn.Parameter) and t.is_cuda and t.dtype == first.dtype and t.device == first.device
                     and t.numel() > 0 and forward_ad.unpack_dual(t).tangent is None for t in tensors))
 
 
@@ -110,6 +130,41 @@ def _project(module: nn.Module, x: torch.Tensor, fuse: bool, *, activation=None,
     return y if residual is None else residual + y
 
 
+def _rotary_tables(cfg: DecoderConfig, T: int, device, dtype):
+    """cos and sin [1, 1, T, rotary_dim] of the configuration."""
+    d = cfg.head_dim if cfg.rotary_dim is None else cfg.rotary_dim
+    if cfg.rope_scaling is None:
+        inv, magnitude = 1.0 / (cfg.rope_theta ** (torch.arange(0, d, 2, device=device, dtype=torch.float32) / d)), 1.0
+    else:
+        scaled, magnitude = rollout.rotary_frequencies(d, cfg.rope_theta, cfg.rope_scaling)
+        inv = torch.tensor(scaled, device=device, dtype=torch.float32)
+    ang = torch.outer(torch.arange(T, device=device, dtype=torch.float32), inv)
+    ang = ang.repeat_interleave(2, dim=-1) if cfg.rope_interleaved else torch.cat((ang, ang), dim=-1)
+    cos, sin = ang.cos(), ang.sin()
+    if magnitude != 1.0:
+        cos, sin = cos * magnitude, sin * magnitude
+    return cos.to(dtype)[None, None], sin.to(dtype)[None, None]
+
+
+class _Cached:
+    """What a block's attention does in generate(), in the place of its tables: a layer of the cache, with the tokens' slots and positions.  A prompt's
+    tokens attend to one another (and are put into the cache), a new token to its sequence in the cache."""
+
+    def __init__(self, cache, layer, rotary, slots, positions, prompt):
+        self.cache, self.layer, self.rotary, self.slots, self.positions, self.prompt = cache, layer, rotary, slots, positions, prompt
+
+    def __call__(self, q, k, v):
+        """q [B, T, heads, head_dim], k and v [B, T, kv_heads, head_dim] -> [B, T, heads * head_dim]"""
+        B, T, H, D = q.shape
+        if self.prompt:
+            q, k = self.rotary(q, k)
+            self.cache.append(self.layer, None, k.flatten(0, 1), v.flatten(0, 1), self.slots, self.positions)
+            a = Fn.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True, enable_gqa=True)
+            return a.transpose(1, 2).reshape(B, T, H * D)
+        q = self.cache.append(self.layer, q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), self.slots, rotary=self.rotary)
+        return self.cache.attend(self.layer, q, self.slots).view(B, T, H * D)
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: DecoderConfig, fuse_dense: bool = False):
         super().__init__()
@@ -126,8 +181,19 @@ class Attention(nn.Module):
         q, k, v = forward_group((self.q_proj, self.k_proj, self.v_proj), h)     # one shared activation, three branches
         q = q.view(B, T, c.heads, c.head_dim)
         k = k.view(B, T, c.kv_heads, c.head_dim)
-        v = v.view(B, T, c.kv_heads, c.head_dim).transpose(1, 2)
-        if c.head_dim % 8 == 0 and _table_of(cos, T, c.head_dim) and _table_of(sin, T, c.head_dim) and _native(q, k, cos, sin):
+        v = v.view(B, T, c.kv_heads, c.head_dim)
+        if isinstance(cos, _Cached):
+            return _project(self.o_proj, cos(q, k, v), self.fuse_dense, residual=residual)
+        v = v.transpose(1, 2)
+        if isinstance(cos, rollout.Rotary):
+            if _plain(q, k, dtypes=(torch.bfloat16, torch.float32)):
+                q, k = (t.transpose(1, 2) for t in cos(q, k, sin))
+                a = Fn.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
+                return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, c.heads * c.head_dim), self.fuse_dense, residual=residual)
+            cos, sin = _rotary_tables(c, T, h.device, q.dtype)
+        if c.rope_interleaved or c.rotary_dim not in (None, c.head_dim):
+            q, k = _rope_part(q.transpose(1, 2), cos, sin, c.rope_interleaved), _rope_part(k.transpose(1, 2), cos, sin, c.rope_interleaved)
+        elif c.head_dim % 8 == 0 and _table_of(cos, T, c.head_dim) and _table_of(sin, T, c.head_dim) and _native(q, k, cos, sin):
             q, k = (t.transpose(1, 2) for t in ops.rope_pair(q, k, cos, sin))
         else:
             q, k = _rope(q.transpose(1, 2), cos, sin), _rope(k.transpose(1, 2), cos, sin)
@@ -181,26 +247,35 @@ class Block(nn.Module):
 
 
 class Decoder(nn.Module):
-    def __init__(self, cfg: DecoderConfig, fuse_norms: bool = True, fuse_dense: bool = False):
+    def __init__(self, cfg: DecoderConfig, fuse_norms: bool = True, fuse_dense: bool = False, fuse_rotary: bool = False):
         super().__init__()
         self.cfg = cfg
         self.fuse_dense = fuse_dense
+        self.fuse_rotary = fuse_rotary
+        self._rotaries = {}              # by device: the frequencies, no parameter of the model
         self.embed_tokens = nn.Embedding(cfg.vocab, cfg.hidden)
         self.layers = nn.ModuleList(Block(cfg, fuse_norms, fuse_dense) for _ in range(cfg.layers))
         self.norm = RMSNorm(cfg.hidden, cfg.eps)
         self.lm_head = nn.Linear(cfg.hidden, cfg.vocab, bias=False)      # stays bf16: not in the reference's target list
 
     def rotary(self, T: int, device, dtype):
-        d = self.cfg.head_dim
-        inv = 1.0 / (self.cfg.rope_theta ** (torch.arange(0, d, 2, device=device, dtype=torch.float32) / d))
-        ang = torch.outer(torch.arange(T, device=device, dtype=torch.float32), inv)
-        ang = torch.cat((ang, ang), dim=-1)
-        return ang.cos().to(dtype)[None, None], ang.sin().to(dtype)[None, None]
+        return _rotary_tables(self.cfg, T, device, dtype)
+
+    def _rotary_of(self, device: torch.device) -> rollout.Rotary:
+        """The configuration's rotary positions on a device, made once."""
+        c = self.cfg
+        r = self._rotaries.get(device)
+        if r is None:
+            r = self._rotaries[device] = rollout.Rotary(c.head_dim, theta=c.rope_theta, rotary_dim=c.rotary_dim, interleaved=c.rope_interleaved, scaling=c.rope_scaling, device=device)
+        return r
 
     def hidden(self, ids: torch.Tensor) -> torch.Tensor:
         """What the head reads: the normalised hidden states [B, T, hidden]."""
         x = self.embed_tokens(ids)
-        cos, sin = self.rotary(ids.shape[1], ids.device, x.dtype)
+        if self.fuse_rotary and self.cfg.head_dim % 8 == 0 and self.cfg.head_dim <= 256 and _plain(x, dtypes=(torch.bfloat16, torch.float32)):
+            cos, sin = self._rotary_of(x.device), None
+        else:
+            cos, sin = self.rotary(ids.shape[1], ids.device, x.dtype)
         for blk in self.layers:
             x = blk(x, cos, sin)
         return self.norm(x)
@@ -239,3 +314,101 @@ class Decoder(nn.Module):
         logp = torch.log_softmax(logits[:, :-1].float() / temperature, dim=-1)
         picked = logp.gather(-1, ids[:, 1:, None])[..., 0]
         return (picked, -(logp.detach().exp() * logp.detach()).sum(dim=-1)) if entropy else picked
+
+    @torch.no_grad()
+    def generate(self, ids: torch.Tensor, lengths=None, *, max_new_tokens: int, answers: int = 1, temperature=1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 eos: Optional[int] = None, generator: Optional[torch.Generator] = None, logprobs: bool = False, page_size: int = 16,
+                 cache_dtype: torch.dtype = torch.bfloat16, graphed: bool = False):
+        """`answers` sampled continuations of each prompt: tokens [B * answers, n <= max_new_tokens] (and their log-probabilities under the model at
+        that temperature, float32), the answers of a prompt behind one another.
+
+        ids [B, T] on the GPU, prompts padded behind their `lengths` (None: all T).  A prompt is prefilled once and its pages are shared by its answers;
+        keys and values are kept in bfloat16 or (cache_dtype) float8_e4m3fn.  eos ends an answer: what follows it is eos again, with log-probability 0,
+        and takes no more pages.  temperature, top_k, top_p, min_p: see rollout.sample; generator draws its random numbers.  graphed: the
+        decode step is captured after its first run and replayed (weights and what layers cache of them must not change meanwhile, shapes are fixed).
+        The model is bfloat16; rotary positions are formed in fp32, as fuse_rotary has them in forward()."""
+        c = self.cfg
+        if ids.dim() != 2 or ids.shape[0] == 0 or ids.shape[1] == 0:
+            raise ValueError(f"ids must be [prompts, tokens], not {tuple(ids.shape)}")
+        if not ids.is_cuda:
+            raise RuntimeError("generate() runs on a paged cache on the GPU: there is no CPU fallback")
+        if max_new_tokens < 1 or answers < 1:
+            raise ValueError("max_new_tokens and answers must be positive")
+        B, T = ids.shape
+        lengths = [T] * B if lengths is None else [int(n) for n in lengths]
+        if len(lengths) != B or min(lengths) < 1 or max(lengths) > T:
+            raise ValueError(f"lengths must be {B} numbers from 1 to {T}")
+        dev, rows = ids.device, B * answers
+        # a prompt's pages, and of each answer those behind the whole ones that it shares
+        whole = [n // page_size for n in lengths]
+        pages = sum(-(-n // page_size) for n in lengths) + answers * sum(-(-(n + max_new_tokens) // page_size) - w for n, w in zip(lengths, whole))
+        cache = rollout.PagedCache(c.layers, c.kv_heads, c.head_dim, pages=pages, sequences=B + rows, max_length=T + max_new_tokens, page_size=page_size,
+                                   dtype=cache_dtype, device=dev)
+        rotary = self._rotary_of(dev)
+        count = torch.tensor(lengths, dtype=torch.int64, device=dev)
+        prompts, slots = torch.arange(B, device=dev), torch.arange(B, B + rows, device=dev)
+
+        def run(x, place):
+            for i, blk in enumerate(self.layers):
+                x = blk(x, place(i), None)
+            return x
+
+        def pick(x, u):
+            logits = self.lm_head(self.norm(x))
+            if logits.dtype not in (torch.bfloat16, torch.float32):
+                logits = logits.float()
+            return rollout.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, logprobs=True)
+
+        # prompts: what is behind one belongs to no sequence
+        cache.reserve(prompts, count)
+        at = torch.arange(T, device=dev).expand(B, T)
+        owner = torch.where(at < count[:, None], prompts[:, None], -1).reshape(-1)
+        x = run(self.embed_tokens(ids), lambda i: _Cached(cache, i, rotary, owner, at.reshape(-1), True))
+        last = x[prompts, count - 1]
+        cache.fork(prompts.repeat_interleave(answers), slots)
+        cache.free(prompts)
+        draws = torch.rand(max_new_tokens, rows, device=dev, generator=generator)
+        tokens = torch.empty(max_new_tokens, rows, dtype=torch.int64, device=dev)
+        logp = torch.empty(max_new_tokens, rows, dtype=torch.float32, device=dev)
+        token, p = pick(last.repeat_interleave(answers, dim=0), draws[0])
+        tokens[0], logp[0] = token, p
+        live = slots.clone()
+        u = draws[0].clone()
+
+        def step():
+            if eos is not None:
+                live.masked_fill_(token == eos, -1)
+            cache.reserve(live, 1)
+            x = run(self.embed_tokens(token.clamp(min=0))[:, None], lambda i: _Cached(cache, i, rotary, live, None, False))
+            new, p = pick(x[:, 0], u)
+            if eos is not None:
+                done = live < 0
+                new, p = new.masked_fill(done, eos), p.masked_fill(done, 0.0)
+            token.copy_(new)
+            return p
+
+        graph, n = None, 1
+        while n < max_new_tokens:
+            u.copy_(draws[n])
+            if graph is not None:
+                graph.replay()
+            elif graphed and n == 2:
+                # (the first step has run as it is: what a capture must not do for the first time is done)
+                from fp4_post_b200.graphs import _capture_stream
+                torch.cuda.synchronize(dev)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.device(dev), torch.cuda.graph(graph, stream=_capture_stream()):
+                    p = step()
+                graph.replay()
+            else:
+                p = step()
+            tokens[n], logp[n] = token, p
+            n += 1
+            if eos is not None and n % 32 == 0 and bool(((token == eos) | (live < 0)).all()):
+                break
+        cache.check()
+        if graph is not None:
+            torch.cuda.synchronize(dev)
+            graph.reset()
+        tokens, logp = tokens[:n].t().contiguous(), logp[:n].t().contiguous()
+        return (tokens, logp) if logprobs else tokens

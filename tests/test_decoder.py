@@ -62,3 +62,39 @@ def test_fake_tensors_go_through_the_torch_expressions():
             assert x.is_cuda and block(x, table, table).shape == x.shape
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+def test_rotary_options_on_the_cpu():
+    """Neighbouring pairs, a part of the head and scaled frequencies against the definition pair by pair."""
+    import math
+
+    from fp4_post_b200 import rollout
+    from fp4_post_b200.decoder import _rope_part, _rotary_tables
+    scaling = dict(type="yarn", factor=4.0, original_max_position=64)
+    for interleaved in (False, True):
+        for rotary_dim in (16, 6):
+            cfg = DecoderConfig(hidden=64, layers=1, heads=4, kv_heads=2, head_dim=16, ffn=128, vocab=97, rope_theta=1e4, rope_scaling=scaling, rotary_dim=rotary_dim, rope_interleaved=interleaved)
+            freq, m = rollout.rotary_frequencies(rotary_dim, 1e4, scaling)
+            x = torch.randn(2, 4, 5, 16, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+            got = _rope_part(x, *_rotary_tables(cfg, 5, "cpu", torch.float64), interleaved)
+            want = x.clone()
+            for t in range(5):
+                for i, f in enumerate(freq):
+                    a, b = (2 * i, 2 * i + 1) if interleaved else (i, rotary_dim // 2 + i)
+                    c, s = m * math.cos(t * f), m * math.sin(t * f)
+                    want[:, :, t, a] = x[:, :, t, a] * c - x[:, :, t, b] * s
+                    want[:, :, t, b] = x[:, :, t, b] * c + x[:, :, t, a] * s
+            torch.testing.assert_close(got, want, rtol=1e-6, atol=1e-6)        # (angles in fp32)
+            model = Decoder(cfg)
+            assert torch.isfinite(model(torch.randint(0, 97, (2, 5)))).all()
+            model.load_state_dict(Decoder(cfg, fuse_rotary=True).state_dict())
+
+
+def test_generate_refuses_without_a_device():
+    import pytest
+    model = Decoder(TINY, fuse_rotary=True)
+    assert model(torch.randint(0, 97, (2, 5))).shape == (2, 5, 97)             # (the tables, on the CPU)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        model.generate(torch.zeros(1, 4, dtype=torch.long), max_new_tokens=2)
+    with pytest.raises(ValueError):
+        model.generate(torch.zeros(4, dtype=torch.long), max_new_tokens=2)
