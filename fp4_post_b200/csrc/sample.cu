@@ -342,19 +342,30 @@ struct Row {
   __device__ bool by_values(int64_t k, double top_p, Cut& c, double& all_weights) {
     const Values b = values((int)key_of<16>(top));
     clear();
-    double extra = 0.0;                            // weights in the bins of several values: the small ones', and behind them the last one's
+    double extra = 0.0;                            // weights in the bins of several values: the last one's, and the small ones'
     double extra_small = 0.0;
-    const int small_bin = b.has_small ? b.small : -1;
+    // Two elements at a time: their keys are at most the largest one's, so that one subtraction serves both.  Those in bins of several values, and -inf
+    // (which is in no bin), are found by comparing the values and go one by one.
+    const uint32_t top2 = (uint32_t)b.top * 0x10001u, small2 = (uint32_t)b.small * 0x10001u, gap2 = (uint32_t)b.gap * 0x10001u;
+    const int last_key = b.top - (kValues - 1) - (kValues - 1 > b.small ? b.gap : 0);
+    const __nv_bfloat162 last_value = __float2bfloat162_rn(value_of<16>((uint32_t)max(last_key, (int)kLowest16))), tiny = __float2bfloat162_rn(b.has_small ? 0x1p-8f : 0.0f);
     each_word([&](uint32_t w) {
-      const uint32_t two = S::keys(w);
+      const uint32_t d = top2 - S::keys(w), bin = __vmaxu2(__vminu2(d, small2), __vmaxu2(d, gap2) - gap2);
+      const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&w);
+      const uint32_t far = __hle2_mask(v, last_value), small = __hlt2_mask(__habs2(v), tiny);
+      if ((far | small) == 0u) {
+        atomicAdd(&sh.bins[bin & 0xffffu], 1u);
+        atomicAdd(&sh.bins[bin >> 16], 1u);
+        return;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = (int)(h ? two >> 16 : two & 0xffffu), d = b.top - key;
-        const int bin = min(max(min(d, b.small), d - b.gap), kValues - 1);
-        if (key == (int)kLowest16) continue;
-        atomicAdd(&sh.bins[bin], 1u);
-        if (bin == kValues - 1) extra += (double)weight(S::value(w, h));
-        else if (bin == small_bin) extra_small += (double)weight(S::value(w, h));
+        const float x_h = S::value(w, h);
+        const uint32_t half = 0xffffu << (16 * h);
+        if (x_h == -CUDART_INF_F) continue;
+        atomicAdd(&sh.bins[(far & half) ? kValues - 1 : (bin & half) >> (16 * h)], 1u);
+        if (far & half) extra += (double)weight(x_h);
+        else if (small & half) extra_small += (double)weight(x_h);
       }
     });
     // (sums of nothing, mostly)
@@ -577,22 +588,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const float w = r.weight(v);
     return w >= min_p ? (double)w : 0.0;
   };
-  // those above the cut, summed, and those that equal it, counted; all lanes go the same way
+  // those above the cut, summed, and those that equal it, counted
   double sum = 0.0;
   int32_t equal = 0;
+  auto count_in = [&](float v) {
+    if (cut.found && v == cut.at) ++equal; else sum += kept_weight(v);
+  };
+  if (sizeof(T) == 2 && cut.found) {
+    // Few are kept, and not the same ones in all lanes: 32 elements are compared first, two at a time into the bits of two words, and the lanes
+    // then go through theirs (lanes that went through all elements together took 22 thousand cycles of a row's 80).
+    const __nv_bfloat162 from_two = __float2bfloat162_rn(from_value);
+    const uint16_t* const mine = reinterpret_cast<const uint16_t*>(x + from_word);
+    for (int w = 0; w < words; w += 16) {
+      uint32_t in[2] = {0u, 0u};                   // of word j: bit 2 j for its low half, 17 + 2 j for the other
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (w + j < words) {
+          const uint32_t v = x[from_word + w + j];
+          in[j / 8] |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&v), from_two) & (0x00020001u << (2 * (j % 8)));
+        }
+      while (in[0] | in[1]) {
+        const bool second = in[0] == 0u;
+        const uint32_t bits = second ? in[1] : in[0], rest = bits & (bits - 1u);
+        const int at = __ffs(bits) - 1, element = (at & 15) + (second ? 16 : 0);         // (17 + 2 j, less 16, is 2 j + 1)
+        if (second) in[1] = rest; else in[0] = rest;
+        count_in(__uint_as_float((uint32_t)mine[2 * w + element] << 16));
+      }
+    }
+  } else {
 #pragma unroll 4
-  for (int w = from_word; w < from_word + words; ++w) {
-    const uint32_t v = x[w];
-    bool in = false;
+    for (int w = from_word; w < from_word + words; ++w) {
+      const uint32_t v = x[w];
 #pragma unroll
-    for (int h = 0; h < S::kWord; ++h) in |= S::value(v, h) >= from_value;
-    if (!__any_sync(0xffffffffu, in)) continue;
-#pragma unroll
-    for (int h = 0; h < S::kWord; ++h) {
-      const float value = S::value(v, h);
-      const bool tie = cut.found && value == cut.at;
-      equal += tie;
-      sum += value >= from_value && !tie ? kept_weight(value) : 0.0;
+      for (int h = 0; h < S::kWord; ++h)
+        if (S::value(v, h) >= from_value) count_in(S::value(v, h));
     }
   }
   // Which block has the mark goes by the blocks' sums, the same numbers in all of them; there, a thread by its own.
