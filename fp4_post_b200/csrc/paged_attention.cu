@@ -202,55 +202,6 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     const int first_head = head * p.group + chunk * 8 * NT, live = min(8 * NT, p.group - chunk * 8 * NT);
     const float k_scale = p.scales ? p.scales[head] : 1.0f, v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
 
-    // ---- queries as the columns of a product: of step i, elements 16 i + 2 t and + 8 of head g (e4m3: in the order in which the keys come) ----
-    uint32_t q[NT][D / 16][2];
-    float q_scale[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool there = n * 8 + g < live;
-      const __nv_bfloat16* x = p.q + (int64_t)row * p.q_row + (int64_t)(first_head + n * 8 + g) * p.q_head;
-      float biggest = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int e = i * 16 + (kE4m3 ? 4 * t + 2 * j : 2 * t + 8 * j);
-          q[n][i][j] = there && e < p.head_dim ? *reinterpret_cast<const uint32_t*>(x + e) : 0u;
-          if constexpr (kE4m3) biggest = fmaxf(biggest, fmaxf(fabsf(bf16_lo(q[n][i][j])), fabsf(bf16_hi(q[n][i][j]))));
-        }
-      q_scale[n] = 1.0f;
-      if constexpr (kE4m3) {
-        // fp16 holds a row of bf16 exactly where it is brought to [1, 2) by a power of two; what lies 2^14 below the row's largest element
-        // loses bits that are 2^-25 of that one.  (Infinite and NaN rows stay what they are.)
-        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 1));
-        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 2));
-        const int e = min(max((int)((__float_as_uint(biggest) >> 23) & 255u), 2), 252);
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) q[n][i][j] = bits(__floats2half2_rn(bf16_lo(q[n][i][j]) * down, bf16_hi(q[n][i][j]) * down));
-        q_scale[n] = __uint_as_float((uint32_t)e << 23);
-      }
-    }
-    // what scores of the columns 2 t and 2 t + 1 are multiplied by
-    float s_scale[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) s_scale[n][j] = p.scale * k_scale * (kE4m3 ? __shfl_sync(0xffffffffu, q_scale[n], (2 * t + j) * 4) : 1.0f);
-
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
-      m[n][0] = m[n][1] = kNone;
-      l[n][0] = l[n][1] = 0.0f;
-    }
-
     // ---- the warp's tiles: begin + warp, and every fourth from there ----
     const int first = begin + warp, tiles_end = stop, keys_all = length_of[row];
     const int mine_count = first < tiles_end ? (tiles_end - first + kWarps - 1) / kWarps : 0;
@@ -321,6 +272,55 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     };
 #pragma unroll
     for (int i = 0; i < L::kStages - 1; ++i) fetch();
+
+    // ---- queries (behind the first copies, which take longer) as the columns of a product: of step i, elements 16 i + 2 t and + 8 of head g (e4m3: in the order in which the keys come) ----
+    uint32_t q[NT][D / 16][2];
+    float q_scale[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool there = n * 8 + g < live;
+      const __nv_bfloat16* x = p.q + (int64_t)row * p.q_row + (int64_t)(first_head + n * 8 + g) * p.q_head;
+      float biggest = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int e = i * 16 + (kE4m3 ? 4 * t + 2 * j : 2 * t + 8 * j);
+          q[n][i][j] = there && e < p.head_dim ? *reinterpret_cast<const uint32_t*>(x + e) : 0u;
+          if constexpr (kE4m3) biggest = fmaxf(biggest, fmaxf(fabsf(bf16_lo(q[n][i][j])), fabsf(bf16_hi(q[n][i][j]))));
+        }
+      q_scale[n] = 1.0f;
+      if constexpr (kE4m3) {
+        // fp16 holds a row of bf16 exactly where it is brought to [1, 2) by a power of two; what lies 2^14 below the row's largest element
+        // loses bits that are 2^-25 of that one.  (Infinite and NaN rows stay what they are.)
+        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 1));
+        biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, 2));
+        const int e = min(max((int)((__float_as_uint(biggest) >> 23) & 255u), 2), 252);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) q[n][i][j] = bits(__floats2half2_rn(bf16_lo(q[n][i][j]) * down, bf16_hi(q[n][i][j]) * down));
+        q_scale[n] = __uint_as_float((uint32_t)e << 23);
+      }
+    }
+    // what scores of the columns 2 t and 2 t + 1 are multiplied by
+    float s_scale[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s_scale[n][j] = p.scale * k_scale * (kE4m3 ? __shfl_sync(0xffffffffu, q_scale[n], (2 * t + j) * 4) : 1.0f);
+
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+      m[n][0] = m[n][1] = kNone;
+      l[n][0] = l[n][1] = 0.0f;
+    }
 
     const uint32_t k_base = piece_base<L::kRowBytes>(lane & 15, lane >> 4);
     const uint32_t v_base = kE4m3 ? k_base : piece_base<L::kRowBytes>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
@@ -465,7 +465,6 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     }
     copies_wait<0>();
     __syncwarp();
-
     // ---- join the warps; element of o[n][i]: c0, c1 of row g, c2, c3 of row g + 8 of the output's 16 i, columns 2 t, 2 t + 1 ----
     float* const left_o = reinterpret_cast<float*>(mine);
 #pragma unroll
@@ -521,11 +520,14 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
 }
 
 // Joins the pieces of a unit that several blocks wrote, for one query head of the group.  A warp takes every eighth piece, a lane D / 32 elements.
-template <int D, int NT>
-__global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
+// kMany pieces (few units, so that there are few blocks): a lane looks at one piece's maximum and sum, and eight outputs are on their way at once; else
+// fewer registers, so that an SM takes twice the blocks, most of which have nothing to do.  32768 keys of one row, 111 pieces: 21.5 us with, 23.0
+// without; 256 rows in two or three pieces: 57.9 with, 54.5 without.
+template <int D, int NT, bool kMany>
+__global__ void __launch_bounds__(256, kMany ? 4 : 8) join_kernel(const AttendParams p) {
   constexpr int E = D / 32;
   __shared__ float acc_of[8][D];
-  __shared__ float2 ml_of[8];
+  __shared__ float sum_of[8];
   grid_dependency_wait();
   const int4 job = p.join[blockIdx.x];
   if (job.x < 0) return;
@@ -542,24 +544,45 @@ __global__ void __launch_bounds__(256) join_kernel(const AttendParams p) {
   float acc[E], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (int i = warp; i < pieces; i += 8) {
-    const int64_t at = place(i);
-    const float2 ml = p.part_ml[at];
-    const float f = exp2_fast(ml.x - top);
-    sum += ml.y * f;
+  if constexpr (kMany) {
+    const int mine = (pieces - warp + 7) / 8;
+    for (int base = 0; base < mine; base += 32) {
+      // a lane has the maximum and sum of one piece, all lanes then go through the outputs of 32
+      const int own = (base + lane) * 8 + warp;
+      const float2 ml = own < pieces ? p.part_ml[place(own)] : make_float2(kNone, 0.0f);
+      const float f = own < pieces ? exp2_fast(ml.x - top) : 0.0f;
+      sum += ml.y * f;
+      const int here = min(32, mine - base);
+#pragma unroll 8
+      for (int j = 0; j < here; ++j) {
+        const float* from = p.part_o + place((base + j) * 8 + warp) * D + lane;
+        const float fj = __shfl_sync(0xffffffffu, f, j);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += p.part_o[at * D + e * 32 + lane] * f;
+        for (int e = 0; e < E; ++e) acc[e] += from[e * 32] * fj;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  } else {
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += 8) {
+      const int64_t at = place(i);
+      const float2 ml = p.part_ml[at];
+      const float f = exp2_fast(ml.x - top);
+      sum += ml.y * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += p.part_o[at * D + e * 32 + lane] * f;
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) acc_of[warp][e * 32 + lane] = acc[e];
-  if (lane == 0) ml_of[warp] = make_float2(0.0f, sum);
+  if (lane == 0) sum_of[warp] = sum;
   __syncthreads();
   const int64_t to = (int64_t)job.x * p.heads_q + head * p.group + chunk * 8 * NT + column;
   const float v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
   float all = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) all += ml_of[w].y;
+  for (int w = 0; w < 8; ++w) all += sum_of[w];
   for (int e = threadIdx.x; e < p.head_dim; e += 256) {
     float a = 0.0f;
 #pragma unroll
@@ -600,7 +623,8 @@ struct Launch {
     p.part_o = reinterpret_cast<float*>(w + n * (16 + 16 * NT * 8));
     METIS_CUDA_OK(launch_overlapped(kLaunchShort, attend_kernel<D, NT, kE4m3>, dim3((unsigned)n), dim3(kThreads), L::kSmem, st, p));
     const int64_t joins = p.by_unit ? units : n;
-    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT>, dim3((unsigned)joins, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
+    const auto join = p.by_unit && units * 8 <= n ? join_kernel<D, NT, true> : join_kernel<D, NT, false>;
+    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join, dim3((unsigned)joins, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
     count_rollout_launches(2);
     return METIS_OK;
   }

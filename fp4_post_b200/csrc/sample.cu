@@ -371,8 +371,10 @@ struct Row {
     // (sums of nothing, mostly)
     double rest = 0.0, small = 0.0;
     if (__syncthreads_or(extra != 0.0 || extra_small != 0.0)) {
-      rest = block_scan<kThreads>(extra, sh.sums).all;
-      small = block_scan<kThreads>(extra_small, sh.sums).all;
+      Scan<double> of_rest, of_small;
+      block_scan_two<kThreads>(extra, extra_small, sh.sums, sh.more_sums, of_rest, of_small);
+      rest = of_rest.all;
+      small = of_small.all;
     }
     {
       const double (*g)[2] = gather(rest, small);  // (and the counts are there)
