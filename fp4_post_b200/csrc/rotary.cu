@@ -27,8 +27,7 @@ struct RotaryShape {
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int kWide = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&v)[8]) {
     v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
     v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
   }
@@ -46,9 +45,8 @@ template <> struct Vec<__nv_bfloat16> {
 };
 template <> struct Vec<float> {
   static constexpr int kWide = 4;
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 w = *reinterpret_cast<const float4*>(p);
-    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&v)[4]) {
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
@@ -63,48 +61,85 @@ __device__ __forceinline__ float2 cos_sin(uint64_t turn, int64_t position, const
   return make_float2(cs * s.magnitude, sn * s.magnitude * s.sign);
 }
 
-// One unit of a head: the two pieces of W elements (half layout), one piece of W elements (neighbouring pairs; c[] by pairs), or W elements that
-// are copied.  kPair: W = 1, the elements of one pair.
+// A unit of a head: the two pieces of W elements of the half layout, one piece of W elements of neighbouring pairs, with W = 1 the two elements of a
+// pair.  What does not turn goes in units of the same kind: two pieces behind one another (the last one twice where there is an odd one) or one.
+// Where they are is the same in all heads, and nothing branches: the arrays of a batch have to stay in registers.
+template <int W, bool kInterleaved> __host__ __device__ constexpr bool two_pieces() { return W == 1 || !kInterleaved; }
+struct Unit {
+  int at, bt;
+  bool turns;
+};
+template <int W, bool kInterleaved>
+__device__ __forceinline__ Unit unit_of(int unit, const RotaryShape& s) {
+  constexpr bool kTwo = two_pieces<W, kInterleaved>();
+  if (unit >= s.rotary_units) {
+    const int at = s.rotary_dim + (unit - s.rotary_units) * W * (kTwo ? 2 : 1);
+    return {at, min(at + W, s.head_dim - W), false};
+  }
+  if (W == 1 && kInterleaved) return {2 * unit, 2 * unit + 1, true};
+  return {unit * W, unit * W + s.rotary_dim / 2, true};
+}
+template <typename T, int W, bool kTwo>
+struct Raw {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const T* x, const Unit& u) {
+    a = *reinterpret_cast<const uint4*>(x + u.at);
+    if constexpr (kTwo) b = *reinterpret_cast<const uint4*>(x + u.bt);
+  }
+};
+template <typename T>
+struct Raw<T, 1, true> {
+  float a, b;
+  __device__ __forceinline__ void load(const T* x, const Unit& u) {
+    a = Vec<T>::one(x + u.at);
+    b = Vec<T>::one(x + u.bt);
+  }
+};
 template <typename T, int W, bool kInterleaved, typename Put>
-__device__ __forceinline__ void turn_unit(const T* x, int unit, const float2 (&c)[W], const RotaryShape& s, bool turns, const Put& put) {
+__device__ __forceinline__ void turn_unit(const Raw<T, W, two_pieces<W, kInterleaved>()>& r, const Unit& at, const float2 (&c)[W], const Put& put) {
   if constexpr (W == 1) {
-    if (!turns) {
-      put.one(s.rotary_dim + unit - s.rotary_units, Vec<T>::one(x + s.rotary_dim + unit - s.rotary_units));
-      return;
-    }
-    const int i = kInterleaved ? 2 * unit : unit, j = kInterleaved ? 2 * unit + 1 : unit + s.rotary_dim / 2;
-    const float a = Vec<T>::one(x + i), b = Vec<T>::one(x + j);
-    put.one(i, fmaf(a, c[0].x, -b * c[0].y));
-    put.one(j, fmaf(b, c[0].x, a * c[0].y));
+    put.one(at.at, at.turns ? fmaf(r.a, c[0].x, -r.b * c[0].y) : r.a);
+    put.one(at.bt, at.turns ? fmaf(r.b, c[0].x, r.a * c[0].y) : r.b);
   } else {
     float a[W];
-    if (!turns) {
-      const int at = s.rotary_dim + (unit - s.rotary_units) * W;
-      Vec<T>::load(x + at, a);
-      put.wide(at, a);
-    } else if constexpr (kInterleaved) {
-      Vec<T>::load(x + unit * W, a);
+    Vec<T>::unpack(r.a, a);
+    if constexpr (kInterleaved) {
 #pragma unroll
       for (int i = 0; i < W; i += 2) {
         const float u = a[i], v = a[i + 1];
-        a[i] = fmaf(u, c[i / 2].x, -v * c[i / 2].y);
-        a[i + 1] = fmaf(v, c[i / 2].x, u * c[i / 2].y);
+        a[i] = at.turns ? fmaf(u, c[i / 2].x, -v * c[i / 2].y) : u;
+        a[i + 1] = at.turns ? fmaf(v, c[i / 2].x, u * c[i / 2].y) : v;
       }
-      put.wide(unit * W, a);
+      put.wide(at.at, a);
     } else {
       float b[W];
-      const int at = unit * W, bt = at + s.rotary_dim / 2;
-      Vec<T>::load(x + at, a);
-      Vec<T>::load(x + bt, b);
+      Vec<T>::unpack(r.b, b);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float u = a[i], v = b[i];
-        a[i] = fmaf(u, c[i].x, -v * c[i].y);
-        b[i] = fmaf(v, c[i].x, u * c[i].y);
+        a[i] = at.turns ? fmaf(u, c[i].x, -v * c[i].y) : u;
+        b[i] = at.turns ? fmaf(v, c[i].x, u * c[i].y) : v;
       }
-      put.wide(at, a);
-      put.wide(bt, b);
+      put.wide(at.at, a);
+      put.wide(at.bt, b);
     }
+  }
+}
+// Heads of one token, kPieces pieces read before the first is written (outputs might be inputs, for all that the compiler knows, and each load would
+// wait for the store before it).  Behind the last head the last is read again, and not written.  Four pieces and four blocks an SM: 8192 tokens of 28 + 4
+// heads 26.2 -> 23.9 us, pairs of neighbours 33.6 -> 26.1; eight and three: 27.3 and 27.1.  Appending, which has keys and values on their way as well, takes eight
+// and three (50.4 us for the padded prompts, 52.1 with four).
+template <typename T, int W, bool kInterleaved, int kPieces, typename MakePut>
+__device__ __forceinline__ void turn_heads(const T* x, int64_t head_stride, int lane, int heads, int lanes, const Unit& at, const float2 (&c)[W], const MakePut& put_of) {
+  constexpr bool kTwo = two_pieces<W, kInterleaved>();
+  constexpr int kBatch = kTwo ? kPieces / 2 : kPieces;
+  for (int h = lane; h < heads; h += kBatch * lanes) {
+    Raw<T, W, kTwo> r[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) r[i].load(x + min(h + i * lanes, heads - 1) * head_stride, at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (h + i * lanes < heads) turn_unit<T, W, kInterleaved>(r[i], at, c, put_of(h + i * lanes));
   }
 }
 
@@ -150,22 +185,19 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryTensors
   __syncthreads();
   const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
   const int lane = rest % s.head_lanes;
-  const bool turns = unit < s.rotary_units;
+  const Unit at_unit = unit_of<W, kInterleaved>(unit, s);
   if (rest >= s.head_lanes * s.block_tokens) return;
   for (int token = rest / s.head_lanes; token < here; token += s.block_tokens) {
     float2 c[W];
-    unit_table<W, kInterleaved>(table, token, unit, pairs, turns, c);
+    unit_table<W, kInterleaved>(table, token, unit, pairs, at_unit.turns, c);
     const int64_t at = first + token, outer = at / t.inner, inner = at - outer * t.inner;
     const T* q = static_cast<const T*>(t.q) + outer * t.q_outer + inner * t.q_token;
     T* q_out = static_cast<T*>(t.q_out) + at * s.heads_q * s.head_dim;
-#pragma unroll 8
-    for (int h = lane; h < s.heads_q; h += s.head_lanes)
-      turn_unit<T, W, kInterleaved>(q + h * t.q_head, unit, c, s, turns, PutDense<T>{q_out + (int64_t)h * s.head_dim});
+    turn_heads<T, W, kInterleaved, 4>(q, t.q_head, lane, s.heads_q, s.head_lanes, at_unit, c, [&](int h) { return PutDense<T>{q_out + (int64_t)h * s.head_dim}; });
     if (s.heads_k == 0) continue;
     const T* k = static_cast<const T*>(t.k) + outer * t.k_outer + inner * t.k_token;
     T* k_out = static_cast<T*>(t.k_out) + at * s.heads_k * s.head_dim;
-    for (int h = lane; h < s.heads_k; h += s.head_lanes)
-      turn_unit<T, W, kInterleaved>(k + h * t.k_head, unit, c, s, turns, PutDense<T>{k_out + (int64_t)h * s.head_dim});
+    turn_heads<T, W, kInterleaved, 4>(k, t.k_head, lane, s.heads_k, s.head_lanes, at_unit, c, [&](int h) { return PutDense<T>{k_out + (int64_t)h * s.head_dim}; });
   }
 }
 
@@ -211,7 +243,7 @@ template <> struct PutCache<true> {
 
 // One block takes tokens, and the heads of q, k and v of each, as rotary_kernel does.  What a token goes to is looked up once, by one thread.
 template <int W, bool kInterleaved, bool kE4m3>
-__global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendTensors t, const RotaryShape s) {
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendTensors t, const RotaryShape s) {
   extern __shared__ float2 table[];
   int64_t* const token_at = reinterpret_cast<int64_t*>(table + s.span * (s.rotary_dim / 2));      // bytes from layer_pool to the token's row in the keys of head 0, -1: nowhere, -2: no sequence
   int64_t* const token_position = token_at + s.span;
@@ -243,13 +275,13 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendTensors
   __syncthreads();
   const int unit = threadIdx.x % s.units, rest = threadIdx.x / s.units;
   const int lane = rest % s.head_lanes;
-  const bool turns = unit < s.rotary_units;
+  const Unit at_unit = unit_of<W, kInterleaved>(unit, s);
   if (rest >= s.head_lanes * s.block_tokens) return;
   using Out = std::conditional_t<kE4m3, uint8_t, __nv_bfloat16>;
   const int64_t head_bytes = (int64_t)c.page_size * c.head_dim * c.item, values = c.kv_heads * head_bytes;
   for (int token = rest / s.head_lanes; token < here; token += s.block_tokens) {
     float2 cs[W];
-    unit_table<W, kInterleaved>(table, token, unit, pairs, turns, cs);
+    unit_table<W, kInterleaved>(table, token, unit, pairs, at_unit.turns, cs);
     const int64_t i = first + token, at = token_at[token];
     __nv_bfloat16* q_out = t.q_out + i * s.heads_q * s.head_dim;
     if (at == -2) {
@@ -264,29 +296,25 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendTensors
       }
       continue;
     }
-    const __nv_bfloat16* q = t.q + i * t.q_token;
-#pragma unroll 8
-    for (int h = lane; h < s.heads_q; h += s.head_lanes)
-      turn_unit<__nv_bfloat16, W, kInterleaved>(q + h * t.q_head, unit, cs, s, turns, PutDense<__nv_bfloat16>{q_out + (int64_t)h * s.head_dim});
-    if (at < 0) continue;
+    using B = __nv_bfloat16;
+    constexpr bool kTwo = two_pieces<W, kInterleaved>();
+    // The lane's first key and value are on their way while the queries are turned.  Values go by the keys' units, in pieces behind one another.
+    const B *k = t.k + i * t.k_token, *v = t.v + i * t.v_token;
+    const bool written = at >= 0 && lane < c.kv_heads;
+    const int v_at = unit * W * (kTwo ? 2 : 1);
+    const Unit v_unit = {min(v_at, s.head_dim - W), min(v_at + W, s.head_dim - W), false};
+    Raw<B, W, kTwo> k_first, v_first;
+    k_first.load(k + min(lane, c.kv_heads - 1) * t.k_head, at_unit);
+    v_first.load(v + min(lane, c.kv_heads - 1) * t.v_head, v_unit);
+    turn_heads<B, W, kInterleaved, 8>(t.q + i * t.q_token, t.q_head, lane, s.heads_q, s.head_lanes, at_unit, cs, [&](int h) { return PutDense<B>{q_out + (int64_t)h * s.head_dim}; });
+    if (!written) continue;
     char* const row = t.layer_pool + at;
-    const __nv_bfloat16 *k = t.k + i * t.k_token, *v = t.v + i * t.v_token;
-    for (int h = lane; h < c.kv_heads; h += s.head_lanes)
-      turn_unit<__nv_bfloat16, W, kInterleaved>(k + h * t.k_head, unit, cs, s, turns,
-                                                PutCache<kE4m3>{reinterpret_cast<Out*>(row + h * head_bytes), kE4m3 ? t.scales[h] : 1.0f});
-    for (int h = lane; h < c.kv_heads; h += s.head_lanes) {
-      const __nv_bfloat16* x = v + h * t.v_head;
-      const PutCache<kE4m3> put{reinterpret_cast<Out*>(row + values + h * head_bytes), kE4m3 ? t.scales[c.kv_heads + h] : 1.0f};
-      if constexpr (W == 1) {
-        for (int e = unit; e < s.head_dim; e += s.units) put.one(e, Vec<__nv_bfloat16>::one(x + e));
-      } else {
-        for (int e = unit; e < s.head_dim / W; e += s.units) {
-          float a[W];
-          Vec<__nv_bfloat16>::load(x + e * W, a);
-          put.wide(e * W, a);
-        }
-      }
-    }
+    auto put_key = [&](int h) { return PutCache<kE4m3>{reinterpret_cast<Out*>(row + h * head_bytes), kE4m3 ? t.scales[h] : 1.0f}; };
+    auto put_value = [&](int h) { return PutCache<kE4m3>{reinterpret_cast<Out*>(row + values + h * head_bytes), kE4m3 ? t.scales[c.kv_heads + h] : 1.0f}; };
+    turn_unit<B, W, kInterleaved>(k_first, at_unit, cs, put_key(lane));
+    turn_unit<B, W, kInterleaved>(v_first, v_unit, cs, put_value(lane));
+    turn_heads<B, W, kInterleaved, 8>(k, t.k_head, lane + s.head_lanes, c.kv_heads, s.head_lanes, at_unit, cs, put_key);
+    turn_heads<B, W, kInterleaved, 8>(v, t.v_head, lane + s.head_lanes, c.kv_heads, s.head_lanes, v_unit, cs, put_value);
   }
 }
 
@@ -296,7 +324,8 @@ RotaryShape rotary_shape(int64_t tokens, int heads_q, int heads_k, int head_dim,
   RotaryShape s = {};
   s.heads_q = heads_q; s.heads_k = heads_k; s.head_dim = head_dim; s.rotary_dim = rotary_dim;
   s.rotary_units = wide == 1 ? rotary_dim / 2 : interleaved ? rotary_dim / wide : rotary_dim / 2 / wide;
-  s.units = s.rotary_units + (head_dim - rotary_dim) / wide;
+  const int pieces = (head_dim - rotary_dim) / wide;                      // that do not turn
+  s.units = s.rotary_units + (wide == 1 || !interleaved ? (pieces + 1) / 2 : pieces);
   const int rest = kThreads / s.units, heads = heads_q > heads_k ? heads_q : heads_k;
   const int64_t enough = (int64_t)device_sm_count() * 512;
   int lanes = 1;
@@ -306,12 +335,13 @@ RotaryShape rotary_shape(int64_t tokens, int heads_q, int heads_k, int head_dim,
   return s;
 }
 
-// How many tokens a block takes in all: one wave of blocks where their tables of cosines (and what else a token needs) allow it.  1024 blocks of 8 tokens
-// were 1.4 waves, and 8192 tokens of 28 + 4 heads took 27.6 us.
-int32_t set_span(RotaryShape& s, int64_t tokens, const void* kernel, int token_bytes) {
+// How many tokens a block takes in all: so many waves of blocks where their tables of cosines (and what else a token needs) allow it.  One for tokens that are
+// all alike (1024 blocks of 8 tokens were 1.4 waves); four where a third of them, the padding of a batch, has next to nothing to do (16 prompts of 256
+// to 1024 tokens into e4m3: 54.9 us by one wave, 50.7 by four).
+int32_t set_span(RotaryShape& s, int64_t tokens, const void* kernel, int token_bytes, int waves) {
   const int bytes = s.rotary_dim / 2 * (int)sizeof(float2) + token_bytes;
   const int64_t most = bytes > 0 ? 40960 / bytes : 1 << 20;
-  const int64_t resident = (int64_t)device_sm_count() * resident_ctas(kernel, kThreads, 16384);
+  const int64_t resident = (int64_t)device_sm_count() * resident_ctas(kernel, kThreads, 16384) * waves;
   int64_t span = ceil_div(ceil_div(tokens, resident), s.block_tokens) * s.block_tokens;
   if (span > most) span = most;
   s.span = (int32_t)span;
@@ -326,14 +356,14 @@ bool multiple(std::initializer_list<int64_t> v, int64_t n) {
 template <typename T, int W, bool kInterleaved>
 cudaError_t launch_rotary(const RotaryTensors& t, RotaryShape s, cudaStream_t st) {
   const auto kernel = rotary_kernel<T, W, kInterleaved>;
-  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 0);
+  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 0, 1);
   return launch_overlapped(kLaunchShort, kernel, dim3((unsigned)ceil_div(t.tokens, s.span)), dim3(kThreads), (size_t)smem, st, t, s);
 }
 
 template <int W, bool kInterleaved, bool kE4m3>
 cudaError_t launch_append(const AppendTensors& t, RotaryShape s, cudaStream_t st) {
   const auto kernel = append_kernel<W, kInterleaved, kE4m3>;
-  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 16);
+  const int smem = set_span(s, t.tokens, reinterpret_cast<const void*>(kernel), 16, 4);
   return launch_overlapped(kLaunchShort, kernel, dim3((unsigned)ceil_div(t.tokens, s.span)), dim3(kThreads), (size_t)smem, st, t, s);
 }
 
