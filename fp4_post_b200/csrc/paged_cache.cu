@@ -17,6 +17,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kMoveThreads = 256;
 constexpr int kScan = 4;                   // pages a thread looks at in one pass
 constexpr int kPass = kPlanThreads * kScan;
+constexpr int kNear = 1024;
 constexpr int64_t kMaxSequences = 1 << 17; // a bit for each in shared memory
 
 // A workspace: the header, for each sequence of the call what it needs in front of it, its source and its length, then the moves or the
@@ -54,6 +55,7 @@ struct PlanShared {
   int64_t sums[kPlanThreads / 32];
   int32_t code;                            // why the call is refused, the largest of the reasons
   int32_t found[kPass];                    // free pages of a pass, in order
+  int32_t needs[kNear];                    // those of the call's sequences where it has no more: a search of the others goes to memory at every step
 };
 
 __device__ __forceinline__ void reason(PlanShared& sh, int32_t code) { atomicMax(&sh.code, code); }
@@ -91,11 +93,11 @@ __device__ int64_t lowest_free(const CacheView& c, int64_t want, PlanShared& sh,
 }
 
 // The call's sequence that the rank-th page is for: the last whose needs begin at or before it.
-__device__ __forceinline__ int64_t owner_of(const int64_t* needs, int64_t n, int64_t rank) {
+__device__ __forceinline__ int64_t owner_of(const PlanShared& sh, const int64_t* needs, int64_t n, int64_t rank) {
   int64_t lo = 0, hi = n;
   while (hi - lo > 1) {
     const int64_t mid = (lo + hi) >> 1;
-    if (needs[mid] <= rank) lo = mid; else hi = mid;
+    if ((n <= kNear ? (int64_t)sh.needs[mid] : needs[mid]) <= rank) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -109,6 +111,7 @@ __device__ int64_t count_needs(const Work& w, int64_t n, PlanShared& sh, const N
     int64_t all;
     const int64_t before = total + block_exclusive<kPlanThreads>(i < n ? need(i) : (int64_t)0, sh.sums, all);
     if (i < n) w.needs[i] = before;
+    if (i < n && n <= kNear) sh.needs[i] = (int32_t)min(before, (int64_t)1 << 30);       // (a call that asks for so many is refused)
     total += all;
   }
   if (threadIdx.x == 0) w.needs[n] = total;
@@ -166,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const CacheView c
   }
   __syncthreads();
   lowest_free<true>(c, want, sh, [&](int64_t rank, int64_t p) {
-    const int64_t i = owner_of(w.needs, n, rank), slot = w.to[i];
+    const int64_t i = owner_of(sh, w.needs, n, rank), slot = w.to[i];
     const int64_t first = (c.lengths[slot] + page - 1) / page;
     c.tables[slot * c.width + first + rank - w.needs[i]] = (int32_t)p;
     c.refs[p] = 1;
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
   __syncthreads();
   // (a destination is empty, so that no source's table is written here)
   lowest_free<true>(c, want, sh, [&](int64_t rank, int64_t p) {
-    const int64_t i = owner_of(w.needs, n, rank), from = w.from[i], to = w.to[i], length = w.length[i];
+    const int64_t i = owner_of(sh, w.needs, n, rank), from = w.from[i], to = w.to[i], length = w.length[i];
     const int64_t entry = (share ? length / page : 0) + rank - w.needs[i];
     c.tables[to * c.width + entry] = (int32_t)p;
     c.refs[p] = 1;
