@@ -181,10 +181,11 @@ struct Row {
     const float d = __fmul_rn(__fmul_rn(__fsub_rn(top, v), inverse), kStep);
     return v == top ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
   }
-  // The unit of a bin's weights is 2^unit_of: two bits below the last one of the smallest.  (What lies in the last bin, at most 2^-46 of the largest, loses what it
-  // has below 2^-72.)
-  __device__ static int unit_of(int bin) { return bin == kBins - 1 ? -72 : (int)floorf(-(float)(bin + 1) * (1.44269504f / kStep)) - 2 - 24; }
+  // The unit of a bin's weights is 2^unit_of: at least two bits below the last one of the smallest, e^(-(bin + 1) / 64) (log2(e) / 64 is below 1478 / 65536).  What
+  // lies in the last bin, at most 2^-46 of the largest, loses what it has below 2^-72.
+  __device__ static int unit_of(int bin) { return bin == kBins - 1 ? -72 : -(int)((uint32_t)(bin + 1) * 1478u >> 16) - 1 - 2 - 24; }
   __device__ static uint32_t whole(float w, int unit) { return (uint32_t)(w * __uint_as_float((uint32_t)(127 - unit) << 23)); }
+  __device__ static double units(uint64_t m, int unit) { return (double)m * __hiloint2double((1023 + unit) << 20, 0); }
 
   template <bool kMass> __device__ void add(int bin, float v, int unit) {
     if constexpr (kMass) {
@@ -211,7 +212,7 @@ struct Row {
       uint64_t m;
       if constexpr (kMass) m = of_all_wide(bin) + (of_all_wide(kBins + bin) << kLowBits);
       else m = of_all(bin);
-      if (m) v[i] = kMass ? ldexp((double)m, unit == 1 ? unit_of(bin) : unit) : (double)m;
+      if (m) v[i] = kMass ? units(m, unit == 1 ? unit_of(bin) : unit) : (double)m;
       sum += v[i];
     }
     const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
@@ -238,7 +239,7 @@ struct Row {
 
   // The cut of the elements above `floor`: `at` such that the weights (or the number) of those above it are below the target and with those that equal
   // it are not; what is above, and how many equal it.  False if all of them do not reach the target.
-  template <bool kMass> __device__ __noinline__ bool cut(double target, float floor, float& at, double& above, double& ties) {
+  template <bool kMass> __device__ __forceinline__ bool cut(double target, float floor, float& at, double& above, double& ties) {
     clear();
     each([&](float v) {
       if (v > floor) {
@@ -287,7 +288,7 @@ struct Row {
       low = max(low, high - ((1u << shift) - 1u));
     }
     at = value_of<S::kDrop>(high);
-    ties = kMass ? rint(f.inside / ldexp((double)whole(weight(at), unit), unit)) : f.inside;
+    ties = kMass ? rint(f.inside / units(whole(weight(at), unit), unit)) : f.inside;
     return true;
   }
 
@@ -300,29 +301,31 @@ struct Row {
     return fmin(n, limit);
   }
 
-  // Top-k and top-p by these histograms.  all_weights: of the whole row.
-  __device__ __noinline__ Cut by_weights(int64_t k, int64_t vocab, double top_p, double all_weights) {
+  // Top-k and top-p by these histograms.  all_weights: of the whole row.  (A function of its own, for the registers of the way that needs none of it; by a
+  // copy of the row, whose members would come from memory for every element.)
+  static __device__ __noinline__ Cut by_weights(Row r, int64_t k, int64_t vocab, double top_p, double all_weights, int* turn) {
     Cut c = {-CUDART_INF_F, false, 0.0};
     double above = 0.0;
     if (k > 0 && k < vocab) {
       float at;
       double equal;
-      if (cut<false>((double)k, -CUDART_INF_F, at, above, equal)) c = {at, true, (double)k - above};       // (else there are not so many)
+      if (r.cut<false>((double)k, -CUDART_INF_F, at, above, equal)) c = {at, true, (double)k - above};       // (else there are not so many)
     }
     if (top_p < 1.0) {
       double total = all_weights, over = 0.0;
       if (c.found) {
         double sum = 0.0;
-        each([&](float v) { if (v > c.at) sum += (double)weight(v); });
-        over = sum_of(sum);
-        total = over + c.ties * (double)weight(c.at);
+        r.each([&](float v) { if (v > c.at) sum += (double)r.weight(v); });
+        over = r.sum_of(sum);
+        total = over + c.ties * (double)r.weight(c.at);
       }
       const double target = fmax(top_p * total, 1e-300);                  // (the first one is always kept)
       float at;
       double before, equal;
-      if (cut<true>(target, c.at, at, before, equal)) c = {at, true, ties_below(target, before, at, equal)};
-      else if (c.found) c.ties = ties_below(target, over, c.at, c.ties);  // all that are above the cut of top-k, and some that equal it
+      if (r.cut<true>(target, c.at, at, before, equal)) c = {at, true, r.ties_below(target, before, at, equal)};
+      else if (c.found) c.ties = r.ties_below(target, over, c.at, c.ties);  // all that are above the cut of top-k, and some that equal it
     }
+    *turn = r.turn;
     return c;
   }
 
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     r.each([&](float v) { sum += (double)r.weight(v); });
     all_weights = r.sum_of(sum);
   }
-  if (!settled) cut = r.by_weights(k, p.vocab, top_p, all_weights);
+  if (!settled) cut = Row<T>::by_weights(r, k, p.vocab, top_p, all_weights, &r.turn);
   if (k == 1) cut = {top, true, 1.0};
 
   // ---- the kept weights of this thread's elements, in order of their indices ----
