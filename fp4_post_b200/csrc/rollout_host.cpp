@@ -546,7 +546,7 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       top_p(a, "top_p", device, rows, at::kFloat, "a number or float32"), min_p(a, "min_p", device, rows, at::kFloat, "a number or float32");
   const bool want = a.truth();
   TORCH_CHECK_VALUE(temperature.rows.defined() || temperature.one == 0.0 || (temperature.one >= 0x1p-126 && temperature.one <= 3e38), "temperature must be 0, or from 2^-126 to 3e38, not ", temperature.one);
-  TORCH_CHECK_VALUE(top_k.rows.defined() || (top_k.one >= 0.0 && top_k.one <= 2147483647.0), "top_k must be a whole number, 0 for all, not ", top_k.one);
+  TORCH_CHECK_VALUE(top_k.rows.defined() || (top_k.one >= 0.0 && top_k.one <= 2147483647.0 && top_k.one == (double)(int64_t)top_k.one), "top_k must be a whole number, 0 for all, not ", top_k.one);
   TORCH_CHECK_VALUE(top_p.rows.defined() || (top_p.one >= 0.0 && top_p.one <= 1.0), "top_p must be from 0 to 1, not ", top_p.one);
   TORCH_CHECK_VALUE(min_p.rows.defined() || (min_p.one >= 0.0 && min_p.one <= 1.0), "min_p must be from 0 to 1, not ", min_p.one);
   Tensor token, logprob;

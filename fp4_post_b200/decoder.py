@@ -334,6 +334,8 @@ class Decoder(nn.Module):
             raise RuntimeError("generate() runs on a paged cache on the GPU: there is no CPU fallback")
         if max_new_tokens < 1 or answers < 1:
             raise ValueError("max_new_tokens and answers must be positive")
+        if page_size <= 0 or page_size % 16:
+            raise ValueError(f"page_size must be a multiple of 16, not {page_size}")
         B, T = ids.shape
         lengths = [T] * B if lengths is None else [int(n) for n in lengths]
         if len(lengths) != B or min(lengths) < 1 or max(lengths) > T:

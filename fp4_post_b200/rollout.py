@@ -23,6 +23,7 @@ The reference leaves all of this to the Hugging Face model that it generates wit
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Union
 
 import torch
@@ -184,10 +185,13 @@ class PagedCache:
 
     def reserve(self, slots=None, counts: Union[int, torch.Tensor, list] = 1) -> None:
         """Lengthens the sequences `slots` (None: all) by `counts` tokens, one number or one for each, with pages for them."""
-        if isinstance(counts, int):
-            self._host.reserve(self._handle, self._index(slots), None, counts)
-        else:
-            self._host.reserve(self._handle, self._index(slots), self._index(counts), 0)
+        one = counts if isinstance(counts, int) else None
+        if one is None and not isinstance(counts, torch.Tensor):
+            try:
+                one = operator.index(counts)
+            except TypeError:                # (one for each)
+                pass
+        self._host.reserve(self._handle, self._index(slots), None if one is not None else self._index(counts), one or 0)
 
     def append(self, layer: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots=None, positions=None, *,
                rotary: Optional[Rotary] = None) -> Optional[torch.Tensor]:

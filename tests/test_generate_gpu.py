@@ -146,7 +146,7 @@ def test_generate_one_token_and_refusals():
     assert model.generate(ids, max_new_tokens=1, answers=2).shape == (4, 1)
     assert model.generate(ids, max_new_tokens=2, graphed=True).shape == (2, 2)
     for kw in (dict(max_new_tokens=0), dict(max_new_tokens=1, answers=0), dict(max_new_tokens=1, lengths=[1]), dict(max_new_tokens=1, lengths=[0, 3]), dict(max_new_tokens=1, lengths=[3, 11]),
-               dict(max_new_tokens=1, page_size=10), dict(max_new_tokens=1, top_p=2.0), dict(max_new_tokens=1, temperature=-1.0)):
+               dict(max_new_tokens=1, page_size=10), dict(max_new_tokens=1, page_size=0), dict(max_new_tokens=1, top_p=2.0), dict(max_new_tokens=1, temperature=-1.0)):
         with pytest.raises(ValueError):
             model.generate(ids, kw.pop("lengths", None), **kw)
     with pytest.raises(TypeError):

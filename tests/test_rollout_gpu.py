@@ -723,6 +723,68 @@ def test_a_decode_step_replays_from_a_graph_as_its_sequences_grow():
     twin.check()
 
 
+@pytest.mark.parametrize("length", [37, 32, 5])
+def test_forked_sequences_grow_apart(length):
+    """Two answers and their prompt each go on by tokens of their own: what they share stays, what they add is theirs."""
+    cache = new_cache(pages=30, sequences=4)
+    k, v = normal(length, 2, 64, seed=30), normal(length, 2, 64, seed=31)
+    cache.reserve([0], length)
+    cache.append(0, None, k, v, [0] * length, list(range(length)))
+    cache.fork([0, 0], [2, 3])
+    want = {s: ([k], [v]) for s in (0, 2, 3)}
+    for step in range(20):
+        slots = [2, 0, 3] if step % 3 else [3, 2]
+        cache.reserve(slots, 1)
+        nk, nv = normal(len(slots), 2, 64, seed=100 + step), normal(len(slots), 2, 64, seed=200 + step)
+        cache.append(0, None, nk, nv, slots)
+        for i, s in enumerate(slots):
+            want[s][0].append(nk[i:i + 1])
+            want[s][1].append(nv[i:i + 1])
+    cache.check()
+    for s, (ks, vs) in want.items():
+        n = int(cache.lengths[s])
+        assert n == sum(len(t) for t in ks)
+        got = keys_values(cache, 0, s, n)
+        assert torch.equal(got[0], torch.cat(ks).double().transpose(0, 1)) and torch.equal(got[1], torch.cat(vs).double().transpose(0, 1))
+    cache.free([0])
+    for s in (2, 3):
+        assert torch.equal(keys_values(cache, 0, s, int(cache.lengths[s]))[0], torch.cat(want[s][0]).double().transpose(0, 1))
+    before = {s: keys_values(cache, 0, s, int(cache.lengths[s])) for s in (2, 3)}
+    cache.compact()
+    for s in (2, 3):
+        assert torch.equal(keys_values(cache, 0, s, int(cache.lengths[s])), before[s])
+
+
+def test_graphs_of_several_caches_replay_in_turn():
+    caches = [filled([900, 3, 40], seed=32, head_dim=128), filled([20, 1300, 0], seed=33, head_dim=128)]
+    qs = [normal(3, 14, 128, seed=34), normal(3, 14, 128, seed=35)]
+    x, u = normal(2, 9000, seed=36), torch.rand(2, device=DEV, generator=gen(37))
+    graphs, outs = [], []
+    for c, q in zip(caches, qs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append((c.attend(0, q, return_lse=True), rollout.sample(x, u, top_p=0.8)))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for i in range(6):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    for c, q, ((out, lse), token) in zip(caches, qs, outs):
+        want = c.attend(0, q, return_lse=True)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and torch.equal(token, rollout.sample(x, u, top_p=0.8))
+
+
+def test_counts_are_whole_numbers_of_any_kind():
+    import numpy as np
+    cache = new_cache()
+    cache.reserve([0], np.int64(3))
+    cache.reserve(np.array([1, 2]), np.array([4, 5]))
+    cache.check()
+    assert cache.lengths.tolist() == [3, 4, 5, 0, 0, 0]
+
+
 # ---- sampling -----------------------------------------------------------------------------------------------------------
 
 def chosen(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -885,8 +947,9 @@ def test_sample_frequencies_follow_the_distribution():
 
 
 def test_sample_the_largest_vocabulary():
-    x = normal(2, 393216, seed=10, scale=2.0)
-    check_samples(x, torch.tensor([0.3, 0.9], device=DEV), top_p=0.9)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = normal(2, 393216, seed=10, scale=2.0, dtype=dtype)
+        check_samples(x, torch.tensor([0.3, 0.9], device=DEV), top_p=0.9)
     with pytest.raises(ValueError, match="393216"):
         rollout.sample(torch.zeros(1, 393217, device=DEV), torch.zeros(1, device=DEV))
 
@@ -905,7 +968,7 @@ def test_sample_replays_from_a_graph():
 def test_sample_refuses():
     x, u = normal(2, 8), torch.zeros(2, device=DEV)
     for kw, error in [(dict(temperature=-1.0), ValueError), (dict(temperature=math.nan), ValueError), (dict(temperature=math.inf), ValueError), (dict(top_p=1.5), ValueError), (dict(top_p=-0.1), ValueError),
-                      (dict(min_p=2.0), ValueError), (dict(top_k=-1), ValueError), (dict(temperature="hot"), TypeError), (dict(temperature=torch.ones(3, device=DEV)), ValueError),
+                      (dict(min_p=2.0), ValueError), (dict(top_k=-1), ValueError), (dict(top_k=2.5), ValueError), (dict(temperature="hot"), TypeError), (dict(temperature=torch.ones(3, device=DEV)), ValueError),
                       (dict(top_k=torch.ones(2, device=DEV)), TypeError), (dict(top_p=torch.ones(2)), RuntimeError)]:
         with pytest.raises(error):
             rollout.sample(x, u, **kw)
