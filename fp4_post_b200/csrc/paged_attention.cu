@@ -29,12 +29,13 @@ constexpr int kRows = 16;                 // keys of one product, which lie on o
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxRows = 512;             // of one launch: their sequences and lengths are kept in shared memory
+constexpr int kMaxGroup = 1024;           // query heads of a key-value head: their chunks are far fewer than the blocks of a launch
 constexpr int64_t kMaxTiles = (int64_t)1 << 30;      // of one launch and one head
 constexpr int kMinTiles = 8;              // of a part: two for each warp
 // What beginning and ending a row costs a block, in tiles: parts are equal in tiles and this for each row.  A batch of 256 rows of 1 to 2047 keys took
 // 85 us where short rows were counted by their tiles alone, 75 with 4, 57 with 16, 56 with 20 to 32; few long rows do not change.
 constexpr int kBegin = 20;
-constexpr float kNone = -3e38f;           // the maximum of no scores: finite, so that a score of -inf weighs nothing behind it
+constexpr float kNone = -3.4028235e38f;   // the maximum of no scores: the lowest finite number, so that a score of -inf weighs nothing behind it, and any other something
 constexpr float kSlack = 8.0f;            // weights may be up to 2^8 before the maximum they are relative to is moved
 
 struct AttendParams {
@@ -44,7 +45,7 @@ struct AttendParams {
   float* lse;
   const void* slots;
   bool slots_64;
-  int32_t rows, heads_q, group, chunks;   // chunks: pieces of a group that a block takes at once, each a unit of work beside others
+  int32_t rows, heads_q, group, chunks;   // chunks: pieces of a group that a block takes at once
   const int32_t* lengths;
   const int32_t* tables;
   int64_t sequences, width, pages, page_bytes;
@@ -55,8 +56,8 @@ struct AttendParams {
   float scale;                            // times log2(e)
   float* part_o;                          // [2 blocks, 8 NT, D]
   float2* part_ml;                        // [2 blocks, 8 NT]
-  // What the second launch joins: row, unit (key-value head and chunk), first and last block.  One place for each unit of each row where those are no more
-  // than blocks, else one for each block: that of the second piece.
+  // What the second launch joins: row, key-value head and chunk as one number, first and last part.  One place for each of those of each row where they are no
+  // more than blocks, else one for each block: that of the second piece.
   int4* join;
   bool by_unit;
 };
@@ -164,18 +165,20 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     if (threadIdx.x == kThreads - 1 && row < p.rows) before[row + 1] = ahead + s.upto;
     __syncthreads();
   }
-  const int heads = p.kv_heads * p.chunks;                               // units of work beside one another on the same row
+  // blocks of the same part are neighbours, one for each chunk of its groups: they read the same tiles at about the same time, and memory once
+  // (80 heads on one, 32 rows of 20000 keys: 246 us where each chunk was work of its own, 154 so; 64 on 2: 205 and 128)
+  const int heads = p.kv_heads, chunk = blockIdx.x % p.chunks;
   const int64_t total = (int64_t)before[p.rows] * heads;
-  const int64_t parts = min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
-  const int64_t cta = blockIdx.x;
+  const int64_t parts = min((int64_t)(gridDim.x / p.chunks), (total + kMinTiles - 1) / kMinTiles);
+  const int64_t cta = blockIdx.x / p.chunks;
   // rows without keys
   for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
     if (before[row + 1] != before[row]) continue;
     for (int i = threadIdx.x; i < p.heads_q * p.head_dim; i += kThreads) p.out[(int64_t)row * p.heads_q * p.head_dim + i] = __float2bfloat16_rn(0.0f);
     if (p.lse) for (int i = threadIdx.x; i < p.heads_q; i += kThreads) p.lse[(int64_t)row * p.heads_q + i] = -CUDART_INF_F;
-    if (p.by_unit) for (int i = threadIdx.x; i < heads; i += kThreads) p.join[row * heads + i] = make_int4(-1, 0, 0, 0);
+    if (p.by_unit) for (int i = threadIdx.x; i < heads * p.chunks; i += kThreads) p.join[row * heads * p.chunks + i] = make_int4(-1, 0, 0, 0);
   }
-  if (!p.by_unit && threadIdx.x == 0) p.join[cta] = make_int4(-1, 0, 0, 0);
+  if (!p.by_unit && threadIdx.x == 0) p.join[blockIdx.x] = make_int4(-1, 0, 0, 0);
   if (cta >= parts) return;
   int64_t at = cta * total / parts;
   const int64_t end = (cta + 1) * total / parts;
@@ -192,12 +195,12 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     const int row = lo;
     const int row_cost = before[row + 1] - before[row], row_tiles = row_cost - kBegin;
     const int64_t inside = at - (int64_t)before[row] * heads;
-    const int unit = (int)(inside / row_cost), head = unit / p.chunks, chunk = unit - head * p.chunks;
-    // this block's tiles of the unit; its first kBegin places stand for none
-    const int here = (int)(inside - (int64_t)unit * row_cost);
+    const int head = (int)(inside / row_cost);
+    // this block's tiles of the row and head; their first kBegin places stand for none
+    const int here = (int)(inside - (int64_t)head * row_cost);
     const int begin = max(here - kBegin, 0), stop = (int)min((int64_t)row_tiles, here - kBegin + (end - at));
     at += stop > begin ? stop + kBegin - here : end - at;
-    if (stop <= begin) continue;           // (the part ends before the unit's first tile)
+    if (stop <= begin) continue;           // (the part ends before their first tile)
     const int64_t slot = slot_of[row];
     const int first_head = head * p.group + chunk * 8 * NT, live = min(8 * NT, p.group - chunk * 8 * NT);
     const float k_scale = p.scales ? p.scales[head] : 1.0f, v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
       }
     __syncthreads();
     const bool whole = begin == 0 && stop == row_tiles;
-    const int64_t place = (cta * 2 + (begin == 0 ? 1 : 0)) * 8 * NT;
+    const int64_t place = ((int64_t)blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * 8 * NT;
     for (int i = threadIdx.x; i < live * D; i += kThreads) {
       const int column = i / D, e = i - column * D;
       float top = kNone;
@@ -510,16 +513,17 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
       }
     }
     if (threadIdx.x == 0 && (p.by_unit ? begin == 0 : begin > 0)) {
-      const int64_t start = (int64_t)before[row] * heads + (int64_t)unit * row_cost + kBegin, last = start + row_tiles - 1;
+      const int64_t start = (int64_t)before[row] * heads + (int64_t)head * row_cost + kBegin, last = start + row_tiles - 1;
       const int64_t c0 = ((start + 1) * parts - 1) / total, c1 = ((last + 1) * parts - 1) / total;
-      if (p.by_unit) p.join[row * heads + unit] = make_int4(whole ? -1 : row, unit, (int)c0, (int)c1);
-      else if (c0 == cta - 1) p.join[cta] = make_int4(row, unit, (int)c0, (int)c1);
+      const int unit = head * p.chunks + chunk;
+      if (p.by_unit) p.join[row * heads * p.chunks + unit] = make_int4(whole ? -1 : row, unit, (int)c0, (int)c1);
+      else if (c0 == cta - 1) p.join[blockIdx.x] = make_int4(row, unit, (int)c0, (int)c1);
     }
     __syncthreads();                       // the ring is free again
   }
 }
 
-// Joins the pieces of a unit that several blocks wrote, for one query head of the group.  A warp takes every eighth piece, a lane D / 32 elements.
+// Joins the pieces of a row and head that several blocks wrote, for one query head of the group.  A warp takes every eighth piece, a lane D / 32 elements.
 // kMany pieces (few units, so that there are few blocks): a lane looks at one piece's maximum and sum, and eight outputs are on their way at once; else
 // fewer registers, so that an SM takes twice the blocks, most of which have nothing to do.  32768 keys of one row, 111 pieces: 21.5 us with, 23.0
 // without; 256 rows in two or three pieces: 57.9 with, 54.5 without.
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 8) join_kernel(const AttendPa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t c0 = job.z;
   const int pieces = job.w - job.z + 1;
-  auto place = [&](int i) { return ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
+  auto place = [&](int i) { return (((c0 + i) * p.chunks + chunk) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
   float top = kNone;
   for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
 #pragma unroll
@@ -595,11 +599,10 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 8) join_kernel(const AttendPa
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-// Columns of eight that a block takes at once: the whole group up to 32 heads (16 of 256 elements: registers), in pieces beyond.
-int column_tiles(int group, int D) {
-  const int nt = group <= 8 ? 1 : group <= 16 ? 2 : 4;
-  return D == 256 && nt > 2 ? 2 : nt;
-}
+// Columns of eight that a block takes at once; of larger groups, 16 heads each.  (Four of them hold 255 registers and one block an SM: 256 rows of 1000 keys,
+// 64 heads on 2 of 128 elements, 96.8 us, 98.2 in e4m3, for 88.0 and 77.7; 80 heads on one, 32 rows of 20000 keys, 185 and 151 us for 154 and 121; of 64 elements, 48
+// on 2, 72 and 58 for 79 and 64.)
+int column_tiles(int group) { return group <= 8 ? 1 : 2; }
 
 template <int D, int NT, bool kE4m3>
 struct Launch {
@@ -633,11 +636,9 @@ struct Launch {
 // f(Launch<...>()) of the kernel for these sizes
 template <typename F>
 int32_t with_kernel(int head_dim, int group, bool e4m3, const F& f) {
-  const int D = padded_dim(head_dim), nt = column_tiles(group, D);
-  if (D == 64)  return nt == 1 ? (e4m3 ? f(Launch<64, 1, true>()) : f(Launch<64, 1, false>())) : nt == 2 ? (e4m3 ? f(Launch<64, 2, true>()) : f(Launch<64, 2, false>()))
-                                                                                              : (e4m3 ? f(Launch<64, 4, true>()) : f(Launch<64, 4, false>()));
-  if (D == 128) return nt == 1 ? (e4m3 ? f(Launch<128, 1, true>()) : f(Launch<128, 1, false>())) : nt == 2 ? (e4m3 ? f(Launch<128, 2, true>()) : f(Launch<128, 2, false>()))
-                                                                                                : (e4m3 ? f(Launch<128, 4, true>()) : f(Launch<128, 4, false>()));
+  const int D = padded_dim(head_dim), nt = column_tiles(group);
+  if (D == 64)  return nt == 1 ? (e4m3 ? f(Launch<64, 1, true>()) : f(Launch<64, 1, false>())) : (e4m3 ? f(Launch<64, 2, true>()) : f(Launch<64, 2, false>()));
+  if (D == 128) return nt == 1 ? (e4m3 ? f(Launch<128, 1, true>()) : f(Launch<128, 1, false>())) : (e4m3 ? f(Launch<128, 2, true>()) : f(Launch<128, 2, false>()));
   return nt == 1 ? (e4m3 ? f(Launch<256, 1, true>()) : f(Launch<256, 1, false>())) : (e4m3 ? f(Launch<256, 2, true>()) : f(Launch<256, 2, false>()));
 }
 
@@ -666,7 +667,8 @@ extern "C" int32_t metis_cache_attend(const metis_cache* cache, const metis_atte
     return fail(METIS_ERR_BAD_SHAPE, "rows must be positive, heads_q a multiple of kv_heads and the layer one of the cache");
   if (a->q_row % 2 != 0 || a->q_head % 2 != 0 || (reinterpret_cast<uintptr_t>(a->q) & 3) || !aligned16(a->workspace))
     return fail(METIS_ERR_BAD_ALIGNMENT, "rows of q must be 4-byte aligned and the workspace 16");
-  const int group = a->heads_q / c.kv_heads, nt = column_tiles(group, padded_dim(c.head_dim));
+  const int group = a->heads_q / c.kv_heads, nt = column_tiles(group);
+  if (group > kMaxGroup) return fail(METIS_ERR_TOO_LARGE, "at most %d query heads share a key-value head", kMaxGroup);
   const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;
   const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   // more rows than one launch counts go in several, one after the other: they share the workspace

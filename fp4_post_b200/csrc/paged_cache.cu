@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const CacheView c
     if (slot >= c.sequences) { reason(sh, METIS_CACHE_BAD_SLOT); return 0; }
     if (marked(marks, slot)) { reason(sh, METIS_CACHE_TWICE); return 0; }
     const int64_t length = c.lengths[slot];
-    // (a count near 2^63 is too long, not negative again)
-    if (more < 0 || more > c.width * page || length + more > c.width * page) { reason(sh, METIS_CACHE_TOO_LONG); return 0; }
+    // (a count near 2^63 is too long, not negative again; nor is a length taken that no call has left)
+    if (length < 0 || more < 0 || more > c.width * page || length + more > c.width * page) { reason(sh, METIS_CACHE_TOO_LONG); return 0; }
     w.to[i] = (int32_t)slot;
     w.length[i] = (int32_t)(length + more);
     return (length + more + page - 1) / page - (length + page - 1) / page;
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
     if (marked(marks, to)) { reason(sh, METIS_CACHE_TWICE); return 0; }
     if (c.lengths[to] != 0) { reason(sh, METIS_CACHE_NOT_EMPTY); return 0; }
     const int64_t length = c.lengths[from];
+    if (length < 0 || length > c.width * page) { reason(sh, METIS_CACHE_TOO_LONG); return 0; }
     w.from[i] = (int32_t)from;
     w.to[i] = (int32_t)to;
     w.length[i] = (int32_t)length;

@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     for (int i = 0; i < blocks; ++i) best = max(best, (uint32_t)g[i][0]);
   }
   const float top = value_of<S::kDrop>(best);
-  const bool fine = (t == 0.0f || (t >= 0x1p-126f && t <= 3.4028235e38f)) && top_p >= 0.0 && min_p >= 0.0f && min_p <= 1.0f && k >= 0 && u >= 0.0 && u < 1.0 &&
+  const bool fine = (t == 0.0f || (t >= 0x1p-126f && t <= 3.4028235e38f)) && top_p >= 0.0 && top_p <= 1.0 && min_p >= 0.0f && min_p <= 1.0f && k >= 0 && u >= 0.0 && u < 1.0 &&
                     top > -CUDART_INF_F;
   if (!fine) {                                     // (for all blocks of the cluster)
     if (rank == 0 && threadIdx.x == 0) {

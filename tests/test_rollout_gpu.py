@@ -989,3 +989,50 @@ def test_the_exponential_is_torch_s():
     x = torch.stack((torch.zeros(4096, device=DEV), z[pick]), dim=1)
     _, logp = rollout.sample(x, torch.zeros(4096, device=DEV), logprobs=True)
     assert torch.equal(logp, (-torch.log1p(w[pick].double())).float()) or ((logp.double() + torch.log1p(w[pick].double())).abs() <= 2.0 ** -24 * logp.double().abs() + 2.0 ** -53).all()
+
+
+def test_lengths_that_no_call_has_left_are_refused():
+    cache = new_cache()
+    cache.reserve([0, 1], [20, 5])
+    for length in (-1, -100, -2 ** 31, 129, 2 ** 31 - 1):
+        cache.lengths[2] = length
+        before = [t.clone() for t in (cache.tables, cache.lengths, cache.refs)]
+        for call in (lambda: cache.reserve([1, 2], 3), lambda: cache.reserve([2], 128), lambda: cache.fork([0, 2], [3, 4]), lambda: cache.fork([2], [3], share=False)):
+            call()
+            assert all(torch.equal(a, b) for a, b in zip(before, (cache.tables, cache.lengths, cache.refs)))
+            with pytest.raises(RuntimeError, match="longer"):
+                cache.check()
+
+
+def test_a_nucleus_of_more_than_all_is_out_of_range():
+    x, u = normal(3, 500, seed=5), torch.full((3,), 0.5, device=DEV)
+    token = rollout.sample(x, u, top_p=torch.tensor([1.0, 1.0 + 2.0 ** -20, 0.5], device=DEV))
+    assert token[1] == -1 and token[0] == rollout.sample(x, u)[0] and token[2] == rollout.sample(x, u, top_p=0.5)[2]
+
+
+def test_attend_scores_near_the_lowest_number_still_weigh():
+    cache = filled([1, 3], kv_heads=1, seed=30)
+    q = torch.zeros(2, 2, 64, device=DEV, dtype=torch.bfloat16)
+    q[:, :, 0] = -(2.0 ** 64)
+    for slot, n in ((0, 1), (1, 3)):
+        cache.pool[int(cache.tables[slot, 0]), 0, 0, 0, :n] = 0.0
+        cache.pool[int(cache.tables[slot, 0]), 0, 0, 0, :n, 0] = 1.3125 * 2.0 ** 63          # scores of -1.3125 2^127, -3.2e38 in powers of 2
+    out = cache.attend(0, q, scale=1.0)
+    for slot, n in ((0, 1), (1, 3)):
+        v = keys_values(cache, 0, slot, n)[1, 0].double()
+        assert torch.allclose(out[slot].double(), v.mean(dim=0).expand(2, 64), rtol=2.0 ** -8, atol=2.0 ** -14)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("heads, kv_heads, head_dim, lengths", [(70, 2, 64, [3000, 0, 17]), (48, 1, 256, [1, 5000]), (100, 1, 128, [40] * 70), (40, 1, 128, [0, 0]), (1024, 1, 16, [33, 700])])
+def test_attend_groups_in_several_chunks(dtype, heads, kv_heads, head_dim, lengths):
+    cache = filled(lengths, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, seed=heads)
+    q = normal(len(lengths), heads, head_dim, seed=31)
+    out, lse = cache.attend(0, q, return_lse=True)
+    check_attend(cache, q, out, lse, range(len(lengths)))
+
+
+def test_attend_refuses_groups_beyond_its_blocks():
+    cache = filled([5], kv_heads=1, head_dim=16, seed=32)
+    with pytest.raises(RuntimeError, match="1024 query heads"):
+        cache.attend(0, normal(1, 1025, 16))
