@@ -132,7 +132,7 @@ template <int D, int NT, bool kE4m3> struct Plan {
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kPieces = kRowBytes / 16;
   static constexpr int kHeld = D / 16 * NT * 6;                         // registers of output and queries
-  static constexpr int kBlocks = kHeld <= 48 ? 3 : kHeld <= 96 ? 2 : 1;
+  static constexpr int kBlocks = kHeld <= 48 ? 3 : 2;
   static_assert(8 * NT * D * 4 <= kWarpBytes, "a warp's output goes where its tiles were");
 };
 
@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     // copies: lane's row and piece of the first of a part's 512-byte steps (all further ones by constants where the head has D elements)
     constexpr int kStepRows = 32 / L::kPieces;
     const uint32_t copy_base = piece_base<L::kRowBytes>(lane / L::kPieces, lane % L::kPieces);
+    const int column = lane % L::kPieces * 16 < row_bytes ? lane % L::kPieces * 16 : -1;             // of a head of other than D elements; -1: behind its last
+    const bool whole_pieces = row_bytes % 16 == 0;
     int32_t page = -1, piece_on_page = 0;  // of the lane's 16 keys among the 32 times 16 that are looked up at once
     int fetched = 0;                       // tiles whose copies have been issued
     uint32_t absent = 0;                   // bit i: the 16 keys i before the last fetched ones lie on no page of the pool
@@ -248,6 +250,18 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
               copy16(dst, src + i * 512, 16);
               copy16(dst + L::kPartBytes, src_v + i * 512, 16);
             }
+          } else if (keys == kRows && (!kE4m3 || whole_pieces)) {
+            // Heads of other sizes: a lane's column is the same in all steps, with zeros behind the last one.  (32 rows of 17000 keys, 192 elements: 145 -> 133 us,
+            // e4m3 117 -> 78, against the way below; of 80, 20000 keys: 140 -> 138 and 100 -> 84.  Rows on 8 bytes, four copies for two, gain nothing by it.)
+            const char* src = from + lane / L::kPieces * row_bytes + max(column, 0);
+#pragma unroll
+            for (int i = 0; i < L::kPartBytes / 512; ++i) {
+              constexpr int kMask = L::kRowBytes == 64 ? 0 : 7;
+              const uint32_t dst = to + ((copy_base ^ ((i * kStepRows & kMask) << 4)) + i * 512);
+              copy16(dst, src, column < 0 ? 0 : 16);
+              copy16(dst + L::kPartBytes, src + p.values_off, column < 0 ? 0 : 16);
+              src += kStepRows * row_bytes;
+            }
           } else {
 #pragma unroll 1
             for (int i = 0; i < L::kPartBytes / 512; ++i) {
@@ -255,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
               const bool in = r < keys && c * 16 < row_bytes;
               const char* src = from + (in ? r * row_bytes + c * 16 : 0);
               const uint32_t dst = to + piece_base<L::kRowBytes>(r, c);
-              if (!kE4m3 || row_bytes % 16 == 0) {
+              if (!kE4m3 || whole_pieces) {
                 copy16(dst, src, in ? 16 : 0);
                 copy16(dst + L::kPartBytes, src + p.values_off, in ? 16 : 0);
               } else {
@@ -599,10 +613,11 @@ __global__ void __launch_bounds__(256, kMany ? 4 : 8) join_kernel(const AttendPa
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-// Columns of eight that a block takes at once; of larger groups, 16 heads each.  (Four of them hold 255 registers and one block an SM: 256 rows of 1000 keys,
-// 64 heads on 2 of 128 elements, 96.8 us, 98.2 in e4m3, for 88.0 and 77.7; 80 heads on one, 32 rows of 20000 keys, 185 and 151 us for 154 and 121; of 64 elements, 48
-// on 2, 72 and 58 for 79 and 64.)
-int column_tiles(int group) { return group <= 8 ? 1 : 2; }
+// Columns of eight that a block takes at once; of larger groups, 16 heads each, 8 of more than 128 elements.  (Four of them hold 255 registers and one block an
+// SM: 256 rows of 1000 keys, 64 heads on 2 of 128 elements, 96.8 us, 98.2 in e4m3, for 88.0 and 77.7; 80 heads on one, 32 rows of 20000 keys, 185 and 151 us for 154
+// and 121; of 64 elements, 48 on 2, 72 and 58 for 79 and 64.  Two of 256 elements are one block an SM, too: 40 heads on one, 32 rows of 13000 keys, 205 and 154 us for
+// 177 and 137; 24 on 2, 7000 keys, 86.9 and 71.9 for 90.6 and 66.4; one row of 20000, 21.3 and 22.2 for 17.8 and 16.5.)
+int column_tiles(int group, int D) { return group <= 8 || D == 256 ? 1 : 2; }
 
 template <int D, int NT, bool kE4m3>
 struct Launch {
@@ -636,10 +651,10 @@ struct Launch {
 // f(Launch<...>()) of the kernel for these sizes
 template <typename F>
 int32_t with_kernel(int head_dim, int group, bool e4m3, const F& f) {
-  const int D = padded_dim(head_dim), nt = column_tiles(group);
+  const int D = padded_dim(head_dim), nt = column_tiles(group, D);
   if (D == 64)  return nt == 1 ? (e4m3 ? f(Launch<64, 1, true>()) : f(Launch<64, 1, false>())) : (e4m3 ? f(Launch<64, 2, true>()) : f(Launch<64, 2, false>()));
   if (D == 128) return nt == 1 ? (e4m3 ? f(Launch<128, 1, true>()) : f(Launch<128, 1, false>())) : (e4m3 ? f(Launch<128, 2, true>()) : f(Launch<128, 2, false>()));
-  return nt == 1 ? (e4m3 ? f(Launch<256, 1, true>()) : f(Launch<256, 1, false>())) : (e4m3 ? f(Launch<256, 2, true>()) : f(Launch<256, 2, false>()));
+  return e4m3 ? f(Launch<256, 1, true>()) : f(Launch<256, 1, false>());
 }
 
 }  // namespace
@@ -667,7 +682,7 @@ extern "C" int32_t metis_cache_attend(const metis_cache* cache, const metis_atte
     return fail(METIS_ERR_BAD_SHAPE, "rows must be positive, heads_q a multiple of kv_heads and the layer one of the cache");
   if (a->q_row % 2 != 0 || a->q_head % 2 != 0 || (reinterpret_cast<uintptr_t>(a->q) & 3) || !aligned16(a->workspace))
     return fail(METIS_ERR_BAD_ALIGNMENT, "rows of q must be 4-byte aligned and the workspace 16");
-  const int group = a->heads_q / c.kv_heads, nt = column_tiles(group);
+  const int group = a->heads_q / c.kv_heads, nt = column_tiles(group, padded_dim(c.head_dim));
   if (group > kMaxGroup) return fail(METIS_ERR_TOO_LARGE, "at most %d query heads share a key-value head", kMaxGroup);
   const int64_t part = (int64_t)c.kv_heads * c.page_size * c.head_dim * c.item;
   const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
