@@ -73,23 +73,35 @@ __device__ __forceinline__ uint32_t pages_with(const CacheView& c, int64_t at, c
   return with;
 }
 
-// Free pages in the order of their numbers: take(rank, page) for the first `want`; returns how many of those there are.
-template <bool kTake, typename Take>
-__device__ int64_t lowest_free(const CacheView& c, int64_t want, PlanShared& sh, const Take& take) {
-  int64_t found = 0;
-  for (int64_t base = 0; base < c.pages && found < want; base += kPass) {
+// Free pages in the order of their numbers: take(rank, page) for each of the first `want`; false, and nothing taken, where there are not so many.  The first kPass are
+// kept in shared memory while they are counted; a call for more goes through refs once more.
+template <typename Take>
+__device__ bool take_lowest(const CacheView& c, int64_t want, PlanShared& sh, const Take& take) {
+  auto pass = [&](int64_t base, int64_t found, int64_t from) -> int64_t {        // found: before this pass; from: the rank that sh.found begins with
     const int64_t at = base + (int64_t)threadIdx.x * kScan;
     uint32_t free_ = pages_with(c, at, [](int32_t refs, int64_t) { return refs == 0; });
-    int64_t all, rank = block_exclusive<kPlanThreads>((int64_t)__popc(free_), sh.sums, all);
-    if constexpr (kTake) {
-      for (; free_; free_ &= free_ - 1) sh.found[rank++] = (int32_t)(at + __ffs(free_) - 1);
-      __syncthreads();
-      for (int64_t r = threadIdx.x; r < all && found + r < want; r += kPlanThreads) take(found + r, (int64_t)sh.found[r]);
-      // (the next pass writes behind block_exclusive's barriers)
-    }
-    found += all;
+    int64_t all, rank = found - from + block_exclusive<kPlanThreads>((int64_t)__popc(free_), sh.sums, all);
+    for (; free_; free_ &= free_ - 1, ++rank)
+      if (rank < kPass) sh.found[rank] = (int32_t)(at + __ffs(free_) - 1);
+    return all;
+  };
+  int64_t found = 0;
+  for (int64_t base = 0; base < c.pages && found < want; base += kPass) found += pass(base, found, 0);
+  if (found < want) return false;
+  __syncthreads();
+  if (want <= kPass) {
+    for (int64_t r = threadIdx.x; r < want; r += kPlanThreads) take(r, (int64_t)sh.found[r]);
+    return true;
   }
-  return found < want ? found : want;
+  found = 0;
+  for (int64_t base = 0; base < c.pages && found < want; base += kPass) {
+    const int64_t all = pass(base, found, found);
+    __syncthreads();
+    for (int64_t r = threadIdx.x; r < all && found + r < want; r += kPlanThreads) take(found + r, (int64_t)sh.found[r]);
+    found += all;
+    // (the next pass writes behind block_exclusive's barriers)
+  }
+  return true;
 }
 
 // The call's sequence that the rank-th page is for: the last whose needs begin at or before it.
@@ -163,17 +175,16 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const CacheView c
     return (length + more + page - 1) / page - (length + page - 1) / page;
   });
   if (!agreed(c, sh, w.header)) return;
-  if (want > 0 && lowest_free<false>(c, want, sh, [](int64_t, int64_t) {}) < want) {
-    if (threadIdx.x == 0) refuse(c.status, METIS_CACHE_NO_PAGES);
-    return;
-  }
-  __syncthreads();
-  lowest_free<true>(c, want, sh, [&](int64_t rank, int64_t p) {
+  const bool done = take_lowest(c, want, sh, [&](int64_t rank, int64_t p) {
     const int64_t i = owner_of(sh, w.needs, n, rank), slot = w.to[i];
     const int64_t first = (c.lengths[slot] + page - 1) / page;
     c.tables[slot * c.width + first + rank - w.needs[i]] = (int32_t)p;
     c.refs[p] = 1;
   });
+  if (!done) {
+    if (threadIdx.x == 0) refuse(c.status, METIS_CACHE_NO_PAGES);
+    return;
+  }
   __syncthreads();
   for (int64_t i = threadIdx.x; i < n; i += kPlanThreads)
     if (w.to[i] >= 0) c.lengths[w.to[i]] = w.length[i];
@@ -204,16 +215,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
     return share ? (length % page != 0) : (length + page - 1) / page;
   });
   if (!agreed(c, sh, w.header)) return;
-  if (want > 0 && lowest_free<false>(c, want, sh, [](int64_t, int64_t) {}) < want) {
-    if (threadIdx.x == 0) {
-      refuse(c.status, METIS_CACHE_NO_PAGES);
-      w.header->moves = -1;
-    }
-    return;
-  }
-  __syncthreads();
   // (a destination is empty, so that no source's table is written here)
-  lowest_free<true>(c, want, sh, [&](int64_t rank, int64_t p) {
+  const bool done = take_lowest(c, want, sh, [&](int64_t rank, int64_t p) {
     const int64_t i = owner_of(sh, w.needs, n, rank), from = w.from[i], to = w.to[i], length = w.length[i];
     const int64_t entry = (share ? length / page : 0) + rank - w.needs[i];
     c.tables[to * c.width + entry] = (int32_t)p;
@@ -221,6 +224,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
     const int32_t old = c.tables[from * c.width + entry];
     w.moves[rank] = Move{old, (int32_t)p, (int32_t)min(page, length - entry * page), 0};
   });
+  if (!done) {
+    if (threadIdx.x == 0) {
+      refuse(c.status, METIS_CACHE_NO_PAGES);
+      w.header->moves = -1;
+    }
+    return;
+  }
   __syncthreads();
   for (int64_t i = threadIdx.x; i < n; i += kPlanThreads)
     if (w.to[i] >= 0) c.lengths[w.to[i]] = w.length[i];
