@@ -304,9 +304,11 @@ enum MoveKind { kFork, kCompact };
 
 // Rows of kRun moves in a row of the plan's list, as pieces of V (16 bytes, or 8 where the rows of 8-bit elements end on half a piece): the filled rows
 // of a page lie in `places`, one for each layer, key or value and head, and are taken as one list, so that all threads have work whatever a page is filled with.
-// A block takes kBatch pieces a thread, all of its loads before its first store; what a prompt's group of answers copies is read once for kRun of them.
-constexpr int kBatch = 8, kRun = 4;
-template <typename V>
+// A block takes kBatch pieces a thread, all of its loads before its first store; what a prompt's group of answers copies is read once for kRun of them.  Forks, which
+// write more than they read, take four (92 registers a thread are 54): 32 prompts for 16 answers each, 500 tokens, 28 layers of 2 heads of 128, 32.4 -> 28.8 us with
+// free (511 tokens, last pages all but full: 56.5 -> 58.4); compactions eight (64 sequences of 30 pages of 28 layers: 293 us, 302 with four).  Runs of 8 or 16: 30.3 and 33.5.
+constexpr int kRun = 4;
+template <int kBatch, typename V>
 __device__ __forceinline__ void move_rows(const CacheView& c, const Move* moves, int count, int place_bytes, int places, int part) {
   const int row = c.head_dim * c.item;
   V v[kBatch];
@@ -343,12 +345,14 @@ __device__ __forceinline__ void move_rows(const CacheView& c, const Move* moves,
 
 // The plan's moves, and what goes with them: of a fork with shared pages the tables' rows and one more holder for each page; of a compaction the
 // pages' new numbers in all tables, and their holders.
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, const Work w, MoveKind kind, int64_t n) {
+template <MoveKind kKind>
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, const Work w, int64_t n) {
+  constexpr int kBatch = kKind == kFork ? 4 : 8;
   grid_dependency_wait();
   const int32_t moves = w.header->moves;
   if (moves < 0) return;
   const int64_t threads = (int64_t)gridDim.x * kMoveThreads, thread = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x;
-  if (kind == kFork) {
+  if constexpr (kKind == kFork) {
     for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
       if (w.to[i] < 0) continue;
       // the entries that the plan has not written are the source's
@@ -377,13 +381,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, c
   const int row = c.head_dim * c.item, piece = row * c.page_size, pieces = (int)(c.page_bytes / piece);
   const int unit = row % 16 == 0 ? 16 : 8;
   const int parts = (int)((c.page_bytes / unit + kBatch * kMoveThreads - 1) / (kBatch * kMoveThreads));      // of a full page
-  const int run = kind == kFork ? kRun : 1;
+  const int run = kKind == kFork ? kRun : 1;
   const int64_t runs = (moves + run - 1) / run;
   for (int64_t j = blockIdx.x; j < runs * parts; j += gridDim.x) {
     const int64_t r = j / parts;
     const int part = (int)(j - r * parts), count = (int)min((int64_t)run, moves - r * run);
-    if (unit == 16) move_rows<uint4>(c, w.moves + r * run, count, piece, pieces, part);
-    else            move_rows<uint2>(c, w.moves + r * run, count, piece, pieces, part);
+    if (unit == 16) move_rows<kBatch, uint4>(c, w.moves + r * run, count, piece, pieces, part);
+    else            move_rows<kBatch, uint2>(c, w.moves + r * run, count, piece, pieces, part);
   }
 }
 
@@ -398,7 +402,7 @@ int32_t check_call(const metis_cache* cache, CacheView* c, int64_t n, const void
 size_t mark_bytes(const CacheView& c) { return (size_t)((c.sequences + 31) / 32) * 4; }
 
 cudaError_t launch_moves(const CacheView& c, const Work& w, MoveKind kind, int64_t n, cudaStream_t st) {
-  return launch_overlapped(kLaunchShort, move_kernel, dim3((unsigned)device_sm_count() * 8), dim3(kMoveThreads), 0, st, c, w, kind, n);
+  return launch_overlapped(kLaunchShort, kind == kFork ? move_kernel<kFork> : move_kernel<kCompact>, dim3((unsigned)device_sm_count() * 8), dim3(kMoveThreads), 0, st, c, w, n);
 }
 
 std::atomic<int64_t> launches{0};
