@@ -197,8 +197,8 @@ struct Row {
       atomicAdd(&sh.bins[bin], 1u);
     }
   }
-  // Where the bins' sums, in order, reach the target; false if they do not.  unit: the bins', or their own where it is 1.
-  template <bool kMass> __device__ bool reach(double target, int unit, Found& out) {
+  // Where the bins' sums, in order, reach the target; false if they do not.  unit: the bins', or their own where it is 1.  A negative target stands for that share of all.
+  template <bool kMass> __device__ bool reach(double& target, int unit, Found& out, double& all) {
     cluster.sync();
     constexpr int kMost = kBins / kThreads;
     const int slice = kBins / blocks, mine = slice > kThreads ? slice / kThreads : 1;
@@ -217,8 +217,8 @@ struct Row {
       sum += v[i];
     }
     const Scan<double> s = block_scan<kThreads>(sum, sh.sums);
-    double all;
     const double base = ahead(s.all, all);
+    if (target < 0.0) target = fmax(-target * all, 1e-300);
     if (all < target) return false;                // the same for all blocks
     const double before = base + s.before, upto = base + s.upto;
     if (before < target && target <= upto) {
@@ -239,8 +239,9 @@ struct Row {
   }
 
   // The cut of the elements above `floor`: `at` such that the weights (or the number) of those above it are below the target and with those that equal
-  // it are not; what is above, and how many equal it.  False if all of them do not reach the target.
-  template <bool kMass> __device__ __forceinline__ bool cut(double target, float floor, float& at, double& above, double& ties) {
+  // it are not; what is above, how many equal it, and the sum of all.  False if all of them do not reach the target; a negative one is a share of all, and comes back as
+  // what that is.
+  template <bool kMass> __device__ __forceinline__ bool cut(double& target, float floor, float& at, double& above, double& ties, double& all) {
     clear();
     each([&](float v) {
       if (v > floor) {
@@ -250,7 +251,7 @@ struct Row {
     });
     if (threadIdx.x == 0) { sh.low = 0xffffffffu; sh.high = 0u; }
     Found f;
-    if (!reach<kMass>(target, 1, f)) return false;
+    if (!reach<kMass>(target, 1, f, all)) return false;
     above = f.above;
     const int bin = f.bin, unit = unit_of(bin);
     // the bin's smallest and largest keys
@@ -281,7 +282,8 @@ struct Row {
       });
       // (a target that rounding puts in front of the bin's first element, or behind its last, is met by that one)
       Found next;
-      if (!reach<kMass>(fmax(fmin(target - above, f.inside), 1e-300), unit, next)) return false;
+      double left = fmax(fmin(target - above, f.inside), 1e-300), of_bin;
+      if (!reach<kMass>(left, unit, next, of_bin)) return false;
       above += next.above;
       f.inside = next.inside;
       high -= (uint32_t)next.bin << shift;
@@ -302,28 +304,32 @@ struct Row {
     return fmin(n, limit);
   }
 
-  // Top-k and top-p by these histograms.  all_weights: of the whole row.  (A function of its own, for the registers of the way that needs none of it; by a
+  // Top-k and top-p by these histograms.  all_weights: of the whole row; where it is not known (0) and the nucleus is one of all, it comes out of the histogram: a pass over the row
+  // less, 256 rows of 151936 fp32 logits 505 -> 000 us.  (A function of its own, for the registers of the way that needs none of it; by a
   // copy of the row, whose members would come from memory for every element.)
-  static __device__ __noinline__ Cut by_weights(Row r, int64_t k, int64_t vocab, double top_p, double all_weights, int* turn) {
+  static __device__ __noinline__ Cut by_weights(Row r, int64_t k, int64_t vocab, double top_p, double* all_weights, int* turn) {
     Cut c = {-CUDART_INF_F, false, 0.0};
     double above = 0.0;
     if (k > 0 && k < vocab) {
       float at;
-      double equal;
-      if (r.cut<false>((double)k, -CUDART_INF_F, at, above, equal)) c = {at, true, (double)k - above};       // (else there are not so many)
+      double want = (double)k, equal, all;
+      if (r.cut<false>(want, -CUDART_INF_F, at, above, equal, all)) c = {at, true, (double)k - above};       // (else there are not so many)
     }
     if (top_p < 1.0) {
-      double total = all_weights, over = 0.0;
+      double total = *all_weights, over = 0.0;
       if (c.found) {
         double sum = 0.0;
         r.each([&](float v) { if (v > c.at) sum += (double)r.weight(v); });
         over = r.sum_of(sum);
         total = over + c.ties * (double)r.weight(c.at);
       }
-      const double target = fmax(top_p * total, 1e-300);                  // (the first one is always kept)
+      const bool share = !c.found && total == 0.0 && top_p > 0.0;
+      double target = share ? -top_p : fmax(top_p * total, 1e-300);       // (the first one is always kept)
       float at;
-      double before, equal;
-      if (r.cut<true>(target, c.at, at, before, equal)) c = {at, true, r.ties_below(target, before, at, equal)};
+      double before, equal, all;
+      const bool reached = r.cut<true>(target, c.at, at, before, equal, all);
+      if (share) *all_weights = all;
+      if (reached) c = {at, true, r.ties_below(target, before, at, equal)};
       else if (c.found) c.ties = r.ties_below(target, over, c.at, c.ties);  // all that are above the cut of top-k, and some that equal it
     }
     *turn = r.turn;
@@ -580,12 +586,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       settled = r.by_values(k, top_p, cut, all_weights);
       counted = true;
     }
-  if (!counted && !everything && (p.logprob || (filtered && top_p < 1.0))) {
+  // (a nucleus of all, without top-k, finds it by itself)
+  const bool found_later = !settled && top_p > 0.0 && top_p < 1.0 && !(k > 0 && k < p.vocab);
+  if (!counted && !everything && !found_later && (p.logprob || (filtered && top_p < 1.0))) {
     double sum = 0.0;
     r.each([&](float v) { sum += (double)r.weight(v); });
     all_weights = r.sum_of(sum);
   }
-  if (!settled) cut = Row<T>::by_weights(r, k, p.vocab, top_p, all_weights, &r.turn);
+  if (!settled) cut = Row<T>::by_weights(r, k, p.vocab, top_p, &all_weights, &r.turn);
   if (k == 1) cut = {top, true, 1.0};
 
   // ---- the kept weights of this thread's elements, in order of their indices ----
