@@ -8,7 +8,7 @@
 //   bf16  The bins are the values themselves, from the largest one on: 4095 of them, those below 2^-8 in magnitude together in one.  That is every logit
 //         within +-256.  A pass counts, five instructions and an addition in shared memory an element; a bin's weight is its count times the
 //         weight of its value, so that one histogram serves top-k, top-p and the sum of all.  (A cut in the bin of small values or behind the last one goes the other way.)
-//   fp32  2048 bins, first of (max - x) / T in steps of 1/64, then of the bits of the logits in the bin where the cut lies until one value is left.
+//   fp32  2048 bins of (max - x) / T in steps of 1/64, then 1024 at a time of the bits of the logits in the bin where the cut lies until one value is left.
 //
 // Whether a token is in or out goes by sums over up to all the vocabulary, and an fp32 sum would move borders with the order of its terms.  Here the
 // sums have 64 bits: counts times weights; or, of fp32, a bin's weights lie within a factor of 2^(1/44), all 24 bits of each are multiples of one unit, and the

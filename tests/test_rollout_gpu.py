@@ -1036,3 +1036,15 @@ def test_attend_refuses_groups_beyond_its_blocks():
     cache = filled([5], kv_heads=1, head_dim=16, seed=32)
     with pytest.raises(RuntimeError, match="1024 query heads"):
         cache.attend(0, normal(1, 1025, 16))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [2000, 40000, 152064])
+def test_sample_a_bin_that_holds_nearly_all(dtype, vocab):
+    """Distinct logits closer to one another than a first bin is wide, and a few far from them: more in the cut's bin than a block lists."""
+    x = (normal(2, vocab, seed=vocab, scale=1e-3, dtype=torch.float32) + 3.0).to(dtype)
+    x[0, 5:9] = 3.5
+    x[1, 100:150] = -40.0
+    u = torch.tensor([0.3, 0.9], device=DEV)
+    for kw in (dict(top_p=0.5), dict(top_k=777), dict(top_k=1500, top_p=0.25), dict(temperature=0.05, top_p=0.9)):
+        check_samples(x, u, **kw)
