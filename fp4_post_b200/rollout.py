@@ -210,7 +210,7 @@ class PagedCache:
     def attend(self, layer: int, q: torch.Tensor, slots=None, *, scale: Optional[float] = None, return_lse: bool = False):
         """softmax(scale q K^T) V of one token for each row over all keys of its sequence: bfloat16, shaped like q [rows, heads, head_dim].
 
-        Row i belongs to sequence slots[i] (None: i).  heads is a multiple of kv_heads; query head h reads key-value head h // (heads / kv_heads).  scale:
+        Row i belongs to sequence slots[i] (None: i).  heads is a multiple of kv_heads, at most 1024 times; query head h reads key-value head h // (heads / kv_heads).  scale:
         1 / sqrt(head_dim) where None.  A row without keys, or of no sequence, is zeros.  Products on the tensor core, statistics and sums in fp32; the
         result does not depend on the other rows of the call beyond where its keys are split.  return_lse: also the logarithm of each row's sum of
         exp(scale q k), float32 [rows, heads] (-inf without keys)."""

@@ -604,7 +604,7 @@ int32_t metis_rotary(const metis_rotary_args* args);
  */
 #define METIS_CACHE_NO_PAGES  16  /* not enough free pages */
 #define METIS_CACHE_BAD_SLOT  17  /* a sequence that the cache does not have */
-#define METIS_CACHE_TOO_LONG  18  /* longer than `width` pages, or a negative count */
+#define METIS_CACHE_TOO_LONG  18  /* longer than `width` pages, a negative count, or a length that no call leaves */
 #define METIS_CACHE_TWICE     19  /* the same sequence twice in one call */
 #define METIS_CACHE_NOT_EMPTY 20  /* a fork's destination that has a length */
 typedef struct metis_cache {
@@ -645,7 +645,7 @@ int32_t metis_cache_append(const metis_cache* cache, const metis_append_args* ar
 
 /*
  * Attention of one new token for each row: out[i] = softmax(scale q[i] K^T) V over the lengths[s] keys of sequence s = slots[i] (null: i),
- * head h of heads_q on key-value head h / (heads_q / kv_heads).  q and out bf16 [rows, heads_q, head_dim] (q with strides in elements, multiples
+ * head h of heads_q on key-value head h / (heads_q / kv_heads), at most 1024 on one.  q and out bf16 [rows, heads_q, head_dim] (q with strides in elements, multiples
  * of 2; out contiguous), lse (may be null) fp32 [rows, heads_q]: log of the sum of exp(scale q k).  No keys, or a sequence that the cache does not
  * have: zeros and -inf.  Work is split over all keys of all rows in equal parts whatever the lengths, parts of one row are joined in a second launch.
  */
