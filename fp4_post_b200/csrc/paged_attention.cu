@@ -633,6 +633,7 @@ struct Launch {
     int64_t n = 0;
     if (const int32_t rc = blocks(&n)) return rc;
     if (ws_bytes < workspace(n)) return fail(METIS_ERR_WORKSPACE, "the workspace has %lld bytes, %lld are needed", (long long)ws_bytes, (long long)workspace(n));
+    if (p.chunks > n) return fail(METIS_ERR_UNSUPPORTED, "the GPU holds %lld blocks, fewer than the group has pieces (%d)", (long long)n, p.chunks);
     const int64_t units = (int64_t)p.rows * p.kv_heads * p.chunks;
     p.by_unit = units <= n;
     char* w = static_cast<char*>(ws);

@@ -100,7 +100,8 @@ class Rotary:
 
     q [..., heads, head_dim] and k [..., kv_heads, head_dim] (or None), both bfloat16 or both float32, of any strides over a dense last dimension;
     positions int32 or int64, of the leading dimensions' shape or one that broadcasts to it (None: 0, 1, ... along the last of them).  Computed in
-    fp32, rounded once.  Results are contiguous.  Differentiable, any number of times, in q and k."""
+    fp32, rounded once.  Results are contiguous.  Differentiable, any number of times, in q and k; both directions can be captured in a CUDA graph (a
+    backward pass while no eager graph of the same leaves is kept: see graphs.py)."""
 
     def __init__(self, head_dim: int, *, theta: float = 1e4, rotary_dim: Optional[int] = None, interleaved: bool = False,
                  scaling: Optional[dict] = None, device: Union[str, torch.device] = "cuda"):
