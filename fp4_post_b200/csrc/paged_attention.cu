@@ -35,6 +35,7 @@ constexpr int kMinTiles = 8;              // of a part: two for each warp
 // What beginning and ending a row costs a block, in tiles: parts are equal in tiles and this for each row.  A batch of 256 rows of 1 to 2047 keys took
 // 85 us where short rows were counted by their tiles alone, 75 with 4, 57 with 16, 56 with 20 to 32; few long rows do not change.
 constexpr int kBegin = 20;
+constexpr int kUnitThreads = 512;         // of a block that joins one column of many pieces (111 of them: 20.5 us for the call, 20.7 with 256 threads, 21.8 with 1024)
 constexpr float kNone = -3.4028235e38f;   // the maximum of no scores: the lowest finite number, so that a score of -inf weighs nothing behind it, and any other something
 constexpr float kSlack = 8.0f;            // weights may be up to 2^8 before the maximum they are relative to is moved
 
@@ -56,8 +57,8 @@ struct AttendParams {
   float scale;                            // times log2(e)
   float* part_o;                          // [2 blocks, 8 NT, D]
   float2* part_ml;                        // [2 blocks, 8 NT]
-  // What the second launch joins: row, key-value head and chunk as one number, first and last part.  One place for each of those of each row where they are no
-  // more than blocks, else one for each block: that of the second piece.
+  // What the second launch joins: row, key-value head and chunk as one number, first and last part.  One place for each of those of each row where they are few (by_unit),
+  // else one for each block that goes on with what another one began.
   int4* join;
   bool by_unit;
 };
@@ -528,86 +529,95 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     }
     if (threadIdx.x == 0 && (p.by_unit ? begin == 0 : begin > 0)) {
       const int64_t start = (int64_t)before[row] * heads + (int64_t)head * row_cost + kBegin, last = start + row_tiles - 1;
-      const int64_t c0 = ((start + 1) * parts - 1) / total, c1 = ((last + 1) * parts - 1) / total;
       const int unit = head * p.chunks + chunk;
-      if (p.by_unit) p.join[row * heads * p.chunks + unit] = make_int4(whole ? -1 : row, unit, (int)c0, (int)c1);
-      else if (c0 == cta - 1) p.join[blockIdx.x] = make_int4(row, unit, (int)c0, (int)c1);
+      p.join[p.by_unit ? row * heads * p.chunks + unit : (int)blockIdx.x] =
+          make_int4(whole ? -1 : row, unit, (int)(((start + 1) * parts - 1) / total), (int)(((last + 1) * parts - 1) / total));
     }
     __syncthreads();                       // the ring is free again
   }
 }
 
-// Joins the pieces of a row and head that several blocks wrote, for one query head of the group.  A warp takes every eighth piece, a lane D / 32 elements.
-// kMany pieces (few units, so that there are few blocks): a lane looks at one piece's maximum and sum, and eight outputs are on their way at once; else
-// fewer registers, so that an SM takes twice the blocks, most of which have nothing to do.  32768 keys of one row, 111 pieces: 21.5 us with, 23.0
-// without; 256 rows in two or three pieces: 57.9 with, 54.5 without.
-template <int D, int NT, bool kMany>
-__global__ void __launch_bounds__(256, kMany ? 4 : 8) join_kernel(const AttendParams p) {
-  constexpr int E = D / 32;
-  __shared__ float acc_of[8][D];
-  __shared__ float sum_of[8];
+// Joins the pieces of a row and head that several blocks wrote.  A lane has D / 32 elements of one column (query head of the group), a warp some of its pieces, kAhead of them on
+// their way at once and the maxima beside them.
+//   by_unit   few rows and heads, of many pieces: a block for each column, whose warps share the pieces
+//   else      as many blocks as wrote pieces, and all but the first of those of one row and head share its columns among them, and a block's warps their pieces: of two pieces
+//             one block joins all columns, a warp each; of 100 a block joins one column with all its warps.  (256 rows in two or three pieces, with the rest of
+//             the call: 55.0 us by a block for each column and piece, 52.5 so; one row of 32768 keys 20.5 by unit, 23.6 this way.  64 rows of four
+//             pieces 31.1 by unit in blocks of 256 threads, 29.4 so.)
+template <int D> struct alignas(D == 64 ? 8 : 16) Lane { float v[D / 32]; };
+template <int D, int NT, bool kByUnit, int kJoinThreads>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendParams p) {
+  constexpr int kJoinWarps = kJoinThreads / 32, E = D / 32, kAhead = 4;
+  __shared__ Lane<D> acc_of[kJoinWarps][32];
+  __shared__ float sum_of[kJoinWarps];
   grid_dependency_wait();
   const int4 job = p.join[blockIdx.x];
   if (job.x < 0) return;
-  const int head = job.y / p.chunks, chunk = job.y - head * p.chunks, column = blockIdx.y;
-  if (chunk * 8 * NT + column >= p.group) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c0 = job.z;
-  const int pieces = job.w - job.z + 1;
-  auto place = [&](int i) { return (((c0 + i) * p.chunks + chunk) * 2 + (i == 0 ? 1 : 0)) * 8 * NT + column; };
-  float top = kNone;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[place(i)].x);
+  const int head = job.y / p.chunks, chunk = job.y - head * p.chunks;
+  const int columns = min(8 * NT, p.group - chunk * 8 * NT), pieces = job.w - job.z + 1;
+  const int helpers = kByUnit ? gridDim.y : pieces - 1, mine = kByUnit ? (int)blockIdx.y : (int)(blockIdx.x / p.chunks) - job.z - 1;        // blocks that share the columns
+  const int here = (columns - mine + helpers - 1) / helpers;
+  if (here <= 0) return;
+  int share = kJoinWarps;                  // warps of a column
+  while (share > 1 && share * here > kJoinWarps) share >>= 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp % share;
+  const float v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
+  for (int i = warp / share; i - warp / share < here; i += kJoinWarps / share) {
+    const int column = mine + i * helpers;
+    const bool live = i < here;
+    auto place = [&](int piece) { return (((int64_t)(job.z + piece) * p.chunks + chunk) * 2 + (piece == 0 ? 1 : 0)) * 8 * NT + column; };
+    Lane<D> acc;
+    float sum = 0.0f, top = kNone;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float acc[E], sum = 0.0f;
+    for (int e = 0; e < E; ++e) acc.v[e] = 0.0f;
+    if (live) {
+      float2 ml[kAhead];
+      Lane<D> o[kAhead];
+      auto load = [&](int from) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-  if constexpr (kMany) {
-    const int mine = (pieces - warp + 7) / 8;
-    for (int base = 0; base < mine; base += 32) {
-      // a lane has the maximum and sum of one piece, all lanes then go through the outputs of 32
-      const int own = (base + lane) * 8 + warp;
-      const float2 ml = own < pieces ? p.part_ml[place(own)] : make_float2(kNone, 0.0f);
-      const float f = own < pieces ? exp2_fast(ml.x - top) : 0.0f;
-      sum += ml.y * f;
-      const int here = min(32, mine - base);
-#pragma unroll 8
-      for (int j = 0; j < here; ++j) {
-        const float* from = p.part_o + place((base + j) * 8 + warp) * D + lane;
-        const float fj = __shfl_sync(0xffffffffu, f, j);
+        for (int a = 0; a < kAhead; ++a) {
+          const int64_t at = place(min(from + a * share, pieces - 1));
+          ml[a] = p.part_ml[at];
+          o[a] = reinterpret_cast<const Lane<D>*>(p.part_o + at * D)[lane];
+        }
+      };
+      load(first);
+      for (int j = lane; j < pieces; j += 32) top = fmaxf(top, p.part_ml[place(j)].x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += from[e * 32] * fj;
+      for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+      for (int from = first; from < pieces;) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          if (from + a * share >= pieces) continue;
+          const float f = exp2_fast(ml[a].x - top);
+          sum += ml[a].y * f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc.v[e] += o[a].v[e] * f;
+        }
+        from += kAhead * share;
+        if (from < pieces) load(from);
       }
     }
+    if (share > 1) {                       // (then there is one round, and all threads are in it)
+      acc_of[warp][lane] = acc;
+      if (lane == 0) sum_of[warp] = sum;
+      __syncthreads();
+      if (first > 0) continue;
+      for (int w = 1; w < share; ++w) {
+        const Lane<D> other = acc_of[warp + w][lane];
+        sum += sum_of[warp + w];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  } else {
-#pragma unroll 4
-    for (int i = warp; i < pieces; i += 8) {
-      const int64_t at = place(i);
-      const float2 ml = p.part_ml[at];
-      const float f = exp2_fast(ml.x - top);
-      sum += ml.y * f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += p.part_o[at * D + e * 32 + lane] * f;
+        for (int e = 0; e < E; ++e) acc.v[e] += other.v[e];
+      }
     }
+    if (!live) continue;
+    const int64_t to = (int64_t)job.x * p.heads_q + head * p.group + chunk * 8 * NT + column;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      if (lane * E + e < p.head_dim)
+        *reinterpret_cast<__nv_bfloat162*>(p.out + to * p.head_dim + lane * E + e) = __floats2bfloat162_rn(__fdiv_rn(acc.v[e], sum) * v_scale, __fdiv_rn(acc.v[e + 1], sum) * v_scale);
+    if (lane == 0 && p.lse) p.lse[to] = (top + log2f(sum)) * 0.69314718055994531f;
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc_of[warp][e * 32 + lane] = acc[e];
-  if (lane == 0) sum_of[warp] = sum;
-  __syncthreads();
-  const int64_t to = (int64_t)job.x * p.heads_q + head * p.group + chunk * 8 * NT + column;
-  const float v_scale = p.scales ? p.scales[p.kv_heads + head] : 1.0f;
-  float all = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) all += sum_of[w];
-  for (int e = threadIdx.x; e < p.head_dim; e += 256) {
-    float a = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) a += acc_of[w][e];
-    p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(a, all) * v_scale);
-  }
-  if (threadIdx.x == 0 && p.lse) p.lse[to] = (top + log2f(all)) * 0.69314718055994531f;
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -635,15 +645,15 @@ struct Launch {
     if (ws_bytes < workspace(n)) return fail(METIS_ERR_WORKSPACE, "the workspace has %lld bytes, %lld are needed", (long long)ws_bytes, (long long)workspace(n));
     if (p.chunks > n) return fail(METIS_ERR_UNSUPPORTED, "the GPU holds %lld blocks, fewer than the group has pieces (%d)", (long long)n, p.chunks);
     const int64_t units = (int64_t)p.rows * p.kv_heads * p.chunks;
-    p.by_unit = units <= n;
+    p.by_unit = units * 8 <= n;
     char* w = static_cast<char*>(ws);
     p.join = reinterpret_cast<int4*>(w);
     p.part_ml = reinterpret_cast<float2*>(w + n * 16);
     p.part_o = reinterpret_cast<float*>(w + n * (16 + 16 * NT * 8));
     METIS_CUDA_OK(launch_overlapped(kLaunchShort, attend_kernel<D, NT, kE4m3>, dim3((unsigned)n), dim3(kThreads), L::kSmem, st, p));
-    const int64_t joins = p.by_unit ? units : n;
-    const auto join = p.by_unit && units * 8 <= n ? join_kernel<D, NT, true> : join_kernel<D, NT, false>;
-    METIS_CUDA_OK(launch_overlapped(kLaunchShort, join, dim3((unsigned)joins, (unsigned)(p.group < 8 * NT ? p.group : 8 * NT)), dim3(256), 0, st, p));
+    const int columns = p.group < 8 * NT ? p.group : 8 * NT;
+    if (p.by_unit) METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT, true, kUnitThreads>, dim3((unsigned)units, (unsigned)columns), dim3(kUnitThreads), 0, st, p));
+    else           METIS_CUDA_OK(launch_overlapped(kLaunchShort, join_kernel<D, NT, false, 256>, dim3((unsigned)n), dim3(256), 0, st, p));
     count_rollout_launches(2);
     return METIS_OK;
   }
