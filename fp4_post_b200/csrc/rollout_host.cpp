@@ -1,7 +1,7 @@
 // The host side of rollout.py: checks, allocations and calls of the kernels of a rollout, and the rotary positions as a native autograd function.
 //
 // A decode step makes two of these calls in every layer, for kernels of a few microseconds: from Python, with its checks and a foreign call of twenty
-// arguments, each would cost several times that.  A cache is a capsule of its tensors, checked once.
+// arguments, each would cost several times that.  A cache is a capsule of its tensors: what they are is settled once, where their memory is at each call.
 #include <Python.h>
 
 #include <torch/csrc/Exceptions.h>
@@ -290,10 +290,36 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // ---- the cache --------------------------------------------------------------------------------------------------------
 
+// A tensor of a cache, as it was when the cache was made.
+struct Held {
+  const char* name;
+  Tensor t;
+  at::ScalarType type = at::kInt;
+  std::vector<int64_t> shape;
+  void keep(const Tensor& tensor) { t = tensor; type = t.scalar_type(); shape = t.sizes().vec(); }
+  // Where its memory is now: a storage may be given back and taken again between two calls, or a tensor be set to another one's.
+  void* address(const c10::Device& device) const {
+    if (!t.defined()) return nullptr;
+    TORCH_CHECK_VALUE(t.device() == device && t.scalar_type() == type && t.sizes() == shape && t.is_contiguous(),
+                      "the cache's ", name, " has become another tensor: ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", it was ", type, " ", at::IntArrayRef(shape), " on ", device);
+    const size_t has = t.storage().nbytes(), needs = (size_t)(t.storage_offset() + t.numel()) * t.element_size();
+    TORCH_CHECK_VALUE(has >= needs, "the cache's ", name, " has no memory: a storage of ", has, " bytes for ", needs);
+    return t.data_ptr();
+  }
+};
 struct Cache {
-  Tensor pool, tables, lengths, refs, scales, status;
-  metis_cache c = {};
+  Held pool{"pool"}, tables{"tables"}, lengths{"lengths"}, refs{"refs"}, scales{"scales"}, status{"status"};
+  metis_cache c = {};                   // sizes; addresses are those of `now`
   c10::Device device = c10::Device(c10::kCPU);
+  metis_cache now() const {
+    metis_cache m = c;
+    m.pool = pool.address(device);
+    TORCH_CHECK_VALUE((reinterpret_cast<uintptr_t>(m.pool) & 15) == 0, "the cache's pool must be 16-byte aligned");
+    m.tables = static_cast<int32_t*>(tables.address(device)); m.lengths = static_cast<int32_t*>(lengths.address(device));
+    m.refs = static_cast<int32_t*>(refs.address(device)); m.scales = static_cast<const float*>(scales.address(device));
+    m.status = static_cast<int32_t*>(status.address(device));
+    return m;
+  }
 };
 constexpr const char* kCapsule = "metis_cache";
 
@@ -309,35 +335,35 @@ Cache& cache_of(Args& a) {
 PyObject* cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ROLLOUT_BEGIN(args, nargs)
   auto h = std::make_unique<Cache>();
-  h->pool = a.tensor("pool"); h->tables = a.tensor("tables"); h->lengths = a.tensor("lengths"); h->refs = a.tensor("refs");
-  h->scales = a.optional("scales"); h->status = a.tensor("status");
-  const Tensor& pool = h->pool;
+  const Tensor pool = a.tensor("pool"), tables = a.tensor("tables"), lengths = a.tensor("lengths"), refs = a.tensor("refs"), scales = a.optional("scales"), status = a.tensor("status");
   const bool e4m3 = pool.scalar_type() == at::kFloat8_e4m3fn;
   check_tensor(pool, "pool", e4m3 ? at::kFloat8_e4m3fn : at::kBFloat16, "bfloat16 or float8_e4m3fn");
   TORCH_CHECK_VALUE(pool.dim() == 6 && pool.size(2) == 2, "pool must be [pages, layers, 2, kv_heads, page_size, head_dim], not ", pool.sizes());
   h->device = pool.device();
-  for (const auto& [t, name] : {std::make_pair(&h->tables, "tables"), std::make_pair(&h->lengths, "lengths"), std::make_pair(&h->refs, "refs"), std::make_pair(&h->status, "status")}) {
+  for (const auto& [t, name] : {std::make_pair(&tables, "tables"), std::make_pair(&lengths, "lengths"), std::make_pair(&refs, "refs"), std::make_pair(&status, "status")}) {
     check_tensor(*t, name, at::kInt, "int32");
     check_device(*t, name, h->device);
     TORCH_CHECK_VALUE(t->is_contiguous(), name, " must be contiguous");
   }
   TORCH_CHECK_VALUE(pool.is_contiguous() && aligned16(pool), "pool must be contiguous and 16-byte aligned");
-  TORCH_CHECK_VALUE(h->tables.dim() == 2 && h->lengths.dim() == 1 && h->lengths.size(0) == h->tables.size(0), "tables ", h->tables.sizes(), " and lengths ", h->lengths.sizes(), " do not fit");
-  TORCH_CHECK_VALUE(h->refs.dim() == 1 && h->refs.size(0) == pool.size(0), "refs ", h->refs.sizes(), " do not fit a pool of ", pool.size(0), " pages");
-  TORCH_CHECK_VALUE(h->status.numel() == 1, "status must have one element");
-  TORCH_CHECK_VALUE(e4m3 == h->scales.defined(), "scales go with float8_e4m3fn, and with nothing else");
+  TORCH_CHECK_VALUE(tables.dim() == 2 && lengths.dim() == 1 && lengths.size(0) == tables.size(0), "tables ", tables.sizes(), " and lengths ", lengths.sizes(), " do not fit");
+  TORCH_CHECK_VALUE(refs.dim() == 1 && refs.size(0) == pool.size(0), "refs ", refs.sizes(), " do not fit a pool of ", pool.size(0), " pages");
+  TORCH_CHECK_VALUE(status.numel() == 1, "status must have one element");
+  TORCH_CHECK_VALUE(e4m3 == scales.defined(), "scales go with float8_e4m3fn, and with nothing else");
   if (e4m3) {
-    check_tensor(h->scales, "scales", at::kFloat, "float32");
-    check_device(h->scales, "scales", h->device);
-    TORCH_CHECK_VALUE(h->scales.is_contiguous() && h->scales.dim() == 3 && h->scales.size(0) == pool.size(1) && h->scales.size(1) == 2 && h->scales.size(2) == pool.size(3),
-                      "scales must be contiguous [layers, 2, kv_heads], not ", h->scales.sizes());
+    check_tensor(scales, "scales", at::kFloat, "float32");
+    check_device(scales, "scales", h->device);
+    TORCH_CHECK_VALUE(scales.is_contiguous() && scales.dim() == 3 && scales.size(0) == pool.size(1) && scales.size(1) == 2 && scales.size(2) == pool.size(3),
+                      "scales must be contiguous [layers, 2, kv_heads], not ", scales.sizes());
+    h->scales.keep(scales);
   }
+  h->pool.keep(pool); h->tables.keep(tables); h->lengths.keep(lengths); h->refs.keep(refs); h->status.keep(status);
   metis_cache& c = h->c;
-  c.pool = pool.data_ptr(); c.pages = pool.size(0); c.layers = (int32_t)pool.size(1); c.kv_heads = (int32_t)pool.size(3);
+  c.pages = pool.size(0); c.layers = (int32_t)pool.size(1); c.kv_heads = (int32_t)pool.size(3);
   c.page_size = (int32_t)pool.size(4); c.head_dim = (int32_t)pool.size(5); c.dtype = e4m3 ? METIS_DTYPE_E4M3 : METIS_DTYPE_BF16;
-  c.tables = ptr<int32_t>(h->tables); c.sequences = h->tables.size(0); c.width = h->tables.size(1);
-  c.lengths = ptr<int32_t>(h->lengths); c.refs = ptr<int32_t>(h->refs); c.scales = ptr<float>(h->scales); c.status = ptr<int32_t>(h->status);
-  check(lib.metis_cache_check(&c), "metis_cache_check");
+  c.sequences = tables.size(0); c.width = tables.size(1);
+  const metis_cache m = h->now();
+  check(lib.metis_cache_check(&m), "metis_cache_check");
   PyObject* o = PyCapsule_New(h.get(), kCapsule, drop_cache);
   if (o) h.release();
   return o;
@@ -368,6 +394,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool interleaved = a.truth();
   check_untraced();
   TORCH_CHECK_VALUE(layer >= 0 && layer < h.c.layers, "layer ", layer, " of a cache of ", h.c.layers);
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   k = heads_of(k, "k", h, -1, h.c.kv_heads, 8);
   const int64_t tokens = k.size(0);
@@ -393,7 +420,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       g.k = k.data_ptr(); g.k_token = k.stride(0); g.k_head = k.stride(1);
       g.v = v.data_ptr(); g.v_token = v.stride(0); g.v_head = v.stride(1);
       g.stream = stream_of(h.device);
-      check(lib.metis_cache_append(&h.c, &g), "metis_cache_append");
+      check(lib.metis_cache_append(&m, &g), "metis_cache_append");
     }
   }
   return out.defined() ? THPVariable_Wrap(out) : Py_NewRef(Py_None);
@@ -410,6 +437,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool want_lse = a.truth();
   check_untraced();
   TORCH_CHECK_VALUE(layer >= 0 && layer < h.c.layers, "layer ", layer, " of a cache of ", h.c.layers);
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   q = heads_of(q, "q", h, -1, -1, 2);
   TORCH_CHECK_VALUE(q.size(1) > 0 && q.size(1) % h.c.kv_heads == 0, "q has ", q.size(1), " heads, which ", h.c.kv_heads, " key-value heads do not divide");
@@ -425,11 +453,11 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       g.slots = ptr(slots); g.slots_64 = wide(slots); g.scale = (float)scale;
       g.q = q.data_ptr(); g.q_row = q.stride(0); g.q_head = q.stride(1);
       g.out = out.data_ptr(); g.lse = ptr<float>(lse);
-      const int64_t bytes = lib.metis_cache_attend_workspace_bytes(&h.c, g.rows, g.heads_q);
+      const int64_t bytes = lib.metis_cache_attend_workspace_bytes(&m, g.rows, g.heads_q);
       const Tensor ws = empty_on(h.device, {bytes < 16 ? 16 : bytes}, at::kByte);
       g.workspace = ws.data_ptr(); g.workspace_bytes = ws.numel();
       g.stream = stream_of(h.device);
-      check(lib.metis_cache_attend(&h.c, &g), "metis_cache_attend");
+      check(lib.metis_cache_attend(&m, &g), "metis_cache_attend");
     }
   }
   return tuple_of({out, lse});
@@ -443,6 +471,7 @@ PyObject* reserve(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Tensor slots = a.optional("slots"), counts = a.optional("counts");
   const int64_t count = a.i64();
   check_untraced();
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   slots = indices(slots, "slots", h.device, -1);
   const int64_t n = slots.defined() ? slots.numel() : h.c.sequences;
@@ -451,8 +480,8 @@ PyObject* reserve(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (slots.defined() && counts.defined() && wide(slots) != wide(counts)) { slots = slots.to(at::kLong); counts = counts.to(at::kLong); }
   if (n > 0) {
     NoGil free_;
-    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&h.c, n)}, at::kByte);
-    check(lib.metis_cache_reserve(&h.c, ptr(slots), ptr(counts), count, wide(slots) || wide(counts), n, ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_reserve");
+    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&m, n)}, at::kByte);
+    check(lib.metis_cache_reserve(&m, ptr(slots), ptr(counts), count, wide(slots) || wide(counts), n, ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_reserve");
   }
   Py_RETURN_NONE;
   ROLLOUT_END
@@ -465,6 +494,7 @@ PyObject* fork(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Tensor src = a.tensor("src"), dst = a.tensor("dst");
   const bool share = a.truth();
   check_untraced();
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   src = indices(src, "src", h.device, -1);
   dst = indices(dst, "dst", h.device, src.numel());
@@ -472,8 +502,8 @@ PyObject* fork(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t n = src.numel();
   if (n > 0) {
     NoGil free_;
-    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&h.c, n)}, at::kByte);
-    check(lib.metis_cache_fork(&h.c, src.data_ptr(), dst.data_ptr(), wide(src), n, share, ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_fork");
+    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&m, n)}, at::kByte);
+    check(lib.metis_cache_fork(&m, src.data_ptr(), dst.data_ptr(), wide(src), n, share, ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_fork");
   }
   Py_RETURN_NONE;
   ROLLOUT_END
@@ -485,9 +515,10 @@ PyObject* release(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Cache& h = cache_of(a);
   const Tensor slots = indices(a.optional("slots"), "slots", h.device, -1);
   check_untraced();
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   const int64_t n = slots.defined() ? slots.numel() : h.c.sequences;
-  if (n > 0) check(lib.metis_cache_free(&h.c, ptr(slots), wide(slots), n, stream_of(h.device)), "metis_cache_free");
+  if (n > 0) check(lib.metis_cache_free(&m, ptr(slots), wide(slots), n, stream_of(h.device)), "metis_cache_free");
   Py_RETURN_NONE;
   ROLLOUT_END
 }
@@ -497,13 +528,14 @@ PyObject* compact(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ROLLOUT_BEGIN(args, nargs)
   Cache& h = cache_of(a);
   check_untraced();
+  const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   Tensor live;
   {
     NoGil free_;
     live = empty_on(h.device, {1}, at::kInt);
-    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&h.c, 1)}, at::kByte);
-    check(lib.metis_cache_compact(&h.c, ptr<int32_t>(live), ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_compact");
+    const Tensor ws = empty_on(h.device, {lib.metis_cache_workspace_bytes(&m, 1)}, at::kByte);
+    check(lib.metis_cache_compact(&m, ptr<int32_t>(live), ws.data_ptr(), ws.numel(), stream_of(h.device)), "metis_cache_compact");
   }
   return THPVariable_Wrap(live);
   ROLLOUT_END
