@@ -15,8 +15,9 @@
 // and output to the workspace, and a second launch joins them in order.
 //
 // p goes into its product as two bf16 numbers (off by 2^-15 together: the first is less than 2^-7 of p below it, the second rounds that by 2^-8 of
-// itself), or one fp16 number (2^-12, with e4m3): the rounding of the output, 2^-9 on the average, is the only one that counts.  Statistics and sums
-// are fp32.
+// itself), or with e4m3 one fp16 number, of 2^11 to 2^15 times what it is to the warp's largest: off by 2^-12 of itself, or, below 2^-25 of that one, where it is subnormal,
+// by 2^-36 of it (taken as it is, a row with 95 % of its weight on one token lost the others' bits: 2^-25, and all of what lay below).  The rounding of the
+// output, 2^-9 on the average, is the only one that counts.  Statistics and sums are fp32.
 #include "rollout.cuh"
 
 #include <cuda_fp16.h>
@@ -37,7 +38,10 @@ constexpr int kMinTiles = 8;              // of a part: two for each warp
 constexpr int kBegin = 20;
 constexpr int kUnitThreads = 512;         // of a block that joins one column of many pieces (111 of them: 20.5 us for the call, 20.7 with 256 threads, 21.8 with 1024)
 constexpr float kNone = -3.4028235e38f;   // the maximum of no scores: the lowest finite number, so that a score of -inf weighs nothing behind it, and any other something
-constexpr float kSlack = 8.0f;            // weights may be up to 2^8 before the maximum they are relative to is moved
+// Weights are relative to a number that is moved when one of them would pass 2^slack: to the largest score, so that bf16 weights are 1 then, or as far under it as fp16, whose smallest
+// normal number is 2^-14, is better filled from above.
+template <bool kE4m3> constexpr float kSlack = kE4m3 ? 15.0f : 8.0f;
+template <bool kE4m3> constexpr float kUnder = kE4m3 ? 11.0f : 0.0f;
 
 struct AttendParams {
   const __nv_bfloat16* q;
@@ -399,25 +403,26 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
               if (g + (e >> 1) * 8 >= live_keys) s[u][n][e] = -CUDART_INF_F;
         }
       }
-      // ---- softmax: the maximum that weights are relative to moves when one of them would pass 2^8, and the sums with it ----
+      // ---- softmax: what weights are relative to moves when one of them would be too large, and the sums with it ----
       bool over = false;
 #pragma unroll
       for (int u = 0; u < MT; ++u)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) over |= s[u][n][e] - m[n][e & 1] > kSlack;
+          for (int e = 0; e < 4; ++e) over |= s[u][n][e] - m[n][e & 1] > kSlack<kE4m3>;
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = m[n][j];
+            float top = -CUDART_INF_F;
 #pragma unroll
             for (int u = 0; u < MT; ++u) top = fmaxf(top, fmaxf(s[u][n][j], s[u][n][2 + j]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(m[n][j], top - kUnder<kE4m3>);
             const float keep = exp2_fast(m[n][j] - top);
             m[n][j] = top;
             l[n][j] *= keep;

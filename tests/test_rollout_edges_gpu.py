@@ -80,3 +80,43 @@ def test_a_cache_whose_tensors_have_become_others_is_refused():
     cache.scales.untyped_storage().resize_(0)
     with pytest.raises(ValueError, match="scales"):
         cache.attend(0, q)
+
+
+# ---- weights far below the largest ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("spread", [0.0, 0.5])
+@pytest.mark.parametrize("n, low", [(65536, 26.0), (16384, 20.0), (3000, 12.0)])
+def test_attend_keeps_what_lies_under_a_heavy_token(n, low, spread):
+    """One token with nearly all of the weight and a value of zero, as a row's first one is in many models: the others' weights are 2^-low of its own, and the output is theirs
+    alone.  All rows read the same pages, and there are as many of them as keep a row in one or two blocks.  8-bit pages: a weight goes into its product as fp16 of 2^11 times what it
+    is to the largest at least: off by 2^-12 of itself, or where that is subnormal by 2^-25, 2^-36 of the largest."""
+    rows, d = 512, 64
+    pages = n // 16 + 1
+    k, v = torch.zeros(n, d, device=DEV), 1.0 + 0.25 * torch.randn(n, d, device=DEV, generator=gen(50))
+    k[:, 1:] = torch.randn(n, d - 1, device=DEV, generator=gen(51)) * spread
+    k[0], v[0] = 0.0, 0.0
+    k[0, 0] = 256.0
+    pool = torch.zeros(pages, 1, 2, 1, 16, d, device=DEV)
+    for i, t in enumerate((k, v)):
+        pool[:, 0, i, 0] = torch.cat((t, torch.zeros(pages * 16 - n, d, device=DEV))).view(pages, 16, d)
+    q = (torch.randn(rows, 1, d, device=DEV, generator=gen(52)) * 0.25).bfloat16()
+    q[:, :, 0] = low * math.log(2.0) / 32.0
+    slots = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    cache = rollout.PagedCache.of(pool.to(torch.float8_e4m3fn), torch.arange(pages, device=DEV, dtype=torch.int32)[None].contiguous(), torch.tensor([n], device=DEV, dtype=torch.int32),
+                                  torch.ones(pages, device=DEV, dtype=torch.int32), scales=torch.ones(1, 2, 1, device=DEV))
+    out, lse = cache.attend(0, q, slots, scale=0.125, return_lse=True)
+    kv = keys_values(cache, 0, 0, n)[:, 0]
+    x = q[:, 0].double() @ kv[0].t() * 0.125
+    p = torch.softmax(x, dim=1)
+    want, spread_v = p @ kv[1], p @ kv[1].abs()
+    # (scores: fp32 sums of 64 products, queries to 2^-25 of their largest; see check_attend)
+    e = 6 * 2.0 ** -22 * (q[:, 0].double().abs() @ kv[0].abs().t() * 0.125).amax(dim=1, keepdim=True) + 2.0 ** -20
+    e = e + q[:, 0].double().abs().amax(dim=1, keepdim=True) * 2.0 ** -25 * kv[0].abs().sum(dim=1).max() * 0.125
+    # A lane adds up to an eighth of a warp's fourth of a row's weights one after the other in fp32, each addition off by up to 2^-24 of the sum (behind the heavy one all that are below
+    # 2^-24 of it leave it as it is); the tensor core 16 keys at a time, cut by 2^-22.
+    summed = (n / 32 + 8) * 2.0 ** -24
+    bound = 2.0 ** -8 * want.abs() + (2 * (e + 2.0 ** -12) + summed + (n / 64 + 8) * 2.0 ** -22) * spread_v + 2.0 ** -36 * p.amax(dim=1, keepdim=True) * kv[1].abs().sum(dim=0)
+    off = (out[:, 0].double() - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+    true_lse = torch.logsumexp(x, dim=1)
+    assert ((lse[:, 0].double() - true_lse).abs() <= e[:, 0] + summed + 2.0 ** -22 * true_lse.abs() + 2.0 ** -20).all()
