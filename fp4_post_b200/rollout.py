@@ -115,7 +115,8 @@ class Rotary:
         frequencies, self.magnitude = rotary_frequencies(self.rotary_dim, theta, scaling)
         # fractions of a turn in 64 bits: a product with a position, taken modulo 2^64, is the angle modulo a turn
         bits = [round(f / (2.0 * math.pi) * 2.0 ** 64) % 2 ** 64 for f in frequencies]
-        self.turns = torch.tensor([b - 2 ** 64 if b >= 2 ** 63 else b for b in bits], dtype=torch.int64, device=device)
+        with torch.inference_mode(False):        # (one made while generating is there to train with afterwards: an inference tensor cannot be saved for a backward pass)
+            self.turns = torch.tensor([b - 2 ** 64 if b >= 2 ** 63 else b for b in bits], dtype=torch.int64, device=device)
 
     def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None):
         """(q, k) turned; q alone where there is no k."""

@@ -120,3 +120,26 @@ def test_attend_keeps_what_lies_under_a_heavy_token(n, low, spread):
     assert (off <= bound).all(), float((off / bound).max())
     true_lse = torch.logsumexp(x, dim=1)
     assert ((lse[:, 0].double() - true_lse).abs() <= e[:, 0] + summed + 2.0 ** -22 * true_lse.abs() + 2.0 ** -20).all()
+
+
+# ---- inference mode ---------------------------------------------------------------------------------------------------
+
+def test_rotary_positions_made_in_inference_mode_train():
+    with torch.inference_mode():
+        r = rollout.Rotary(64)
+        r(normal(3, 2, 64))
+    x = normal(3, 2, 64).requires_grad_()
+    (g,) = torch.autograd.grad(r(x).float().sum(), x)
+    assert torch.equal(g, torch.autograd.grad(rollout.Rotary(64)(x).float().sum(), x)[0])
+
+
+@pytest.mark.parametrize("graphed", [False, True])
+def test_training_goes_on_behind_a_rollout_in_inference_mode(graphed):
+    model, twin = decoder(fuse_rotary=True), decoder(fuse_rotary=True)
+    ids = prompts(2, 24)
+    with torch.inference_mode():
+        tokens = model.generate(ids, max_new_tokens=5, answers=2, temperature=0.0, graphed=graphed)
+    assert torch.equal(tokens, twin.generate(ids, max_new_tokens=5, answers=2, temperature=0.0))
+    for m in (model, twin):
+        m.loss(ids).backward()
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(model.parameters(), twin.parameters()))
