@@ -164,7 +164,8 @@ class PagedCache:
     def _set(self, pool, tables, lengths, refs, scales):
         if not isinstance(pool, torch.Tensor):
             raise TypeError(f"pool must be a tensor, not {type(pool).__name__}")
-        status = torch.zeros(1, dtype=torch.int32, device=pool.device)
+        with torch.inference_mode(False):        # (check() writes to it in whatever mode)
+            status = torch.zeros(1, dtype=torch.int32, device=pool.device)
         self._handle = cabi.rollout_host().cache(pool, tables, lengths, refs, scales, status)
         self._tensors = (pool, tables, lengths, refs, scales, status)
         self._host = cabi.rollout_host()

@@ -143,3 +143,16 @@ def test_training_goes_on_behind_a_rollout_in_inference_mode(graphed):
     for m in (model, twin):
         m.loss(ids).backward()
     assert all(torch.equal(a.grad, b.grad) for a, b in zip(model.parameters(), twin.parameters()))
+
+
+def test_a_cache_made_in_inference_mode_tells_its_reason_outside():
+    with torch.inference_mode():
+        cache = new_cache(pages=2)
+    cache.reserve([0], 100)
+    with pytest.raises(RuntimeError, match="not enough free pages"):
+        cache.check()
+    cache.check()
+    with torch.inference_mode():
+        cache.reserve([9], 1)
+        with pytest.raises(RuntimeError, match="does not have"):
+            cache.check()
