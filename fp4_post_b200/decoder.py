@@ -252,7 +252,7 @@ class Decoder(nn.Module):
         self.cfg = cfg
         self.fuse_dense = fuse_dense
         self.fuse_rotary = fuse_rotary
-        self._rotaries = {}              # by device: the frequencies, no parameter of the model
+        self._rotaries = {}              # by device and configuration: the frequencies, no parameter of the model
         self.embed_tokens = nn.Embedding(cfg.vocab, cfg.hidden)
         self.layers = nn.ModuleList(Block(cfg, fuse_norms, fuse_dense) for _ in range(cfg.layers))
         self.norm = RMSNorm(cfg.hidden, cfg.eps)
@@ -262,11 +262,12 @@ class Decoder(nn.Module):
         return _rotary_tables(self.cfg, T, device, dtype)
 
     def _rotary_of(self, device: torch.device) -> rollout.Rotary:
-        """The configuration's rotary positions on a device, made once."""
+        """The configuration's rotary positions on a device, made once for what the configuration is.  (All are kept: a captured graph reads its own.)"""
         c = self.cfg
-        r = self._rotaries.get(device)
+        key = device, c.head_dim, c.rope_theta, c.rotary_dim, c.rope_interleaved, None if c.rope_scaling is None else tuple(sorted(c.rope_scaling.items()))
+        r = self._rotaries.get(key)
         if r is None:
-            r = self._rotaries[device] = rollout.Rotary(c.head_dim, theta=c.rope_theta, rotary_dim=c.rotary_dim, interleaved=c.rope_interleaved, scaling=c.rope_scaling, device=device)
+            r = self._rotaries[key] = rollout.Rotary(c.head_dim, theta=c.rope_theta, rotary_dim=c.rotary_dim, interleaved=c.rope_interleaved, scaling=c.rope_scaling, device=device)
         return r
 
     def hidden(self, ids: torch.Tensor) -> torch.Tensor:

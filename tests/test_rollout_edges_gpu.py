@@ -156,3 +156,25 @@ def test_a_cache_made_in_inference_mode_tells_its_reason_outside():
         cache.reserve([9], 1)
         with pytest.raises(RuntimeError, match="does not have"):
             cache.check()
+
+
+# ---- configurations that change ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("change", [dict(rope_theta=1e4), dict(rope_scaling=dict(type="linear", factor=4.0)), dict(rotary_dim=32), dict(rope_interleaved=True)])
+def test_fused_rotary_positions_follow_the_configuration(change):
+    """As the tables do, which are made anew for each call."""
+    import dataclasses
+    model = decoder(dataclasses.replace(SMALL), fuse_rotary=True)
+    ids = prompts(2, 40)
+    model.generate(ids, max_new_tokens=2)
+    for name, value in change.items():
+        setattr(model.cfg, name, value)
+    fresh = decoder(dataclasses.replace(SMALL, **change), fuse_rotary=True)
+    with torch.no_grad():
+        assert torch.equal(model(ids), fresh(ids))
+    assert torch.equal(model.generate(ids, max_new_tokens=6, temperature=0.0), fresh.generate(ids, max_new_tokens=6, temperature=0.0))
+    if "rope_scaling" in change:
+        model.cfg.rope_scaling["factor"] = 8.0               # (changed in place)
+        fresh = decoder(dataclasses.replace(SMALL, rope_scaling=dict(type="linear", factor=8.0)), fuse_rotary=True)
+        with torch.no_grad():
+            assert torch.equal(model(ids), fresh(ids))
