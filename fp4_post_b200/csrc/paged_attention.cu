@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
       length_of[row] = length;
     }
     const int32_t ahead = base ? before[base] : 0;
-    const Scan<int32_t> s = block_scan<kThreads>(length ? (length + L::kTile - 1) / L::kTile + kBegin : 0, warp_sums);
+    const Scan<int32_t> s = block_scan<kThreads>(length ? (length - 1) / L::kTile + 1 + kBegin : 0, warp_sums);
     if (row <= p.rows) before[row] = ahead + s.before;
     if (threadIdx.x == kThreads - 1 && row < p.rows) before[row + 1] = ahead + s.upto;
     __syncthreads();
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
       if (fetched < mine_count) {
         if ((fetched * MT & 31) == 0) {
           const int which = (first + (fetched + lane / MT) * kWarps) * MT + lane % MT;
-          const bool in = which * kRows < keys_all && which < tiles_end * MT;
+          const bool in = which < tiles_end * MT && which * kRows < keys_all;          // (a number of tiles behind the last one may be past 32 bits in keys)
           page = in ? table[which / page_rows] : -1;
           piece_on_page = which % page_rows;
         }

@@ -178,3 +178,19 @@ def test_fused_rotary_positions_follow_the_configuration(change):
         fresh = decoder(dataclasses.replace(SMALL, rope_scaling=dict(type="linear", factor=8.0)), fuse_rotary=True)
         with torch.no_grad():
             assert torch.equal(model(ids), fresh(ids))
+
+
+# ---- the longest sequences ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_attend_at_the_longest_length(dtype):
+    """2^31 - 16 tokens are what a table's 32-bit lengths end at; all pages but three are absent, so that no memory is asked for but the table's."""
+    short = filled([43], seed=26, dtype=dtype)
+    longest = 2 ** 31 - 16
+    tables = torch.full((1, longest // 16), -1, dtype=torch.int32, device=DEV)
+    for at, page in ((0, 0), (2 ** 26 + 5, 1), (longest // 16 - 1, 2)):
+        tables[0, at] = short.tables[0, page]
+    cache = rollout.PagedCache.of(short.pool, tables, torch.tensor([longest - 5], dtype=torch.int32, device=DEV), short.refs, scales=short.scales)
+    q = normal(1, 4, 64, seed=27)
+    out, lse = cache.attend(0, q, return_lse=True)
+    check_attend(short, q, out, lse, [0])
