@@ -127,9 +127,9 @@ class CacheArgs(C.Structure):
     """struct metis_cache"""
     _fields_ = [
         ("pool", C.c_void_p), ("pages", C.c_int64),
-        ("layers", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("layers", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("flags", C.c_int32),
         ("tables", C.c_void_p), ("sequences", C.c_int64), ("width", C.c_int64), ("lengths", C.c_void_p), ("refs", C.c_void_p),
-        ("scales", C.c_void_p), ("status", C.c_void_p),
+        ("scales", C.c_void_p), ("status", C.c_void_p), ("refused", C.c_void_p),
     ]
 
 

@@ -140,6 +140,15 @@ __device__ __forceinline__ void clear_marks(uint32_t* marks, int64_t sequences) 
   for (int64_t i = threadIdx.x; i < (sequences + 31) / 32; i += kPlanThreads) marks[i] = 0;
 }
 
+// The call's sequences have no room for what comes to their ends: append goes by it.
+__device__ __forceinline__ void hold_back(const CacheView& c, const void* slots, bool wide, int64_t n) {
+  if (!c.refused) return;
+  for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int64_t slot = slots ? load_index(slots, wide, i) : i;
+    if (slot >= 0 && slot < c.sequences) c.refused[slot] = 1;
+  }
+}
+
 // Whether the call goes ahead; all threads.
 __device__ __forceinline__ bool agreed(const CacheView& c, PlanShared& sh, Header* header) {
   __syncthreads();
@@ -174,7 +183,10 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const CacheView c
     w.length[i] = (int32_t)(length + more);
     return (length + more + page - 1) / page - (length + page - 1) / page;
   });
-  if (!agreed(c, sh, w.header)) return;
+  if (!agreed(c, sh, w.header)) {
+    hold_back(c, slots, wide, n);
+    return;
+  }
   const bool done = take_lowest(c, want, sh, [&](int64_t rank, int64_t p) {
     const int64_t i = owner_of(sh, w.needs, n, rank), slot = w.to[i];
     const int64_t first = (c.lengths[slot] + page - 1) / page;
@@ -183,11 +195,15 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const CacheView c
   });
   if (!done) {
     if (threadIdx.x == 0) refuse(c.status, METIS_CACHE_NO_PAGES);
+    hold_back(c, slots, wide, n);
     return;
   }
   __syncthreads();
   for (int64_t i = threadIdx.x; i < n; i += kPlanThreads)
-    if (w.to[i] >= 0) c.lengths[w.to[i]] = w.length[i];
+    if (w.to[i] >= 0) {
+      c.lengths[w.to[i]] = w.length[i];
+      if (c.refused) c.refused[w.to[i]] = 0;
+    }
 }
 
 // ---- fork -----------------------------------------------------------------------------------------------------------
@@ -233,7 +249,10 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
   }
   __syncthreads();
   for (int64_t i = threadIdx.x; i < n; i += kPlanThreads)
-    if (w.to[i] >= 0) c.lengths[w.to[i]] = w.length[i];
+    if (w.to[i] >= 0) {
+      c.lengths[w.to[i]] = w.length[i];
+      if (c.refused) c.refused[w.to[i]] = 0;
+    }
   if (threadIdx.x == 0) w.header->moves = (int32_t)want;
 }
 
@@ -415,6 +434,7 @@ int32_t check_cache(const metis_cache* c, CacheView* v) {
   if (!c || !c->pool || !c->tables || !c->lengths || !c->refs || !c->status) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
   if (c->dtype != METIS_DTYPE_BF16 && c->dtype != METIS_DTYPE_E4M3) return fail(METIS_ERR_BAD_ARGUMENT, "the cache's dtype must be bf16 or e4m3");
   if ((c->dtype == METIS_DTYPE_E4M3) != (c->scales != nullptr)) return fail(METIS_ERR_BAD_ARGUMENT, "scales go with e4m3, and with nothing else");
+  if ((c->flags & METIS_CACHE_HAS_REFUSED) && !c->refused) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
   const int item = c->dtype == METIS_DTYPE_BF16 ? 2 : 1;
   if (c->pages <= 0 || c->pages >= ((int64_t)1 << 31) || c->layers <= 0 || c->kv_heads <= 0 || c->sequences <= 0 || c->sequences > kMaxSequences || c->width <= 0)
     return fail(METIS_ERR_BAD_SHAPE, "pages, layers, heads, sequences and width must be positive, sequences at most 2^17");
@@ -424,7 +444,7 @@ int32_t check_cache(const metis_cache* c, CacheView* v) {
   if ((int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim >= (int64_t)1 << 30) return fail(METIS_ERR_TOO_LARGE, "a page of all layers has less than 2^30 elements");
   if (!aligned16(c->pool)) return fail(METIS_ERR_BAD_ALIGNMENT, "the pool must be 16-byte aligned");
   *v = {static_cast<char*>(c->pool), (int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim * item, c->pages, c->tables, c->sequences, c->width, c->lengths,
-        c->refs, c->status, c->layers, c->kv_heads, c->page_size, c->head_dim, item};
+        c->refs, c->status, (c->flags & METIS_CACHE_HAS_REFUSED) ? c->refused : nullptr, c->layers, c->kv_heads, c->page_size, c->head_dim, item};
   return METIS_OK;
 }
 

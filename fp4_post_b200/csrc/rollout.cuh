@@ -19,6 +19,7 @@ struct CacheView {
   int32_t* lengths;
   int32_t* refs;
   int32_t* status;
+  int32_t* refused;         // [sequences], or null
   int32_t layers, kv_heads, page_size, head_dim, item;      // item: bytes of an element
 };
 int32_t check_cache(const metis_cache* c, CacheView* view);

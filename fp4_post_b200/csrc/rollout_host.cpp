@@ -308,7 +308,7 @@ struct Held {
   }
 };
 struct Cache {
-  Held pool{"pool"}, tables{"tables"}, lengths{"lengths"}, refs{"refs"}, scales{"scales"}, status{"status"};
+  Held pool{"pool"}, tables{"tables"}, lengths{"lengths"}, refs{"refs"}, scales{"scales"}, status{"status"}, refused{"refused"};
   metis_cache c = {};                   // sizes; addresses are those of `now`
   c10::Device device = c10::Device(c10::kCPU);
   metis_cache now() const {
@@ -317,7 +317,7 @@ struct Cache {
     TORCH_CHECK_VALUE((reinterpret_cast<uintptr_t>(m.pool) & 15) == 0, "the cache's pool must be 16-byte aligned");
     m.tables = static_cast<int32_t*>(tables.address(device)); m.lengths = static_cast<int32_t*>(lengths.address(device));
     m.refs = static_cast<int32_t*>(refs.address(device)); m.scales = static_cast<const float*>(scales.address(device));
-    m.status = static_cast<int32_t*>(status.address(device));
+    m.status = static_cast<int32_t*>(status.address(device)); m.refused = static_cast<int32_t*>(refused.address(device));
     return m;
   }
 };
@@ -331,16 +331,16 @@ Cache& cache_of(Args& a) {
   return *static_cast<Cache*>(p);
 }
 
-// pool, tables, lengths, refs, scales or None, status -> the cache
+// pool, tables, lengths, refs, scales or None, status, refused -> the cache
 PyObject* cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ROLLOUT_BEGIN(args, nargs)
   auto h = std::make_unique<Cache>();
-  const Tensor pool = a.tensor("pool"), tables = a.tensor("tables"), lengths = a.tensor("lengths"), refs = a.tensor("refs"), scales = a.optional("scales"), status = a.tensor("status");
+  const Tensor pool = a.tensor("pool"), tables = a.tensor("tables"), lengths = a.tensor("lengths"), refs = a.tensor("refs"), scales = a.optional("scales"), status = a.tensor("status"), refused = a.tensor("refused");
   const bool e4m3 = pool.scalar_type() == at::kFloat8_e4m3fn;
   check_tensor(pool, "pool", e4m3 ? at::kFloat8_e4m3fn : at::kBFloat16, "bfloat16 or float8_e4m3fn");
   TORCH_CHECK_VALUE(pool.dim() == 6 && pool.size(2) == 2, "pool must be [pages, layers, 2, kv_heads, page_size, head_dim], not ", pool.sizes());
   h->device = pool.device();
-  for (const auto& [t, name] : {std::make_pair(&tables, "tables"), std::make_pair(&lengths, "lengths"), std::make_pair(&refs, "refs"), std::make_pair(&status, "status")}) {
+  for (const auto& [t, name] : {std::make_pair(&tables, "tables"), std::make_pair(&lengths, "lengths"), std::make_pair(&refs, "refs"), std::make_pair(&status, "status"), std::make_pair(&refused, "refused")}) {
     check_tensor(*t, name, at::kInt, "int32");
     check_device(*t, name, h->device);
     TORCH_CHECK_VALUE(t->is_contiguous(), name, " must be contiguous");
@@ -348,7 +348,7 @@ PyObject* cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   TORCH_CHECK_VALUE(pool.is_contiguous() && aligned16(pool), "pool must be contiguous and 16-byte aligned");
   TORCH_CHECK_VALUE(tables.dim() == 2 && lengths.dim() == 1 && lengths.size(0) == tables.size(0), "tables ", tables.sizes(), " and lengths ", lengths.sizes(), " do not fit");
   TORCH_CHECK_VALUE(refs.dim() == 1 && refs.size(0) == pool.size(0), "refs ", refs.sizes(), " do not fit a pool of ", pool.size(0), " pages");
-  TORCH_CHECK_VALUE(status.numel() == 1, "status must have one element");
+  TORCH_CHECK_VALUE(status.numel() == 1 && refused.dim() == 1 && refused.size(0) == tables.size(0), "status must have one element, refused one for each sequence");
   TORCH_CHECK_VALUE(e4m3 == scales.defined(), "scales go with float8_e4m3fn, and with nothing else");
   if (e4m3) {
     check_tensor(scales, "scales", at::kFloat, "float32");
@@ -357,11 +357,11 @@ PyObject* cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                       "scales must be contiguous [layers, 2, kv_heads], not ", scales.sizes());
     h->scales.keep(scales);
   }
-  h->pool.keep(pool); h->tables.keep(tables); h->lengths.keep(lengths); h->refs.keep(refs); h->status.keep(status);
+  h->pool.keep(pool); h->tables.keep(tables); h->lengths.keep(lengths); h->refs.keep(refs); h->status.keep(status); h->refused.keep(refused);
   metis_cache& c = h->c;
   c.pages = pool.size(0); c.layers = (int32_t)pool.size(1); c.kv_heads = (int32_t)pool.size(3);
   c.page_size = (int32_t)pool.size(4); c.head_dim = (int32_t)pool.size(5); c.dtype = e4m3 ? METIS_DTYPE_E4M3 : METIS_DTYPE_BF16;
-  c.sequences = tables.size(0); c.width = tables.size(1);
+  c.sequences = tables.size(0); c.width = tables.size(1); c.flags = METIS_CACHE_HAS_REFUSED;
   const metis_cache m = h->now();
   check(lib.metis_cache_check(&m), "metis_cache_check");
   PyObject* o = PyCapsule_New(h.get(), kCapsule, drop_cache);

@@ -257,9 +257,11 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendTensors
     int64_t position = t.positions ? load_index(t.positions, t.positions_64, i) : 0, at = -2;
     if (slot >= 0 && slot < c.sequences) {
       const int64_t length = c.lengths[slot];
+      // (a sequence's end is where its last token is, while there is no room for another one)
+      const bool held_back = !t.positions && (c.refused ? c.refused[slot] : *c.status) != 0;
       if (!t.positions) position = length - 1;
       at = -1;
-      if (position >= 0 && position < length && position < c.width * c.page_size) {
+      if (!held_back && position >= 0 && position < length && position < c.width * c.page_size) {
         const int64_t page = c.tables[slot * c.width + position / c.page_size];
         if (page >= 0 && page < c.pages) at = page * c.page_bytes + (position % c.page_size) * c.head_dim * c.item;
       }

@@ -166,7 +166,9 @@ class PagedCache:
             raise TypeError(f"pool must be a tensor, not {type(pool).__name__}")
         with torch.inference_mode(False):        # (check() writes to it in whatever mode)
             status = torch.zeros(1, dtype=torch.int32, device=pool.device)
-        self._handle = cabi.rollout_host().cache(pool, tables, lengths, refs, scales, status)
+        # by sequence, whether the last reserve() that named it could not be done
+        refused = torch.zeros(lengths.numel() if isinstance(lengths, torch.Tensor) else 0, dtype=torch.int32, device=pool.device)
+        self._handle = cabi.rollout_host().cache(pool, tables, lengths, refs, scales, status, refused)
         self._tensors = (pool, tables, lengths, refs, scales, status)
         self._host = cabi.rollout_host()
 
@@ -188,7 +190,8 @@ class PagedCache:
         return t if t is None or isinstance(t, torch.Tensor) else torch.tensor(list(t), dtype=torch.int64, device=self.pool.device)
 
     def reserve(self, slots=None, counts: Union[int, torch.Tensor, list] = 1) -> None:
-        """Lengthens the sequences `slots` (None: all) by `counts` tokens, one number or one for each, with pages for them."""
+        """Lengthens the sequences `slots` (None: all) by `counts` tokens, one number or one for each, with pages for them.  Where that cannot be done, append()
+        without positions writes nothing to any of them until a reserve() for it goes through."""
         one = counts if isinstance(counts, int) else None
         if one is None and not isinstance(counts, torch.Tensor):
             try:
@@ -202,7 +205,8 @@ class PagedCache:
         """Writes keys and values of reserved tokens, the keys (and q) turned by their rotary positions first; returns the queries.
 
         q [tokens, heads, head_dim] (or None), k and v [tokens, kv_heads, head_dim], bfloat16.  Token i belongs to sequence slots[i] (None: i) at
-        positions[i] (None: its last one).  A token of no sequence is not written, and its query comes back as zeros; one at a position that is not
+        positions[i] (None: its last one, and the token is not written where the reserve() that was to make room for it could not be done; its query is turned as
+        at the last position then).  A token of no sequence is not written, and its query comes back as zeros; one at a position that is not
         reserved is not written.  8-bit pools take round to nearest of x / scale, saturating.  A page that several sequences hold changes for all of
         them.  Two tokens of one call must not go to the same place: one of them is there afterwards."""
         if rotary is None:

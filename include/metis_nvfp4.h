@@ -601,29 +601,33 @@ int32_t metis_rotary(const metis_rotary_args* args);
  * page_size is a multiple of 16, head_dim of 8 up to 256.  Everything is on the device, so that a decode step with its bookkeeping can
  * be captured.  status (int32, required): a call that cannot be done leaves everything as it is and puts its METIS_CACHE_* code there, unless there
  * is one already.  Indices on the device are checked there: a page number outside the pool is read as an absent one.
+ * refused (int32 [sequences], zeros at first; read with METIS_CACHE_HAS_REFUSED in flags): the sequences for which the last metis_cache_reserve that named
+ * them could not be done.  metis_cache_append writes no token to the end of one, which would go over its last one; without it, to the end of none while there is a status.
  */
 #define METIS_CACHE_NO_PAGES  16  /* not enough free pages */
 #define METIS_CACHE_BAD_SLOT  17  /* a sequence that the cache does not have */
 #define METIS_CACHE_TOO_LONG  18  /* longer than `width` pages, a negative count, or a length that no call leaves */
 #define METIS_CACHE_TWICE     19  /* the same sequence twice in one call */
 #define METIS_CACHE_NOT_EMPTY 20  /* a fork's destination that has a length */
+#define METIS_CACHE_HAS_REFUSED 1 /* flags */
 typedef struct metis_cache {
   void* pool;
   int64_t pages;
-  int32_t layers, kv_heads, page_size, head_dim, dtype, reserved;
+  int32_t layers, kv_heads, page_size, head_dim, dtype, flags;
   int32_t* tables;
   int64_t sequences, width;
   int32_t* lengths;
   int32_t* refs;
   const float* scales;
   int32_t* status;
+  int32_t* refused;
 } metis_cache;
 /* Whether the calls below take this cache: its sizes and pointers, nothing on the device. */
 int32_t metis_cache_check(const metis_cache* cache);
 
 /*
  * Rotary positions of q and k (turns null: none) and k and v written into the pages, in one launch.  Token i belongs to sequence slots[i]
- * (null: i) at positions[i] (null: its last one, lengths - 1).  A token whose sequence or position the cache does not have is not written, and its
+ * (null: i) at positions[i] (null: its last one, lengths - 1; not written where the call that was to make room for it was refused).  A token whose sequence or position the cache does not have is not written, and its
  * q_out is zeros where it is the sequence that is missing.  q [tokens, heads_q, head_dim] may be null; strides in elements, multiples of 8; bf16.
  * e4m3: round to nearest of x / scale, saturating.  Two tokens of one call for the same place: one of them is there afterwards.
  */

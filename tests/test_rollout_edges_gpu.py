@@ -194,3 +194,130 @@ def test_attend_at_the_longest_length(dtype):
     q = normal(1, 4, 64, seed=27)
     out, lse = cache.attend(0, q, return_lse=True)
     check_attend(short, q, out, lse, [0])
+
+
+# ---- calls behind one that was refused --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_tokens_that_no_reserve_made_room_for_are_not_written(dtype):
+    """A group of answers that runs out of pages: what its sequences hold, shared pages among it, stays; behind pages that were freed the step is made again."""
+    cache = new_cache(pages=6, sequences=7, dtype=dtype)
+    bits = torch.uint8 if dtype == torch.float8_e4m3fn else torch.int16
+    k, v = normal(32, 2, 64, seed=60), normal(32, 2, 64, seed=61)
+    cache.reserve([0, 6], [32, 20])
+    cache.append(0, None, k, v, [0] * 32, list(range(32)))
+    cache.append(0, None, k[:20], v[:20], [6] * 20, list(range(20)))
+    cache.fork([0] * 4, [1, 2, 3, 4])
+    cache.check()
+    live = torch.tensor([1, 2, -1, 3, 4, 6], device=DEV)
+    before = [t.clone() for t in (cache.pool.view(bits), cache.tables, cache.lengths, cache.refs)]
+    q, nk, nv = normal(6, 4, 64, seed=62), normal(6, 2, 64, seed=63), normal(6, 2, 64, seed=64)
+    r = rollout.Rotary(64)
+    for _ in range(2):                                       # four pages are asked for, two are there
+        cache.reserve(live, 1)
+        out = cache.append(0, q, nk, nv, live, rotary=r)
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.pool.view(bits), cache.tables, cache.lengths, cache.refs)))
+        assert torch.equal(out[[0, 5]], r(q[[0, 5]], None, torch.tensor([31, 19], device=DEV))) and (out[2] == 0).all()
+        with pytest.raises(RuntimeError, match="not enough free pages"):
+            cache.check()
+        cache.append(0, q, nk, nv, live, rotary=r)           # (the reason has been read: there is still no room)
+        assert torch.equal(cache.pool.view(bits), before[0])
+    # explicit positions are the caller's own
+    cache.append(0, None, v[:1], k[:1], [6], [3])
+    assert not torch.equal(cache.pool.view(bits), before[0])
+    cache.append(0, None, k[3:4], v[3:4], [6], [3])
+    assert torch.equal(cache.pool.view(bits), before[0])
+    cache.free([6])
+    cache.reserve(live[:5], 1)
+    cache.append(0, q[:5], nk[:5], nv[:5], live[:5], rotary=r)
+    cache.check()
+    plain_k = r(nk, None, torch.full((6,), 32, device=DEV))
+    for i, s in ((0, 1), (1, 2), (3, 3), (4, 4)):
+        got = keys_values(cache, 0, s, 33)
+        want = torch.stack((plain_k[i], nv[i])).to(dtype).double() if dtype == torch.bfloat16 else torch.stack((r(nk[i:i + 1].float(), None, torch.tensor([32], device=DEV))[0], nv[i].float())).to(dtype).double()
+        assert torch.equal(got[:, :, 32], want) and torch.equal(got[0, :, :32], k.to(dtype).double().transpose(0, 1))
+
+
+def test_what_one_refused_call_asked_for_keeps_no_other_sequence_from_its_tokens():
+    cache = new_cache(pages=4, sequences=5)
+    k = normal(2, 2, 64, seed=65)
+    cache.reserve([0, 1], 16)
+    cache.reserve([0], 100)                                  # refused
+    cache.fork([0], [1])                                     # refused
+    cache.reserve([1, 2], 1)
+    cache.append(0, None, k, k, [1, 2])
+    cache.append(0, None, k, k, [0, 3])                      # (no room for 0, nothing in 3)
+    assert torch.equal(keys_values(cache, 0, 1, 17)[0][:, 16], k[0].double()) and torch.equal(keys_values(cache, 0, 2, 1)[1][:, 0], k[1].double())
+    assert (keys_values(cache, 0, 0, 16) == 0).all()
+    with pytest.raises(RuntimeError, match="not enough"):
+        cache.check()
+    # a sequence that is emptied and begun again has nothing left of it
+    cache.free([0])
+    cache.reserve([0], 1)
+    cache.append(0, None, k[:1], k[:1], [0])
+    assert torch.equal(keys_values(cache, 0, 0, 1)[0][:, 0], k[0].double())
+    # refused for a sequence given twice, a slot that is none, a sequence too long: all that were named are held back, and others are not
+    for slots, counts in (([0, 1, 1], 1), ([0, 9], 1), ([0, 1], [1, 200]), ([0, 1], [1, -1])):
+        cache.reserve(slots, counts)
+        before = cache.pool.clone()
+        cache.append(0, None, k[1:], k[1:], [0])
+        assert torch.equal(cache.pool, before)
+        cache.append(0, None, k[:1], k[:1], [2])
+        assert not torch.equal(cache.pool, before)
+        cache.append(0, None, k[1:], k[1:], [2])
+        cache.reserve([0, 1], 0)                             # (a call that goes through, for no more room)
+        cache.append(0, None, k[1:], k[1:], [0])
+        assert not torch.equal(cache.pool, before)
+        cache.append(0, None, k[:1], k[:1], [0])
+        assert torch.equal(cache.pool, before)
+        with pytest.raises(RuntimeError):
+            cache.check()
+
+
+def test_a_captured_step_that_ran_out_of_pages_goes_on_when_there_are_some():
+    cache, twin = (new_cache(pages=5, sequences=4) for _ in range(2))
+    slots = torch.tensor([0, 1], device=DEV)
+    q, k = normal(2, 4, 64, seed=66), normal(2, 2, 64, seed=67)
+    for c in (cache, twin):
+        c.reserve([0, 1, 2], [15, 16, 32])
+
+    def step(c):
+        c.reserve(slots, 1)
+        return c.attend(0, c.append(0, q, k, k, slots), slots)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache)
+    for i in range(20):
+        k.copy_(normal(2, 2, 64, seed=70 + i))
+        if i == 6:
+            before = cache.pool.clone(), cache.lengths.clone()
+            cache.reserve([3], 16)                           # the last page
+            cache.lengths[0] = twin.lengths[0] = 16
+            graph.replay()
+            assert torch.equal(cache.pool, before[0]) and int(cache.lengths[1]) == int(before[1][1])
+            with pytest.raises(RuntimeError, match="not enough"):
+                cache.check()
+            cache.free([3, 2])
+            twin.free([2])
+        graph.replay()
+        assert torch.equal(step(twin), out) and torch.equal(cache.lengths, twin.lengths)
+    cache.check()
+
+
+def test_without_a_word_for_each_sequence_nothing_goes_to_an_end_while_there_is_a_status():
+    """The entry points as a program in C has them."""
+    import ctypes as C
+    from fp4_post_b200 import cabi
+    L, cache, k = cabi.lib(), new_cache(pages=2, sequences=2), normal(2, 2, 64, seed=68)
+    pool, status = cache.pool, torch.zeros(1, dtype=torch.int32, device=DEV)
+    c = cabi.CacheArgs(pool=pool.data_ptr(), pages=2, layers=1, kv_heads=2, page_size=16, head_dim=64, dtype=cabi.DTYPE_BF16, tables=cache.tables.data_ptr(), sequences=2, width=cache.tables.shape[1],
+                       lengths=cache.lengths.data_ptr(), refs=cache.refs.data_ptr(), status=status.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(L.metis_cache_workspace_bytes(C.byref(c), 2), dtype=torch.uint8, device=DEV)
+    reserve = lambda n: L.metis_cache_reserve(C.byref(c), None, None, n, 0, 2, ws.data_ptr(), ws.numel(), stream)  # noqa: E731
+    a = cabi.AppendArgs(tokens=2, layer=0, heads_q=0, k=k.data_ptr(), v=k.data_ptr(), k_token=128, k_head=64, v_token=128, v_head=64, stream=stream)
+    assert reserve(16) == 0 and reserve(1) == 0 and L.metis_cache_append(C.byref(c), C.byref(a)) == 0
+    assert int(status) == 16 and cache.lengths.tolist() == [16, 16] and (pool == 0).all()
+    status.zero_()
+    assert L.metis_cache_append(C.byref(c), C.byref(a)) == 0
+    assert torch.equal(pool[:, 0, 0, :, 15], k) and int((pool != 0).any(dim=-1).sum()) == 8
