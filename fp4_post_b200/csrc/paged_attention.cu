@@ -37,7 +37,9 @@ constexpr int kMinTiles = 8;              // of a part: two for each warp
 // 85 us where short rows were counted by their tiles alone, 75 with 4, 57 with 16, 56 with 20 to 32; few long rows do not change.
 constexpr int kBegin = 20;
 constexpr int kUnitThreads = 512;         // of a block that joins one column of many pieces (111 of them: 20.5 us for the call, 20.7 with 256 threads, 21.8 with 1024)
-constexpr float kNone = -3.4028235e38f;   // the maximum of no scores: the lowest finite number, so that a score of -inf weighs nothing behind it, and any other something
+// The maximum of no scores: the lowest finite number, so that a score of -inf weighs nothing behind it, and any other something.  Keys that all score -inf leave it, and 0 / 0; of
+// no keys at all (their pages are absent) the maximum is -inf, and the row is zeros.
+constexpr float kNone = -3.4028235e38f;
 // Weights are relative to a number that is moved when one of them would pass 2^slack: to the largest score, so that bf16 weights are 1 then, or as far under it as fp16, whose smallest
 // normal number is 2^-14, is better filled from above.
 template <bool kE4m3> constexpr float kSlack = kE4m3 ? 15.0f : 8.0f;
@@ -226,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     int32_t page = -1, piece_on_page = 0;  // of the lane's 16 keys among the 32 times 16 that are looked up at once
     int fetched = 0;                       // tiles whose copies have been issued
     uint32_t absent = 0;                   // bit i: the 16 keys i before the last fetched ones lie on no page of the pool
+    bool any = false;                      // keys that do
     auto fetch = [&]() {
       if (fetched < mine_count) {
         if ((fetched * MT & 31) == 0) {
@@ -241,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
           const int at_page = __shfl_sync(0xffffffffu, piece_on_page, from_lane);
           const bool good = pg >= 0 && pg < p.pages;
           absent = absent << 1 | (good ? 0u : 1u);
+          any |= good;
           const int keys = good ? min(kRows, keys_all - ((first + fetched * kWarps) * MT + part) * kRows) : 0;
           const char* from = good ? head_keys + (int64_t)pg * p.page_bytes + at_page * (kRows * row_bytes) : p.keys;
           const uint32_t to = mine_at + (uint32_t)(fetched % L::kStages) * L::kTileBytes + part * 2 * L::kPartBytes;
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int column = n * 8 + 2 * t + j;
-        if (g == 0) warp_ml[warp][column] = make_float2(m[n][j], sum);
+        if (g == 0) warp_ml[warp][column] = make_float2(any ? m[n][j] : -CUDART_INF_F, sum);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           const int e0 = i * 16 + (kE4m3 ? 2 * g : g), e1 = i * 16 + (kE4m3 ? 2 * g + 1 : g + 8);
@@ -512,9 +516,10 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
     const int64_t place = ((int64_t)blockIdx.x * 2 + (begin == 0 ? 1 : 0)) * 8 * NT;
     for (int i = threadIdx.x; i < live * D; i += kThreads) {
       const int column = i / D, e = i - column * D;
-      float top = kNone;
+      float top = -CUDART_INF_F;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][column].x);
+      const bool none = top == -CUDART_INF_F;
       float sum = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
@@ -523,9 +528,10 @@ __global__ void __launch_bounds__(kThreads, Plan<D, NT, kE4m3>::kBlocks) attend_
         sum += ml.y * f;
         acc += reinterpret_cast<const float*>(ring + w * L::kWarpBytes)[i] * f;
       }
+      if (none) sum = acc = 0.0f;          // (NaN of -inf less -inf)
       if (whole) {
         const int64_t to = (int64_t)row * p.heads_q + first_head + column;
-        if (e < p.head_dim) p.out[to * p.head_dim + e] = __float2bfloat16_rn(__fdiv_rn(acc, sum) * v_scale);
+        if (e < p.head_dim) p.out[to * p.head_dim + e] = __float2bfloat16_rn(none ? 0.0f : __fdiv_rn(acc, sum) * v_scale);
         if (e == 0 && p.lse) p.lse[to] = (top + log2f(sum)) * 0.69314718055994531f;
       } else {
         p.part_o[(place + column) * D + e] = acc;
@@ -572,7 +578,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendParams p
     const bool live = i < here;
     auto place = [&](int piece) { return (((int64_t)(job.z + piece) * p.chunks + chunk) * 2 + (piece == 0 ? 1 : 0)) * 8 * NT + column; };
     Lane<D> acc;
-    float sum = 0.0f, top = kNone;
+    float sum = 0.0f, top = -CUDART_INF_F;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc.v[e] = 0.0f;
     if (live) {
@@ -617,11 +623,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendParams p
     }
     if (!live) continue;
     const int64_t to = (int64_t)job.x * p.heads_q + head * p.group + chunk * 8 * NT + column;
+    const bool none = top == -CUDART_INF_F;
 #pragma unroll
     for (int e = 0; e < E; e += 2)
       if (lane * E + e < p.head_dim)
-        *reinterpret_cast<__nv_bfloat162*>(p.out + to * p.head_dim + lane * E + e) = __floats2bfloat162_rn(__fdiv_rn(acc.v[e], sum) * v_scale, __fdiv_rn(acc.v[e + 1], sum) * v_scale);
-    if (lane == 0 && p.lse) p.lse[to] = (top + log2f(sum)) * 0.69314718055994531f;
+        *reinterpret_cast<__nv_bfloat162*>(p.out + to * p.head_dim + lane * E + e) =
+            __floats2bfloat162_rn(none ? 0.0f : __fdiv_rn(acc.v[e], sum) * v_scale, none ? 0.0f : __fdiv_rn(acc.v[e + 1], sum) * v_scale);
+    if (lane == 0 && p.lse) p.lse[to] = none ? top : (top + log2f(sum)) * 0.69314718055994531f;
   }
 }
 

@@ -321,3 +321,31 @@ def test_without_a_word_for_each_sequence_nothing_goes_to_an_end_while_there_is_
     status.zero_()
     assert L.metis_cache_append(C.byref(c), C.byref(a)) == 0
     assert torch.equal(pool[:, 0, 0, :, 15], k) and int((pool != 0).any(dim=-1).sum()) == 8
+
+
+# ---- pages that are absent ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("lengths", [[40, 33], [20000, 33], [700] * 300])
+@pytest.mark.parametrize("heads, head_dim", [(4, 64), (40, 128)])
+def test_a_row_whose_pages_are_all_absent_is_one_without_keys(lengths, dtype, heads, head_dim):
+    """In one block, and split over several: zeros, and a logarithm of -inf.  Rows beside it stay."""
+    cache = filled(lengths, head_dim=head_dim, dtype=dtype, seed=21)
+    q = normal(len(lengths), heads, head_dim, seed=22)
+    want, want_lse = cache.attend(0, q, return_lse=True)
+    cache.tables[0] = torch.tensor([-1, cache.pool.shape[0], 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=DEV).repeat(cache.tables.shape[1])[:cache.tables.shape[1]]
+    out, lse = cache.attend(0, q, return_lse=True)
+    assert (out[0] == 0).all() and (lse[0] == -math.inf).all()
+    assert torch.equal(out[1:], want[1:]) and torch.equal(lse[1:], want_lse[1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_a_row_with_one_page_among_absent_ones_is_that_page(dtype):
+    cache = filled([20000, 16, 33], seed=23, dtype=dtype)
+    q = normal(3, 4, 64, seed=24)
+    for at in (0, 700, 1249):
+        cache.tables[0] = -1
+        cache.tables[0, at] = cache.tables[1, 0]
+        out, lse = cache.attend(0, q[[1, 1]], [0, 1], return_lse=True)
+        check_attend(cache, q[1:2], out[1:], lse[1:], [1])
+        check_attend(cache, q[1:2], out[:1], lse[:1], [1])
