@@ -297,13 +297,18 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CacheV
 __global__ void __launch_bounds__(256) free_kernel(const CacheView c, const void* slots, bool wide, int64_t n) {
   __shared__ int32_t length;
   grid_dependency_wait();
+  // A block goes through all of the list before it empties anything: a call that names a sequence that the cache does not have does nothing.
+  if (slots) {
+    bool bad = false;
+    for (int64_t i = threadIdx.x; i < n; i += 256) bad |= load_index(slots, wide, i) >= c.sequences;
+    if (__syncthreads_or(bad)) {
+      if (blockIdx.x == 0 && threadIdx.x == 0) refuse(c.status, METIS_CACHE_BAD_SLOT);
+      return;
+    }
+  }
   for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
     const int64_t slot = slots ? load_index(slots, wide, i) : i;
-    if (slot < 0) continue;
-    if (slot >= c.sequences) {
-      if (threadIdx.x == 0) refuse(c.status, METIS_CACHE_BAD_SLOT);
-      continue;
-    }
+    if (slot < 0 || slot >= c.sequences) continue;
     __syncthreads();
     if (threadIdx.x == 0) length = atomicExch(&c.lengths[slot], 0);          // (whoever comes second finds it empty)
     __syncthreads();

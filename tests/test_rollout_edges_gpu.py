@@ -349,3 +349,17 @@ def test_a_row_with_one_page_among_absent_ones_is_that_page(dtype):
         out, lse = cache.attend(0, q[[1, 1]], [0, 1], return_lse=True)
         check_attend(cache, q[1:2], out[1:], lse[1:], [1])
         check_attend(cache, q[1:2], out[:1], lse[:1], [1])
+
+
+def test_a_free_that_names_a_sequence_that_is_none_does_nothing():
+    cache = new_cache()
+    cache.reserve([0, 2, 5], [20, 3, 100])
+    before = [t.clone() for t in (cache.tables, cache.lengths, cache.refs)]
+    for slots in ([0, 17], [6, 2], [0, 2, -1, 5, 1 << 40], [0] * 3000 + [6], torch.tensor([5, 2 ** 31 - 1], dtype=torch.int32, device=DEV)):
+        cache.free(slots)
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.tables, cache.lengths, cache.refs)))
+        with pytest.raises(RuntimeError, match="does not have"):
+            cache.check()
+    cache.free([0, -1, 0, 5] * 2000)
+    cache.check()
+    assert cache.lengths.tolist() == [0, 0, 3, 0, 0, 0] and cache.free_pages() == 39
