@@ -53,12 +53,15 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 };
 
-// cos and sin of the pair of frequency `turn` at a position: the angle in half turns, in [-1, 1)
+// cos and sin of the pair of frequency `turn` at a position.  Whole quarter turns are taken off while the angle is a whole number: what is left, at most an eighth of a turn, keeps
+// its own 24 bits in fp32, where the whole angle would be rounded to 2^-25 of half a turn and a sine near zero lose most of its bits.
 __device__ __forceinline__ float2 cos_sin(uint64_t turn, int64_t position, const RotaryShape& s) {
   const uint64_t part = turn * (uint64_t)position;
+  const uint32_t quarter = (uint32_t)((part + (1ull << 61)) >> 62);
   float sn, cs;
-  sincospif((float)(int32_t)(part >> 32) * 0x1p-31f, &sn, &cs);
-  return make_float2(cs * s.magnitude, sn * s.magnitude * s.sign);
+  sincospif((float)(int32_t)((int64_t)(part - ((uint64_t)quarter << 62)) >> 30) * 0x1p-33f, &sn, &cs);
+  const float c = (quarter & 1) ? sn : cs, d = (quarter & 1) ? cs : sn;
+  return make_float2((((quarter + 1) & 2) ? -c : c) * s.magnitude, ((quarter & 2) ? -d : d) * s.magnitude * s.sign);
 }
 
 // A unit of a head: the two pieces of W elements of the half layout, one piece of W elements of neighbouring pairs, with W = 1 the two elements of a

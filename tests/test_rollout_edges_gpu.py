@@ -363,3 +363,25 @@ def test_a_free_that_names_a_sequence_that_is_none_does_nothing():
     cache.free([0, -1, 0, 5] * 2000)
     cache.check()
     assert cache.lengths.tolist() == [0, 0, 3, 0, 0, 0] and cache.free_pages() == 39
+
+
+# ---- rotary positions' own precision --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_cosines_and_sines_are_as_exact_as_fp32_has_them(interleaved):
+    """Of pairs (1, 0) the results are the cosine and the sine themselves.  The angle, less whole quarter turns, is phi in [-pi/4, pi/4]: cut off below 2^-34 of a turn and rounded to fp32,
+    it is off by 2^-24 |phi| + 2^-31; sincospif by a step, 2^-23 of its result."""
+    n = 16
+    r = rollout.Rotary(n, theta=500.0, interleaved=interleaved)
+    x = torch.zeros(40000, 1, n, device=DEV)
+    first, second = (slice(0, n, 2), slice(1, n, 2)) if interleaved else (slice(0, n // 2), slice(n // 2, n))
+    x[..., first] = 1.0
+    positions = torch.cat((torch.arange(30000, device=DEV), torch.randint(-2 ** 40, 2 ** 40, (10000,), device=DEV, generator=gen(80))))
+    y = r(x, None, positions)[:, 0].double()
+    turn = torch.tensor([[(p * b) % 2 ** 64 / 2 ** 64 for b in r.turns.tolist()] for p in positions.tolist()], dtype=torch.float64, device=DEV)
+    c, s = torch.cos(2 * math.pi * turn), torch.sin(2 * math.pi * turn)
+    phi = 2 * math.pi * (turn - torch.round(turn * 4) / 4).abs()
+    off = 2.0 ** -24 * phi + 2.0 ** -31
+    for got, value, other in ((y[:, first], c, s), (y[:, second], s, c)):
+        bound = 2.0 ** -23 * value.abs() + off * (other.abs() + off) + 2.0 ** -50
+        assert ((got - value).abs() <= bound).all(), float(((got - value).abs() / bound).max())
