@@ -1,8 +1,10 @@
 // Rotary positions, and the same with the keys and values written into a paged cache.
 //
 // A pair (a, b) of a head at position p goes to m (a cos - b sin, b cos + a sin) of the angle 2 pi p f, f a frequency in turns per position.  f is held
-// as a 64-bit fraction of a turn: p f modulo 1 is then one integer product whose high bits are thrown away, exact to p 2^-65 turns at any
-// position, and the angle never needs a range reduction (fp32 products of positions and frequencies are off by p 2^-24, a whole radian at 2^24).
+// as a 64-bit fraction of a turn: p f modulo 1 is then one integer product whose high bits are thrown away, exact for the fraction that is given, and the angle never needs a
+// range reduction (fp32 products of positions and frequencies are off by p 2^-24, a whole radian at 2^24).  The fractions that rollout.Rotary gives come from the
+// host's 64-bit floats: off by up to 2^-53 turns (theta^(-2i / d) and its quotient by 2 pi, a few steps of what is at most 0.16), so that an angle is off by
+// p 2^-53 turns: below fp32's own rounding to p = 2^26.
 // No table of cosines is kept or read: a block forms those of its tokens once, in shared memory, and uses them for all heads.
 //
 // Bound by memory: every element is read and written once.  A thread holds the cosines of one unit (16 bytes of each half, or 16 bytes of

@@ -93,8 +93,8 @@ class Rotary:
     """Rotary positions of the first rotary_dim (None: all) of head_dim elements.
 
     interleaved: pairs are neighbours (2i, 2i + 1); else they lie half of rotary_dim apart (i, rotary_dim / 2 + i).  theta, scaling: see
-    rotary_frequencies.  Angles are formed from the positions in whole numbers, exactly modulo a turn: there is no table, no longest position,
-    and the millionth one is as exact as the first.
+    rotary_frequencies.  Angles are formed from the positions in whole numbers, exactly modulo a turn: there is no table and no longest position.
+    Frequencies are 64-bit floats, off by up to 2^-53 turns per position, which is below the rounding of fp32 up to position 2^26.
 
         q, k = rotary(q, k, positions)
 

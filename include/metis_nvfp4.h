@@ -572,8 +572,8 @@ int64_t metis_rollout_launches(void);
  * Rotary positions of x [tokens, heads, head_dim] for up to two tensors (queries and keys; k may be null) in one launch:
  * of the first rotary_dim elements of a head the pair i, (i, rotary_dim/2 + i) or with `interleaved` (2i, 2i + 1), is turned by the
  * angle 2 pi position turns[i] / 2^64 and multiplied by `magnitude`; the others are copied.  turns[i] is the pair's frequency as a
- * fraction of a turn per position, in units of 2^-64: the product with a position is exact modulo a whole turn, so that an angle is as
- * exact at position 2^31 as at 1.  inverse: by minus the angle (what a gradient takes).  Computed in fp32, rounded once.
+ * fraction of a turn per position, in units of 2^-64: the product with a position is exact modulo a whole turn, so that an angle is off by
+ * the position times what turns[i] is off by, and by fp32's rounding of what is left of a quarter turn.  inverse: by minus the angle (what a gradient takes).  Computed in fp32, rounded once.
  * Token t of `tokens` is (t / inner, t % inner) under the two token strides; strides in elements, the last dimension dense.  positions:
  * one for each token (int32, or int64 with positions_64), or null: t % inner.  Outputs are contiguous.  dtype bf16 or fp32.  What the
  * reference leaves to the attention of its models (src/Metis/models/llama.py, or the Hugging Face model around its layers).
