@@ -385,3 +385,26 @@ def test_cosines_and_sines_are_as_exact_as_fp32_has_them(interleaved):
     for got, value, other in ((y[:, first], c, s), (y[:, second], s, c)):
         bound = 2.0 ** -23 * value.abs() + off * (other.abs() + off) + 2.0 ** -50
         assert ((got - value).abs() <= bound).all(), float(((got - value).abs() / bound).max())
+
+
+# ---- sampling on the borders between two tokens -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [512, 3000])
+def test_sample_takes_a_kept_token_at_every_border(vocab, dtype):
+    """Random numbers on the borders between two tokens and a few steps of 64 bits beside them, half of the vocabulary masked: whatever the sums' roundings are, the token is one that is
+    kept, and no farther from the border than the sums' own error."""
+    for seed in range(12):
+        x = (torch.rand(vocab, device=DEV, generator=gen(seed)) * -30).to(dtype)
+        x[torch.rand(vocab, device=DEV, generator=gen(100 + seed)) < 0.5] = -math.inf
+        x[(seed * 97) % vocab] = 0.0
+        w = x.float().exp().double()
+        sums = w.cumsum(0)
+        u = (sums / sums[-1])[w > 0][:-1][:500]
+        u = torch.cat([u + k * 2.0 ** -54 for k in range(-3, 4)] + [torch.tensor([1 - 2.0 ** -53], device=DEV, dtype=torch.float64)])
+        u = u[(u >= 0) & (u < 1)].contiguous()
+        for kw in (dict(), dict(top_p=1 - 2.0 ** -53), dict(top_k=vocab - 1)):
+            token = rollout.sample(x.expand(u.numel(), vocab), u, **kw)
+            assert int(token.min()) >= 0 and int(token.max()) < vocab and (w[token] > 0).all(), (seed, kw)
+            mark, slack = u * sums[-1], float(sums[-1]) * 2.0 ** -44
+            assert ((sums - w)[token] <= mark + slack).all() and (sums[token] >= mark - slack).all(), (seed, kw)
