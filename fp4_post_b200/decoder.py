@@ -323,7 +323,7 @@ class Decoder(nn.Module):
         """`answers` sampled continuations of each prompt: tokens [B * answers, n <= max_new_tokens] (and their log-probabilities under the model at
         that temperature, float32), the answers of a prompt behind one another.
 
-        ids [B, T] on the GPU, prompts padded behind their `lengths` (None: all T).  A prompt is prefilled once and its pages are shared by its answers;
+        ids [B, T] on the GPU, prompts padded behind their `lengths` with anything (None: all T).  A prompt is prefilled once and its pages are shared by its answers;
         keys and values are kept in bfloat16 or (cache_dtype) float8_e4m3fn.  eos ends an answer: what follows it is eos again, with log-probability 0,
         and takes no more pages.  temperature, top_k, top_p, min_p: see rollout.sample; generator draws its random numbers.  graphed: the
         decode step is captured after its first run and replayed (weights and what layers cache of them must not change meanwhile, shapes are fixed).
@@ -362,11 +362,12 @@ class Decoder(nn.Module):
                 logits = logits.float()
             return rollout.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, logprobs=True)
 
-        # prompts: what is behind one belongs to no sequence
+        # prompts: what is behind one belongs to no sequence, and is no token of the vocabulary perhaps (an embedding reads where it says)
         cache.reserve(prompts, count)
         at = torch.arange(T, device=dev).expand(B, T)
-        owner = torch.where(at < count[:, None], prompts[:, None], -1).reshape(-1)
-        x = run(self.embed_tokens(ids), lambda i: _Cached(cache, i, rotary, owner, at.reshape(-1), True))
+        inside = at < count[:, None]
+        owner = torch.where(inside, prompts[:, None], -1).reshape(-1)
+        x = run(self.embed_tokens(torch.where(inside, ids, 0)), lambda i: _Cached(cache, i, rotary, owner, at.reshape(-1), True))
         last = x[prompts, count - 1]
         cache.fork(prompts.repeat_interleave(answers), slots)
         cache.free(prompts)

@@ -408,3 +408,18 @@ def test_sample_takes_a_kept_token_at_every_border(vocab, dtype):
             assert int(token.min()) >= 0 and int(token.max()) < vocab and (w[token] > 0).all(), (seed, kw)
             mark, slack = u * sums[-1], float(sums[-1]) * 2.0 ** -44
             assert ((sums - w)[token] <= mark + slack).all() and (sums[token] >= mark - slack).all(), (seed, kw)
+
+
+# ---- what calls take ------------------------------------------------------------------------------------------------------
+
+def test_prompts_are_padded_with_anything():
+    """Behind a prompt's length ids are not read: -100, or any other number that is no token, is as good as one."""
+    model = decoder()
+    ids = prompts(3, 20)
+    lengths = [20, 1, 7]
+    run = lambda x: model.generate(x, lengths, max_new_tokens=6, temperature=0.0, logprobs=True)  # noqa: E731
+    want, want_p = run(torch.where(torch.arange(20, device=DEV) < torch.tensor(lengths, device=DEV)[:, None], ids, 0))
+    behind = torch.arange(20, device=DEV)[None] >= torch.tensor(lengths, device=DEV)[:, None]
+    for pad in (-100, -1, SMALL.vocab, 2 ** 40):
+        got, got_p = run(ids.masked_fill(behind, pad))
+        assert torch.equal(got, want) and torch.equal(got_p, want_p)
