@@ -24,6 +24,7 @@ the paged cache, attends over it and samples on kernels of that module, eagerly 
 """
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass
 from typing import Optional
 
@@ -338,7 +339,7 @@ class Decoder(nn.Module):
         if page_size <= 0 or page_size % 16:
             raise ValueError(f"page_size must be a multiple of 16, not {page_size}")
         B, T = ids.shape
-        lengths = [T] * B if lengths is None else [int(n) for n in lengths]
+        lengths = [T] * B if lengths is None else [operator.index(n) for n in lengths]
         if len(lengths) != B or min(lengths) < 1 or max(lengths) > T:
             raise ValueError(f"lengths must be {B} numbers from 1 to {T}")
         dev, rows = ids.device, B * answers

@@ -186,8 +186,8 @@ class PagedCache:
     max_length = property(lambda self: self.tables.shape[1] * self.page_size)
 
     def _index(self, t):
-        """Slots, counts or positions; what is not a tensor is copied to the device."""
-        return t if t is None or isinstance(t, torch.Tensor) else torch.tensor(list(t), dtype=torch.int64, device=self.pool.device)
+        """Slots, counts or positions; what is not a tensor is copied to the device, and has to be whole numbers (torch cuts others)."""
+        return t if t is None or isinstance(t, torch.Tensor) else torch.tensor([operator.index(i) for i in t], dtype=torch.int64, device=self.pool.device)
 
     def reserve(self, slots=None, counts: Union[int, torch.Tensor, list] = 1) -> None:
         """Lengthens the sequences `slots` (None: all) by `counts` tokens, one number or one for each, with pages for them.  Where that cannot be done, append()

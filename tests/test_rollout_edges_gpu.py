@@ -423,3 +423,28 @@ def test_prompts_are_padded_with_anything():
     for pad in (-100, -1, SMALL.vocab, 2 ** 40):
         got, got_p = run(ids.masked_fill(behind, pad))
         assert torch.equal(got, want) and torch.equal(got_p, want_p)
+
+
+def test_slots_counts_and_positions_are_whole_numbers():
+    cache = new_cache()
+    cache.reserve([0], 20)
+    k = normal(1, 2, 64)
+    for call in (lambda: cache.reserve([0.5], 1), lambda: cache.reserve([1.0], 1), lambda: cache.reserve([0], [1.5]), lambda: cache.reserve([0], 1.5), lambda: cache.free([0.0]), lambda: cache.fork([0.2], [1]),
+                 lambda: cache.fork([0], [1.7]), lambda: cache.append(0, None, k, k, [0.3]), lambda: cache.append(0, None, k, k, [0], [2.5]), lambda: cache.attend(0, k, [0.9]),
+                 lambda: cache.reserve(["0"], 1), lambda: cache.reserve([None], 1)):
+        with pytest.raises(TypeError):
+            call()
+    assert cache.lengths.tolist() == [20, 0, 0, 0, 0, 0]
+    cache.reserve((i for i in (1, 2)), iter([3, 4]))
+    cache.reserve(range(3, 5), [True, 2])
+    assert cache.lengths.tolist() == [20, 3, 4, 1, 2, 0]
+    with pytest.raises((ValueError, OverflowError, RuntimeError)):
+        cache.reserve([2 ** 70], 1)
+    cache.check()
+    model, ids = decoder(), prompts(2, 8)
+    for lengths in ([3, 2.5], torch.tensor([3.0, 2.0]), ["3", "2"]):
+        with pytest.raises(TypeError):
+            model.generate(ids, lengths, max_new_tokens=1)
+    want = model.generate(ids, [3, 2], max_new_tokens=3, temperature=0.0)
+    for lengths in (torch.tensor([3, 2]), torch.tensor([3, 2], device=DEV, dtype=torch.int32)):
+        assert torch.equal(model.generate(ids, lengths, max_new_tokens=3, temperature=0.0), want)
