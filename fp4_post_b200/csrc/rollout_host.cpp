@@ -320,6 +320,11 @@ struct Cache {
     m.status = static_cast<int32_t*>(status.address(device)); m.refused = static_cast<int32_t*>(refused.address(device));
     return m;
   }
+  // Of a call that reads or writes elements.
+  void check_constants() const {
+    check_constant(pool.t, "pool");
+    check_constant(scales.t, "scales");
+  }
 };
 constexpr const char* kCapsule = "metis_cache";
 
@@ -394,6 +399,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool interleaved = a.truth();
   check_untraced();
   TORCH_CHECK_VALUE(layer >= 0 && layer < h.c.layers, "layer ", layer, " of a cache of ", h.c.layers);
+  h.check_constants();
   const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   k = heads_of(k, "k", h, -1, h.c.kv_heads, 8);
@@ -437,6 +443,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool want_lse = a.truth();
   check_untraced();
   TORCH_CHECK_VALUE(layer >= 0 && layer < h.c.layers, "layer ", layer, " of a cache of ", h.c.layers);
+  h.check_constants();
   const metis_cache m = h.now();
   c10::OptionalDeviceGuard guard(h.device);
   q = heads_of(q, "q", h, -1, -1, 2);
@@ -552,6 +559,7 @@ struct Parameter {
     rows = a.tensor(what);
     check_tensor(rows, what, type, type_name);
     check_device(rows, what, device);
+    check_constant(rows, what);
     TORCH_CHECK_VALUE(rows.dim() == 1 && rows.size(0) == count, what, " has shape ", rows.sizes(), ", not (", count, ",)");
     rows = rows.resolve_neg().contiguous();
   }
@@ -572,6 +580,7 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool u_64 = u.scalar_type() == at::kDouble;
   check_tensor(u, "u", u_64 ? at::kDouble : at::kFloat, "float32 or float64");
   check_device(u, "u", device);
+  check_constant(u, "u");
   TORCH_CHECK_VALUE(u.dim() == 1 && u.size(0) == rows, "u has shape ", u.sizes(), ", not (", rows, ",)");
   c10::OptionalDeviceGuard guard(device);
   const Parameter temperature(a, "temperature", device, rows, at::kFloat, "a number or float32"), top_k(a, "top_k", device, rows, at::kInt, "a number or int32"),

@@ -448,3 +448,26 @@ def test_slots_counts_and_positions_are_whole_numbers():
     want = model.generate(ids, [3, 2], max_new_tokens=3, temperature=0.0)
     for lengths in (torch.tensor([3, 2]), torch.tensor([3, 2], device=DEV, dtype=torch.int32)):
         assert torch.equal(model.generate(ids, lengths, max_new_tokens=3, temperature=0.0), want)
+
+
+def test_gradients_that_no_call_forms_are_refused_for_every_argument():
+    x, u = normal(2, 50, dtype=torch.float32), torch.full((2,), 0.5, device=DEV)
+    for kw in (dict(temperature=torch.ones(2, device=DEV)), dict(top_p=torch.full((2,), 0.5, device=DEV)), dict(min_p=torch.zeros(2, device=DEV))):
+        (name, t), = kw.items()
+        t.requires_grad_()
+        with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+            rollout.sample(x, u, logprobs=True, **kw)
+        with torch.no_grad():
+            rollout.sample(x, u, logprobs=True, **kw)
+    with pytest.raises(RuntimeError, match="u requires a gradient"):
+        rollout.sample(x, u.clone().requires_grad_())
+    q = normal(2, 4, 64)
+    for name, dtype in (("pool", torch.bfloat16), ("scales", torch.float8_e4m3fn)):
+        cache = filled([20, 5], seed=90, dtype=dtype)
+        want = cache.attend(0, q)
+        getattr(cache, name).requires_grad_()
+        for call in (lambda: cache.attend(0, q), lambda: cache.append(0, q, q[:, :2], q[:, :2])):
+            with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+                call()
+        with torch.no_grad():
+            assert torch.equal(cache.attend(0, q), want)
