@@ -155,6 +155,14 @@ struct Turn {
   bool interleaved = false;
 };
 
+// Kernels read rotary_dim / 2 of them: Rotary's attributes are plain ones, which a program can set.
+void check_turns(const Tensor& turns, int64_t rotary_dim) {
+  TORCH_CHECK(turns.is_cuda(), "the rotary positions' frequencies must be a CUDA tensor: there is no CPU fallback");
+  TORCH_CHECK_TYPE(turns.scalar_type() == at::kLong, "the rotary positions' frequencies must be int64, got ", turns.scalar_type());
+  TORCH_CHECK_VALUE(rotary_dim > 0 && rotary_dim % 2 == 0 && turns.dim() == 1 && turns.size(0) == rotary_dim / 2 && turns.is_contiguous(),
+                    "rotary positions of ", rotary_dim, " elements with frequencies ", turns.sizes(), " of strides ", turns.strides());
+}
+
 // x [..., heads, D] as tokens of two strides, the inner ones those of the third dimension from behind; copied where it has more
 struct Tokens {
   Tensor t;
@@ -259,6 +267,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                       name, " must be [..., heads, head_dim] with head_dim a multiple of 8 from ", by.rotary_dim, " to 256, not ", t->sizes());
     check_device(*t, name, by.turns.device());
   }
+  check_turns(by.turns, by.rotary_dim);
   const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 2);
   if (k.defined()) {
     TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "q is ", q.scalar_type(), " and k ", k.scalar_type());
@@ -409,6 +418,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   slots = indices(slots, "slots", h.device, tokens);
   positions = indices(positions, "positions", h.device, tokens);
   if (turns.defined()) {
+    check_turns(turns, rotary_dim);
     check_device(turns, "the rotary positions' frequencies", h.device);
     TORCH_CHECK_VALUE(rotary_dim <= h.c.head_dim, "rotary positions of ", rotary_dim, " elements on heads of ", h.c.head_dim);
   }

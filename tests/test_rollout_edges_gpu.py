@@ -471,3 +471,17 @@ def test_gradients_that_no_call_forms_are_refused_for_every_argument():
                 call()
         with torch.no_grad():
             assert torch.equal(cache.attend(0, q), want)
+
+
+def test_frequencies_that_do_not_fit_are_refused():
+    """Rotary's attributes are plain ones."""
+    q, cache = normal(2, 4, 64), new_cache()
+    cache.reserve(None, 3)
+    for name, value in (("rotary_dim", 128), ("rotary_dim", 32), ("turns", lambda t: t[:-1]), ("turns", lambda t: t.float()), ("turns", lambda t: t.repeat_interleave(2)[::2]), ("turns", lambda t: t.cpu()),
+                        ("rotary_dim", 0), ("rotary_dim", -64)):
+        r = rollout.Rotary(64)
+        setattr(r, name, value(r.turns) if callable(value) else value)
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            r(q)
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            cache.append(0, q, q[:, :2], q[:, :2], [0, 1], rotary=r)
