@@ -320,13 +320,14 @@ class Decoder(nn.Module):
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, lengths=None, *, max_new_tokens: int, answers: int = 1, temperature=1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
                  eos: Optional[int] = None, generator: Optional[torch.Generator] = None, logprobs: bool = False, page_size: int = 16,
-                 cache_dtype: torch.dtype = torch.bfloat16, graphed: bool = False):
+                 cache_dtype: torch.dtype = torch.bfloat16, cache_scales: Optional[torch.Tensor] = None, graphed: bool = False):
         """`answers` sampled continuations of each prompt: tokens [B * answers, n <= max_new_tokens] (and their log-probabilities under the model at
         that temperature, float32), the answers of a prompt behind one another.
 
         ids [B, T] on the GPU, prompts padded behind their `lengths` with anything (None: all T).  A prompt is prefilled once and its pages are shared by its answers;
-        keys and values are kept in bfloat16 or (cache_dtype) float8_e4m3fn.  eos ends an answer: what follows it is eos again, with log-probability 0,
-        and takes no more pages.  temperature, top_k, top_p, min_p: see rollout.sample; generator draws its random numbers.  graphed: the
+        keys and values are kept in bfloat16 or (cache_dtype) float8_e4m3fn, there as x / cache_scales (float32 [layers, 2, kv_heads], see rollout.PagedCache; ones
+        where None), which saturates at 448.  The pool has pages for max_new_tokens of every answer from the start.  eos ends an answer: what follows it is eos again, with
+        log-probability 0, and takes no more pages.  temperature, top_k, top_p, min_p: see rollout.sample; generator draws its random numbers.  graphed: the
         decode step is captured after its first run and replayed (weights and what layers cache of them must not change meanwhile, shapes are fixed).
         The model is bfloat16; rotary positions are formed in fp32, as fuse_rotary has them in forward()."""
         c = self.cfg
@@ -347,7 +348,7 @@ class Decoder(nn.Module):
         whole = [n // page_size for n in lengths]
         pages = sum(-(-n // page_size) for n in lengths) + answers * sum(-(-(n + max_new_tokens) // page_size) - w for n, w in zip(lengths, whole))
         cache = rollout.PagedCache(c.layers, c.kv_heads, c.head_dim, pages=pages, sequences=B + rows, max_length=T + max_new_tokens, page_size=page_size,
-                                   dtype=cache_dtype, device=dev)
+                                   dtype=cache_dtype, scales=cache_scales, device=dev)
         rotary = self._rotary_of(dev)
         count = torch.tensor(lengths, dtype=torch.int64, device=dev)
         prompts, slots = torch.arange(B, device=dev), torch.arange(B, B + rows, device=dev)

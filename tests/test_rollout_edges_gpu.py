@@ -485,3 +485,23 @@ def test_frequencies_that_do_not_fit_are_refused():
             r(q)
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             cache.append(0, q, q[:, :2], q[:, :2], [0, 1], rotary=r)
+
+
+def test_generate_takes_the_scales_of_an_8_bit_cache():
+    """Keys of 2000 and more saturate at 448 unless they are scaled."""
+    model = decoder()
+    with torch.no_grad():
+        for blk in model.layers:
+            blk.self_attn.k_proj.bias.fill_(2000.0)
+            blk.self_attn.v_proj.bias.fill_(1500.0)
+    ids = prompts(2, 12)
+    run = lambda **kw: model.generate(ids, max_new_tokens=10, temperature=0.0, logprobs=True, **kw)  # noqa: E731
+    want, want_p = run()
+    scales = torch.full((SMALL.layers, 2, SMALL.kv_heads), 16.0, device=DEV)
+    got, got_p = run(cache_dtype=torch.float8_e4m3fn, cache_scales=scales)
+    _, cut_p = run(cache_dtype=torch.float8_e4m3fn)
+    assert float((got_p[:, 1:] - want_p[:, 1:]).abs().max()) < float((cut_p[:, 1:] - want_p[:, 1:]).abs().max())
+    with pytest.raises(ValueError, match="scales"):
+        run(cache_scales=scales)
+    with pytest.raises(ValueError, match="scales"):
+        run(cache_dtype=torch.float8_e4m3fn, cache_scales=scales[:1])
