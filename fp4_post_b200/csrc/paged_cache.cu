@@ -216,6 +216,11 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
   clear_marks(marks, c.sequences);
   __syncthreads();
   const int64_t page = c.page_size;
+  // A page that is absent in the source is absent in its fork: one of its own would hold keys of whoever had it before.
+  auto present = [&](int64_t from, int64_t e) {
+    const int32_t p = c.tables[from * c.width + e];
+    return p >= 0 && p < c.pages;
+  };
   const int64_t want = count_needs(w, n, sh, [&](int64_t i) -> int64_t {
     const int64_t from = load_index(src, wide, i), to = load_index(dst, wide, i);
     w.to[i] = -1;
@@ -228,13 +233,21 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const CacheView
     w.from[i] = (int32_t)from;
     w.to[i] = (int32_t)to;
     w.length[i] = (int32_t)length;
-    return share ? (length % page != 0) : (length + page - 1) / page;
+    int64_t there = 0;
+#pragma unroll 16
+    for (int64_t e = share ? length / page : 0; e * page < length; ++e) there += present(from, e);
+    return there;
   });
   if (!agreed(c, sh, w.header)) return;
   // (a destination is empty, so that no source's table is written here)
   const bool done = take_lowest(c, want, sh, [&](int64_t rank, int64_t p) {
     const int64_t i = owner_of(sh, w.needs, n, rank), from = w.from[i], to = w.to[i], length = w.length[i];
-    const int64_t entry = (share ? length / page : 0) + rank - w.needs[i];
+    const int64_t first = share ? length / page : 0, last = (length - 1) / page, mine = rank - w.needs[i];
+    int64_t entry = first + mine;
+    if (w.needs[i + 1] - w.needs[i] != last + 1 - first) {      // (some are absent)
+      entry = first;
+      for (int64_t ahead = mine; entry < last && (!present(from, entry) || ahead-- > 0); ) ++entry;
+    }
     c.tables[to * c.width + entry] = (int32_t)p;
     c.refs[p] = 1;
     const int32_t old = c.tables[from * c.width + entry];
@@ -340,7 +353,7 @@ __device__ __forceinline__ void move_rows(const CacheView& c, const Move* moves,
 #pragma unroll 1
   for (int m = 0; m < count; ++m) {
     const Move mv = moves[m];
-    if (mv.from < 0 || mv.from >= c.pages) continue;       // (a table that named no page)
+    if (mv.from < 0 || mv.from >= c.pages) continue;
     const int in_place = mv.filled * row / (int)sizeof(V), all = in_place * places;
     int at = part * kBatch * kMoveThreads + (int)threadIdx.x;
     if (at >= all) continue;
@@ -370,7 +383,7 @@ __device__ __forceinline__ void move_rows(const CacheView& c, const Move* moves,
 // The plan's moves, and what goes with them: of a fork with shared pages the tables' rows and one more holder for each page; of a compaction the
 // pages' new numbers in all tables, and their holders.
 template <MoveKind kKind>
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, const Work w, int64_t n) {
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, const Work w, int64_t n, bool share) {
   constexpr int kBatch = kKind == kFork ? 4 : 8;
   grid_dependency_wait();
   const int32_t moves = w.header->moves;
@@ -379,13 +392,15 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const CacheView c, c
   if constexpr (kKind == kFork) {
     for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
       if (w.to[i] < 0) continue;
-      // the entries that the plan has not written are the source's
+      // the entries that the plan has not written are the source's: those that are shared, and absent ones
       const int64_t from = w.from[i], to = w.to[i], length = w.length[i];
-      const int64_t entries = (length + c.page_size - 1) / c.page_size - (w.needs[i + 1] - w.needs[i]);
-      for (int64_t e = threadIdx.x; e < entries; e += kMoveThreads) {
+      const int64_t shared = share ? length / c.page_size : 0, entries = (length + c.page_size - 1) / c.page_size;
+      const bool absent = w.needs[i + 1] - w.needs[i] != entries - shared;
+      for (int64_t e = threadIdx.x; e < (absent ? entries : shared); e += kMoveThreads) {
         const int32_t p = c.tables[from * c.width + e];
-        c.tables[to * c.width + e] = p;
-        if (p >= 0 && p < c.pages) atomicAdd(&c.refs[p], 1);
+        const bool there = p >= 0 && p < c.pages;
+        if (e < shared || !there) c.tables[to * c.width + e] = there ? p : -1;
+        if (e < shared && there) atomicAdd(&c.refs[p], 1);
       }
     }
   } else {
@@ -425,8 +440,8 @@ int32_t check_call(const metis_cache* cache, CacheView* c, int64_t n, const void
 
 size_t mark_bytes(const CacheView& c) { return (size_t)((c.sequences + 31) / 32) * 4; }
 
-cudaError_t launch_moves(const CacheView& c, const Work& w, MoveKind kind, int64_t n, cudaStream_t st) {
-  return launch_overlapped(kLaunchShort, kind == kFork ? move_kernel<kFork> : move_kernel<kCompact>, dim3((unsigned)device_sm_count() * 8), dim3(kMoveThreads), 0, st, c, w, n);
+cudaError_t launch_moves(const CacheView& c, const Work& w, MoveKind kind, int64_t n, bool share, cudaStream_t st) {
+  return launch_overlapped(kLaunchShort, kind == kFork ? move_kernel<kFork> : move_kernel<kCompact>, dim3((unsigned)device_sm_count() * 8), dim3(kMoveThreads), 0, st, c, w, n, share);
 }
 
 std::atomic<int64_t> launches{0};
@@ -484,7 +499,7 @@ extern "C" int32_t metis_cache_fork(const metis_cache* cache, const void* src, c
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Work w = work_view(workspace, n, c.pages);
   METIS_CUDA_OK(launch_overlapped(kLaunchShort, fork_plan_kernel, dim3(1), dim3(kPlanThreads), mark_bytes(c), st, c, src, dst, index_64 != 0, n, share != 0, w));
-  METIS_CUDA_OK(launch_moves(c, w, kFork, n, st));
+  METIS_CUDA_OK(launch_moves(c, w, kFork, n, share != 0, st));
   count_rollout_launches(2);
   return METIS_OK;
 }
@@ -506,7 +521,7 @@ extern "C" int32_t metis_cache_compact(const metis_cache* cache, int32_t* live, 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Work w = work_view(workspace, 1, c.pages);
   METIS_CUDA_OK(launch_overlapped(kLaunchShort, compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, c, live, w));
-  METIS_CUDA_OK(launch_moves(c, w, kCompact, 1, st));
+  METIS_CUDA_OK(launch_moves(c, w, kCompact, 1, false, st));
   count_rollout_launches(2);
   return METIS_OK;
 }

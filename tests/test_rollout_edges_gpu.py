@@ -505,3 +505,25 @@ def test_generate_takes_the_scales_of_an_8_bit_cache():
         run(cache_scales=scales)
     with pytest.raises(ValueError, match="scales"):
         run(cache_dtype=torch.float8_e4m3fn, cache_scales=scales[:1])
+
+
+@pytest.mark.parametrize("share", [True, False])
+def test_a_fork_of_absent_pages_has_them_absent(share):
+    """Not pages of its own with what somebody else has left there."""
+    cache = filled([40, 50, 0, 0, 0], seed=91)
+    cache.pool[cache.refs == 0] = 100.0                      # (what a free page happens to hold)
+    q = normal(5, 4, 64, seed=92)
+    cache.tables[0, 2] = -1                                  # the part that a fork copies
+    cache.tables[1, 0], cache.tables[1, 1] = cache.pool.shape[0] + 3, -7
+    want, want_lse = cache.attend(0, q[[0, 1, 0, 1]], [0, 1, 0, 1], return_lse=True)
+    refs, tables = cache.refs.clone(), cache.tables.clone()
+    cache.fork([0, 1], [2, 4], share=share)
+    cache.check()
+    got, lse = cache.attend(0, q[[0, 1, 0, 1]], [0, 1, 2, 4], return_lse=True)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    assert int(cache.tables[2, 2]) == -1 and all(not 0 <= int(p) < cache.pool.shape[0] for p in cache.tables[4, :2])
+    own = cache.tables[[2, 4], :4].flatten()
+    own = own[(own >= 0) & (own < cache.pool.shape[0])].long()
+    assert torch.equal(cache.refs, refs.index_add(0, own, torch.ones_like(own, dtype=torch.int32)))
+    cache.free([2, 4])
+    assert torch.equal(cache.refs, refs) and torch.equal(cache.tables, tables)
