@@ -20,6 +20,7 @@ ROLLOUT_PATH = HOST_PATH.with_name(HOST_PATH.name.replace("metis_host", "metis_r
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmetis_nvfp4.so"
 
 DTYPE_BF16, DTYPE_F32, DTYPE_E4M3 = 0, 1, 2
+CACHE_HAS_REFUSED = 0x52464453
 SF_ROWMAJOR, SF_MMA = 0, 1
 ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
 Q_TRANSPOSE, Q_STOCHASTIC, Q_OFFSET_ON_DEVICE, Q_HADAMARD = 1, 2, 4, 8

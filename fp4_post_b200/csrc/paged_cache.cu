@@ -454,7 +454,7 @@ int32_t check_cache(const metis_cache* c, CacheView* v) {
   if (!c || !c->pool || !c->tables || !c->lengths || !c->refs || !c->status) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
   if (c->dtype != METIS_DTYPE_BF16 && c->dtype != METIS_DTYPE_E4M3) return fail(METIS_ERR_BAD_ARGUMENT, "the cache's dtype must be bf16 or e4m3");
   if ((c->dtype == METIS_DTYPE_E4M3) != (c->scales != nullptr)) return fail(METIS_ERR_BAD_ARGUMENT, "scales go with e4m3, and with nothing else");
-  if ((c->flags & METIS_CACHE_HAS_REFUSED) && !c->refused) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
+  if (c->flags == METIS_CACHE_HAS_REFUSED && !c->refused) return fail(METIS_ERR_BAD_ARGUMENT, "null pointer");
   const int item = c->dtype == METIS_DTYPE_BF16 ? 2 : 1;
   if (c->pages <= 0 || c->pages >= ((int64_t)1 << 31) || c->layers <= 0 || c->kv_heads <= 0 || c->sequences <= 0 || c->sequences > kMaxSequences || c->width <= 0)
     return fail(METIS_ERR_BAD_SHAPE, "pages, layers, heads, sequences and width must be positive, sequences at most 2^17");
@@ -464,7 +464,7 @@ int32_t check_cache(const metis_cache* c, CacheView* v) {
   if ((int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim >= (int64_t)1 << 30) return fail(METIS_ERR_TOO_LARGE, "a page of all layers has less than 2^30 elements");
   if (!aligned16(c->pool)) return fail(METIS_ERR_BAD_ALIGNMENT, "the pool must be 16-byte aligned");
   *v = {static_cast<char*>(c->pool), (int64_t)c->layers * 2 * c->kv_heads * c->page_size * c->head_dim * item, c->pages, c->tables, c->sequences, c->width, c->lengths,
-        c->refs, c->status, (c->flags & METIS_CACHE_HAS_REFUSED) ? c->refused : nullptr, c->layers, c->kv_heads, c->page_size, c->head_dim, item};
+        c->refs, c->status, c->flags == METIS_CACHE_HAS_REFUSED ? c->refused : nullptr, c->layers, c->kv_heads, c->page_size, c->head_dim, item};
   return METIS_OK;
 }
 

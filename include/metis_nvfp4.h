@@ -601,7 +601,7 @@ int32_t metis_rotary(const metis_rotary_args* args);
  * page_size is a multiple of 16, head_dim of 8 up to 256.  Everything is on the device, so that a decode step with its bookkeeping can
  * be captured.  status (int32, required): a call that cannot be done leaves everything as it is and puts its METIS_CACHE_* code there, unless there
  * is one already.  Indices on the device are checked there: a page number outside the pool is read as an absent one.
- * refused (int32 [sequences], zeros at first; read with METIS_CACHE_HAS_REFUSED in flags): the sequences for which the last metis_cache_reserve that named
+ * refused (int32 [sequences], zeros at first; read where flags is METIS_CACHE_HAS_REFUSED): the sequences for which the last metis_cache_reserve that named
  * them could not be done.  metis_cache_append writes no token to the end of one, which would go over its last one; without it, to the end of none while there is a status.
  */
 #define METIS_CACHE_NO_PAGES  16  /* not enough free pages */
@@ -609,7 +609,7 @@ int32_t metis_rotary(const metis_rotary_args* args);
 #define METIS_CACHE_TOO_LONG  18  /* longer than `width` pages, a negative count, or a length that no call leaves */
 #define METIS_CACHE_TWICE     19  /* the same sequence twice in one call */
 #define METIS_CACHE_NOT_EMPTY 20  /* a fork's destination that has a length */
-#define METIS_CACHE_HAS_REFUSED 1 /* flags */
+#define METIS_CACHE_HAS_REFUSED 0x52464453 /* flags, as a whole: a caller that was built without `refused` may have left anything in its place but this */
 typedef struct metis_cache {
   void* pool;
   int64_t pages;

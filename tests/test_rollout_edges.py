@@ -17,9 +17,12 @@ def test_frequencies_are_plain_tensors_whatever_mode_they_are_made_in():
 def test_a_cache_that_says_it_has_refused_sequences_has_them(built_library):
     buf = (C.c_uint8 * 4096)()
     p = C.addressof(buf) + (-C.addressof(buf)) % 256
-    c = cabi.CacheArgs(pool=p, pages=4, layers=1, kv_heads=2, page_size=16, head_dim=64, dtype=cabi.DTYPE_BF16, tables=p, sequences=2, width=2, lengths=p, refs=p, status=p, flags=1)
+    c = cabi.CacheArgs(pool=p, pages=4, layers=1, kv_heads=2, page_size=16, head_dim=64, dtype=cabi.DTYPE_BF16, tables=p, sequences=2, width=2, lengths=p, refs=p, status=p, flags=cabi.CACHE_HAS_REFUSED)
     assert cabi.lib().metis_cache_check(C.byref(c)) == -1
-    c.refused = p
+    for anything_else in (0, 1, -1, 0x52464452):
+        c.flags = anything_else
+        assert cabi.lib().metis_cache_check(C.byref(c)) == 0
+    c.flags, c.refused = cabi.CACHE_HAS_REFUSED, p
     assert cabi.lib().metis_cache_check(C.byref(c)) == 0
 
 
