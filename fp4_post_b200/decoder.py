@@ -373,7 +373,7 @@ class Decoder(nn.Module):
         last = x[prompts, count - 1]
         cache.fork(prompts.repeat_interleave(answers), slots)
         cache.free(prompts)
-        draws = torch.rand(max_new_tokens, rows, device=dev, generator=generator)
+        draws = torch.rand(max_new_tokens, rows, dtype=torch.float32, device=dev, generator=generator)
         tokens = torch.empty(max_new_tokens, rows, dtype=torch.int64, device=dev)
         logp = torch.empty(max_new_tokens, rows, dtype=torch.float32, device=dev)
         token, p = pick(last.repeat_interleave(answers, dim=0), draws[0])

@@ -527,3 +527,18 @@ def test_a_fork_of_absent_pages_has_them_absent(share):
     assert torch.equal(cache.refs, refs.index_add(0, own, torch.ones_like(own, dtype=torch.int32)))
     cache.free([2, 4])
     assert torch.equal(cache.refs, refs) and torch.equal(cache.tables, tables)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_generate_under_another_default_type(dtype):
+    """Random numbers are fp32, whatever a program has set for its tensors."""
+    model, ids = decoder(), prompts(2, 8)
+    run = lambda: model.generate(ids, max_new_tokens=8, answers=2, top_p=0.9, generator=gen(5), logprobs=True)  # noqa: E731
+    want, want_p = run()
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(dtype)
+        got, got_p = run()
+    finally:
+        torch.set_default_dtype(before)
+    assert torch.equal(got, want) and torch.equal(got_p, want_p)
