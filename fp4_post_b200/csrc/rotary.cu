@@ -8,7 +8,8 @@
 // No table of cosines is kept or read: a block forms those of its tokens once, in shared memory, and uses them for all heads.
 //
 // Bound by memory: every element is read and written once.  A thread holds the cosines of one unit (16 bytes of each half, or 16 bytes of
-// neighbouring pairs) in registers and takes it through the heads of its token; of few tokens, heads are spread over the block instead.
+// neighbouring pairs) in registers and takes it through the heads of its token; of few tokens, heads are spread over the block instead.  Appending prompts is bound by
+// latency: 45 % of the memory's rate and of the issue slots, with 24 warps an SM and a thread's keys and values behind its queries.
 #include "rollout.cuh"
 
 #include <type_traits>
@@ -343,8 +344,9 @@ RotaryShape rotary_shape(int64_t tokens, int heads_q, int heads_k, int head_dim,
 }
 
 // How many tokens a block takes in all: so many waves of blocks where their tables of cosines (and what else a token needs) allow it.  One for tokens that are
-// all alike (1024 blocks of 8 tokens were 1.4 waves); four where a third of them, the padding of a batch, has next to nothing to do (16 prompts of 256
-// to 1024 tokens into e4m3: 54.9 us by one wave, 50.7 by four).
+// all alike (1024 blocks of 8 tokens were 1.4 waves); four where some of them, the padding of a batch, may have next to nothing to do (16 prompts of 256
+// to 976 tokens, bf16 48.1 us by one wave, 45.8 by four; e4m3 51.2 and 49.0.  Of 1024 tokens each, bf16 61.2 and 60.2, and e4m3, which alone has more by it, 58.3 and 64.2: which tokens
+// are padding is on the device).
 int32_t set_span(RotaryShape& s, int64_t tokens, const void* kernel, int token_bytes, int waves) {
   const int bytes = s.rotary_dim / 2 * (int)sizeof(float2) + token_bytes;
   const int64_t most = bytes > 0 ? 40960 / bytes : 1 << 20;

@@ -6,7 +6,7 @@
 //
 // A cluster of up to eight blocks takes a row: it is read once from memory, 16 bytes at a time, and stays in shared memory (in its type) for all passes.  Nothing is sorted; a cut is found by histograms:
 //   bf16  The bins are the values themselves, from the largest one on: 4095 of them, those below 2^-8 in magnitude together in one.  That is every logit
-//         within +-256.  A pass counts, five instructions and an addition in shared memory an element; a bin's weight is its count times the
+//         within +-256.  A pass counts, five instructions and an addition in shared memory an element (the whole kernel runs 50); a bin's weight is its count times the
 //         weight of its value, so that one histogram serves top-k, top-p and the sum of all.  (A cut in the bin of small values or behind the last one goes the other way.)
 //   fp32  2048 bins of (max - x) / T in steps of 1/64, then 1024 at a time of the bits of the logits in the bin where the cut lies until one value is left.
 //
