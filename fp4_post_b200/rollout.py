@@ -156,7 +156,8 @@ class PagedCache:
     @classmethod
     def of(cls, pool: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, *, scales: Optional[torch.Tensor] = None) -> "PagedCache":
         """A cache of tensors that are there already; they are used as they are, and have to agree with one another.  Their memory is looked up at each
-        call (a pool's storage may be given back for a while), what they are is not to change; a captured graph keeps the addresses that it was captured with."""
+        call (a pool's storage may be given back for a while), what they are is not to change; a captured graph keeps the addresses that it was captured with.  The status, and which
+        sequences reserve() could not lengthen, are this cache's own: two caches of the same tensors do not know one another's."""
         self = cls.__new__(cls)
         self._set(pool, tables, lengths, refs, scales)
         return self
