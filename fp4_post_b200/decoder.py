@@ -265,7 +265,7 @@ class Decoder(nn.Module):
     def _rotary_of(self, device: torch.device) -> rollout.Rotary:
         """The configuration's rotary positions on a device, made once for what the configuration is.  (All are kept: a captured graph reads its own.)"""
         c = self.cfg
-        key = device, c.head_dim, c.rope_theta, c.rotary_dim, c.rope_interleaved, None if c.rope_scaling is None else tuple(sorted(c.rope_scaling.items()))
+        key = device, c.head_dim, c.rope_theta, c.rotary_dim, c.rope_interleaved, repr(c.rope_scaling)
         r = self._rotaries.get(key)
         if r is None:
             r = self._rotaries[key] = rollout.Rotary(c.head_dim, theta=c.rope_theta, rotary_dim=c.rotary_dim, interleaved=c.rope_interleaved, scaling=c.rope_scaling, device=device)

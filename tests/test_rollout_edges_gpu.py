@@ -542,3 +542,11 @@ def test_generate_under_another_default_type(dtype):
     finally:
         torch.set_default_dtype(before)
     assert torch.equal(got, want) and torch.equal(got_p, want_p)
+
+
+def test_a_scaling_that_is_not_known_is_named():
+    import dataclasses
+    model = decoder(dataclasses.replace(SMALL, rope_scaling=dict(type="linear", factor=2.0, long_factor=[1.0, 2.0])), fuse_rotary=True)
+    for call in (lambda: model(prompts(1, 4)), lambda: model.generate(prompts(1, 4), max_new_tokens=1)):
+        with pytest.raises(ValueError, match="long_factor"):
+            call()
